@@ -56,8 +56,10 @@ typedef enum pk_status {
     PK_ERR_DEVICE     = 9   /* a device-side index check failed (bad token / frame index) */
 } pk_status;
 
-/* ggml tensor type ids accepted in pk_tensor.type (values of enum ggml_type). */
-enum { PK_GGML_F32 = 0, PK_GGML_F16 = 1, PK_GGML_Q8_0 = 8 };
+/* ggml tensor type ids (values of enum ggml_type). pk_tensor.type of a decoder tensor:
+ * F32, F16 or Q8_0; of a pk_mx4 weight: any of the five. Element type of a plain array
+ * (pk_mx4_*, pk_sample): F32, F16 or BF16. */
+enum { PK_GGML_F32 = 0, PK_GGML_F16 = 1, PK_GGML_Q8_0 = 8, PK_GGML_BF16 = 30, PK_GGML_MXFP4 = 39 };
 
 /* Decoder families (ParakeetModelType, src/parakeet_ctc.h:225-230). */
 enum { PK_MODEL_TDT = 1, PK_MODEL_EOU = 2 };
@@ -454,6 +456,134 @@ PK_API void      pk_vocab_destroy(pk_vocab * v);
 PK_API pk_status pk_detokenize(pk_vocab * v, const int32_t * tokens, int32_t tokens_on_device,
                                const int64_t * token_offsets, int32_t B, char * text, int64_t text_cap,
                                int64_t * text_offsets, int64_t * text_needed);
+
+/* ---- 4-bit microscaled floating point (MXFP4) --------------------------------
+ *
+ * No counterpart in the reference. A row of values is held as one 4-bit e2m1 code
+ * per value (magnitudes 0, 0.5, 1, 1.5, 2, 3, 4, 6) and one power-of-two scale byte
+ * (e8m0) per block of 32 consecutive values: value = e2m1 * 2^(byte - 127); byte 255
+ * makes its whole block NaN. This is the OCP microscaling format and the arithmetic
+ * of a GGUF MXFP4 tensor.
+ *
+ * Quantisation of a block: with a = the largest magnitude, the exponent is
+ * floor(log2 a) - 2, not below -127, and each code the e2m1 value nearest to
+ * x / 2^exponent, a tie going to the even code, magnitudes above 6 to 6. A block of
+ * zeros gets byte 0; a block that holds an infinity or a NaN gets byte 255. A last
+ * block that a row's end cuts short is filled up with zeros.
+ *
+ * These entry points take DEVICE pointers on `device` (the handle's device), queue
+ * their work on `stream` (a cudaStream_t; NULL: the default stream) and return
+ * without waiting for it; they allocate nothing and may be captured into a CUDA
+ * graph. They leave the caller's current device as it was. Pointers are aligned to
+ * their element; rows may start at any multiple of that (16-byte aligned rows are
+ * read fastest). Inputs, outputs and workspace must not overlap. */
+
+/* x: [rows][row_stride] of x_type, of which the first `cols` of each row are read.
+ * codes: [rows][16 * nb], nb = ceil(cols / 32), value 2i of a row in the low half of
+ * its byte i, value 2i + 1 in the high half (4-byte aligned); scales: [rows][nb]. */
+PK_API pk_status pk_mx4_quantize(int device, const void * x, int32_t x_type, int64_t rows, int64_t cols,
+                                 int64_t row_stride, uint8_t * codes, uint8_t * scales, void * stream);
+/* The values that codes and scales stand for, rounded to y_type: y is [rows][row_stride],
+ * the first `cols` of each row are written. */
+PK_API pk_status pk_mx4_dequantize(int device, const uint8_t * codes, const uint8_t * scales, int64_t rows,
+                                   int64_t cols, void * y, int32_t y_type, int64_t row_stride, void * stream);
+
+/* A linear layer [N][K] held in MXFP4 on one device (a CTC head, a projection). */
+typedef struct pk_mx4 pk_mx4;
+
+/* weight: ne0 = K input features (contiguous), ne1 = N outputs; MXFP4 blocks are taken
+ * as they are, the other types are quantised as above. K and N at most 2^20 (a
+ * multiple of 32 for Q8_0 and MXFP4). bias: N floats or NULL. on_device: weight->data
+ * and bias are device pointers (earlier work on the device is waited for), else host
+ * pointers. Blocks until the layer is laid out; the caller keeps its buffers. */
+PK_API pk_status pk_mx4_create(int device, const pk_tensor * weight, int32_t on_device, const float * bias, pk_mx4 ** out);
+/* Waits for the device's queued work, so no call on the layer is still running. */
+PK_API void      pk_mx4_destroy(pk_mx4 * w);
+/* Bytes of device workspace that pk_mx4_linear needs for `rows` rows (never less for
+ * more rows); 0 for rows <= 0, -1 for a null layer. */
+PK_API int64_t   pk_mx4_workspace(const pk_mx4 * w, int64_t rows);
+/* y[m][n] = bias[n] + sum_k q(x)[m][k] * W[n][k]: each row of x is quantised to MXFP4
+ * as pk_mx4_quantize does, products are exact and sums are held in 32 bits; y rounds
+ * once to y_type. x: [rows][x_stride], y: [rows][y_stride] (strides in elements; what
+ * lies past K or N in a row is neither read nor written). rows from 0 to 2^31 - 1.
+ * workspace: pk_mx4_workspace(w, rows) bytes, 256-byte aligned, for this call alone
+ * until it has run: calls that may overlap (two streams, two captured graphs) each
+ * need their own. Calls on one layer may overlap otherwise. PK_ERR_TIMEOUT: a bounded
+ * device-side wait of an EARLIER call on this layer ran out and that call's y is not
+ * to be used (reported once). */
+PK_API pk_status pk_mx4_linear(pk_mx4 * w, const void * x, int32_t x_type, int64_t rows, int64_t x_stride, void * y,
+                               int32_t y_type, int64_t y_stride, void * workspace, int64_t workspace_bytes,
+                               void * stream);
+
+/* ---- drawing tokens from logits -----------------------------------------------
+ *
+ * No counterpart in the reference, whose decoders take the argmax. For each row of
+ * logits l with settings T (temperature), k, p, m and the caller's random number u:
+ *
+ *   a_i = (l_i - max l) / T,  w_i = exp(a_i)         NaN logits count as -infinity; if the
+ *                                                    maximum is +infinity, w = 1 there, else 0
+ *   order: larger logit first, among equal ones the lower index
+ *   kept:  the first k tokens; of these, those before which less than p of these k
+ *          tokens' weight lies (the first always); of these, those with w_i >= m
+ *   token: the lowest index at which the running sum (in index order) of the kept
+ *          weights exceeds u times their total
+ *   log-probability: that of the token under the kept weights
+ *
+ * k <= 0, p >= 1 and m <= 0 each turn their filter off; p <= 0 (or NaN) and m >= 1 leave the
+ * largest. T <= 0 or NaN: the first index of the largest logit, log-probability 0. A row
+ * without any logit above -infinity gets token -1 and log-probability -infinity. u is
+ * clamped to [0, 1), NaN to 0. Weights are held in 64-bit fixed point (2^-43 of the
+ * largest, exponentials in 64-bit floating point), so sums are exact, the same whatever
+ * the batch, and tokens with less than 2^-44 of the largest weight are never drawn. */
+#define PK_SAMPLE_MAX_VOCAB 524288
+
+typedef struct pk_sample_args {
+    const void *    logits;       /* [rows][row_stride] of logits_type; the first `vocab` of a row are read */
+    int32_t         logits_type;  /* PK_GGML_F32, PK_GGML_F16 or PK_GGML_BF16 */
+    int32_t         vocab;        /* 1 .. PK_SAMPLE_MAX_VOCAB */
+    int64_t         rows;         /* 0 .. 2^31 - 1 */
+    int64_t         row_stride;   /* elements, >= vocab */
+    const float *   uniforms;     /* [rows] random numbers in [0, 1) */
+    int32_t *       tokens;       /* [rows] */
+    float *         logprobs;     /* [rows] or NULL */
+    /* settings of every row, or, where the array is not NULL, of each row by itself */
+    float           temperature;
+    int32_t         top_k;
+    float           top_p;
+    float           min_p;
+    const float *   temperatures; /* [rows] or NULL */
+    const int32_t * top_ks;       /* [rows] or NULL */
+    const float *   top_ps;       /* [rows] or NULL */
+    const float *   min_ps;       /* [rows] or NULL */
+} pk_sample_args;
+
+/* Every pointer is a device pointer on `device`; stream, waiting, alignment and overlap
+ * as for pk_mx4_quantize above. Needs no workspace. */
+PK_API pk_status pk_sample(int device, const pk_sample_args * args, void * stream);
+
+/* ---- CTC decode from encoder frames, greedy or drawn ---------------------------- */
+
+/* Settings of a drawn CTC path (see pk_sample); one random number per frame. */
+typedef struct pk_ctc_draw {
+    float         temperature;
+    int32_t       top_k;
+    float         top_p;
+    float         min_p;
+    const float * uniforms;            /* by frame, indexed as the frames are */
+    int32_t       uniforms_on_device;
+    int32_t       reserved;            /* 0 */
+} pk_ctc_draw;
+
+/* pk_ctc_greedy with the two steps around it: `frames` are encoder frames [frames][K]
+ * whose logits the layer `head` (N = vocab_size, on the handle's device) computes, or,
+ * with head = NULL, logits [frames][vocab_size]; each frame's token is the argmax
+ * (draw = NULL) or drawn (pk_sample). Repeats and blanks then collapse as in
+ * pk_ctc_greedy, whose other arguments, results and waiting these are. A frame
+ * without any logit above -infinity counts as blank when drawn. */
+PK_API pk_status pk_ctc_decode(pk_ctc * c, pk_mx4 * head, const float * frames, int32_t frames_on_device,
+                               const int64_t * frame_offsets, const int32_t * n_frames, int32_t B,
+                               const pk_ctc_draw * draw, int32_t * prev_inout, int32_t * tokens, int64_t tokens_cap,
+                               int64_t * token_offsets, int32_t * first_frame, int64_t * tokens_needed);
 
 #ifdef __cplusplus
 }

@@ -8,6 +8,10 @@ mirrors the reference's decoder entry points for tests and benchmarks:
 * ``Decoder.decode_batch(...)``      -> tdt_greedy_decode / eou_greedy_decode (batched)
 * ``Decoder.stream()`` + ``.window`` -> tdt_decode_window / eou_decode_window with state
 
+Beside the token loop: ``CtcGreedy`` (greedy and drawn CTC paths) and ``Vocab``; on device
+pointers and a stream of the caller's, ``sample`` (tokens from logits), ``mx4_quantize`` /
+``mx4_dequantize`` and ``Mx4Linear`` (4-bit microscaled rows and layers).
+
 There is no CPU fallback: if the library cannot be loaded or has no CUDA
 device, calls raise.
 """
@@ -63,6 +67,13 @@ def lib():
             "pk_ctc_greedy": ([P, P, I32, P, P, I32, P, P, I64, P, P, P], I32),
             "pk_vocab_create": ([I32, P, P, I32, I32, I32, I32, I32, P], I32), "pk_vocab_destroy": ([P], None),
             "pk_detokenize": ([P, P, I32, P, I32, P, I64, P, P], I32),
+            "pk_mx4_quantize": ([I32, P, I32, I64, I64, I64, P, P, P], I32),
+            "pk_mx4_dequantize": ([I32, P, P, I64, I64, P, I32, I64, P], I32),
+            "pk_mx4_create": ([I32, P, I32, P, P], I32), "pk_mx4_destroy": ([P], None),
+            "pk_mx4_workspace": ([P, I64], I64),
+            "pk_mx4_linear": ([P, P, I32, I64, I64, P, I32, I64, P, I64, P], I32),
+            "pk_sample": ([I32, P, P], I32),
+            "pk_ctc_decode": ([P, P, P, I32, P, P, I32, P, P, P, I64, P, P, P], I32),
         }
         for name, (args, res) in sigs.items():
             f = getattr(L, name)
@@ -373,6 +384,46 @@ class CtcGreedy:
         fo = [frs[toff[b]:toff[b + 1]].copy() for b in range(B)] if with_frames else None
         return out, fo, prev
 
+    def decode_frames(self, frames, frame_offsets, n_frames, head=None, uniforms=None, temperature=1.0, top_k=0, top_p=1.0,
+                      min_p=0.0, prev=None, on_device=False, uniforms_on_device=False, with_frames=False):
+        """pk_ctc_decode: decode() from encoder frames through `head` (an Mx4Linear, vocab_size wide), or from logits
+        without one; with `uniforms` (one random number per frame) each frame's token is drawn, else the argmax.
+        frames / uniforms: float32 arrays, or device pointers (int) with their flag."""
+        n_frames = np.ascontiguousarray(n_frames, dtype=np.int32)
+        B = len(n_frames)
+        foff = np.ascontiguousarray(frame_offsets, dtype=np.int64)
+        prev = np.full(B, -1, np.int32) if prev is None else np.array(prev, dtype=np.int32, copy=True)
+        cap = int(n_frames.sum())
+        total = int((foff + n_frames).max()) if B else 0
+        toks = np.zeros(max(cap, 1), np.int32)
+        frs = np.zeros(max(cap, 1), np.int32) if with_frames else None
+        toff = np.zeros(B + 1, np.int64)
+        need = C.c_int64(0)
+        if on_device:
+            fp = C.c_void_p(int(frames))
+        else:
+            frames = np.ascontiguousarray(frames, dtype=np.float32)
+            width = self.vocab_size if head is None else head.k
+            if frames.size < total * width:
+                raise ValueError(f"frames hold {frames.size} values, the utterances read {total} x {width}")
+            fp = _p(frames)
+        draw = None
+        if uniforms is not None:
+            if uniforms_on_device:
+                up = C.c_void_p(int(uniforms))
+            else:
+                uniforms = np.ascontiguousarray(uniforms, dtype=np.float32)
+                if uniforms.size < total:
+                    raise ValueError(f"{uniforms.size} random numbers for {total} frames")
+                up = _p(uniforms)
+            draw = abi.pk_ctc_draw(temperature, top_k, top_p, min_p, up, 1 if uniforms_on_device else 0, 0)
+        _check(lib().pk_ctc_decode(self._h, head.h if head is not None else None, fp, 1 if on_device else 0, _p(foff),
+                                   _p(n_frames), B, C.byref(draw) if draw is not None else None, _p(prev), _p(toks), cap,
+                                   _p(toff), _p(frs) if with_frames else None, C.byref(need)), "pk_ctc_decode")
+        out = [toks[toff[b]:toff[b + 1]].copy() for b in range(B)]
+        fo = [frs[toff[b]:toff[b + 1]].copy() for b in range(B)] if with_frames else None
+        return out, fo, prev
+
 
 class Vocab:
     """SentencePiece BPE detokenizer (parakeet::detokenize, src/sentencepiece_bpe.cpp:9-37)
@@ -418,3 +469,85 @@ class Vocab:
         _check(lib().pk_detokenize(self._h, _p(toks), 0, _p(toff), B, _p(text), cap, _p(tof), C.byref(need)),
                "pk_detokenize")
         return [text[tof[b]:tof[b + 1]].tobytes() for b in range(B)]
+
+
+_DTYPE = {"f32": abi.PK_GGML_F32, "f16": abi.PK_GGML_F16, "bf16": abi.PK_GGML_BF16}
+
+
+def mx4_quantize(x: int, rows: int, cols: int, codes: int, scales: int, dtype: str = "f32",
+                 row_stride: Optional[int] = None, device: int = 0, stream: int = 0) -> None:
+    """pk_mx4_quantize on device pointers: rows of `dtype` ("f32", "f16", "bf16") to MXFP4 codes
+    [rows][16 * ceil(cols / 32)] and scales [rows][ceil(cols / 32)]. Queued on `stream`."""
+    _check(lib().pk_mx4_quantize(device, x, _DTYPE[dtype], rows, cols, cols if row_stride is None else row_stride,
+                                 codes, scales, stream), "pk_mx4_quantize")
+
+
+def mx4_dequantize(codes: int, scales: int, rows: int, cols: int, out: int, dtype: str = "f32",
+                   row_stride: Optional[int] = None, device: int = 0, stream: int = 0) -> None:
+    """pk_mx4_dequantize on device pointers: the values of codes and scales. Queued on `stream`."""
+    _check(lib().pk_mx4_dequantize(device, codes, scales, rows, cols, out, _DTYPE[dtype],
+                                   cols if row_stride is None else row_stride, stream), "pk_mx4_dequantize")
+
+
+class Mx4Linear:
+    """A linear layer [n][k] held in MXFP4 on one device (pk_mx4)."""
+
+    def __init__(self, weight, n: Optional[int] = None, k: Optional[int] = None, bias=None, dtype: str = "f32",
+                 on_device: bool = False, device: int = 0):
+        """weight: a synth.Tensor (GGUF blocks), a float32 / float16 array [n][k], or, with
+        on_device, a device pointer to [n][k] of `dtype` (bias then a device pointer too)."""
+        if on_device:
+            t = abi.pk_tensor(C.c_void_p(int(weight)), _DTYPE[dtype], 0, k, n, n * k * (4 if dtype == "f32" else 2))
+            bp = C.c_void_p(int(bias) if bias is not None else 0)
+        else:
+            if isinstance(weight, synth.Tensor):
+                t, k, n = abi._tensor(weight), weight.ne0, weight.ne1
+            else:
+                weight = np.ascontiguousarray(weight, None if np.asarray(weight).dtype == np.float16 else np.float32)
+                n, k = weight.shape
+                t = abi.pk_tensor(_p(weight), abi.PK_GGML_F16 if weight.dtype == np.float16 else abi.PK_GGML_F32, 0, k, n,
+                                  weight.nbytes)
+            if bias is not None:
+                bias = np.ascontiguousarray(bias, np.float32)
+                if bias.size != n:
+                    raise ValueError(f"bias has {bias.size} entries for {n} outputs")
+            bp = _p(bias)
+        h = C.c_void_p()
+        _check(lib().pk_mx4_create(device, C.byref(t), 1 if on_device else 0, bp, C.byref(h)), "pk_mx4_create")
+        self.h = h
+        self.n, self.k, self.device = int(n), int(k), device
+
+    def close(self):
+        if getattr(self, "h", None) is not None and self.h.value:
+            lib().pk_mx4_destroy(self.h)
+            self.h = C.c_void_p()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def workspace(self, rows: int) -> int:
+        """Bytes of device workspace that forward() needs for `rows` rows."""
+        return int(lib().pk_mx4_workspace(self.h, rows))
+
+    def forward(self, x: int, rows: int, y: int, x_dtype: str = "f32", y_dtype: str = "f32",
+                x_stride: Optional[int] = None, y_stride: Optional[int] = None, workspace: int = 0,
+                workspace_bytes: int = 0, stream: int = 0) -> None:
+        """pk_mx4_linear on device pointers: y = q(x) W^T + bias. Queued on `stream`."""
+        _check(lib().pk_mx4_linear(self.h, x, _DTYPE[x_dtype], rows, self.k if x_stride is None else x_stride, y,
+                                   _DTYPE[y_dtype], self.n if y_stride is None else y_stride, workspace, workspace_bytes,
+                                   stream), "pk_mx4_linear")
+
+
+def sample(logits: int, rows: int, vocab: int, uniforms: int, tokens: int, dtype: str = "f32",
+           row_stride: Optional[int] = None, logprobs: int = 0, temperature: float = 1.0, top_k: int = 0,
+           top_p: float = 1.0, min_p: float = 0.0, temperatures: int = 0, top_ks: int = 0, top_ps: int = 0,
+           min_ps: int = 0, device: int = 0, stream: int = 0) -> None:
+    """pk_sample on device pointers: one token per row of logits, by the row's random number.
+    The settings are numbers for every row, or device arrays with one entry per row (0: not
+    given). Queued on `stream`."""
+    a = abi.pk_sample_args(logits, _DTYPE[dtype], vocab, rows, vocab if row_stride is None else row_stride, uniforms,
+                           tokens, logprobs, temperature, top_k, top_p, min_p, temperatures, top_ks, top_ps, min_ps)
+    _check(lib().pk_sample(device, C.byref(a), stream), "pk_sample")

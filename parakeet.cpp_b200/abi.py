@@ -11,6 +11,8 @@ PK_ERR_OOM, PK_ERR_TIMEOUT, PK_ERR_CAPACITY, PK_ERR_NO_DEVICE, PK_ERR_DEVICE = 5
 PK_MODEL_TDT, PK_MODEL_EOU = 1, 2
 PK_OPT_TIMEOUT_US, PK_OPT_MATH, PK_OPT_MAX_SYMBOLS, PK_OPT_TEST_STALL, PK_OPT_BULK_MIN_LIVE = 1, 2, 3, 4, 5
 PK_OPT_BULK_SCREEN, PK_OPT_BULK_I8, PK_OPT_BULK_TMA_A = 6, 7, 8
+PK_GGML_F32, PK_GGML_F16, PK_GGML_Q8_0, PK_GGML_BF16, PK_GGML_MXFP4 = 0, 1, 8, 30, 39
+PK_SAMPLE_MAX_VOCAB = 524288
 PK_MATH_F32, PK_MATH_TC, PK_MATH_Q8 = 0, 1, 2
 
 STATUS_NAMES = {0: "PK_OK", 1: "PK_ERR_DMODEL", 2: "PK_ERR_INVALID", 3: "PK_ERR_MODEL",
@@ -84,6 +86,18 @@ class pk_stream_state(C.Structure):
                 ("segment_start_token", C.c_int32)]
 
 
+class pk_sample_args(C.Structure):
+    _fields_ = [("logits", C.c_void_p), ("logits_type", C.c_int32), ("vocab", C.c_int32), ("rows", C.c_int64),
+                ("row_stride", C.c_int64), ("uniforms", C.c_void_p), ("tokens", C.c_void_p), ("logprobs", C.c_void_p),
+                ("temperature", C.c_float), ("top_k", C.c_int32), ("top_p", C.c_float), ("min_p", C.c_float),
+                ("temperatures", C.c_void_p), ("top_ks", C.c_void_p), ("top_ps", C.c_void_p), ("min_ps", C.c_void_p)]
+
+
+class pk_ctc_draw(C.Structure):
+    _fields_ = [("temperature", C.c_float), ("top_k", C.c_int32), ("top_p", C.c_float), ("min_p", C.c_float),
+                ("uniforms", C.c_void_p), ("uniforms_on_device", C.c_int32), ("reserved", C.c_int32)]
+
+
 # Every symbol include/parakeet_cuda.h declares (checked by the CPU test suite).
 EXPORTED_SYMBOLS = [
     "pk_create", "pk_destroy", "pk_get_info", "pk_set_option", "pk_last_error",
@@ -92,6 +106,8 @@ EXPORTED_SYMBOLS = [
     "pk_stream_get_state", "pk_stream_set_state", "pk_shard_lpt", "pk_decode_noalloc",
     "pk_ctc_create", "pk_ctc_destroy", "pk_ctc_greedy", "pk_vocab_create", "pk_vocab_destroy",
     "pk_detokenize", "pk_prefetch_batch", "pk_shard_balanced",
+    "pk_mx4_quantize", "pk_mx4_dequantize", "pk_mx4_create", "pk_mx4_destroy", "pk_mx4_workspace",
+    "pk_mx4_linear", "pk_sample", "pk_ctc_decode",
 ]
 
 

@@ -279,6 +279,9 @@ cudaError_t launch_copy_segments(const HostSegments & g, cudaStream_t s);
 cudaError_t launch_extract_field(const int32_t * ust, int B, int field, int32_t * dst,
                                  cudaStream_t s);
 
+// pk_mx4.cu: a layer's device, outputs N and inputs K (any may be null).
+void mx4_dims(const pk_mx4 * w, int * device, int * N, int * K);
+
 // Read-only view of a context for entry points defined outside pk_api.cu.
 struct CtxView {
     int device, grid, chunk, ldx;

@@ -1,0 +1,467 @@
+// pk_mx4.cu -- 4-bit microscaled floating point: quantisation of rows, the values back,
+// and the product of quantised rows with a quantised weight matrix.
+//
+// A block of 32 values of a row is held as 32 e2m1 codes (sign, two exponent bits, one
+// mantissa bit: magnitudes 0, .5, 1, 1.5, 2, 3, 4, 6) and one e8m0 scale byte B, value =
+// code * 2^(B - 127). With a = max |x| of the block, B - 127 = max(floor(log2 a) - 2, -127):
+// the top code's exponent is 2, so a / 2^(B - 127) lies in [4, 8) and what exceeds 6 saturates.
+// floor(log2 a) is a's exponent field, so B = max(field - 2, 0), exactly, subnormals included;
+// x / 2^(B - 127) is an exact f32 product with 2^(127 - B) and the code its nearest value, ties
+// to the even code.
+
+#include "pk_ops.cuh"
+
+#include <algorithm>
+#include <new>
+
+namespace pk {
+namespace {
+
+constexpr int kQThreads = 256;
+
+// Scales in the layout of the product: 128-row atoms of 4 blocks (K = 128) each, 512 bytes; row r,
+// block b at byte (r % 32) * 16 + (r / 32) * 4 + b: 32 rows of four words, a word = the four
+// blocks of one row. `chunks` atoms per 128 rows, an even number: stages are two atoms deep.
+__host__ __device__ inline int scale_chunks(int K) { return 2 * ((K + 255) / 256); }
+__device__ __forceinline__ size_t scale_at(long long row, int blk, int chunks) {
+    return ((size_t) (row >> 7) * chunks + (blk >> 2)) * 512 + (size_t) ((row & 31) * 16 + ((row >> 5) & 3) * 4 + (blk & 3));
+}
+
+// Scale byte of a block from the bits of its largest magnitude; 255 (NaN) for Inf or NaN.
+__device__ __forceinline__ unsigned scale_byte(unsigned amax_bits) {
+    const unsigned field = amax_bits >> 23;
+    return field == 255u ? 255u : (field > 2u ? field - 2u : 0u);
+}
+
+// 2^(127 - B) and 2^(B - 127).
+__device__ __forceinline__ float scale_inv(unsigned b) { return __uint_as_float((254u - b) << 23); }
+__device__ __forceinline__ float scale_val(unsigned b) {
+    return __uint_as_float(b == 255u ? 0x7FC00000u : b == 0u ? 0x00400000u : b << 23);
+}
+
+// Two e2m1 codes, lo in bits 0-3 and hi in bits 4-7: nearest, ties to even, saturating.
+__device__ __forceinline__ unsigned cvt_e2m1x2(float lo, float hi) {
+    unsigned r;
+    asm("{ .reg .b8 t; cvt.rn.satfinite.e2m1x2.f32 t, %1, %2; cvt.u32.u8 %0, t; }" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+// Eight consecutive elements of a row from column c; zeros from column K on.
+template <class T, bool VEC>
+__device__ __forceinline__ void load8(const T * __restrict__ row, int c, int K, float * v) {
+    if (VEC && c + 8 <= K) {
+        if constexpr (sizeof(T) == 4) {
+            const float4 a = *reinterpret_cast<const float4 *>(row + c), b = *reinterpret_cast<const float4 *>(row + c + 4);
+            v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+            v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+        } else {
+            const uint4 a = *reinterpret_cast<const uint4 *>(row + c);
+            const unsigned w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                T e[2];
+                *reinterpret_cast<unsigned *>(e) = w[i];
+                v[2 * i] = to_f32(e[0]);
+                v[2 * i + 1] = to_f32(e[1]);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = c + i < K ? to_f32(row[c + i]) : 0.0f;
+    }
+}
+
+// One warp quantises 256 consecutive values of a row: eight per lane, four lanes a block.
+// ATOMS: scales in the product's layout, zeros for the blocks past K that its stages read.
+template <class T, bool VEC, bool ATOMS>
+__global__ void __launch_bounds__(kQThreads) mx4_quantize_kernel(const T * __restrict__ x, long long rows, int K, long long ldx,
+                                                                 unsigned char * __restrict__ codes,
+                                                                 unsigned char * __restrict__ scales) {
+    const int lane = threadIdx.x & 31;
+    const int segs = (K + 255) >> 8, nb = (K + 31) >> 5;
+    const long long tasks = rows * segs, stride = (long long) gridDim.x * (kQThreads / 32);
+    for (long long t = (long long) blockIdx.x * (kQThreads / 32) + (threadIdx.x >> 5); t < tasks; t += stride) {
+        const long long row = t / segs;
+        const int seg = (int) (t - row * segs);
+        const int c = seg * 256 + lane * 8;
+        const int blk = seg * 8 + (lane >> 2);
+        float v[8];
+        load8<T, VEC>(x + row * ldx, c, K, v);
+        unsigned m = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7FFFFFFFu);   // Inf < NaN as integers
+        m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
+        m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 2));
+        const unsigned sb = scale_byte(m);
+        unsigned q = 0;
+        if (sb != 255u) {
+            const float inv = scale_inv(sb);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) q |= cvt_e2m1x2(v[2 * i] * inv, v[2 * i + 1] * inv) << (8 * i);
+        }
+        if (blk < nb) *reinterpret_cast<unsigned *>(codes + (size_t) row * nb * 16 + (size_t) seg * 128 + lane * 4) = q;
+        if (ATOMS) {
+            // the four bytes of a chunk's word, gathered to lanes 0 and 16
+            unsigned w = sb;
+            w |= __shfl_down_sync(0xFFFFFFFFu, sb, 4) << 8;
+            w |= __shfl_down_sync(0xFFFFFFFFu, sb, 8) << 16;
+            w |= __shfl_down_sync(0xFFFFFFFFu, sb, 12) << 24;
+            if ((lane & 15) == 0)
+                *reinterpret_cast<unsigned *>(scales + scale_at(row, blk, scale_chunks(K))) = w;
+        } else if ((lane & 3) == 0 && blk < nb) {
+            scales[(size_t) row * nb + blk] = (unsigned char) sb;
+        }
+    }
+}
+
+// The value of each code: one thread per eight values.
+template <class T, bool VEC>
+__global__ void __launch_bounds__(kQThreads) mx4_dequantize_kernel(const unsigned char * __restrict__ codes,
+                                                                   const unsigned char * __restrict__ scales, long long rows,
+                                                                   int K, T * __restrict__ y, long long ldy) {
+    const int lane = threadIdx.x & 31;
+    const int segs = (K + 255) >> 8, nb = (K + 31) >> 5;
+    const long long tasks = rows * segs, stride = (long long) gridDim.x * (kQThreads / 32);
+    for (long long t = (long long) blockIdx.x * (kQThreads / 32) + (threadIdx.x >> 5); t < tasks; t += stride) {
+        const long long row = t / segs;
+        const int seg = (int) (t - row * segs);
+        const int c = seg * 256 + lane * 8;
+        const int blk = seg * 8 + (lane >> 2);
+        if (c >= K) continue;
+        const unsigned q = *reinterpret_cast<const unsigned *>(codes + (size_t) row * nb * 16 + (size_t) seg * 128 + lane * 4);
+        const float s = scale_val(scales[(size_t) row * nb + blk]);
+        T o[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const unsigned code = (q >> (4 * i)) & 15u, e = (code >> 1) & 3u, man = code & 1u;
+            const float mag = e == 0u ? 0.5f * (float) man : __uint_as_float(((126u + e) << 23) | (man << 22));
+            o[i] = from_f32<T>((code & 8u) ? -mag * s : mag * s);
+        }
+        T * d = y + row * ldy + c;
+        if (VEC && c + 8 <= K) {
+            const uint4 * w = reinterpret_cast<const uint4 *>(o);
+#pragma unroll
+            for (int i = 0; i < (int) (8 * sizeof(T) / 16); ++i) reinterpret_cast<uint4 *>(d)[i] = w[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (c + i < K) d[i] = o[i];
+        }
+    }
+}
+
+// GGUF MXFP4 blocks (17 bytes: the scale byte, then 16 bytes whose low halves are values 0-15 and
+// high halves values 16-31) to codes in value order and scale atoms. One thread per block.
+__global__ void __launch_bounds__(kQThreads) mx4_repack_kernel(const unsigned char * __restrict__ src, long long rows, int nb,
+                                                               unsigned char * __restrict__ codes,
+                                                               unsigned char * __restrict__ scales) {
+    const long long i = (long long) blockIdx.x * kQThreads + threadIdx.x;
+    if (i >= rows * nb) return;
+    const long long row = i / nb;
+    const int blk = (int) (i - row * nb);
+    const unsigned char * b = src + i * 17;
+    unsigned char * c = codes + i * 16;
+    const int chunks = scale_chunks(nb * 32);
+    scales[scale_at(row, blk, chunks)] = b[0];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const unsigned lo = b[1 + 2 * j], hi = b[2 + 2 * j];
+        c[j] = (unsigned char) ((lo & 15u) | (hi & 15u) << 4);
+        c[8 + j] = (unsigned char) (lo >> 4 | (hi & 0xF0u));
+    }
+}
+
+// ---- product -------------------------------------------------------------------
+
+// Eight codes to eight signed bytes of twice their value (0, 1, 2, 3, 4, 6, 8, 12).
+__device__ __forceinline__ void codes_to_s8(unsigned q, unsigned & even, unsigned & odd) {
+    auto four = [](unsigned nib) {   // a code in the low half of each byte
+        const unsigned sel = nib & 0x07070707u;
+        const unsigned packed = (sel & 7u) | (sel >> 4 & 0x70u) | (sel >> 8 & 0x700u) | (sel >> 12 & 0x7000u);
+        const unsigned mag = __byte_perm(0x03020100u, 0x0C080604u, packed);
+        const unsigned neg = (nib >> 3 & 0x01010101u) * 0xFFu;
+        return __vsub4(mag ^ neg, neg);
+    };
+    even = four(q & 0x0F0F0F0Fu);
+    odd = four(q >> 4 & 0x0F0F0F0Fu);
+}
+
+constexpr int kSM = 32, kSN = 64;   // tile of the CUDA-core product
+
+// A thread holds eight rows of one column; block dot products are exact integers.
+template <class T>
+__global__ void __launch_bounds__(256) mx4_simple_kernel(const unsigned char * __restrict__ xc, const unsigned char * __restrict__ xs,
+                                                         long long M, int K, const unsigned char * __restrict__ wc,
+                                                         const unsigned char * __restrict__ ws, int N,
+                                                         const float * __restrict__ bias, T * __restrict__ y, long long ldy) {
+    __shared__ unsigned sx[kSM][8], sw[kSN][9];
+    __shared__ float fx[kSM], fw[kSN];
+    const int nb = (K + 31) >> 5, chunks = scale_chunks(K);
+    const long long m0 = (long long) blockIdx.x * kSM;
+    const int n0 = blockIdx.y * kSN;
+    const int col = threadIdx.x & 63, r0 = (threadIdx.x >> 6) * 8;
+    float acc[8] = {};
+    for (int b = 0; b < nb; ++b) {
+        for (int i = threadIdx.x; i < (kSM + kSN) * 4; i += 256) {
+            const int r = i >> 2, part = i & 3;
+            const bool is_x = r < kSM;
+            const long long row = is_x ? m0 + r : n0 + (r - kSM);
+            unsigned q = 0;
+            if (row < (is_x ? M : (long long) N)) {
+                q = *reinterpret_cast<const unsigned *>((is_x ? xc : wc) + ((size_t) row * nb + b) * 16 + part * 4);
+                if (part == 0) (is_x ? fx[r] : fw[r - kSM]) = scale_val((is_x ? xs : ws)[scale_at(row, b, chunks)]);
+            }
+            unsigned e, o;
+            codes_to_s8(q, e, o);
+            unsigned * d = is_x ? &sx[r][part * 2] : &sw[r - kSM][part * 2];
+            d[0] = e;
+            d[1] = o;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            int dot = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) dot = __dp4a((int) sx[r0 + j][i], (int) sw[col][i], dot);
+            acc[j] += 0.25f * (float) dot * fx[r0 + j] * fw[col];
+        }
+        __syncthreads();
+    }
+    if (n0 + col < N) {
+        const float bv = bias ? bias[n0 + col] : 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (m0 + r0 + j < M) y[(m0 + r0 + j) * ldy + n0 + col] = from_f32<T>(acc[j] + bv);
+    }
+}
+
+// Launch of a row kernel: one warp per 256 values, as many blocks as that takes up to a few waves.
+inline unsigned row_blocks(long long rows, long long K) {
+    const long long tasks = rows * ((K + 255) / 256);
+    return (unsigned) std::min<long long>((tasks + kQThreads / 32 - 1) / (kQThreads / 32), 148LL * 64);
+}
+
+template <bool ATOMS>
+cudaError_t launch_quantize(const void * x, int type, long long rows, int K, long long ldx, unsigned char * codes,
+                            unsigned char * scales, cudaStream_t s) {
+    if (rows <= 0) return cudaSuccess;
+    const bool vec = aligned_to(x, 16) && (ldx * elem_size(type)) % 16 == 0;
+    const unsigned g = row_blocks(rows, K);
+#define PK_Q(T) \
+    if (vec) mx4_quantize_kernel<T, true, ATOMS><<<g, kQThreads, 0, s>>>(static_cast<const T *>(x), rows, K, ldx, codes, scales); \
+    else mx4_quantize_kernel<T, false, ATOMS><<<g, kQThreads, 0, s>>>(static_cast<const T *>(x), rows, K, ldx, codes, scales)
+    if (type == PK_GGML_F32) { PK_Q(float); }
+    else if (type == PK_GGML_F16) { PK_Q(__half); }
+    else { PK_Q(__nv_bfloat16); }
+#undef PK_Q
+    return cudaGetLastError();
+}
+
+cudaError_t launch_simple(const unsigned char * xc, const unsigned char * xs, long long M, int K, const unsigned char * wc,
+                          const unsigned char * ws, int N, const float * bias, void * y, int type, long long ldy,
+                          cudaStream_t s) {
+    const dim3 g((unsigned) ((M + kSM - 1) / kSM), (unsigned) ((N + kSN - 1) / kSN));
+    if (type == PK_GGML_F32)
+        mx4_simple_kernel<float><<<g, 256, 0, s>>>(xc, xs, M, K, wc, ws, N, bias, static_cast<float *>(y), ldy);
+    else if (type == PK_GGML_F16)
+        mx4_simple_kernel<__half><<<g, 256, 0, s>>>(xc, xs, M, K, wc, ws, N, bias, static_cast<__half *>(y), ldy);
+    else
+        mx4_simple_kernel<__nv_bfloat16><<<g, 256, 0, s>>>(xc, xs, M, K, wc, ws, N, bias, static_cast<__nv_bfloat16 *>(y), ldy);
+    return cudaGetLastError();
+}
+
+constexpr int64_t kMaxDim = 1 << 20;        // K, N
+constexpr int64_t kMaxRows = 0x7FFFFFFF;
+
+}  // namespace
+}  // namespace pk
+
+struct pk_mx4 {
+    int device = 0;
+    int N = 0, K = 0, nb = 0, chunks = 0;
+    unsigned char * codes = nullptr;    // [N][16 nb]
+    unsigned char * scales = nullptr;   // atoms
+    float * bias = nullptr;
+};
+
+namespace pk {
+
+void mx4_dims(const pk_mx4 * w, int * device, int * N, int * K) {
+    if (device) *device = w->device;
+    if (N) *N = w->N;
+    if (K) *K = w->K;
+}
+
+}  // namespace pk
+
+namespace {
+
+using namespace pk;
+
+// What quantize and dequantize refuse alike.
+pk_status check_rows(const char * fn, int device, int type, int64_t rows, int64_t cols, int64_t stride, const void * a, int a_align,
+                     const void * codes, const void * scales) {
+    if (elem_size(type) == 0) return op_fail(PK_ERR_INVALID, fn, "element type must be F32, F16 or BF16");
+    if (rows < 0 || rows > kMaxRows || cols < 1 || cols > kMaxDim || stride < cols || stride > (INT64_MAX >> 34))
+        return op_fail(PK_ERR_INVALID, fn, "rows must be in [0, 2^31), cols in [1, 2^20], row_stride >= cols");
+    if (rows > 0 && (!a || !codes || !scales)) return op_fail(PK_ERR_INVALID, fn, "null pointer");
+    if (!aligned_to(a, (size_t) a_align)) return op_fail(PK_ERR_INVALID, fn, "rows must be aligned to their element");
+    if (!aligned_to(codes, 4)) return op_fail(PK_ERR_INVALID, fn, "codes must be 4-byte aligned");
+    if (!device_ok(device)) return op_fail(PK_ERR_NO_DEVICE, fn, "no sm_100 device with that index");
+    return PK_OK;
+}
+
+}  // namespace
+
+extern "C" PK_API pk_status pk_mx4_quantize(int device, const void * x, int32_t x_type, int64_t rows, int64_t cols,
+                                            int64_t row_stride, uint8_t * codes, uint8_t * scales, void * stream) {
+    const char * fn = "pk_mx4_quantize";
+    const pk_status st = check_rows(fn, device, x_type, rows, cols, row_stride, x, elem_size(x_type), codes, scales);
+    if (st != PK_OK || rows == 0) return st;
+    DeviceScope dev(device);
+    if (dev.err != cudaSuccess) return op_cuda_fail(dev.err, fn);
+    const cudaError_t e = launch_quantize<false>(x, x_type, rows, (int) cols, row_stride, codes, scales, (cudaStream_t) stream);
+    return e == cudaSuccess ? PK_OK : op_cuda_fail(e, fn);
+}
+
+extern "C" PK_API pk_status pk_mx4_dequantize(int device, const uint8_t * codes, const uint8_t * scales, int64_t rows, int64_t cols,
+                                              void * y, int32_t y_type, int64_t row_stride, void * stream) {
+    const char * fn = "pk_mx4_dequantize";
+    const pk_status st = check_rows(fn, device, y_type, rows, cols, row_stride, y, elem_size(y_type), codes, scales);
+    if (st != PK_OK || rows == 0) return st;
+    DeviceScope dev(device);
+    if (dev.err != cudaSuccess) return op_cuda_fail(dev.err, fn);
+    const bool vec = aligned_to(y, 16) && (row_stride * elem_size(y_type)) % 16 == 0;
+    const unsigned g = row_blocks(rows, cols);
+    cudaStream_t s = (cudaStream_t) stream;
+#define PK_D(T) \
+    if (vec) mx4_dequantize_kernel<T, true><<<g, kQThreads, 0, s>>>(codes, scales, rows, (int) cols, static_cast<T *>(y), row_stride); \
+    else mx4_dequantize_kernel<T, false><<<g, kQThreads, 0, s>>>(codes, scales, rows, (int) cols, static_cast<T *>(y), row_stride)
+    if (y_type == PK_GGML_F32) { PK_D(float); }
+    else if (y_type == PK_GGML_F16) { PK_D(__half); }
+    else { PK_D(__nv_bfloat16); }
+#undef PK_D
+    const cudaError_t e = cudaGetLastError();
+    return e == cudaSuccess ? PK_OK : op_cuda_fail(e, fn);
+}
+
+extern "C" PK_API void pk_mx4_destroy(pk_mx4 * w) {
+    if (!w) return;
+    DeviceScope dev(w->device);
+    cudaDeviceSynchronize();
+    cudaFree(w->codes);
+    cudaFree(w->scales);
+    cudaFree(w->bias);
+    delete w;
+}
+
+extern "C" PK_API pk_status pk_mx4_create(int device, const pk_tensor * weight, int32_t on_device, const float * bias, pk_mx4 ** out) {
+    const char * fn = "pk_mx4_create";
+    if (!out) return op_fail(PK_ERR_INVALID, fn, "null output");
+    *out = nullptr;
+    if (!weight || !weight->data) return op_fail(PK_ERR_INVALID, fn, "null weight");
+    const int64_t K = weight->ne0, N = weight->ne1;
+    if (K < 1 || K > kMaxDim || N < 1 || N > kMaxDim) return op_fail(PK_ERR_MODEL, fn, "weight dimensions must be in [1, 2^20]");
+    const int type = weight->type;
+    const bool blocks = type == PK_GGML_Q8_0 || type == PK_GGML_MXFP4;
+    if (!blocks && elem_size(type) == 0) return op_fail(PK_ERR_MODEL, fn, "weight type must be F32, F16, BF16, Q8_0 or MXFP4");
+    if (blocks && K % 32 != 0) return op_fail(PK_ERR_MODEL, fn, "ne0 of a block type must be a multiple of 32");
+    const uint64_t want = blocks ? (uint64_t) N * (K / 32) * (type == PK_GGML_Q8_0 ? 34 : 17) : (uint64_t) N * K * elem_size(type);
+    if (weight->nbytes != want) return op_fail(PK_ERR_MODEL, fn, "weight nbytes does not match its type and shape");
+    const size_t w_align = type == PK_GGML_MXFP4 ? 1 : type == PK_GGML_Q8_0 ? 2 : (size_t) elem_size(type);
+    if (on_device && (!aligned_to(weight->data, w_align) || (bias && !aligned_to(bias, 4))))
+        return op_fail(PK_ERR_INVALID, fn, "device weight and bias must be aligned to their element");
+    if (!device_ok(device)) return op_fail(PK_ERR_NO_DEVICE, fn, "no sm_100 device with that index");
+    DeviceScope dev(device);
+    if (dev.err != cudaSuccess) return op_cuda_fail(dev.err, fn);
+    pk_mx4 * w = new (std::nothrow) pk_mx4();
+    if (!w) return op_fail(PK_ERR_OOM, fn, "host memory");
+    w->device = device;
+    w->N = (int) N;
+    w->K = (int) K;
+    w->nb = (int) ((K + 31) / 32);
+    w->chunks = scale_chunks((int) K);
+    const size_t code_bytes = (size_t) N * w->nb * 16, scale_bytes = (size_t) ((N + 127) / 128) * w->chunks * 512;
+    void * raw = nullptr;    // a host weight's copy
+    void * f32 = nullptr;    // q8_0 blocks dequantised
+    cudaStream_t s = nullptr;
+    cudaError_t e = on_device ? cudaDeviceSynchronize() : cudaSuccess;
+    if (e == cudaSuccess) e = cudaStreamCreateWithFlags(&s, cudaStreamNonBlocking);
+    if (e == cudaSuccess) e = cudaMalloc(&w->codes, code_bytes);
+    if (e == cudaSuccess) e = cudaMalloc(&w->scales, scale_bytes);
+    if (e == cudaSuccess) e = cudaMemsetAsync(w->scales, 0, scale_bytes, s);
+    const void * src = weight->data;
+    if (e == cudaSuccess && !on_device) {
+        e = cudaMalloc(&raw, want);
+        if (e == cudaSuccess) e = cudaMemcpyAsync(raw, weight->data, want, cudaMemcpyHostToDevice, s);
+        src = raw;
+    }
+    if (e == cudaSuccess && type == PK_GGML_MXFP4) {
+        const long long n = N * (long long) w->nb;
+        mx4_repack_kernel<<<(unsigned) ((n + kQThreads - 1) / kQThreads), kQThreads, 0, s>>>(
+            static_cast<const unsigned char *>(src), N, w->nb, w->codes, w->scales);
+        e = cudaGetLastError();
+    } else if (e == cudaSuccess && type == PK_GGML_Q8_0) {
+        e = cudaMalloc(&f32, (size_t) N * K * 4);
+        if (e == cudaSuccess) e = launch_dequant(src, type, K, N, static_cast<float *>(f32), s);
+        if (e == cudaSuccess) e = launch_quantize<true>(f32, PK_GGML_F32, N, (int) K, K, w->codes, w->scales, s);
+    } else if (e == cudaSuccess) {
+        e = launch_quantize<true>(src, type, N, (int) K, K, w->codes, w->scales, s);
+    }
+    if (e == cudaSuccess && bias) {
+        e = cudaMalloc(&w->bias, (size_t) N * 4);
+        if (e == cudaSuccess)
+            e = cudaMemcpyAsync(w->bias, bias, (size_t) N * 4, on_device ? cudaMemcpyDeviceToDevice : cudaMemcpyHostToDevice, s);
+    }
+    if (s) {
+        const cudaError_t e2 = cudaStreamSynchronize(s);
+        if (e == cudaSuccess) e = e2;
+        cudaStreamDestroy(s);
+    }
+    cudaFree(raw);
+    cudaFree(f32);
+    if (e != cudaSuccess) {
+        pk_mx4_destroy(w);
+        return op_cuda_fail(e, fn);
+    }
+    *out = w;
+    return PK_OK;
+}
+
+namespace {
+
+size_t ws_codes(const pk_mx4 * w, int64_t rows) { return ((size_t) rows * w->nb * 16 + 255) / 256 * 256; }
+
+}  // namespace
+
+extern "C" PK_API int64_t pk_mx4_workspace(const pk_mx4 * w, int64_t rows) {
+    if (!w) return -1;
+    if (rows <= 0) return 0;
+    return (int64_t) (ws_codes(w, rows) + (size_t) ((rows + 127) / 128) * w->chunks * 512);
+}
+
+extern "C" PK_API pk_status pk_mx4_linear(pk_mx4 * w, const void * x, int32_t x_type, int64_t rows, int64_t x_stride, void * y,
+                                          int32_t y_type, int64_t y_stride, void * workspace, int64_t workspace_bytes,
+                                          void * stream) {
+    const char * fn = "pk_mx4_linear";
+    if (!w) return op_fail(PK_ERR_INVALID, fn, "null layer");
+    if (elem_size(x_type) == 0 || elem_size(y_type) == 0) return op_fail(PK_ERR_INVALID, fn, "element types must be F32, F16 or BF16");
+    if (rows < 0 || rows > kMaxRows) return op_fail(PK_ERR_INVALID, fn, "rows must be in [0, 2^31)");
+    if (x_stride < w->K || y_stride < w->N || x_stride > (INT64_MAX >> 34) || y_stride > (INT64_MAX >> 34))
+        return op_fail(PK_ERR_INVALID, fn, "x_stride must be at least K and y_stride at least N");
+    if (rows == 0) return PK_OK;
+    if (!x || !y || !workspace) return op_fail(PK_ERR_INVALID, fn, "null pointer");
+    if (!aligned_to(x, (size_t) elem_size(x_type)) || !aligned_to(y, (size_t) elem_size(y_type)))
+        return op_fail(PK_ERR_INVALID, fn, "x and y must be aligned to their element");
+    if (!aligned_to(workspace, 256)) return op_fail(PK_ERR_INVALID, fn, "workspace must be 256-byte aligned");
+    if (workspace_bytes < pk_mx4_workspace(w, rows))
+        return op_fail(PK_ERR_INVALID, fn, "workspace_bytes is below pk_mx4_workspace(w, rows)");
+    DeviceScope dev(w->device);
+    if (dev.err != cudaSuccess) return op_cuda_fail(dev.err, fn);
+    cudaStream_t s = (cudaStream_t) stream;
+    unsigned char * xc = static_cast<unsigned char *>(workspace);
+    unsigned char * xs = xc + ws_codes(w, rows);
+    cudaError_t e = launch_quantize<true>(x, x_type, rows, w->K, x_stride, xc, xs, s);
+    if (e == cudaSuccess) e = launch_simple(xc, xs, rows, w->K, w->codes, w->scales, w->N, w->bias, y, y_type, y_stride, s);
+    return e == cudaSuccess ? PK_OK : op_cuda_fail(e, fn);
+}

@@ -1,5 +1,5 @@
-// pk_text.cu -- the two steps beside the token loop: CTC greedy decode
-// (src/parakeet_ctc.cpp:1820-1865) and SentencePiece detokenize
+// pk_text.cu -- the two steps beside the token loop: CTC decode (greedy,
+// src/parakeet_ctc.cpp:1820-1865, or a drawn path) and SentencePiece detokenize
 // (src/sentencepiece_bpe.cpp:9-37), batched over utterances on the GPU.
 //
 // Both are byte / integer work bound by HBM (the logits) or by latency (the
@@ -144,10 +144,13 @@ __global__ void __launch_bounds__(kTxtThreads) ctc_argmax_kernel(const float * _
     }
 }
 
+__device__ __forceinline__ int frame_token(const int * best, int64_t f, int blank) { return best[f] < 0 ? blank : best[f]; }
+
 // One CTA per utterance: a frame emits its argmax when it is not blank and
 // differs from the previous frame's (the window's first frame compares with
 // prev_in); emitted tokens and their frames go compacted to the utterance's
-// region (n_frames entries at region_off: at most one token per frame).
+// region (n_frames entries at region_off: at most one token per frame). A frame
+// that could draw nothing (token -1) counts as blank.
 __global__ void __launch_bounds__(kTxtThreads) ctc_collapse_kernel(const int * __restrict__ best,
                                                                    const int64_t * __restrict__ frame_off,
                                                                    const int * __restrict__ n_frames,
@@ -165,8 +168,8 @@ __global__ void __launch_bounds__(kTxtThreads) ctc_collapse_kernel(const int * _
         const int t = t0 + (int) threadIdx.x;
         int tok = 0, e = 0;
         if (t < n) {
-            tok = best[f0 + t];
-            const int prev = t == 0 ? p0 : best[f0 + t - 1];
+            tok = frame_token(best, f0 + t, blank);
+            const int prev = t == 0 ? p0 : frame_token(best, f0 + t - 1, blank);
             e = (tok != blank && tok != prev) ? 1 : 0;
         }
         int tot = 0;
@@ -179,7 +182,7 @@ __global__ void __launch_bounds__(kTxtThreads) ctc_collapse_kernel(const int * _
     }
     if (threadIdx.x == 0) {
         counts[b] = count;
-        prev_out[b] = n > 0 ? best[f0 + n - 1] : p0;
+        prev_out[b] = n > 0 ? frame_token(best, f0 + n - 1, blank) : p0;
     }
 }
 
@@ -280,6 +283,7 @@ struct pk_ctc {
     cudaStream_t stream = nullptr;
     int V = 0, blank = 0;
     pk::Buf logits, best, foff, roff, nfr, prev_in, prev_out, rtok, rframe, counts, offs, otok, oframe;
+    pk::Buf frames, work, uniforms;   // pk_ctc_decode: encoder frames, product workspace, random numbers
 };
 
 struct pk_vocab {
@@ -326,20 +330,79 @@ extern "C" PK_API void pk_ctc_destroy(pk_ctc * c) {
     cudaSetDevice(c->device);
     if (c->stream) cudaStreamSynchronize(c->stream);
     for (pk::Buf * b : {&c->logits, &c->best, &c->foff, &c->roff, &c->nfr, &c->prev_in, &c->prev_out, &c->rtok, &c->rframe,
-                        &c->counts, &c->offs, &c->otok, &c->oframe})
+                        &c->counts, &c->offs, &c->otok, &c->oframe, &c->frames, &c->work, &c->uniforms})
         b->release();
     if (c->stream) cudaStreamDestroy(c->stream);
     delete c;
 }
 
-extern "C" PK_API pk_status pk_ctc_greedy(pk_ctc * c, const float * logits, int32_t logits_on_device,
-                                          const int64_t * frame_offsets, const int32_t * n_frames, int32_t B,
-                                          int32_t * prev_inout, int32_t * tokens, int64_t tokens_cap,
-                                          int64_t * token_offsets, int32_t * first_frame, int64_t * tokens_needed) {
+namespace {
+
+// Frames per product of pk_ctc_decode: bounds its logits (0.5 GB at 8193 tokens).
+constexpr int64_t kHeadFrames = 16384;
+
+// Logits of every frame (`x` itself, or head * x) to its token in c->best: the argmax or a draw.
+pk_status ctc_frame_tokens(pk_ctc * c, const char * fn, pk_mx4 * head, const float * dx, int64_t frames, const pk_ctc_draw * draw,
+                           const float * duni) {
     using namespace pk;
+    cudaStream_t s = c->stream;
+    int K = c->V;
+    if (head) mx4_dims(head, nullptr, nullptr, &K);
+    const int64_t step = head ? std::min(frames, kHeadFrames) : frames;
+    if (head) {
+        const int64_t ws = pk_mx4_workspace(head, step);
+        TX_CK(c->logits.ensure((size_t) step * c->V * 4), fn);
+        TX_CK(c->work.ensure((size_t) ws), fn);
+    }
+    for (int64_t f = 0; f < frames; f += step) {
+        const int64_t n = std::min(step, frames - f);
+        const float * logits = dx + f * (int64_t) K;
+        int * best = c->best.as<int>() + f;
+        if (head) {
+            const pk_status st = pk_mx4_linear(head, logits, PK_GGML_F32, n, K, c->logits.p, PK_GGML_F32, c->V, c->work.p,
+                                               (int64_t) c->work.cap, s);
+            if (st != PK_OK) return st;
+            logits = c->logits.as<float>();
+        }
+        if (draw) {
+            pk_sample_args a{};
+            a.logits = logits;
+            a.logits_type = PK_GGML_F32;
+            a.vocab = c->V;
+            a.rows = n;
+            a.row_stride = c->V;
+            a.uniforms = duni + f;
+            a.tokens = best;
+            a.temperature = draw->temperature;
+            a.top_k = draw->top_k;
+            a.top_p = draw->top_p;
+            a.min_p = draw->min_p;
+            const pk_status st = pk_sample(c->device, &a, s);
+            if (st != PK_OK) return st;
+        } else {
+            const int blocks = (int) std::min<long long>((n + 7) / 8, 148LL * 8);
+            ctc_argmax_kernel<<<blocks, kTxtThreads, 0, s>>>(logits, n, c->V, best);
+            TX_CK(cudaGetLastError(), fn);
+        }
+    }
+    return PK_OK;
+}
+
+// pk_ctc_greedy and pk_ctc_decode: frames -> tokens -> collapse -> host arrays. `logits` are logits,
+// or, with a head, its input frames.
+pk_status ctc_decode(pk_ctc * c, const char * fn, pk_mx4 * head, const float * logits, int32_t logits_on_device,
+                     const int64_t * frame_offsets, const int32_t * n_frames, int32_t B, const pk_ctc_draw * draw,
+                     int32_t * prev_inout, int32_t * tokens, int64_t tokens_cap, int64_t * token_offsets, int32_t * first_frame,
+                     int64_t * tokens_needed) {
+    using namespace pk;
+    auto invalid = [&](const char * what) {
+        char msg[200];
+        std::snprintf(msg, sizeof(msg), "%s: %s", fn, what);
+        return set_error(PK_ERR_INVALID, msg);
+    };
     if (!c || B < 0 || (B > 0 && (!frame_offsets || !n_frames || !prev_inout || !token_offsets)) ||
         (tokens_cap > 0 && !tokens) || tokens_cap < 0)
-        return set_error(PK_ERR_INVALID, "pk_ctc_greedy: null argument or negative size");
+        return invalid("null argument or negative size");
     if (B == 0) {
         if (token_offsets) token_offsets[0] = 0;
         if (tokens_needed) *tokens_needed = 0;
@@ -351,61 +414,70 @@ extern "C" PK_API pk_status pk_ctc_greedy(pk_ctc * c, const float * logits, int3
     int64_t rtotal = 0;
     for (int b = 0; b < B; ++b) {
         if (n_frames[b] < 0 || frame_offsets[b] < 0)
-            return set_error(PK_ERR_INVALID, "pk_ctc_greedy: negative frame offset or count");
+            return invalid("negative frame offset or count");
         frames = std::max<int64_t>(frames, frame_offsets[b] + n_frames[b]);
         roff[b] = rtotal;
         rtotal += n_frames[b];
     }
     if (logits_on_device && (reinterpret_cast<uintptr_t>(logits) & 3u))
-        return set_error(PK_ERR_INVALID, "pk_ctc_greedy: device logits must be 4-byte aligned");
-    if (frames > 0 && !logits) return set_error(PK_ERR_INVALID, "pk_ctc_greedy: null logits");
-    TX_CK(cudaSetDevice(c->device), "pk_ctc_greedy: cudaSetDevice");
+        return invalid("device logits must be 4-byte aligned");
+    if (frames > 0 && !logits) return invalid("null logits");
+    if (frames > 0 && draw && !draw->uniforms) return invalid("null random numbers");
+    if (draw && draw->uniforms_on_device && (reinterpret_cast<uintptr_t>(draw->uniforms) & 3u))
+        return invalid("device random numbers must be 4-byte aligned");
+    TX_CK(cudaSetDevice(c->device), fn);
     cudaStream_t s = c->stream;
     const size_t fb = (size_t) std::max<int64_t>(frames, 1);
     const float * dlog = logits;
+    int width = c->V;
+    if (head) mx4_dims(head, nullptr, nullptr, &width);
     if (!logits_on_device && frames > 0) {
-        TX_CK(c->logits.ensure(fb * c->V * 4), "pk_ctc_greedy: alloc");
-        TX_CK(cudaMemcpyAsync(c->logits.p, logits, (size_t) frames * c->V * 4, cudaMemcpyHostToDevice, s),
-              "pk_ctc_greedy: logits copy");
-        dlog = c->logits.as<float>();
+        Buf & in = head ? c->frames : c->logits;
+        TX_CK(in.ensure(fb * width * 4), fn);
+        TX_CK(cudaMemcpyAsync(in.p, logits, (size_t) frames * width * 4, cudaMemcpyHostToDevice, s), fn);
+        dlog = in.as<float>();
+    }
+    const float * duni = draw ? draw->uniforms : nullptr;
+    if (draw && !draw->uniforms_on_device && frames > 0) {
+        TX_CK(c->uniforms.ensure(fb * 4), fn);
+        TX_CK(cudaMemcpyAsync(c->uniforms.p, draw->uniforms, (size_t) frames * 4, cudaMemcpyHostToDevice, s), fn);
+        duni = c->uniforms.as<float>();
     }
     const size_t rb = (size_t) std::max<int64_t>(rtotal, 1);
-    TX_CK(c->best.ensure(fb * 4), "pk_ctc_greedy: alloc");
-    TX_CK(c->rtok.ensure(rb * 4), "pk_ctc_greedy: alloc");
-    TX_CK(c->rframe.ensure(rb * 4), "pk_ctc_greedy: alloc");
-    TX_CK(c->otok.ensure(rb * 4), "pk_ctc_greedy: alloc");
-    TX_CK(c->oframe.ensure(rb * 4), "pk_ctc_greedy: alloc");
-    TX_CK(c->roff.ensure((size_t) B * 8), "pk_ctc_greedy: alloc");
-    TX_CK(c->foff.ensure((size_t) B * 8), "pk_ctc_greedy: alloc");
-    TX_CK(c->nfr.ensure((size_t) B * 4), "pk_ctc_greedy: alloc");
-    TX_CK(c->prev_in.ensure((size_t) B * 4), "pk_ctc_greedy: alloc");
-    TX_CK(c->prev_out.ensure((size_t) B * 4), "pk_ctc_greedy: alloc");
-    TX_CK(c->counts.ensure((size_t) B * 4), "pk_ctc_greedy: alloc");
-    TX_CK(c->offs.ensure((size_t) (B + 1) * 8), "pk_ctc_greedy: alloc");
-    TX_CK(cudaMemcpyAsync(c->foff.p, frame_offsets, (size_t) B * 8, cudaMemcpyHostToDevice, s), "pk_ctc_greedy: copy");
-    TX_CK(cudaMemcpyAsync(c->roff.p, roff.data(), (size_t) B * 8, cudaMemcpyHostToDevice, s), "pk_ctc_greedy: copy");
-    TX_CK(cudaMemcpyAsync(c->nfr.p, n_frames, (size_t) B * 4, cudaMemcpyHostToDevice, s), "pk_ctc_greedy: copy");
-    TX_CK(cudaMemcpyAsync(c->prev_in.p, prev_inout, (size_t) B * 4, cudaMemcpyHostToDevice, s), "pk_ctc_greedy: copy");
+    TX_CK(c->best.ensure(fb * 4), fn);
+    TX_CK(c->rtok.ensure(rb * 4), fn);
+    TX_CK(c->rframe.ensure(rb * 4), fn);
+    TX_CK(c->otok.ensure(rb * 4), fn);
+    TX_CK(c->oframe.ensure(rb * 4), fn);
+    TX_CK(c->roff.ensure((size_t) B * 8), fn);
+    TX_CK(c->foff.ensure((size_t) B * 8), fn);
+    TX_CK(c->nfr.ensure((size_t) B * 4), fn);
+    TX_CK(c->prev_in.ensure((size_t) B * 4), fn);
+    TX_CK(c->prev_out.ensure((size_t) B * 4), fn);
+    TX_CK(c->counts.ensure((size_t) B * 4), fn);
+    TX_CK(c->offs.ensure((size_t) (B + 1) * 8), fn);
+    TX_CK(cudaMemcpyAsync(c->foff.p, frame_offsets, (size_t) B * 8, cudaMemcpyHostToDevice, s), fn);
+    TX_CK(cudaMemcpyAsync(c->roff.p, roff.data(), (size_t) B * 8, cudaMemcpyHostToDevice, s), fn);
+    TX_CK(cudaMemcpyAsync(c->nfr.p, n_frames, (size_t) B * 4, cudaMemcpyHostToDevice, s), fn);
+    TX_CK(cudaMemcpyAsync(c->prev_in.p, prev_inout, (size_t) B * 4, cudaMemcpyHostToDevice, s), fn);
     if (frames > 0) {
-        const long long warps = frames;
-        const int blocks = (int) std::min<long long>((warps + 7) / 8, 148LL * 8);
-        ctc_argmax_kernel<<<blocks, kTxtThreads, 0, s>>>(dlog, frames, c->V, c->best.as<int>());
-        TX_CK(cudaGetLastError(), "pk_ctc_greedy: argmax launch");
+        const pk_status st = ctc_frame_tokens(c, fn, head, dlog, frames, draw, duni);
+        if (st != PK_OK) return st;
     }
     ctc_collapse_kernel<<<B, kTxtThreads, 0, s>>>(c->best.as<int>(), c->foff.as<int64_t>(), c->nfr.as<int>(),
                                                   c->roff.as<int64_t>(), c->prev_in.as<int>(), c->blank, c->rtok.as<int>(),
                                                   c->rframe.as<int>(), c->counts.as<int>(), c->prev_out.as<int>());
-    TX_CK(cudaGetLastError(), "pk_ctc_greedy: collapse launch");
+    TX_CK(cudaGetLastError(), fn);
     scan_offsets_kernel<<<1, kTxtThreads, 0, s>>>(c->counts.as<int>(), B, c->offs.as<int64_t>());
-    TX_CK(cudaGetLastError(), "pk_ctc_greedy: scan launch");
+    TX_CK(cudaGetLastError(), fn);
     TX_CK(cudaMemcpyAsync(token_offsets, c->offs.p, (size_t) (B + 1) * 8, cudaMemcpyDeviceToHost, s),
-          "pk_ctc_greedy: offsets copy");
-    TX_CK(cudaStreamSynchronize(s), "pk_ctc_greedy: sync");
+          fn);
+    TX_CK(cudaStreamSynchronize(s), fn);
     const int64_t total = token_offsets[B];
     if (tokens_needed) *tokens_needed = total;
     if (total > tokens_cap) {
         char msg[160];
-        std::snprintf(msg, sizeof(msg), "pk_ctc_greedy: %lld tokens > tokens_cap %lld", (long long) total,
+        std::snprintf(msg, sizeof(msg), "%s: %lld tokens > tokens_cap %lld", fn, (long long) total,
                       (long long) tokens_cap);
         return set_error(PK_ERR_CAPACITY, msg);
     }
@@ -414,16 +486,43 @@ extern "C" PK_API pk_status pk_ctc_greedy(pk_ctc * c, const float * logits, int3
     if (first_frame)
         gather_regions_kernel<<<B, kTxtThreads, 0, s>>>(c->rframe.as<int>(), c->roff.as<int64_t>(),
                                                         c->offs.as<int64_t>(), c->oframe.as<int>());
-    TX_CK(cudaGetLastError(), "pk_ctc_greedy: gather launch");
+    TX_CK(cudaGetLastError(), fn);
     if (total > 0) {
-        TX_CK(cudaMemcpyAsync(tokens, c->otok.p, (size_t) total * 4, cudaMemcpyDeviceToHost, s), "pk_ctc_greedy: copy");
+        TX_CK(cudaMemcpyAsync(tokens, c->otok.p, (size_t) total * 4, cudaMemcpyDeviceToHost, s), fn);
         if (first_frame)
             TX_CK(cudaMemcpyAsync(first_frame, c->oframe.p, (size_t) total * 4, cudaMemcpyDeviceToHost, s),
-                  "pk_ctc_greedy: copy");
+                  fn);
     }
-    TX_CK(cudaMemcpyAsync(prev_inout, c->prev_out.p, (size_t) B * 4, cudaMemcpyDeviceToHost, s), "pk_ctc_greedy: copy");
-    TX_CK(cudaStreamSynchronize(s), "pk_ctc_greedy: sync");
+    TX_CK(cudaMemcpyAsync(prev_inout, c->prev_out.p, (size_t) B * 4, cudaMemcpyDeviceToHost, s), fn);
+    TX_CK(cudaStreamSynchronize(s), fn);
     return PK_OK;
+}
+
+}  // namespace
+
+extern "C" PK_API pk_status pk_ctc_greedy(pk_ctc * c, const float * logits, int32_t logits_on_device,
+                                          const int64_t * frame_offsets, const int32_t * n_frames, int32_t B,
+                                          int32_t * prev_inout, int32_t * tokens, int64_t tokens_cap,
+                                          int64_t * token_offsets, int32_t * first_frame, int64_t * tokens_needed) {
+    return ctc_decode(c, "pk_ctc_greedy", nullptr, logits, logits_on_device, frame_offsets, n_frames, B, nullptr, prev_inout, tokens,
+                      tokens_cap, token_offsets, first_frame, tokens_needed);
+}
+
+extern "C" PK_API pk_status pk_ctc_decode(pk_ctc * c, pk_mx4 * head, const float * frames, int32_t frames_on_device,
+                                          const int64_t * frame_offsets, const int32_t * n_frames, int32_t B,
+                                          const pk_ctc_draw * draw, int32_t * prev_inout, int32_t * tokens, int64_t tokens_cap,
+                                          int64_t * token_offsets, int32_t * first_frame, int64_t * tokens_needed) {
+    using namespace pk;
+    if (c && head) {
+        int device = 0, N = 0;
+        mx4_dims(head, &device, &N, nullptr);
+        if (device != c->device || N != c->V)
+            return set_error(PK_ERR_INVALID, "pk_ctc_decode: the head must be on the handle's device and vocab_size wide");
+    }
+    if (c && c->V > PK_SAMPLE_MAX_VOCAB && draw)
+        return set_error(PK_ERR_INVALID, "pk_ctc_decode: vocab_size is above PK_SAMPLE_MAX_VOCAB");
+    return ctc_decode(c, "pk_ctc_decode", head, frames, frames_on_device, frame_offsets, n_frames, B, draw, prev_inout, tokens,
+                      tokens_cap, token_offsets, first_frame, tokens_needed);
 }
 
 extern "C" PK_API pk_status pk_vocab_create(int device, const uint8_t * piece_bytes, const int64_t * piece_offsets,

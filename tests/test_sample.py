@@ -1,0 +1,396 @@
+"""Drawing tokens from logits: pk_sample against the definition in f64, the CTC path that
+calls it, and the refusals."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+DEFAULTS = dict(temperature=1.0, top_k=0, top_p=1.0, min_p=0.0)
+
+
+@pytest.fixture(scope="module")
+def built(pk):
+    pk.build()
+    return pk
+
+
+def ref_row(l, u, temperature, top_k, top_p, min_p):
+    """(token, log-probability) of one row by sorting and summing in f64."""
+    l = np.asarray(l, np.float64)
+    v = len(l)
+    l = np.where(np.isnan(l), -np.inf, l)
+    top = l.max()
+    if top == -np.inf:
+        return -1, -np.inf
+    if not temperature > 0:
+        return int(np.argmax(l)), 0.0
+    a = np.full(v, -np.inf)
+    fine = (l > -np.inf) & (l < top) & (top < np.inf)   # a maximum of +infinity leaves the others nothing
+    with np.errstate(over="ignore"):
+        a[fine] = (l[fine] - top) / np.float64(np.float32(temperature))
+    a[l == top] = 0.0
+    w = np.exp(a)
+    w[w <= 2.0 ** -44] = 0.0                            # what 64-bit fixed point drops
+    order = np.argsort(-l, kind="stable")
+    n = v if top_k <= 0 else min(top_k, v)
+    s = w[order]
+    s[n:] = 0.0
+    if not top_p >= 1:
+        before = np.cumsum(s) - s
+        keep = before < np.float64(np.float32(top_p)) * s.sum() if top_p > 0 else np.zeros(v, bool)
+        keep[0] = True
+        s = np.where(keep, s, 0.0)
+    if min_p > 0:
+        s = np.where(s >= min(np.float64(np.float32(min_p)), 1.0), s, 0.0)
+    w = np.zeros(v)
+    w[order] = s
+    run = np.cumsum(w)
+    u = 0.0 if not u > 0 else min(float(np.float32(u)), float(np.float32(1 - 2 ** -24)))
+    tok = int(np.searchsorted(run, u * run[-1], side="right"))
+    tok = min(tok, int(np.flatnonzero(w)[-1]))
+    return tok, a[tok] - np.log(run[-1])
+
+
+def run(pk, l, u, dtype="f32", pad=0, shift=0, stream=None, rows_apart=False, **kw):
+    import torch
+    t = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}[dtype]
+    l = np.asarray(l, np.float32)
+    r, v = l.shape
+    buf = torch.full((r * (v + pad) + shift + 32,), 1e4, dtype=t, device="cuda")     # larger than any logit
+    x = buf[shift:shift + r * (v + pad)].view(r, v + pad)
+    x[:, :v] = torch.from_numpy(l).cuda().to(t)
+    uu = torch.from_numpy(np.asarray(u, np.float32)).cuda()
+    tok = torch.full((r + 8,), -7, dtype=torch.int32, device="cuda")
+    lp = torch.full((r + 8,), 123.0, device="cuda")
+    args, keep = {}, []
+    for name, val in kw.items():
+        if np.ndim(val):
+            d = torch.from_numpy(np.asarray(val, np.int32 if name == "top_k" else np.float32)).cuda()
+            keep.append(d)
+            args[name + "s"] = d.data_ptr()
+        else:
+            args[name] = val
+    s = torch.cuda.current_stream().cuda_stream if stream is None else stream
+    pk.sample(x.data_ptr(), r, v, uu.data_ptr(), tok.data_ptr(), dtype=dtype, row_stride=v + pad, logprobs=lp.data_ptr(),
+              stream=s, **args)
+    torch.cuda.synchronize()
+    assert (tok[r:] == -7).all() and (lp[r:] == 123.0).all()
+    return x[:, :v].float().cpu().numpy(), tok[:r].cpu().numpy(), lp[:r].cpu().numpy()
+
+
+def check(seen, u, tok, lp, **kw):
+    """Tokens equal; log-probabilities: a f64 number rounded once (2^-24 of it) whose sum of weights
+    is off by 2^-44 a token at most."""
+    kw = {**DEFAULTS, **kw}
+    r, v = seen.shape
+    for i in range(r):
+        one = {n: (x[i] if np.ndim(x) else x) for n, x in kw.items()}
+        t, p = ref_row(seen[i], u[i], **one)
+        assert tok[i] == t, (i, tok[i], t, one, u[i])
+        if np.isinf(p):
+            assert lp[i] == p
+        else:
+            assert abs(lp[i] - p) <= 2.0 ** -24 * abs(p) + v * 2.0 ** -43 + 2.0 ** -40, (i, lp[i], p)
+
+
+# ---- CPU -----------------------------------------------------------------------
+
+def test_reference_known_answers():
+    l = np.log([0.5, 0.25, 0.125, 0.125])
+    assert [ref_row(l, u, 1.0, 0, 1.0, 0.0)[0] for u in (0.0, 0.49, 0.51, 0.76, 0.9)] == [0, 0, 1, 2, 3]
+    assert [ref_row(l, u, 1.0, 2, 1.0, 0.0)[0] for u in (0.66, 0.67)] == [0, 1]
+    assert [ref_row(l, u, 1.0, 3, 1.0, 0.0)[0] for u in (0.99,)] == [2]           # the tie keeps the lower index
+    assert ref_row(l, 0.99, 1.0, 0, 0.5, 0.0) == (0, 0.0)
+    assert ref_row(l, 0.99, 1.0, 0, 0.51, 0.0)[0] == 1
+    assert ref_row(l, 0.99, 1.0, 0, 1.0, 0.3)[0] == 1
+    assert ref_row([1, 3, 3], 0.9, 0.0, 0, 1.0, 0.0) == (1, 0.0)
+    assert ref_row([-np.inf, np.nan], 0.5, 1.0, 0, 1.0, 0.0) == (-1, -np.inf)
+
+
+def test_refusals(built):
+    pk, abi, L = built, built.abi, built.lib()
+    assert C.sizeof(abi.pk_sample_args) == 104 and C.sizeof(abi.pk_ctc_draw) == 32
+    p = 1 << 20
+
+    def call(device=99, **kw):
+        d = dict(logits=p, logits_type=0, vocab=10, rows=3, row_stride=10, uniforms=p, tokens=p)
+        d.update(kw)
+        return L.pk_sample(device, C.byref(abi.pk_sample_args(**d)), None)
+
+    assert call() == abi.PK_ERR_NO_DEVICE and call(device=-1) == abi.PK_ERR_NO_DEVICE
+    for kw in (dict(logits_type=8), dict(vocab=0), dict(vocab=abi.PK_SAMPLE_MAX_VOCAB + 1, row_stride=1 << 20), dict(rows=-1),
+               dict(rows=1 << 31), dict(row_stride=9), dict(row_stride=1 << 40), dict(logits=None), dict(uniforms=None),
+               dict(tokens=None), dict(logits=p + 2), dict(logits_type=1, logits=p + 1), dict(tokens=p + 2), dict(uniforms=p + 1),
+               dict(logprobs=p + 2), dict(temperatures=p + 2), dict(top_ks=p + 1), dict(top_ps=p + 3), dict(min_ps=p + 2)):
+        assert call(**kw) == abi.PK_ERR_INVALID, kw
+        assert b"pk_sample" in L.pk_last_error()
+    assert L.pk_sample(0, None, None) == abi.PK_ERR_INVALID
+    assert L.pk_ctc_decode(None, None, None, 0, None, None, 0, None, None, None, 0, None, None, None) == abi.PK_ERR_INVALID
+
+
+# ---- GPU -----------------------------------------------------------------------
+
+SETS = [dict(), dict(temperature=0.7), dict(top_k=1), dict(top_k=5), dict(top_k=64, temperature=1.3), dict(top_p=0.9),
+        dict(top_p=0.3, temperature=2.0), dict(min_p=0.05), dict(top_k=50, top_p=0.95, min_p=0.02, temperature=0.8),
+        dict(temperature=0.0), dict(top_p=0.0), dict(min_p=1.0), dict(top_k=7, top_p=0.999, min_p=1e-6)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kw", SETS, ids=lambda d: "-".join(f"{k}={v}" for k, v in d.items()) or "plain")
+@pytest.mark.parametrize("v", [1, 2, 31, 33, 257, 1025, 8193])
+def test_matches_definition(built, v, kw):
+    rng = np.random.default_rng(v)
+    r = 40
+    l = rng.standard_normal((r, v)) * rng.choice([0.0, 0.5, 3.0, 12.0], (r, 1))
+    u = rng.random(r).astype(np.float32)
+    u[:3] = (0.0, 1.0 - 2.0 ** -24, 0.5)
+    seen, tok, lp = run(built, l, u, **kw)
+    check(seen, u, tok, lp, **kw)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,pad,shift", [("f32", 1, 1), ("f32", 4, 0), ("f16", 0, 0), ("f16", 3, 1), ("bf16", 0, 0), ("bf16", 7, 1), ("bf16", 8, 0)])
+@pytest.mark.parametrize("v", [5, 1024, 1030, 8193])
+def test_types_and_strides(built, v, dtype, pad, shift):
+    """Half precision makes many equal logits: ties go by index."""
+    rng = np.random.default_rng(v + pad)
+    r = 30
+    l = rng.standard_normal((r, v)) * 2
+    u = rng.random(r).astype(np.float32)
+    for kw in (dict(), dict(top_k=20), dict(top_p=0.8), dict(top_k=100, top_p=0.7, min_p=0.01, temperature=0.9)):
+        seen, tok, lp = run(built, l, u, dtype, pad, shift, **kw)
+        check(seen, u, tok, lp, **kw)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("v", [20000, 131072, 262145])
+@pytest.mark.parametrize("r", [1, 5])
+def test_large_vocabularies(built, v, r):
+    rng = np.random.default_rng(v)
+    l = rng.standard_normal((r, v)) * 2.5
+    u = rng.random(r).astype(np.float32)
+    for dtype in ("f32", "bf16"):
+        for kw in (dict(), dict(top_k=50), dict(top_p=0.95, temperature=0.8), dict(top_k=3000, top_p=0.9, min_p=0.001)):
+            seen, tok, lp = run(built, l, u, dtype, **kw)
+            check(seen, u, tok, lp, **kw)
+
+
+@pytest.mark.gpu
+def test_largest_vocabulary(built):
+    """2^19 equal logits: the fixed-point sum's largest value; the token is u's place among them."""
+    v = built.abi.PK_SAMPLE_MAX_VOCAB
+    u = np.array([0.0, 0.25, 0.75, 1 - 2.0 ** -24], np.float32)
+    _, tok, lp = run(built, np.zeros((4, v)), u)
+    assert tok.tolist() == [int(x * v) for x in u.astype(np.float64)]
+    assert np.allclose(lp, -np.log(v), rtol=2.0 ** -23)
+    _, tok, _ = run(built, np.zeros((4, v)), u, top_p=0.5)
+    assert tok.tolist() == [int(x * (v // 2)) for x in u.astype(np.float64)]
+    _, tok, _ = run(built, np.zeros((4, v)), u, top_k=1000)
+    assert tok.tolist() == [int(x * 1000) for x in u.astype(np.float64)]
+
+
+@pytest.mark.gpu
+def test_settings_of_each_row(built):
+    rng = np.random.default_rng(8)
+    r, v = 300, 2000
+    l = rng.standard_normal((r, v)) * 3
+    l[rng.random((r, v)) < 0.3] = -np.inf
+    l[17] = -np.inf
+    u = rng.random(r).astype(np.float32)
+    kw = dict(temperature=np.where(rng.random(r) < 0.2, 0.0, rng.uniform(0.2, 2, r)).astype(np.float32),
+              top_k=rng.choice([0, -3, 1, 2, 50, 1999, 2000, 5000], r).astype(np.int32),
+              top_p=rng.choice([0.1, 0.5, 0.9, 1.0, 2.0], r).astype(np.float32),
+              min_p=rng.choice([0.0, -1.0, 0.01, 0.5], r).astype(np.float32))
+    seen, tok, lp = run(built, l, u, **kw)
+    check(seen, u, tok, lp, **kw)
+    # a row by itself draws what it draws in the batch
+    for i in (0, 17, 123, 299):
+        one = {n: x[i:i + 1] for n, x in kw.items()}
+        _, t1, p1 = run(built, l[i:i + 1], u[i:i + 1], **one)
+        assert t1[0] == tok[i] and (p1[0] == lp[i])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("v", [6, 700, 9000, 40000])
+def test_masks_and_special_values(built, v):
+    low = float(np.finfo(np.float32).min)
+    rng = np.random.default_rng(v)
+    base = rng.standard_normal(v)
+    rows = []
+    rows.append(np.full(v, -np.inf))                                  # nothing left
+    rows.append(np.full(v, np.nan))
+    rows.append(np.where(np.arange(v) % 2, np.nan, -np.inf))
+    rows.append(np.full(v, low))                                      # masked by the lowest number: all equal
+    rows.append(np.where(np.arange(v) == v - 2, base, -np.inf))       # one token left
+    rows.append(np.where(np.arange(v) % 3, low, base))
+    x = base.copy(); x[0] = np.nan; x[3] = np.inf; x[5] = np.inf
+    rows.append(x)                                                    # two infinities share it all
+    x = base.copy(); x[1] = np.nan
+    rows.append(x)
+    rows.append(np.zeros(v))
+    rows.append(np.where(np.arange(v) % 2, 0.0, -0.0))                # signed zeros are equal
+    rows.append(base * 1e30)
+    x = np.full(v, low); x[2] = -low
+    rows.append(x)                                                    # a difference past f32's range
+    l = np.array(rows)
+    for u in (0.0, 0.37, 0.99999):
+        uu = np.full(len(l), u, np.float32)
+        for kw in (dict(), dict(temperature=0.0), dict(top_k=3), dict(top_p=0.6), dict(min_p=0.2), dict(top_k=2, top_p=0.99, min_p=0.1),
+                   dict(temperature=1e-30), dict(temperature=float("inf")), dict(temperature=float("nan"))):
+            seen, tok, lp = run(built, l, uu, **kw)
+            check(seen, uu, tok, lp, **kw)
+
+
+@pytest.mark.gpu
+def test_cut_inside_equal_logits(built):
+    """Ties at the border of top-k and top-p keep the lower indices, wherever they lie."""
+    rng = np.random.default_rng(4)
+    r, v = 64, 3001
+    l = rng.integers(-3, 4, (r, v)).astype(np.float64)
+    for kw in (dict(top_k=1), dict(top_k=10), dict(top_k=450), dict(top_k=1500), dict(top_p=0.25), dict(top_p=0.7),
+               dict(top_k=777, top_p=0.613, temperature=3.0)):
+        u = rng.random(r).astype(np.float32)
+        u[0], u[1] = 0.0, 1 - 2.0 ** -24
+        seen, tok, lp = run(built, l, u, **kw)
+        check(seen, u, tok, lp, **kw)
+
+
+@pytest.mark.gpu
+def test_random_numbers_out_of_range(built):
+    l = np.random.default_rng(0).standard_normal((5, 50))
+    u = np.array([-1.0, np.nan, 1.0, 7.0, np.inf], np.float32)
+    seen, tok, lp = run(built, l, u, top_k=10)
+    check(seen, u, tok, lp, top_k=10)
+
+
+@pytest.mark.gpu
+def test_drawn_frequencies(built):
+    """10^5 evenly spread random numbers: each token is drawn as often as its probability says, to one draw."""
+    n = 100_000
+    l = np.log(np.array([0.4, 0.05, 0.3, 0.2, 0.05]))
+    u = ((np.arange(n) + 0.5) / n).astype(np.float32)
+    _, tok, _ = run(built, np.tile(l, (n, 1)), u)
+    got = np.bincount(tok, minlength=5)
+    assert np.abs(got - n * np.array([0.4, 0.05, 0.3, 0.2, 0.05])).max() <= 2
+
+
+@pytest.mark.gpu
+def test_no_rows_and_other_stream(built):
+    import torch
+    pk = built
+    pk.sample(0, 0, 10, 0, 0)
+    s = torch.cuda.Stream()
+    rng = np.random.default_rng(2)
+    l, u = rng.standard_normal((20, 500)), rng.random(20).astype(np.float32)
+    torch.cuda.synchronize()
+    seen, tok, lp = run(pk, l, u, stream=s.cuda_stream, top_p=0.9)
+    check(seen, u, tok, lp, top_p=0.9)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("v", [300, 9000, 140000])
+def test_captured_and_replayed(built, v):
+    import torch
+    pk = built
+    rng = np.random.default_rng(v)
+    r = 6
+    l = torch.zeros(r, v, device="cuda")
+    u = torch.zeros(r, device="cuda")
+    tok = torch.zeros(r, dtype=torch.int32, device="cuda")
+    lp = torch.zeros(r, device="cuda")
+    g = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g):
+        pk.sample(l.data_ptr(), r, v, u.data_ptr(), tok.data_ptr(), logprobs=lp.data_ptr(), temperature=0.8, top_k=40, top_p=0.95,
+                  stream=torch.cuda.current_stream().cuda_stream)
+    for _ in range(3):
+        a, b = rng.standard_normal((r, v)).astype(np.float32), rng.random(r).astype(np.float32)
+        l.copy_(torch.from_numpy(a))
+        u.copy_(torch.from_numpy(b))
+        g.replay()
+        torch.cuda.synchronize()
+        check(a, b, tok.cpu().numpy(), lp.cpu().numpy(), temperature=0.8, top_k=40, top_p=0.95)
+
+
+def collapse(path, blank, prev):
+    toks, frs = [], []
+    for t, x in enumerate(path):
+        if x != blank and x != prev:
+            toks.append(int(x))
+            frs.append(t)
+        prev = int(x)
+    return toks, frs, prev
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("drawn", [False, True])
+@pytest.mark.parametrize("with_head", [False, True])
+@pytest.mark.parametrize("on_device", [False, True])
+def test_ctc_decode(built, with_head, drawn, on_device):
+    """Frames through the 4-bit head, the draw and the collapse in one call: the same as the
+    parts by themselves, utterance by utterance, windows carried."""
+    import torch
+    pk = built
+    rng = np.random.default_rng(11)
+    v, k, n_frames = 65, 96, np.array([40, 0, 1, 300, 77], np.int32)
+    offs = np.concatenate([[0], np.cumsum(n_frames)[:-1]]).astype(np.int64) + 2
+    total = int(n_frames.sum()) + 2
+    w = rng.standard_normal((v, k)).astype(np.float32)
+    b = rng.standard_normal(v).astype(np.float32)
+    b[v - 1] += 6
+    head = pk.Mx4Linear(w, bias=b) if with_head else None
+    x = rng.standard_normal((total, k if with_head else v)).astype(np.float32) * 0.5
+    if not with_head:
+        x[:, v - 1] += 2
+        x[50] = -np.inf                                   # a frame with nothing to draw
+    u = rng.random(total).astype(np.float32)
+    kw = dict(temperature=0.9, top_k=30, top_p=0.95, min_p=0.001)
+    # the parts
+    s = torch.cuda.current_stream().cuda_stream
+    dx, du = torch.from_numpy(x).cuda(), torch.from_numpy(u).cuda()
+    lg = dx
+    if with_head:
+        lg = torch.empty(total, v, device="cuda")
+        ws = torch.empty(head.workspace(total), dtype=torch.uint8, device="cuda")
+        head.forward(dx.data_ptr(), total, lg.data_ptr(), workspace=ws.data_ptr(), workspace_bytes=ws.numel(), stream=s)
+    if drawn:
+        tok = torch.empty(total, dtype=torch.int32, device="cuda")
+        pk.sample(lg.data_ptr(), total, v, du.data_ptr(), tok.data_ptr(), stream=s, **kw)
+        path = tok.cpu().numpy()
+        path[path < 0] = v - 1
+    else:
+        path = lg.cpu().numpy().argmax(1)
+    ctc = pk.CtcGreedy(v, v - 1)
+    prev0 = np.array([3, 5, int(path[offs[2]]), -1, 2], np.int32)
+    torch.cuda.synchronize()
+    got, frames, prev = ctc.decode_frames(dx.data_ptr() if on_device else x, offs, n_frames, head=head,
+                                          uniforms=(du.data_ptr() if on_device else u) if drawn else None,
+                                          uniforms_on_device=on_device, prev=prev0, on_device=on_device, with_frames=True,
+                                          **(kw if drawn else {}))
+    for i in range(len(n_frames)):
+        t, f, p = collapse(path[offs[i]:offs[i] + n_frames[i]], v - 1, prev0[i])
+        assert got[i].tolist() == t and frames[i].tolist() == f and prev[i] == p
+    if not with_head and not drawn:
+        again, _, _ = ctc.decode(x, offs, n_frames, prev=prev0)
+        assert all(np.array_equal(a, c) for a, c in zip(got, again))
+    ctc.close()
+
+
+@pytest.mark.gpu
+def test_ctc_decode_many_frames_and_refusals(built):
+    """More frames than one product takes; a head of another width is refused."""
+    pk = built
+    rng = np.random.default_rng(1)
+    v, k, total = 40, 64, 40_000
+    head = pk.Mx4Linear(rng.standard_normal((v, k)).astype(np.float32))
+    ctc = pk.CtcGreedy(v, 0)
+    x = rng.standard_normal((total, k)).astype(np.float32)
+    got, _, _ = ctc.decode_frames(x, [0, 15_000], [15_000, 25_000], head=head)
+    parts = [ctc.decode_frames(x[a:a + n], [0], [n], head=head)[0][0] for a, n in ((0, 15_000), (15_000, 25_000))]
+    assert all(np.array_equal(a, b) for a, b in zip(got, parts))
+    with pytest.raises(pk.PkError, match="vocab_size wide"):
+        pk.CtcGreedy(v + 1, 0).decode_frames(x, [0], [10], head=head)
+    with pytest.raises(ValueError, match="random numbers"):
+        ctc.decode_frames(x, [0], [10], head=head, uniforms=np.zeros(9, np.float32))
+    out, _, prev = ctc.decode_frames(np.zeros((0, k), np.float32), [], [], head=head)
+    assert out == [] and len(prev) == 0
