@@ -281,6 +281,8 @@ cudaError_t launch_extract_field(const int32_t * ust, int B, int field, int32_t 
 
 // pk_mx4.cu: a layer's device, outputs N and inputs K (any may be null).
 void mx4_dims(const pk_mx4 * w, int * device, int * N, int * K);
+// Whether a device-side wait of a finished call on the layer ran out (asked once).
+bool mx4_take_timeout(pk_mx4 * w);
 
 // Read-only view of a context for entry points defined outside pk_api.cu.
 struct CtxView {

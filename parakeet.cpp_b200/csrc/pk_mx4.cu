@@ -10,11 +10,18 @@
 // to the even code.
 
 #include "pk_ops.cuh"
+#include "pk_umma.cuh"
 
 #include <algorithm>
+#include <mutex>
 #include <new>
+#include <vector>
 
 namespace pk {
+
+cudaError_t encode_2d(void * map, CUtensorMapDataType type, size_t esize, const void * base, long long rows, long long cols,
+                      int box_rows, int box_cols, CUtensorMapSwizzle swz);   // pk_encproj.cu
+
 namespace {
 
 constexpr int kQThreads = 256;
@@ -171,68 +178,173 @@ __global__ void __launch_bounds__(kQThreads) mx4_repack_kernel(const unsigned ch
     }
 }
 
-// ---- product -------------------------------------------------------------------
+// ---- product on the tensor cores ------------------------------------------------
+//
+// tcgen05.mma kind::mxf4 with block scales: 64 values of K a product, accumulator in tensor memory.
+// One persistent CTA an SM walks over 128 x BN tiles of y. Warp 0 loads (codes by TMA, 256 values =
+// one 128-byte swizzled row a stage; scale atoms by bulk copies), warp 1 copies the stage's scales to
+// tensor memory and issues its four products, warps 4-7 empty the accumulator, of which there are
+// two, so that a tile's epilogue runs under the next tile's products. Each stage has tensor-memory
+// columns of its own for its scales: they are free when the stage is.
+constexpr int kTM = 128;
+constexpr int kTStages = 4;
+constexpr int kTThreads = 256;
+constexpr unsigned kScaleA = 1024, kScaleB = 2048;      // two atoms of A rows; two of each of two of B's
+constexpr unsigned kScaleCols = 24;                     // tensor-memory columns of a stage's scales: 8 + 16
+constexpr long long kWaitNs = 2000000000LL;             // bound on every device-side wait
 
-// Eight codes to eight signed bytes of twice their value (0, 1, 2, 3, 4, 6, 8, 12).
-__device__ __forceinline__ void codes_to_s8(unsigned q, unsigned & even, unsigned & odd) {
-    auto four = [](unsigned nib) {   // a code in the low half of each byte
-        const unsigned sel = nib & 0x07070707u;
-        const unsigned packed = (sel & 7u) | (sel >> 4 & 0x70u) | (sel >> 8 & 0x700u) | (sel >> 12 & 0x7000u);
-        const unsigned mag = __byte_perm(0x03020100u, 0x0C080604u, packed);
-        const unsigned neg = (nib >> 3 & 0x01010101u) * 0xFFu;
-        return __vsub4(mag ^ neg, neg);
-    };
-    even = four(q & 0x0F0F0F0Fu);
-    odd = four(q >> 4 & 0x0F0F0F0Fu);
+struct TcSmem {
+    unsigned long long full[kTStages], empty[kTStages], acc_full[2], acc_empty[2], done;
+    unsigned tmem;
+    int err;
+};
+
+template <int BN> constexpr unsigned tc_stage_bytes() { return kTM * 128u + BN * 128u + kScaleA + kScaleB; }
+constexpr unsigned kOutPitch = 33;                      // floats per staged row of the epilogue
+template <int BN> constexpr size_t tc_smem_bytes() {
+    return 1024 + (size_t) kTStages * tc_stage_bytes<BN>() + 4 * 32 * kOutPitch * 4 + sizeof(TcSmem);
 }
 
-constexpr int kSM = 32, kSN = 64;   // tile of the CUDA-core product
+// Wait with a bound and nothing else to end it: for copies in flight before an early exit.
+__device__ __forceinline__ void mbar_drain(unsigned long long * b, unsigned parity) {
+    unsigned long long t0, now;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t0));
+    now = t0;
+    while (!mbar_test(b, parity) && (long long) (now - t0) <= kWaitNs) asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
+}
 
-// A thread holds eight rows of one column; block dot products are exact integers.
-template <class T>
-__global__ void __launch_bounds__(256) mx4_simple_kernel(const unsigned char * __restrict__ xc, const unsigned char * __restrict__ xs,
-                                                         long long M, int K, const unsigned char * __restrict__ wc,
-                                                         const unsigned char * __restrict__ ws, int N,
-                                                         const float * __restrict__ bias, T * __restrict__ y, long long ldy) {
-    __shared__ unsigned sx[kSM][8], sw[kSN][9];
-    __shared__ float fx[kSM], fw[kSN];
-    const int nb = (K + 31) >> 5, chunks = scale_chunks(K);
-    const long long m0 = (long long) blockIdx.x * kSM;
-    const int n0 = blockIdx.y * kSN;
-    const int col = threadIdx.x & 63, r0 = (threadIdx.x >> 6) * 8;
-    float acc[8] = {};
-    for (int b = 0; b < nb; ++b) {
-        for (int i = threadIdx.x; i < (kSM + kSN) * 4; i += 256) {
-            const int r = i >> 2, part = i & 3;
-            const bool is_x = r < kSM;
-            const long long row = is_x ? m0 + r : n0 + (r - kSM);
-            unsigned q = 0;
-            if (row < (is_x ? M : (long long) N)) {
-                q = *reinterpret_cast<const unsigned *>((is_x ? xc : wc) + ((size_t) row * nb + b) * 16 + part * 4);
-                if (part == 0) (is_x ? fx[r] : fw[r - kSM]) = scale_val((is_x ? xs : ws)[scale_at(row, b, chunks)]);
+template <class T, int BN>
+__global__ void __launch_bounds__(kTThreads, 1)
+mx4_tc_kernel(const __grid_constant__ CUtensorMap amap, const unsigned char * __restrict__ ascale, long long M, int K,
+              const __grid_constant__ CUtensorMap wmap, const unsigned char * __restrict__ wscale, int N,
+              const float * __restrict__ bias, T * __restrict__ y, long long ldy, int * err_out) {
+    extern __shared__ __align__(1024) unsigned char raw[];
+    unsigned char * ring = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t) 1023);
+    float * out = reinterpret_cast<float *>(ring + kTStages * tc_stage_bytes<BN>());
+    TcSmem & S = *reinterpret_cast<TcSmem *>(out + 4 * 32 * kOutPitch);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int chunks = scale_chunks(K), nks = chunks / 2, atoms = (N + 127) / 128;
+    const int nt = (N + BN - 1) / BN;
+    const long long tiles = ((M + kTM - 1) / kTM) * nt;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kTStages; ++s) {
+            mbar_init(&S.full[s], 1);
+            mbar_init(&S.empty[s], 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(&S.acc_full[b], 1);
+            mbar_init(&S.acc_empty[b], 4);
+        }
+        mbar_init(&S.done, 1);
+        S.err = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 2) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+                     :: "r"(smem_u32(&S.tmem)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const unsigned tmem = S.tmem;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            unsigned it = 0;
+            bool ok = true;
+            for (long long t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+                const int m = (int) (t / nt), n0 = (int) (t % nt) * BN;
+                const int atom = n0 >> 7, have = min(((n0 & 127) + BN + 127) >> 7, atoms - atom);
+                const unsigned char * as = ascale + (size_t) m * chunks * 512;
+                const unsigned char * bs = wscale + (size_t) atom * chunks * 512;
+                for (int ks = 0; ks < nks; ++ks, ++it) {
+                    const int s = (int) (it % kTStages);
+                    if (!mbar_wait(&S.empty[s], ((it / kTStages) & 1u) ^ 1u, kWaitNs, &S.err)) { ok = false; break; }
+                    unsigned char * a = ring + s * tc_stage_bytes<BN>(), * b = a + kTM * 128, * sa = b + BN * 128;
+                    mbar_expect(&S.full[s], kTM * 128u + BN * 128u + kScaleA + 1024u * (unsigned) have);
+                    tma_load_2d(a, &amap, ks * 128, m * kTM, &S.full[s]);
+                    tma_load_2d(b, &wmap, ks * 128, n0, &S.full[s]);
+                    bulk_load(sa, as + (size_t) ks * 1024, 1024, &S.full[s]);
+                    for (int j = 0; j < have; ++j)
+                        bulk_load(sa + kScaleA + j * 1024, bs + ((size_t) j * chunks + 2 * ks) * 512, 1024, &S.full[s]);
+                }
             }
-            unsigned e, o;
-            codes_to_s8(q, e, o);
-            unsigned * d = is_x ? &sx[r][part * 2] : &sw[r - kSM][part * 2];
-            d[0] = e;
-            d[1] = o;
+            // nothing in flight when the block ends, however the others ended
+            for (unsigned j = it > kTStages ? it - kTStages : 0; j < it; ++j) mbar_drain(&S.full[j % kTStages], (j / kTStages) & 1u);
         }
-        __syncthreads();
+    } else if (warp == 1) {
+        if (lane == 0) {
+            unsigned it = 0, tile = 0;
+            bool ok = true;
+            for (long long t = blockIdx.x; t < tiles && ok; t += gridDim.x, ++tile) {
+                const int n0 = (int) (t % nt) * BN;
+                const unsigned buf = tile & 1u, d = tmem + buf * BN;
+                const unsigned shift = (unsigned) (n0 & 127) >> 5;
+                if (!mbar_wait(&S.acc_empty[buf], ((tile >> 1) & 1u) ^ 1u, kWaitNs, &S.err)) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                for (int ks = 0; ks < nks; ++ks, ++it) {
+                    const int s = (int) (it % kTStages);
+                    if (!mbar_wait(&S.full[s], (it / kTStages) & 1u, kWaitNs, &S.err)) { ok = false; break; }
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const unsigned a = smem_u32(ring + s * tc_stage_bytes<BN>()), b = a + kTM * 128u, sa = b + BN * 128u;
+                    const unsigned ca = tmem + 2 * 192 + (unsigned) s * kScaleCols, cb = ca + 8;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            int dot = 0;
+                    for (unsigned c = 0; c < 2; ++c) {
+                        umma_copy_scales(ca + c * 4, sa + c * 512);
+                        umma_copy_scales(cb + c * 8, sa + kScaleA + c * 512);
+                        if (BN > 128) umma_copy_scales(cb + c * 8 + 4, sa + kScaleA + 1024 + c * 512);
+                    }
 #pragma unroll
-            for (int i = 0; i < 8; ++i) dot = __dp4a((int) sx[r0 + j][i], (int) sw[col][i], dot);
-            acc[j] += 0.25f * (float) dot * fx[r0 + j] * fw[col];
+                    for (unsigned j = 0; j < 4; ++j)
+                        umma_mxf4(d, umma_desc_sw128(a + j * 32), umma_desc_sw128(b + j * 32), umma_idesc_mxf4(kTM, BN, 2 * (j & 1)),
+                                  ca + (j >> 1) * 4, cb + (j >> 1) * 8 + shift, (ks | (int) j) ? 1u : 0u);
+                    umma_commit(&S.empty[s]);
+                }
+                if (ok) umma_commit(&S.acc_full[buf]);
+            }
+            umma_commit(&S.done);                        // no product in flight either
+            mbar_drain(&S.done, 0u);
         }
-        __syncthreads();
-    }
-    if (n0 + col < N) {
-        const float bv = bias ? bias[n0 + col] : 0.0f;
+    } else if (warp >= 4) {
+        const int q = warp - 4;                          // this warp's tensor-memory lanes: rows 32 q ..
+        float * st = out + q * 32 * kOutPitch;
+        unsigned tile = 0;
+        for (long long t = blockIdx.x; t < tiles; t += gridDim.x, ++tile) {
+            const long long m0 = (t / nt) * kTM + q * 32;
+            const int n0 = (int) (t % nt) * BN;
+            const unsigned buf = tile & 1u;
+            if (!mbar_wait(&S.acc_full[buf], (tile >> 1) & 1u, kWaitNs, &S.err)) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const int rows = (int) min(32LL, M - m0);
+#pragma unroll 1
+            for (int c = 0; c < BN && n0 + c < N; c += 32) {
+                unsigned v[32];
+                tmem_load32(tmem + buf * BN + c + ((unsigned) (q * 32) << 16), v);
+                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-            if (m0 + r0 + j < M) y[(m0 + r0 + j) * ldy + n0 + col] = from_f32<T>(acc[j] + bv);
+                for (int i = 0; i < 32; ++i) st[lane * kOutPitch + i] = __uint_as_float(v[i]);
+                __syncwarp();
+                const int n = n0 + c + lane;
+                if (n < N) {
+                    const float bv = bias ? __ldg(bias + n) : 0.0f;
+                    T * o = y + m0 * ldy + n;
+                    for (int r = 0; r < rows; ++r, o += ldy) *o = from_f32<T>(st[r * kOutPitch + lane] + bv);
+                }
+                __syncwarp();
+            }
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            if (lane == 0) mbar_arrive(&S.acc_empty[buf]);
+        }
     }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (warp == 2) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(512u) : "memory");
+    }
+    if (threadIdx.x == 0 && S.err != 0) atomicExch_system(err_out, 1);
 }
 
 // Launch of a row kernel: one warp per 256 values, as many blocks as that takes up to a few waves.
@@ -257,17 +369,28 @@ cudaError_t launch_quantize(const void * x, int type, long long rows, int K, lon
     return cudaGetLastError();
 }
 
-cudaError_t launch_simple(const unsigned char * xc, const unsigned char * xs, long long M, int K, const unsigned char * wc,
-                          const unsigned char * ws, int N, const float * bias, void * y, int type, long long ldy,
-                          cudaStream_t s) {
-    const dim3 g((unsigned) ((M + kSM - 1) / kSM), (unsigned) ((N + kSN - 1) / kSN));
-    if (type == PK_GGML_F32)
-        mx4_simple_kernel<float><<<g, 256, 0, s>>>(xc, xs, M, K, wc, ws, N, bias, static_cast<float *>(y), ldy);
-    else if (type == PK_GGML_F16)
-        mx4_simple_kernel<__half><<<g, 256, 0, s>>>(xc, xs, M, K, wc, ws, N, bias, static_cast<__half *>(y), ldy);
-    else
-        mx4_simple_kernel<__nv_bfloat16><<<g, 256, 0, s>>>(xc, xs, M, K, wc, ws, N, bias, static_cast<__nv_bfloat16 *>(y), ldy);
-    return cudaGetLastError();
+// Host-visible error words of the layers, from pages that stay: a layer's creation pays for no
+// pinned allocation of its own.
+std::mutex error_lock;
+std::vector<int *> free_words;
+
+void give_error_word(int * w) {
+    std::lock_guard<std::mutex> g(error_lock);
+    free_words.push_back(w);
+}
+
+int * take_error_word(cudaError_t & e) {
+    std::lock_guard<std::mutex> g(error_lock);
+    if (free_words.empty()) {
+        void * page = nullptr;
+        e = cudaHostAlloc(&page, 4096, cudaHostAllocMapped | cudaHostAllocPortable);
+        if (e != cudaSuccess) return nullptr;
+        for (int i = 0; i < 1024; ++i) free_words.push_back(static_cast<int *>(page) + i);
+    }
+    int * w = free_words.back();
+    free_words.pop_back();
+    *w = 0;
+    return w;
 }
 
 constexpr int64_t kMaxDim = 1 << 20;        // K, N
@@ -282,7 +405,67 @@ struct pk_mx4 {
     unsigned char * codes = nullptr;    // [N][16 nb]
     unsigned char * scales = nullptr;   // atoms
     float * bias = nullptr;
+    int * err = nullptr;                // host memory that the device sees: a bounded wait ran out
+    int * err_dev = nullptr;
+    alignas(64) CUtensorMap map[3];     // codes in boxes of kBN[i] rows
 };
+
+namespace pk {
+namespace {
+
+constexpr int kBN[3] = {64, 128, 192};
+
+template <int BN>
+cudaError_t configure_tc() {
+    const int n = (int) tc_smem_bytes<BN>();
+    cudaError_t e = cudaFuncSetAttribute(mx4_tc_kernel<float, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, n);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(mx4_tc_kernel<__half, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, n);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(mx4_tc_kernel<__nv_bfloat16, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, n);
+    return e;
+}
+
+template <int BN>
+cudaError_t launch_tc(const pk_mx4 * w, const CUtensorMap & amap, const unsigned char * xs, long long M, void * y, int type,
+                      long long ldy, const CUtensorMap & wmap, cudaStream_t s) {
+    const long long tiles = (M + kTM - 1) / kTM * ((w->N + BN - 1) / BN);
+    const unsigned g = (unsigned) std::min<long long>(tiles, 148);
+    const size_t smem = tc_smem_bytes<BN>();
+#define PK_T(T) \
+    mx4_tc_kernel<T, BN><<<g, kTThreads, smem, s>>>(amap, xs, M, w->K, wmap, w->scales, w->N, w->bias, static_cast<T *>(y), ldy, w->err_dev)
+    if (type == PK_GGML_F32) PK_T(float);
+    else if (type == PK_GGML_F16) PK_T(__half);
+    else PK_T(__nv_bfloat16);
+#undef PK_T
+    return cudaGetLastError();
+}
+
+// Tile width: fewest rounds of tiles over the SMs, a round costed by the rows that a tile loads.
+int pick_bn(long long M, int N) {
+    int best = 0;
+    long long cost = 0;
+    for (int i = 0; i < 3; ++i) {
+        const long long tiles = (M + kTM - 1) / kTM * ((N + kBN[i] - 1) / kBN[i]);
+        const long long c = (tiles + 147) / 148 * (kTM + kBN[i]);
+        if (i == 0 || c <= cost) { best = i; cost = c; }
+    }
+    return best;
+}
+
+cudaError_t launch_product(const pk_mx4 * w, const unsigned char * xc, const unsigned char * xs, long long M, void * y, int type,
+                           long long ldy, cudaStream_t s) {
+    alignas(64) CUtensorMap amap;
+    const cudaError_t e = encode_2d(&amap, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, xc, M, (long long) w->nb * 16, kTM, 128,
+                                    CU_TENSOR_MAP_SWIZZLE_128B);
+    if (e != cudaSuccess) return e;
+    switch (pick_bn(M, w->N)) {
+        case 0: return launch_tc<64>(w, amap, xs, M, y, type, ldy, w->map[0], s);
+        case 1: return launch_tc<128>(w, amap, xs, M, y, type, ldy, w->map[1], s);
+        default: return launch_tc<192>(w, amap, xs, M, y, type, ldy, w->map[2], s);
+    }
+}
+
+}  // namespace
+}  // namespace pk
 
 namespace pk {
 
@@ -291,6 +474,8 @@ void mx4_dims(const pk_mx4 * w, int * device, int * N, int * K) {
     if (N) *N = w->N;
     if (K) *K = w->K;
 }
+
+bool mx4_take_timeout(pk_mx4 * w) { return __atomic_exchange_n(w->err, 0, __ATOMIC_ACQ_REL) != 0; }
 
 }  // namespace pk
 
@@ -352,6 +537,7 @@ extern "C" PK_API void pk_mx4_destroy(pk_mx4 * w) {
     cudaFree(w->codes);
     cudaFree(w->scales);
     cudaFree(w->bias);
+    if (w->err) give_error_word(w->err);
     delete w;
 }
 
@@ -413,6 +599,14 @@ extern "C" PK_API pk_status pk_mx4_create(int device, const pk_tensor * weight, 
         if (e == cudaSuccess)
             e = cudaMemcpyAsync(w->bias, bias, (size_t) N * 4, on_device ? cudaMemcpyDeviceToDevice : cudaMemcpyHostToDevice, s);
     }
+    if (e == cudaSuccess) w->err = take_error_word(e);
+    if (e == cudaSuccess) e = cudaHostGetDevicePointer(reinterpret_cast<void **>(&w->err_dev), w->err, 0);
+    for (int i = 0; i < 3 && e == cudaSuccess; ++i)
+        e = encode_2d(&w->map[i], CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, w->codes, N, (long long) w->nb * 16, kBN[i], 128,
+                      CU_TENSOR_MAP_SWIZZLE_128B);
+    if (e == cudaSuccess) e = configure_tc<64>();
+    if (e == cudaSuccess) e = configure_tc<128>();
+    if (e == cudaSuccess) e = configure_tc<192>();
     if (s) {
         const cudaError_t e2 = cudaStreamSynchronize(s);
         if (e == cudaSuccess) e = e2;
@@ -456,12 +650,13 @@ extern "C" PK_API pk_status pk_mx4_linear(pk_mx4 * w, const void * x, int32_t x_
     if (!aligned_to(workspace, 256)) return op_fail(PK_ERR_INVALID, fn, "workspace must be 256-byte aligned");
     if (workspace_bytes < pk_mx4_workspace(w, rows))
         return op_fail(PK_ERR_INVALID, fn, "workspace_bytes is below pk_mx4_workspace(w, rows)");
+    if (mx4_take_timeout(w)) return op_fail(PK_ERR_TIMEOUT, fn, "a device-side wait of an earlier call ran out");
     DeviceScope dev(w->device);
     if (dev.err != cudaSuccess) return op_cuda_fail(dev.err, fn);
     cudaStream_t s = (cudaStream_t) stream;
     unsigned char * xc = static_cast<unsigned char *>(workspace);
     unsigned char * xs = xc + ws_codes(w, rows);
     cudaError_t e = launch_quantize<true>(x, x_type, rows, w->K, x_stride, xc, xs, s);
-    if (e == cudaSuccess) e = launch_simple(xc, xs, rows, w->K, w->codes, w->scales, w->N, w->bias, y, y_type, y_stride, s);
+    if (e == cudaSuccess) e = launch_product(w, xc, xs, rows, y, y_type, y_stride, s);
     return e == cudaSuccess ? PK_OK : op_cuda_fail(e, fn);
 }

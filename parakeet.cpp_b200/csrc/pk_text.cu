@@ -473,6 +473,11 @@ pk_status ctc_decode(pk_ctc * c, const char * fn, pk_mx4 * head, const float * l
     TX_CK(cudaMemcpyAsync(token_offsets, c->offs.p, (size_t) (B + 1) * 8, cudaMemcpyDeviceToHost, s),
           fn);
     TX_CK(cudaStreamSynchronize(s), fn);
+    if (head && mx4_take_timeout(head)) {
+        char msg[160];
+        std::snprintf(msg, sizeof(msg), "%s: a device-side wait of the head's product ran out", fn);
+        return set_error(PK_ERR_TIMEOUT, msg);
+    }
     const int64_t total = token_offsets[B];
     if (tokens_needed) *tokens_needed = total;
     if (total > tokens_cap) {

@@ -1,6 +1,6 @@
 // pk_umma.cuh -- sm_100a building blocks shared by libparakeet_cuda's tensor-memory
 // kernels (pk_encproj.cu: the enc-proj GEMM; pk_bulk.cu: the step loop for large
-// live batches): mbarrier waits bounded in time, tcgen05.mma operand descriptors
+// live batches; pk_mx4.cu: the 4-bit product): mbarrier waits bounded in time, tcgen05.mma operand descriptors
 // for 128-byte-swizzled K-major f16 tiles, the kind::f16 instruction descriptor,
 // MMA issue / commit and 2-D TMA tile loads.
 #pragma once
@@ -88,6 +88,37 @@ __device__ __forceinline__ void umma_i8(unsigned tmem_d, unsigned long long ades
                  :: "r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
 }
 
+// kind::mxf4 instruction descriptor: f32 accumulator, e2m1 A and B, both K-major, e8m0 scales, one
+// per 32 values; `id` (0 or 2) names the first of the two scale bytes that a K = 64 product reads of
+// each row's 4-byte scale word.
+__host__ __device__ constexpr unsigned umma_idesc_mxf4(int m, int n, int id) {
+    return ((unsigned) id << 4)               // B scale id
+         | (1u << 7) | (1u << 10)             // A, B format e2m1
+         | ((unsigned) (n >> 3) << 17)        // N / 8
+         | (1u << 23)                         // e8m0 scales
+         | ((unsigned) (m >> 7) << 27)        // M / 128
+         | ((unsigned) id << 29);             // A scale id
+}
+
+// One block-scaled product of 64 values of K (32 bytes of each operand row); sfa, sfb: tensor-memory
+// addresses of the rows' scale words (row r in lane r % 32, column r / 32).
+__device__ __forceinline__ void umma_mxf4(unsigned tmem_d, unsigned long long adesc, unsigned long long bdesc, unsigned idesc,
+                                          unsigned sfa, unsigned sfb, unsigned accumulate) {
+    asm volatile("{ .reg .pred p; setp.ne.b32 p, %6, 0;\n"
+                 "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p; }"
+                 :: "r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate) : "memory");
+}
+
+// 512 bytes of scale words (32 rows of 16 bytes) from shared memory to four tensor-memory columns,
+// the same for each of the four lane quarters. Ordered before products that the same thread issues.
+__device__ __forceinline__ void umma_copy_scales(unsigned tmem, unsigned saddr) {
+    unsigned long long d = 0;
+    d |= (unsigned long long) ((saddr >> 4) & 0x3FFFu);          // start address
+    d |= (unsigned long long) (128u >> 4) << 32;                  // stride byte offset: next 8 rows of 16 bytes
+    d |= (unsigned long long) 1u << 46;                           // descriptor version (tcgen05); no swizzle
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" :: "r"(tmem), "l"(d) : "memory");
+}
+
 __device__ __forceinline__ void umma_commit(unsigned long long * b) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];"
                  :: "r"(smem_u32(b)) : "memory");
@@ -96,6 +127,27 @@ __device__ __forceinline__ void umma_commit(unsigned long long * b) {
 __device__ __forceinline__ void tma_load_2d(void * dst, const CUtensorMap * map, int x, int y, unsigned long long * bar) {
     asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
                  :: "r"(smem_u32(dst)), "l"(map), "r"(x), "r"(y), "r"(smem_u32(bar)) : "memory");
+}
+
+// Untiled copy of `bytes` (a multiple of 16, both addresses 16-byte aligned) to shared memory.
+__device__ __forceinline__ void bulk_load(void * dst, const void * src, unsigned bytes, unsigned long long * bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 :: "r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
+}
+
+__device__ __forceinline__ void mbar_expect(unsigned long long * b, unsigned bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" :: "r"(smem_u32(b)), "r"(bytes) : "memory");
+}
+
+// 32 columns of this warp's 32 tensor-memory lanes (issue only; tcgen05.wait::ld before use).
+__device__ __forceinline__ void tmem_load32(unsigned taddr, unsigned * v) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+                 "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+                   "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]),
+                   "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]),
+                   "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+                 : "r"(taddr));
 }
 
 }  // namespace
