@@ -8,16 +8,17 @@
 // Weights w = exp((l - max) / T) are held as integers, round(w * 2^43): their sums are exact
 // whatever their order, so the cut and the draw do not depend on how a row is split over threads
 // and no atomic's order shows. A token is lost only below 2^-44 of the largest weight, and 2^19
-// tokens of weight one stay below 2^63. The exponential is a polynomial in f64, off by 2^-44 at
-// most: with f32's 2^-22 the running sum would pass the random number at another token in one of
-// a few hundred rows, since a row has as many borders as tokens.
+// tokens of weight one stay below 2^63. The exponential is taken in f64, to 2^-42 of itself: with
+// f32's 2^-22 the running sum would pass the random number at another token in one of a few hundred
+// rows, since a row has as many borders as tokens.
 //
 // A team of threads (a warp, a block, or a cluster of blocks) holds one row in shared memory:
 //  1. load, largest and smallest logit;
-//  2. with top-k or top-p, the cut: a histogram over the range that can matter (31 T below the
-//     top: weights below are zero), linear in the logit, of counts or of weights; the bin in which
-//     the running sum passes what is asked; its tokens, if few, ranked against each other, else a
-//     histogram of that bin, and so on;
+//  2. with top-k or top-p, a histogram over the range that can matter, linear in the logit, of
+//     counts or of weights, and the bin in which the running sum reaches what is asked. If few
+//     tokens lie in that bin and above, they are listed, ranked against each other, cut and drawn
+//     from: done. Else the cut is found inside the bin: its tokens ranked if few, or a histogram of
+//     that bin alone, and so on;
 //  3. each thread the sum over a run of consecutive indices, a scan of those sums, and the run that
 //     the random number falls in searched by a warp.
 
@@ -34,45 +35,70 @@ namespace cg = cooperative_groups;
 using u64 = unsigned long long;
 
 constexpr double kOne = 8796093022208.0;   // 2^43
-constexpr float kMaxF = 3.402823466e+38f;
 constexpr int kList = 128;                 // tokens that are ranked against each other
 constexpr int kMaxCluster = 8;
+constexpr unsigned kFull = 0xFFFFFFFFu;
 
-// 2^x * 2^43 rounded to an integer, for -50 <= x <= 0: x = n + r with |r| <= 1/2, 2^r = 1 + r q(r),
-// q interpolating (2^r - 1) / r at the nine Chebyshev nodes of [-1/2, 1/2] (relative error of 2^r
-// below 2^-44.6; exactly 1 at r = 0). `x` comes as d * c, reduced with fused products.
-__device__ __forceinline__ u64 exp2_fixed(double d, double c) {
-    const double magic = 6755399441055744.0;            // 1.5 * 2^52: the sum's low word is round(x)
-    const double y = fma(d, c, magic);
-    const double r = fma(d, c, magic - y);
-    double q = 1.0203121045191294e-07;
-    q = fma(q, r, 1.3255224877814737e-06);
-    q = fma(q, r, 1.5252686846287112e-05);
-    q = fma(q, r, 0.00015403455852457495);
-    q = fma(q, r, 0.0013333558179043266);
-    q = fma(q, r, 0.009618129159402555);
-    q = fma(q, r, 0.055504108664760424);
-    q = fma(q, r, 0.2402265069581299);
-    q = fma(q, r, 0.6931471805599453);
-    q = fma(q, r, 1.0);
-    const double w = __hiloint2double(__double2hiint(q) + ((__double2loint(y) + 43) << 20), __double2loint(q));
-    return (u64) __double_as_longlong(w + 4503599627370496.0) & 0xFFFFFFFFFFFFFull;   // 2^52 holds the integer
-}
+// 2^(j / 32), j = 0 .. 31.
+__device__ const double kExp2[32] = {
+    0x1.0000000000000p+0, 0x1.059b0d3158574p+0, 0x1.0b5586cf9890fp+0, 0x1.11301d0125b51p+0,
+    0x1.172b83c7d517bp+0, 0x1.1d4873168b9aap+0, 0x1.2387a6e756238p+0, 0x1.29e9df51fdee1p+0,
+    0x1.306fe0a31b715p+0, 0x1.371a7373aa9cbp+0, 0x1.3dea64c123422p+0, 0x1.44e086061892dp+0,
+    0x1.4bfdad5362a27p+0, 0x1.5342b569d4f82p+0, 0x1.5ab07dd485429p+0, 0x1.6247eb03a5585p+0,
+    0x1.6a09e667f3bcdp+0, 0x1.71f75e8ec5f74p+0, 0x1.7a11473eb0187p+0, 0x1.82589994cce13p+0,
+    0x1.8ace5422aa0dbp+0, 0x1.93737b0cdc5e5p+0, 0x1.9c49182a3f090p+0, 0x1.a5503b23e255dp+0,
+    0x1.ae89f995ad3adp+0, 0x1.b7f76f2fb5e47p+0, 0x1.c199bdd85529cp+0, 0x1.cb720dcef9069p+0,
+    0x1.d5818dcfba487p+0, 0x1.dfc97337b9b5fp+0, 0x1.ea4afa2a490dap+0, 0x1.f50765b6e4540p+0};
 
 struct Row {
-    double top;       // largest logit; the largest number in a row that holds +infinity
-    double c;         // log2(e) / T
-    float base;       // logits below have weight zero
+    double top;       // largest logit
+    double c;         // 32 log2(e) / T
+    float base;       // logits below have weight zero (and lie outside the exponential's range)
 };
 
-__device__ __forceinline__ u64 weight(float v, const Row & r) {
-    return v >= r.base ? exp2_fixed((double) fminf(v, kMaxF) - r.top, r.c) : 0ull;
+// Weight of a logit v >= base. 2^x * 2^43 for x = (v - top) c / 32 >= -45: 32 x = n + t, n whole,
+// |t| <= 1/2; 2^(n / 32) from the table's entry n % 32 and n / 32 added to its exponent, 2^(t / 32)
+// = 1 + t q(t) with q cubic, interpolating at the four Chebyshev nodes of [-1/2, 1/2] (off by
+// 2^-42.5 at most; exactly 1 at t = 0). Adding 2^52 rounds the product to an integer in the low bits.
+// `entry(j)` gives 2^43 * table[j]; all callers share these operations, so a logit has one weight.
+template <class F>
+__device__ __forceinline__ u64 weight_of(float v, const Row & r, F entry) {
+    const double magic = 6755399441055744.0;            // 1.5 * 2^52: the sum's low word is the nearest integer
+    const double d = (double) v - r.top;
+    const double y = fma(d, r.c, magic);
+    const double t = fma(d, r.c, magic - y);
+    double q = 9.172598566078425e-09;
+    q = fma(q, t, 1.6938609067364243e-06);
+    q = fma(q, t, 0.00023459619820112603);
+    q = fma(q, t, 0.021660849392187844);
+    q = fma(q, t, 1.0);
+    const int n = __double2loint(y);
+    const double e = entry(n & 31);
+    const double s = __hiloint2double(__double2hiint(e) + ((n & ~31) << 15), __double2loint(e));
+    const double w = fma(q, s, 4503599627370496.0);
+    return (u64) __double_as_longlong(w) - 0x4330000000000000ull;
+}
+// The table across a warp's lanes: every lane calls, and drops what it gets for v < base.
+__device__ __forceinline__ u64 weight_warp(float v, const Row & r, double mine) {
+    return weight_of(v, r, [&](int j) { return __shfl_sync(kFull, mine, j); });
+}
+// Any thread by itself.
+__device__ __forceinline__ u64 weight_one(float v, const Row & r) {
+    return v >= r.base ? weight_of(v, r, [](int j) { return kExp2[j] * kOne; }) : 0ull;
 }
 
 template <class V> __device__ __forceinline__ V warp_sum(V v) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
     return v;
+}
+template <class V> __device__ __forceinline__ V warp_scan(V x, int lane) {   // inclusive
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const V y = __shfl_up_sync(kFull, x, o);
+        if (lane >= o) x += y;
+    }
+    return x;
 }
 
 struct Pair { float v; int i; };
@@ -80,7 +106,6 @@ struct Pair { float v; int i; };
 // What the blocks of a cluster tell each other, in each one's shared memory.
 struct Xchg {
     u64 a;
-    u64 b;
     float hi, lo;
 };
 
@@ -89,10 +114,10 @@ template <int NT> constexpr int bins_of() { return NT == 32 ? 256 : 1024; }
 template <int NT>
 struct TeamSmem {
     u64 wscan[NT / 32 + 1];
-    u64 found_before;
+    u64 found_before, found_sum;
     Xchg x[2];
     float whi[NT / 32], wlo[NT / 32];
-    int found_thread, found_ties;
+    int found, found_ties;
     int listed;                              // tokens put on the list
     float cut;
     u64 cut_ties;
@@ -101,59 +126,54 @@ template <int NT>
 struct TeamBins {
     unsigned lo[bins_of<NT>()], hi[bins_of<NT>()];     // sums of weights, or counts in lo
     Pair list[kList];
-    Pair all[kList];
+    Pair all[kList];                                   // of all blocks of a cluster
+    u64 w[kList];
 };
 
 // The threads of one row. CL: several blocks of a cluster, each with a slice of the row.
 template <int NT, bool CL>
 struct Team {
     int tid, rank, blocks;
-    unsigned phase = 0;
+    unsigned phase;
     TeamSmem<NT> * s;
+    double mine;                             // this lane's entry of the exponential's table
 
+    __device__ __forceinline__ int lane() const { return tid & 31; }
     __device__ __forceinline__ void sync() const {
         if (NT == 32) __syncwarp(); else __syncthreads();
     }
-    // Every block's slot written before it is complete; the other slot is free again after it.
-    __device__ __forceinline__ void meet() { cg::this_cluster().sync(); }
+    // Every block's slot written before it is complete, what was read before it may be overwritten.
+    __device__ __forceinline__ void meet() const { cg::this_cluster().sync(); }
 
-    __device__ u64 block_sum(u64 v) {
-        v = warp_sum(v);
-        if (NT == 32) return v;
-        sync();
-        if ((tid & 31) == 0) s->wscan[tid >> 5] = v;
-        sync();
-        u64 t = 0;
-#pragma unroll
-        for (int i = 0; i < NT / 32; ++i) t += s->wscan[i];
-        return t;
-    }
     __device__ u64 sum(u64 v) {
-        u64 t = block_sum(v);
+        v = warp_sum(v);
+        if (NT > 32) {
+            sync();
+            if (lane() == 0) s->wscan[tid >> 5] = v;
+            sync();
+            v = 0;
+#pragma unroll
+            for (int i = 0; i < NT / 32; ++i) v += s->wscan[i];
+        }
         if (CL) {
             Xchg & x = s->x[phase];
-            if (tid == 0) x.a = t;
+            if (tid == 0) x.a = v;
             meet();
-            t = 0;
-            for (int b = 0; b < blocks; ++b) t += cg::this_cluster().map_shared_rank(&x, b)->a;
+            v = 0;
+            for (int b = 0; b < blocks; ++b) v += cg::this_cluster().map_shared_rank(&x, b)->a;
             phase ^= 1;
         }
-        return t;
+        return v;
     }
     // Sum over the threads before this one (blocks before included); the sum of all in `total`.
     __device__ u64 scan(u64 v, u64 & total) {
-        u64 x = v;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const u64 y = __shfl_up_sync(0xFFFFFFFFu, x, o);
-            if ((tid & 31) >= o) x += y;
-        }
+        const u64 x = warp_scan(v, lane());
         u64 before = x - v, t;
         if (NT == 32) {
-            t = __shfl_sync(0xFFFFFFFFu, x, 31);
+            t = __shfl_sync(kFull, x, 31);
         } else {
             sync();
-            if ((tid & 31) == 31) s->wscan[tid >> 5] = x;
+            if (lane() == 31) s->wscan[tid >> 5] = x;
             sync();
             t = 0;
 #pragma unroll
@@ -163,14 +183,14 @@ struct Team {
             }
         }
         if (CL) {
-            Xchg & x2 = s->x[phase];
-            if (tid == 0) x2.a = t;
+            Xchg & o = s->x[phase];
+            if (tid == 0) o.a = t;
             meet();
             t = 0;
             for (int b = 0; b < blocks; ++b) {
-                const u64 o = cg::this_cluster().map_shared_rank(&x2, b)->a;
-                if (b < rank) before += o;
-                t += o;
+                const u64 w = cg::this_cluster().map_shared_rank(&o, b)->a;
+                if (b < rank) before += w;
+                t += w;
             }
             phase ^= 1;
         }
@@ -181,12 +201,12 @@ struct Team {
     __device__ void range(float & hi, float & lo) {
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) {
-            hi = fmaxf(hi, __shfl_xor_sync(0xFFFFFFFFu, hi, o));
-            lo = fminf(lo, __shfl_xor_sync(0xFFFFFFFFu, lo, o));
+            hi = fmaxf(hi, __shfl_xor_sync(kFull, hi, o));
+            lo = fminf(lo, __shfl_xor_sync(kFull, lo, o));
         }
         if (NT > 32) {
             sync();
-            if ((tid & 31) == 0) { s->whi[tid >> 5] = hi; s->wlo[tid >> 5] = lo; }
+            if (lane() == 0) { s->whi[tid >> 5] = hi; s->wlo[tid >> 5] = lo; }
             sync();
 #pragma unroll
             for (int i = 0; i < NT / 32; ++i) { hi = fmaxf(hi, s->whi[i]); lo = fminf(lo, s->wlo[i]); }
@@ -205,30 +225,58 @@ struct Team {
     }
 };
 
-// The slice of a row that this block holds: shared memory, or the logits themselves where a slice
-// is larger than that.
-template <class T>
+// The slice of a row that this block holds. RES: in shared memory, `skew` elements after a 16-byte
+// boundary, as in global memory, -infinity before and after it up to whole 16 bytes. Otherwise, for
+// slices larger than that, the logits are read again and again. `inf`: the row's maximum is
+// +infinity, whose logits count as 0 and all others as -infinity.
+template <class T, bool RES>
 struct Slice {
-    const float * sm;
+    float * sm;
     const T * gl;
-    int n;
-    __device__ __forceinline__ float operator()(int i) const { return sm ? sm[i] : to_f32(gl[i]); }
+    int n, skew;
+    bool inf;
+    __device__ __forceinline__ float operator()(int i) const {
+        if (RES) return sm[skew + i];
+        const float v = to_f32(gl[i]);
+        return inf ? (v == CUDART_INF_F ? 0.0f : -CUDART_INF_F) : v;
+    }
+    // f(value, index in the slice) for every element and some -infinities around them, a whole warp at a time
+    template <int NT, class F>
+    __device__ __forceinline__ void each(int tid, F f) const {
+        if constexpr (RES) {
+            const int quads = (skew + n + 3) >> 2;
+            for (int q = tid & ~31; q < quads; q += NT) {
+                const int i = q + (tid & 31);
+                const float4 v = i < quads ? reinterpret_cast<const float4 *>(sm)[i]
+                                           : make_float4(-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F);
+                const int e = 4 * i - skew;
+                f(v.x, e);
+                f(v.y, e + 1);
+                f(v.z, e + 2);
+                f(v.w, e + 3);
+            }
+        } else {
+            for (int q = tid & ~31; q < n; q += NT) {
+                const int i = q + (tid & 31);
+                f(i < n ? (*this)(i) : -CUDART_INF_F, i);
+            }
+        }
+    }
 };
 
 template <class T, int NT>
-__device__ __forceinline__ void load_slice(const T * __restrict__ g, int n, float * sm, int tid) {
+__device__ __forceinline__ void load_slice(const Slice<T, true> & l, int tid) {
     constexpr int W = 16 / (int) sizeof(T);
+    const T * g = l.gl;
+    const int n = l.n;
     const int head = min(n, (int) ((16 - (reinterpret_cast<uintptr_t>(g) & 15)) & 15) / (int) sizeof(T));
     const int vecs = (n - head) / W;
-    // sm is placed so that its element `head` is 16-byte aligned
+    float * sm = l.sm + l.skew;                          // its element `head` is 16-byte aligned
     if constexpr (sizeof(T) == 4) {
         for (int i = tid; i < vecs; i += NT) {
             const unsigned d = (unsigned) __cvta_generic_to_shared(sm + head + i * 4);
             asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" :: "r"(d), "l"(g + head + i * 4) : "memory");
         }
-        for (int i = tid; i < head; i += NT) sm[i] = to_f32(g[i]);
-        for (int i = head + vecs * W + tid; i < n; i += NT) sm[i] = to_f32(g[i]);
-        asm volatile("cp.async.wait_all;" ::: "memory");
     } else {
 #pragma unroll 4
         for (int i = tid; i < vecs; i += NT) {
@@ -246,138 +294,185 @@ __device__ __forceinline__ void load_slice(const T * __restrict__ g, int n, floa
             d[0] = make_float4(f[0], f[1], f[2], f[3]);
             d[1] = make_float4(f[4], f[5], f[6], f[7]);
         }
-        for (int i = tid; i < head; i += NT) sm[i] = to_f32(g[i]);
-        for (int i = head + vecs * W + tid; i < n; i += NT) sm[i] = to_f32(g[i]);
     }
+    for (int i = tid; i < head; i += NT) sm[i] = to_f32(g[i]);
+    for (int i = head + vecs * W + tid; i < n; i += NT) sm[i] = to_f32(g[i]);
+    if (tid < l.skew) l.sm[tid] = -CUDART_INF_F;
+    if (tid < ((l.skew + n + 3) & ~3) - (l.skew + n)) sm[n + tid] = -CUDART_INF_F;
+    if constexpr (sizeof(T) == 4) asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
-// The cut at which the running sum over falling logits reaches `need` >= 1, among logits of
-// [lo, hi], which hold that much: counts of tokens, or (WEIGHTS) their weights. Everything above the
-// returned logit is kept, and `ties` of those equal to it.
-template <bool WEIGHTS, class T, int NT, bool CL>
-__device__ float find_cut(Team<NT, CL> & team, TeamBins<NT> * B, const Slice<T> & l, const Row & row, float hi, float lo, u64 need,
-                          u64 & ties) {
+// A range of logits parted evenly into bins. Bins rise as the logit falls: each operation of bin_of is
+// monotone, `hi` lies in bin 0 and `lo` in the last (0 * inf, a NaN, is 0 as an integer), so a level
+// parts the two and leaves a range 1 / NB as wide: 28 levels for NB = 1024 at the very most.
+struct Level {
+    float hi, lo, top, inv, half;
+    int bin;
+    u64 above, with;      // sums over what lies above the bin, and over that and the bin
+    __device__ __forceinline__ void range(float h, float l, int nb) {
+        hi = h;
+        lo = l;
+        // halves where the difference could overflow; not otherwise, since half of the smallest number is zero
+        half = fmaxf(fabsf(h), fabsf(l)) > 1e37f ? 0.5f : 1.0f;
+        top = half * h;
+        inv = (float) nb / (top - half * l);
+    }
+    template <int NB> __device__ __forceinline__ int bin_of(float v) const { return min(NB - 1, (int) ((top - half * v) * inv)); }
+    __device__ __forceinline__ bool holds(float v) const { return v <= hi && v >= lo; }
+};
+
+// What top-p asks for: a share of the weights of [from, hi] (those below the level's range are summed
+// without a bin) and of `lump`.
+struct Share {
+    double p;
+    float from;
+    u64 lump;
+};
+
+// Bins the level's range and finds the bin in which the running sum over falling logits (from L.above
+// on) reaches `need` >= 1: of counts, or (WEIGHTS) of weights. With `share`, need is worked out from
+// it first. False: the range does not hold that much; L.with is then what it and its tail hold.
+template <bool WEIGHTS, class T, int NT, bool CL, bool RES>
+__device__ bool find_bin(Team<NT, CL> & team, TeamBins<NT> * B, const Slice<T, RES> & l, const Row & row, Level & L, u64 & need,
+                         const Share * share) {
     constexpr int NB = bins_of<NT>(), PER = NB / NT;
     TeamSmem<NT> * s = team.s;
-    u64 above = 0;
-    for (;;) {
-        if (!(hi > lo)) {                       // one value left
-            const u64 each = WEIGHTS ? weight(hi, row) : 1ull;
-            ties = (need - above + each - 1) / max(each, 1ull);
-            return hi;
-        }
-        for (int b = team.tid; b < NB; b += NT) { B->lo[b] = 0; if (WEIGHTS) B->hi[b] = 0; }
-        if (team.tid == 0) { s->listed = 0; }
-        team.sync();
-        // Falling logits in rising bins: each operation is monotone, `hi` falls in bin 0 and `lo` in the
-        // last (0 * inf, a NaN, is 0 as an integer), so every level parts the two and takes a range
-        // 1 / NB as wide: 28 levels for NB = 1024 at the very most. Halves where the difference could
-        // overflow; not otherwise, since half of the smallest number is zero.
-        const float half = fmaxf(fabsf(hi), fabsf(lo)) > 1e37f ? 0.5f : 1.0f;
-        const float top = half * hi, inv = (float) NB / (top - half * lo);
-        auto bin_of = [&](float v) { return min(NB - 1, (int) ((top - half * v) * inv)); };
-        for (int i = team.tid; i < l.n; i += NT) {
-            const float v = l(i);
-            if (v <= hi && v >= lo) {
-                const int b = bin_of(v);
-                if (WEIGHTS) {
-                    const u64 w = weight(v, row);
+    for (int b = team.tid; b < NB; b += NT) { B->lo[b] = 0; if (WEIGHTS) B->hi[b] = 0; }
+    if (team.tid == 0) { s->found = -1; s->listed = 0; }
+    team.sync();
+    u64 rest = 0;
+    const float from = share ? share->from : L.lo;
+    l.template each<NT>(team.tid, [&](float v, int) {
+        if (WEIGHTS) {
+            const bool any = v <= L.hi && v >= from;
+            if (!__any_sync(kFull, any)) return;
+            const u64 w = weight_warp(v, row, team.mine);
+            if (any) {
+                if (v >= L.lo) {
+                    const int b = L.bin_of<NB>(v);
                     const unsigned wl = (unsigned) w, old = atomicAdd(&B->lo[b], wl);
                     const unsigned up = (unsigned) (w >> 32) + (old + wl < old ? 1u : 0u);
                     if (up) atomicAdd(&B->hi[b], up);
                 } else {
-                    atomicAdd(&B->lo[b], 1u);
+                    rest += w;
                 }
             }
+        } else if (L.holds(v)) {
+            atomicAdd(&B->lo[L.bin_of<NB>(v)], 1u);
         }
-        if (CL) team.meet();
-        team.sync();
-        // each thread PER consecutive bins
-        u64 mine[PER], sum = 0;
+    });
+    if (WEIGHTS && share) rest = team.sum(rest);                 // in a cluster, all bins are complete after it
+    else if (CL) team.meet();
+    team.sync();
+    u64 mine[PER], sum = 0;                                      // PER consecutive bins a thread
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        const int b = team.tid * PER + j;
+        u64 w = 0;
+        if (CL) {
+            for (int q = 0; q < team.blocks; ++q) {
+                const TeamBins<NT> * o = cg::this_cluster().map_shared_rank(B, q);
+                w += (WEIGHTS ? (u64) o->hi[b] << 32 : 0ull) + o->lo[b];
+            }
+        } else {
+            w = (WEIGHTS ? (u64) B->hi[b] << 32 : 0ull) + B->lo[b];
+        }
+        mine[j] = w;
+        sum += w;
+    }
+    u64 total;
+    Team<NT, false> block{team.tid, 0, 1, 0, s, 0.0};            // the bins are the cluster's already
+    u64 before = L.above + block.scan(sum, total);
+    total += L.above + rest;
+    if (WEIGHTS && share) need = max((u64) ceil(share->p * (double) (total + share->lump)), 1ull);
+    if (before < need && need <= before + sum) {
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
-            const int b = team.tid * PER + j;
-            u64 w = 0;
-            if (CL) {
-                for (int q = 0; q < team.blocks; ++q) {
-                    const TeamBins<NT> * o = cg::this_cluster().map_shared_rank(B, q);
-                    w += (WEIGHTS ? (u64) o->hi[b] << 32 : 0ull) + o->lo[b];
-                }
-            } else {
-                w = (WEIGHTS ? (u64) B->hi[b] << 32 : 0ull) + B->lo[b];
+            if (before < need && need <= before + mine[j]) {
+                s->found = team.tid * PER + j;
+                s->found_before = before;
+                s->found_sum = before + mine[j];
             }
-            mine[j] = w;
-            sum += w;
+            before += mine[j];
         }
-        // the scan over this block's threads alone: the bins are the cluster's already
-        u64 total;
-        Team<NT, false> block{team.tid, 0, 1, 0, s};
-        u64 before = above + block.scan(sum, total);
-        if (before < need && need <= before + sum) {
-#pragma unroll
-            for (int j = 0; j < PER; ++j) {
-                if (before < need && need <= before + mine[j]) {
-                    s->found_thread = team.tid * PER + j;
-                    s->found_before = before;
-                }
-                before += mine[j];
-            }
-        }
-        team.sync();
-        const int bin = s->found_thread;
-        above = s->found_before;
-        // the tokens of that bin: listed if they fit, and their range
-        float bhi = -CUDART_INF_F, blo = CUDART_INF_F;
-        for (int i = team.tid; i < l.n; i += NT) {
-            const float v = l(i);
-            if (v <= hi && v >= lo && bin_of(v) == bin) {
-                bhi = fmaxf(bhi, v);
-                blo = fminf(blo, v);
-                const int at = atomicAdd(&s->listed, 1);
-                if (at < kList) B->list[at] = Pair{v, i};
-            }
-        }
-        team.range(bhi, blo);
-        team.sync();
-        hi = bhi;
-        lo = blo;
-        int n = s->listed;
-        const Pair * list = B->list;
-        team.sync();                            // read by all before it is set back
-        if (CL) {
-            Xchg & x = s->x[team.phase];
-            if (team.tid == 0) x.a = (u64) n;
-            team.meet();
-            int base = 0;
-            n = 0;
-            for (int q = 0; q < team.blocks; ++q) n += (int) cg::this_cluster().map_shared_rank(&x, q)->a;
-            if (n <= kList) {
-                for (int q = 0; q < team.blocks; ++q) {
-                    const int c = (int) cg::this_cluster().map_shared_rank(&x, q)->a;
-                    const TeamBins<NT> * o = cg::this_cluster().map_shared_rank(B, q);
-                    for (int i = team.tid; i < c; i += NT) B->all[base + i] = o->list[i];
-                    base += c;
-                }
-                list = B->all;
-            }
-            team.phase ^= 1;
-            team.meet();                        // nobody lists anew while another still reads
-            team.sync();
-        }
+    }
+    if (CL) team.meet(); else team.sync();                       // and nobody clears bins that another reads
+    L.bin = s->found;
+    if (L.bin < 0) {
+        L.with = total;
+        return false;
+    }
+    L.above = s->found_before;
+    L.with = s->found_sum;
+    return true;
+}
+
+// Puts the slice's elements that `want` names on the list, and joins the lists of a cluster's blocks.
+// The number of them; past kList the list is not complete and not to be used.
+template <class T, int NT, bool CL, bool RES, class F>
+__device__ int gather(Team<NT, CL> & team, TeamBins<NT> * B, const Slice<T, RES> & l, int s0, const Pair *& list, F want) {
+    TeamSmem<NT> * s = team.s;
+    l.template each<NT>(team.tid, [&](float v, int i) {
+        const bool w = want(v);
+        const unsigned who = __ballot_sync(kFull, w);
+        if (who == 0) return;
+        int at = 0;
+        if (team.lane() == 0) at = atomicAdd(&s->listed, __popc(who));
+        at = __shfl_sync(kFull, at, 0) + __popc(who & ((1u << team.lane()) - 1u));
+        if (w && at < kList) B->list[at] = Pair{v, s0 + i};
+    });
+    team.sync();
+    int n = s->listed;
+    list = B->list;
+    if (CL) {
+        Xchg & x = s->x[team.phase];
+        if (team.tid == 0) x.a = (u64) n;
+        team.meet();
+        n = 0;
+        for (int q = 0; q < team.blocks; ++q) n += (int) cg::this_cluster().map_shared_rank(&x, q)->a;
         if (n <= kList) {
+            int base = 0;
+            for (int q = 0; q < team.blocks; ++q) {
+                const int c = (int) cg::this_cluster().map_shared_rank(&x, q)->a;
+                const TeamBins<NT> * o = cg::this_cluster().map_shared_rank(B, q);
+                for (int i = team.tid; i < c; i += NT) B->all[base + i] = o->list[i];
+                base += c;
+            }
+            list = B->all;
+        }
+        team.phase ^= 1;
+        team.meet();                            // nobody lists anew while another still reads
+    }
+    team.sync();
+    if (team.tid == 0) s->listed = 0;           // read by all: the next list starts empty
+    team.sync();
+    return n;
+}
+
+// The cut inside the bin that find_bin found: everything above the returned logit is kept, and
+// `ties` of those equal to it.
+template <bool WEIGHTS, class T, int NT, bool CL, bool RES>
+__device__ float find_cut(Team<NT, CL> & team, TeamBins<NT> * B, const Slice<T, RES> & l, const Row & row, Level L, u64 need,
+                          u64 & ties) {
+    constexpr int NB = bins_of<NT>();
+    TeamSmem<NT> * s = team.s;
+    for (;;) {
+        const Pair * list;
+        const int n = gather<T, NT, CL, RES>(team, B, l, 0, list, [&](float v) { return L.holds(v) && L.bin_of<NB>(v) == L.bin; });
+        if (n <= kList) {
+            for (int j = team.tid; j < n; j += NT) B->w[j] = WEIGHTS ? weight_one(list[j].v, row) : 1ull;
+            team.sync();
             for (int j = team.tid; j < n; j += NT) {
                 const float v = list[j].v;
-                u64 over = above, same = 0;
+                u64 over = L.above, same = 0;
                 for (int i = 0; i < n; ++i) {
                     const float o = list[i].v;
-                    const u64 w = WEIGHTS ? (o >= v ? weight(o, row) : 0ull) : 1ull;
-                    if (o > v) over += w;
-                    else if (o == v) same += w;
+                    if (o > v) over += B->w[i];
+                    else if (o == v) same += B->w[i];
                 }
-                if (over < need && need <= over + same) {
-                    const u64 each = WEIGHTS ? weight(v, row) : 1ull;
+                if (over < need && need <= over + same) {        // threads with equal logits write the same
                     s->cut = v;
-                    s->cut_ties = (need - over + each - 1) / each;
+                    s->cut_ties = (need - over + B->w[j] - 1) / B->w[j];
                 }
             }
             team.sync();
@@ -386,10 +481,94 @@ __device__ float find_cut(Team<NT, CL> & team, TeamBins<NT> * B, const Slice<T> 
             team.sync();
             return v;
         }
+        float hi = -CUDART_INF_F, lo = CUDART_INF_F;
+        l.template each<NT>(team.tid, [&](float v, int) {
+            if (L.holds(v) && L.bin_of<NB>(v) == L.bin) {
+                hi = fmaxf(hi, v);
+                lo = fminf(lo, v);
+            }
+        });
+        team.range(hi, lo);
+        if (!(hi > lo)) {                       // one value
+            const u64 each = WEIGHTS ? weight_one(hi, row) : 1ull;
+            ties = (need - L.above + each - 1) / max(each, 1ull);
+            return hi;
+        }
+        L.range(hi, lo, NB);
+        find_bin<WEIGHTS, T, NT, CL, RES>(team, B, l, row, L, need, nullptr);
     }
 }
 
-template <class T, int NT, bool FILTERS, bool CL>
+__device__ __forceinline__ void write_token(const pk_sample_args & a, long long row, int token, float v, float hi, double temp, u64 total) {
+    a.tokens[row] = token;
+    if (a.logprobs) a.logprobs[row] = (float) ((v == hi ? 0.0 : ((double) v - (double) hi) / temp) - log((double) total / kOne));
+}
+
+__device__ __forceinline__ u64 place_of(float u, u64 total) {
+    u = u > 0.0f ? fminf(u, 0x1.fffffep-1f) : 0.0f;
+    return min((u64) ((double) u * (double) total), total - 1);
+}
+
+// All tokens that may be kept are on the list: of the first k of them those before which less than
+// `need` lies (0: the share p of the k tokens' weight), of these those that reach `least`; the draw.
+template <int NT, bool CL>
+__device__ void draw_listed(Team<NT, CL> & team, TeamBins<NT> * B, const Pair * list, int n, const pk_sample_args & a, long long row,
+                            const Row & r, float hi, double temp, int k, float p, u64 need, float least) {
+    for (int j = team.tid; j < n; j += NT) B->w[j] = weight_one(list[j].v, r);
+    team.sync();
+    constexpr int PER = (kList + NT - 1) / NT;                   // tokens of a thread
+    u64 over[PER], sum = 0;                                      // weight before each in the order
+    int place[PER];
+#pragma unroll
+    for (int q = 0; q < PER; ++q) {
+        const int j = team.tid + q * NT;
+        over[q] = 0;
+        place[q] = kList;
+        if (j < n) {
+            const Pair me = list[j];
+            int c = 0;
+            u64 w = 0;
+            for (int i = 0; i < n; ++i) {
+                const Pair o = list[i];
+                if (o.v > me.v || (o.v == me.v && o.i < me.i)) { w += B->w[i]; ++c; }
+            }
+            over[q] = w;
+            place[q] = c;
+            if (c < k) sum += B->w[j];
+        }
+    }
+    Team<NT, false> block{team.tid, 0, 1, 0, team.s, 0.0};
+    if (need == 0) {
+        sum = block.sum(sum);
+        need = p >= 1.0f ? ~0ull : max((u64) ceil(p > 0.0f ? (double) p * (double) sum : 0.0), 1ull);
+    }
+    team.sync();
+    u64 kept = 0;
+#pragma unroll
+    for (int q = 0; q < PER; ++q) {
+        const int j = team.tid + q * NT;
+        if (j < n) {
+            const bool keep = place[q] < k && over[q] < need && list[j].v >= least;
+            if (!keep) B->w[j] = 0;
+            else kept += B->w[j];
+        }
+    }
+    const u64 total = block.sum(kept);
+    team.sync();
+    const u64 t = place_of(a.uniforms[row], total);
+#pragma unroll
+    for (int q = 0; q < PER; ++q) {
+        const int j = team.tid + q * NT;
+        if (j < n && B->w[j] > 0) {
+            u64 before = 0;
+            for (int i = 0; i < n; ++i)
+                if (list[i].i < list[j].i) before += B->w[i];
+            if (before <= t && t < before + B->w[j] && team.rank == 0) write_token(a, row, list[j].i, list[j].v, hi, temp, total);
+        }
+    }
+}
+
+template <class T, int NT, bool FILTERS, bool CL, bool RES>
 __global__ void __launch_bounds__(NT == 32 ? 256 : NT)
 sample_kernel(pk_sample_args a, int slice, int teams, int row_floats) {
     extern __shared__ __align__(16) unsigned char raw[];
@@ -398,46 +577,44 @@ sample_kernel(pk_sample_args a, int slice, int teams, int row_floats) {
     team.tid = NT == 32 ? (int) threadIdx.x & 31 : (int) threadIdx.x;
     team.blocks = CL ? (int) cg::this_cluster().num_blocks() : 1;
     team.rank = CL ? (int) cg::this_cluster().block_rank() : 0;
-    team.s = reinterpret_cast<TeamSmem<NT> *>(raw) + t_in;
-    TeamBins<NT> * bins = reinterpret_cast<TeamBins<NT> *>(reinterpret_cast<TeamSmem<NT> *>(raw) + teams) + t_in;
-    float * rows_at = FILTERS ? reinterpret_cast<float *>(reinterpret_cast<TeamBins<NT> *>(reinterpret_cast<TeamSmem<NT> *>(raw) + teams) + teams)
-                              : reinterpret_cast<float *>(reinterpret_cast<TeamSmem<NT> *>(raw) + teams);
-    rows_at = reinterpret_cast<float *>((reinterpret_cast<uintptr_t>(rows_at) + 15) & ~(uintptr_t) 15) + (size_t) t_in * row_floats;
+    team.phase = 0;
     const long long row = CL ? (long long) (blockIdx.x / team.blocks) : (long long) blockIdx.x * teams + t_in;
     if (NT == 32 && row >= a.rows) return;                       // warps by themselves: nothing to meet
+    float * rows_at = reinterpret_cast<float *>(raw);
+    TeamSmem<NT> * state = reinterpret_cast<TeamSmem<NT> *>(rows_at + (size_t) teams * row_floats);
+    team.s = state + t_in;
+    TeamBins<NT> * bins = reinterpret_cast<TeamBins<NT> *>(state + teams) + t_in;
+    team.mine = kExp2[team.lane()] * kOne;
     const int s0 = min(team.rank * slice, a.vocab);
-    Slice<T> l;
+    Slice<T, RES> l;
     l.n = min(slice, a.vocab - s0);
     l.gl = static_cast<const T *>(a.logits) + row * a.row_stride + s0;
-    l.sm = nullptr;
-    if (row_floats > 0) {
-        // element i in the slice at the same place of its 16 bytes (in f32) as the logits have
-        const int skew = (int) ((reinterpret_cast<uintptr_t>(l.gl) & 15) / sizeof(T)) & 3;
-        float * sm = rows_at + skew;
-        load_slice<T, NT>(l.gl, l.n, sm, team.tid);
+    l.sm = rows_at + (size_t) t_in * row_floats;
+    l.skew = RES ? (int) ((reinterpret_cast<uintptr_t>(l.gl) & 15) / sizeof(T)) & 3 : 0;
+    l.inf = false;
+    if constexpr (RES) {
+        load_slice<T, NT>(l, team.tid);
         team.sync();
-        l.sm = sm;
     }
+    const float temp_f = a.temperatures ? a.temperatures[row] : a.temperature;
+    const double temp = (double) temp_f;
     float hi = -CUDART_INF_F, lo = CUDART_INF_F;                 // fmaxf and fminf pass over NaN
-    for (int i = team.tid; i < l.n; i += NT) {
-        const float v = l(i);
+    l.template each<NT>(team.tid, [&](float v, int) {
         hi = fmaxf(hi, v);
-        if (v > -CUDART_INF_F) lo = fminf(lo, v);
-    }
+        if (FILTERS && v > -CUDART_INF_F) lo = fminf(lo, v);
+    });
     team.range(hi, lo);
-    const bool writer = team.tid == 0 && team.rank == 0;
-    const float temp = a.temperatures ? a.temperatures[row] : a.temperature;
-    if (hi == -CUDART_INF_F || !(temp > 0.0f)) {
+    if (hi == -CUDART_INF_F || !(temp_f > 0.0f)) {
         // nothing to draw, or the first index of the largest
         u64 first = ~0ull;
         if (hi > -CUDART_INF_F)
             for (int i = team.tid; i < l.n && first == ~0ull; i += NT)
                 if (l(i) == hi) first = (u64) (s0 + i);
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) first = min(first, __shfl_xor_sync(0xFFFFFFFFu, first, o));
+        for (int o = 16; o > 0; o >>= 1) first = min(first, __shfl_xor_sync(kFull, first, o));
         if (NT > 32) {
             team.sync();
-            if ((team.tid & 31) == 0) team.s->wscan[team.tid >> 5] = first;
+            if (team.lane() == 0) team.s->wscan[team.tid >> 5] = first;
             team.sync();
 #pragma unroll
             for (int i = 0; i < NT / 32; ++i) first = min(first, team.s->wscan[i]);
@@ -449,55 +626,98 @@ sample_kernel(pk_sample_args a, int slice, int teams, int row_floats) {
             for (int b = 0; b < team.blocks; ++b) first = min(first, cg::this_cluster().map_shared_rank(&x, b)->a);
             team.meet();
         }
-        if (writer) {
+        if (team.tid == 0 && team.rank == 0) {
             a.tokens[row] = hi == -CUDART_INF_F ? -1 : (int) first;
             if (a.logprobs) a.logprobs[row] = hi == -CUDART_INF_F ? -CUDART_INF_F : 0.0f;
         }
         return;
     }
+    if (hi == CUDART_INF_F) {                                    // zeros where it is +infinity, nothing elsewhere
+        if constexpr (RES) {
+            team.sync();
+            for (int i = team.tid; i < l.n; i += NT) l.sm[l.skew + i] = l.sm[l.skew + i] == CUDART_INF_F ? 0.0f : -CUDART_INF_F;
+            team.sync();
+        }
+        l.inf = true;
+        hi = lo = 0.0f;
+    }
     Row r;
-    const bool inf = hi == CUDART_INF_F;
-    r.top = (double) fminf(hi, kMaxF);
-    r.c = 1.4426950408889634074 / (double) temp;                 // 0 for an infinite T
+    r.top = (double) hi;
+    r.c = 46.166241308446828384 / temp;                          // 32 log2(e) / T; 0 for an infinite T
     // below 2^-44 of the largest: 31 T is more than 44 ln 2 = 30.5 T; rounded up, so that what is
     // not below lies within the exponential's range
-    r.base = inf ? hi : fmaxf(__double2float_ru(r.top - 31.0 * (double) temp), -kMaxF);
+    r.base = fmaxf(__double2float_ru(r.top - 31.0 * temp), -3.402823466e+38f);
     float least = r.base;                                        // kept: >= least, and what the cut says
     float cut = -CUDART_INF_F;
     u64 ties = ~0ull;
-    if (FILTERS) {
+    if constexpr (FILTERS) {
+        constexpr int NB = bins_of<NT>();
         const float m = a.min_ps ? a.min_ps[row] : a.min_p;
         const float p = a.top_ps ? a.top_ps[row] : a.top_p;
         const int k = a.top_ks ? a.top_ks[row] : a.top_k;
         if (m >= 1.0f) least = hi;
-        else if (m > 0.0f && !inf) least = fmaxf(least, __double2float_ru(r.top + (double) temp * log((double) m)));
+        else if (m > 0.0f) least = fmaxf(least, __double2float_ru(r.top + temp * log((double) m)));
         const float low = fmaxf(r.base, lo);                     // the range that can have weight
+        Level L;
+        u64 need = 0;
         if (k > 0 && k < a.vocab) {
-            u64 n = 0;
-            for (int i = team.tid; i < l.n; i += NT) n += l(i) >= low ? 1u : 0u;
-            if (team.sum(n) > (u64) k) cut = find_cut<false>(team, bins, l, r, hi, low, (u64) k, ties);
+            // with p off, what min-p drops need not be counted
+            L.range(hi, p >= 1.0f ? fmaxf(low, least) : low, NB);
+            L.above = 0;
+            need = (u64) k;
+            if (find_bin<false, T, NT, CL, RES>(team, bins, l, r, L, need, nullptr)) {
+                if (L.with <= (u64) kList) {
+                    const Pair * list;
+                    const int n = gather<T, NT, CL, RES>(team, bins, l, s0, list,
+                                                         [&](float v) { return L.holds(v) && L.bin_of<NB>(v) <= L.bin; });
+                    draw_listed<NT, CL>(team, bins, list, n, a, row, r, hi, temp, k, p, 0, least);
+                    return;
+                }
+                cut = find_cut<false, T, NT, CL, RES>(team, bins, l, r, L, need, ties);
+            }
         }
         if (!(p >= 1.0f)) {
-            u64 w = 0;
-            for (int i = team.tid; i < l.n; i += NT) {
-                const float v = l(i);
-                if (v > cut) w += weight(v, r);
+            Share share;
+            share.p = p > 0.0f ? (double) p : 0.0;
+            share.from = low;
+            share.lump = 0;
+            u64 each = 0;
+            if (cut > -CUDART_INF_F) {
+                // above the cut of k, from the next number on; equal logits there count as many as are kept
+                const float up = cut == 0.0f ? 1.401298464e-45f : __int_as_float(__float_as_int(cut) + (cut > 0.0f ? 1 : -1));
+                share.from = fmaxf(low, up);
+                each = weight_one(cut, r);
+                share.lump = each * ties;
             }
-            w = team.sum(w);
-            const u64 at_cut = cut > -CUDART_INF_F ? weight(cut, r) * ties : 0ull;
-            const u64 need = max((u64) ceil(p > 0.0f ? (double) p * (double) (w + at_cut) : 0.0), 1ull);
-            if (need > w) {
-                // the cut stays, with fewer ties
-                if (cut > -CUDART_INF_F) ties = min(ties, (need - w + weight(cut, r) - 1) / max(weight(cut, r), 1ull));
+            // Tokens of less than (1 - p) / V of the largest weight cannot be at the cut of p, all of them
+            // together being less than the share 1 - p: no bins for them (half of that, against rounding).
+            const double tail = 0.5 * (1.0 - share.p) / (double) a.vocab;
+            float from = share.from;
+            if (tail > 0x1p-40) from = fmaxf(from, __double2float_rd(r.top + temp * log(tail)));
+            L.with = 0;
+            bool found = false;
+            if (share.from <= hi) {
+                L.range(hi, from, NB);
+                L.above = 0;
+                found = find_bin<true, T, NT, CL, RES>(team, bins, l, r, L, need, &share);
             } else {
-                // above the cut of k: from the next number on
-                float from = low;
-                if (cut > -CUDART_INF_F) {
-                    const float up = cut == 0.0f ? 1.401298464e-45f
-                                                 : __int_as_float(__float_as_int(cut) + (cut > 0.0f ? 1 : -1));
-                    from = fmaxf(low, up);
+                need = max((u64) ceil(share.p * (double) share.lump), 1ull);
+            }
+            if (found) {
+                // few enough for the list, as far as their weight tells: none is lighter than the bin's lower edge
+                const float edge = fmaxf(from, hi - (hi - from) * ((float) (L.bin + 1) / (float) NB));
+                if ((double) L.with <= 4.0 * kList * (double) max(weight_one(edge, r), 1ull)) {
+                    const Pair * list;
+                    const int n = gather<T, NT, CL, RES>(team, bins, l, s0, list,
+                                                         [&](float v) { return L.holds(v) && L.bin_of<NB>(v) <= L.bin; });
+                    if (n <= kList) {
+                        draw_listed<NT, CL>(team, bins, list, n, a, row, r, hi, temp, kList, p, need, least);
+                        return;
+                    }
                 }
-                cut = find_cut<true>(team, bins, l, r, hi, from, need, ties);
+                cut = find_cut<true, T, NT, CL, RES>(team, bins, l, r, L, need, ties);
+            } else if (each > 0) {
+                ties = min(ties, (need - L.with + each - 1) / each);   // the cut of k, with fewer ties
             }
         }
     }
@@ -514,61 +734,58 @@ sample_kernel(pk_sample_args a, int slice, int teams, int row_floats) {
         partial = ties < all;
     }
     u64 sum = 0, seen = tie0;
+    const float from = fmaxf(least, cut);
 #pragma unroll 4
-    for (int i = i0; i < i1; ++i) {
-        const float v = l(i);
-        if (v >= least) {
-            if (FILTERS) {
-                bool keep = v >= cut;
-                if (partial && v == cut) keep = seen++ < ties;
-                if (keep) sum += weight(v, r);
-            } else {
-                sum += weight(v, r);
-            }
+    for (int j = 0; j < len; ++j) {
+        const float v = i0 + j < i1 ? l(i0 + j) : -CUDART_INF_F;
+        bool keep = v >= from;
+        if (FILTERS) {
+            if (partial && v == cut) keep = seen++ < ties && keep;
+            if (!__any_sync(kFull, keep)) continue;
         }
+        const u64 w = weight_warp(v, r, team.mine);
+        if (keep) sum += w;
     }
     u64 total = 0;
     const u64 before = team.scan(sum, total);
-    float u = a.uniforms[row];
-    u = u > 0.0f ? fminf(u, 0x1.fffffep-1f) : 0.0f;
-    const u64 t = min((u64) ((double) u * (double) total), total - 1);
-    if (team.tid == 0) team.s->found_thread = -1;
+    const u64 t = place_of(a.uniforms[row], total);
+    if (team.tid == 0) team.s->found = -1;
     team.sync();
     if (before <= t && t < before + sum) {
-        team.s->found_thread = team.tid;
+        team.s->found = team.tid;
         team.s->found_before = before;
-        team.s->found_ties = (int) min(tie0, (u64) 0x7FFFFFFF);
+        team.s->found_ties = (int) tie0;
     }
     team.sync();
-    const int who = team.s->found_thread;
+    const int who = team.s->found;
     if (who >= 0 && team.tid < 32) {
-        u64 run = team.s->found_before;
-        u64 tie = (u64) team.s->found_ties;
-        const int b = who * len, e = min(b + len, l.n);
-        for (int c = b; c < e; c += 32) {
-            const int i = c + team.tid;
-            const float v = i < e ? l(i) : -CUDART_INF_F;
-            u64 w = 0;
-            if (v >= least && v >= cut) w = weight(v, r);
-            if (FILTERS && partial) {
-                const unsigned eq = __ballot_sync(0xFFFFFFFFu, i < e && v == cut);
-                if (v == cut && tie + __popc(eq & ((1u << team.tid) - 1u)) >= ties) w = 0;
-                tie += __popc(eq);
+        // the run again, a few consecutive elements a lane
+        const int b = who * len, e = min(b + len, l.n), per = (len + 31) / 32;
+        const int c0 = min(b + team.tid * per, e), c1 = min(c0 + per, e);
+        u64 tie = 0;
+        if (FILTERS && partial) {
+            int eq = 0;
+            for (int i = c0; i < c1; ++i) eq += l(i) == cut ? 1 : 0;
+            tie = (u64) (team.s->found_ties + warp_scan(eq, team.tid) - eq);
+        }
+        u64 x = 0, tie1 = tie;
+        for (int j = 0; j < per; ++j) {
+            const float v = c0 + j < c1 ? l(c0 + j) : -CUDART_INF_F;
+            bool keep = v >= from;
+            if (FILTERS && partial && v == cut) keep = tie1++ < ties && keep;
+            const u64 w = weight_warp(v, r, team.mine);
+            if (keep) x += w;
+        }
+        u64 run = team.s->found_before + warp_scan(x, team.tid) - x;
+        if (run <= t && t < run + x) {
+            for (int i = c0; i < c1; ++i) {
+                const float v = l(i);
+                bool keep = v >= from;
+                if (FILTERS && partial && v == cut) keep = tie++ < ties && keep;
+                const u64 w = keep ? weight_one(v, r) : 0ull;
+                if (run <= t && t < run + w) write_token(a, row, s0 + i, v, hi, temp, total);
+                run += w;
             }
-            u64 x = w;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const u64 y = __shfl_up_sync(0xFFFFFFFFu, x, o);
-                if (team.tid >= o) x += y;
-            }
-            if (w > 0 && run + x - w <= t && t < run + x) {
-                a.tokens[row] = s0 + i;
-                if (a.logprobs) {
-                    const double scaled = v == hi ? 0.0 : ((double) v - (double) hi) / (double) temp;
-                    a.logprobs[row] = (float) (scaled - log((double) total / kOne));
-                }
-            }
-            run += __shfl_sync(0xFFFFFFFFu, x, 31);
         }
     }
     if (CL) team.meet();                                         // a block's memory stays while others may read it
@@ -576,19 +793,10 @@ sample_kernel(pk_sample_args a, int slice, int teams, int row_floats) {
 
 constexpr size_t kSmemCap = 220 * 1024;
 
-template <class T, int NT, bool FILTERS, bool CL>
-cudaError_t launch(const pk_sample_args & a, int blocks, cudaStream_t s) {
+template <class T, int NT, bool FILTERS, bool CL, bool RES>
+cudaError_t launch(const pk_sample_args & a, int blocks, int slice, int row_floats, size_t smem, cudaStream_t s) {
     const int teams = NT == 32 ? 8 : 1;
-    // slices of whole 16 bytes, so that every slice is aligned as its row is
-    const int slice = CL ? ((a.vocab + blocks - 1) / blocks + 31) / 32 * 32 : a.vocab;
-    const size_t fixed = teams * (sizeof(TeamSmem<NT>) + (FILTERS ? sizeof(TeamBins<NT>) : 0)) + 16;
-    int row_floats = (slice + 4 + 3) / 4 * 4;
-    size_t smem = fixed + (size_t) teams * row_floats * 4;
-    if (smem > kSmemCap) {                                       // read from the logits each time
-        row_floats = 0;
-        smem = fixed;
-    }
-    auto kernel = sample_kernel<T, NT, FILTERS, CL>;
+    auto kernel = sample_kernel<T, NT, FILTERS, CL, RES>;
     static unsigned long long set;                               // devices on which the limit is raised
     int device = 0;
     cudaError_t e = cudaGetDevice(&device);
@@ -614,15 +822,39 @@ cudaError_t launch(const pk_sample_args & a, int blocks, cudaStream_t s) {
     return cudaLaunchKernelEx(&cfg, kernel, a, slice, teams, row_floats);
 }
 
+// Shared memory of a block: the teams' rows, then their state, then their bins.
+template <int NT, bool FILTERS>
+size_t team_bytes(int slice, int & row_floats) {
+    row_floats = (slice + 3 + 3) / 4 * 4;
+    return (NT == 32 ? 8 : 1) * ((size_t) row_floats * 4 + sizeof(TeamSmem<NT>) + (FILTERS ? sizeof(TeamBins<NT>) : 0));
+}
+
+template <class T, bool FILTERS, int NT>
+cudaError_t launch_block(const pk_sample_args & a, cudaStream_t s) {
+    int row_floats;
+    const size_t smem = team_bytes<NT, FILTERS>(a.vocab, row_floats);
+    return launch<T, NT, FILTERS, false, true>(a, 1, a.vocab, row_floats, smem, s);
+}
+
+template <class T, bool FILTERS>
+cudaError_t launch_cluster(const pk_sample_args & a, int blocks, cudaStream_t s) {
+    // slices of whole 16 bytes, so that every slice is aligned as its row is
+    const int slice = ((a.vocab + blocks - 1) / blocks + 31) / 32 * 32;
+    int row_floats;
+    const size_t smem = team_bytes<512, FILTERS>(slice, row_floats);
+    if (smem <= kSmemCap) return launch<T, 512, FILTERS, true, true>(a, blocks, slice, row_floats, smem, s);
+    return launch<T, 512, FILTERS, true, false>(a, blocks, slice, 0, smem - (size_t) row_floats * 4, s);
+}
+
 template <class T, bool FILTERS>
 cudaError_t dispatch(const pk_sample_args & a, cudaStream_t s) {
-    if (a.vocab <= 1280 && a.rows >= 512) return launch<T, 32, FILTERS, false>(a, 1, s);
-    if (a.vocab <= 2048) return launch<T, 128, FILTERS, false>(a, 1, s);
+    if (a.vocab <= 1280 && a.rows >= 512) return launch_block<T, FILTERS, 32>(a, s);
+    if (a.vocab <= 2048) return launch_block<T, FILTERS, 128>(a, s);
     int blocks = 1;
     while (blocks < kMaxCluster && a.rows * blocks * 2 <= 148 && a.vocab / (blocks * 2) >= 1024) blocks *= 2;
     while (blocks < kMaxCluster && (size_t) (a.vocab / blocks) * 4 > 200 * 1024) blocks *= 2;
-    if (blocks > 1) return launch<T, 512, FILTERS, true>(a, blocks, s);
-    return launch<T, 512, FILTERS, false>(a, 1, s);
+    if (blocks > 1) return launch_cluster<T, FILTERS>(a, blocks, s);
+    return launch_block<T, FILTERS, 512>(a, s);
 }
 
 }  // namespace
