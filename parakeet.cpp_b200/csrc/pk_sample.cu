@@ -120,6 +120,7 @@ struct TeamSmem {
     int found, found_ties;
     int listed;                              // tokens put on the list
     float cut;
+    int cut_partial;
     u64 cut_ties;
 };
 template <int NT>
@@ -151,9 +152,9 @@ struct Team {
             sync();
             if (lane() == 0) s->wscan[tid >> 5] = v;
             sync();
-            v = 0;
+            v = s->wscan[lane() & (NT / 32 - 1)];
 #pragma unroll
-            for (int i = 0; i < NT / 32; ++i) v += s->wscan[i];
+            for (int o = NT / 64; o > 0; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
         }
         if (CL) {
             Xchg & x = s->x[phase];
@@ -175,12 +176,15 @@ struct Team {
             sync();
             if (lane() == 31) s->wscan[tid >> 5] = x;
             sync();
-            t = 0;
+            u64 w = s->wscan[lane() & (NT / 32 - 1)];
 #pragma unroll
-            for (int i = 0; i < NT / 32; ++i) {
-                if (i < (tid >> 5)) before += s->wscan[i];
-                t += s->wscan[i];
+            for (int o = 1; o < NT / 32; o <<= 1) {
+                const u64 y = __shfl_up_sync(kFull, w, o, NT / 32);
+                if ((lane() & (NT / 32 - 1)) >= o) w += y;
             }
+            t = __shfl_sync(kFull, w, NT / 32 - 1);
+            w = __shfl_sync(kFull, w, max((tid >> 5) - 1, 0));
+            if (tid >= 32) before += w;
         }
         if (CL) {
             Xchg & o = s->x[phase];
@@ -198,7 +202,7 @@ struct Team {
         return before;
     }
     // Largest of hi, smallest of lo, over the team.
-    __device__ void range(float & hi, float & lo) {
+    __device__ __forceinline__ void range(float & hi, float & lo) {
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) {
             hi = fmaxf(hi, __shfl_xor_sync(kFull, hi, o));
@@ -208,8 +212,13 @@ struct Team {
             sync();
             if (lane() == 0) { s->whi[tid >> 5] = hi; s->wlo[tid >> 5] = lo; }
             sync();
+            hi = s->whi[lane() & (NT / 32 - 1)];
+            lo = s->wlo[lane() & (NT / 32 - 1)];
 #pragma unroll
-            for (int i = 0; i < NT / 32; ++i) { hi = fmaxf(hi, s->whi[i]); lo = fminf(lo, s->wlo[i]); }
+            for (int o = NT / 64; o > 0; o >>= 1) {
+                hi = fmaxf(hi, __shfl_xor_sync(kFull, hi, o));
+                lo = fminf(lo, __shfl_xor_sync(kFull, lo, o));
+            }
         }
         if (CL) {
             Xchg & x = s->x[phase];
@@ -225,15 +234,18 @@ struct Team {
     }
 };
 
+// Consecutive elements of a thread: an odd number, whose first ones lie in different banks.
+template <int NT> __host__ __device__ __forceinline__ int run_of(int n) { return ((n + NT - 1) / NT) | 1; }
+
 // The slice of a row that this block holds. RES: in shared memory, `skew` elements after a 16-byte
-// boundary, as in global memory, -infinity before and after it up to whole 16 bytes. Otherwise, for
-// slices larger than that, the logits are read again and again. `inf`: the row's maximum is
+// boundary, as in global memory, -infinity before it and after it up to `pad` elements: whole 16 bytes
+// and whole runs. Otherwise, for slices larger than that, the logits are read again and again. `inf`: the row's maximum is
 // +infinity, whose logits count as 0 and all others as -infinity.
 template <class T, bool RES>
 struct Slice {
     float * sm;
     const T * gl;
-    int n, skew;
+    int n, skew, pad;
     bool inf;
     __device__ __forceinline__ float operator()(int i) const {
         if (RES) return sm[skew + i];
@@ -245,6 +257,7 @@ struct Slice {
     __device__ __forceinline__ void each(int tid, F f) const {
         if constexpr (RES) {
             const int quads = (skew + n + 3) >> 2;
+#pragma unroll 2
             for (int q = tid & ~31; q < quads; q += NT) {
                 const int i = q + (tid & 31);
                 const float4 v = i < quads ? reinterpret_cast<const float4 *>(sm)[i]
@@ -298,7 +311,7 @@ __device__ __forceinline__ void load_slice(const Slice<T, true> & l, int tid) {
     for (int i = tid; i < head; i += NT) sm[i] = to_f32(g[i]);
     for (int i = head + vecs * W + tid; i < n; i += NT) sm[i] = to_f32(g[i]);
     if (tid < l.skew) l.sm[tid] = -CUDART_INF_F;
-    if (tid < ((l.skew + n + 3) & ~3) - (l.skew + n)) sm[n + tid] = -CUDART_INF_F;
+    for (int i = n + tid; i < l.pad; i += NT) sm[i] = -CUDART_INF_F;
     if constexpr (sizeof(T) == 4) asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
@@ -450,10 +463,10 @@ __device__ int gather(Team<NT, CL> & team, TeamBins<NT> * B, const Slice<T, RES>
 }
 
 // The cut inside the bin that find_bin found: everything above the returned logit is kept, and
-// `ties` of those equal to it.
+// `ties` of those equal to it, which may be all (`partial` false).
 template <bool WEIGHTS, class T, int NT, bool CL, bool RES>
 __device__ float find_cut(Team<NT, CL> & team, TeamBins<NT> * B, const Slice<T, RES> & l, const Row & row, Level L, u64 need,
-                          u64 & ties) {
+                          u64 & ties, bool & partial) {
     constexpr int NB = bins_of<NT>();
     TeamSmem<NT> * s = team.s;
     for (;;) {
@@ -473,10 +486,12 @@ __device__ float find_cut(Team<NT, CL> & team, TeamBins<NT> * B, const Slice<T, 
                 if (over < need && need <= over + same) {        // threads with equal logits write the same
                     s->cut = v;
                     s->cut_ties = (need - over + B->w[j] - 1) / B->w[j];
+                    s->cut_partial = s->cut_ties * B->w[j] < same;
                 }
             }
             team.sync();
             ties = s->cut_ties;
+            partial = s->cut_partial != 0;
             const float v = s->cut;
             team.sync();
             return v;
@@ -492,6 +507,7 @@ __device__ float find_cut(Team<NT, CL> & team, TeamBins<NT> * B, const Slice<T, 
         if (!(hi > lo)) {                       // one value
             const u64 each = WEIGHTS ? weight_one(hi, row) : 1ull;
             ties = (need - L.above + each - 1) / max(each, 1ull);
+            partial = true;
             return hi;
         }
         L.range(hi, lo, NB);
@@ -499,9 +515,9 @@ __device__ float find_cut(Team<NT, CL> & team, TeamBins<NT> * B, const Slice<T, 
     }
 }
 
-__device__ __forceinline__ void write_token(const pk_sample_args & a, long long row, int token, float v, float hi, double temp, u64 total) {
+__device__ __forceinline__ void write_token(const pk_sample_args & a, long long row, int token, float v, float hi, double inv_t, u64 total) {
     a.tokens[row] = token;
-    if (a.logprobs) a.logprobs[row] = (float) ((v == hi ? 0.0 : ((double) v - (double) hi) / temp) - log((double) total / kOne));
+    if (a.logprobs) a.logprobs[row] = (float) ((v == hi ? 0.0 : ((double) v - (double) hi) * inv_t) - log((double) total * (1.0 / kOne)));
 }
 
 __device__ __forceinline__ u64 place_of(float u, u64 total) {
@@ -513,7 +529,7 @@ __device__ __forceinline__ u64 place_of(float u, u64 total) {
 // `need` lies (0: the share p of the k tokens' weight), of these those that reach `least`; the draw.
 template <int NT, bool CL>
 __device__ void draw_listed(Team<NT, CL> & team, TeamBins<NT> * B, const Pair * list, int n, const pk_sample_args & a, long long row,
-                            const Row & r, float hi, double temp, int k, float p, u64 need, float least) {
+                            const Row & r, float hi, double inv_t, int k, float p, u64 need, float least) {
     for (int j = team.tid; j < n; j += NT) B->w[j] = weight_one(list[j].v, r);
     team.sync();
     constexpr int PER = (kList + NT - 1) / NT;                   // tokens of a thread
@@ -563,7 +579,7 @@ __device__ void draw_listed(Team<NT, CL> & team, TeamBins<NT> * B, const Pair * 
             u64 before = 0;
             for (int i = 0; i < n; ++i)
                 if (list[i].i < list[j].i) before += B->w[i];
-            if (before <= t && t < before + B->w[j] && team.rank == 0) write_token(a, row, list[j].i, list[j].v, hi, temp, total);
+            if (before <= t && t < before + B->w[j] && team.rank == 0) write_token(a, row, list[j].i, list[j].v, hi, inv_t, total);
         }
     }
 }
@@ -592,6 +608,8 @@ sample_kernel(pk_sample_args a, int slice, int teams, int row_floats) {
     l.sm = rows_at + (size_t) t_in * row_floats;
     l.skew = RES ? (int) ((reinterpret_cast<uintptr_t>(l.gl) & 15) / sizeof(T)) & 3 : 0;
     l.inf = false;
+    const int len = run_of<NT>(l.n);
+    l.pad = max(((l.skew + l.n + 3) & ~3) - l.skew, NT * len);
     if constexpr (RES) {
         load_slice<T, NT>(l, team.tid);
         team.sync();
@@ -643,13 +661,15 @@ sample_kernel(pk_sample_args a, int slice, int teams, int row_floats) {
     }
     Row r;
     r.top = (double) hi;
-    r.c = 46.166241308446828384 / temp;                          // 32 log2(e) / T; 0 for an infinite T
+    const double inv_t = 1.0 / temp;                             // 0 for an infinite T
+    r.c = 46.166241308446828384 * inv_t;                         // 32 log2(e) / T
     // below 2^-44 of the largest: 31 T is more than 44 ln 2 = 30.5 T; rounded up, so that what is
     // not below lies within the exponential's range
     r.base = fmaxf(__double2float_ru(r.top - 31.0 * temp), -3.402823466e+38f);
     float least = r.base;                                        // kept: >= least, and what the cut says
     float cut = -CUDART_INF_F;
     u64 ties = ~0ull;
+    bool partial = false;
     if constexpr (FILTERS) {
         constexpr int NB = bins_of<NT>();
         const float m = a.min_ps ? a.min_ps[row] : a.min_p;
@@ -670,10 +690,10 @@ sample_kernel(pk_sample_args a, int slice, int teams, int row_floats) {
                     const Pair * list;
                     const int n = gather<T, NT, CL, RES>(team, bins, l, s0, list,
                                                          [&](float v) { return L.holds(v) && L.bin_of<NB>(v) <= L.bin; });
-                    draw_listed<NT, CL>(team, bins, list, n, a, row, r, hi, temp, k, p, 0, least);
+                    draw_listed<NT, CL>(team, bins, list, n, a, row, r, hi, inv_t, k, p, 0, least);
                     return;
                 }
-                cut = find_cut<false, T, NT, CL, RES>(team, bins, l, r, L, need, ties);
+                cut = find_cut<false, T, NT, CL, RES>(team, bins, l, r, L, need, ties, partial);
             }
         }
         if (!(p >= 1.0f)) {
@@ -711,33 +731,31 @@ sample_kernel(pk_sample_args a, int slice, int teams, int row_floats) {
                     const int n = gather<T, NT, CL, RES>(team, bins, l, s0, list,
                                                          [&](float v) { return L.holds(v) && L.bin_of<NB>(v) <= L.bin; });
                     if (n <= kList) {
-                        draw_listed<NT, CL>(team, bins, list, n, a, row, r, hi, temp, kList, p, need, least);
+                        draw_listed<NT, CL>(team, bins, list, n, a, row, r, hi, inv_t, kList, p, need, least);
                         return;
                     }
                 }
-                cut = find_cut<true, T, NT, CL, RES>(team, bins, l, r, L, need, ties);
+                cut = find_cut<true, T, NT, CL, RES>(team, bins, l, r, L, need, ties, partial);
             } else if (each > 0) {
-                ties = min(ties, (need - L.with + each - 1) / each);   // the cut of k, with fewer ties
+                // the cut of k, with fewer ties
+                const u64 fewer = (need - L.with + each - 1) / each;
+                if (fewer < ties) { ties = fewer; partial = true; }
             }
         }
     }
-    // runs of consecutive indices; an odd length keeps their first elements in different banks
-    const int len = ((l.n + NT - 1) / NT) | 1;
-    const int i0 = min(team.tid * len, l.n), i1 = min(i0 + len, l.n);
+    const int i0 = RES ? team.tid * len : min(team.tid * len, l.n), i1 = RES ? i0 + len : min(i0 + len, l.n);
     // equal logits at the cut, where not all of them are kept, go by index
     u64 tie0 = 0;
-    bool partial = false;
-    if (FILTERS && cut > -CUDART_INF_F) {
+    if (FILTERS && partial) {
         u64 n = 0, all = 0;
         for (int i = i0; i < i1; ++i) n += l(i) == cut ? 1u : 0u;
         tie0 = team.scan(n, all);
-        partial = ties < all;
     }
     u64 sum = 0, seen = tie0;
     const float from = fmaxf(least, cut);
 #pragma unroll 4
     for (int j = 0; j < len; ++j) {
-        const float v = i0 + j < i1 ? l(i0 + j) : -CUDART_INF_F;
+        const float v = RES || i0 + j < i1 ? l(i0 + j) : -CUDART_INF_F;
         bool keep = v >= from;
         if (FILTERS) {
             if (partial && v == cut) keep = seen++ < ties && keep;
@@ -759,33 +777,24 @@ sample_kernel(pk_sample_args a, int slice, int teams, int row_floats) {
     team.sync();
     const int who = team.s->found;
     if (who >= 0 && team.tid < 32) {
-        // the run again, a few consecutive elements a lane
-        const int b = who * len, e = min(b + len, l.n), per = (len + 31) / 32;
-        const int c0 = min(b + team.tid * per, e), c1 = min(c0 + per, e);
-        u64 tie = 0;
-        if (FILTERS && partial) {
-            int eq = 0;
-            for (int i = c0; i < c1; ++i) eq += l(i) == cut ? 1 : 0;
-            tie = (u64) (team.s->found_ties + warp_scan(eq, team.tid) - eq);
-        }
-        u64 x = 0, tie1 = tie;
-        for (int j = 0; j < per; ++j) {
-            const float v = c0 + j < c1 ? l(c0 + j) : -CUDART_INF_F;
+        // the run again, 32 elements at a time
+        const int e = min((who + 1) * len, l.n);
+        u64 run = team.s->found_before, tie = FILTERS ? (u64) team.s->found_ties : 0ull;
+        for (int c = who * len; c < e; c += 32) {
+            const int i = c + team.tid;
+            const float v = i < e ? l(i) : -CUDART_INF_F;
             bool keep = v >= from;
-            if (FILTERS && partial && v == cut) keep = tie1++ < ties && keep;
-            const u64 w = weight_warp(v, r, team.mine);
-            if (keep) x += w;
-        }
-        u64 run = team.s->found_before + warp_scan(x, team.tid) - x;
-        if (run <= t && t < run + x) {
-            for (int i = c0; i < c1; ++i) {
-                const float v = l(i);
-                bool keep = v >= from;
-                if (FILTERS && partial && v == cut) keep = tie++ < ties && keep;
-                const u64 w = keep ? weight_one(v, r) : 0ull;
-                if (run <= t && t < run + w) write_token(a, row, s0 + i, v, hi, temp, total);
-                run += w;
+            if (FILTERS && partial) {
+                const unsigned eq = __ballot_sync(kFull, v == cut);
+                if (v == cut) keep = keep && tie + __popc(eq & ((1u << team.tid) - 1u)) < ties;
+                tie += __popc(eq);
             }
+            u64 w = weight_warp(v, r, team.mine);
+            if (!keep) w = 0;
+            const u64 x = run + warp_scan(w, team.tid);
+            if (x - w <= t && t < x) write_token(a, row, s0 + i, v, hi, inv_t, total);
+            run = __shfl_sync(kFull, x, 31);
+            if (run > t) break;
         }
     }
     if (CL) team.meet();                                         // a block's memory stays while others may read it
@@ -825,7 +834,7 @@ cudaError_t launch(const pk_sample_args & a, int blocks, int slice, int row_floa
 // Shared memory of a block: the teams' rows, then their state, then their bins.
 template <int NT, bool FILTERS>
 size_t team_bytes(int slice, int & row_floats) {
-    row_floats = (slice + 3 + 3) / 4 * 4;
+    row_floats = (std::max(slice, NT * run_of<NT>(slice)) + 3 + 3) / 4 * 4;
     return (NT == 32 ? 8 : 1) * ((size_t) row_floats * 4 + sizeof(TeamSmem<NT>) + (FILTERS ? sizeof(TeamBins<NT>) : 0));
 }
 
@@ -854,6 +863,7 @@ cudaError_t dispatch(const pk_sample_args & a, cudaStream_t s) {
     while (blocks < kMaxCluster && a.rows * blocks * 2 <= 148 && a.vocab / (blocks * 2) >= 1024) blocks *= 2;
     while (blocks < kMaxCluster && (size_t) (a.vocab / blocks) * 4 > 200 * 1024) blocks *= 2;
     if (blocks > 1) return launch_cluster<T, FILTERS>(a, blocks, s);
+    if (a.vocab <= 16384) return launch_block<T, FILTERS, 256>(a, s);
     return launch_block<T, FILTERS, 512>(a, s);
 }
 
