@@ -59,10 +59,11 @@ struct Row {
 // Weight of a logit v >= base. 2^x * 2^43 for x = (v - top) c / 32 >= -45: 32 x = n + t, n whole,
 // |t| <= 1/2; 2^(n / 32) from the table's entry n % 32 and n / 32 added to its exponent, 2^(t / 32)
 // = 1 + t q(t) with q cubic, interpolating at the four Chebyshev nodes of [-1/2, 1/2] (off by
-// 2^-42.5 at most; exactly 1 at t = 0). Adding 2^52 rounds the product to an integer in the low bits.
-// `entry(j)` gives 2^43 * table[j]; all callers share these operations, so a logit has one weight.
+// 2^-42.5 at most; exactly 1 at t = 0). Adding a number of [2^52, 2^53) rounds the product to an
+// integer in the low bits. `entry(n)` gives 2^43 * table[n % 32] with n % 32 taken off the exponent
+// field's place 15 bits up, where all of n is added. All callers share these operations.
 template <class F>
-__device__ __forceinline__ u64 weight_of(float v, const Row & r, F entry) {
+__device__ __forceinline__ double weight_onto(float v, const Row & r, double onto, F entry) {
     const double magic = 6755399441055744.0;            // 1.5 * 2^52: the sum's low word is the nearest integer
     const double d = (double) v - r.top;
     const double y = fma(d, r.c, magic);
@@ -73,18 +74,23 @@ __device__ __forceinline__ u64 weight_of(float v, const Row & r, F entry) {
     q = fma(q, t, 0.021660849392187844);
     q = fma(q, t, 1.0);
     const int n = __double2loint(y);
-    const double e = entry(n & 31);
-    const double s = __hiloint2double(__double2hiint(e) + ((n & ~31) << 15), __double2loint(e));
-    const double w = fma(q, s, 4503599627370496.0);
-    return (u64) __double_as_longlong(w) - 0x4330000000000000ull;
+    const double e = entry(n);
+    return fma(q, __hiloint2double(__double2hiint(e) + (n << 15), __double2loint(e)), onto);
 }
-// The table across a warp's lanes: every lane calls, and drops what it gets for v < base.
-__device__ __forceinline__ u64 weight_warp(float v, const Row & r, double mine) {
-    return weight_of(v, r, [&](int j) { return __shfl_sync(kFull, mine, j); });
+constexpr double kZero = 4503599627370496.0;             // 2^52
+__device__ __forceinline__ u64 whole(double onto) { return (u64) __double_as_longlong(onto) - 0x4330000000000000ull; }
+__device__ __forceinline__ double table_entry(int j) {
+    const double e = kExp2[j] * kOne;
+    return __hiloint2double(__double2hiint(e) - (j << 15), __double2loint(e));
+}
+// The table across a warp's lanes: every lane calls, and drops what it gets for v < base. A shuffle
+// takes n modulo 32.
+__device__ __forceinline__ double weight_warp(float v, const Row & r, double mine, double onto = kZero) {
+    return weight_onto(v, r, onto, [&](int n) { return __shfl_sync(kFull, mine, n); });
 }
 // Any thread by itself.
 __device__ __forceinline__ u64 weight_one(float v, const Row & r) {
-    return v >= r.base ? weight_of(v, r, [](int j) { return kExp2[j] * kOne; }) : 0ull;
+    return v >= r.base ? whole(weight_onto(v, r, kZero, [](int n) { return table_entry(n & 31); })) : 0ull;
 }
 
 template <class V> __device__ __forceinline__ V warp_sum(V v) {
@@ -359,7 +365,7 @@ __device__ bool find_bin(Team<NT, CL> & team, TeamBins<NT> * B, const Slice<T, R
         if (WEIGHTS) {
             const bool any = v <= L.hi && v >= from;
             if (!__any_sync(kFull, any)) return;
-            const u64 w = weight_warp(v, row, team.mine);
+            const u64 w = whole(weight_warp(v, row, team.mine));
             if (any) {
                 if (v >= L.lo) {
                     const int b = L.bin_of<NB>(v);
@@ -600,7 +606,7 @@ sample_kernel(pk_sample_args a, int slice, int teams, int row_floats) {
     TeamSmem<NT> * state = reinterpret_cast<TeamSmem<NT> *>(rows_at + (size_t) teams * row_floats);
     team.s = state + t_in;
     TeamBins<NT> * bins = reinterpret_cast<TeamBins<NT> *>(state + teams) + t_in;
-    team.mine = kExp2[team.lane()] * kOne;
+    team.mine = table_entry(team.lane());
     const int s0 = min(team.rank * slice, a.vocab);
     Slice<T, RES> l;
     l.n = min(slice, a.vocab - s0);
@@ -751,7 +757,10 @@ sample_kernel(pk_sample_args a, int slice, int teams, int row_floats) {
         for (int i = i0; i < i1; ++i) n += l(i) == cut ? 1u : 0u;
         tie0 = team.scan(n, all);
     }
-    u64 sum = 0, seen = tie0;
+    // a run has fewer than 2^9 elements, so its sum stays below 2^53 and is whole. (A product that
+    // lies halfway between two integers may round the other way here than by itself; see the search.)
+    double onto = kZero;
+    u64 seen = tie0;
     const float from = fmaxf(least, cut);
 #pragma unroll 4
     for (int j = 0; j < len; ++j) {
@@ -761,9 +770,10 @@ sample_kernel(pk_sample_args a, int slice, int teams, int row_floats) {
             if (partial && v == cut) keep = seen++ < ties && keep;
             if (!__any_sync(kFull, keep)) continue;
         }
-        const u64 w = weight_warp(v, r, team.mine);
-        if (keep) sum += w;
+        const double w = weight_warp(v, r, team.mine, onto);
+        if (keep) onto = w;
     }
+    const u64 sum = whole(onto);
     u64 total = 0;
     const u64 before = team.scan(sum, total);
     const u64 t = place_of(a.uniforms[row], total);
@@ -780,6 +790,7 @@ sample_kernel(pk_sample_args a, int slice, int teams, int row_floats) {
         // the run again, 32 elements at a time
         const int e = min((who + 1) * len, l.n);
         u64 run = team.s->found_before, tie = FILTERS ? (u64) team.s->found_ties : 0ull;
+        int last = -1;                       // should rounding have left t at the run's very end: its last token
         for (int c = who * len; c < e; c += 32) {
             const int i = c + team.tid;
             const float v = i < e ? l(i) : -CUDART_INF_F;
@@ -789,13 +800,16 @@ sample_kernel(pk_sample_args a, int slice, int teams, int row_floats) {
                 if (v == cut) keep = keep && tie + __popc(eq & ((1u << team.tid) - 1u)) < ties;
                 tie += __popc(eq);
             }
-            u64 w = weight_warp(v, r, team.mine);
+            u64 w = whole(weight_warp(v, r, team.mine));
             if (!keep) w = 0;
             const u64 x = run + warp_scan(w, team.tid);
             if (x - w <= t && t < x) write_token(a, row, s0 + i, v, hi, inv_t, total);
             run = __shfl_sync(kFull, x, 31);
             if (run > t) break;
+            const unsigned some = __ballot_sync(kFull, w > 0);
+            if (some) last = c + 31 - __clz(some);
         }
+        if (run <= t && team.tid == 0 && last >= 0) write_token(a, row, s0 + last, l(last), hi, inv_t, total);
     }
     if (CL) team.meet();                                         // a block's memory stays while others may read it
 }
