@@ -53,106 +53,151 @@ __device__ __forceinline__ unsigned cvt_e2m1x2(float lo, float hi) {
     return r;
 }
 
-// Eight consecutive elements of a row from column c; zeros from column K on.
+// Eight consecutive elements of a row, as loaded.
+template <class T> struct Eight { T e[8]; };
+
 template <class T, bool VEC>
-__device__ __forceinline__ void load8(const T * __restrict__ row, int c, int K, float * v) {
+__device__ __forceinline__ Eight<T> load8(const T * __restrict__ row, int c, int K) {
+    Eight<T> v;
     if (VEC && c + 8 <= K) {
-        if constexpr (sizeof(T) == 4) {
-            const float4 a = *reinterpret_cast<const float4 *>(row + c), b = *reinterpret_cast<const float4 *>(row + c + 4);
-            v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-            v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-        } else {
-            const uint4 a = *reinterpret_cast<const uint4 *>(row + c);
-            const unsigned w[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                T e[2];
-                *reinterpret_cast<unsigned *>(e) = w[i];
-                v[2 * i] = to_f32(e[0]);
-                v[2 * i + 1] = to_f32(e[1]);
-            }
-        }
+        for (int i = 0; i < (int) sizeof(T) / 2; ++i)
+            reinterpret_cast<uint4 *>(v.e)[i] = __ldcs(reinterpret_cast<const uint4 *>(row + c) + i);
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = c + i < K ? to_f32(row[c + i]) : 0.0f;
+        for (int i = 0; i < 8; ++i) v.e[i] = c + i < K ? row[c + i] : from_f32<T>(0.0f);   // zeros from column K on
     }
+    return v;
 }
 
-// One warp quantises 256 consecutive values of a row: eight per lane, four lanes a block.
+// Bits of the largest magnitude (as f32; Inf < NaN as integers, in each type).
+__device__ __forceinline__ unsigned amax_bits(const Eight<float> & v) {
+    unsigned m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v.e[i]) & 0x7FFFFFFFu);
+    return m;
+}
+template <class T> __device__ __forceinline__ unsigned amax_bits(const Eight<T> & v) {
+    const unsigned * w = reinterpret_cast<const unsigned *>(v.e);
+    const unsigned m = __vmaxu2(__vmaxu2(w[0] & 0x7FFF7FFFu, w[1] & 0x7FFF7FFFu), __vmaxu2(w[2] & 0x7FFF7FFFu, w[3] & 0x7FFF7FFFu));
+    const unsigned short h = (unsigned short) max(m & 0xFFFFu, m >> 16);
+    return __float_as_uint(to_f32(*reinterpret_cast<const T *>(&h)));
+}
+
+// Eight codes and their block's scale byte; four neighbouring lanes hold a block.
+template <class T>
+__device__ __forceinline__ unsigned quantize8(const Eight<T> & v, unsigned & sb) {
+    unsigned m = amax_bits(v);
+    m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
+    m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 2));
+    sb = scale_byte(m);
+    const float inv = scale_inv(sb);                 // garbage for byte 255, whose codes are dropped
+    unsigned q = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) q |= cvt_e2m1x2(to_f32(v.e[2 * i]) * inv, to_f32(v.e[2 * i + 1]) * inv) << (8 * i);
+    return sb == 255u ? 0u : q;
+}
+
+// A warp's 256 values of a row: eight per lane. Where a row goes on, the next 256 follow in the same
+// warp, gridDim.y segments further on; several loads are in flight before the first is used.
 // ATOMS: scales in the product's layout, zeros for the blocks past K that its stages read.
+// Bound: HBM. Rows of 1024 f32: 5.4 TB/s read and written.
 template <class T, bool VEC, bool ATOMS>
 __global__ void __launch_bounds__(kQThreads) mx4_quantize_kernel(const T * __restrict__ x, long long rows, int K, long long ldx,
                                                                  unsigned char * __restrict__ codes,
                                                                  unsigned char * __restrict__ scales) {
+    constexpr int UN = sizeof(T) == 4 ? 2 : 4;
     const int lane = threadIdx.x & 31;
-    const int segs = (K + 255) >> 8, nb = (K + 31) >> 5;
-    const long long tasks = rows * segs, stride = (long long) gridDim.x * (kQThreads / 32);
-    for (long long t = (long long) blockIdx.x * (kQThreads / 32) + (threadIdx.x >> 5); t < tasks; t += stride) {
-        const long long row = t / segs;
-        const int seg = (int) (t - row * segs);
-        const int c = seg * 256 + lane * 8;
-        const int blk = seg * 8 + (lane >> 2);
-        float v[8];
-        load8<T, VEC>(x + row * ldx, c, K, v);
-        unsigned m = 0;
+    const int segs = (K + 255) >> 8, nb = (K + 31) >> 5, chunks = scale_chunks(K);
+    const long long stride = (long long) gridDim.x * (kQThreads / 32);
+    for (long long row = (long long) blockIdx.x * (kQThreads / 32) + (threadIdx.x >> 5); row < rows; row += stride) {
+        const T * xr = x + row * ldx;
+        unsigned char * cr = codes + (size_t) row * nb * 16 + lane * 4;
+        for (int s0 = blockIdx.y; s0 < segs; s0 += UN * (int) gridDim.y) {
+            Eight<T> v[UN];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7FFFFFFFu);   // Inf < NaN as integers
-        m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
-        m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 2));
-        const unsigned sb = scale_byte(m);
-        unsigned q = 0;
-        if (sb != 255u) {
-            const float inv = scale_inv(sb);
+            for (int u = 0; u < UN; ++u) {
+                const int seg = s0 + u * (int) gridDim.y;
+                v[u] = load8<T, VEC>(xr, seg < segs ? seg * 256 + lane * 8 : K, K);
+            }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) q |= cvt_e2m1x2(v[2 * i] * inv, v[2 * i + 1] * inv) << (8 * i);
-        }
-        if (blk < nb) *reinterpret_cast<unsigned *>(codes + (size_t) row * nb * 16 + (size_t) seg * 128 + lane * 4) = q;
-        if (ATOMS) {
-            // the four bytes of a chunk's word, gathered to lanes 0 and 16
-            unsigned w = sb;
-            w |= __shfl_down_sync(0xFFFFFFFFu, sb, 4) << 8;
-            w |= __shfl_down_sync(0xFFFFFFFFu, sb, 8) << 16;
-            w |= __shfl_down_sync(0xFFFFFFFFu, sb, 12) << 24;
-            if ((lane & 15) == 0)
-                *reinterpret_cast<unsigned *>(scales + scale_at(row, blk, scale_chunks(K))) = w;
-        } else if ((lane & 3) == 0 && blk < nb) {
-            scales[(size_t) row * nb + blk] = (unsigned char) sb;
+            for (int u = 0; u < UN; ++u) {
+                const int seg = s0 + u * (int) gridDim.y;
+                if (seg >= segs) break;
+                const int blk = seg * 8 + (lane >> 2);
+                unsigned sb;
+                const unsigned q = quantize8(v[u], sb);
+                if (blk < nb) *reinterpret_cast<unsigned *>(cr + (size_t) seg * 128) = q;
+                if (ATOMS) {
+                    // the four bytes of a chunk's word, gathered to lanes 0 and 16
+                    unsigned w = sb | __shfl_down_sync(0xFFFFFFFFu, sb, 4) << 8;
+                    w |= __shfl_down_sync(0xFFFFFFFFu, w, 8) << 16;
+                    if ((lane & 15) == 0) *reinterpret_cast<unsigned *>(scales + scale_at(row, blk, chunks)) = w;
+                } else if ((lane & 3) == 0 && blk < nb) {
+                    scales[(size_t) row * nb + blk] = (unsigned char) sb;
+                }
+            }
         }
     }
 }
 
-// The value of each code: one thread per eight values.
+// Eight codes as bf16 bit patterns, two a word: 0, 0x3F00, 0x3F80, 0x3FC0, 0x4000, 0x4040, 0x4080,
+// 0x40C0 and the sign. Four codes' low and high bytes are each one byte permutation.
+__device__ __forceinline__ void codes_to_bf16(unsigned q, unsigned * w) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const unsigned c = (q >> (16 * h)) & 0xFFFFu, sel = c & 0x7777u;
+        const unsigned lo = __byte_perm(0xC0800000u, 0xC0804000u, sel), hi = __byte_perm(0x3F3F3F00u, 0x40404040u, sel);
+        const unsigned sign = (c & 0x8u) << 4 | (c & 0x80u) << 8 | (c & 0x800u) << 12 | (c & 0x8000u) << 16;
+        w[2 * h] = __byte_perm(lo, hi | sign, 0x5140);
+        w[2 * h + 1] = __byte_perm(lo, hi | sign, 0x7362);
+    }
+}
+
+// The value of each code, eight a lane. Bound: HBM, writing y.
 template <class T, bool VEC>
 __global__ void __launch_bounds__(kQThreads) mx4_dequantize_kernel(const unsigned char * __restrict__ codes,
                                                                    const unsigned char * __restrict__ scales, long long rows,
                                                                    int K, T * __restrict__ y, long long ldy) {
+    constexpr int UN = 4;
     const int lane = threadIdx.x & 31;
     const int segs = (K + 255) >> 8, nb = (K + 31) >> 5;
-    const long long tasks = rows * segs, stride = (long long) gridDim.x * (kQThreads / 32);
-    for (long long t = (long long) blockIdx.x * (kQThreads / 32) + (threadIdx.x >> 5); t < tasks; t += stride) {
-        const long long row = t / segs;
-        const int seg = (int) (t - row * segs);
-        const int c = seg * 256 + lane * 8;
-        const int blk = seg * 8 + (lane >> 2);
-        if (c >= K) continue;
-        const unsigned q = *reinterpret_cast<const unsigned *>(codes + (size_t) row * nb * 16 + (size_t) seg * 128 + lane * 4);
-        const float s = scale_val(scales[(size_t) row * nb + blk]);
-        T o[8];
+    const long long stride = (long long) gridDim.x * (kQThreads / 32);
+    for (long long row = (long long) blockIdx.x * (kQThreads / 32) + (threadIdx.x >> 5); row < rows; row += stride) {
+        const unsigned char * cr = codes + (size_t) row * nb * 16 + lane * 4, * sr = scales + (size_t) row * nb + (lane >> 2);
+        for (int s0 = blockIdx.y; s0 < segs; s0 += UN * (int) gridDim.y) {
+            unsigned q[UN];
+            unsigned char b[UN];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const unsigned code = (q >> (4 * i)) & 15u, e = (code >> 1) & 3u, man = code & 1u;
-            const float mag = e == 0u ? 0.5f * (float) man : __uint_as_float(((126u + e) << 23) | (man << 22));
-            o[i] = from_f32<T>((code & 8u) ? -mag * s : mag * s);
-        }
-        T * d = y + row * ldy + c;
-        if (VEC && c + 8 <= K) {
-            const uint4 * w = reinterpret_cast<const uint4 *>(o);
+            for (int u = 0; u < UN; ++u) {
+                const int seg = s0 + u * (int) gridDim.y;
+                const bool in = seg * 256 + lane * 8 < K;
+                q[u] = in ? __ldcs(reinterpret_cast<const unsigned *>(cr + (size_t) seg * 128)) : 0u;
+                b[u] = in ? __ldcs(sr + seg * 8) : (unsigned char) 0;
+            }
 #pragma unroll
-            for (int i = 0; i < (int) (8 * sizeof(T) / 16); ++i) reinterpret_cast<uint4 *>(d)[i] = w[i];
-        } else {
+            for (int u = 0; u < UN; ++u) {
+                const int c = (s0 + u * (int) gridDim.y) * 256 + lane * 8;
+                if (c >= K) continue;
+                const float s = scale_val(b[u]);
+                unsigned w[4];
+                codes_to_bf16(q[u], w);
+                Eight<T> o;
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (c + i < K) d[i] = o[i];
+                for (int i = 0; i < 4; ++i) {
+                    o.e[2 * i] = from_f32<T>(__uint_as_float(w[i] << 16) * s);
+                    o.e[2 * i + 1] = from_f32<T>(__uint_as_float(w[i] & 0xFFFF0000u) * s);
+                }
+                T * d = y + row * ldy + c;
+                if (VEC && c + 8 <= K) {
+#pragma unroll
+                    for (int i = 0; i < (int) sizeof(T) / 2; ++i) reinterpret_cast<uint4 *>(d)[i] = reinterpret_cast<const uint4 *>(o.e)[i];
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        if (c + i < K) d[i] = o.e[i];
+                }
+            }
         }
     }
 }
@@ -183,12 +228,13 @@ __global__ void __launch_bounds__(kQThreads) mx4_repack_kernel(const unsigned ch
 // tcgen05.mma kind::mxf4 with block scales: 64 values of K a product, accumulator in tensor memory.
 // One persistent CTA an SM walks over 128 x BN tiles of y. Warp 0 loads (codes by TMA, 256 values =
 // one 128-byte swizzled row a stage; scale atoms by bulk copies), warp 1 copies the stage's scales to
-// tensor memory and issues its four products, warps 4-7 empty the accumulator, of which there are
+// tensor memory and issues its four products, warps 4-11 empty the accumulator, of which there are
 // two, so that a tile's epilogue runs under the next tile's products. Each stage has tensor-memory
 // columns of its own for its scales: they are free when the stage is.
 constexpr int kTM = 128;
 constexpr int kTStages = 4;
-constexpr int kTThreads = 256;
+constexpr int kTThreads = 384;
+constexpr int kTEpi = 8;                                // warps of the epilogue: two for each 32 rows
 constexpr unsigned kScaleA = 1024, kScaleB = 2048;      // two atoms of A rows; two of each of two of B's
 constexpr unsigned kScaleCols = 24;                     // tensor-memory columns of a stage's scales: 8 + 16
 constexpr long long kWaitNs = 2000000000LL;             // bound on every device-side wait
@@ -202,7 +248,7 @@ struct TcSmem {
 template <int BN> constexpr unsigned tc_stage_bytes() { return kTM * 128u + BN * 128u + kScaleA + kScaleB; }
 constexpr unsigned kOutPitch = 33;                      // floats per staged row of the epilogue
 template <int BN> constexpr size_t tc_smem_bytes() {
-    return 1024 + (size_t) kTStages * tc_stage_bytes<BN>() + 4 * 32 * kOutPitch * 4 + sizeof(TcSmem);
+    return 1024 + (size_t) kTStages * tc_stage_bytes<BN>() + kTEpi * 32 * kOutPitch * 4 + sizeof(TcSmem);
 }
 
 // Wait with a bound and nothing else to end it: for copies in flight before an early exit.
@@ -221,7 +267,7 @@ mx4_tc_kernel(const __grid_constant__ CUtensorMap amap, const unsigned char * __
     extern __shared__ __align__(1024) unsigned char raw[];
     unsigned char * ring = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t) 1023);
     float * out = reinterpret_cast<float *>(ring + kTStages * tc_stage_bytes<BN>());
-    TcSmem & S = *reinterpret_cast<TcSmem *>(out + 4 * 32 * kOutPitch);
+    TcSmem & S = *reinterpret_cast<TcSmem *>(out + kTEpi * 32 * kOutPitch);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int chunks = scale_chunks(K), nks = chunks / 2, atoms = (N + 127) / 128;
     const int nt = (N + BN - 1) / BN;
@@ -234,7 +280,7 @@ mx4_tc_kernel(const __grid_constant__ CUtensorMap amap, const unsigned char * __
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(&S.acc_full[b], 1);
-            mbar_init(&S.acc_empty[b], 4);
+            mbar_init(&S.acc_empty[b], kTEpi);
         }
         mbar_init(&S.done, 1);
         S.err = 0;
@@ -308,8 +354,9 @@ mx4_tc_kernel(const __grid_constant__ CUtensorMap amap, const unsigned char * __
             mbar_drain(&S.done, 0u);
         }
     } else if (warp >= 4) {
-        const int q = warp - 4;                          // this warp's tensor-memory lanes: rows 32 q ..
-        float * st = out + q * 32 * kOutPitch;
+        const int q = warp & 3;                          // this warp's tensor-memory lanes: rows 32 q ..
+        const int half = (warp - 4) >> 2;                // its columns: every other 32
+        float * st = out + (warp - 4) * 32 * kOutPitch;
         unsigned tile = 0;
         for (long long t = blockIdx.x; t < tiles; t += gridDim.x, ++tile) {
             const long long m0 = (t / nt) * kTM + q * 32;
@@ -319,18 +366,23 @@ mx4_tc_kernel(const __grid_constant__ CUtensorMap amap, const unsigned char * __
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const int rows = (int) min(32LL, M - m0);
 #pragma unroll 1
-            for (int c = 0; c < BN && n0 + c < N; c += 32) {
+            for (int c = half * 32; c < BN && n0 + c < N; c += 64) {
                 unsigned v[32];
                 tmem_load32(tmem + buf * BN + c + ((unsigned) (q * 32) << 16), v);
+                const int n = n0 + c + lane;
+                const float bv = bias && n < N ? __ldg(bias + n) : 0.0f;
                 asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
                 for (int i = 0; i < 32; ++i) st[lane * kOutPitch + i] = __uint_as_float(v[i]);
                 __syncwarp();
-                const int n = n0 + c + lane;
                 if (n < N) {
-                    const float bv = bias ? __ldg(bias + n) : 0.0f;
                     T * o = y + m0 * ldy + n;
-                    for (int r = 0; r < rows; ++r, o += ldy) *o = from_f32<T>(st[r * kOutPitch + lane] + bv);
+                    if (rows == 32) {
+#pragma unroll
+                        for (int r = 0; r < 32; ++r, o += ldy) *o = from_f32<T>(st[r * kOutPitch + lane] + bv);
+                    } else {
+                        for (int r = 0; r < rows; ++r, o += ldy) *o = from_f32<T>(st[r * kOutPitch + lane] + bv);
+                    }
                 }
                 __syncwarp();
             }
@@ -347,10 +399,11 @@ mx4_tc_kernel(const __grid_constant__ CUtensorMap amap, const unsigned char * __
     if (threadIdx.x == 0 && S.err != 0) atomicExch_system(err_out, 1);
 }
 
-// Launch of a row kernel: one warp per 256 values, as many blocks as that takes up to a few waves.
-inline unsigned row_blocks(long long rows, long long K) {
-    const long long tasks = rows * ((K + 255) / 256);
-    return (unsigned) std::min<long long>((tasks + kQThreads / 32 - 1) / (kQThreads / 32), 148LL * 64);
+// Launch of a row kernel: a warp a row, up to a few waves; with few rows a warp for each 256 values.
+inline dim3 row_blocks(long long rows, long long K) {
+    const long long x = std::min<long long>((rows + kQThreads / 32 - 1) / (kQThreads / 32), 148LL * 32);
+    const long long segs = (K + 255) / 256;
+    return dim3((unsigned) x, (unsigned) std::max<long long>(1, std::min<long long>(segs, 148 * 8 / x)));
 }
 
 template <bool ATOMS>
@@ -358,7 +411,7 @@ cudaError_t launch_quantize(const void * x, int type, long long rows, int K, lon
                             unsigned char * scales, cudaStream_t s) {
     if (rows <= 0) return cudaSuccess;
     const bool vec = aligned_to(x, 16) && (ldx * elem_size(type)) % 16 == 0;
-    const unsigned g = row_blocks(rows, K);
+    const dim3 g = row_blocks(rows, K);
 #define PK_Q(T) \
     if (vec) mx4_quantize_kernel<T, true, ATOMS><<<g, kQThreads, 0, s>>>(static_cast<const T *>(x), rows, K, ldx, codes, scales); \
     else mx4_quantize_kernel<T, false, ATOMS><<<g, kQThreads, 0, s>>>(static_cast<const T *>(x), rows, K, ldx, codes, scales)
@@ -517,7 +570,7 @@ extern "C" PK_API pk_status pk_mx4_dequantize(int device, const uint8_t * codes,
     DeviceScope dev(device);
     if (dev.err != cudaSuccess) return op_cuda_fail(dev.err, fn);
     const bool vec = aligned_to(y, 16) && (row_stride * elem_size(y_type)) % 16 == 0;
-    const unsigned g = row_blocks(rows, cols);
+    const dim3 g = row_blocks(rows, cols);
     cudaStream_t s = (cudaStream_t) stream;
 #define PK_D(T) \
     if (vec) mx4_dequantize_kernel<T, true><<<g, kQThreads, 0, s>>>(codes, scales, rows, (int) cols, static_cast<T *>(y), row_stride); \
