@@ -500,14 +500,14 @@ PK_API pk_status pk_mx4_create(int device, const pk_tensor * weight, int32_t on_
 /* Waits for the device's queued work, so no call on the layer is still running. */
 PK_API void      pk_mx4_destroy(pk_mx4 * w);
 /* Bytes of device workspace that pk_mx4_linear needs for `rows` rows (never less for
- * more rows); 0 for rows <= 0, -1 for a null layer. */
+ * more rows), 0 where it needs none; -1 for a null layer. */
 PK_API int64_t   pk_mx4_workspace(const pk_mx4 * w, int64_t rows);
 /* y[m][n] = bias[n] + sum_k q(x)[m][k] * W[n][k]: each row of x is quantised to MXFP4
  * as pk_mx4_quantize does, products are exact and sums are held in 32 bits; y rounds
  * once to y_type. x: [rows][x_stride], y: [rows][y_stride] (strides in elements; what
  * lies past K or N in a row is neither read nor written). rows from 0 to 2^31 - 1.
- * workspace: pk_mx4_workspace(w, rows) bytes, 256-byte aligned, for this call alone
- * until it has run: calls that may overlap (two streams, two captured graphs) each
+ * workspace: pk_mx4_workspace(w, rows) bytes (0: may be NULL), 256-byte aligned, for this call
+ * alone until it has run: calls that may overlap (two streams, two captured graphs) each
  * need their own. Calls on one layer may overlap otherwise. PK_ERR_TIMEOUT: a bounded
  * device-side wait of an EARLIER call on this layer ran out and that call's y is not
  * to be used (reported once). */

@@ -250,19 +250,25 @@ EncodeFn encode_fn() {
     return fn;
 }
 
-// 2-D row-major tensor map: rows x cols of `type`, box box_rows x box_cols.
-cudaError_t encode_2d(void * map, CUtensorMapDataType type, size_t esize, const void * base, long long rows,
-                      long long cols, int box_rows, int box_cols, CUtensorMapSwizzle swz) {
+// 2-D row-major tensor map: rows x cols of `type`, rows `stride` bytes apart, box box_rows x box_cols.
+cudaError_t encode_2d_strided(void * map, CUtensorMapDataType type, const void * base, long long rows, long long cols,
+                              long long stride, int box_rows, int box_cols, CUtensorMapSwizzle swz) {
     EncodeFn fn = encode_fn();
     if (fn == nullptr) return cudaErrorNotSupported;
     const cuuint64_t dims[2] = {(cuuint64_t) cols, (cuuint64_t) rows};
-    const cuuint64_t strides[1] = {(cuuint64_t) cols * esize};
+    const cuuint64_t strides[1] = {(cuuint64_t) stride};
     const cuuint32_t box[2] = {(cuuint32_t) box_cols, (cuuint32_t) box_rows};
     const cuuint32_t estr[2] = {1, 1};
     const CUresult r = fn(reinterpret_cast<CUtensorMap *>(map), type, 2, const_cast<void *>(base), dims, strides, box,
                           estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swz, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
+// The same, rows back to back.
+cudaError_t encode_2d(void * map, CUtensorMapDataType type, size_t esize, const void * base, long long rows,
+                      long long cols, int box_rows, int box_cols, CUtensorMapSwizzle swz) {
+    return encode_2d_strided(map, type, base, rows, cols, cols * (long long) esize, box_rows, box_cols, swz);
 }
 
 cudaError_t encproj_tc_prepare(const float * w, int J, int K, unsigned short * w16, void * tmap_out, cudaStream_t s) {

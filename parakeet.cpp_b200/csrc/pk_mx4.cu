@@ -21,6 +21,8 @@ namespace pk {
 
 cudaError_t encode_2d(void * map, CUtensorMapDataType type, size_t esize, const void * base, long long rows, long long cols,
                       int box_rows, int box_cols, CUtensorMapSwizzle swz);   // pk_encproj.cu
+cudaError_t encode_2d_strided(void * map, CUtensorMapDataType type, const void * base, long long rows, long long cols,
+                              long long stride, int box_rows, int box_cols, CUtensorMapSwizzle swz);
 
 namespace {
 
@@ -70,12 +72,17 @@ __device__ __forceinline__ Eight<T> load8(const T * __restrict__ row, int c, int
     return v;
 }
 
+// Largest magnitude of three; a NaN if one is.
+__device__ __forceinline__ float max3_abs(float a, float b, float c) {
+    float m;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(fabsf(a)), "f"(fabsf(b)), "f"(fabsf(c)));
+    return m;
+}
+
 // Bits of the largest magnitude (as f32; Inf < NaN as integers, in each type).
 __device__ __forceinline__ unsigned amax_bits(const Eight<float> & v) {
-    unsigned m = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v.e[i]) & 0x7FFFFFFFu);
-    return m;
+    const float m = max3_abs(max3_abs(v.e[0], v.e[1], v.e[2]), max3_abs(v.e[3], v.e[4], v.e[5]), max3_abs(v.e[6], v.e[7], 0.0f));
+    return __float_as_uint(m);
 }
 template <class T> __device__ __forceinline__ unsigned amax_bits(const Eight<T> & v) {
     const unsigned * w = reinterpret_cast<const unsigned *>(v.e);
@@ -92,10 +99,18 @@ __device__ __forceinline__ unsigned quantize8(const Eight<T> & v, unsigned & sb)
     m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 2));
     sb = scale_byte(m);
     const float inv = scale_inv(sb);                 // garbage for byte 255, whose codes are dropped
-    unsigned q = 0;
+    unsigned c[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) q |= cvt_e2m1x2(to_f32(v.e[2 * i]) * inv, to_f32(v.e[2 * i + 1]) * inv) << (8 * i);
+    for (int i = 0; i < 4; ++i) c[i] = cvt_e2m1x2(to_f32(v.e[2 * i]) * inv, to_f32(v.e[2 * i + 1]) * inv);
+    const unsigned q = __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
     return sb == 255u ? 0u : q;
+}
+
+// The scale bytes of a warp's eight blocks (each in four lanes) as two words of four, in lanes 0 and 16.
+__device__ __forceinline__ unsigned scale_word(unsigned sb) {
+    unsigned w = sb | __shfl_down_sync(0xFFFFFFFFu, sb, 4) << 8;
+    w |= __shfl_down_sync(0xFFFFFFFFu, w, 8) << 16;
+    return w;
 }
 
 // A warp's 256 values of a row: eight per lane. Where a row goes on, the next 256 follow in the same
@@ -129,10 +144,8 @@ __global__ void __launch_bounds__(kQThreads) mx4_quantize_kernel(const T * __res
                 const unsigned q = quantize8(v[u], sb);
                 if (blk < nb) *reinterpret_cast<unsigned *>(cr + (size_t) seg * 128) = q;
                 if (ATOMS) {
-                    // the four bytes of a chunk's word, gathered to lanes 0 and 16
-                    unsigned w = sb | __shfl_down_sync(0xFFFFFFFFu, sb, 4) << 8;
-                    w |= __shfl_down_sync(0xFFFFFFFFu, w, 8) << 16;
-                    if ((lane & 15) == 0) *reinterpret_cast<unsigned *>(scales + scale_at(row, blk, chunks)) = w;
+                    const unsigned word = scale_word(sb);
+                    if ((lane & 15) == 0) *reinterpret_cast<unsigned *>(scales + scale_at(row, blk, chunks)) = word;
                 } else if ((lane & 3) == 0 && blk < nb) {
                     scales[(size_t) row * nb + blk] = (unsigned char) sb;
                 }
@@ -246,9 +259,9 @@ struct TcSmem {
 };
 
 template <int BN> constexpr unsigned tc_stage_bytes() { return kTM * 128u + BN * 128u + kScaleA + kScaleB; }
-constexpr unsigned kOutPitch = 33;                      // floats per staged row of the epilogue
+constexpr unsigned kOutBytes = 4096;                    // an epilogue warp's 32 staged rows of 128 bytes
 template <int BN> constexpr size_t tc_smem_bytes() {
-    return 1024 + (size_t) kTStages * tc_stage_bytes<BN>() + kTEpi * 32 * kOutPitch * 4 + sizeof(TcSmem);
+    return 1024 + (size_t) kTStages * tc_stage_bytes<BN>() + kTEpi * kOutBytes + sizeof(TcSmem);
 }
 
 // Wait with a bound and nothing else to end it: for copies in flight before an early exit.
@@ -259,15 +272,97 @@ __device__ __forceinline__ void mbar_drain(unsigned long long * b, unsigned pari
     while (!mbar_test(b, parity) && (long long) (now - t0) <= kWaitNs) asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
 }
 
-template <class T, int BN>
+// A warp's 32 rows of an accumulator to y, every other 128 bytes of them (`half`), through shared
+// memory. BOX: staged as the 128-byte swizzle has it and stored by TMA, which leaves out what lies past
+// M or N; otherwise by the warp, a row's values together.
+template <class T> constexpr int store_cols() { return 128 / (int) sizeof(T); }
+
+__device__ __forceinline__ void box_store(const CUtensorMap * map, int n, long long m, const void * src) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];"
+                 :: "l"(map), "r"(n), "r"((int) m), "r"(smem_u32(src)) : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+
+template <class T, int BN, bool BOX>
+__device__ __forceinline__ void store_tile(unsigned acc, unsigned char * st, int half, int lane, long long m0, int rows, int n0, int N,
+                                           const float * __restrict__ bias, T * __restrict__ y, long long ldy, const CUtensorMap * ymap) {
+    if constexpr (BOX) {
+        constexpr int COLS = store_cols<T>(), PARTS = COLS / 32;
+#pragma unroll 1
+        for (int c = half * COLS; c < BN && n0 + c < N; c += 2 * COLS) {
+            if (rows <= 0) break;
+            if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+            __syncwarp();
+#pragma unroll
+            for (int h = 0; h < PARTS; ++h) {
+                unsigned v[32];
+                tmem_load32(acc + c + h * 32, v);
+                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                if (bias) {                              // padded to whole tiles
+                    const float4 * b4 = reinterpret_cast<const float4 *>(bias + n0 + c + h * 32);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const float4 b = __ldg(b4 + i);
+                        v[4 * i] = __float_as_uint(__uint_as_float(v[4 * i]) + b.x);
+                        v[4 * i + 1] = __float_as_uint(__uint_as_float(v[4 * i + 1]) + b.y);
+                        v[4 * i + 2] = __float_as_uint(__uint_as_float(v[4 * i + 2]) + b.z);
+                        v[4 * i + 3] = __float_as_uint(__uint_as_float(v[4 * i + 3]) + b.w);
+                    }
+                }
+                if constexpr (sizeof(T) == 4) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        *reinterpret_cast<uint4 *>(st + lane * 128 + ((i ^ (lane & 7)) << 4)) =
+                            make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        T e[8];
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) e[j] = from_f32<T>(__uint_as_float(v[8 * i + j]));
+                        *reinterpret_cast<uint4 *>(st + lane * 128 + (((h * 4 + i) ^ (lane & 7)) << 4)) = *reinterpret_cast<const uint4 *>(e);
+                    }
+                }
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) box_store(ymap, n0 + c, m0, st);
+        }
+    } else {
+        float * sf = reinterpret_cast<float *>(st);      // value i of row r at place i ^ r of the row
+#pragma unroll 1
+        for (int c = half * 32; c < BN && n0 + c < N; c += 64) {
+            unsigned v[32];
+            tmem_load32(acc + c, v);
+            const int n = n0 + c + lane;
+            const float bv = bias && n < N ? __ldg(bias + n) : 0.0f;
+            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+            for (int i = 0; i < 32; ++i) sf[lane * 32 + (i ^ lane)] = __uint_as_float(v[i]);
+            __syncwarp();
+            if (n < N) {
+                T * o = y + m0 * ldy + n;
+                if (rows == 32) {
+#pragma unroll
+                    for (int r = 0; r < 32; ++r, o += ldy) *o = from_f32<T>(sf[r * 32 + (lane ^ r)] + bv);
+                } else {
+                    for (int r = 0; r < rows; ++r, o += ldy) *o = from_f32<T>(sf[r * 32 + (lane ^ r)] + bv);
+                }
+            }
+            __syncwarp();
+        }
+    }
+}
+
+template <class T, int BN, bool BOX>
 __global__ void __launch_bounds__(kTThreads, 1)
 mx4_tc_kernel(const __grid_constant__ CUtensorMap amap, const unsigned char * __restrict__ ascale, long long M, int K,
               const __grid_constant__ CUtensorMap wmap, const unsigned char * __restrict__ wscale, int N,
-              const float * __restrict__ bias, T * __restrict__ y, long long ldy, int * err_out) {
+              const float * __restrict__ bias, T * __restrict__ y, long long ldy, const __grid_constant__ CUtensorMap ymap, int * err_out) {
     extern __shared__ __align__(1024) unsigned char raw[];
     unsigned char * ring = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t) 1023);
-    float * out = reinterpret_cast<float *>(ring + kTStages * tc_stage_bytes<BN>());
-    TcSmem & S = *reinterpret_cast<TcSmem *>(out + kTEpi * 32 * kOutPitch);
+    unsigned char * out = reinterpret_cast<unsigned char *>(ring + kTStages * tc_stage_bytes<BN>());
+    TcSmem & S = *reinterpret_cast<TcSmem *>(out + kTEpi * kOutBytes);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int chunks = scale_chunks(K), nks = chunks / 2, atoms = (N + 127) / 128;
     const int nt = (N + BN - 1) / BN;
@@ -356,7 +451,7 @@ mx4_tc_kernel(const __grid_constant__ CUtensorMap amap, const unsigned char * __
     } else if (warp >= 4) {
         const int q = warp & 3;                          // this warp's tensor-memory lanes: rows 32 q ..
         const int half = (warp - 4) >> 2;                // its columns: every other 32
-        float * st = out + (warp - 4) * 32 * kOutPitch;
+        unsigned char * st = out + (warp - 4) * kOutBytes;
         unsigned tile = 0;
         for (long long t = blockIdx.x; t < tiles; t += gridDim.x, ++tile) {
             const long long m0 = (t / nt) * kTM + q * 32;
@@ -364,28 +459,169 @@ mx4_tc_kernel(const __grid_constant__ CUtensorMap amap, const unsigned char * __
             const unsigned buf = tile & 1u;
             if (!mbar_wait(&S.acc_full[buf], (tile >> 1) & 1u, kWaitNs, &S.err)) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const int rows = (int) min(32LL, M - m0);
-#pragma unroll 1
-            for (int c = half * 32; c < BN && n0 + c < N; c += 64) {
-                unsigned v[32];
-                tmem_load32(tmem + buf * BN + c + ((unsigned) (q * 32) << 16), v);
-                const int n = n0 + c + lane;
-                const float bv = bias && n < N ? __ldg(bias + n) : 0.0f;
-                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-                for (int i = 0; i < 32; ++i) st[lane * kOutPitch + i] = __uint_as_float(v[i]);
-                __syncwarp();
-                if (n < N) {
-                    T * o = y + m0 * ldy + n;
-                    if (rows == 32) {
-#pragma unroll
-                        for (int r = 0; r < 32; ++r, o += ldy) *o = from_f32<T>(st[r * kOutPitch + lane] + bv);
-                    } else {
-                        for (int r = 0; r < rows; ++r, o += ldy) *o = from_f32<T>(st[r * kOutPitch + lane] + bv);
-                    }
+            const int rows = (int) max(0LL, min(32LL, M - m0));
+            store_tile<T, BN, BOX>(tmem + buf * BN + ((unsigned) (q * 32) << 16), st, half, lane, m0, rows, n0, N, bias, y, ldy, &ymap);
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            if (lane == 0) mbar_arrive(&S.acc_empty[buf]);
+        }
+        if (BOX && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (warp == 2) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(512u) : "memory");
+    }
+    if (threadIdx.x == 0 && S.err != 0) atomicExch_system(err_out, 1);
+}
+
+// ---- few rows: quantisation and product in one kernel -----------------------------
+//
+// With up to 32 rows the time is that of launches and of single loads, and the weights are nearly all
+// of the bytes: every block quantises the rows for itself, into the products' layout in its shared
+// memory, while the first weights are on their way, and takes its share of the tiles of 64 outputs.
+// One launch: 9.0 us for 1 x 640 by 8198 called from Python, 12.6 us with a kernel for each. Not so
+// for more rows: at 64 the rows' loads, again in every block, take longer than the second launch
+// (14.3 us against 12.8), and at 66044 two kernels are 97 us against 111 with the codes kept on the
+// SM, sixteen warps of one block being too few to keep x streaming.
+constexpr int kFewRows = 32;
+constexpr int kFewK = 2048;                             // the rows' codes stay in shared memory
+constexpr int kFewN = 64;
+constexpr int kFewStages = 4;
+constexpr int kFewQuant = 16;                           // quantising warps
+constexpr int kFewThreads = 32 * (4 + kFewQuant + 8);
+constexpr unsigned kFewSeg = kTM * 128u + kScaleA;      // codes and scales of 256 values of K
+constexpr unsigned kFewStage = kFewN * 128u + 1024u;
+
+struct FewSmem {
+    unsigned long long full[kFewStages], empty[kFewStages], a_full, acc_full[2], acc_empty[2], done;
+    unsigned tmem;
+    int err;
+};
+constexpr size_t few_smem(int nks) { return 1024 + (size_t) nks * kFewSeg + kFewStages * kFewStage + 2 * kOutBytes + sizeof(FewSmem); }
+
+template <class TX, class TY, bool VEC>
+__global__ void __launch_bounds__(kFewThreads, 1)
+mx4_few_kernel(const TX * __restrict__ x, long long ldx, int M, int K, const __grid_constant__ CUtensorMap wmap,
+               const unsigned char * __restrict__ wscale, int N, const float * __restrict__ bias, TY * __restrict__ y, long long ldy,
+               int * err_out) {
+    extern __shared__ __align__(1024) unsigned char raw[];
+    const int chunks = scale_chunks(K), nks = chunks / 2, nt = (N + kFewN - 1) / kFewN;
+    unsigned char * a = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t) 1023);
+    unsigned char * sa = a + (size_t) nks * kTM * 128;    // the rows' scales follow their codes
+    unsigned char * ring = sa + nks * kScaleA;
+    unsigned char * out = ring + kFewStages * kFewStage;
+    FewSmem & S = *reinterpret_cast<FewSmem *>(out + 2 * kOutBytes);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kFewStages; ++s) {
+            mbar_init(&S.full[s], 1);
+            mbar_init(&S.empty[s], 1);
+        }
+        mbar_init(&S.a_full, kFewQuant);
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(&S.acc_full[b], 1);
+            mbar_init(&S.acc_empty[b], 2);
+        }
+        mbar_init(&S.done, 1);
+        S.err = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 2) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+                     :: "r"(smem_u32(&S.tmem)), "r"(256u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const unsigned tmem = S.tmem;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            unsigned it = 0;
+            bool ok = true;
+            for (int t = blockIdx.x; t < nt && ok; t += gridDim.x) {
+                const int n0 = t * kFewN;
+                const unsigned char * bs = wscale + (size_t) (n0 >> 7) * chunks * 512;
+                for (int ks = 0; ks < nks; ++ks, ++it) {
+                    const int s = (int) (it % kFewStages);
+                    if (!mbar_wait(&S.empty[s], ((it / kFewStages) & 1u) ^ 1u, kWaitNs, &S.err)) { ok = false; break; }
+                    unsigned char * b = ring + s * kFewStage;
+                    mbar_expect(&S.full[s], kFewStage);
+                    tma_load_2d(b, &wmap, ks * 128, n0, &S.full[s]);
+                    bulk_load(b + kFewN * 128, bs + (size_t) ks * 1024, 1024, &S.full[s]);
                 }
-                __syncwarp();
             }
+            for (unsigned j = it > kFewStages ? it - kFewStages : 0; j < it; ++j) mbar_drain(&S.full[j % kFewStages], (j / kFewStages) & 1u);
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            unsigned it = 0, tile = 0;
+            bool ok = mbar_wait(&S.a_full, 0u, kWaitNs, &S.err);
+            for (int t = blockIdx.x; t < nt && ok; t += gridDim.x, ++tile) {
+                const unsigned buf = tile & 1u, d = tmem + buf * kFewN, shift = (unsigned) ((t * kFewN) & 127) >> 5;
+                if (!mbar_wait(&S.acc_empty[buf], ((tile >> 1) & 1u) ^ 1u, kWaitNs, &S.err)) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                for (int ks = 0; ks < nks; ++ks, ++it) {
+                    const int s = (int) (it % kFewStages);
+                    if (!mbar_wait(&S.full[s], (it / kFewStages) & 1u, kWaitNs, &S.err)) { ok = false; break; }
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const unsigned ka = smem_u32(a) + (unsigned) ks * kTM * 128u, ksa = smem_u32(sa) + (unsigned) ks * kScaleA;
+                    const unsigned kb = smem_u32(ring + s * kFewStage), ksb = kb + kFewN * 128u;
+                    const unsigned ca = tmem + 2 * kFewN + (unsigned) s * 16u, cb = ca + 8;
+#pragma unroll
+                    for (unsigned c = 0; c < 2; ++c) {
+                        umma_copy_scales(ca + c * 4, ksa + c * 512);
+                        umma_copy_scales(cb + c * 4, ksb + c * 512);
+                    }
+#pragma unroll
+                    for (unsigned j = 0; j < 4; ++j)
+                        umma_mxf4(d, umma_desc_sw128(ka + j * 32), umma_desc_sw128(kb + j * 32), umma_idesc_mxf4(kTM, kFewN, 2 * (j & 1)),
+                                  ca + (j >> 1) * 4, cb + (j >> 1) * 4 + shift, (ks | (int) j) ? 1u : 0u);
+                    umma_commit(&S.empty[s]);
+                }
+                if (ok) umma_commit(&S.acc_full[buf]);
+            }
+            umma_commit(&S.done);
+            mbar_drain(&S.done, 0u);
+        }
+    } else if (warp >= 4 && warp < 4 + kFewQuant) {
+        // the rows past M keep what is there: their part of the accumulator is not stored
+        constexpr int UN = 4;
+        for (int r = warp - 4; r < M; r += kFewQuant) {
+            const TX * xr = x + r * ldx;
+            for (int s0 = 0; s0 < nks; s0 += UN) {
+                Eight<TX> v[UN];
+#pragma unroll
+                for (int u = 0; u < UN; ++u) v[u] = load8<TX, VEC>(xr, s0 + u < nks ? (s0 + u) * 256 + lane * 8 : K, K);
+#pragma unroll
+                for (int u = 0; u < UN; ++u) {
+                    const int seg = s0 + u;
+                    if (seg >= nks) break;
+                    unsigned sb;
+                    const unsigned q = quantize8(v[u], sb);
+                    // 128-byte swizzle: 16-byte piece c of row r at piece c ^ (r % 8)
+                    *reinterpret_cast<unsigned *>(a + (unsigned) (seg * kTM * 128 + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4)) = q;
+                    const unsigned word = scale_word(sb);
+                    if ((lane & 15) == 0)
+                        *reinterpret_cast<unsigned *>(sa + (unsigned) (seg * kScaleA + (lane >> 4) * 512 + (r & 31) * 16 + (r >> 5) * 4)) = word;
+                }
+            }
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&S.a_full);
+    } else if (warp >= 4 + kFewQuant && (warp & 3) == 0) {
+        // rows 0 to 31 are the tensor-memory lanes of the warps whose number is a multiple of four
+        const int half = (warp - 4 - kFewQuant) >> 2;
+        unsigned tile = 0;
+        for (int t = blockIdx.x; t < nt; t += gridDim.x, ++tile) {
+            const unsigned buf = tile & 1u;
+            if (!mbar_wait(&S.acc_full[buf], (tile >> 1) & 1u, kWaitNs, &S.err)) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            store_tile<TY, kFewN, false>(tmem + buf * kFewN, out + half * kOutBytes, half, lane, 0, M, t * kFewN, N, bias, y, ldy, nullptr);
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             if (lane == 0) mbar_arrive(&S.acc_empty[buf]);
         }
@@ -394,7 +630,7 @@ mx4_tc_kernel(const __grid_constant__ CUtensorMap amap, const unsigned char * __
     __syncthreads();
     if (warp == 2) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(512u) : "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(256u) : "memory");
     }
     if (threadIdx.x == 0 && S.err != 0) atomicExch_system(err_out, 1);
 }
@@ -468,29 +704,69 @@ namespace {
 
 constexpr int kBN[3] = {64, 128, 192};
 
-template <int BN>
-cudaError_t configure_tc() {
-    const int n = (int) tc_smem_bytes<BN>();
-    cudaError_t e = cudaFuncSetAttribute(mx4_tc_kernel<float, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, n);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(mx4_tc_kernel<__half, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, n);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(mx4_tc_kernel<__nv_bfloat16, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, n);
+// y as boxes of 32 rows and 128 bytes; false where TMA cannot store it: rows not 16-byte aligned, or
+// not whole 16 bytes long (a store then also writes what follows a row's last value, up to 16 bytes).
+bool map_y(CUtensorMap * map, void * y, int type, long long M, int N, long long ldy, cudaError_t & e) {
+    const int es = elem_size(type);
+    if (!aligned_to(y, 16) || ldy * es % 16 != 0 || (long long) N * es % 16 != 0) return false;
+    e = encode_2d_strided(map, type == PK_GGML_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                               : type == PK_GGML_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                          y, M, N, ldy * es, 32, 128 / es, CU_TENSOR_MAP_SWIZZLE_128B);
+    return true;
+}
+
+// Raises a kernel's limit of shared memory, once per device (`set`: the devices done).
+template <class F> cudaError_t allow_smem(F kernel, size_t bytes, int device, unsigned long long & set) {
+    if (__atomic_load_n(&set, __ATOMIC_RELAXED) >> device & 1) return cudaSuccess;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) bytes);
+    if (e == cudaSuccess) __atomic_fetch_or(&set, 1ull << device, __ATOMIC_RELAXED);
     return e;
 }
 
-template <int BN>
-cudaError_t launch_tc(const pk_mx4 * w, const CUtensorMap & amap, const unsigned char * xs, long long M, void * y, int type,
-                      long long ldy, const CUtensorMap & wmap, cudaStream_t s) {
-    const long long tiles = (M + kTM - 1) / kTM * ((w->N + BN - 1) / BN);
-    const unsigned g = (unsigned) std::min<long long>(tiles, 148);
+struct Call {
+    const pk_mx4 * w;
+    const void * x;
+    long long ldx, M;
+    void * y;
+    long long ldy;
+    cudaStream_t s;
+};
+
+template <class T, int BN, bool BOX>
+cudaError_t launch_tc_as(const Call & c, const CUtensorMap & amap, const unsigned char * xs, const CUtensorMap & wmap, const CUtensorMap & ymap) {
+    auto kernel = mx4_tc_kernel<T, BN, BOX>;
+    static unsigned long long set;
     const size_t smem = tc_smem_bytes<BN>();
-#define PK_T(T) \
-    mx4_tc_kernel<T, BN><<<g, kTThreads, smem, s>>>(amap, xs, M, w->K, wmap, w->scales, w->N, w->bias, static_cast<T *>(y), ldy, w->err_dev)
-    if (type == PK_GGML_F32) PK_T(float);
-    else if (type == PK_GGML_F16) PK_T(__half);
-    else PK_T(__nv_bfloat16);
-#undef PK_T
+    const cudaError_t e = allow_smem(kernel, smem, c.w->device, set);
+    if (e != cudaSuccess) return e;
+    const long long tiles = (c.M + kTM - 1) / kTM * ((c.w->N + BN - 1) / BN);
+    kernel<<<(unsigned) std::min<long long>(tiles, 148), kTThreads, smem, c.s>>>(
+        amap, xs, c.M, c.w->K, wmap, c.w->scales, c.w->N, c.w->bias, static_cast<T *>(c.y), c.ldy, ymap, c.w->err_dev);
     return cudaGetLastError();
 }
+
+template <class TX, class TY, bool VEC>
+cudaError_t launch_few_as(const Call & c) {
+    auto kernel = mx4_few_kernel<TX, TY, VEC>;
+    static unsigned long long set;
+    const cudaError_t e = allow_smem(kernel, few_smem(kFewK / 256), c.w->device, set);
+    if (e != cudaSuccess) return e;
+    const int grid = std::min((c.w->N + kFewN - 1) / kFewN, 148);
+    kernel<<<grid, kFewThreads, few_smem(c.w->chunks / 2), c.s>>>(static_cast<const TX *>(c.x), c.ldx, (int) c.M, c.w->K, c.w->map[0],
+                                                                  c.w->scales, c.w->N, c.w->bias, static_cast<TY *>(c.y), c.ldy, c.w->err_dev);
+    return cudaGetLastError();
+}
+
+template <class TX, class TY> cudaError_t launch_few_xy(const Call & c) {
+    return aligned_to(c.x, 16) && c.ldx * sizeof(TX) % 16 == 0 ? launch_few_as<TX, TY, true>(c) : launch_few_as<TX, TY, false>(c);
+}
+
+template <class TX> cudaError_t launch_few(const Call & c, int y_type) {
+    return y_type == PK_GGML_F32 ? launch_few_xy<TX, float>(c)
+           : y_type == PK_GGML_F16 ? launch_few_xy<TX, __half>(c) : launch_few_xy<TX, __nv_bfloat16>(c);
+}
+
+bool few(const pk_mx4 * w, int64_t rows) { return rows <= kFewRows && w->K <= kFewK; }
 
 // Tile width: fewest rounds of tiles over the SMs, a round costed by the rows that a tile loads.
 int pick_bn(long long M, int N) {
@@ -504,17 +780,19 @@ int pick_bn(long long M, int N) {
     return best;
 }
 
-cudaError_t launch_product(const pk_mx4 * w, const unsigned char * xc, const unsigned char * xs, long long M, void * y, int type,
-                           long long ldy, cudaStream_t s) {
-    alignas(64) CUtensorMap amap;
-    const cudaError_t e = encode_2d(&amap, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, xc, M, (long long) w->nb * 16, kTM, 128,
-                                    CU_TENSOR_MAP_SWIZZLE_128B);
+template <class T> cudaError_t launch_product(const Call & c, int y_type, const unsigned char * xc, const unsigned char * xs) {
+    alignas(64) CUtensorMap amap, ymap{};
+    cudaError_t e = encode_2d(&amap, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, xc, c.M, (long long) c.w->nb * 16, kTM, 128,
+                              CU_TENSOR_MAP_SWIZZLE_128B);
     if (e != cudaSuccess) return e;
-    switch (pick_bn(M, w->N)) {
-        case 0: return launch_tc<64>(w, amap, xs, M, y, type, ldy, w->map[0], s);
-        case 1: return launch_tc<128>(w, amap, xs, M, y, type, ldy, w->map[1], s);
-        default: return launch_tc<192>(w, amap, xs, M, y, type, ldy, w->map[2], s);
-    }
+    const bool box = map_y(&ymap, c.y, y_type, c.M, c.w->N, c.ldy, e);
+    if (e != cudaSuccess) return e;
+    const int i = pick_bn(c.M, c.w->N);
+    const CUtensorMap & wmap = c.w->map[i];
+    if (box) return i == 0 ? launch_tc_as<T, 64, true>(c, amap, xs, wmap, ymap)
+                    : i == 1 ? launch_tc_as<T, 128, true>(c, amap, xs, wmap, ymap) : launch_tc_as<T, 192, true>(c, amap, xs, wmap, ymap);
+    return i == 0 ? launch_tc_as<T, 64, false>(c, amap, xs, wmap, ymap)
+           : i == 1 ? launch_tc_as<T, 128, false>(c, amap, xs, wmap, ymap) : launch_tc_as<T, 192, false>(c, amap, xs, wmap, ymap);
 }
 
 }  // namespace
@@ -648,7 +926,7 @@ extern "C" PK_API pk_status pk_mx4_create(int device, const pk_tensor * weight, 
         e = launch_quantize<true>(src, type, N, (int) K, K, w->codes, w->scales, s);
     }
     if (e == cudaSuccess && bias) {
-        e = cudaMalloc(&w->bias, (size_t) N * 4);
+        e = cudaMalloc(&w->bias, (size_t) (N + 255) / 64 * 64 * 4);      // read in whole tiles
         if (e == cudaSuccess)
             e = cudaMemcpyAsync(w->bias, bias, (size_t) N * 4, on_device ? cudaMemcpyDeviceToDevice : cudaMemcpyHostToDevice, s);
     }
@@ -657,9 +935,6 @@ extern "C" PK_API pk_status pk_mx4_create(int device, const pk_tensor * weight, 
     for (int i = 0; i < 3 && e == cudaSuccess; ++i)
         e = encode_2d(&w->map[i], CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, w->codes, N, (long long) w->nb * 16, kBN[i], 128,
                       CU_TENSOR_MAP_SWIZZLE_128B);
-    if (e == cudaSuccess) e = configure_tc<64>();
-    if (e == cudaSuccess) e = configure_tc<128>();
-    if (e == cudaSuccess) e = configure_tc<192>();
     if (s) {
         const cudaError_t e2 = cudaStreamSynchronize(s);
         if (e == cudaSuccess) e = e2;
@@ -697,11 +972,12 @@ extern "C" PK_API pk_status pk_mx4_linear(pk_mx4 * w, const void * x, int32_t x_
     if (x_stride < w->K || y_stride < w->N || x_stride > (INT64_MAX >> 34) || y_stride > (INT64_MAX >> 34))
         return op_fail(PK_ERR_INVALID, fn, "x_stride must be at least K and y_stride at least N");
     if (rows == 0) return PK_OK;
-    if (!x || !y || !workspace) return op_fail(PK_ERR_INVALID, fn, "null pointer");
+    const int64_t need = pk_mx4_workspace(w, rows);
+    if (!x || !y || (need > 0 && !workspace)) return op_fail(PK_ERR_INVALID, fn, "null pointer");
     if (!aligned_to(x, (size_t) elem_size(x_type)) || !aligned_to(y, (size_t) elem_size(y_type)))
         return op_fail(PK_ERR_INVALID, fn, "x and y must be aligned to their element");
     if (!aligned_to(workspace, 256)) return op_fail(PK_ERR_INVALID, fn, "workspace must be 256-byte aligned");
-    if (workspace_bytes < pk_mx4_workspace(w, rows))
+    if (workspace_bytes < need)
         return op_fail(PK_ERR_INVALID, fn, "workspace_bytes is below pk_mx4_workspace(w, rows)");
     if (mx4_take_timeout(w)) return op_fail(PK_ERR_TIMEOUT, fn, "a device-side wait of an earlier call ran out");
     DeviceScope dev(w->device);
@@ -709,7 +985,16 @@ extern "C" PK_API pk_status pk_mx4_linear(pk_mx4 * w, const void * x, int32_t x_
     cudaStream_t s = (cudaStream_t) stream;
     unsigned char * xc = static_cast<unsigned char *>(workspace);
     unsigned char * xs = xc + ws_codes(w, rows);
-    cudaError_t e = launch_quantize<true>(x, x_type, rows, w->K, x_stride, xc, xs, s);
-    if (e == cudaSuccess) e = launch_product(w, xc, xs, rows, y, y_type, y_stride, s);
+    const Call c{w, x, x_stride, rows, y, y_stride, s};
+    cudaError_t e;
+    if (few(w, rows)) {
+        e = x_type == PK_GGML_F32 ? launch_few<float>(c, y_type)
+            : x_type == PK_GGML_F16 ? launch_few<__half>(c, y_type) : launch_few<__nv_bfloat16>(c, y_type);
+    } else {
+        e = launch_quantize<true>(x, x_type, rows, w->K, x_stride, xc, xs, s);
+        if (e == cudaSuccess)
+            e = y_type == PK_GGML_F32 ? launch_product<float>(c, y_type, xc, xs)
+                : y_type == PK_GGML_F16 ? launch_product<__half>(c, y_type, xc, xs) : launch_product<__nv_bfloat16>(c, y_type, xc, xs);
+    }
     return e == cudaSuccess ? PK_OK : op_cuda_fail(e, fn);
 }

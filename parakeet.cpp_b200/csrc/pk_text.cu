@@ -352,7 +352,7 @@ pk_status ctc_frame_tokens(pk_ctc * c, const char * fn, pk_mx4 * head, const flo
     if (head) {
         const int64_t ws = pk_mx4_workspace(head, step);
         TX_CK(c->logits.ensure((size_t) step * c->V * 4), fn);
-        TX_CK(c->work.ensure((size_t) ws), fn);
+        TX_CK(c->work.ensure((size_t) std::max<int64_t>(ws, 1)), fn);
     }
     for (int64_t f = 0; f < frames; f += step) {
         const int64_t n = std::min(step, frames - f);
