@@ -244,19 +244,47 @@ __global__ void __launch_bounds__(kQThreads) mx4_repack_kernel(const unsigned ch
 // tensor memory and issues its four products, warps 4-11 empty the accumulator, of which there are
 // two, so that a tile's epilogue runs under the next tile's products. Each stage has tensor-memory
 // columns of its own for its scales: they are free when the stage is.
+constexpr long long kWaitNs = 2000000000LL;             // bound on every device-side wait
 constexpr int kTM = 128;
 constexpr int kTStages = 4;
 constexpr int kTThreads = 384;
 constexpr int kTEpi = 8;                                // warps of the epilogue: two for each 32 rows
 constexpr unsigned kScaleA = 1024, kScaleB = 2048;      // two atoms of A rows; two of each of two of B's
 constexpr unsigned kScaleCols = 24;                     // tensor-memory columns of a stage's scales: 8 + 16
-constexpr long long kWaitNs = 2000000000LL;             // bound on every device-side wait
 
 struct TcSmem {
     unsigned long long full[kTStages], empty[kTStages], acc_full[2], acc_empty[2], done;
     unsigned tmem;
     int err;
 };
+
+// The wait of a whole warp, of one mind about its outcome.
+template <bool CLUSTER = false>
+__device__ __forceinline__ bool warp_wait(unsigned long long * b, unsigned parity, int * err) {
+    return __all_sync(0xFFFFFFFFu, mbar_wait<CLUSTER>(b, parity, kWaitNs, err));
+}
+
+// The four products of a stage of 256 values and the copies of their scales (columns ca: 8 for x, then
+// NA per chunk for the weights), by one elected lane. The whole warp runs the loop around it, so that
+// addresses and descriptors stay in uniform registers: with one lane in the loop a stage took as long
+// to issue as 2.5 stages take to multiply.
+template <int BN, bool PAIR>
+__device__ __forceinline__ void issue_stage(unsigned d, unsigned a, unsigned b, unsigned sa, unsigned sb, unsigned ca, unsigned shift,
+                                            bool fresh) {
+    constexpr unsigned NA = BN > 128 ? 8 : 4;
+    const unsigned cb = ca + 8;
+    const unsigned long long da = umma_desc_sw128(a), db = umma_desc_sw128(b), dsa = scale_desc(sa), dsb = scale_desc(sb);
+#pragma unroll
+    for (unsigned c = 0; c < 2; ++c) {                    // an atom of 512 bytes is 32 in a descriptor's units
+        umma_copy_scales<PAIR>(ca + c * 4, dsa + c * 32);
+        umma_copy_scales<PAIR>(cb + c * NA, dsb + c * 32);
+        if (BN > 128) umma_copy_scales<PAIR>(cb + c * NA + 4, dsb + 64 + c * 32);
+    }
+#pragma unroll
+    for (unsigned j = 0; j < 4; ++j)                      // 32 bytes along the swizzled rows
+        umma_mxf4<PAIR>(d, da + 2 * j, db + 2 * j, umma_idesc_mxf4(PAIR ? 2 * kTM : kTM, BN, 2 * (j & 1)), ca + (j >> 1) * 4,
+                        cb + (j >> 1) * NA + shift, j > 0 || !fresh ? 1u : 0u);
+}
 
 template <int BN> constexpr unsigned tc_stage_bytes() { return kTM * 128u + BN * 128u + kScaleA + kScaleB; }
 constexpr unsigned kOutBytes = 4096;                    // an epilogue warp's 32 staged rows of 128 bytes
@@ -363,7 +391,7 @@ mx4_tc_kernel(const __grid_constant__ CUtensorMap amap, const unsigned char * __
     unsigned char * ring = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t) 1023);
     unsigned char * out = reinterpret_cast<unsigned char *>(ring + kTStages * tc_stage_bytes<BN>());
     TcSmem & S = *reinterpret_cast<TcSmem *>(out + kTEpi * kOutBytes);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xFFFFFFFFu, (int) threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const int chunks = scale_chunks(K), nks = chunks / 2, atoms = (N + 127) / 128;
     const int nt = (N + BN - 1) / BN;
     const long long tiles = ((M + kTM - 1) / kTM) * nt;
@@ -389,7 +417,7 @@ mx4_tc_kernel(const __grid_constant__ CUtensorMap amap, const unsigned char * __
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    const unsigned tmem = S.tmem;
+    const unsigned tmem = __shfl_sync(0xFFFFFFFFu, S.tmem, 0);
 
     if (warp == 0) {
         if (lane == 0) {
@@ -416,38 +444,27 @@ mx4_tc_kernel(const __grid_constant__ CUtensorMap amap, const unsigned char * __
             for (unsigned j = it > kTStages ? it - kTStages : 0; j < it; ++j) mbar_drain(&S.full[j % kTStages], (j / kTStages) & 1u);
         }
     } else if (warp == 1) {
-        if (lane == 0) {
-            unsigned it = 0, tile = 0;
-            bool ok = true;
-            for (long long t = blockIdx.x; t < tiles && ok; t += gridDim.x, ++tile) {
-                const int n0 = (int) (t % nt) * BN;
-                const unsigned buf = tile & 1u, d = tmem + buf * BN;
-                const unsigned shift = (unsigned) (n0 & 127) >> 5;
-                if (!mbar_wait(&S.acc_empty[buf], ((tile >> 1) & 1u) ^ 1u, kWaitNs, &S.err)) break;
+        unsigned tile = 0, s = 0, ph = 0;
+        bool ok = true;
+        for (long long t = blockIdx.x; t < tiles && ok; t += gridDim.x, ++tile) {
+            const unsigned buf = tile & 1u, shift = (unsigned) ((int) (t % nt) * BN & 127) >> 5;
+            if (!warp_wait(&S.acc_empty[buf], ((tile >> 1) & 1u) ^ 1u, &S.err)) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            for (int ks = 0; ks < nks; ++ks) {
+                if (!warp_wait(&S.full[s], ph, &S.err)) { ok = false; break; }
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                for (int ks = 0; ks < nks; ++ks, ++it) {
-                    const int s = (int) (it % kTStages);
-                    if (!mbar_wait(&S.full[s], (it / kTStages) & 1u, kWaitNs, &S.err)) { ok = false; break; }
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const unsigned a = smem_u32(ring + s * tc_stage_bytes<BN>()), b = a + kTM * 128u, sa = b + BN * 128u;
-                    const unsigned ca = tmem + 2 * 192 + (unsigned) s * kScaleCols, cb = ca + 8;
-#pragma unroll
-                    for (unsigned c = 0; c < 2; ++c) {
-                        umma_copy_scales(ca + c * 4, sa + c * 512);
-                        umma_copy_scales(cb + c * 8, sa + kScaleA + c * 512);
-                        if (BN > 128) umma_copy_scales(cb + c * 8 + 4, sa + kScaleA + 1024 + c * 512);
-                    }
-#pragma unroll
-                    for (unsigned j = 0; j < 4; ++j)
-                        umma_mxf4(d, umma_desc_sw128(a + j * 32), umma_desc_sw128(b + j * 32), umma_idesc_mxf4(kTM, BN, 2 * (j & 1)),
-                                  ca + (j >> 1) * 4, cb + (j >> 1) * 8 + shift, (ks | (int) j) ? 1u : 0u);
+                const unsigned a = smem_u32(ring) + s * tc_stage_bytes<BN>(), b = a + kTM * 128u, sa = b + BN * 128u;
+                if (elect_one()) {
+                    issue_stage<BN, false>(tmem + buf * BN, a, b, sa, sa + kScaleA, tmem + 2 * 192 + s * kScaleCols, shift, ks == 0);
                     umma_commit(&S.empty[s]);
+                    if (ks == nks - 1) umma_commit(&S.acc_full[buf]);
                 }
-                if (ok) umma_commit(&S.acc_full[buf]);
+                __syncwarp();
+                if (++s == kTStages) { s = 0; ph ^= 1u; }
             }
-            umma_commit(&S.done);                        // no product in flight either
-            mbar_drain(&S.done, 0u);
         }
+        if (elect_one()) umma_commit(&S.done);           // no product in flight either
+        mbar_drain(&S.done, 0u);
     } else if (warp >= 4) {
         const int q = warp & 3;                          // this warp's tensor-memory lanes: rows 32 q ..
         const int half = (warp - 4) >> 2;                // its columns: every other 32
@@ -457,7 +474,7 @@ mx4_tc_kernel(const __grid_constant__ CUtensorMap amap, const unsigned char * __
             const long long m0 = (t / nt) * kTM + q * 32;
             const int n0 = (int) (t % nt) * BN;
             const unsigned buf = tile & 1u;
-            if (!mbar_wait(&S.acc_full[buf], (tile >> 1) & 1u, kWaitNs, &S.err)) break;
+            if (!warp_wait(&S.acc_full[buf], (tile >> 1) & 1u, &S.err)) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const int rows = (int) max(0LL, min(32LL, M - m0));
             store_tile<T, BN, BOX>(tmem + buf * BN + ((unsigned) (q * 32) << 16), st, half, lane, m0, rows, n0, N, bias, y, ldy, &ymap);
@@ -471,6 +488,148 @@ mx4_tc_kernel(const __grid_constant__ CUtensorMap amap, const unsigned char * __
     if (warp == 2) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(512u) : "memory");
+    }
+    if (threadIdx.x == 0 && S.err != 0) atomicExch_system(err_out, 1);
+}
+
+// ---- many rows: pairs of blocks ---------------------------------------------------
+//
+// The tiles above read 44 KB for every 128 x 192 x 256 products, which the L2 gives an SM in twice the
+// time that the products take. Two blocks of a cluster together take 256 rows (cta_group::2): each holds
+// its 128 rows' codes and half of the tile's weights, and the products read the other half from the
+// other SM, so a stage is 31 KB. The pair's first block issues, and both blocks' loads arrive on its
+// barrier. The scales of all BN weight rows are loaded by both, each for its own tensor memory.
+constexpr int kPStages = 5;
+template <int BN> constexpr unsigned pair_stage() { return kTM * 128u + BN / 2 * 128u + kScaleA + kScaleB; }
+// bytes that one block loads a stage
+template <int BN> constexpr unsigned pair_bytes() { return kTM * 128u + BN / 2 * 128u + kScaleA + (BN > 128 ? 2048u : 1024u); }
+struct PairSmem {
+    unsigned long long full[kPStages], empty[kPStages], acc_full[2], acc_empty[2], done;
+    unsigned tmem;
+    int err;
+};
+template <int BN> constexpr size_t pair_smem() {
+    return 1024 + (size_t) kPStages * pair_stage<BN>() + kTEpi * kOutBytes + sizeof(PairSmem);
+}
+
+__device__ __forceinline__ void cluster_meet() {
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+template <class T, int BN, bool BOX>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTThreads, 1)
+mx4_pair_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap asmap, long long M, int K,
+                const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap wsmap, int N,
+                const float * __restrict__ bias, T * __restrict__ y, long long ldy, const __grid_constant__ CUtensorMap ymap, int * err_out) {
+    extern __shared__ __align__(1024) unsigned char raw[];
+    unsigned char * ring = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t) 1023);
+    unsigned char * out = ring + kPStages * pair_stage<BN>();
+    PairSmem & S = *reinterpret_cast<PairSmem *>(out + kTEpi * kOutBytes);
+    const int warp = __shfl_sync(0xFFFFFFFFu, (int) threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+    const unsigned rank = blockIdx.x & 1u;
+    const int nks = scale_chunks(K) / 2, nt = (N + BN - 1) / BN;
+    const long long tiles = ((M + 2 * kTM - 1) / (2 * kTM)) * nt, first = blockIdx.x >> 1, step = gridDim.x >> 1;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kPStages; ++s) {
+            mbar_init(&S.full[s], 1);                     // used in the first block
+            mbar_init(&S.empty[s], 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(&S.acc_full[b], 1);
+            mbar_init(&S.acc_empty[b], 2 * kTEpi);
+        }
+        mbar_init(&S.done, 1);
+        S.err = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 2) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;"
+                     :: "r"(smem_u32(&S.tmem)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    cluster_meet();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const unsigned tmem = __shfl_sync(0xFFFFFFFFu, S.tmem, 0);
+
+    if (warp == 0) {
+        if (lane == 0) {
+            unsigned it = 0;
+            bool ok = true;
+            for (long long t = first; t < tiles && ok; t += step) {
+                const int m = (int) (t / nt) * 2 + (int) rank, n0 = (int) (t % nt) * BN;
+                for (int ks = 0; ks < nks; ++ks, ++it) {
+                    const int s = (int) (it % kPStages);
+                    if (!mbar_wait(&S.empty[s], ((it / kPStages) & 1u) ^ 1u, kWaitNs, &S.err)) { ok = false; break; }
+                    unsigned char * a = ring + s * pair_stage<BN>(), * b = a + kTM * 128, * sa = b + BN / 2 * 128;
+                    // rows past M or N, and their scales, read as zeros
+                    const unsigned bar = mbar_at(&S.full[s], 0);
+                    if (rank == 0) mbar_expect(&S.full[s], 2u * pair_bytes<BN>());
+                    tma_load_2d_pair(a, &amap, ks * 128, m * kTM, bar);
+                    tma_load_2d_pair(b, &wmap, ks * 128, n0 + (int) rank * (BN / 2), bar);
+                    tma_load_2d_pair(sa, &asmap, ks * 256, m, bar);
+                    tma_load_2d_pair(sa + kScaleA, &wsmap, ks * 256, n0 >> 7, bar);
+                }
+            }
+            // nothing in flight when the blocks end, however the others ended
+            if (rank == 0)
+                for (unsigned j = it > kPStages ? it - kPStages : 0; j < it; ++j) mbar_drain(&S.full[j % kPStages], (j / kPStages) & 1u);
+            else if (!ok)
+                for (int j = 0; j < 200; ++j) __nanosleep(1000);
+        }
+    } else if (warp == 1) {
+        if (rank == 0) {
+            unsigned tile = 0, s = 0, ph = 0;
+            bool ok = true;
+            for (long long t = first; t < tiles && ok; t += step, ++tile) {
+                const unsigned buf = tile & 1u, shift = (unsigned) ((int) (t % nt) * BN & 127) >> 5;
+                if (!warp_wait<true>(&S.acc_empty[buf], ((tile >> 1) & 1u) ^ 1u, &S.err)) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                for (int ks = 0; ks < nks; ++ks) {
+                    if (!warp_wait<true>(&S.full[s], ph, &S.err)) { ok = false; break; }
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const unsigned a = smem_u32(ring) + s * pair_stage<BN>(), b = a + kTM * 128u, sa = b + BN / 2 * 128u;
+                    if (elect_one()) {
+                        issue_stage<BN, true>(tmem + buf * BN, a, b, sa, sa + kScaleA, tmem + 2 * 192 + s * kScaleCols, shift, ks == 0);
+                        umma_commit_pair(&S.empty[s]);
+                        if (ks == nks - 1) umma_commit_pair(&S.acc_full[buf]);
+                    }
+                    __syncwarp();
+                    if (++s == kPStages) { s = 0; ph ^= 1u; }
+                }
+            }
+            // no product in flight either
+            if (elect_one()) umma_commit_pair(&S.done);
+            mbar_drain(&S.done, 0u);
+        } else {
+            mbar_drain(&S.done, 0u);                      // the products read this block's memory until then
+        }
+    } else if (warp >= 4) {
+        const int q = warp & 3, half = (warp - 4) >> 2;
+        unsigned char * st = out + (warp - 4) * kOutBytes;
+        unsigned tile = 0;
+        for (long long t = first; t < tiles; t += step, ++tile) {
+            const long long m0 = ((t / nt) * 2 + rank) * kTM + q * 32;
+            const int n0 = (int) (t % nt) * BN;
+            const unsigned buf = tile & 1u;
+            if (!warp_wait(&S.acc_full[buf], (tile >> 1) & 1u, &S.err)) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const int rows = (int) max(0LL, min(32LL, M - m0));
+            store_tile<T, BN, BOX>(tmem + buf * BN + ((unsigned) (q * 32) << 16), st, half, lane, m0, rows, n0, N, bias, y, ldy, &ymap);
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            if (lane == 0) mbar_arrive_at(&S.acc_empty[buf], 0);
+        }
+        if (BOX && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    cluster_meet();                                       // the other's memory and barriers are used no more
+    if (warp == 2) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(512u) : "memory");
     }
     if (threadIdx.x == 0 && S.err != 0) atomicExch_system(err_out, 1);
 }
@@ -512,7 +671,7 @@ mx4_few_kernel(const TX * __restrict__ x, long long ldx, int M, int K, const __g
     unsigned char * ring = sa + nks * kScaleA;
     unsigned char * out = ring + kFewStages * kFewStage;
     FewSmem & S = *reinterpret_cast<FewSmem *>(out + 2 * kOutBytes);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xFFFFFFFFu, (int) threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < kFewStages; ++s) {
@@ -536,7 +695,7 @@ mx4_few_kernel(const TX * __restrict__ x, long long ldx, int M, int K, const __g
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    const unsigned tmem = S.tmem;
+    const unsigned tmem = __shfl_sync(0xFFFFFFFFu, S.tmem, 0);
 
     if (warp == 0) {
         if (lane == 0) {
@@ -557,36 +716,28 @@ mx4_few_kernel(const TX * __restrict__ x, long long ldx, int M, int K, const __g
             for (unsigned j = it > kFewStages ? it - kFewStages : 0; j < it; ++j) mbar_drain(&S.full[j % kFewStages], (j / kFewStages) & 1u);
         }
     } else if (warp == 1) {
-        if (lane == 0) {
-            unsigned it = 0, tile = 0;
-            bool ok = mbar_wait(&S.a_full, 0u, kWaitNs, &S.err);
-            for (int t = blockIdx.x; t < nt && ok; t += gridDim.x, ++tile) {
-                const unsigned buf = tile & 1u, d = tmem + buf * kFewN, shift = (unsigned) ((t * kFewN) & 127) >> 5;
-                if (!mbar_wait(&S.acc_empty[buf], ((tile >> 1) & 1u) ^ 1u, kWaitNs, &S.err)) break;
+        unsigned tile = 0, s = 0, ph = 0;
+        bool ok = warp_wait(&S.a_full, 0u, &S.err);
+        for (int t = blockIdx.x; t < nt && ok; t += gridDim.x, ++tile) {
+            const unsigned buf = tile & 1u, shift = (unsigned) ((t * kFewN) & 127) >> 5;
+            if (!warp_wait(&S.acc_empty[buf], ((tile >> 1) & 1u) ^ 1u, &S.err)) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            for (int ks = 0; ks < nks; ++ks) {
+                if (!warp_wait(&S.full[s], ph, &S.err)) { ok = false; break; }
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                for (int ks = 0; ks < nks; ++ks, ++it) {
-                    const int s = (int) (it % kFewStages);
-                    if (!mbar_wait(&S.full[s], (it / kFewStages) & 1u, kWaitNs, &S.err)) { ok = false; break; }
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const unsigned ka = smem_u32(a) + (unsigned) ks * kTM * 128u, ksa = smem_u32(sa) + (unsigned) ks * kScaleA;
-                    const unsigned kb = smem_u32(ring + s * kFewStage), ksb = kb + kFewN * 128u;
-                    const unsigned ca = tmem + 2 * kFewN + (unsigned) s * 16u, cb = ca + 8;
-#pragma unroll
-                    for (unsigned c = 0; c < 2; ++c) {
-                        umma_copy_scales(ca + c * 4, ksa + c * 512);
-                        umma_copy_scales(cb + c * 4, ksb + c * 512);
-                    }
-#pragma unroll
-                    for (unsigned j = 0; j < 4; ++j)
-                        umma_mxf4(d, umma_desc_sw128(ka + j * 32), umma_desc_sw128(kb + j * 32), umma_idesc_mxf4(kTM, kFewN, 2 * (j & 1)),
-                                  ca + (j >> 1) * 4, cb + (j >> 1) * 4 + shift, (ks | (int) j) ? 1u : 0u);
+                const unsigned kb = smem_u32(ring) + s * kFewStage;
+                if (elect_one()) {
+                    issue_stage<kFewN, false>(tmem + buf * kFewN, smem_u32(a) + (unsigned) ks * kTM * 128u, kb,
+                                              smem_u32(sa) + (unsigned) ks * kScaleA, kb + kFewN * 128u, tmem + 2 * kFewN + s * 16u, shift, ks == 0);
                     umma_commit(&S.empty[s]);
+                    if (ks == nks - 1) umma_commit(&S.acc_full[buf]);
                 }
-                if (ok) umma_commit(&S.acc_full[buf]);
+                __syncwarp();
+                if (++s == kFewStages) { s = 0; ph ^= 1u; }
             }
-            umma_commit(&S.done);
-            mbar_drain(&S.done, 0u);
         }
+        if (elect_one()) umma_commit(&S.done);
+        mbar_drain(&S.done, 0u);
     } else if (warp >= 4 && warp < 4 + kFewQuant) {
         // the rows past M keep what is there: their part of the accumulator is not stored
         constexpr int UN = 4;
@@ -619,7 +770,7 @@ mx4_few_kernel(const TX * __restrict__ x, long long ldx, int M, int K, const __g
         unsigned tile = 0;
         for (int t = blockIdx.x; t < nt; t += gridDim.x, ++tile) {
             const unsigned buf = tile & 1u;
-            if (!mbar_wait(&S.acc_full[buf], (tile >> 1) & 1u, kWaitNs, &S.err)) break;
+            if (!warp_wait(&S.acc_full[buf], (tile >> 1) & 1u, &S.err)) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             store_tile<TY, kFewN, false>(tmem + buf * kFewN, out + half * kOutBytes, half, lane, 0, M, t * kFewN, N, bias, y, ldy, nullptr);
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -696,13 +847,21 @@ struct pk_mx4 {
     float * bias = nullptr;
     int * err = nullptr;                // host memory that the device sees: a bounded wait ran out
     int * err_dev = nullptr;
-    alignas(64) CUtensorMap map[3];     // codes in boxes of kBN[i] rows
+    alignas(64) CUtensorMap map[4];     // codes in boxes of kBox[i] rows
+    alignas(64) CUtensorMap smap[2];    // scales: the two atoms of a stage of 128 rows, of 256 rows
 };
 
 namespace pk {
 namespace {
 
 constexpr int kBN[3] = {64, 128, 192};
+constexpr int kBox[4] = {64, 128, 192, 96};   // the last: half of a pair's 192
+
+// Scale atoms as rows of words, one row for 128 rows of values; a box is a stage's two atoms of `rows`
+// such rows.
+cudaError_t map_scales(CUtensorMap * map, const unsigned char * scales, long long atom_rows, int chunks, int rows) {
+    return encode_2d(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 4, scales, atom_rows, (long long) chunks * 128, rows, 256, CU_TENSOR_MAP_SWIZZLE_NONE);
+}
 
 // y as boxes of 32 rows and 128 bytes; false where TMA cannot store it: rows not 16-byte aligned, or
 // not whole 16 bytes long (a store then also writes what follows a row's last value, up to 16 bytes).
@@ -742,6 +901,22 @@ cudaError_t launch_tc_as(const Call & c, const CUtensorMap & amap, const unsigne
     const long long tiles = (c.M + kTM - 1) / kTM * ((c.w->N + BN - 1) / BN);
     kernel<<<(unsigned) std::min<long long>(tiles, 148), kTThreads, smem, c.s>>>(
         amap, xs, c.M, c.w->K, wmap, c.w->scales, c.w->N, c.w->bias, static_cast<T *>(c.y), c.ldy, ymap, c.w->err_dev);
+    return cudaGetLastError();
+}
+
+template <class T, int BN, bool BOX>
+cudaError_t launch_pair_as(const Call & c, const CUtensorMap & amap, const unsigned char * xs, const CUtensorMap & ymap) {
+    alignas(64) CUtensorMap asmap;
+    cudaError_t e = map_scales(&asmap, xs, (c.M + kTM - 1) / kTM, c.w->chunks, 1);
+    if (e != cudaSuccess) return e;
+    auto kernel = mx4_pair_kernel<T, BN, BOX>;
+    static unsigned long long set;
+    const size_t smem = pair_smem<BN>();
+    e = allow_smem(kernel, smem, c.w->device, set);
+    if (e != cudaSuccess) return e;
+    const long long tiles = (c.M + 2 * kTM - 1) / (2 * kTM) * ((c.w->N + BN - 1) / BN);
+    kernel<<<(unsigned) (2 * std::min<long long>(tiles, 74)), kTThreads, smem, c.s>>>(
+        amap, asmap, c.M, c.w->K, c.w->map[BN > 128 ? 3 : 0], c.w->smap[BN > 128 ? 1 : 0], c.w->N, c.w->bias, static_cast<T *>(c.y), c.ldy, ymap, c.w->err_dev);
     return cudaGetLastError();
 }
 
@@ -787,6 +962,13 @@ template <class T> cudaError_t launch_product(const Call & c, int y_type, const 
     if (e != cudaSuccess) return e;
     const bool box = map_y(&ymap, c.y, y_type, c.M, c.w->N, c.ldy, e);
     if (e != cudaSuccess) return e;
+    // pairs where there are tiles for all of them
+    if ((c.M + 2 * kTM - 1) / (2 * kTM) * ((c.w->N + 127) / 128) >= 74) {
+        const long long mp = (c.M + 2 * kTM - 1) / (2 * kTM);
+        const long long r128 = (mp * ((c.w->N + 127) / 128) + 73) / 74 * (kTM + 64), r192 = (mp * ((c.w->N + 191) / 192) + 73) / 74 * (kTM + 96);
+        if (r192 <= r128) return box ? launch_pair_as<T, 192, true>(c, amap, xs, ymap) : launch_pair_as<T, 192, false>(c, amap, xs, ymap);
+        return box ? launch_pair_as<T, 128, true>(c, amap, xs, ymap) : launch_pair_as<T, 128, false>(c, amap, xs, ymap);
+    }
     const int i = pick_bn(c.M, c.w->N);
     const CUtensorMap & wmap = c.w->map[i];
     if (box) return i == 0 ? launch_tc_as<T, 64, true>(c, amap, xs, wmap, ymap)
@@ -932,9 +1114,10 @@ extern "C" PK_API pk_status pk_mx4_create(int device, const pk_tensor * weight, 
     }
     if (e == cudaSuccess) w->err = take_error_word(e);
     if (e == cudaSuccess) e = cudaHostGetDevicePointer(reinterpret_cast<void **>(&w->err_dev), w->err, 0);
-    for (int i = 0; i < 3 && e == cudaSuccess; ++i)
-        e = encode_2d(&w->map[i], CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, w->codes, N, (long long) w->nb * 16, kBN[i], 128,
+    for (int i = 0; i < 4 && e == cudaSuccess; ++i)
+        e = encode_2d(&w->map[i], CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, w->codes, N, (long long) w->nb * 16, kBox[i], 128,
                       CU_TENSOR_MAP_SWIZZLE_128B);
+    for (int i = 0; i < 2 && e == cudaSuccess; ++i) e = map_scales(&w->smap[i], w->scales, (N + 127) / 128, w->chunks, i + 1);
     if (s) {
         const cudaError_t e2 = cudaStreamSynchronize(s);
         if (e == cudaSuccess) e = e2;

@@ -25,11 +25,20 @@ __device__ __forceinline__ bool mbar_test(unsigned long long * b, unsigned parit
     return done != 0;
 }
 
+// The same, acquiring at cluster scope what the other block's threads released.
+__device__ __forceinline__ bool mbar_test_cluster(unsigned long long * b, unsigned parity) {
+    unsigned done;
+    asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
+                 : "=r"(done) : "r"(smem_u32(b)), "r"(parity) : "memory");
+    return done != 0;
+}
+
 // Bounded wait on one phase of an mbarrier; false (and *err set) on timeout.
+template <bool CLUSTER = false>
 __device__ __forceinline__ bool mbar_wait(unsigned long long * b, unsigned parity, long long timeout_ns, int * err) {
     unsigned long long t0 = 0;
     for (unsigned it = 0;; ++it) {
-        if (mbar_test(b, parity)) return true;
+        if (CLUSTER ? mbar_test_cluster(b, parity) : mbar_test(b, parity)) return true;
         if (*reinterpret_cast<volatile int *>(err) != 0) return false;
         if ((it & 255u) == 0u) {
             unsigned long long now;
@@ -101,22 +110,56 @@ __host__ __device__ constexpr unsigned umma_idesc_mxf4(int m, int n, int id) {
 }
 
 // One block-scaled product of 64 values of K (32 bytes of each operand row); sfa, sfb: tensor-memory
-// addresses of the rows' scale words (row r in lane r % 32, column r / 32).
+// addresses of the rows' scale words (row r in lane r % 32, column r / 32). PAIR: over a pair of blocks
+// (M = 256), issued by the pair's first block, each block's operand and scale rows at the same places
+// of its own shared and tensor memory.
+template <bool PAIR>
 __device__ __forceinline__ void umma_mxf4(unsigned tmem_d, unsigned long long adesc, unsigned long long bdesc, unsigned idesc,
                                           unsigned sfa, unsigned sfb, unsigned accumulate) {
-    asm volatile("{ .reg .pred p; setp.ne.b32 p, %6, 0;\n"
-                 "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p; }"
-                 :: "r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate) : "memory");
+    if (PAIR)
+        asm volatile("{ .reg .pred p; setp.ne.b32 p, %6, 0;\n"
+                     "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p; }"
+                     :: "r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate) : "memory");
+    else
+        asm volatile("{ .reg .pred p; setp.ne.b32 p, %6, 0;\n"
+                     "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p; }"
+                     :: "r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate) : "memory");
 }
 
 // 512 bytes of scale words (32 rows of 16 bytes) from shared memory to four tensor-memory columns,
 // the same for each of the four lane quarters. Ordered before products that the same thread issues.
-__device__ __forceinline__ void umma_copy_scales(unsigned tmem, unsigned saddr) {
-    unsigned long long d = 0;
-    d |= (unsigned long long) ((saddr >> 4) & 0x3FFFu);          // start address
-    d |= (unsigned long long) (128u >> 4) << 32;                  // stride byte offset: next 8 rows of 16 bytes
-    d |= (unsigned long long) 1u << 46;                           // descriptor version (tcgen05); no swizzle
-    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" :: "r"(tmem), "l"(d) : "memory");
+template <bool PAIR>
+__device__ __forceinline__ void umma_copy_scales(unsigned tmem, unsigned long long desc) {
+    if (PAIR) asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" :: "r"(tmem), "l"(desc) : "memory");
+    else asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" :: "r"(tmem), "l"(desc) : "memory");
+}
+// Their descriptor: no swizzle, the next 8 rows of 16 bytes 128 bytes on.
+__device__ __forceinline__ unsigned long long scale_desc(unsigned saddr) {
+    return (unsigned long long) ((saddr >> 4) & 0x3FFFu) | (unsigned long long) (128u >> 4) << 32 | (unsigned long long) 1u << 46;
+}
+
+// One lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+    unsigned p;
+    asm volatile("{ .reg .pred q; elect.sync _|q, 0xFFFFFFFF; selp.u32 %0, 1, 0, q; }" : "=r"(p));
+    return p != 0;
+}
+
+// Arrives on the barrier at this place of both blocks once the pair's products so far are done.
+__device__ __forceinline__ void umma_commit_pair(unsigned long long * b) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+                 :: "r"(smem_u32(b)), "h"((unsigned short) 3) : "memory");
+}
+
+// Address in the cluster's window of what lies at this place of its block `rank`.
+__device__ __forceinline__ unsigned mbar_at(unsigned long long * b, unsigned rank) {
+    unsigned r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(b)), "r"(rank));
+    return r;
+}
+// Arrives there, releasing at cluster scope.
+__device__ __forceinline__ void mbar_arrive_at(unsigned long long * b, unsigned rank) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" :: "r"(mbar_at(b, rank)) : "memory");
 }
 
 __device__ __forceinline__ void umma_commit(unsigned long long * b) {
@@ -127,6 +170,13 @@ __device__ __forceinline__ void umma_commit(unsigned long long * b) {
 __device__ __forceinline__ void tma_load_2d(void * dst, const CUtensorMap * map, int x, int y, unsigned long long * bar) {
     asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
                  :: "r"(smem_u32(dst)), "l"(map), "r"(x), "r"(y), "r"(smem_u32(bar)) : "memory");
+}
+
+// The same for a block of a pair: the bytes arrive on a barrier of either block (`bar`: its address in
+// the cluster's window, see mbar_at).
+__device__ __forceinline__ void tma_load_2d_pair(void * dst, const CUtensorMap * map, int x, int y, unsigned bar) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3}], [%4];"
+                 :: "r"(smem_u32(dst)), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
 }
 
 // Untiled copy of `bytes` (a multiple of 16, both addresses 16-byte aligned) to shared memory.

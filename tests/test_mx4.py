@@ -263,6 +263,19 @@ def test_product_large_rows(built):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("y_dtype,ypad", [("f32", 0), ("f32", 1), ("bf16", 0), ("f16", 6)])
+@pytest.mark.parametrize("r,n,k", [(2600, 1300, 320), (2561, 1152, 1030), (2700, 1147, 96)])
+def test_product_many_tiles(built, r, n, k, y_dtype, ypad):
+    """Tiles for every SM several times over, both tile widths, ragged at each end; y rows that can and
+    cannot be stored 16 bytes at a time."""
+    rng = np.random.default_rng(r + n)
+    w = rng.standard_normal((n, k)).astype(np.float32)
+    b = rng.standard_normal(n).astype(np.float32)
+    seen, y = product(built, w, rng.standard_normal((r, k)), b, "f32", y_dtype, 0, ypad)
+    check_product(ref_quantize(w)[2], seen, y, b, y_dtype)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("r", [3, 40, 200])
 def test_product_nonfinite_rows_stay_apart(built, r):
     rng = np.random.default_rng(r)
