@@ -264,7 +264,7 @@ def test_product_large_rows(built):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("y_dtype,ypad", [("f32", 0), ("f32", 1), ("bf16", 0), ("f16", 6)])
-@pytest.mark.parametrize("r,n,k", [(2600, 1300, 320), (2561, 1152, 1030), (2700, 1147, 96)])
+@pytest.mark.parametrize("r,n,k", [(2600, 1300, 320), (2561, 1152, 1030), (2700, 1147, 96), (2561, 1152, 1600), (2600, 1300, 2055)])
 def test_product_many_tiles(built, r, n, k, y_dtype, ypad):
     """Tiles for every SM several times over, both tile widths, ragged at each end; y rows that can and
     cannot be stored 16 bytes at a time."""
