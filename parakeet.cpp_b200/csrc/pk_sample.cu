@@ -258,28 +258,35 @@ struct Slice {
         const float v = to_f32(gl[i]);
         return inf ? (v == CUDART_INF_F ? 0.0f : -CUDART_INF_F) : v;
     }
-    // f(value, index in the slice) for every element and some -infinities around them, a whole warp at a time
+    // f(four values, index of the first in the slice) over all quads, -infinities around the slice's
+    // elements, a whole warp at a time
+    template <int NT, class F>
+    __device__ __forceinline__ void quads(int tid, F f) const {
+        const int n4 = RES ? (skew + n + 3) >> 2 : (n + 3) >> 2;
+#pragma unroll 2
+        for (int q = tid & ~31; q < n4; q += NT) {
+            const int i = q + (tid & 31);
+            float4 v = make_float4(-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F);
+            if constexpr (RES) {
+                if (i < n4) v = reinterpret_cast<const float4 *>(sm)[i];
+            } else {
+                if (4 * i < n) v.x = (*this)(4 * i);
+                if (4 * i + 1 < n) v.y = (*this)(4 * i + 1);
+                if (4 * i + 2 < n) v.z = (*this)(4 * i + 2);
+                if (4 * i + 3 < n) v.w = (*this)(4 * i + 3);
+            }
+            f(v, 4 * i - (RES ? skew : 0));
+        }
+    }
+    // f(value, index in the slice), the same way
     template <int NT, class F>
     __device__ __forceinline__ void each(int tid, F f) const {
-        if constexpr (RES) {
-            const int quads = (skew + n + 3) >> 2;
-#pragma unroll 2
-            for (int q = tid & ~31; q < quads; q += NT) {
-                const int i = q + (tid & 31);
-                const float4 v = i < quads ? reinterpret_cast<const float4 *>(sm)[i]
-                                           : make_float4(-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F);
-                const int e = 4 * i - skew;
-                f(v.x, e);
-                f(v.y, e + 1);
-                f(v.z, e + 2);
-                f(v.w, e + 3);
-            }
-        } else {
-            for (int q = tid & ~31; q < n; q += NT) {
-                const int i = q + (tid & 31);
-                f(i < n ? (*this)(i) : -CUDART_INF_F, i);
-            }
-        }
+        quads<NT>(tid, [&](float4 v, int e) {
+            f(v.x, e);
+            f(v.y, e + 1);
+            f(v.z, e + 2);
+            f(v.w, e + 3);
+        });
     }
 };
 
@@ -356,7 +363,10 @@ __device__ bool find_bin(Team<NT, CL> & team, TeamBins<NT> * B, const Slice<T, R
                          const Share * share) {
     constexpr int NB = bins_of<NT>(), PER = NB / NT;
     TeamSmem<NT> * s = team.s;
-    for (int b = team.tid; b < NB; b += NT) { B->lo[b] = 0; if (WEIGHTS) B->hi[b] = 0; }
+    for (int b = team.tid; b < NB; b += NT) {
+        B->lo[b] = 0;
+        if (WEIGHTS) B->hi[b] = 0;
+    }
     if (team.tid == 0) { s->found = -1; s->listed = 0; }
     team.sync();
     u64 rest = 0;
@@ -389,10 +399,17 @@ __device__ bool find_bin(Team<NT, CL> & team, TeamBins<NT> * B, const Slice<T, R
         const int b = team.tid * PER + j;
         u64 w = 0;
         if (CL) {
-            for (int q = 0; q < team.blocks; ++q) {
-                const TeamBins<NT> * o = cg::this_cluster().map_shared_rank(B, q);
-                w += (WEIGHTS ? (u64) o->hi[b] << 32 : 0ull) + o->lo[b];
+            // all blocks' words are asked for before the first is used
+            unsigned rl[kMaxCluster], rh[kMaxCluster];
+#pragma unroll
+            for (int q = 0; q < kMaxCluster; ++q) {
+                const TeamBins<NT> * o = cg::this_cluster().map_shared_rank(B, q < team.blocks ? q : 0);
+                rl[q] = o->lo[b];
+                rh[q] = WEIGHTS ? o->hi[b] : 0u;
             }
+#pragma unroll
+            for (int q = 0; q < kMaxCluster; ++q)
+                if (q < team.blocks) w += ((u64) rh[q] << 32) + rl[q];
         } else {
             w = (WEIGHTS ? (u64) B->hi[b] << 32 : 0ull) + B->lo[b];
         }
@@ -431,14 +448,17 @@ __device__ bool find_bin(Team<NT, CL> & team, TeamBins<NT> * B, const Slice<T, R
 template <class T, int NT, bool CL, bool RES, class F>
 __device__ int gather(Team<NT, CL> & team, TeamBins<NT> * B, const Slice<T, RES> & l, int s0, const Pair *& list, F want) {
     TeamSmem<NT> * s = team.s;
-    l.template each<NT>(team.tid, [&](float v, int i) {
-        const bool w = want(v);
-        const unsigned who = __ballot_sync(kFull, w);
-        if (who == 0) return;
-        int at = 0;
-        if (team.lane() == 0) at = atomicAdd(&s->listed, __popc(who));
-        at = __shfl_sync(kFull, at, 0) + __popc(who & ((1u << team.lane()) - 1u));
-        if (w && at < kList) B->list[at] = Pair{v, s0 + i};
+    l.template quads<NT>(team.tid, [&](float4 v, int i) {
+        const bool a = want(v.x), b = want(v.y), c = want(v.z), d = want(v.w);
+        if (!(a || b || c || d)) return;
+        int at = atomicAdd(&s->listed, (int) a + (int) b + (int) c + (int) d);
+        if (a && at < kList) B->list[at] = Pair{v.x, s0 + i};
+        at += a;
+        if (b && at < kList) B->list[at] = Pair{v.y, s0 + i + 1};
+        at += b;
+        if (c && at < kList) B->list[at] = Pair{v.z, s0 + i + 2};
+        at += c;
+        if (d && at < kList) B->list[at] = Pair{v.w, s0 + i + 3};
     });
     team.sync();
     int n = s->listed;
@@ -448,17 +468,13 @@ __device__ int gather(Team<NT, CL> & team, TeamBins<NT> * B, const Slice<T, RES>
         if (team.tid == 0) x.a = (u64) n;
         team.meet();
         n = 0;
-        for (int q = 0; q < team.blocks; ++q) n += (int) cg::this_cluster().map_shared_rank(&x, q)->a;
-        if (n <= kList) {
-            int base = 0;
-            for (int q = 0; q < team.blocks; ++q) {
-                const int c = (int) cg::this_cluster().map_shared_rank(&x, q)->a;
-                const TeamBins<NT> * o = cg::this_cluster().map_shared_rank(B, q);
-                for (int i = team.tid; i < c; i += NT) B->all[base + i] = o->list[i];
-                base += c;
-            }
-            list = B->all;
+        for (int q = 0; q < team.blocks; ++q) {
+            const int c = (int) cg::this_cluster().map_shared_rank(&x, q)->a;
+            const TeamBins<NT> * o = cg::this_cluster().map_shared_rank(B, q);
+            for (int i = team.tid; i < c && n + i < kList; i += NT) B->all[n + i] = o->list[i];
+            n += c;
         }
+        list = B->all;
         team.phase ^= 1;
         team.meet();                            // nobody lists anew while another still reads
     }
@@ -466,6 +482,52 @@ __device__ int gather(Team<NT, CL> & team, TeamBins<NT> * B, const Slice<T, RES>
     if (team.tid == 0) s->listed = 0;           // read by all: the next list starts empty
     team.sync();
     return n;
+}
+
+// For each token of a list of n: f(token, sum of g(token, other token) over the list), a few
+// neighbouring threads sharing a token's sum. Entries behind the list count for nothing.
+template <int NT> constexpr int sharers() { return NT > 2 * kList ? 4 : NT > kList ? 2 : 1; }
+template <int NT, class V, class G, class F>
+__device__ __forceinline__ void over_list(int tid, int n, G g, F f) {
+    constexpr int SH = sharers<NT>(), PER = (kList * SH + NT - 1) / NT;
+    const int padded = min(kList, (n + 4 * SH - 1) / (4 * SH) * (4 * SH));
+#pragma unroll
+    for (int q = 0; q < PER; ++q) {
+        const int j = (tid + q * NT) / SH;
+        V sum{};
+#pragma unroll 4
+        for (int i = tid % SH; i < padded; i += SH) g(sum, j, i);
+#pragma unroll
+        for (int o = 1; o < SH; o <<= 1) sum.add(sum.across(o));
+        if (j < n && tid % SH == 0) f(j, sum, q);
+    }
+}
+struct Rank {                                   // tokens before one in the order, and their weight
+    u64 w = 0;
+    int n = 0;
+    __device__ __forceinline__ void add(const Rank & o) { w += o.w; n += o.n; }
+    __device__ __forceinline__ Rank across(int o) const {
+        Rank r;
+        r.w = __shfl_xor_sync(kFull, w, o);
+        r.n = __shfl_xor_sync(kFull, n, o);
+        return r;
+    }
+};
+struct Around {                                 // weight above a logit, and at it
+    u64 over = 0, same = 0;
+    __device__ __forceinline__ void add(const Around & o) { over += o.over; same += o.same; }
+    __device__ __forceinline__ Around across(int o) const {
+        Around r;
+        r.over = __shfl_xor_sync(kFull, over, o);
+        r.same = __shfl_xor_sync(kFull, same, o);
+        return r;
+    }
+};
+
+// Weights of the list's tokens (1: `ones`), nothing behind them.
+template <int NT>
+__device__ __forceinline__ void weigh_list(int tid, TeamBins<NT> * B, const Pair * list, int n, const Row & r, bool ones) {
+    for (int j = tid; j < kList; j += NT) B->w[j] = j < n ? (ones ? 1ull : weight_one(list[j].v, r)) : 0ull;
 }
 
 // The cut inside the bin that find_bin found: everything above the returned logit is kept, and
@@ -479,22 +541,22 @@ __device__ float find_cut(Team<NT, CL> & team, TeamBins<NT> * B, const Slice<T, 
         const Pair * list;
         const int n = gather<T, NT, CL, RES>(team, B, l, 0, list, [&](float v) { return L.holds(v) && L.bin_of<NB>(v) == L.bin; });
         if (n <= kList) {
-            for (int j = team.tid; j < n; j += NT) B->w[j] = WEIGHTS ? weight_one(list[j].v, row) : 1ull;
+            weigh_list<NT>(team.tid, B, list, n, row, !WEIGHTS);
             team.sync();
-            for (int j = team.tid; j < n; j += NT) {
-                const float v = list[j].v;
-                u64 over = L.above, same = 0;
-                for (int i = 0; i < n; ++i) {
-                    const float o = list[i].v;
-                    if (o > v) over += B->w[i];
-                    else if (o == v) same += B->w[i];
-                }
-                if (over < need && need <= over + same) {        // threads with equal logits write the same
-                    s->cut = v;
-                    s->cut_ties = (need - over + B->w[j] - 1) / B->w[j];
-                    s->cut_partial = s->cut_ties * B->w[j] < same;
-                }
-            }
+            over_list<NT, Around>(team.tid, n,
+                [&](Around & a, int j, int i) {
+                    const float o = list[i].v, v = list[j].v;
+                    if (o > v) a.over += B->w[i];
+                    if (o == v) a.same += B->w[i];
+                },
+                [&](int j, const Around & a, int) {
+                    const u64 over = L.above + a.over;
+                    if (over < need && need <= over + a.same) {  // threads with equal logits write the same
+                        s->cut = list[j].v;
+                        s->cut_ties = (need - over + B->w[j] - 1) / B->w[j];
+                        s->cut_partial = s->cut_ties * B->w[j] < a.same;
+                    }
+                });
             team.sync();
             ties = s->cut_ties;
             partial = s->cut_partial != 0;
@@ -536,29 +598,22 @@ __device__ __forceinline__ u64 place_of(float u, u64 total) {
 template <int NT, bool CL>
 __device__ void draw_listed(Team<NT, CL> & team, TeamBins<NT> * B, const Pair * list, int n, const pk_sample_args & a, long long row,
                             const Row & r, float hi, double inv_t, int k, float p, u64 need, float least) {
-    for (int j = team.tid; j < n; j += NT) B->w[j] = weight_one(list[j].v, r);
+    weigh_list<NT>(team.tid, B, list, n, r, false);
     team.sync();
-    constexpr int PER = (kList + NT - 1) / NT;                   // tokens of a thread
-    u64 over[PER], sum = 0;                                      // weight before each in the order
-    int place[PER];
+    constexpr int PER = (kList * sharers<NT>() + NT - 1) / NT;   // tokens of a thread
+    Rank rank[PER];
+    u64 sum = 0;
 #pragma unroll
-    for (int q = 0; q < PER; ++q) {
-        const int j = team.tid + q * NT;
-        over[q] = 0;
-        place[q] = kList;
-        if (j < n) {
-            const Pair me = list[j];
-            int c = 0;
-            u64 w = 0;
-            for (int i = 0; i < n; ++i) {
-                const Pair o = list[i];
-                if (o.v > me.v || (o.v == me.v && o.i < me.i)) { w += B->w[i]; ++c; }
-            }
-            over[q] = w;
-            place[q] = c;
-            if (c < k) sum += B->w[j];
-        }
-    }
+    for (int q = 0; q < PER; ++q) rank[q].n = kList;
+    over_list<NT, Rank>(team.tid, n,
+        [&](Rank & a, int j, int i) {
+            const Pair me = list[j], o = list[i];
+            if (i < n && (o.v > me.v || (o.v == me.v && o.i < me.i))) { a.w += B->w[i]; ++a.n; }
+        },
+        [&](int j, const Rank & a, int q) {
+            rank[q] = a;
+            if (a.n < k) sum += B->w[j];
+        });
     Team<NT, false> block{team.tid, 0, 1, 0, team.s, 0.0};
     if (need == 0) {
         sum = block.sum(sum);
@@ -568,9 +623,9 @@ __device__ void draw_listed(Team<NT, CL> & team, TeamBins<NT> * B, const Pair * 
     u64 kept = 0;
 #pragma unroll
     for (int q = 0; q < PER; ++q) {
-        const int j = team.tid + q * NT;
-        if (j < n) {
-            const bool keep = place[q] < k && over[q] < need && list[j].v >= least;
+        const int j = (team.tid + q * NT) / sharers<NT>();
+        if (j < n && team.tid % sharers<NT>() == 0) {
+            const bool keep = rank[q].n < k && rank[q].w < need && list[j].v >= least;
             if (!keep) B->w[j] = 0;
             else kept += B->w[j];
         }
@@ -578,16 +633,12 @@ __device__ void draw_listed(Team<NT, CL> & team, TeamBins<NT> * B, const Pair * 
     const u64 total = block.sum(kept);
     team.sync();
     const u64 t = place_of(a.uniforms[row], total);
-#pragma unroll
-    for (int q = 0; q < PER; ++q) {
-        const int j = team.tid + q * NT;
-        if (j < n && B->w[j] > 0) {
-            u64 before = 0;
-            for (int i = 0; i < n; ++i)
-                if (list[i].i < list[j].i) before += B->w[i];
-            if (before <= t && t < before + B->w[j] && team.rank == 0) write_token(a, row, list[j].i, list[j].v, hi, inv_t, total);
-        }
-    }
+    over_list<NT, Rank>(team.tid, n,
+        [&](Rank & a, int j, int i) { if (list[i].i < list[j].i) a.w += B->w[i]; },
+        [&](int j, const Rank & before, int) {
+            const u64 w = B->w[j];
+            if (before.w <= t && t < before.w + w && team.rank == 0) write_token(a, row, list[j].i, list[j].v, hi, inv_t, total);
+        });
 }
 
 template <class T, int NT, bool FILTERS, bool CL, bool RES>
@@ -730,9 +781,10 @@ sample_kernel(pk_sample_args a, int slice, int teams, int row_floats) {
                 need = max((u64) ceil(share.p * (double) share.lump), 1ull);
             }
             if (found) {
-                // few enough for the list, as far as their weight tells: none is lighter than the bin's lower edge
+                // Few enough to be listed? None is lighter than the bin's lower edge. With more than some 32
+                // the list's ranks cost more than the sums below.
                 const float edge = fmaxf(from, hi - (hi - from) * ((float) (L.bin + 1) / (float) NB));
-                if ((double) L.with <= 4.0 * kList * (double) max(weight_one(edge, r), 1ull)) {
+                if ((double) L.with <= 32.0 * (double) max(weight_one(edge, r), 1ull)) {
                     const Pair * list;
                     const int n = gather<T, NT, CL, RES>(team, bins, l, s0, list,
                                                          [&](float v) { return L.holds(v) && L.bin_of<NB>(v) <= L.bin; });
@@ -873,11 +925,14 @@ template <class T, bool FILTERS>
 cudaError_t dispatch(const pk_sample_args & a, cudaStream_t s) {
     if (a.vocab <= 1280 && a.rows >= 512) return launch_block<T, FILTERS, 32>(a, s);
     if (a.vocab <= 2048) return launch_block<T, FILTERS, 128>(a, s);
+    // Few rows of a large vocabulary over clusters. A cluster's barriers cost more than they save
+    // below: one row of 8193 in one block of 512 16 us, in a cluster of eight 20 us.
     int blocks = 1;
-    while (blocks < kMaxCluster && a.rows * blocks * 2 <= 148 && a.vocab / (blocks * 2) >= 1024) blocks *= 2;
+    if (a.vocab > 16384)
+        while (blocks < kMaxCluster && a.rows * blocks * 2 <= 148) blocks *= 2;
     while (blocks < kMaxCluster && (size_t) (a.vocab / blocks) * 4 > 200 * 1024) blocks *= 2;
     if (blocks > 1) return launch_cluster<T, FILTERS>(a, blocks, s);
-    if (a.vocab <= 16384) return launch_block<T, FILTERS, 256>(a, s);
+    if (a.vocab <= 16384 && a.rows > 148) return launch_block<T, FILTERS, 256>(a, s);
     return launch_block<T, FILTERS, 512>(a, s);
 }
 
