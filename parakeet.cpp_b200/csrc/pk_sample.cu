@@ -131,7 +131,7 @@ struct TeamSmem {
 };
 template <int NT>
 struct TeamBins {
-    unsigned lo[bins_of<NT>()], hi[bins_of<NT>()];     // sums of weights, or counts in lo
+    uint2 sum[bins_of<NT>()];                          // of weights, in two halves; or counts in x
     Pair list[kList];
     Pair all[kList];                                   // of all blocks of a cluster
     u64 w[kList];
@@ -364,8 +364,7 @@ __device__ bool find_bin(Team<NT, CL> & team, TeamBins<NT> * B, const Slice<T, R
     constexpr int NB = bins_of<NT>(), PER = NB / NT;
     TeamSmem<NT> * s = team.s;
     for (int b = team.tid; b < NB; b += NT) {
-        B->lo[b] = 0;
-        if (WEIGHTS) B->hi[b] = 0;
+        B->sum[b] = make_uint2(0, 0);
     }
     if (team.tid == 0) { s->found = -1; s->listed = 0; }
     team.sync();
@@ -379,15 +378,15 @@ __device__ bool find_bin(Team<NT, CL> & team, TeamBins<NT> * B, const Slice<T, R
             if (any) {
                 if (v >= L.lo) {
                     const int b = L.bin_of<NB>(v);
-                    const unsigned wl = (unsigned) w, old = atomicAdd(&B->lo[b], wl);
+                    const unsigned wl = (unsigned) w, old = atomicAdd(&B->sum[b].x, wl);
                     const unsigned up = (unsigned) (w >> 32) + (old + wl < old ? 1u : 0u);
-                    if (up) atomicAdd(&B->hi[b], up);
+                    if (up) atomicAdd(&B->sum[b].y, up);
                 } else {
                     rest += w;
                 }
             }
         } else if (L.holds(v)) {
-            atomicAdd(&B->lo[L.bin_of<NB>(v)], 1u);
+            atomicAdd(&B->sum[L.bin_of<NB>(v)].x, 1u);
         }
     });
     if (WEIGHTS && share) rest = team.sum(rest);                 // in a cluster, all bins are complete after it
@@ -400,18 +399,14 @@ __device__ bool find_bin(Team<NT, CL> & team, TeamBins<NT> * B, const Slice<T, R
         u64 w = 0;
         if (CL) {
             // all blocks' words are asked for before the first is used
-            unsigned rl[kMaxCluster], rh[kMaxCluster];
+            uint2 r[kMaxCluster];
 #pragma unroll
-            for (int q = 0; q < kMaxCluster; ++q) {
-                const TeamBins<NT> * o = cg::this_cluster().map_shared_rank(B, q < team.blocks ? q : 0);
-                rl[q] = o->lo[b];
-                rh[q] = WEIGHTS ? o->hi[b] : 0u;
-            }
+            for (int q = 0; q < kMaxCluster; ++q) r[q] = cg::this_cluster().map_shared_rank(B, q < team.blocks ? q : 0)->sum[b];
 #pragma unroll
             for (int q = 0; q < kMaxCluster; ++q)
-                if (q < team.blocks) w += ((u64) rh[q] << 32) + rl[q];
+                if (q < team.blocks) w += ((u64) r[q].y << 32) + r[q].x;
         } else {
-            w = (WEIGHTS ? (u64) B->hi[b] << 32 : 0ull) + B->lo[b];
+            w = ((u64) B->sum[b].y << 32) + B->sum[b].x;
         }
         mine[j] = w;
         sum += w;
@@ -486,7 +481,7 @@ __device__ int gather(Team<NT, CL> & team, TeamBins<NT> * B, const Slice<T, RES>
 
 // For each token of a list of n: f(token, sum of g(token, other token) over the list), a few
 // neighbouring threads sharing a token's sum. Entries behind the list count for nothing.
-template <int NT> constexpr int sharers() { return NT > 2 * kList ? 4 : NT > kList ? 2 : 1; }
+template <int NT> constexpr int sharers() { return NT >= 8 * kList ? 8 : NT >= 4 * kList ? 4 : NT >= 2 * kList ? 2 : 1; }
 template <int NT, class V, class G, class F>
 __device__ __forceinline__ void over_list(int tid, int n, G g, F f) {
     constexpr int SH = sharers<NT>(), PER = (kList * SH + NT - 1) / NT;
@@ -538,8 +533,13 @@ __device__ float find_cut(Team<NT, CL> & team, TeamBins<NT> * B, const Slice<T, 
     constexpr int NB = bins_of<NT>();
     TeamSmem<NT> * s = team.s;
     for (;;) {
-        const Pair * list;
-        const int n = gather<T, NT, CL, RES>(team, B, l, 0, list, [&](float v) { return L.holds(v) && L.bin_of<NB>(v) == L.bin; });
+        // at least this many tokens are in the bin, as none is heavier than its upper edge
+        const float edge = fminf(L.hi, L.hi - (L.hi - L.lo) * (((float) L.bin - 0.01f) / (float) NB));
+        const u64 most = WEIGHTS ? max(weight_one(edge, row), 1ull) : 1ull;
+        const Pair * list = nullptr;
+        int n = kList + 1;
+        if (L.with - L.above <= (u64) kList * most)
+            n = gather<T, NT, CL, RES>(team, B, l, 0, list, [&](float v) { return L.holds(v) && L.bin_of<NB>(v) == L.bin; });
         if (n <= kList) {
             weigh_list<NT>(team.tid, B, list, n, row, !WEIGHTS);
             team.sync();
@@ -916,9 +916,9 @@ cudaError_t launch_cluster(const pk_sample_args & a, int blocks, cudaStream_t s)
     // slices of whole 16 bytes, so that every slice is aligned as its row is
     const int slice = ((a.vocab + blocks - 1) / blocks + 31) / 32 * 32;
     int row_floats;
-    const size_t smem = team_bytes<512, FILTERS>(slice, row_floats);
-    if (smem <= kSmemCap) return launch<T, 512, FILTERS, true, true>(a, blocks, slice, row_floats, smem, s);
-    return launch<T, 512, FILTERS, true, false>(a, blocks, slice, 0, smem - (size_t) row_floats * 4, s);
+    const size_t smem = team_bytes<1024, FILTERS>(slice, row_floats);
+    if (smem <= kSmemCap) return launch<T, 1024, FILTERS, true, true>(a, blocks, slice, row_floats, smem, s);
+    return launch<T, 1024, FILTERS, true, false>(a, blocks, slice, 0, smem - (size_t) row_floats * 4, s);
 }
 
 template <class T, bool FILTERS>
