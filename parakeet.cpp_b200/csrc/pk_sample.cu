@@ -12,6 +12,12 @@
 // f32's 2^-22 the running sum would pass the random number at another token in one of a few hundred
 // rows, since a row has as many borders as tokens.
 //
+// Rows of up to 1280 logits with nothing cut, as a CTC path has them by the ten thousand, are summed in
+// f32 first: five instructions a token instead of twenty. That settles the token unless the random
+// number lies within a proven bound of a border (one or two rows in a hundred), and those rows go on to
+// the f64 sums, so the token is the same; the log-probability then has f32's sum, 2^-18 off at most.
+// 66044 rows of 1025: see draw_f32.
+//
 // A team of threads (a warp, a block, or a cluster of blocks) holds one row in shared memory:
 //  1. load, largest and smallest logit;
 //  2. with top-k or top-p, a histogram over the range that can matter, linear in the logit, of
@@ -641,6 +647,63 @@ __device__ void draw_listed(Team<NT, CL> & team, TeamBins<NT> * B, const Pair * 
         });
 }
 
+// A warp's row by f32 sums; false where they cannot tell the token.
+//
+// w^ = ex2(x^), x^ = fl(fl(v - top) c), three roundings off x by 3.01 2^-24 |x|, ex2.approx by 2^-21 of
+// itself at most: |w^ - w| <= w (2^-21 + 2.11 2^-24 |x|). With p = w / S and S >= 1, the sum of p |x| is
+// the entropy of p less log2 S, so at most log2 V: any sum of w^ over tokens is within
+// S 2^-24 (8 + 2.11 log2 V) <= 30 S 2^-24 of that of w, for V <= 1280. A run's terms go to four
+// accumulators, 11 additions each and two more: 13 S 2^-24. The runs are added in f64. Together below
+// 2^-18 S = E for every prefix and for S, so u S is off by as much: the token is settled if the border
+// before it and the one behind are each more than 2 E (2.5 E, against what is left) from u S.
+template <class T, bool RES>
+__device__ __forceinline__ bool draw_f32(const Slice<T, RES> & l, int len, int lane, float hi, float temp, float u, const pk_sample_args & a,
+                                         long long row) {
+    const float inv_t = 1.0f / temp, c = 1.4426950408889634f * inv_t;
+    if (!(c > 1e-30f && c < 1e30f)) return false;        // a product with 0 or infinity could be a NaN
+    // NaN and -infinity count as the lowest number, whose weight is 0
+    auto weight = [&](float v) {
+        float w;
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w) : "f"(fmaxf(v - hi, -3e38f) * c));
+        return w;
+    };
+    const int i0 = lane * len;
+    float part[4] = {};
+    int j = 0;
+    for (; j + 4 <= len; j += 4) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) part[q] += weight(l(i0 + j + q));
+    }
+    for (; j < len; ++j) part[0] += weight(l(i0 + j));
+    const double sum = (double) ((part[0] + part[1]) + (part[2] + part[3]));
+    const double upto = warp_scan(sum, lane), total = __shfl_sync(kFull, upto, 31);
+    u = u > 0.0f ? fminf(u, 0x1.fffffep-1f) : 0.0f;
+    const double t = (double) u * total, margin = total * 0x1.4p-17;
+    // the run that holds t: the first whose end is past it
+    const unsigned past = __ballot_sync(kFull, upto > t);
+    if (past == 0) return false;
+    const int who = __ffs((int) past) - 1;
+    double run = __shfl_sync(kFull, upto - sum, who);
+    const int e = min((who + 1) * len, l.n);
+    for (int b = who * len; b < e; b += 32) {
+        const int i = b + lane;
+        const float v = i < e ? l(i) : -CUDART_INF_F, w = weight(v);
+        const double end = run + warp_scan((double) w, lane);
+        const unsigned beyond = __ballot_sync(kFull, end > t);
+        if (beyond != 0) {
+            const bool mine = lane == __ffs((int) beyond) - 1;
+            const bool sure = mine && i < e && end - t > margin && (t - (end - (double) w) > margin);
+            if (sure) {
+                a.tokens[row] = i;
+                if (a.logprobs) a.logprobs[row] = (float) ((double) (v - hi) * (double) inv_t - (double) logf((float) total));
+            }
+            return __any_sync(kFull, sure);
+        }
+        run = __shfl_sync(kFull, end, 31);
+    }
+    return false;
+}
+
 template <class T, int NT, bool FILTERS, bool CL, bool RES>
 __global__ void __launch_bounds__(NT == 32 ? 256 : NT)
 sample_kernel(pk_sample_args a, int slice, int teams, int row_floats) {
@@ -716,6 +779,8 @@ sample_kernel(pk_sample_args a, int slice, int teams, int row_floats) {
         l.inf = true;
         hi = lo = 0.0f;
     }
+    if constexpr (!FILTERS && NT == 32)
+        if (draw_f32<T, RES>(l, len, team.tid, hi, temp_f, a.uniforms[row], a, row)) return;
     Row r;
     r.top = (double) hi;
     const double inv_t = 1.0 / temp;                             // 0 for an infinite T
