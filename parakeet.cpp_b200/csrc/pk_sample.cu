@@ -13,7 +13,7 @@
 // rows, since a row has as many borders as tokens.
 //
 // Rows of up to 1280 logits with nothing cut, as a CTC path has them by the ten thousand, are summed in
-// f32 first: five instructions a token instead of twenty. That settles the token unless the random
+// f32 first: four instructions a token instead of twenty. That settles the token unless the random
 // number lies within a proven bound of a border (one or two rows in a hundred), and those rows go on to
 // the f64 sums, so the token is the same; the log-probability then has f32's sum, 2^-18 off at most.
 // 66044 rows of 1025: see draw_f32.
@@ -214,11 +214,12 @@ struct Team {
         return before;
     }
     // Largest of hi, smallest of lo, over the team.
+    template <bool LO = true>
     __device__ __forceinline__ void range(float & hi, float & lo) {
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) {
             hi = fmaxf(hi, __shfl_xor_sync(kFull, hi, o));
-            lo = fminf(lo, __shfl_xor_sync(kFull, lo, o));
+            if (LO) lo = fminf(lo, __shfl_xor_sync(kFull, lo, o));
         }
         if (NT > 32) {
             sync();
@@ -327,8 +328,10 @@ __device__ __forceinline__ void load_slice(const Slice<T, true> & l, int tid) {
             d[1] = make_float4(f[4], f[5], f[6], f[7]);
         }
     }
-    for (int i = tid; i < head; i += NT) sm[i] = to_f32(g[i]);
-    for (int i = head + vecs * W + tid; i < n; i += NT) sm[i] = to_f32(g[i]);
+    if (tid < 16) {                                      // fewer than W at either end
+        const int i = tid < 8 ? tid : head + vecs * W + tid - 8;
+        if (tid < 8 ? i < head : i < n) sm[i] = to_f32(g[i]);
+    }
     if (tid < l.skew) l.sm[tid] = -CUDART_INF_F;
     for (int i = n + tid; i < l.pad; i += NT) sm[i] = -CUDART_INF_F;
     if constexpr (sizeof(T) == 4) asm volatile("cp.async.wait_all;" ::: "memory");
@@ -649,22 +652,23 @@ __device__ void draw_listed(Team<NT, CL> & team, TeamBins<NT> * B, const Pair * 
 
 // A warp's row by f32 sums; false where they cannot tell the token.
 //
-// w^ = ex2(x^), x^ = fl(fl(v - top) c), three roundings off x by 3.01 2^-24 |x|, ex2.approx by 2^-21 of
-// itself at most: |w^ - w| <= w (2^-21 + 2.11 2^-24 |x|). With p = w / S and S >= 1, the sum of p |x| is
-// the entropy of p less log2 S, so at most log2 V: any sum of w^ over tokens is within
-// S 2^-24 (8 + 2.11 log2 V) <= 30 S 2^-24 of that of w, for V <= 1280. A run's terms go to four
-// accumulators, 11 additions each and two more: 13 S 2^-24. The runs are added in f64. Together below
-// 2^-18 S = E for every prefix and for S, so u S is off by as much: the token is settled if the border
-// before it and the one behind are each more than 2 E (2.5 E, against what is left) from u S.
+// w^ = ex2(x^), x^ = fma(v, c, -k) with c = fl(log2(e) / T) and k = fl(hi c). What k is off by is the same
+// for all tokens and drops out (of the log-probability it is taken again). c is off by 3 2^-24, the sum
+// by 2^-24 of itself, so x^ by 4 2^-24 |x|, and ex2.approx by 2^-21 of its result at most:
+// |w^ - w| <= w 2^-24 (8 + 2.78 |x|). With p = w / S and S >= 1, the sum of p |x| is the entropy of p
+// less log2 S, so at most log2 V: any sum of w^ over tokens is within S 2^-24 (8 + 2.78 log2 V) <=
+// 37 S 2^-24 of that of w, for V <= 1280. A run's terms go to four accumulators, 11 additions each and
+// two more: 13 S 2^-24. The runs are added in f64. Together below 2^-18 S = E for every prefix and for
+// S, so u S is off by as much: the token is settled if the border before it and the one behind are each
+// more than 2 E (2.5 E, against what is left) from u S.
 template <class T, bool RES>
 __device__ __forceinline__ bool draw_f32(const Slice<T, RES> & l, int len, int lane, float hi, float temp, float u, const pk_sample_args & a,
                                          long long row) {
-    const float inv_t = 1.0f / temp, c = 1.4426950408889634f * inv_t;
-    if (!(c > 1e-30f && c < 1e30f)) return false;        // a product with 0 or infinity could be a NaN
-    // NaN and -infinity count as the lowest number, whose weight is 0
-    auto weight = [&](float v) {
+    const float inv_t = 1.0f / temp, c = 1.4426950408889634f * inv_t, k = hi * c;
+    if (!(c > 1e-30f && c < 1e30f && fabsf(k) < 1e6f)) return false;
+    auto weight = [&](float v) {                         // 0 for -infinity; a NaN ends in the sum
         float w;
-        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w) : "f"(fmaxf(v - hi, -3e38f) * c));
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w) : "f"(fmaf(v, c, -k)));
         return w;
     };
     const int i0 = lane * len;
@@ -677,6 +681,7 @@ __device__ __forceinline__ bool draw_f32(const Slice<T, RES> & l, int len, int l
     for (; j < len; ++j) part[0] += weight(l(i0 + j));
     const double sum = (double) ((part[0] + part[1]) + (part[2] + part[3]));
     const double upto = warp_scan(sum, lane), total = __shfl_sync(kFull, upto, 31);
+    if (!(total < 1e30)) return false;
     u = u > 0.0f ? fminf(u, 0x1.fffffep-1f) : 0.0f;
     const double t = (double) u * total, margin = total * 0x1.4p-17;
     // the run that holds t: the first whose end is past it
@@ -695,7 +700,9 @@ __device__ __forceinline__ bool draw_f32(const Slice<T, RES> & l, int len, int l
             const bool sure = mine && i < e && end - t > margin && (t - (end - (double) w) > margin);
             if (sure) {
                 a.tokens[row] = i;
-                if (a.logprobs) a.logprobs[row] = (float) ((double) (v - hi) * (double) inv_t - (double) logf((float) total));
+                const double off = (double) k - (double) hi * (double) c;   // every weight is 2^-off of what it should be
+                if (a.logprobs)
+                    a.logprobs[row] = (float) ((double) (v - hi) * (double) inv_t - 0.6931471805599453 * off - (double) logf((float) total));
             }
             return __any_sync(kFull, sure);
         }
@@ -705,7 +712,7 @@ __device__ __forceinline__ bool draw_f32(const Slice<T, RES> & l, int len, int l
 }
 
 template <class T, int NT, bool FILTERS, bool CL, bool RES>
-__global__ void __launch_bounds__(NT == 32 ? 256 : NT)
+__global__ void __launch_bounds__(NT == 32 ? 256 : NT, NT == 32 ? (FILTERS ? 4 : 5) : 1024 / NT)
 sample_kernel(pk_sample_args a, int slice, int teams, int row_floats) {
     extern __shared__ __align__(16) unsigned char raw[];
     const int t_in = NT == 32 ? (int) threadIdx.x >> 5 : 0;      // team within the block
@@ -741,7 +748,7 @@ sample_kernel(pk_sample_args a, int slice, int teams, int row_floats) {
         hi = fmaxf(hi, v);
         if (FILTERS && v > -CUDART_INF_F) lo = fminf(lo, v);
     });
-    team.range(hi, lo);
+    team.template range<FILTERS>(hi, lo);
     if (hi == -CUDART_INF_F || !(temp_f > 0.0f)) {
         // nothing to draw, or the first index of the largest
         u64 first = ~0ull;
