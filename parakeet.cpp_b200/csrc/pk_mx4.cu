@@ -56,7 +56,7 @@ __device__ __forceinline__ unsigned cvt_e2m1x2(float lo, float hi) {
 }
 
 // Eight consecutive elements of a row, as loaded.
-template <class T> struct Eight { T e[8]; };
+template <class T> struct alignas(16) Eight { T e[8]; };
 
 template <class T, bool VEC>
 __device__ __forceinline__ Eight<T> load8(const T * __restrict__ row, int c, int K) {
@@ -66,8 +66,14 @@ __device__ __forceinline__ Eight<T> load8(const T * __restrict__ row, int c, int
         for (int i = 0; i < (int) sizeof(T) / 2; ++i)
             reinterpret_cast<uint4 *>(v.e)[i] = __ldcs(reinterpret_cast<const uint4 *>(row + c) + i);
     } else {
+        // zeros from column K on
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v.e[i] = c + i < K ? row[c + i] : from_f32<T>(0.0f);   // zeros from column K on
+        for (int i = 0; i < 8; ++i) v.e[i] = from_f32<T>(0.0f);
+        if (c < K) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (c + i < K) v.e[i] = row[c + i];
+        }
     }
     return v;
 }
@@ -84,16 +90,21 @@ __device__ __forceinline__ unsigned amax_bits(const Eight<float> & v) {
     const float m = max3_abs(max3_abs(v.e[0], v.e[1], v.e[2]), max3_abs(v.e[3], v.e[4], v.e[5]), max3_abs(v.e[6], v.e[7], 0.0f));
     return __float_as_uint(m);
 }
-template <class T> __device__ __forceinline__ unsigned amax_bits(const Eight<T> & v) {
+// In half precision two at a time; the larger of the two halves is taken once four lanes have theirs.
+template <class T2> __device__ __forceinline__ T2 pair_of(unsigned w) { return *reinterpret_cast<const T2 *>(&w); }
+template <class T2> __device__ __forceinline__ unsigned word_of(T2 p) { return *reinterpret_cast<const unsigned *>(&p); }
+template <class T2, class T>
+__device__ __forceinline__ T2 amax_pair(const Eight<T> & v) {
     const unsigned * w = reinterpret_cast<const unsigned *>(v.e);
-    const unsigned m = __vmaxu2(__vmaxu2(w[0] & 0x7FFF7FFFu, w[1] & 0x7FFF7FFFu), __vmaxu2(w[2] & 0x7FFF7FFFu, w[3] & 0x7FFF7FFFu));
-    const unsigned short h = (unsigned short) max(m & 0xFFFFu, m >> 16);
-    return __float_as_uint(to_f32(*reinterpret_cast<const T *>(&h)));
+    return __hmax2_nan(__hmax2_nan(__habs2(pair_of<T2>(w[0])), __habs2(pair_of<T2>(w[1]))),
+                       __hmax2_nan(__habs2(pair_of<T2>(w[2])), __habs2(pair_of<T2>(w[3]))));
 }
 
 // Eight codes and their block's scale byte; four neighbouring lanes hold a block.
-template <class T>
-__device__ __forceinline__ unsigned quantize8(const Eight<T> & v, unsigned & sb) {
+__device__ __forceinline__ unsigned join_codes(const unsigned * c) {
+    return __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
+}
+__device__ __forceinline__ unsigned quantize8(const Eight<float> & v, unsigned & sb) {
     unsigned m = amax_bits(v);
     m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
     m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 2));
@@ -101,8 +112,45 @@ __device__ __forceinline__ unsigned quantize8(const Eight<T> & v, unsigned & sb)
     const float inv = scale_inv(sb);                 // garbage for byte 255, whose codes are dropped
     unsigned c[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) c[i] = cvt_e2m1x2(to_f32(v.e[2 * i]) * inv, to_f32(v.e[2 * i + 1]) * inv);
-    const unsigned q = __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
+    for (int i = 0; i < 4; ++i) c[i] = cvt_e2m1x2(v.e[2 * i] * inv, v.e[2 * i + 1] * inv);
+    const unsigned q = join_codes(c);
+    return sb == 255u ? 0u : q;
+}
+__device__ __forceinline__ unsigned quantize8(const Eight<__nv_bfloat16> & v, unsigned & sb) {
+    using T2 = __nv_bfloat162;
+    T2 m = amax_pair<T2>(v);
+    m = __hmax2_nan(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
+    m = __hmax2_nan(m, __shfl_xor_sync(0xFFFFFFFFu, m, 2));
+    const unsigned both = word_of(m);
+    sb = scale_byte(max(both << 16, both & 0xFFFF0000u));
+    // the product with a power of two is exact in bf16 too, what underflows being far below a half code
+    const unsigned inv = (254u - sb) << 7;
+    const T2 inv2 = pair_of<T2>(inv << 16 | inv);
+    const unsigned * w = reinterpret_cast<const unsigned *>(v.e);
+    unsigned c[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const unsigned x = word_of(__hmul2(pair_of<T2>(w[i]), inv2));
+        c[i] = cvt_e2m1x2(__uint_as_float(x << 16), __uint_as_float(x & 0xFFFF0000u));
+    }
+    const unsigned q = join_codes(c);
+    return sb == 255u ? 0u : q;
+}
+__device__ __forceinline__ unsigned quantize8(const Eight<__half> & v, unsigned & sb) {
+    using T2 = __half2;
+    T2 m = amax_pair<T2>(v);
+    m = __hmax2_nan(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
+    m = __hmax2_nan(m, __shfl_xor_sync(0xFFFFFFFFu, m, 2));
+    sb = scale_byte(__float_as_uint(__half2float(__hmax_nan(__low2half(m), __high2half(m)))));
+    const float inv = scale_inv(sb);
+    const unsigned * w = reinterpret_cast<const unsigned *>(v.e);
+    unsigned c[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 x = __half22float2(pair_of<T2>(w[i]));
+        c[i] = cvt_e2m1x2(x.x * inv, x.y * inv);
+    }
+    const unsigned q = join_codes(c);
     return sb == 255u ? 0u : q;
 }
 
@@ -167,6 +215,27 @@ __device__ __forceinline__ void codes_to_bf16(unsigned q, unsigned * w) {
     }
 }
 
+// Eight codes' values. In bf16 the product with the scale, a power of two, is exact (subnormals are
+// bf16's as they are f32's), or infinite as the rounded value is.
+template <class T> __device__ __forceinline__ void codes_to_values(unsigned q, unsigned b, Eight<T> & o) {
+    unsigned w[4];
+    codes_to_bf16(q, w);
+    const float s = scale_val(b);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        o.e[2 * i] = from_f32<T>(__uint_as_float(w[i] << 16) * s);
+        o.e[2 * i + 1] = from_f32<T>(__uint_as_float(w[i] & 0xFFFF0000u) * s);
+    }
+}
+template <> __device__ __forceinline__ void codes_to_values(unsigned q, unsigned b, Eight<__nv_bfloat16> & o) {
+    unsigned w[4];
+    codes_to_bf16(q, w);
+    const unsigned s = b == 255u ? 0x7FC0u : b == 0u ? 0x0040u : b << 7;
+    const __nv_bfloat162 s2 = pair_of<__nv_bfloat162>(s << 16 | s);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) reinterpret_cast<unsigned *>(o.e)[i] = word_of(__hmul2(pair_of<__nv_bfloat162>(w[i]), s2));
+}
+
 // The value of each code, eight a lane. Bound: HBM, writing y.
 template <class T, bool VEC>
 __global__ void __launch_bounds__(kQThreads) mx4_dequantize_kernel(const unsigned char * __restrict__ codes,
@@ -192,15 +261,8 @@ __global__ void __launch_bounds__(kQThreads) mx4_dequantize_kernel(const unsigne
             for (int u = 0; u < UN; ++u) {
                 const int c = (s0 + u * (int) gridDim.y) * 256 + lane * 8;
                 if (c >= K) continue;
-                const float s = scale_val(b[u]);
-                unsigned w[4];
-                codes_to_bf16(q[u], w);
                 Eight<T> o;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    o.e[2 * i] = from_f32<T>(__uint_as_float(w[i] << 16) * s);
-                    o.e[2 * i + 1] = from_f32<T>(__uint_as_float(w[i] & 0xFFFF0000u) * s);
-                }
+                codes_to_values(q[u], b[u], o);
                 T * d = y + row * ldy + c;
                 if (VEC && c + 8 <= K) {
 #pragma unroll
