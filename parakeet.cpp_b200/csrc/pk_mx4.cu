@@ -308,11 +308,11 @@ __global__ void __launch_bounds__(kQThreads) mx4_repack_kernel(const unsigned ch
 // columns of its own for its scales: they are free when the stage is.
 constexpr long long kWaitNs = 2000000000LL;             // bound on every device-side wait
 constexpr int kTM = 128;
-constexpr int kTStages = 4;
+constexpr int kTStages = 5;
 constexpr int kTThreads = 384;
 constexpr int kTEpi = 8;                                // warps of the epilogue: two for each 32 rows
-constexpr unsigned kScaleA = 1024, kScaleB = 2048;      // two atoms of A rows; two of each of two of B's
-constexpr unsigned kScaleCols = 24;                     // tensor-memory columns of a stage's scales: 8 + 16
+constexpr unsigned kScaleA = 1024;                      // two atoms of 128 rows
+constexpr unsigned kScaleCols = 16;                     // tensor-memory columns of a stage's scales: 8 + 8
 
 struct TcSmem {
     unsigned long long full[kTStages], empty[kTStages], acc_full[2], acc_empty[2], done;
@@ -348,7 +348,7 @@ __device__ __forceinline__ void issue_stage(unsigned d, unsigned a, unsigned b, 
                         cb + (j >> 1) * NA + shift, j > 0 || !fresh ? 1u : 0u);
 }
 
-template <int BN> constexpr unsigned tc_stage_bytes() { return kTM * 128u + BN * 128u + kScaleA + kScaleB; }
+template <int BN> constexpr unsigned tc_stage_bytes() { return kTM * 128u + BN * 128u + 2 * kScaleA; }
 constexpr unsigned kOutBytes = 4096;                    // an epilogue warp's 32 staged rows of 128 bytes
 template <int BN> constexpr size_t tc_smem_bytes() {
     return 1024 + (size_t) kTStages * tc_stage_bytes<BN>() + kTEpi * kOutBytes + sizeof(TcSmem);
@@ -454,8 +454,7 @@ mx4_tc_kernel(const __grid_constant__ CUtensorMap amap, const unsigned char * __
     unsigned char * out = reinterpret_cast<unsigned char *>(ring + kTStages * tc_stage_bytes<BN>());
     TcSmem & S = *reinterpret_cast<TcSmem *>(out + kTEpi * kOutBytes);
     const int warp = __shfl_sync(0xFFFFFFFFu, (int) threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-    const int chunks = scale_chunks(K), nks = chunks / 2, atoms = (N + 127) / 128;
-    const int nt = (N + BN - 1) / BN;
+    const int chunks = scale_chunks(K), nks = chunks / 2, nt = (N + BN - 1) / BN;
     const long long tiles = ((M + kTM - 1) / kTM) * nt;
 
     if (threadIdx.x == 0) {
@@ -487,19 +486,17 @@ mx4_tc_kernel(const __grid_constant__ CUtensorMap amap, const unsigned char * __
             bool ok = true;
             for (long long t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
                 const int m = (int) (t / nt), n0 = (int) (t % nt) * BN;
-                const int atom = n0 >> 7, have = min(((n0 & 127) + BN + 127) >> 7, atoms - atom);
                 const unsigned char * as = ascale + (size_t) m * chunks * 512;
-                const unsigned char * bs = wscale + (size_t) atom * chunks * 512;
+                const unsigned char * bs = wscale + (size_t) (n0 >> 7) * chunks * 512;
                 for (int ks = 0; ks < nks; ++ks, ++it) {
                     const int s = (int) (it % kTStages);
                     if (!mbar_wait(&S.empty[s], ((it / kTStages) & 1u) ^ 1u, kWaitNs, &S.err)) { ok = false; break; }
                     unsigned char * a = ring + s * tc_stage_bytes<BN>(), * b = a + kTM * 128, * sa = b + BN * 128;
-                    mbar_expect(&S.full[s], kTM * 128u + BN * 128u + kScaleA + 1024u * (unsigned) have);
+                    mbar_expect(&S.full[s], tc_stage_bytes<BN>());
                     tma_load_2d(a, &amap, ks * 128, m * kTM, &S.full[s]);
                     tma_load_2d(b, &wmap, ks * 128, n0, &S.full[s]);
                     bulk_load(sa, as + (size_t) ks * 1024, 1024, &S.full[s]);
-                    for (int j = 0; j < have; ++j)
-                        bulk_load(sa + kScaleA + j * 1024, bs + ((size_t) j * chunks + 2 * ks) * 512, 1024, &S.full[s]);
+                    bulk_load(sa + kScaleA, bs + (size_t) ks * 1024, 1024, &S.full[s]);
                 }
             }
             // nothing in flight when the block ends, however the others ended
@@ -517,7 +514,7 @@ mx4_tc_kernel(const __grid_constant__ CUtensorMap amap, const unsigned char * __
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const unsigned a = smem_u32(ring) + s * tc_stage_bytes<BN>(), b = a + kTM * 128u, sa = b + BN * 128u;
                 if (elect_one()) {
-                    issue_stage<BN, false>(tmem + buf * BN, a, b, sa, sa + kScaleA, tmem + 2 * 192 + s * kScaleCols, shift, ks == 0);
+                    issue_stage<BN, false>(tmem + buf * BN, a, b, sa, sa + kScaleA, tmem + 2 * BN + s * kScaleCols, shift, ks == 0);
                     umma_commit(&S.empty[s]);
                     if (ks == nks - 1) umma_commit(&S.acc_full[buf]);
                 }
@@ -562,6 +559,8 @@ mx4_tc_kernel(const __grid_constant__ CUtensorMap amap, const unsigned char * __
 // other SM, so a stage is 31 KB. The pair's first block issues, and both blocks' loads arrive on its
 // barrier. The scales of all BN weight rows are loaded by both, each for its own tensor memory.
 constexpr int kPStages = 5;
+constexpr unsigned kScaleB = 2048;                      // two atoms of each of two times 128 weight rows
+constexpr unsigned kPScaleCols = 24;
 template <int BN> constexpr unsigned pair_stage() { return kTM * 128u + BN / 2 * 128u + kScaleA + kScaleB; }
 // bytes that one block loads a stage
 template <int BN> constexpr unsigned pair_bytes() { return kTM * 128u + BN / 2 * 128u + kScaleA + (BN > 128 ? 2048u : 1024u); }
@@ -655,7 +654,7 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant_
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     const unsigned a = smem_u32(ring) + s * pair_stage<BN>(), b = a + kTM * 128u, sa = b + BN / 2 * 128u;
                     if (elect_one()) {
-                        issue_stage<BN, true>(tmem + buf * BN, a, b, sa, sa + kScaleA, tmem + 2 * 192 + s * kScaleCols, shift, ks == 0);
+                        issue_stage<BN, true>(tmem + buf * BN, a, b, sa, sa + kScaleA, tmem + 2 * 192 + s * kPScaleCols, shift, ks == 0);
                         umma_commit_pair(&S.empty[s]);
                         if (ks == nks - 1) umma_commit_pair(&S.acc_full[buf]);
                     }
@@ -909,15 +908,14 @@ struct pk_mx4 {
     float * bias = nullptr;
     int * err = nullptr;                // host memory that the device sees: a bounded wait ran out
     int * err_dev = nullptr;
-    alignas(64) CUtensorMap map[4];     // codes in boxes of kBox[i] rows
+    alignas(64) CUtensorMap map[3];     // codes in boxes of kBox[i] rows
     alignas(64) CUtensorMap smap[2];    // scales: the two atoms of a stage of 128 rows, of 256 rows
 };
 
 namespace pk {
 namespace {
 
-constexpr int kBN[3] = {64, 128, 192};
-constexpr int kBox[4] = {64, 128, 192, 96};   // the last: half of a pair's 192
+constexpr int kBox[3] = {64, 128, 96};   // the last: half of a pair's 192
 
 // Scale atoms as rows of words, one row for 128 rows of values; a box is a stage's two atoms of `rows`
 // such rows.
@@ -978,7 +976,7 @@ cudaError_t launch_pair_as(const Call & c, const CUtensorMap & amap, const unsig
     if (e != cudaSuccess) return e;
     const long long tiles = (c.M + 2 * kTM - 1) / (2 * kTM) * ((c.w->N + BN - 1) / BN);
     kernel<<<(unsigned) (2 * std::min<long long>(tiles, 74)), kTThreads, smem, c.s>>>(
-        amap, asmap, c.M, c.w->K, c.w->map[BN > 128 ? 3 : 0], c.w->smap[BN > 128 ? 1 : 0], c.w->N, c.w->bias, static_cast<T *>(c.y), c.ldy, ymap, c.w->err_dev);
+        amap, asmap, c.M, c.w->K, c.w->map[BN > 128 ? 2 : 0], c.w->smap[BN > 128 ? 1 : 0], c.w->N, c.w->bias, static_cast<T *>(c.y), c.ldy, ymap, c.w->err_dev);
     return cudaGetLastError();
 }
 
@@ -1005,16 +1003,12 @@ template <class TX> cudaError_t launch_few(const Call & c, int y_type) {
 
 bool few(const pk_mx4 * w, int64_t rows) { return rows <= kFewRows && w->K <= kFewK; }
 
-// Tile width: fewest rounds of tiles over the SMs, a round costed by the rows that a tile loads.
-int pick_bn(long long M, int N) {
-    int best = 0;
-    long long cost = 0;
-    for (int i = 0; i < 3; ++i) {
-        const long long tiles = (M + kTM - 1) / kTM * ((N + kBN[i] - 1) / kBN[i]);
-        const long long c = (tiles + 147) / 148 * (kTM + kBN[i]);
-        if (i == 0 || c <= cost) { best = i; cost = c; }
-    }
-    return best;
+// Tile width of the single blocks: fewest rounds of tiles over the SMs, a round costed by the rows that
+// a tile loads. (192, with fewer loads a product, was slower where K is short: 66044 x 640 x 1024 97 us
+// against 94, 16391 x 1025 44 against 41; where K is long the pairs are faster.)
+bool narrow_tiles(long long M, int N) {
+    auto cost = [&](int bn) { return ((M + kTM - 1) / kTM * ((N + bn - 1) / bn) + 147) / 148 * (kTM + bn); };
+    return cost(64) < cost(128);
 }
 
 template <class T> cudaError_t launch_product(const Call & c, int y_type, const unsigned char * xc, const unsigned char * xs) {
@@ -1032,12 +1026,9 @@ template <class T> cudaError_t launch_product(const Call & c, int y_type, const 
         if (r192 <= r128) return box ? launch_pair_as<T, 192, true>(c, amap, xs, ymap) : launch_pair_as<T, 192, false>(c, amap, xs, ymap);
         return box ? launch_pair_as<T, 128, true>(c, amap, xs, ymap) : launch_pair_as<T, 128, false>(c, amap, xs, ymap);
     }
-    const int i = pick_bn(c.M, c.w->N);
-    const CUtensorMap & wmap = c.w->map[i];
-    if (box) return i == 0 ? launch_tc_as<T, 64, true>(c, amap, xs, wmap, ymap)
-                    : i == 1 ? launch_tc_as<T, 128, true>(c, amap, xs, wmap, ymap) : launch_tc_as<T, 192, true>(c, amap, xs, wmap, ymap);
-    return i == 0 ? launch_tc_as<T, 64, false>(c, amap, xs, wmap, ymap)
-           : i == 1 ? launch_tc_as<T, 128, false>(c, amap, xs, wmap, ymap) : launch_tc_as<T, 192, false>(c, amap, xs, wmap, ymap);
+    if (narrow_tiles(c.M, c.w->N))
+        return box ? launch_tc_as<T, 64, true>(c, amap, xs, c.w->map[0], ymap) : launch_tc_as<T, 64, false>(c, amap, xs, c.w->map[0], ymap);
+    return box ? launch_tc_as<T, 128, true>(c, amap, xs, c.w->map[1], ymap) : launch_tc_as<T, 128, false>(c, amap, xs, c.w->map[1], ymap);
 }
 
 }  // namespace
@@ -1177,7 +1168,7 @@ extern "C" PK_API pk_status pk_mx4_create(int device, const pk_tensor * weight, 
     }
     if (e == cudaSuccess) w->err = take_error_word(e);
     if (e == cudaSuccess) e = cudaHostGetDevicePointer(reinterpret_cast<void **>(&w->err_dev), w->err, 0);
-    for (int i = 0; i < 4 && e == cudaSuccess; ++i)
+    for (int i = 0; i < 3 && e == cudaSuccess; ++i)
         e = encode_2d(&w->map[i], CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, w->codes, N, (long long) w->nb * 16, kBox[i], 128,
                       CU_TENSOR_MAP_SWIZZLE_128B);
     for (int i = 0; i < 2 && e == cudaSuccess; ++i) e = map_scales(&w->smap[i], w->scales, (N + 127) / 128, w->chunks, i + 1);
