@@ -15,6 +15,7 @@
 #include <algorithm>
 #include <mutex>
 #include <new>
+#include <utility>
 #include <vector>
 
 namespace pk {
@@ -171,6 +172,8 @@ __global__ void __launch_bounds__(kQThreads) mx4_quantize_kernel(const T * __res
                                                                  unsigned char * __restrict__ scales) {
     constexpr int UN = sizeof(T) == 4 ? 2 : 4;
     const int lane = threadIdx.x & 31;
+    // the product may set itself up while the last blocks work; it waits for all of them before it loads
+    if (ATOMS) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int segs = (K + 255) >> 8, nb = (K + 31) >> 5, chunks = scale_chunks(K);
     const long long stride = (long long) gridDim.x * (kQThreads / 32);
     for (long long row = (long long) blockIdx.x * (kQThreads / 32) + (threadIdx.x >> 5); row < rows; row += stride) {
@@ -484,6 +487,7 @@ mx4_tc_kernel(const __grid_constant__ CUtensorMap amap, const unsigned char * __
         if (lane == 0) {
             unsigned it = 0;
             bool ok = true;
+            asm volatile("griddepcontrol.wait;" ::: "memory");   // the rows' codes and scales are there
             for (long long t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
                 const int m = (int) (t / nt), n0 = (int) (t % nt) * BN;
                 const unsigned char * as = ascale + (size_t) m * chunks * 512;
@@ -620,6 +624,7 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant_
         if (lane == 0) {
             unsigned it = 0;
             bool ok = true;
+            asm volatile("griddepcontrol.wait;" ::: "memory");   // the rows' codes and scales are there
             for (long long t = first; t < tiles && ok; t += step) {
                 const int m = (int) (t / nt) * 2 + (int) rank, n0 = (int) (t % nt) * BN;
                 for (int ks = 0; ks < nks; ++ks, ++it) {
@@ -951,6 +956,22 @@ struct Call {
     cudaStream_t s;
 };
 
+// Launch of a product behind the quantisation of its rows, which lets it start before it has ended.
+template <class... P, class... A>
+cudaError_t launch_after(void (*kernel)(P...), unsigned grid, size_t smem, cudaStream_t s, A &&... args) {
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute at[1];
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(kTThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, std::forward<A>(args)...);
+}
+
 template <class T, int BN, bool BOX>
 cudaError_t launch_tc_as(const Call & c, const CUtensorMap & amap, const unsigned char * xs, const CUtensorMap & wmap, const CUtensorMap & ymap) {
     auto kernel = mx4_tc_kernel<T, BN, BOX>;
@@ -959,9 +980,8 @@ cudaError_t launch_tc_as(const Call & c, const CUtensorMap & amap, const unsigne
     const cudaError_t e = allow_smem(kernel, smem, c.w->device, set);
     if (e != cudaSuccess) return e;
     const long long tiles = (c.M + kTM - 1) / kTM * ((c.w->N + BN - 1) / BN);
-    kernel<<<(unsigned) std::min<long long>(tiles, 148), kTThreads, smem, c.s>>>(
+    return launch_after(kernel, (unsigned) std::min<long long>(tiles, 148), smem, c.s,
         amap, xs, c.M, c.w->K, wmap, c.w->scales, c.w->N, c.w->bias, static_cast<T *>(c.y), c.ldy, ymap, c.w->err_dev);
-    return cudaGetLastError();
 }
 
 template <class T, int BN, bool BOX>
@@ -975,9 +995,8 @@ cudaError_t launch_pair_as(const Call & c, const CUtensorMap & amap, const unsig
     e = allow_smem(kernel, smem, c.w->device, set);
     if (e != cudaSuccess) return e;
     const long long tiles = (c.M + 2 * kTM - 1) / (2 * kTM) * ((c.w->N + BN - 1) / BN);
-    kernel<<<(unsigned) (2 * std::min<long long>(tiles, 74)), kTThreads, smem, c.s>>>(
+    return launch_after(kernel, (unsigned) (2 * std::min<long long>(tiles, 74)), smem, c.s,
         amap, asmap, c.M, c.w->K, c.w->map[BN > 128 ? 2 : 0], c.w->smap[BN > 128 ? 1 : 0], c.w->N, c.w->bias, static_cast<T *>(c.y), c.ldy, ymap, c.w->err_dev);
-    return cudaGetLastError();
 }
 
 template <class TX, class TY, bool VEC>
