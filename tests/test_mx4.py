@@ -196,6 +196,57 @@ def test_quantize_borders(built):
     assert np.array_equal(scales[:x.shape[0] * 2].view(-1, 2).cpu().numpy(), byte)
 
 
+@pytest.mark.gpu
+def test_values_at_the_ends(built):
+    """Every code at every scale byte, in each type: subnormal, infinite and NaN values as rounding the
+    exact value gives them; and back to the same bytes from bf16 where the block's largest code says so."""
+    import torch
+    pk = built
+    byte = np.arange(256, dtype=np.uint8)
+    code = np.tile(np.arange(16, dtype=np.uint8), (256, 2))                    # 32 values a row
+    codes = torch.from_numpy(pack(code, 1)).cuda()
+    scales = torch.from_numpy(byte).cuda()
+    val = np.where(code & 8, -1.0, 1.0) * GRID[code & 7] * np.exp2(byte.astype(np.float64) - 127)[:, None]
+    val[255] = np.nan
+    s = torch.cuda.current_stream().cuda_stream
+    for name, t in (("f32", torch.float32), ("f16", torch.float16), ("bf16", torch.bfloat16)):
+        out = torch.empty(256, 32, dtype=t, device="cuda")
+        pk.mx4_dequantize(codes.data_ptr(), scales.data_ptr(), 256, 32, out.data_ptr(), dtype=name, stream=s)
+        want = torch.from_numpy(val).to(t).float().numpy()
+        assert np.array_equal(out.float().cpu().numpy(), want, equal_nan=True), name
+    # bf16 holds every one of them below 2^126 x 4: quantised again they keep codes and bytes (a block's
+    # largest code is 6, so its exponent is the byte's; byte 0 and 1 both end at 2^-127)
+    keep = byte[2:252]
+    x = torch.from_numpy(val[2:252]).to(torch.bfloat16).cuda()
+    c2 = torch.empty(250, 16, dtype=torch.uint8, device="cuda")
+    s2 = torch.empty(250, dtype=torch.uint8, device="cuda")
+    pk.mx4_quantize(x.data_ptr(), 250, 32, c2.data_ptr(), s2.data_ptr(), dtype="bf16", stream=s)
+    assert np.array_equal(s2.cpu().numpy(), keep) and np.array_equal(c2.cpu().numpy(), pack(code[2:252], 1))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_quantize_half_precision_borders(built, dtype):
+    """All magnitudes of half precision of six binades under one block maximum of four, at several scales."""
+    import torch
+    pk = built
+    t = torch.bfloat16 if dtype == "bf16" else torch.float16
+    step = 2.0 ** -7 if dtype == "bf16" else 2.0 ** -10
+    m = np.concatenate([(1 + np.arange(0, 1, step)) * 2.0 ** e for e in range(-4, 3)])
+    m = m[m <= 7.99]
+    n = -(-len(m) // 31) * 31
+    m = np.concatenate([m, np.zeros(n - len(m))]).reshape(-1, 31)
+    x = np.concatenate([np.full((len(m), 1), 4.0), m], 1)
+    x = np.concatenate([x, -x])
+    for e in ((-126, -30, 0, 100) if dtype == "bf16" else (-10, 0, 10)):
+        seen, codes, scales = run_quantize(pk, np.ldexp(x, e), dtype)
+        code, byte, _ = ref_quantize(seen)
+        r = len(x)
+        assert np.array_equal(codes[:r * 16].view(r, -1).cpu().numpy(), pack(code, 1))
+        assert np.array_equal(scales[:r].view(r, 1).cpu().numpy(), byte)
+    assert t is not None
+
+
 def product(pk, w, x, bias=None, x_dtype="f32", y_dtype="f32", xpad=0, ypad=0, shift=0, layer=None, stream=None):
     import torch
     r, k = x.shape
@@ -388,3 +439,34 @@ def test_rows_do_not_depend_on_the_batch(built):
         check_product(ref_quantize(w)[2], seen, y)
         assert np.array_equal(y, product(pk, w, x[:r], layer=layer)[1])
     assert torch.cuda.current_device() == 0
+
+
+@pytest.mark.gpu
+def test_first_call_may_be_captured(built):
+    """A process whose first product and first draw are captured into a graph."""
+    import subprocess
+    import sys
+    code = """
+import importlib.util, sys, torch
+spec = importlib.util.spec_from_file_location("parakeet_b200", sys.argv[1] + "/__init__.py", submodule_search_locations=[sys.argv[1]])
+pk = importlib.util.module_from_spec(spec); sys.modules["parakeet_b200"] = pk; spec.loader.exec_module(pk)
+w = torch.randn(200, 2100, device="cuda")
+layer = pk.Mx4Linear(w.data_ptr(), 200, 2100, on_device=True)
+x = torch.randn(300, 2100, device="cuda"); y = torch.zeros(300, 200, device="cuda")
+u = torch.rand(300, device="cuda"); tok = torch.full((300,), -5, dtype=torch.int32, device="cuda")
+ws = torch.empty(layer.workspace(300), dtype=torch.uint8, device="cuda")
+g = torch.cuda.CUDAGraph(); torch.cuda.synchronize()
+with torch.cuda.graph(g):
+    s = torch.cuda.current_stream().cuda_stream
+    layer.forward(x.data_ptr(), 300, y.data_ptr(), workspace=ws.data_ptr(), workspace_bytes=ws.numel(), stream=s)
+    pk.sample(y.data_ptr(), 300, 200, u.data_ptr(), tok.data_ptr(), top_p=0.9, stream=s)
+g.replay(); torch.cuda.synchronize()
+a, b = y.clone(), tok.clone()
+layer.forward(x.data_ptr(), 300, y.data_ptr(), workspace=ws.data_ptr(), workspace_bytes=ws.numel())
+pk.sample(y.data_ptr(), 300, 200, u.data_ptr(), tok.data_ptr(), top_p=0.9)
+torch.cuda.synchronize()
+assert torch.equal(a, y) and torch.equal(b, tok) and (tok >= 0).all()
+print("same")
+"""
+    r = subprocess.run([sys.executable, "-c", code, built.PKG_DIR], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "same" in r.stdout, r.stderr[-2000:]

@@ -357,6 +357,49 @@ def test_captured_and_replayed(built, v):
         check(a, b, tok.cpu().numpy(), lp.cpu().numpy(), temperature=0.8, top_k=40, top_p=0.95)
 
 
+@pytest.mark.gpu
+def test_two_streams_at_once(built):
+    """Calls that overlap on two streams, large and small, draw what they draw alone."""
+    import torch
+    pk = built
+    rng = np.random.default_rng(12)
+    jobs = []
+    for r, v, kw in ((3, 70000, dict(top_p=0.9)), (700, 1025, dict()), (40, 9000, dict(top_k=300, top_p=0.8)), (2000, 300, dict(top_k=5))):
+        l = torch.from_numpy(rng.standard_normal((r, v)).astype(np.float32) * 2).cuda()
+        u = torch.from_numpy(rng.random(r).astype(np.float32)).cuda()
+        alone = torch.empty(r, dtype=torch.int32, device="cuda")
+        pk.sample(l.data_ptr(), r, v, u.data_ptr(), alone.data_ptr(), **kw)       # the default stream
+        jobs.append((l, u, alone, torch.empty_like(alone), kw))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for n in range(6):
+        for i, (l, u, alone, out, kw) in enumerate(jobs):
+            out.fill_(-9)
+        torch.cuda.synchronize()
+        for i, (l, u, alone, out, kw) in enumerate(jobs):
+            pk.sample(l.data_ptr(), l.shape[0], l.shape[1], u.data_ptr(), out.data_ptr(), stream=streams[(i + n) % 2].cuda_stream, **kw)
+        torch.cuda.synchronize()
+        assert all(torch.equal(alone, out) for _, _, alone, out, _ in jobs)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("r", [600, 3])
+def test_values_too_close_for_a_bin(built, r):
+    """More equal and all but equal logits than a list takes, down to the smallest numbers: every level of
+    the histogram has to part them."""
+    tiny = np.float32(1.401298464e-45)
+    rng = np.random.default_rng(1)
+    v = 3000
+    rows = [np.where(rng.random(v) < 0.5, tiny, 0.0), rng.integers(0, 5, v) * tiny, np.float32(1.0) + rng.integers(0, 3, v) * np.float32(2 ** -23),
+            np.where(rng.random(v) < 0.5, 3.4028235e38, 3.4028233e38), -np.abs(rng.standard_normal(v)) * np.float32(1e-38),
+            np.where(np.arange(v) % 2, 0.0, -tiny)]
+    l = np.array(rows)[np.arange(r) % len(rows)].astype(np.float32)
+    u = rng.random(r).astype(np.float32)
+    for kw in (dict(top_k=700), dict(top_p=0.37), dict(top_k=1600, top_p=0.9), dict(top_k=1600, top_p=0.9, temperature=1e-30)):
+        seen, tok, lp = run(built, l, u, **kw)
+        check(seen, u, tok, lp, **kw)
+
+
 def collapse(path, blank, prev):
     toks, frs = [], []
     for t, x in enumerate(path):
