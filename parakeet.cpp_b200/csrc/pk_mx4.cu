@@ -908,9 +908,9 @@ constexpr int64_t kMaxRows = 0x7FFFFFFF;
 struct pk_mx4 {
     int device = 0;
     int N = 0, K = 0, nb = 0, chunks = 0;
-    unsigned char * codes = nullptr;    // [N][16 nb]
+    unsigned char * codes = nullptr;    // [N][16 nb]; owns the memory of all three
     unsigned char * scales = nullptr;   // atoms
-    float * bias = nullptr;
+    float * bias = nullptr;             // padded to whole tiles, or null
     int * err = nullptr;                // host memory that the device sees: a bounded wait ran out
     int * err_dev = nullptr;
     alignas(64) CUtensorMap map[3];     // codes in boxes of kBox[i] rows
@@ -1121,8 +1121,6 @@ extern "C" PK_API void pk_mx4_destroy(pk_mx4 * w) {
     DeviceScope dev(w->device);
     cudaDeviceSynchronize();
     cudaFree(w->codes);
-    cudaFree(w->scales);
-    cudaFree(w->bias);
     if (w->err) give_error_word(w->err);
     delete w;
 }
@@ -1153,15 +1151,17 @@ extern "C" PK_API pk_status pk_mx4_create(int device, const pk_tensor * weight, 
     w->K = (int) K;
     w->nb = (int) ((K + 31) / 32);
     w->chunks = scale_chunks((int) K);
-    const size_t code_bytes = (size_t) N * w->nb * 16, scale_bytes = (size_t) ((N + 127) / 128) * w->chunks * 512;
+    const size_t code_bytes = ((size_t) N * w->nb * 16 + 511) / 512 * 512, scale_bytes = (size_t) ((N + 127) / 128) * w->chunks * 512;
     void * raw = nullptr;    // a host weight's copy
     void * f32 = nullptr;    // q8_0 blocks dequantised
-    cudaStream_t s = nullptr;
+    const cudaStream_t s = cudaStreamPerThread;
     cudaError_t e = on_device ? cudaDeviceSynchronize() : cudaSuccess;
-    if (e == cudaSuccess) e = cudaStreamCreateWithFlags(&s, cudaStreamNonBlocking);
-    if (e == cudaSuccess) e = cudaMalloc(&w->codes, code_bytes);
-    if (e == cudaSuccess) e = cudaMalloc(&w->scales, scale_bytes);
-    if (e == cudaSuccess) e = cudaMemsetAsync(w->scales, 0, scale_bytes, s);
+    if (e == cudaSuccess) e = cudaMalloc(&w->codes, code_bytes + scale_bytes + (bias ? (size_t) (N + 255) / 64 * 64 * 4 : 0));
+    if (e == cudaSuccess) {
+        w->scales = w->codes + code_bytes;
+        if (bias) w->bias = reinterpret_cast<float *>(w->scales + scale_bytes);
+        e = cudaMemsetAsync(w->scales, 0, scale_bytes, s);
+    }
     const void * src = weight->data;
     if (e == cudaSuccess && !on_device) {
         e = cudaMalloc(&raw, want);
@@ -1180,22 +1180,16 @@ extern "C" PK_API pk_status pk_mx4_create(int device, const pk_tensor * weight, 
     } else if (e == cudaSuccess) {
         e = launch_quantize<true>(src, type, N, (int) K, K, w->codes, w->scales, s);
     }
-    if (e == cudaSuccess && bias) {
-        e = cudaMalloc(&w->bias, (size_t) (N + 255) / 64 * 64 * 4);      // read in whole tiles
-        if (e == cudaSuccess)
-            e = cudaMemcpyAsync(w->bias, bias, (size_t) N * 4, on_device ? cudaMemcpyDeviceToDevice : cudaMemcpyHostToDevice, s);
-    }
+    if (e == cudaSuccess && bias)
+        e = cudaMemcpyAsync(w->bias, bias, (size_t) N * 4, on_device ? cudaMemcpyDeviceToDevice : cudaMemcpyHostToDevice, s);
     if (e == cudaSuccess) w->err = take_error_word(e);
     if (e == cudaSuccess) e = cudaHostGetDevicePointer(reinterpret_cast<void **>(&w->err_dev), w->err, 0);
     for (int i = 0; i < 3 && e == cudaSuccess; ++i)
         e = encode_2d(&w->map[i], CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, w->codes, N, (long long) w->nb * 16, kBox[i], 128,
                       CU_TENSOR_MAP_SWIZZLE_128B);
     for (int i = 0; i < 2 && e == cudaSuccess; ++i) e = map_scales(&w->smap[i], w->scales, (N + 127) / 128, w->chunks, i + 1);
-    if (s) {
-        const cudaError_t e2 = cudaStreamSynchronize(s);
-        if (e == cudaSuccess) e = e2;
-        cudaStreamDestroy(s);
-    }
+    const cudaError_t e2 = cudaStreamSynchronize(s);
+    if (e == cudaSuccess) e = e2;
     cudaFree(raw);
     cudaFree(f32);
     if (e != cudaSuccess) {

@@ -661,24 +661,40 @@ __device__ void draw_listed(Team<NT, CL> & team, TeamBins<NT> * B, const Pair * 
 // two more: 13 S 2^-24. The runs are added in f64. Together below 2^-18 S = E for every prefix and for
 // S, so u S is off by as much: the token is settled if the border before it and the one behind are each
 // more than 2 E (2.5 E, against what is left) from u S.
-template <class T, bool RES>
-__device__ __forceinline__ bool draw_f32(const Slice<T, RES> & l, int len, int lane, float hi, float temp, float u, const pk_sample_args & a,
-                                         long long row) {
-    const float inv_t = 1.0f / temp, c = 1.4426950408889634f * inv_t, k = hi * c;
-    if (!(c > 1e-30f && c < 1e30f && fabsf(k) < 1e6f)) return false;
-    auto weight = [&](float v) {                         // 0 for -infinity; a NaN ends in the sum
+struct Row32 {
+    float inv_t, c, k, hi;
+    bool fine;            // no product is NaN or far from what the bound assumes
+    __device__ __forceinline__ Row32(float top, float temp) {
+        inv_t = 1.0f / temp;
+        c = 1.4426950408889634f * inv_t;
+        k = top * c;
+        hi = top;
+        fine = c > 1e-30f && c < 1e30f && fabsf(k) < 1e6f;
+    }
+    __device__ __forceinline__ float weight(float v) const {     // 0 for -infinity; a NaN ends in the sum
         float w;
         asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w) : "f"(fmaf(v, c, -k)));
         return w;
-    };
+    }
+    __device__ __forceinline__ float logprob(float v, double total) const {
+        const double off = (double) k - (double) hi * (double) c;   // every weight is 2^-off of what it should be
+        return (float) ((double) (v - hi) * (double) inv_t - 0.6931471805599453 * off - (double) logf((float) total));
+    }
+};
+
+template <class T, bool RES>
+__device__ __forceinline__ bool draw_f32(const Slice<T, RES> & l, int len, int lane, float hi, float temp, float u, const pk_sample_args & a,
+                                         long long row) {
+    const Row32 r(hi, temp);
+    if (!r.fine) return false;
     const int i0 = lane * len;
     float part[4] = {};
     int j = 0;
     for (; j + 4 <= len; j += 4) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) part[q] += weight(l(i0 + j + q));
+        for (int q = 0; q < 4; ++q) part[q] += r.weight(l(i0 + j + q));
     }
-    for (; j < len; ++j) part[0] += weight(l(i0 + j));
+    for (; j < len; ++j) part[0] += r.weight(l(i0 + j));
     const double sum = (double) ((part[0] + part[1]) + (part[2] + part[3]));
     const double upto = warp_scan(sum, lane), total = __shfl_sync(kFull, upto, 31);
     if (!(total < 1e30)) return false;
@@ -692,7 +708,7 @@ __device__ __forceinline__ bool draw_f32(const Slice<T, RES> & l, int len, int l
     const int e = min((who + 1) * len, l.n);
     for (int b = who * len; b < e; b += 32) {
         const int i = b + lane;
-        const float v = i < e ? l(i) : -CUDART_INF_F, w = weight(v);
+        const float v = i < e ? l(i) : -CUDART_INF_F, w = r.weight(v);
         const double end = run + warp_scan((double) w, lane);
         const unsigned beyond = __ballot_sync(kFull, end > t);
         if (beyond != 0) {
@@ -700,15 +716,198 @@ __device__ __forceinline__ bool draw_f32(const Slice<T, RES> & l, int len, int l
             const bool sure = mine && i < e && end - t > margin && (t - (end - (double) w) > margin);
             if (sure) {
                 a.tokens[row] = i;
-                const double off = (double) k - (double) hi * (double) c;   // every weight is 2^-off of what it should be
-                if (a.logprobs)
-                    a.logprobs[row] = (float) ((double) (v - hi) * (double) inv_t - 0.6931471805599453 * off - (double) logf((float) total));
+                if (a.logprobs) a.logprobs[row] = r.logprob(v, total);
             }
             return __any_sync(kFull, sure);
         }
         run = __shfl_sync(kFull, end, 31);
     }
     return false;
+}
+
+// Top-p by f32 sums, for a block's row with nothing cut by k: what they can tell, with bounds as above.
+//
+// One pass sums all weights and counts the tokens of each bin. A bin's weight lies between its count times
+// the weights at its two edges, so the bins in which the sum over falling logits may reach the share p
+// are known; a second pass sums what lies above them and lists their tokens, and the cut is read from
+// the list's ranks. A third pass draws. For V <= 16384 a sum of f32 weights is off by less than
+// S 2^-24 (8 + 2.78 * 14 + 19) < 70 2^-24 S = E (19: the additions of a thread's quarter); sums are
+// joined as integers of 2^-40. A step that a sum within 2.5 E of its border decides is left to the f64
+// sums (some 3 rows in 100 of 8193 logits).
+enum { kNothing = 0, kCut = 1, kDrawn = 2 };
+constexpr double kOff = 70.0 * 0x1p-24;
+constexpr double kFix = 1099511627776.0;        // 2^40
+
+template <class T, int NT>
+__device__ int nucleus_f32(Team<NT, false> & team, TeamBins<NT> * B, const Slice<T, true> & l, int len, float hi, float low, float temp,
+                           float least, float p, float u, const pk_sample_args & a, long long row, float & cut, u64 & ties, bool & partial) {
+    constexpr int NB = bins_of<NT>(), PER = NB / NT;
+    TeamSmem<NT> * s = team.s;
+    const Row32 r(hi, temp);
+    if (!(r.fine && p > 0.0f)) return kNothing;
+    // tokens of less than (1 - p) / V of the largest weight cannot be at the cut, see below
+    const float tail = 0.5f * (1.0f - p) / (float) a.vocab;
+    const float from = fmaxf(low, hi + 0.6931f * log2f(fmaxf(tail, 1e-13f)) * temp * 1.001f);
+    if (!(from < hi)) return kNothing;
+    Level L;
+    L.range(hi, from, NB);
+    if (L.half != 1.0f || !(L.inv < 1e30f)) return kNothing;
+    for (int b = team.tid; b < NB; b += NT) B->sum[b].x = 0;
+    if (team.tid == 0) { s->found = NB - 1; s->found_ties = NB - 1; s->listed = 0; }
+    team.sync();
+    float part[4] = {};
+    l.template quads<NT>(team.tid, [&](float4 v, int) {
+        auto one = [&](float x, float & sum) {
+            sum += r.weight(x);
+            if (x >= from) atomicAdd(&B->sum[L.bin_of<NB>(x)].x, 1u);
+        };
+        one(v.x, part[0]);
+        one(v.y, part[1]);
+        one(v.z, part[2]);
+        one(v.w, part[3]);
+    });
+    auto fixed = [](float w) { return (u64) __double2ull_rn((double) w * kFix); };
+    const float mine = (part[0] + part[1]) + (part[2] + part[3]);
+    // a NaN or an overflow shows in every sum it enters; weights are at most about one each
+    const u64 total = team.sum(mine < 1e6f ? fixed(mine) : 1ull << 62);
+    if (total >= 1ull << 58) return kNothing;
+    const double S = (double) total, E = S * kOff;
+    // bounds of what the bins hold, and the first that may and the first that must reach the share
+    const float width = (hi - from) / (float) NB;
+    // in units of 2^-29 of the sum, rounded outwards, the upper bound in the high word
+    const float unit = (float) (kFix * 536870912.0 / S);
+    u64 bound[PER], sum_bound = 0;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        const int b = team.tid * PER + j;
+        const float n = (float) B->sum[b].x * unit;
+        // the edges moved out by more than bin_of's rounding
+        const float up = n * r.weight(hi - ((float) b - 0.01f) * width) * 1.0001f, down = n * r.weight(hi - ((float) b + 1.01f) * width) * 0.9999f;
+        bound[j] = n > 0.0f ? (u64) (__float2uint_ru(fminf(up, 1e9f))) << 32 | __float2uint_rd(fminf(down, 1e9f)) : 0ull;
+        sum_bound += bound[j];
+    }
+    u64 all;
+    u64 before = team.scan(sum_bound, all);
+    const unsigned need_lo = (unsigned) max(1.0, (double) p * 536870912.0 * (1.0 - kOff)), need_hi = (unsigned) ((double) p * 536870912.0 * (1.0 + kOff)) + 2;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        const u64 upto = before + bound[j];
+        if ((unsigned) (before >> 32) < need_lo && need_lo <= (unsigned) (upto >> 32)) s->found = team.tid * PER + j;
+        if ((unsigned) before < need_hi && need_hi <= (unsigned) upto) s->found_ties = team.tid * PER + j;
+        before = upto;
+    }
+    team.sync();
+    const int b1 = s->found, b2 = s->found_ties;
+    // down to `sure` a token lies above those bins, down to `reach` it goes on the list
+    const float reach = fmaxf(from, hi - ((float) b2 + 1.01f) * width), sure = hi - ((float) b1 - 0.02f) * width;
+    float above[4] = {};
+    l.template quads<NT>(team.tid, [&](float4 v, int i) {
+        const float top4 = fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w));
+        if (!__any_sync(kFull, top4 >= reach)) return;
+        auto one = [&](float x, float & sum) {
+            const float w = r.weight(x);
+            if (x >= sure) sum += w;
+            return x >= reach && x < sure;
+        };
+        const bool bx = one(v.x, above[0]), by = one(v.y, above[1]), bz = one(v.z, above[2]), bw = one(v.w, above[3]);
+        if (bx || by || bz || bw) {
+            int n = atomicAdd(&s->listed, (int) bx + (int) by + (int) bz + (int) bw);
+            if (bx && n < kList) B->list[n] = Pair{v.x, i};
+            n += bx;
+            if (by && n < kList) B->list[n] = Pair{v.y, i + 1};
+            n += by;
+            if (bz && n < kList) B->list[n] = Pair{v.z, i + 2};
+            n += bz;
+            if (bw && n < kList) B->list[n] = Pair{v.w, i + 3};
+        }
+    });
+    const u64 over0 = team.sum(fixed((above[0] + above[1]) + (above[2] + above[3])));
+    team.sync();
+    const int n = s->listed;
+    if (team.tid == 0) s->found = kNothing;
+    team.sync();
+    if (team.tid == 0) s->listed = 0;
+    if (n > kList) return kNothing;
+    for (int j = team.tid; j < kList; j += NT) B->w[j] = j < n ? max(fixed(r.weight(B->list[j].v)), 1ull) : 0ull;
+    team.sync();
+    const double want = (double) p * S, margin = 2.5 * E;
+    over_list<NT, Around>(team.tid, n,
+        [&](Around & x, int j, int i) {
+            const float o = B->list[i].v, v = B->list[j].v;
+            if (o > v) x.over += B->w[i];
+            if (o == v) x.same += B->w[i];
+        },
+        [&](int j, const Around & x, int) {
+            const u64 w = B->w[j], over = over0 + x.over;
+            if ((double) over < want && want <= (double) (over + x.same)) {
+                const u64 t = (u64) ceil((want - (double) over) / (double) w);
+                // without its last tie the sum falls short, with it it does not, whatever f32 is off by
+                if (t >= 1 && t * w <= x.same && (double) (over + (t - 1) * w) + margin < want && (double) (over + t * w) - margin > want) {
+                    s->cut = B->list[j].v;
+                    s->cut_ties = t;
+                    s->cut_partial = t * w < x.same;
+                    s->found = kCut;
+                }
+            }
+        });
+    team.sync();
+    const int state = s->found;
+    if (state == kCut) {
+        cut = s->cut;
+        ties = s->cut_ties;
+        partial = s->cut_partial != 0;
+    }
+    team.sync();
+    if (state != kCut || partial) return state;
+    // the draw, over runs of consecutive indices
+    const float keep = fmaxf(least, cut);
+    const int i0 = team.tid * len;
+    float run[4] = {};
+    int j = 0;
+    auto kept = [&](int i) {
+        const float v = l(i);
+        return v >= keep ? r.weight(v) : 0.0f;
+    };
+    for (; j + 4 <= len; j += 4) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) run[q] += kept(i0 + j + q);
+    }
+    for (; j < len; ++j) run[0] += kept(i0 + j);
+    const u64 sum = fixed((run[0] + run[1]) + (run[2] + run[3]));
+    u64 S2 = 0;
+    before = team.scan(sum, S2);
+    const u64 t = place_of(u, S2), edge = (u64) ((double) S2 * (2.5 * kOff)) + 1;
+    if (team.tid == 0) s->found = -1;
+    team.sync();
+    if (before <= t && t < before + sum) {
+        s->found = team.tid;
+        s->found_before = before;
+    }
+    team.sync();
+    const int who = s->found;
+    team.sync();
+    if (team.tid == 0) s->found = kCut;
+    team.sync();
+    if (who >= 0 && team.tid < 32) {
+        const int e = min((who + 1) * len, l.n);
+        u64 at = s->found_before;
+        for (int b = who * len; b < e; b += 32) {
+            const int i = b + team.tid;
+            const u64 w = i < e ? fixed(kept(i)) : 0ull;
+            const u64 end = at + warp_scan(w, team.tid);
+            if (end - w <= t && t < end && end - t > edge && t - (end - w) >= edge) {
+                a.tokens[row] = i;
+                if (a.logprobs) a.logprobs[row] = r.logprob(l(i), (double) S2 * (1.0 / kFix));
+                s->found = kDrawn;
+            }
+            at = __shfl_sync(kFull, end, 31);
+            if (at > t) break;
+        }
+    }
+    team.sync();
+    const int done = s->found;
+    team.sync();
+    return done;
 }
 
 template <class T, int NT, bool FILTERS, bool CL, bool RES>
@@ -825,7 +1024,16 @@ sample_kernel(pk_sample_args a, int slice, int teams, int row_floats) {
                 cut = find_cut<false, T, NT, CL, RES>(team, bins, l, r, L, need, ties, partial);
             }
         }
-        if (!(p >= 1.0f)) {
+        int known = kNothing;
+        // With many rows; a single one is sooner through the f64 sums, which take fewer steps one after another
+        // (64 rows of 8193, each with its own settings: 16 us against 19).
+        if constexpr (RES && !CL && (NT == 128 || NT == 256)) {
+            if (!(p >= 1.0f) && !(cut > -CUDART_INF_F) && a.vocab <= 16384) {
+                known = nucleus_f32<T, NT>(team, bins, l, len, hi, low, temp_f, least, p, a.uniforms[row], a, row, cut, ties, partial);
+                if (known == kDrawn) return;
+            }
+        }
+        if (!(p >= 1.0f) && known == kNothing) {
             Share share;
             share.p = p > 0.0f ? (double) p : 0.0;
             share.from = low;
