@@ -532,9 +532,11 @@ PK_API pk_status pk_mx4_linear(pk_mx4 * w, const void * x, int32_t x_type, int64
  * k <= 0, p >= 1 and m <= 0 each turn their filter off; p <= 0 (or NaN) and m >= 1 leave the
  * largest. T <= 0 or NaN: the first index of the largest logit, log-probability 0. A row
  * without any logit above -infinity gets token -1 and log-probability -infinity. u is
- * clamped to [0, 1), NaN to 0. Weights are held in 64-bit fixed point (2^-43 of the
- * largest, exponentials in 64-bit floating point), so sums are exact, the same whatever
- * the batch, and tokens with less than 2^-44 of the largest weight are never drawn. */
+ * clamped to [0, 1), NaN to 0. Weights count in 64-bit fixed point (2^-43 of the largest,
+ * exponentials in 64-bit floating point), so the token is the same whatever the batch, and
+ * tokens with less than 2^-44 of the largest weight are never drawn. Where 32-bit sums with
+ * a proven bound tell the token they are used instead: it is the same one, and the
+ * log-probability is then within 2^-17, mostly 2^-23, of its value. */
 #define PK_SAMPLE_MAX_VOCAB 524288
 
 typedef struct pk_sample_args {
