@@ -307,19 +307,21 @@ __global__ void __launch_bounds__(kQThreads) mx4_repack_kernel(const unsigned ch
 // tcgen05.mma kind::mxf4 with block scales: 64 values of K a product, accumulator in tensor memory.
 // One persistent CTA an SM walks over 128 x BN tiles of y. Warp 0 loads (codes by TMA, 256 values =
 // one 128-byte swizzled row a stage; scale atoms by bulk copies), warp 1 copies the stage's scales to
-// tensor memory and issues its four products, warps 4-11 empty the accumulator, of which there are
+// tensor memory and issues its four products, warps from 4 on empty the accumulator, of which there are
 // two, so that a tile's epilogue runs under the next tile's products. Each stage has tensor-memory
 // columns of its own for its scales: they are free when the stage is.
 constexpr long long kWaitNs = 2000000000LL;             // bound on every device-side wait
 constexpr int kTM = 128;
-constexpr int kTStages = 5;
-constexpr int kTThreads = 384;
-constexpr int kTEpi = 8;                                // warps of the epilogue: two for each 32 rows
+template <bool BOX> constexpr int tc_stages() { return BOX ? 5 : 4; }
+// Warps of the epilogue, for each 32 rows two where TMA stores y and four where the warps do (16391 x 1025:
+// 37 us against 41 with two; 66044 x 640 by TMA: 92 us against 99 with four).
+template <bool BOX> constexpr int epi_warps() { return BOX ? 8 : 16; }
+template <bool BOX> constexpr int tc_threads() { return 32 * (4 + epi_warps<BOX>()); }
 constexpr unsigned kScaleA = 1024;                      // two atoms of 128 rows
 constexpr unsigned kScaleCols = 16;                     // tensor-memory columns of a stage's scales: 8 + 8
 
 struct TcSmem {
-    unsigned long long full[kTStages], empty[kTStages], acc_full[2], acc_empty[2], done;
+    unsigned long long full[5], empty[5], acc_full[2], acc_empty[2], done;
     unsigned tmem;
     int err;
 };
@@ -354,8 +356,8 @@ __device__ __forceinline__ void issue_stage(unsigned d, unsigned a, unsigned b, 
 
 template <int BN> constexpr unsigned tc_stage_bytes() { return kTM * 128u + BN * 128u + 2 * kScaleA; }
 constexpr unsigned kOutBytes = 4096;                    // an epilogue warp's 32 staged rows of 128 bytes
-template <int BN> constexpr size_t tc_smem_bytes() {
-    return 1024 + (size_t) kTStages * tc_stage_bytes<BN>() + kTEpi * kOutBytes + sizeof(TcSmem);
+template <int BN, bool BOX> constexpr size_t tc_smem_bytes() {
+    return 1024 + (size_t) tc_stages<BOX>() * tc_stage_bytes<BN>() + epi_warps<BOX>() * kOutBytes + sizeof(TcSmem);
 }
 
 // Wait with a bound and nothing else to end it: for copies in flight before an early exit.
@@ -366,7 +368,7 @@ __device__ __forceinline__ void mbar_drain(unsigned long long * b, unsigned pari
     while (!mbar_test(b, parity) && (long long) (now - t0) <= kWaitNs) asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
 }
 
-// A warp's 32 rows of an accumulator to y, every other 128 bytes of them (`half`), through shared
+// A warp's 32 rows of an accumulator to y, 128 bytes of them in every STEP (the `half`-th), through shared
 // memory. BOX: staged as the 128-byte swizzle has it and stored by TMA, which leaves out what lies past
 // M or N; otherwise by the warp, a row's values together.
 template <class T> constexpr int store_cols() { return 128 / (int) sizeof(T); }
@@ -377,13 +379,13 @@ __device__ __forceinline__ void box_store(const CUtensorMap * map, int n, long l
     asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
 
-template <class T, int BN, bool BOX>
+template <class T, int BN, bool BOX, int STEP>
 __device__ __forceinline__ void store_tile(unsigned acc, unsigned char * st, int half, int lane, long long m0, int rows, int n0, int N,
                                            const float * __restrict__ bias, T * __restrict__ y, long long ldy, const CUtensorMap * ymap) {
     if constexpr (BOX) {
         constexpr int COLS = store_cols<T>(), PARTS = COLS / 32;
 #pragma unroll 1
-        for (int c = half * COLS; c < BN && n0 + c < N; c += 2 * COLS) {
+        for (int c = half * COLS; c < BN && n0 + c < N; c += STEP * COLS) {
             if (rows <= 0) break;
             if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
             __syncwarp();
@@ -425,7 +427,7 @@ __device__ __forceinline__ void store_tile(unsigned acc, unsigned char * st, int
     } else {
         float * sf = reinterpret_cast<float *>(st);      // value i of row r at place i ^ r of the row
 #pragma unroll 1
-        for (int c = half * 32; c < BN && n0 + c < N; c += 64) {
+        for (int c = half * 32; c < BN && n0 + c < N; c += STEP * 32) {
             unsigned v[32];
             tmem_load32(acc + c, v);
             const int n = n0 + c + lane;
@@ -449,26 +451,27 @@ __device__ __forceinline__ void store_tile(unsigned acc, unsigned char * st, int
 }
 
 template <class T, int BN, bool BOX>
-__global__ void __launch_bounds__(kTThreads, 1)
+__global__ void __launch_bounds__(tc_threads<BOX>(), 1)
 mx4_tc_kernel(const __grid_constant__ CUtensorMap amap, const unsigned char * __restrict__ ascale, long long M, int K,
               const __grid_constant__ CUtensorMap wmap, const unsigned char * __restrict__ wscale, int N,
               const float * __restrict__ bias, T * __restrict__ y, long long ldy, const __grid_constant__ CUtensorMap ymap, int * err_out) {
+    constexpr int STAGES = tc_stages<BOX>(), EPI = epi_warps<BOX>();
     extern __shared__ __align__(1024) unsigned char raw[];
     unsigned char * ring = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t) 1023);
-    unsigned char * out = reinterpret_cast<unsigned char *>(ring + kTStages * tc_stage_bytes<BN>());
-    TcSmem & S = *reinterpret_cast<TcSmem *>(out + kTEpi * kOutBytes);
+    unsigned char * out = reinterpret_cast<unsigned char *>(ring + STAGES * tc_stage_bytes<BN>());
+    TcSmem & S = *reinterpret_cast<TcSmem *>(out + EPI * kOutBytes);
     const int warp = __shfl_sync(0xFFFFFFFFu, (int) threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const int chunks = scale_chunks(K), nks = chunks / 2, nt = (N + BN - 1) / BN;
     const long long tiles = ((M + kTM - 1) / kTM) * nt;
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < kTStages; ++s) {
+        for (int s = 0; s < STAGES; ++s) {
             mbar_init(&S.full[s], 1);
             mbar_init(&S.empty[s], 1);
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(&S.acc_full[b], 1);
-            mbar_init(&S.acc_empty[b], kTEpi);
+            mbar_init(&S.acc_empty[b], EPI);
         }
         mbar_init(&S.done, 1);
         S.err = 0;
@@ -494,8 +497,8 @@ mx4_tc_kernel(const __grid_constant__ CUtensorMap amap, const unsigned char * __
                 const unsigned char * as = ascale + (size_t) m * chunks * 512;
                 const unsigned char * bs = wscale + (size_t) (n0 >> 7) * chunks * 512;
                 for (int ks = 0; ks < nks; ++ks, ++it) {
-                    const int s = (int) (it % kTStages);
-                    if (!mbar_wait(&S.empty[s], ((it / kTStages) & 1u) ^ 1u, kWaitNs, &S.err)) { ok = false; break; }
+                    const int s = (int) (it % STAGES);
+                    if (!mbar_wait(&S.empty[s], ((it / STAGES) & 1u) ^ 1u, kWaitNs, &S.err)) { ok = false; break; }
                     unsigned char * a = ring + s * tc_stage_bytes<BN>(), * b = a + kTM * 128, * sa = b + BN * 128;
                     mbar_expect(&S.full[s], tc_stage_bytes<BN>());
                     tma_load_2d(a, &amap, ks * 128, m * kTM, &S.full[s]);
@@ -505,7 +508,7 @@ mx4_tc_kernel(const __grid_constant__ CUtensorMap amap, const unsigned char * __
                 }
             }
             // nothing in flight when the block ends, however the others ended
-            for (unsigned j = it > kTStages ? it - kTStages : 0; j < it; ++j) mbar_drain(&S.full[j % kTStages], (j / kTStages) & 1u);
+            for (unsigned j = it > STAGES ? it - STAGES : 0; j < it; ++j) mbar_drain(&S.full[j % STAGES], (j / STAGES) & 1u);
         }
     } else if (warp == 1) {
         unsigned tile = 0, s = 0, ph = 0;
@@ -524,7 +527,7 @@ mx4_tc_kernel(const __grid_constant__ CUtensorMap amap, const unsigned char * __
                     if (ks == nks - 1) umma_commit(&S.acc_full[buf]);
                 }
                 __syncwarp();
-                if (++s == kTStages) { s = 0; ph ^= 1u; }
+                if (++s == STAGES) { s = 0; ph ^= 1u; }
             }
         }
         if (elect_one()) umma_commit(&S.done);           // no product in flight either
@@ -541,7 +544,7 @@ mx4_tc_kernel(const __grid_constant__ CUtensorMap amap, const unsigned char * __
             if (!warp_wait(&S.acc_full[buf], (tile >> 1) & 1u, &S.err)) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const int rows = (int) max(0LL, min(32LL, M - m0));
-            store_tile<T, BN, BOX>(tmem + buf * BN + ((unsigned) (q * 32) << 16), st, half, lane, m0, rows, n0, N, bias, y, ldy, &ymap);
+            store_tile<T, BN, BOX, EPI / 4>(tmem + buf * BN + ((unsigned) (q * 32) << 16), st, half, lane, m0, rows, n0, N, bias, y, ldy, &ymap);
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             if (lane == 0) mbar_arrive(&S.acc_empty[buf]);
         }
@@ -574,8 +577,8 @@ struct PairSmem {
     unsigned tmem;
     int err;
 };
-template <int BN> constexpr size_t pair_smem() {
-    return 1024 + (size_t) kPStages * pair_stage<BN>() + kTEpi * kOutBytes + sizeof(PairSmem);
+template <int BN, bool BOX> constexpr size_t pair_smem() {
+    return 1024 + (size_t) kPStages * pair_stage<BN>() + epi_warps<BOX>() * kOutBytes + sizeof(PairSmem);
 }
 
 __device__ __forceinline__ void cluster_meet() {
@@ -584,14 +587,15 @@ __device__ __forceinline__ void cluster_meet() {
 }
 
 template <class T, int BN, bool BOX>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(tc_threads<BOX>(), 1)
 mx4_pair_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap asmap, long long M, int K,
                 const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap wsmap, int N,
                 const float * __restrict__ bias, T * __restrict__ y, long long ldy, const __grid_constant__ CUtensorMap ymap, int * err_out) {
+    constexpr int EPI = epi_warps<BOX>();
     extern __shared__ __align__(1024) unsigned char raw[];
     unsigned char * ring = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t) 1023);
     unsigned char * out = ring + kPStages * pair_stage<BN>();
-    PairSmem & S = *reinterpret_cast<PairSmem *>(out + kTEpi * kOutBytes);
+    PairSmem & S = *reinterpret_cast<PairSmem *>(out + EPI * kOutBytes);
     const int warp = __shfl_sync(0xFFFFFFFFu, (int) threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const unsigned rank = blockIdx.x & 1u;
     const int nks = scale_chunks(K) / 2, nt = (N + BN - 1) / BN;
@@ -604,7 +608,7 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant_
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(&S.acc_full[b], 1);
-            mbar_init(&S.acc_empty[b], 2 * kTEpi);
+            mbar_init(&S.acc_empty[b], 2 * EPI);
         }
         mbar_init(&S.done, 1);
         S.err = 0;
@@ -685,7 +689,7 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant_
             if (!warp_wait(&S.acc_full[buf], (tile >> 1) & 1u, &S.err)) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const int rows = (int) max(0LL, min(32LL, M - m0));
-            store_tile<T, BN, BOX>(tmem + buf * BN + ((unsigned) (q * 32) << 16), st, half, lane, m0, rows, n0, N, bias, y, ldy, &ymap);
+            store_tile<T, BN, BOX, EPI / 4>(tmem + buf * BN + ((unsigned) (q * 32) << 16), st, half, lane, m0, rows, n0, N, bias, y, ldy, &ymap);
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             if (lane == 0) mbar_arrive_at(&S.acc_empty[buf], 0);
         }
@@ -839,7 +843,7 @@ mx4_few_kernel(const TX * __restrict__ x, long long ldx, int M, int K, const __g
             const unsigned buf = tile & 1u;
             if (!warp_wait(&S.acc_full[buf], (tile >> 1) & 1u, &S.err)) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            store_tile<TY, kFewN, false>(tmem + buf * kFewN, out + half * kOutBytes, half, lane, 0, M, t * kFewN, N, bias, y, ldy, nullptr);
+            store_tile<TY, kFewN, false, 2>(tmem + buf * kFewN, out + half * kOutBytes, half, lane, 0, M, t * kFewN, N, bias, y, ldy, nullptr);
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             if (lane == 0) mbar_arrive(&S.acc_empty[buf]);
         }
@@ -959,11 +963,11 @@ struct Call {
 
 // Launch of a product behind the quantisation of its rows, which lets it start before it has ended.
 template <class... P, class... A>
-cudaError_t launch_after(void (*kernel)(P...), unsigned grid, size_t smem, cudaStream_t s, A &&... args) {
+cudaError_t launch_after(void (*kernel)(P...), unsigned grid, unsigned threads, size_t smem, cudaStream_t s, A &&... args) {
     cudaLaunchConfig_t cfg{};
     cudaLaunchAttribute at[1];
     cfg.gridDim = dim3(grid);
-    cfg.blockDim = dim3(kTThreads);
+    cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -977,11 +981,11 @@ template <class T, int BN, bool BOX>
 cudaError_t launch_tc_as(const Call & c, const CUtensorMap & amap, const unsigned char * xs, const CUtensorMap & wmap, const CUtensorMap & ymap) {
     auto kernel = mx4_tc_kernel<T, BN, BOX>;
     static unsigned long long set;
-    const size_t smem = tc_smem_bytes<BN>();
+    const size_t smem = tc_smem_bytes<BN, BOX>();
     const cudaError_t e = allow_smem(kernel, smem, c.w->device, set);
     if (e != cudaSuccess) return e;
     const long long tiles = (c.M + kTM - 1) / kTM * ((c.w->N + BN - 1) / BN);
-    return launch_after(kernel, (unsigned) std::min<long long>(tiles, 148), smem, c.s,
+    return launch_after(kernel, (unsigned) std::min<long long>(tiles, 148), tc_threads<BOX>(), smem, c.s,
         amap, xs, c.M, c.w->K, wmap, c.w->scales, c.w->N, c.w->bias, static_cast<T *>(c.y), c.ldy, ymap, c.w->err_dev);
 }
 
@@ -992,11 +996,11 @@ cudaError_t launch_pair_as(const Call & c, const CUtensorMap & amap, const unsig
     if (e != cudaSuccess) return e;
     auto kernel = mx4_pair_kernel<T, BN, BOX>;
     static unsigned long long set;
-    const size_t smem = pair_smem<BN>();
+    const size_t smem = pair_smem<BN, BOX>();
     e = allow_smem(kernel, smem, c.w->device, set);
     if (e != cudaSuccess) return e;
     const long long tiles = (c.M + 2 * kTM - 1) / (2 * kTM) * ((c.w->N + BN - 1) / BN);
-    return launch_after(kernel, (unsigned) (2 * std::min<long long>(tiles, 74)), smem, c.s,
+    return launch_after(kernel, (unsigned) (2 * std::min<long long>(tiles, 74)), tc_threads<BOX>(), smem, c.s,
         amap, asmap, c.M, c.w->K, c.w->map[BN > 128 ? 2 : 0], c.w->smap[BN > 128 ? 1 : 0], c.w->N, c.w->bias, static_cast<T *>(c.y), c.ldy, ymap, c.w->err_dev);
 }
 
