@@ -123,6 +123,8 @@ struct Xchg {
 
 template <int NT> constexpr int bins_of() { return NT == 32 ? 256 : 1024; }
 
+template <int NT> constexpr int sets_of() { return NT == 1024 ? 2 : 1; }   // clusters are of 1024 threads
+
 template <int NT>
 struct TeamSmem {
     u64 wscan[NT / 32 + 1];
@@ -137,7 +139,9 @@ struct TeamSmem {
 };
 template <int NT>
 struct TeamBins {
-    uint2 sum[bins_of<NT>()];                          // of weights, in two halves; or counts in x
+    // sums of weights, in two halves, or counts in x; in a cluster levels take turns with two sets, so that
+    // one may be cleared while other blocks still read the other
+    uint2 sum[sets_of<NT>()][bins_of<NT>()];
     Pair list[kList];
     Pair all[kList];                                   // of all blocks of a cluster
     u64 w[kList];
@@ -150,6 +154,7 @@ struct Team {
     unsigned phase;
     TeamSmem<NT> * s;
     double mine;                             // this lane's entry of the exponential's table
+    unsigned level = 0;                      // levels of bins so far
 
     __device__ __forceinline__ int lane() const { return tid & 31; }
     __device__ __forceinline__ void sync() const {
@@ -213,9 +218,9 @@ struct Team {
         total = t;
         return before;
     }
-    // Largest of hi, smallest of lo, over the team.
+    // Largest of hi, smallest of lo, over the block, over the team.
     template <bool LO = true>
-    __device__ __forceinline__ void range(float & hi, float & lo) {
+    __device__ __forceinline__ void block_range(float & hi, float & lo) {
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) {
             hi = fmaxf(hi, __shfl_xor_sync(kFull, hi, o));
@@ -233,6 +238,10 @@ struct Team {
                 lo = fminf(lo, __shfl_xor_sync(kFull, lo, o));
             }
         }
+    }
+    template <bool LO = true>
+    __device__ __forceinline__ void range(float & hi, float & lo) {
+        block_range<LO>(hi, lo);
         if (CL) {
             Xchg & x = s->x[phase];
             if (tid == 0) { x.hi = hi; x.lo = lo; }
@@ -372,8 +381,10 @@ __device__ bool find_bin(Team<NT, CL> & team, TeamBins<NT> * B, const Slice<T, R
                          const Share * share) {
     constexpr int NB = bins_of<NT>(), PER = NB / NT;
     TeamSmem<NT> * s = team.s;
+    const unsigned set = CL ? team.level++ & 1u : 0u;
+    uint2 * bins = B->sum[set];
     for (int b = team.tid; b < NB; b += NT) {
-        B->sum[b] = make_uint2(0, 0);
+        bins[b] = make_uint2(0, 0);
     }
     if (team.tid == 0) { s->found = -1; s->listed = 0; }
     team.sync();
@@ -387,15 +398,15 @@ __device__ bool find_bin(Team<NT, CL> & team, TeamBins<NT> * B, const Slice<T, R
             if (any) {
                 if (v >= L.lo) {
                     const int b = L.bin_of<NB>(v);
-                    const unsigned wl = (unsigned) w, old = atomicAdd(&B->sum[b].x, wl);
+                    const unsigned wl = (unsigned) w, old = atomicAdd(&bins[b].x, wl);
                     const unsigned up = (unsigned) (w >> 32) + (old + wl < old ? 1u : 0u);
-                    if (up) atomicAdd(&B->sum[b].y, up);
+                    if (up) atomicAdd(&bins[b].y, up);
                 } else {
                     rest += w;
                 }
             }
         } else if (L.holds(v)) {
-            atomicAdd(&B->sum[L.bin_of<NB>(v)].x, 1u);
+            atomicAdd(&bins[L.bin_of<NB>(v)].x, 1u);
         }
     });
     if (WEIGHTS && share) rest = team.sum(rest);                 // in a cluster, all bins are complete after it
@@ -410,12 +421,12 @@ __device__ bool find_bin(Team<NT, CL> & team, TeamBins<NT> * B, const Slice<T, R
             // all blocks' words are asked for before the first is used
             uint2 r[kMaxCluster];
 #pragma unroll
-            for (int q = 0; q < kMaxCluster; ++q) r[q] = cg::this_cluster().map_shared_rank(B, q < team.blocks ? q : 0)->sum[b];
+            for (int q = 0; q < kMaxCluster; ++q) r[q] = cg::this_cluster().map_shared_rank(B, q < team.blocks ? q : 0)->sum[set][b];
 #pragma unroll
             for (int q = 0; q < kMaxCluster; ++q)
                 if (q < team.blocks) w += ((u64) r[q].y << 32) + r[q].x;
         } else {
-            w = ((u64) B->sum[b].y << 32) + B->sum[b].x;
+            w = ((u64) bins[b].y << 32) + bins[b].x;
         }
         mine[j] = w;
         sum += w;
@@ -436,7 +447,7 @@ __device__ bool find_bin(Team<NT, CL> & team, TeamBins<NT> * B, const Slice<T, R
             before += mine[j];
         }
     }
-    if (CL) team.meet(); else team.sync();                       // and nobody clears bins that another reads
+    team.sync();
     L.bin = s->found;
     if (L.bin < 0) {
         L.with = total;
@@ -448,13 +459,25 @@ __device__ bool find_bin(Team<NT, CL> & team, TeamBins<NT> * B, const Slice<T, R
 }
 
 // Puts the slice's elements that `want` names on the list, and joins the lists of a cluster's blocks.
-// The number of them; past kList the list is not complete and not to be used.
-template <class T, int NT, bool CL, bool RES, class F>
-__device__ int gather(Team<NT, CL> & team, TeamBins<NT> * B, const Slice<T, RES> & l, int s0, const Pair *& list, F want) {
+// The number of them; past kList the list is not complete and not to be used. RANGE: also their largest
+// and smallest value; with `few` false nothing is listed, as there are more than kList.
+template <bool RANGE, class T, int NT, bool CL, bool RES, class F>
+__device__ int gather(Team<NT, CL> & team, TeamBins<NT> * B, const Slice<T, RES> & l, int s0, const Pair *& list, F want, bool few,
+                      float & hi, float & lo) {
     TeamSmem<NT> * s = team.s;
+    if (RANGE) {
+        hi = -CUDART_INF_F;
+        lo = CUDART_INF_F;
+    }
     l.template quads<NT>(team.tid, [&](float4 v, int i) {
         const bool a = want(v.x), b = want(v.y), c = want(v.z), d = want(v.w);
         if (!(a || b || c || d)) return;
+        if (RANGE) {
+            const float inf = CUDART_INF_F;
+            hi = fmaxf(fmaxf(hi, fmaxf(a ? v.x : -inf, b ? v.y : -inf)), fmaxf(c ? v.z : -inf, d ? v.w : -inf));
+            lo = fminf(fminf(lo, fminf(a ? v.x : inf, b ? v.y : inf)), fminf(c ? v.z : inf, d ? v.w : inf));
+            if (!few) return;
+        }
         int at = atomicAdd(&s->listed, (int) a + (int) b + (int) c + (int) d);
         if (a && at < kList) B->list[at] = Pair{v.x, s0 + i};
         at += a;
@@ -465,22 +488,40 @@ __device__ int gather(Team<NT, CL> & team, TeamBins<NT> * B, const Slice<T, RES>
         if (d && at < kList) B->list[at] = Pair{v.w, s0 + i + 3};
     });
     team.sync();
-    int n = s->listed;
+    int n = few ? s->listed : kList + 1;
     list = B->list;
+    if (RANGE && (CL || n > kList)) team.block_range(hi, lo);
     if (CL) {
         Xchg & x = s->x[team.phase];
-        if (team.tid == 0) x.a = (u64) n;
+        if (team.tid == 0) {
+            x.a = (u64) n;
+            x.hi = hi;
+            x.lo = lo;
+        }
         team.meet();
         n = 0;
         for (int q = 0; q < team.blocks; ++q) {
-            const int c = (int) cg::this_cluster().map_shared_rank(&x, q)->a;
-            const TeamBins<NT> * o = cg::this_cluster().map_shared_rank(B, q);
-            for (int i = team.tid; i < c && n + i < kList; i += NT) B->all[n + i] = o->list[i];
-            n += c;
+            const Xchg * o = cg::this_cluster().map_shared_rank(&x, q);
+            n += (int) o->a;
+            if (RANGE) {
+                hi = fmaxf(hi, o->hi);
+                lo = fminf(lo, o->lo);
+            }
         }
-        list = B->all;
-        team.phase ^= 1;
-        team.meet();                            // nobody lists anew while another still reads
+        if (n <= kList) {
+            int at = 0;
+            for (int q = 0; q < team.blocks; ++q) {
+                const int c = (int) cg::this_cluster().map_shared_rank(&x, q)->a;
+                const TeamBins<NT> * o = cg::this_cluster().map_shared_rank(B, q);
+                for (int i = team.tid; i < c; i += NT) B->all[at + i] = o->list[i];
+                at += c;
+            }
+            list = B->all;
+            team.phase ^= 1;
+            team.meet();                        // nobody lists anew while another still reads
+        } else {
+            team.phase ^= 1;
+        }
     }
     team.sync();
     if (team.tid == 0) s->listed = 0;           // read by all: the next list starts empty
@@ -545,10 +586,10 @@ __device__ float find_cut(Team<NT, CL> & team, TeamBins<NT> * B, const Slice<T, 
         // at least this many tokens are in the bin, as none is heavier than its upper edge
         const float edge = fminf(L.hi, L.hi - (L.hi - L.lo) * (((float) L.bin - 0.01f) / (float) NB));
         const u64 most = WEIGHTS ? max(weight_one(edge, row), 1ull) : 1ull;
-        const Pair * list = nullptr;
-        int n = kList + 1;
-        if (L.with - L.above <= (u64) kList * most)
-            n = gather<T, NT, CL, RES>(team, B, l, 0, list, [&](float v) { return L.holds(v) && L.bin_of<NB>(v) == L.bin; });
+        const Pair * list;
+        float hi, lo;
+        const int n = gather<true, T, NT, CL, RES>(team, B, l, 0, list, [&](float v) { return L.holds(v) && L.bin_of<NB>(v) == L.bin; },
+                                                   L.with - L.above <= (u64) kList * most, hi, lo);
         if (n <= kList) {
             weigh_list<NT>(team.tid, B, list, n, row, !WEIGHTS);
             team.sync();
@@ -573,14 +614,6 @@ __device__ float find_cut(Team<NT, CL> & team, TeamBins<NT> * B, const Slice<T, 
             team.sync();
             return v;
         }
-        float hi = -CUDART_INF_F, lo = CUDART_INF_F;
-        l.template each<NT>(team.tid, [&](float v, int) {
-            if (L.holds(v) && L.bin_of<NB>(v) == L.bin) {
-                hi = fmaxf(hi, v);
-                lo = fminf(lo, v);
-            }
-        });
-        team.range(hi, lo);
         if (!(hi > lo)) {                       // one value
             const u64 each = WEIGHTS ? weight_one(hi, row) : 1ull;
             ties = (need - L.above + each - 1) / max(each, 1ull);
@@ -752,14 +785,15 @@ __device__ int nucleus_f32(Team<NT, false> & team, TeamBins<NT> * B, const Slice
     Level L;
     L.range(hi, from, NB);
     if (L.half != 1.0f || !(L.inv < 1e30f)) return kNothing;
-    for (int b = team.tid; b < NB; b += NT) B->sum[b].x = 0;
+    uint2 * bins = B->sum[0];
+    for (int b = team.tid; b < NB; b += NT) bins[b].x = 0;
     if (team.tid == 0) { s->found = NB - 1; s->found_ties = NB - 1; s->listed = 0; }
     team.sync();
     float part[4] = {};
     l.template quads<NT>(team.tid, [&](float4 v, int) {
         auto one = [&](float x, float & sum) {
             sum += r.weight(x);
-            if (x >= from) atomicAdd(&B->sum[L.bin_of<NB>(x)].x, 1u);
+            if (x >= from) atomicAdd(&bins[L.bin_of<NB>(x)].x, 1u);
         };
         one(v.x, part[0]);
         one(v.y, part[1]);
@@ -780,7 +814,7 @@ __device__ int nucleus_f32(Team<NT, false> & team, TeamBins<NT> * B, const Slice
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
         const int b = team.tid * PER + j;
-        const float n = (float) B->sum[b].x * unit;
+        const float n = (float) bins[b].x * unit;
         // the edges moved out by more than bin_of's rounding
         const float up = n * r.weight(hi - ((float) b - 0.01f) * width) * 1.0001f, down = n * r.weight(hi - ((float) b + 1.01f) * width) * 0.9999f;
         bound[j] = n > 0.0f ? (u64) (__float2uint_ru(fminf(up, 1e9f))) << 32 | __float2uint_rd(fminf(down, 1e9f)) : 0ull;
@@ -1016,8 +1050,9 @@ sample_kernel(pk_sample_args a, int slice, int teams, int row_floats) {
             if (find_bin<false, T, NT, CL, RES>(team, bins, l, r, L, need, nullptr)) {
                 if (L.with <= (u64) kList) {
                     const Pair * list;
-                    const int n = gather<T, NT, CL, RES>(team, bins, l, s0, list,
-                                                         [&](float v) { return L.holds(v) && L.bin_of<NB>(v) <= L.bin; });
+                    float h, w;
+                    const int n = gather<false, T, NT, CL, RES>(team, bins, l, s0, list,
+                        [&](float v) { return L.holds(v) && L.bin_of<NB>(v) <= L.bin; }, true, h, w);
                     draw_listed<NT, CL>(team, bins, list, n, a, row, r, hi, inv_t, k, p, 0, least);
                     return;
                 }
@@ -1066,8 +1101,9 @@ sample_kernel(pk_sample_args a, int slice, int teams, int row_floats) {
                 const float edge = fmaxf(from, hi - (hi - from) * ((float) (L.bin + 1) / (float) NB));
                 if ((double) L.with <= 32.0 * (double) max(weight_one(edge, r), 1ull)) {
                     const Pair * list;
-                    const int n = gather<T, NT, CL, RES>(team, bins, l, s0, list,
-                                                         [&](float v) { return L.holds(v) && L.bin_of<NB>(v) <= L.bin; });
+                    float h, w;
+                    const int n = gather<false, T, NT, CL, RES>(team, bins, l, s0, list,
+                        [&](float v) { return L.holds(v) && L.bin_of<NB>(v) <= L.bin; }, true, h, w);
                     if (n <= kList) {
                         draw_listed<NT, CL>(team, bins, list, n, a, row, r, hi, inv_t, kList, p, need, least);
                         return;
@@ -1082,30 +1118,32 @@ sample_kernel(pk_sample_args a, int slice, int teams, int row_floats) {
         }
     }
     const int i0 = RES ? team.tid * len : min(team.tid * len, l.n), i1 = RES ? i0 + len : min(i0 + len, l.n);
-    // equal logits at the cut, where not all of them are kept, go by index
-    u64 tie0 = 0;
-    if (FILTERS && partial) {
-        u64 n = 0, all = 0;
-        for (int i = i0; i < i1; ++i) n += l(i) == cut ? 1u : 0u;
-        tie0 = team.scan(n, all);
-    }
     // a run has fewer than 2^9 elements, so its sum stays below 2^53 and is whole. (A product that
     // lies halfway between two integers may round the other way here than by itself; see the search.)
     double onto = kZero;
-    u64 seen = tie0;
     const float from = fmaxf(least, cut);
+    unsigned equal = 0;
 #pragma unroll 4
     for (int j = 0; j < len; ++j) {
         const float v = RES || i0 + j < i1 ? l(i0 + j) : -CUDART_INF_F;
         bool keep = v >= from;
         if (FILTERS) {
-            if (partial && v == cut) keep = seen++ < ties && keep;
+            if (partial && v == cut) {
+                ++equal;
+                keep = false;
+            }
             if (!__any_sync(kFull, keep)) continue;
         }
         const double w = weight_warp(v, r, team.mine, onto);
         if (keep) onto = w;
     }
-    const u64 sum = whole(onto);
+    u64 sum = whole(onto), tie0 = 0;
+    if (FILTERS && partial) {
+        // equal logits at the cut, not all of which are kept, go by index
+        u64 all;
+        tie0 = team.scan((u64) equal, all);
+        if (cut >= least && tie0 < ties) sum += min((u64) equal, ties - tie0) * weight_one(cut, r);
+    }
     u64 total = 0;
     const u64 before = team.scan(sum, total);
     const u64 t = place_of(a.uniforms[row], total);
