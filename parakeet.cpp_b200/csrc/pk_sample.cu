@@ -163,6 +163,16 @@ struct Team {
     // Every block's slot written before it is complete, what was read before it may be overwritten.
     __device__ __forceinline__ void meet() const { cg::this_cluster().sync(); }
 
+    // All blocks' slots, asked for before the first is used: f(block, slot) in turn.
+    template <class F> __device__ __forceinline__ void hear(const Xchg & mine, F f) const {
+        Xchg o[kMaxCluster];
+#pragma unroll
+        for (int b = 0; b < kMaxCluster; ++b) o[b] = *cg::this_cluster().map_shared_rank(const_cast<Xchg *>(&mine), b < blocks ? b : 0);
+#pragma unroll
+        for (int b = 0; b < kMaxCluster; ++b)
+            if (b < blocks) f(b, o[b]);
+    }
+
     __device__ u64 sum(u64 v) {
         v = warp_sum(v);
         if (NT > 32) {
@@ -178,7 +188,7 @@ struct Team {
             if (tid == 0) x.a = v;
             meet();
             v = 0;
-            for (int b = 0; b < blocks; ++b) v += cg::this_cluster().map_shared_rank(&x, b)->a;
+            hear(x, [&](int, const Xchg & o) { v += o.a; });
             phase ^= 1;
         }
         return v;
@@ -208,11 +218,10 @@ struct Team {
             if (tid == 0) o.a = t;
             meet();
             t = 0;
-            for (int b = 0; b < blocks; ++b) {
-                const u64 w = cg::this_cluster().map_shared_rank(&o, b)->a;
-                if (b < rank) before += w;
-                t += w;
-            }
+            hear(o, [&](int b, const Xchg & w) {
+                if (b < rank) before += w.a;
+                t += w.a;
+            });
             phase ^= 1;
         }
         total = t;
@@ -246,11 +255,10 @@ struct Team {
             Xchg & x = s->x[phase];
             if (tid == 0) { x.hi = hi; x.lo = lo; }
             meet();
-            for (int b = 0; b < blocks; ++b) {
-                const Xchg * o = cg::this_cluster().map_shared_rank(&x, b);
-                hi = fmaxf(hi, o->hi);
-                lo = fminf(lo, o->lo);
-            }
+            hear(x, [&](int, const Xchg & o) {
+                hi = fmaxf(hi, o.hi);
+                lo = fminf(lo, o.lo);
+            });
             phase ^= 1;
         }
     }
@@ -500,22 +508,21 @@ __device__ int gather(Team<NT, CL> & team, TeamBins<NT> * B, const Slice<T, RES>
         }
         team.meet();
         n = 0;
-        for (int q = 0; q < team.blocks; ++q) {
-            const Xchg * o = cg::this_cluster().map_shared_rank(&x, q);
-            n += (int) o->a;
+        // entry tid of the joint list is entry tid - start of block `from`'s
+        int from = 0, start = 0;
+        team.hear(x, [&](int q, const Xchg & o) {
+            if (n <= team.tid) {
+                from = q;
+                start = n;
+            }
+            n += (int) o.a;
             if (RANGE) {
-                hi = fmaxf(hi, o->hi);
-                lo = fminf(lo, o->lo);
+                hi = fmaxf(hi, o.hi);
+                lo = fminf(lo, o.lo);
             }
-        }
+        });
         if (n <= kList) {
-            int at = 0;
-            for (int q = 0; q < team.blocks; ++q) {
-                const int c = (int) cg::this_cluster().map_shared_rank(&x, q)->a;
-                const TeamBins<NT> * o = cg::this_cluster().map_shared_rank(B, q);
-                for (int i = team.tid; i < c; i += NT) B->all[at + i] = o->list[i];
-                at += c;
-            }
+            if (team.tid < n) B->all[team.tid] = cg::this_cluster().map_shared_rank(B, from)->list[team.tid - start];
             list = B->all;
             team.phase ^= 1;
             team.meet();                        // nobody lists anew while another still reads
@@ -1001,7 +1008,7 @@ sample_kernel(pk_sample_args a, int slice, int teams, int row_floats) {
             Xchg & x = team.s->x[team.phase];
             if (team.tid == 0) x.a = first;
             team.meet();
-            for (int b = 0; b < team.blocks; ++b) first = min(first, cg::this_cluster().map_shared_rank(&x, b)->a);
+            team.hear(x, [&](int, const Xchg & o) { first = min(first, o.a); });
             team.meet();
         }
         if (team.tid == 0 && team.rank == 0) {
