@@ -166,7 +166,7 @@ __device__ __forceinline__ unsigned scale_word(unsigned sb) {
 // warp, gridDim.y segments further on; several loads are in flight before the first is used.
 // ATOMS: scales in the product's layout, zeros for the blocks past K that its stages read.
 // Bound: HBM from f32 (66044 x 1024: 44 us, 6.9 TB/s read and written), instructions from half precision
-// (66043 x 1000 bf16: 37 us, 4.5 TB/s).
+// (66043 x 1000 bf16: 34 us, 4.9 TB/s).
 template <class T, bool VEC, bool ATOMS>
 __global__ void __launch_bounds__(kQThreads) mx4_quantize_kernel(const T * __restrict__ x, long long rows, int K, long long ldx,
                                                                  unsigned char * __restrict__ codes,
@@ -240,7 +240,7 @@ template <> __device__ __forceinline__ void codes_to_values(unsigned q, unsigned
     for (int i = 0; i < 4; ++i) reinterpret_cast<unsigned *>(o.e)[i] = word_of(__hmul2(pair_of<__nv_bfloat162>(w[i]), s2));
 }
 
-// The value of each code, eight a lane. Bound: HBM, writing y (66043 x 1000 bf16: 31 us, 5.4 TB/s).
+// The value of each code, eight a lane. Bound: HBM, writing y (66043 x 1000 bf16: 34 us, 4.9 TB/s).
 template <class T, bool VEC>
 __global__ void __launch_bounds__(kQThreads) mx4_dequantize_kernel(const unsigned char * __restrict__ codes,
                                                                    const unsigned char * __restrict__ scales, long long rows,
