@@ -707,15 +707,18 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant_
 
 // ---- few rows: quantisation and product in one kernel -----------------------------
 //
-// With up to 32 rows the time is that of launches and of single loads, and the weights are nearly all
+// With few rows the time is that of launches and of single loads, and the weights are nearly all
 // of the bytes: every block quantises the rows for itself, into the products' layout in its shared
 // memory, while the first weights are on their way, and takes its share of the tiles of 64 outputs.
-// One launch: 9.0 us for 1 x 640 by 8198 called from Python, 12.6 us with a kernel for each. Not so
+// One launch: 9.0 us for 1 x 640 by 8198 called from Python, 12.6 us with a kernel for each. Replayed from
+// a graph 5.2 and 6.6 us for 1 x 1024, 6.4 and 6.8 for 16, 7.8 and 7.0 for 32; 8.5 and 8.2 for 16 x 2048,
+// 10.8 and 8.6 for 32: hence the bound on the values of x. Not so
 // for more rows: at 64 the rows' loads, again in every block, take longer than the second launch
 // (14.3 us against 11.4), and at 66044 two kernels are 97 us against 111 with the codes kept on the
 // SM, sixteen warps of one block being too few to keep x streaming.
 constexpr int kFewRows = 32;
 constexpr int kFewK = 2048;                             // the rows' codes stay in shared memory
+constexpr int kFewX = 32768;                            // every block quantises all of x
 constexpr int kFewN = 64;
 constexpr int kFewStages = 4;
 constexpr int kFewQuant = 16;                           // quantising warps
@@ -893,9 +896,17 @@ void give_error_word(int * w) {
 int * take_error_word(cudaError_t & e) {
     std::lock_guard<std::mutex> g(error_lock);
     if (free_words.empty()) {
+        static size_t words;
+        try {
+            free_words.reserve(words + 1024);       // giving back never allocates
+        } catch (const std::bad_alloc &) {
+            e = cudaErrorMemoryAllocation;
+            return nullptr;
+        }
         void * page = nullptr;
         e = cudaHostAlloc(&page, 4096, cudaHostAllocMapped | cudaHostAllocPortable);
         if (e != cudaSuccess) return nullptr;
+        words += 1024;
         for (int i = 0; i < 1024; ++i) free_words.push_back(static_cast<int *>(page) + i);
     }
     int * w = free_words.back();
@@ -1025,7 +1036,7 @@ template <class TX> cudaError_t launch_few(const Call & c, int y_type) {
            : y_type == PK_GGML_F16 ? launch_few_xy<TX, __half>(c) : launch_few_xy<TX, __nv_bfloat16>(c);
 }
 
-bool few(const pk_mx4 * w, int64_t rows) { return rows <= kFewRows && w->K <= kFewK; }
+bool few(const pk_mx4 * w, int64_t rows) { return rows <= kFewRows && w->K <= kFewK && rows * w->K <= kFewX; }
 
 // Tile width of the single blocks: fewest rounds of tiles over the SMs, a round costed by the rows that
 // a tile loads. (192, with fewer loads a product, was slower where K is short: 66044 x 640 x 1024 97 us
@@ -1213,7 +1224,7 @@ size_t ws_codes(const pk_mx4 * w, int64_t rows) { return ((size_t) rows * w->nb 
 
 extern "C" PK_API int64_t pk_mx4_workspace(const pk_mx4 * w, int64_t rows) {
     if (!w) return -1;
-    if (rows <= 0) return 0;
+    if (rows <= 0 || few(w, rows)) return 0;
     return (int64_t) (ws_codes(w, rows) + (size_t) ((rows + 127) / 128) * w->chunks * 512);
 }
 

@@ -442,6 +442,29 @@ def test_rows_do_not_depend_on_the_batch(built):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("k,most", [(640, 32), (1024, 32), (1025, 31), (2048, 16), (2049, 0)])
+def test_few_rows_need_no_workspace(built, k, most):
+    """No workspace up to the row count at which the rows get a launch of their own; never less for more rows."""
+    import torch
+    pk = built
+    rng = np.random.default_rng(k)
+    w = rng.standard_normal((130, k)).astype(np.float32)
+    layer = pk.Mx4Linear(w)
+    need = [layer.workspace(r) for r in range(0, 70)]
+    assert all(n == 0 for n in need[:most + 1]) and all(n > 0 for n in need[most + 1:]) and need == sorted(need)
+    for r in (most, most + 1):
+        if r == 0:
+            continue
+        x = rng.standard_normal((r, k)).astype(np.float32)
+        if r == most:
+            xd, y = torch.from_numpy(x).cuda(), torch.zeros(r, 130, device="cuda")
+            layer.forward(xd.data_ptr(), r, y.data_ptr())
+            torch.cuda.synchronize()
+            check_product(ref_quantize(w)[2], x, y.cpu().numpy())
+        check_product(ref_quantize(w)[2], *product(pk, w, x, layer=layer))
+
+
+@pytest.mark.gpu
 def test_first_call_may_be_captured(built):
     """A process whose first product and first draw are captured into a graph."""
     import subprocess
