@@ -12,7 +12,7 @@
 // f32's 2^-22 the running sum would pass the random number at another token in one of a few hundred
 // rows, since a row has as many borders as tokens.
 //
-// Rows of up to 1280 logits with nothing cut, as a CTC path has them by the ten thousand, are summed in
+// Rows of up to 2048 logits with nothing cut, as a CTC path has them by the ten thousand, are summed in
 // f32 first: four instructions a token instead of twenty. That settles the token unless the random
 // number lies within a proven bound of a border (one or two rows in a hundred), and those rows go on to
 // the f64 sums, so the token is the same; the log-probability then has f32's sum, 2^-18 off at most.
@@ -697,8 +697,8 @@ __device__ void draw_listed(Team<NT, CL> & team, TeamBins<NT> * B, const Pair * 
 // by 2^-24 of itself, so x^ by 4 2^-24 |x|, and ex2.approx by 2^-21 of its result at most:
 // |w^ - w| <= w 2^-24 (8 + 2.78 |x|). With p = w / S and S >= 1, the sum of p |x| is the entropy of p
 // less log2 S, so at most log2 V: any sum of w^ over tokens is within S 2^-24 (8 + 2.78 log2 V) <=
-// 37 S 2^-24 of that of w, for V <= 1280. A run's terms go to four accumulators, 11 additions each and
-// two more: 13 S 2^-24. The runs are added in f64. Together below 2^-18 S = E for every prefix and for
+// 39 S 2^-24 of that of w, for V <= 2048. A run's terms (65 at most) go to four accumulators, 17 additions
+// each and two more: 19 S 2^-24. The runs are added in f64. Together below 2^-18 S = E for every prefix and for
 // S, so u S is off by as much: the token is settled if the border before it and the one behind are each
 // more than 2 E (2.5 E, against what is left) from u S.
 struct Row32 {
@@ -770,7 +770,7 @@ __device__ __forceinline__ bool draw_f32(const Slice<T, RES> & l, int len, int l
 // One pass sums all weights and counts the tokens of each bin. A bin's weight lies between its count times
 // the weights at its two edges, so the bins in which the sum over falling logits may reach the share p
 // are known; a second pass sums what lies above them and lists their tokens, and the cut is read from
-// the list's ranks. A third pass draws. For V <= 16384 a sum of f32 weights is off by less than
+// the list's ranks. A third pass draws. For V <= 16384, and at most 64 logits a thread, a sum of f32 weights is off by less than
 // S 2^-24 (8 + 2.78 * 14 + 19) < 70 2^-24 S = E (19: the additions of a thread's quarter); sums are
 // joined as integers of 2^-40. A step that a sum within 2.5 E of its border decides is left to the f64
 // sums (some 3 rows in 100 of 8193 logits).
@@ -1070,7 +1070,7 @@ sample_kernel(pk_sample_args a, int slice, int teams, int row_floats) {
         // With many rows; a single one is sooner through the f64 sums, which take fewer steps one after another
         // (64 rows of 8193, each with its own settings: 16 us against 19).
         if constexpr (RES && !CL && (NT == 128 || NT == 256)) {
-            if (!(p >= 1.0f) && !(cut > -CUDART_INF_F) && a.vocab <= 16384) {
+            if (!(p >= 1.0f) && !(cut > -CUDART_INF_F) && a.vocab <= 64 * NT) {
                 known = nucleus_f32<T, NT>(team, bins, l, len, hi, low, temp_f, least, p, a.uniforms[row], a, row, cut, ties, partial);
                 if (known == kDrawn) return;
             }
@@ -1248,17 +1248,28 @@ cudaError_t launch_cluster(const pk_sample_args & a, int blocks, cudaStream_t s)
 
 template <class T, bool FILTERS>
 cudaError_t dispatch(const pk_sample_args & a, cudaStream_t s) {
-    if (a.vocab <= 1280 && a.rows >= 512) return launch_block<T, FILTERS, 32>(a, s);
-    if (a.vocab <= 2048) return launch_block<T, FILTERS, 128>(a, s);
-    // Few rows of a large vocabulary over clusters. A cluster's barriers cost more than they save
-    // below: one row of 8193 in one block of 512 16 us, in a cluster of eight 20 us.
+    // A row a warp, in blocks of eight, from one block an SM on with nothing cut (1500 rows of 600: 5.7 us, with
+    // a block of 128 a row 6.1; 700 rows: 5.3 and 3.9; 20000 rows of 2048: 43 and 81) and from 20 rows an SM on
+    // with filters, if three such blocks and their bins fit an SM (6000 rows of 1025, top-p: 52 us and 58, 1500
+    // rows of top-k: 42 and 30; 6000 rows of 1150: 69 and 59).
+    if (FILTERS ? a.vocab <= 1056 && a.rows >= 20 * 148 : a.vocab <= 2048 && a.rows >= 8 * 148) return launch_block<T, FILTERS, 32>(a, s);
+    // Few rows of a large vocabulary over clusters. A cluster's barriers cost more than they save below (one
+    // row with top-p, in one block of 512 and in a cluster of eight: of 8193 13 us and 20, of 20000 22 us
+    // and 21, of 50000 45 us and 23).
     int blocks = 1;
     if (a.vocab > 16384)
         while (blocks < kMaxCluster && a.rows * blocks * 2 <= 148) blocks *= 2;
     while (blocks < kMaxCluster && (size_t) (a.vocab / blocks) * 4 > 200 * 1024) blocks *= 2;
     if (blocks > 1) return launch_cluster<T, FILTERS>(a, blocks, s);
-    if (a.vocab <= 16384 && a.rows > 148) return launch_block<T, FILTERS, 256>(a, s);
-    return launch_block<T, FILTERS, 512>(a, s);
+    // Otherwise a row a block, of as many threads as let every row have its block at once (450 rows of 4097,
+    // top-p, in blocks of 128, 256 and 512: 26 us, 20, 25; 296 rows: 25, 18, 14), though of at least 256 for
+    // up to 2048 logits (one row of 1600: 6.3 us, of 512 7.8). Past that the fewest threads that a row's length
+    // leaves busy: 128 up to 5120 (4096 rows of 4097: 79 us, 89, 170), 256 up to 16384 (4096 rows of 8193:
+    // 143 us, 131, 232), 512.
+    const bool wave512 = a.rows <= 2 * 148 && a.vocab > 2048, wave256 = a.rows <= 4 * 148;
+    if (a.vocab > 16384 || wave512) return launch_block<T, FILTERS, 512>(a, s);
+    if (a.vocab > 5120 || wave256) return launch_block<T, FILTERS, 256>(a, s);
+    return launch_block<T, FILTERS, 128>(a, s);
 }
 
 }  // namespace

@@ -87,12 +87,12 @@ def check(seen, u, tok, lp, **kw):
     """Tokens equal; log-probabilities: a f64 number rounded once (2^-24 of it) whose sum of weights
     is off by 2^-44 a token at most. Where f32 sums may have settled the token, its sum of weights is off
     by their bound instead, and (l - max) / T by three roundings, 3 2^-24 of it:
-    rows of up to 1280 tokens with nothing cut, 512 and more of them: 8 2^-24 for each exponential,
-    2.78 log2 V <= 29 for its argument, 13 for the additions, 50 2^-24 < 2^-18 of the sum;
+    rows of up to 2048 tokens with nothing cut, 512 and more of them: 8 2^-24 for each exponential,
+    2.78 log2 V <= 31 for its argument, 19 for the additions, 58 2^-24 < 2^-18 of the sum;
     rows of up to 16384 tokens with top-p: 8, 2.78 log2 V <= 39 and 19, 66 2^-24 < 2^-17 of the sum."""
     kw = {**DEFAULTS, **kw}
     r, v = seen.shape
-    f32 = r >= 512 and v <= 1280 and all(np.ndim(x) == 0 for x in kw.values()) and not (
+    f32 = r >= 512 and v <= 2048 and all(np.ndim(x) == 0 for x in kw.values()) and not (
         0 < kw["top_k"] < v or kw["top_p"] < 1 or kw["min_p"] > 0)   # one short row in a warp
     for i in range(r):
         one = {n: (x[i] if np.ndim(x) else x) for n, x in kw.items()}
@@ -194,6 +194,42 @@ def test_many_short_rows(built, v, dtype, pad, shift):
     for kw in (dict(), dict(temperature=0.6), dict(temperature=1e-35), dict(temperature=float("inf"))):
         seen, tok, lp = run(built, l, u, dtype, pad, shift, **kw)
         check(seen, u, tok, lp, **kw)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("v", [1281, 2047, 2048])
+def test_many_rows_of_two_thousand(built, v):
+    """The longest rows that f32 sums may settle, flat ones among them: their sums are off the most."""
+    rng = np.random.default_rng(v)
+    r = 1184
+    l = rng.standard_normal((r, v)) * rng.choice([0.0, 0.3, 2.0, 8.0], (r, 1))
+    l[rng.random((r, v)) < 0.05] = -np.inf
+    u = rng.random(r)
+    w = np.exp(l - l.max(1, keepdims=True))
+    u[200:] = (np.cumsum(w, 1) / w.sum(1, keepdims=True))[np.arange(r), rng.integers(v, size=r)][200:]   # at borders
+    u = np.clip(u, 0, 1 - 2.0 ** -24).astype(np.float32)
+    seen, tok, lp = run(built, l, u, "f32", 1, 1)
+    check(seen, u, tok, lp)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kw", [dict(top_k=9), dict(top_p=0.9, temperature=0.8), dict(top_k=200, top_p=0.97, min_p=0.002)],
+                         ids=["k", "p", "all"])
+@pytest.mark.parametrize("r,v", [(2960, 33), (2960, 1056), (3000, 1057), (593, 257), (593, 5120), (593, 5121), (592, 2049), (297, 2049),
+                                 (296, 2049), (592, 2048)])
+def test_either_side_of_each_team(built, r, v, kw):
+    """Row counts and lengths where one size of team gives way to the next; the same row is the same token
+    in the batch and among few."""
+    rng = np.random.default_rng(r + v)
+    l = rng.standard_normal((r, v)) * rng.choice([0.0, 0.5, 2.5, 9.0], (r, 1))
+    l[rng.random((r, v)) < 0.02] = -np.inf
+    l[3] = -np.inf
+    u = rng.random(r).astype(np.float32)
+    seen, tok, lp = run(built, l, u, "f32", 3, 0, **kw)
+    some = np.unique(np.concatenate([np.arange(40), rng.integers(r, size=160), [r - 1]]))
+    check(seen[some], u[some], tok[some], lp[some], **kw)
+    _, few, _ = run(built, l[some[:60]], u[some[:60]], **kw)
+    assert np.array_equal(few, tok[some[:60]])
 
 
 @pytest.mark.gpu
