@@ -416,6 +416,7 @@ class CtcGreedy:
                 if uniforms.size < total:
                     raise ValueError(f"{uniforms.size} random numbers for {total} frames")
                 up = _p(uniforms)
+            top_k = max(0, min(int(top_k), self.vocab_size))
             draw = abi.pk_ctc_draw(temperature, top_k, top_p, min_p, up, 1 if uniforms_on_device else 0, 0)
         _check(lib().pk_ctc_decode(self._h, head.h if head is not None else None, fp, 1 if on_device else 0, _p(foff),
                                    _p(n_frames), B, C.byref(draw) if draw is not None else None, _p(prev), _p(toks), cap,
@@ -548,6 +549,9 @@ def sample(logits: int, rows: int, vocab: int, uniforms: int, tokens: int, dtype
     """pk_sample on device pointers: one token per row of logits, by the row's random number.
     The settings are numbers for every row, or device arrays with one entry per row (0: not
     given). Queued on `stream`."""
+    if not 0 < vocab <= abi.PK_SAMPLE_MAX_VOCAB:
+        raise ValueError(f"vocab {vocab} is not in [1, {abi.PK_SAMPLE_MAX_VOCAB}]")
+    top_k = max(0, min(int(top_k), vocab))
     a = abi.pk_sample_args(logits, _DTYPE[dtype], vocab, rows, vocab if row_stride is None else row_stride, uniforms,
                            tokens, logprobs, temperature, top_k, top_p, min_p, temperatures, top_ks, top_ps, min_ps)
     _check(lib().pk_sample(device, C.byref(a), stream), "pk_sample")

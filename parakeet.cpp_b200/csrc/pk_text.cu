@@ -338,8 +338,8 @@ extern "C" PK_API void pk_ctc_destroy(pk_ctc * c) {
 
 namespace {
 
-// Frames per product of pk_ctc_decode: bounds its logits (0.5 GB at 8193 tokens).
-constexpr int64_t kHeadFrames = 16384;
+// Frames per product of pk_ctc_decode, and values of its logits (1 GiB of them).
+constexpr int64_t kHeadFrames = 16384, kHeadLogits = 1ll << 28;
 
 // Logits of every frame (`x` itself, or head * x) to its token in c->best: the argmax or a draw.
 pk_status ctc_frame_tokens(pk_ctc * c, const char * fn, pk_mx4 * head, const float * dx, int64_t frames, const pk_ctc_draw * draw,
@@ -348,7 +348,7 @@ pk_status ctc_frame_tokens(pk_ctc * c, const char * fn, pk_mx4 * head, const flo
     cudaStream_t s = c->stream;
     int K = c->V;
     if (head) mx4_dims(head, nullptr, nullptr, &K);
-    const int64_t step = head ? std::min(frames, kHeadFrames) : frames;
+    const int64_t step = head ? std::min({frames, kHeadFrames, std::max<int64_t>(kHeadLogits / c->V, 1)}) : frames;
     if (head) {
         const int64_t ws = pk_mx4_workspace(head, step);
         TX_CK(c->logits.ensure((size_t) step * c->V * 4), fn);

@@ -148,6 +148,9 @@ def test_refusals(built):
         assert call(**kw) == abi.PK_ERR_INVALID, kw
         assert b"pk_sample" in L.pk_last_error()
     assert L.pk_sample(0, None, None) == abi.PK_ERR_INVALID
+    for vocab in (0, -1, abi.PK_SAMPLE_MAX_VOCAB + 1, (1 << 32) + 4):       # nothing that 32 bits would cut to a size
+        with pytest.raises(ValueError, match="vocab"):
+            pk.sample(p, 1, vocab, p, p)
     assert L.pk_ctc_decode(None, None, None, 0, None, None, 0, None, None, None, 0, None, None, None) == abi.PK_ERR_INVALID
 
 
@@ -500,6 +503,24 @@ def test_ctc_decode(built, with_head, drawn, on_device):
     if not with_head and not drawn:
         again, _, _ = ctc.decode(x, offs, n_frames, prev=prev0)
         assert all(np.array_equal(a, c) for a, c in zip(got, again))
+    ctc.close()
+
+
+@pytest.mark.gpu
+def test_ctc_decode_wide_head(built):
+    """A head so wide that its logits, not the frames, bound a product. Small integers throughout: every
+    sum is exact, whichever kernel takes it."""
+    import torch
+    pk = built
+    rng = np.random.default_rng(2)
+    v, k, total = 40_000, 64, 7_000
+    w = rng.integers(-2, 3, (v, k)).astype(np.float32)
+    x = rng.integers(-2, 3, (total, k)).astype(np.float32)
+    path = (torch.from_numpy(x).cuda() @ torch.from_numpy(w).cuda().T).cpu().numpy().argmax(1)   # the first of equal ones
+    ctc = pk.CtcGreedy(v, v - 1)
+    got, _, prev = ctc.decode_frames(x, [0], [total], head=pk.Mx4Linear(w))
+    t, _, p = collapse(path, v - 1, -1)
+    assert got[0].tolist() == t and prev[0] == p
     ctc.close()
 
 
