@@ -59,15 +59,60 @@ __device__ __forceinline__ unsigned cvt_e2m1x2(float lo, float hi) {
 // Eight consecutive elements of a row, as loaded.
 template <class T> struct alignas(16) Eight { T e[8]; };
 
+// The four values from column c of a row on, zeros for what is not in the row. 16-byte aligned.
+__device__ __forceinline__ void four_of(const float * __restrict__ row, int c, int K, unsigned * w) {
+    if (c >= 0 && c + 4 <= K) {
+        const uint4 q = __ldg(reinterpret_cast<const uint4 *>(row + c));
+        w[0] = q.x;
+        w[1] = q.y;
+        w[2] = q.z;
+        w[3] = q.w;
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = 0;
+    if (c >= K) return;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (c + i < 0 || c + i >= K) continue;
+        w[i] = __float_as_uint(__ldg(row + c + i));
+    }
+}
+
+// Words from byte `off` (below 16, whole elements) of N + 4 words on, N of them, to the front.
+template <int N, int ES>
+__device__ __forceinline__ void shift_words(unsigned * w, int off) {
+#pragma unroll
+    for (int i = 0; i < N + 2; ++i) w[i] = off & 8 ? w[i + 2] : w[i];
+#pragma unroll
+    for (int i = 0; i < N + 1; ++i) w[i] = off & 4 ? w[i + 1] : w[i];
+    if constexpr (ES == 2) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], (off & 2) * 8);
+    }
+}
+
+// Eight elements of a row from column c (a multiple of eight) on, zeros from column K on. VEC: rows are
+// 16-byte aligned. Otherwise f32 loads the aligned 16 bytes around and shifts them into place (66043 x 1000:
+// 62 us, element by element 74); half precision goes by elements, whose second to eighth load hits the first
+// one's lines (49 us; the other way 66, for the row ends' sake).
 template <class T, bool VEC>
 __device__ __forceinline__ Eight<T> load8(const T * __restrict__ row, int c, int K) {
     Eight<T> v;
-    if (VEC && c + 8 <= K) {
+    if constexpr (!VEC && sizeof(T) == 4) {
+        const int off = (int) (reinterpret_cast<uintptr_t>(row) & 15), at = c - off / 4;
+        unsigned w[12];
+        four_of(row, at, K, w);
+        four_of(row, at + 4, K, w + 4);
+        four_of(row, at + 8, off ? K : 0, w + 8);
+        shift_words<8, 4>(w, off);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v.e[i] = __uint_as_float(w[i]);
+    } else if (VEC && c + 8 <= K) {
 #pragma unroll
         for (int i = 0; i < (int) sizeof(T) / 2; ++i)
             reinterpret_cast<uint4 *>(v.e)[i] = __ldcs(reinterpret_cast<const uint4 *>(row + c) + i);
     } else {
-        // zeros from column K on
 #pragma unroll
         for (int i = 0; i < 8; ++i) v.e[i] = from_f32<T>(0.0f);
         if (c < K) {
@@ -77,6 +122,62 @@ __device__ __forceinline__ Eight<T> load8(const T * __restrict__ row, int c, int
         }
     }
     return v;
+}
+
+// The other way: a group of `lanes` neighbouring lanes, this one the sub-th, has eight elements each from
+// column c on; what lies before column K is stored. The whole warp calls. `on`: this lane's row is there.
+// Not VEC: each lane stores the aligned 16 bytes that its neighbour's elements begin, what the ends of a row
+// or of the warp's piece of it cut by elements (66043 x 1000 bf16: 67 us, by elements throughout 175).
+template <class T, bool VEC>
+__device__ __forceinline__ void store8(T * __restrict__ row, int c, int K, const Eight<T> & o, int sub, int lanes, bool on) {
+    if constexpr (VEC) {
+        if (!on) return;
+        if (c + 8 <= K) {
+#pragma unroll
+            for (int i = 0; i < (int) sizeof(T) / 2; ++i) reinterpret_cast<uint4 *>(row + c)[i] = reinterpret_cast<const uint4 *>(o.e)[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (c + i < K) row[c + i] = o.e[i];
+        }
+    } else {
+        constexpr int ES = (int) sizeof(T), N = 2 * ES, PER = 16 / ES;
+        const unsigned * own = reinterpret_cast<const unsigned *>(o.e);
+        const int off = (int) (reinterpret_cast<uintptr_t>(row) & 15), bytes = K * ES;
+        unsigned w[N + 4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = __shfl_up_sync(0xFFFFFFFFu, own[N - 4 + i], 1);
+#pragma unroll
+        for (int i = 0; i < N; ++i) w[4 + i] = own[i];
+        if (!on) return;
+        shift_words<N, ES>(w, (16 - off) & 15);
+        char * at = reinterpret_cast<char *>(row);
+        const int from = sub == 0 ? c * ES : 0;          // what lies before is another warp's
+#pragma unroll
+        for (int i = 0; i < N; i += 4) {
+            if (off == 0) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) w[i + j] = own[i + j];
+            }
+            const int b = c * ES - off + 4 * i;
+            if (b >= from && b + 16 <= bytes) {
+                *reinterpret_cast<uint4 *>(at + b) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
+            } else if (b < bytes) {
+#pragma unroll
+                for (int j = 0; j < PER; ++j) {
+                    const int e = b + j * ES;
+                    if (e < from || e >= bytes) continue;
+                    if constexpr (ES == 4) *reinterpret_cast<unsigned *>(at + e) = w[i + j];
+                    else *reinterpret_cast<unsigned short *>(at + e) = (unsigned short) (w[i + (j >> 1)] >> (16 * (j & 1)));
+                }
+            }
+        }
+        if (sub == lanes - 1) {                          // the end of the last lane's elements has no lane behind it
+#pragma unroll
+            for (int j = 1; j < 8; ++j)
+                if ((8 - j) * ES <= off && c + j < K) row[c + j] = o.e[j];
+        }
+    }
 }
 
 // Largest magnitude of three; a NaN if one is.
@@ -163,12 +264,14 @@ __device__ __forceinline__ unsigned scale_word(unsigned sb) {
 }
 
 // A warp's 256 values of a row: eight per lane. Where a row goes on, the next 256 follow in the same
-// warp, gridDim.y segments further on; several loads are in flight before the first is used.
+// warp, gridDim.y segments further on; several loads are in flight before the first is used. SHORT, for
+// rows of up to 256 values: 2^gs lanes a row, and the next rows instead of the next segments (483966 rows of
+// 49 bf16: 24 us, a warp a row 114).
 // ATOMS: scales in the product's layout, zeros for the blocks past K that its stages read.
 // Bound: HBM from f32 (66044 x 1024: 44 us, 6.9 TB/s read and written), instructions from half precision
 // (66043 x 1000 bf16: 34 us, 4.9 TB/s).
-template <class T, bool VEC, bool ATOMS>
-__global__ void __launch_bounds__(kQThreads) mx4_quantize_kernel(const T * __restrict__ x, long long rows, int K, long long ldx,
+template <class T, bool VEC, bool ATOMS, bool SHORT>
+__global__ void __launch_bounds__(kQThreads) mx4_quantize_kernel(const T * __restrict__ x, long long rows, int K, long long ldx, int gs,
                                                                  unsigned char * __restrict__ codes,
                                                                  unsigned char * __restrict__ scales) {
     constexpr int UN = sizeof(T) == 4 ? 2 : 4;
@@ -176,30 +279,64 @@ __global__ void __launch_bounds__(kQThreads) mx4_quantize_kernel(const T * __res
     // the product may set itself up while the last blocks work; it waits for all of them before it loads
     if (ATOMS) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int segs = (K + 255) >> 8, nb = (K + 31) >> 5, chunks = scale_chunks(K);
-    const long long stride = (long long) gridDim.x * (kQThreads / 32);
-    for (long long row = (long long) blockIdx.x * (kQThreads / 32) + (threadIdx.x >> 5); row < rows; row += stride) {
-        const T * xr = x + row * ldx;
-        unsigned char * cr = codes + (size_t) row * nb * 16 + lane * 4;
-        for (int s0 = blockIdx.y; s0 < segs; s0 += UN * (int) gridDim.y) {
+    long long row = (long long) blockIdx.x * (kQThreads / 32) + (threadIdx.x >> 5);
+    long long stride = (long long) gridDim.x * (kQThreads / 32);
+    if constexpr (SHORT) {
+        const int sub = lane & ((1 << gs) - 1), blk = sub >> 2;
+        row = (row << (5 - gs)) + (lane >> gs);
+        stride <<= 5 - gs;
+        for (; __any_sync(0xFFFFFFFFu, row < rows); row += UN * stride) {
             Eight<T> v[UN];
 #pragma unroll
             for (int u = 0; u < UN; ++u) {
-                const int seg = s0 + u * (int) gridDim.y;
-                v[u] = load8<T, VEC>(xr, seg < segs ? seg * 256 + lane * 8 : K, K);
+                const bool on = row + u * stride < rows;
+                v[u] = load8<T, VEC>(x + (on ? (row + u * stride) * ldx : 0), on ? sub * 8 : 256, on ? K : 0);
             }
 #pragma unroll
             for (int u = 0; u < UN; ++u) {
-                const int seg = s0 + u * (int) gridDim.y;
-                if (seg >= segs) break;
-                const int blk = seg * 8 + (lane >> 2);
+                const long long r = row + u * stride;
                 unsigned sb;
                 const unsigned q = quantize8(v[u], sb);
-                if (blk < nb) *reinterpret_cast<unsigned *>(cr + (size_t) seg * 128) = q;
+                if (r < rows && blk < nb) *reinterpret_cast<unsigned *>(codes + (size_t) r * nb * 16 + sub * 4) = q;
                 if (ATOMS) {
+                    // two words a row: with fewer lanes than blocks in them, other rows' bytes are zeros here
                     const unsigned word = scale_word(sb);
-                    if ((lane & 15) == 0) *reinterpret_cast<unsigned *>(scales + scale_at(row, blk, chunks)) = word;
-                } else if ((lane & 3) == 0 && blk < nb) {
-                    scales[(size_t) row * nb + blk] = (unsigned char) sb;
+                    if (gs == 5) {
+                        if (r < rows && (lane & 15) == 0) *reinterpret_cast<unsigned *>(scales + scale_at(r, blk, chunks)) = word;
+                    } else if (r < rows && sub < 2) {
+                        *reinterpret_cast<unsigned *>(scales + scale_at(r, sub * 4, chunks)) =
+                            sub == 0 ? word & (0xFFFFFFFFu >> (32 - 8 * nb)) : 0u;
+                    }
+                } else if (r < rows && (lane & 3) == 0 && blk < nb) {
+                    scales[(size_t) r * nb + blk] = (unsigned char) sb;
+                }
+            }
+        }
+    } else {
+        for (; row < rows; row += stride) {
+            const T * xr = x + row * ldx;
+            unsigned char * cr = codes + (size_t) row * nb * 16 + lane * 4;
+            for (int s0 = blockIdx.y; s0 < segs; s0 += UN * (int) gridDim.y) {
+                Eight<T> v[UN];
+#pragma unroll
+                for (int u = 0; u < UN; ++u) {
+                    const int seg = s0 + u * (int) gridDim.y;
+                    v[u] = load8<T, VEC>(xr, seg < segs ? seg * 256 + lane * 8 : (K + 7) & ~7, K);
+                }
+#pragma unroll
+                for (int u = 0; u < UN; ++u) {
+                    const int seg = s0 + u * (int) gridDim.y;
+                    if (seg >= segs) break;
+                    const int blk = seg * 8 + (lane >> 2);
+                    unsigned sb;
+                    const unsigned q = quantize8(v[u], sb);
+                    if (blk < nb) *reinterpret_cast<unsigned *>(cr + (size_t) seg * 128) = q;
+                    if (ATOMS) {
+                        const unsigned word = scale_word(sb);
+                        if ((lane & 15) == 0) *reinterpret_cast<unsigned *>(scales + scale_at(row, blk, chunks)) = word;
+                    } else if ((lane & 3) == 0 && blk < nb) {
+                        scales[(size_t) row * nb + blk] = (unsigned char) sb;
+                    }
                 }
             }
         }
@@ -240,41 +377,59 @@ template <> __device__ __forceinline__ void codes_to_values(unsigned q, unsigned
     for (int i = 0; i < 4; ++i) reinterpret_cast<unsigned *>(o.e)[i] = word_of(__hmul2(pair_of<__nv_bfloat162>(w[i]), s2));
 }
 
-// The value of each code, eight a lane. Bound: HBM, writing y (66043 x 1000 bf16: 34 us, 4.9 TB/s).
-template <class T, bool VEC>
+// The value of each code, eight a lane, rows and lanes as in the quantisation. Bound: HBM, writing y
+// (66043 x 1000 bf16: 34 us, 4.9 TB/s).
+template <class T, bool VEC, bool SHORT>
 __global__ void __launch_bounds__(kQThreads) mx4_dequantize_kernel(const unsigned char * __restrict__ codes,
                                                                    const unsigned char * __restrict__ scales, long long rows,
-                                                                   int K, T * __restrict__ y, long long ldy) {
+                                                                   int K, T * __restrict__ y, long long ldy, int gs) {
     constexpr int UN = 4;
     const int lane = threadIdx.x & 31;
     const int segs = (K + 255) >> 8, nb = (K + 31) >> 5;
-    const long long stride = (long long) gridDim.x * (kQThreads / 32);
-    for (long long row = (long long) blockIdx.x * (kQThreads / 32) + (threadIdx.x >> 5); row < rows; row += stride) {
-        const unsigned char * cr = codes + (size_t) row * nb * 16 + lane * 4, * sr = scales + (size_t) row * nb + (lane >> 2);
-        for (int s0 = blockIdx.y; s0 < segs; s0 += UN * (int) gridDim.y) {
+    long long row = (long long) blockIdx.x * (kQThreads / 32) + (threadIdx.x >> 5);
+    long long stride = (long long) gridDim.x * (kQThreads / 32);
+    if constexpr (SHORT) {
+        const int sub = lane & ((1 << gs) - 1);
+        row = (row << (5 - gs)) + (lane >> gs);
+        stride <<= 5 - gs;
+        for (; __any_sync(0xFFFFFFFFu, row < rows); row += UN * stride) {
             unsigned q[UN];
             unsigned char b[UN];
 #pragma unroll
             for (int u = 0; u < UN; ++u) {
-                const int seg = s0 + u * (int) gridDim.y;
-                const bool in = seg * 256 + lane * 8 < K;
-                q[u] = in ? __ldcs(reinterpret_cast<const unsigned *>(cr + (size_t) seg * 128)) : 0u;
-                b[u] = in ? __ldcs(sr + seg * 8) : (unsigned char) 0;
+                const long long r = row + u * stride;
+                const bool in = r < rows && sub * 8 < K;
+                q[u] = in ? __ldcs(reinterpret_cast<const unsigned *>(codes + (size_t) r * nb * 16 + sub * 4)) : 0u;
+                b[u] = in ? __ldcs(scales + (size_t) r * nb + (sub >> 2)) : (unsigned char) 0;
             }
 #pragma unroll
             for (int u = 0; u < UN; ++u) {
-                const int c = (s0 + u * (int) gridDim.y) * 256 + lane * 8;
-                if (c >= K) continue;
+                const long long r = row + u * stride;
                 Eight<T> o;
                 codes_to_values(q[u], b[u], o);
-                T * d = y + row * ldy + c;
-                if (VEC && c + 8 <= K) {
+                store8<T, VEC>(y + (r < rows ? r * ldy : 0), sub * 8, K, o, sub, 1 << gs, r < rows);
+            }
+        }
+    } else {
+        for (; row < rows; row += stride) {
+            const unsigned char * cr = codes + (size_t) row * nb * 16 + lane * 4, * sr = scales + (size_t) row * nb + (lane >> 2);
+            for (int s0 = blockIdx.y; s0 < segs; s0 += UN * (int) gridDim.y) {
+                unsigned q[UN];
+                unsigned char b[UN];
 #pragma unroll
-                    for (int i = 0; i < (int) sizeof(T) / 2; ++i) reinterpret_cast<uint4 *>(d)[i] = reinterpret_cast<const uint4 *>(o.e)[i];
-                } else {
+                for (int u = 0; u < UN; ++u) {
+                    const int seg = s0 + u * (int) gridDim.y;
+                    const bool in = seg * 256 + lane * 8 < K;
+                    q[u] = in ? __ldcs(reinterpret_cast<const unsigned *>(cr + (size_t) seg * 128)) : 0u;
+                    b[u] = in ? __ldcs(sr + seg * 8) : (unsigned char) 0;
+                }
 #pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        if (c + i < K) d[i] = o.e[i];
+                for (int u = 0; u < UN; ++u) {
+                    const int seg = s0 + u * (int) gridDim.y;
+                    if (seg >= segs) break;
+                    Eight<T> o;
+                    codes_to_values(q[u], b[u], o);
+                    store8<T, VEC>(y + row * ldy, seg * 256 + lane * 8, K, o, lane, 32, true);
                 }
             }
         }
@@ -860,9 +1015,12 @@ mx4_few_kernel(const TX * __restrict__ x, long long ldx, int M, int K, const __g
     if (threadIdx.x == 0 && S.err != 0) atomicExch_system(err_out, 1);
 }
 
-// Launch of a row kernel: a warp a row, up to a few waves; with few rows a warp for each 256 values.
+// Lanes of a row, as a power of two.
+inline int row_lanes(long long K) { return K <= 32 ? 2 : K <= 64 ? 3 : K <= 128 ? 4 : 5; }
+
+// Launch of a row kernel: a warp for 32 lanes' rows, up to a few waves; with few rows a warp for each 256 values.
 inline dim3 row_blocks(long long rows, long long K) {
-    const long long x = std::min<long long>((rows + kQThreads / 32 - 1) / (kQThreads / 32), 148LL * 32);
+    const long long per = (kQThreads / 32) << (5 - row_lanes(K)), x = std::min<long long>((rows + per - 1) / per, 148LL * 32);
     const long long segs = (K + 255) / 256;
     return dim3((unsigned) x, (unsigned) std::max<long long>(1, std::min<long long>(segs, 148 * 8 / x)));
 }
@@ -872,14 +1030,18 @@ cudaError_t launch_quantize(const void * x, int type, long long rows, int K, lon
                             unsigned char * scales, cudaStream_t s) {
     if (rows <= 0) return cudaSuccess;
     const bool vec = aligned_to(x, 16) && (ldx * elem_size(type)) % 16 == 0;
+    const int gs = row_lanes(K);
     const dim3 g = row_blocks(rows, K);
+#define PK_Q2(T, V, S) mx4_quantize_kernel<T, V, ATOMS, S><<<g, kQThreads, 0, s>>>(static_cast<const T *>(x), rows, K, ldx, gs, codes, scales)
 #define PK_Q(T) \
-    if (vec) mx4_quantize_kernel<T, true, ATOMS><<<g, kQThreads, 0, s>>>(static_cast<const T *>(x), rows, K, ldx, codes, scales); \
-    else mx4_quantize_kernel<T, false, ATOMS><<<g, kQThreads, 0, s>>>(static_cast<const T *>(x), rows, K, ldx, codes, scales)
+    if (K <= 256) { if (vec) PK_Q2(T, true, true); else PK_Q2(T, false, true); } \
+    else if (vec) PK_Q2(T, true, false); \
+    else PK_Q2(T, false, false)
     if (type == PK_GGML_F32) { PK_Q(float); }
     else if (type == PK_GGML_F16) { PK_Q(__half); }
     else { PK_Q(__nv_bfloat16); }
 #undef PK_Q
+#undef PK_Q2
     return cudaGetLastError();
 }
 
@@ -1120,14 +1282,18 @@ extern "C" PK_API pk_status pk_mx4_dequantize(int device, const uint8_t * codes,
     if (dev.err != cudaSuccess) return op_cuda_fail(dev.err, fn);
     const bool vec = aligned_to(y, 16) && (row_stride * elem_size(y_type)) % 16 == 0;
     const dim3 g = row_blocks(rows, cols);
+    const int gs = row_lanes(cols);
     cudaStream_t s = (cudaStream_t) stream;
+#define PK_D2(T, V, S) mx4_dequantize_kernel<T, V, S><<<g, kQThreads, 0, s>>>(codes, scales, rows, (int) cols, static_cast<T *>(y), row_stride, gs)
 #define PK_D(T) \
-    if (vec) mx4_dequantize_kernel<T, true><<<g, kQThreads, 0, s>>>(codes, scales, rows, (int) cols, static_cast<T *>(y), row_stride); \
-    else mx4_dequantize_kernel<T, false><<<g, kQThreads, 0, s>>>(codes, scales, rows, (int) cols, static_cast<T *>(y), row_stride)
+    if (cols <= 256) { if (vec) PK_D2(T, true, true); else PK_D2(T, false, true); } \
+    else if (vec) PK_D2(T, true, false); \
+    else PK_D2(T, false, false)
     if (y_type == PK_GGML_F32) { PK_D(float); }
     else if (y_type == PK_GGML_F16) { PK_D(__half); }
     else { PK_D(__nv_bfloat16); }
 #undef PK_D
+#undef PK_D2
     const cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? PK_OK : op_cuda_fail(e, fn);
 }

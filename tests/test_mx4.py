@@ -168,6 +168,51 @@ def test_quantize_and_back(built, dtype, pad, shift, r, k):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,pad,shift", [("f32", 0, 0), ("f32", 3, 1), ("f16", 1, 3), ("bf16", 0, 0), ("bf16", 2, 1)])
+@pytest.mark.parametrize("k", [1, 7, 24, 31, 32, 33, 49, 64, 65, 104, 128, 129, 250, 256])
+def test_many_short_rows(built, k, dtype, pad, shift):
+    """Several rows a warp and several warps' rounds of them, every phase of a row's start; a NaN and an
+    infinity stay with their own row's block."""
+    import torch
+    pk = built
+    r = 3001
+    x = values_like(np.random.default_rng(k), r, k)
+    if dtype == "f16":
+        x = np.clip(x, -6e4, 6e4)
+    x[5, k // 2], x[900, 0], x[3000, k - 1] = np.nan, np.inf, -np.inf
+    seen, codes, scales = run_quantize(pk, x, dtype, pad, shift)
+    nb = -(-k // 32)
+    code, byte, val = ref_quantize(seen)
+    assert np.array_equal(codes[:r * nb * 16].view(r, -1).cpu().numpy(), pack(code, nb))
+    assert np.array_equal(scales[:r * nb].view(r, nb).cpu().numpy(), byte)
+    s = torch.cuda.current_stream().cuda_stream
+    for out, opad, oshift in (("f32", 0, 0), ("f32", 1, 1), ("f32", 2, 2), ("bf16", 0, 0), ("bf16", 7, 5), ("f16", 3, 7)):
+        buf, y = cuda(np.full((r, k), 5.0), out, opad, oshift)
+        before = buf.clone()
+        pk.mx4_dequantize(codes.data_ptr(), scales.data_ptr(), r, k, y.data_ptr(), dtype=out, row_stride=k + opad, stream=s)
+        want = torch.from_numpy(val).to(y.dtype).float().numpy()
+        assert np.array_equal(y[:, :k].float().cpu().numpy(), want, equal_nan=True)
+        y[:, :k] = 5.0
+        assert torch.equal(buf, before)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,pad,shift", [("f32", 0, 0), ("bf16", 3, 1)])
+@pytest.mark.parametrize("k", [1, 24, 32, 33, 64, 65, 128, 129, 256])
+def test_product_of_short_rows(built, k, dtype, pad, shift):
+    """Rows whose scales do not fill the words that the product reads, next to a row of NaN."""
+    pk = built
+    rng = np.random.default_rng(k)
+    w = rng.standard_normal((70, k)).astype(np.float32)
+    x = rng.standard_normal((515, k)).astype(np.float32)
+    x[11] = np.nan
+    seen, y = product(pk, w, x, x_dtype=dtype, xpad=pad, shift=shift)
+    assert np.isnan(y[11]).all()
+    keep = np.arange(515) != 11
+    check_product(ref_quantize(w)[2], seen[keep], y[keep])
+
+
+@pytest.mark.gpu
 def test_quantize_borders(built):
     """Every tie and neighbour of a tie, at the lowest, a middle and the highest scale; special blocks."""
     pk = built
