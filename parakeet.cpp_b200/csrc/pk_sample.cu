@@ -809,9 +809,13 @@ __device__ int nucleus_f32(Team<NT, false> & team, TeamBins<NT> * B, const Slice
     });
     auto fixed = [](float w) { return (u64) __double2ull_rn((double) w * kFix); };
     const float mine = (part[0] + part[1]) + (part[2] + part[3]);
-    // a NaN or an overflow shows in every sum it enters; weights are at most about one each
-    const u64 total = team.sum(mine < 1e6f ? fixed(mine) : 1ull << 62);
-    if (total >= 1ull << 58) return kNothing;
+    // A thread's at most 64 weights of at most 2^(2^-24 |k|) < 1.05 each stay below 128; a NaN shows in the sum that
+    // it enters. What such a thread gives instead is more than all threads' honest sums (NT 68 2^40) together, and
+    // less than would wrap if every thread gave it.
+    constexpr u64 kBad = 1ull << 55;
+    static_assert(NT <= 256, "honest sums below kBad, NT times kBad below 2^64");
+    const u64 total = team.sum(mine < 128.0f ? fixed(mine) : kBad);
+    if (total >= kBad) return kNothing;
     const double S = (double) total, E = S * kOff;
     // bounds of what the bins hold, and the first that may and the first that must reach the share
     const float width = (hi - from) / (float) NB;

@@ -542,3 +542,22 @@ def test_ctc_decode_many_frames_and_refusals(built):
         ctc.decode_frames(x, [0], [10], head=head, uniforms=np.zeros(9, np.float32))
     out, _, prev = ctc.decode_frames(np.zeros((0, k), np.float32), [], [], head=head)
     assert out == [] and len(prev) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("r,v", [(1, 1000), (40, 1000), (300, 1500), (297, 8193), (600, 4000)])
+@pytest.mark.parametrize("quads", [1, 4, 8, 128])
+def test_nan_logits_with_top_p(built, r, v, quads, dtype):
+    """NaN logits count as -infinity however many threads meet one: a multiple of four of them, each with one
+    of the heaviest tokens beside it, must not pass for a sum without them."""
+    rng = np.random.default_rng(quads * 100 + v)
+    l = rng.standard_normal((r, v)) * 0.3
+    for q in range(quads):
+        l[:, 4 * q] = np.nan
+        l[:, 4 * q + 1] = 4.0 + 0.25 * (q % 7)
+    u = rng.random(r).astype(np.float32)
+    for kw in (dict(top_p=0.9), dict(top_p=0.5, temperature=0.7), dict(top_p=0.99, min_p=0.001)):
+        seen, tok, lp = run(built, l, u, dtype, **kw)
+        check(seen, u, tok, lp, **kw)
+        assert not np.isnan(seen[np.arange(r), tok]).any()
