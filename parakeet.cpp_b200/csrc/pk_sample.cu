@@ -66,7 +66,10 @@ struct Row {
 // |t| <= 1/2; 2^(n / 32) from the table's entry n % 32 and n / 32 added to its exponent, 2^(t / 32)
 // = 1 + t q(t) with q cubic, interpolating at the four Chebyshev nodes of [-1/2, 1/2] (off by
 // 2^-42.5 at most; exactly 1 at t = 0). Adding a number of [2^52, 2^53) rounds the product to an
-// integer in the low bits. `entry(n)` gives 2^43 * table[n % 32] with n % 32 taken off the exponent
+// integer in the low bits. A product halfway between two integers would go to the one that makes the
+// sum so far even, and sums would depend on their order: the last bit of the value at t is set (1 still
+// rounds to 2^43), which leaves the product its lowest bit far below a half, 2^-9 at the most, and no
+// product is halfway. `entry(n)` gives 2^43 * table[n % 32] with n % 32 taken off the exponent
 // field's place 15 bits up, where all of n is added. All callers share these operations.
 template <class F>
 __device__ __forceinline__ double weight_onto(float v, const Row & r, double onto, F entry) {
@@ -79,6 +82,7 @@ __device__ __forceinline__ double weight_onto(float v, const Row & r, double ont
     q = fma(q, t, 0.00023459619820112603);
     q = fma(q, t, 0.021660849392187844);
     q = fma(q, t, 1.0);
+    q = __hiloint2double(__double2hiint(q), __double2loint(q) | 1);
     const int n = __double2loint(y);
     const double e = entry(n);
     return fma(q, __hiloint2double(__double2hiint(e) + (n << 15), __double2loint(e)), onto);
@@ -1129,8 +1133,7 @@ sample_kernel(pk_sample_args a, int slice, int teams, int row_floats) {
         }
     }
     const int i0 = RES ? team.tid * len : min(team.tid * len, l.n), i1 = RES ? i0 + len : min(i0 + len, l.n);
-    // a run has fewer than 2^9 elements, so its sum stays below 2^53 and is whole. (A product that
-    // lies halfway between two integers may round the other way here than by itself; see the search.)
+    // a run has fewer than 2^9 elements, so its sum stays below 2^53 and is whole
     double onto = kZero;
     const float from = fmaxf(least, cut);
     unsigned equal = 0;
@@ -1171,7 +1174,6 @@ sample_kernel(pk_sample_args a, int slice, int teams, int row_floats) {
         // the run again, 32 elements at a time
         const int e = min((who + 1) * len, l.n);
         u64 run = team.s->found_before, tie = FILTERS ? (u64) team.s->found_ties : 0ull;
-        int last = -1;                       // should rounding have left t at the run's very end: its last token
         for (int c = who * len; c < e; c += 32) {
             const int i = c + team.tid;
             const float v = i < e ? l(i) : -CUDART_INF_F;
@@ -1187,10 +1189,7 @@ sample_kernel(pk_sample_args a, int slice, int teams, int row_floats) {
             if (x - w <= t && t < x) write_token(a, row, s0 + i, v, hi, inv_t, total);
             run = __shfl_sync(kFull, x, 31);
             if (run > t) break;
-            const unsigned some = __ballot_sync(kFull, w > 0);
-            if (some) last = c + 31 - __clz(some);
         }
-        if (run <= t && team.tid == 0 && last >= 0) write_token(a, row, s0 + last, l(last), hi, inv_t, total);
     }
     if (CL) team.meet();                                         // a block's memory stays while others may read it
 }

@@ -561,3 +561,21 @@ def test_nan_logits_with_top_p(built, r, v, quads, dtype):
         seen, tok, lp = run(built, l, u, dtype, **kw)
         check(seen, u, tok, lp, **kw)
         assert not np.isnan(seen[np.arange(r), tok]).any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kw", [dict(), dict(min_p=1e-6), dict(top_p=0.9999999)], ids=["plain", "m", "p"])
+@pytest.mark.parametrize("v", [64, 450, 900])
+def test_halves_of_the_same_weights(built, v, kw):
+    """Rows whose second half holds the first one's weights in another order, all of them near the largest: with
+    u = 1/2 the running sum over the first half is u times the total exactly, so the token is the second half's
+    first, whatever the order in which the weights were added up (v weights of 2^43 stay below 2^53: u times
+    their total is not rounded)."""
+    rng = np.random.default_rng(v)
+    h = v // 2
+    for r in (1, 7, 300, 700, 1300, 3100):
+        base = (-0.01 * rng.random((r, h))).astype(np.float32)
+        base[:, 0] = 0.0
+        l = np.concatenate([rng.permuted(base, axis=1), rng.permuted(base, axis=1)], 1)
+        _, tok, _ = run(built, l, np.full(r, 0.5, np.float32), **kw)
+        assert (tok == h).all(), (r, np.unique(tok))
