@@ -389,6 +389,8 @@ class CtcGreedy:
         """pk_ctc_decode: decode() from encoder frames through `head` (an Mx4Linear, vocab_size wide), or from logits
         without one; with `uniforms` (one random number per frame) each frame's token is drawn, else the argmax.
         frames / uniforms: float32 arrays, or device pointers (int) with their flag."""
+        if head is not None and not head.h.value:
+            raise ValueError("the head is closed")
         n_frames = np.ascontiguousarray(n_frames, dtype=np.int32)
         B = len(n_frames)
         foff = np.ascontiguousarray(frame_offsets, dtype=np.int64)

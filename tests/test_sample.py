@@ -579,3 +579,14 @@ def test_halves_of_the_same_weights(built, v, kw):
         l = np.concatenate([rng.permuted(base, axis=1), rng.permuted(base, axis=1)], 1)
         _, tok, _ = run(built, l, np.full(r, 0.5, np.float32), **kw)
         assert (tok == h).all(), (r, np.unique(tok))
+
+
+def test_closed_head_is_refused(built):
+    """A closed layer's handle is null, which the C entry point takes for frames that are logits already."""
+    pk = built
+    ctc = pk.CtcGreedy.__new__(pk.CtcGreedy)               # no device here: nothing is called with these handles
+    ctc._h, ctc.vocab_size, ctc.blank_id = None, 1025, 1024
+    head = pk.Mx4Linear.__new__(pk.Mx4Linear)
+    head.h, head.n, head.k, head.device = C.c_void_p(), 1025, 1024, 0      # as close() leaves it
+    with pytest.raises(ValueError, match="closed"):
+        ctc.decode_frames(np.zeros((4, 1024), np.float32), [0], [4], head=head)
