@@ -360,13 +360,22 @@ class CtcGreedy:
         except Exception:
             pass
 
+    @staticmethod
+    def _windows(frame_offsets, n_frames, prev):
+        """The utterances' arrays as the C entry points read them: one entry of each for every utterance."""
+        n_frames = np.ascontiguousarray(n_frames, dtype=np.int32).reshape(-1)
+        B = len(n_frames)
+        foff = np.ascontiguousarray(frame_offsets, dtype=np.int64).reshape(-1)
+        prev = np.full(B, -1, np.int32) if prev is None else np.array(prev, dtype=np.int32, copy=True).reshape(-1)
+        if len(foff) != B or len(prev) != B:
+            raise ValueError(f"{len(foff)} frame offsets and {len(prev)} previous tokens for {B} utterances")
+        return n_frames, foff, prev
+
     def decode(self, logits, frame_offsets, n_frames, prev=None, on_device=False, with_frames=False):
         """logits: [frames][vocab] float32 (numpy, or a device pointer int with on_device).
         Returns (token lists, frame lists or None, new prev array)."""
-        n_frames = np.ascontiguousarray(n_frames, dtype=np.int32)
+        n_frames, foff, prev = self._windows(frame_offsets, n_frames, prev)
         B = len(n_frames)
-        foff = np.ascontiguousarray(frame_offsets, dtype=np.int64)
-        prev = np.full(B, -1, np.int32) if prev is None else np.array(prev, dtype=np.int32, copy=True)
         cap = int(n_frames.sum())
         toks = np.zeros(max(cap, 1), np.int32)
         frs = np.zeros(max(cap, 1), np.int32) if with_frames else None
@@ -376,6 +385,9 @@ class CtcGreedy:
             lp = C.c_void_p(int(logits))
         else:
             logits = np.ascontiguousarray(logits, dtype=np.float32)
+            total = int((foff + n_frames).max()) if B else 0
+            if logits.size < total * self.vocab_size:
+                raise ValueError(f"logits hold {logits.size} values, the utterances read {total} x {self.vocab_size}")
             lp = _p(logits)
         _check(lib().pk_ctc_greedy(self._h, lp, 1 if on_device else 0, _p(foff), _p(n_frames), B, _p(prev),
                                    _p(toks), cap, _p(toff), _p(frs) if with_frames else None, C.byref(need)),
@@ -391,10 +403,8 @@ class CtcGreedy:
         frames / uniforms: float32 arrays, or device pointers (int) with their flag."""
         if head is not None and not head.h.value:
             raise ValueError("the head is closed")
-        n_frames = np.ascontiguousarray(n_frames, dtype=np.int32)
+        n_frames, foff, prev = self._windows(frame_offsets, n_frames, prev)
         B = len(n_frames)
-        foff = np.ascontiguousarray(frame_offsets, dtype=np.int64)
-        prev = np.full(B, -1, np.int32) if prev is None else np.array(prev, dtype=np.int32, copy=True)
         cap = int(n_frames.sum())
         total = int((foff + n_frames).max()) if B else 0
         toks = np.zeros(max(cap, 1), np.int32)

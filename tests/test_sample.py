@@ -590,3 +590,19 @@ def test_closed_head_is_refused(built):
     head.h, head.n, head.k, head.device = C.c_void_p(), 1025, 1024, 0      # as close() leaves it
     with pytest.raises(ValueError, match="closed"):
         ctc.decode_frames(np.zeros((4, 1024), np.float32), [0], [4], head=head)
+
+
+def test_arrays_too_short_are_refused(built):
+    """Offsets, previous tokens or logits for fewer utterances than there are: the C entry points would read past them."""
+    pk = built
+    ctc = pk.CtcGreedy.__new__(pk.CtcGreedy)
+    ctc._h, ctc.vocab_size, ctc.blank_id = None, 5, 0
+    x = np.zeros((8, 5), np.float32)
+    for call in (ctc.decode, ctc.decode_frames):
+        for offs, n, prev in (([0], [4, 4], None), ([0, 4, 8], [4, 4], None), ([0, 4], [4, 4], [1]), ([0, 4], [4, 4], [1, 2, 3])):
+            with pytest.raises(ValueError, match="utterances"):
+                call(x, offs, n, prev=prev)
+        with pytest.raises(ValueError, match="values"):
+            call(x, [0, 4], [4, 5])
+        with pytest.raises(pk.PkError):                    # lengths agree: on to the handle, which is null here
+            call(x, [0, 4], [4, 4], prev=[1, 2])
