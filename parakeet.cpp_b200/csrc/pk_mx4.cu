@@ -1032,17 +1032,12 @@ cudaError_t launch_quantize(const void * x, int type, long long rows, int K, lon
     const bool vec = aligned_to(x, 16) && (ldx * elem_size(type)) % 16 == 0;
     const int gs = row_lanes(K);
     const dim3 g = row_blocks(rows, K);
-#define PK_Q2(T, V, S) mx4_quantize_kernel<T, V, ATOMS, S><<<g, kQThreads, 0, s>>>(static_cast<const T *>(x), rows, K, ldx, gs, codes, scales)
+#define PK_Q2(T, V, S) launch_on(mx4_quantize_kernel<T, V, ATOMS, S>, g, kQThreads, 0, s, static_cast<const T *>(x), rows, K, ldx, gs, codes, scales)
 #define PK_Q(T) \
-    if (K <= 256) { if (vec) PK_Q2(T, true, true); else PK_Q2(T, false, true); } \
-    else if (vec) PK_Q2(T, true, false); \
-    else PK_Q2(T, false, false)
-    if (type == PK_GGML_F32) { PK_Q(float); }
-    else if (type == PK_GGML_F16) { PK_Q(__half); }
-    else { PK_Q(__nv_bfloat16); }
+    (K <= 256 ? (vec ? PK_Q2(T, true, true) : PK_Q2(T, false, true)) : vec ? PK_Q2(T, true, false) : PK_Q2(T, false, false))
+    return type == PK_GGML_F32 ? PK_Q(float) : type == PK_GGML_F16 ? PK_Q(__half) : PK_Q(__nv_bfloat16);
 #undef PK_Q
 #undef PK_Q2
-    return cudaGetLastError();
 }
 
 // Host-visible error words of the layers, from pages that stay: a layer's creation pays for no
@@ -1184,9 +1179,8 @@ cudaError_t launch_few_as(const Call & c) {
     const cudaError_t e = allow_smem(kernel, few_smem(kFewK / 256), c.w->device, set);
     if (e != cudaSuccess) return e;
     const int grid = std::min((c.w->N + kFewN - 1) / kFewN, 148);
-    kernel<<<grid, kFewThreads, few_smem(c.w->chunks / 2), c.s>>>(static_cast<const TX *>(c.x), c.ldx, (int) c.M, c.w->K, c.w->map[0],
-                                                                  c.w->scales, c.w->N, c.w->bias, static_cast<TY *>(c.y), c.ldy, c.w->err_dev);
-    return cudaGetLastError();
+    return launch_on(kernel, dim3(grid), kFewThreads, few_smem(c.w->chunks / 2), c.s, static_cast<const TX *>(c.x), c.ldx, (int) c.M, c.w->K,
+                     c.w->map[0], c.w->scales, c.w->N, c.w->bias, static_cast<TY *>(c.y), c.ldy, c.w->err_dev);
 }
 
 template <class TX, class TY> cudaError_t launch_few_xy(const Call & c) {
@@ -1284,17 +1278,12 @@ extern "C" PK_API pk_status pk_mx4_dequantize(int device, const uint8_t * codes,
     const dim3 g = row_blocks(rows, cols);
     const int gs = row_lanes(cols);
     cudaStream_t s = (cudaStream_t) stream;
-#define PK_D2(T, V, S) mx4_dequantize_kernel<T, V, S><<<g, kQThreads, 0, s>>>(codes, scales, rows, (int) cols, static_cast<T *>(y), row_stride, gs)
+#define PK_D2(T, V, S) launch_on(mx4_dequantize_kernel<T, V, S>, g, kQThreads, 0, s, codes, scales, rows, (int) cols, static_cast<T *>(y), row_stride, gs)
 #define PK_D(T) \
-    if (cols <= 256) { if (vec) PK_D2(T, true, true); else PK_D2(T, false, true); } \
-    else if (vec) PK_D2(T, true, false); \
-    else PK_D2(T, false, false)
-    if (y_type == PK_GGML_F32) { PK_D(float); }
-    else if (y_type == PK_GGML_F16) { PK_D(__half); }
-    else { PK_D(__nv_bfloat16); }
+    (cols <= 256 ? (vec ? PK_D2(T, true, true) : PK_D2(T, false, true)) : vec ? PK_D2(T, true, false) : PK_D2(T, false, false))
+    const cudaError_t e = y_type == PK_GGML_F32 ? PK_D(float) : y_type == PK_GGML_F16 ? PK_D(__half) : PK_D(__nv_bfloat16);
 #undef PK_D
 #undef PK_D2
-    const cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? PK_OK : op_cuda_fail(e, fn);
 }
 
@@ -1352,9 +1341,8 @@ extern "C" PK_API pk_status pk_mx4_create(int device, const pk_tensor * weight, 
     }
     if (e == cudaSuccess && type == PK_GGML_MXFP4) {
         const long long n = N * (long long) w->nb;
-        mx4_repack_kernel<<<(unsigned) ((n + kQThreads - 1) / kQThreads), kQThreads, 0, s>>>(
-            static_cast<const unsigned char *>(src), N, w->nb, w->codes, w->scales);
-        e = cudaGetLastError();
+        e = launch_on(mx4_repack_kernel, dim3((unsigned) ((n + kQThreads - 1) / kQThreads)), kQThreads, 0, s,
+                      static_cast<const unsigned char *>(src), N, w->nb, w->codes, w->scales);
     } else if (e == cudaSuccess && type == PK_GGML_Q8_0) {
         e = cudaMalloc(&f32, (size_t) N * K * 4);
         if (e == cudaSuccess) e = launch_dequant(src, type, K, N, static_cast<float *>(f32), s);

@@ -9,6 +9,7 @@
 #include <cuda_fp16.h>
 
 #include <cstdio>
+#include <utility>
 
 namespace pk {
 namespace {
@@ -38,8 +39,21 @@ inline pk_status op_fail(pk_status s, const char * fn, const char * what) {
     return set_error(s, msg);
 }
 
+// The runtime keeps an error until somebody asks for the last one: it is this call's, and no later launch's.
 inline pk_status op_cuda_fail(cudaError_t e, const char * fn) {
+    cudaGetLastError();
     return op_fail(e == cudaErrorMemoryAllocation ? PK_ERR_OOM : PK_ERR_CUDA, fn, cudaGetErrorString(e));
+}
+
+// A launch whose status is its own, not an earlier call's that nobody has asked for.
+template <class... P, class... A>
+inline cudaError_t launch_on(void (*kernel)(P...), dim3 grid, unsigned threads, size_t smem, cudaStream_t s, A &&... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    return cudaLaunchKernelEx(&cfg, kernel, std::forward<A>(args)...);
 }
 
 // Whether `device` exists and is sm_100 (asked of the runtime once per device).
@@ -54,7 +68,10 @@ inline bool device_ok(int device) {
             cudaGetLastError();
             return false;
         }
-        if (cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, device) != cudaSuccess) return false;
+        if (cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, device) != cudaSuccess) {
+            cudaGetLastError();
+            return false;
+        }
         k = major == 10 ? 1 : 2;
         __atomic_store_n(&known[device], k, __ATOMIC_RELAXED);
     }

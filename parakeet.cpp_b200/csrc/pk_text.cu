@@ -42,7 +42,9 @@ struct Buf {
     template <class T> T * as() const { return static_cast<T *>(p); }
 };
 
+// The runtime keeps an error until somebody asks for the last one: it is this call's, and no later launch's.
 pk_status cuda_fail(cudaError_t e, const char * where) {
+    cudaGetLastError();
     char msg[256];
     std::snprintf(msg, sizeof(msg), "%s: %s", where, cudaGetErrorString(e));
     return set_error(e == cudaErrorMemoryAllocation ? PK_ERR_OOM : PK_ERR_CUDA, msg);

@@ -538,3 +538,25 @@ print("same")
 """
     r = subprocess.run([sys.executable, "-c", code, built.PKG_DIR], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and "same" in r.stdout, r.stderr[-2000:]
+
+
+@pytest.mark.gpu
+def test_an_error_stays_with_its_call(built):
+    """A layer too large for the device is refused for memory; neither the next call nor torch finds that error again."""
+    import torch
+    pk, L, abi = built, built.lib(), built.abi
+    x = torch.randn(4, 64, device="cuda")
+    codes, scales = torch.zeros(4, 32, dtype=torch.uint8, device="cuda"), torch.zeros(4, 2, dtype=torch.uint8, device="cuda")
+    small = pk.Mx4Linear(np.ones((8, 64), np.float32))
+    y = torch.zeros(4, 8, device="cuda")
+    n = 1 << 20                                            # 512 GiB of codes: never laid out, the weight never read
+    for after in range(3):
+        t = abi.pk_tensor(codes.data_ptr(), abi.PK_GGML_F32, 0, n, n, n * n * 4)
+        h = C.c_void_p()
+        assert L.pk_mx4_create(0, C.byref(t), 1, None, C.byref(h)) == abi.PK_ERR_OOM and not h.value
+        if after == 0:
+            pk.mx4_quantize(x.data_ptr(), 4, 64, codes.data_ptr(), scales.data_ptr())
+        elif after == 1:
+            small.forward(x.data_ptr(), 4, y.data_ptr())
+        torch.cuda.synchronize()
+        assert torch.ones(3, device="cuda").sum().item() == 3
