@@ -56,6 +56,18 @@ pk_status cuda_fail(cudaError_t e, const char * where) {
         if (e_ != cudaSuccess) return cuda_fail(e_, where); \
     } while (0)
 
+// The same in a body that two entry points share: its name and the step.
+pk_status cuda_fail(cudaError_t e, const char * fn, const char * step) {
+    char where[96];
+    std::snprintf(where, sizeof(where), "%s: %s", fn, step);
+    return cuda_fail(e, where);
+}
+#define TX_STEP(call, fn, step)                               \
+    do {                                                      \
+        const cudaError_t e_ = (call);                        \
+        if (e_ != cudaSuccess) return cuda_fail(e_, fn, step); \
+    } while (0)
+
 // Block-wide exclusive scan of one int per thread (kTxtThreads threads).
 __device__ __forceinline__ int block_scan(int v, int * s_warp, int & total) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -353,8 +365,8 @@ pk_status ctc_frame_tokens(pk_ctc * c, const char * fn, pk_mx4 * head, const flo
     const int64_t step = head ? std::min({frames, kHeadFrames, std::max<int64_t>(kHeadLogits / c->V, 1)}) : frames;
     if (head) {
         const int64_t ws = pk_mx4_workspace(head, step);
-        TX_CK(c->logits.ensure((size_t) step * c->V * 4), fn);
-        TX_CK(c->work.ensure((size_t) std::max<int64_t>(ws, 1)), fn);
+        TX_STEP(c->logits.ensure((size_t) step * c->V * 4), fn, "alloc");
+        TX_STEP(c->work.ensure((size_t) std::max<int64_t>(ws, 1)), fn, "alloc");
     }
     for (int64_t f = 0; f < frames; f += step) {
         const int64_t n = std::min(step, frames - f);
@@ -384,7 +396,7 @@ pk_status ctc_frame_tokens(pk_ctc * c, const char * fn, pk_mx4 * head, const flo
         } else {
             const int blocks = (int) std::min<long long>((n + 7) / 8, 148LL * 8);
             ctc_argmax_kernel<<<blocks, kTxtThreads, 0, s>>>(logits, n, c->V, best);
-            TX_CK(cudaGetLastError(), fn);
+            TX_STEP(cudaGetLastError(), fn, "argmax launch");
         }
     }
     return PK_OK;
@@ -427,7 +439,7 @@ pk_status ctc_decode(pk_ctc * c, const char * fn, pk_mx4 * head, const float * l
     if (frames > 0 && draw && !draw->uniforms) return invalid("null random numbers");
     if (draw && draw->uniforms_on_device && (reinterpret_cast<uintptr_t>(draw->uniforms) & 3u))
         return invalid("device random numbers must be 4-byte aligned");
-    TX_CK(cudaSetDevice(c->device), fn);
+    TX_STEP(cudaSetDevice(c->device), fn, "cudaSetDevice");
     cudaStream_t s = c->stream;
     const size_t fb = (size_t) std::max<int64_t>(frames, 1);
     const float * dlog = logits;
@@ -435,33 +447,33 @@ pk_status ctc_decode(pk_ctc * c, const char * fn, pk_mx4 * head, const float * l
     if (head) mx4_dims(head, nullptr, nullptr, &width);
     if (!logits_on_device && frames > 0) {
         Buf & in = head ? c->frames : c->logits;
-        TX_CK(in.ensure(fb * width * 4), fn);
-        TX_CK(cudaMemcpyAsync(in.p, logits, (size_t) frames * width * 4, cudaMemcpyHostToDevice, s), fn);
+        TX_STEP(in.ensure(fb * width * 4), fn, "alloc");
+        TX_STEP(cudaMemcpyAsync(in.p, logits, (size_t) frames * width * 4, cudaMemcpyHostToDevice, s), fn, head ? "frames copy" : "logits copy");
         dlog = in.as<float>();
     }
     const float * duni = draw ? draw->uniforms : nullptr;
     if (draw && !draw->uniforms_on_device && frames > 0) {
-        TX_CK(c->uniforms.ensure(fb * 4), fn);
-        TX_CK(cudaMemcpyAsync(c->uniforms.p, draw->uniforms, (size_t) frames * 4, cudaMemcpyHostToDevice, s), fn);
+        TX_STEP(c->uniforms.ensure(fb * 4), fn, "alloc");
+        TX_STEP(cudaMemcpyAsync(c->uniforms.p, draw->uniforms, (size_t) frames * 4, cudaMemcpyHostToDevice, s), fn, "random numbers copy");
         duni = c->uniforms.as<float>();
     }
     const size_t rb = (size_t) std::max<int64_t>(rtotal, 1);
-    TX_CK(c->best.ensure(fb * 4), fn);
-    TX_CK(c->rtok.ensure(rb * 4), fn);
-    TX_CK(c->rframe.ensure(rb * 4), fn);
-    TX_CK(c->otok.ensure(rb * 4), fn);
-    TX_CK(c->oframe.ensure(rb * 4), fn);
-    TX_CK(c->roff.ensure((size_t) B * 8), fn);
-    TX_CK(c->foff.ensure((size_t) B * 8), fn);
-    TX_CK(c->nfr.ensure((size_t) B * 4), fn);
-    TX_CK(c->prev_in.ensure((size_t) B * 4), fn);
-    TX_CK(c->prev_out.ensure((size_t) B * 4), fn);
-    TX_CK(c->counts.ensure((size_t) B * 4), fn);
-    TX_CK(c->offs.ensure((size_t) (B + 1) * 8), fn);
-    TX_CK(cudaMemcpyAsync(c->foff.p, frame_offsets, (size_t) B * 8, cudaMemcpyHostToDevice, s), fn);
-    TX_CK(cudaMemcpyAsync(c->roff.p, roff.data(), (size_t) B * 8, cudaMemcpyHostToDevice, s), fn);
-    TX_CK(cudaMemcpyAsync(c->nfr.p, n_frames, (size_t) B * 4, cudaMemcpyHostToDevice, s), fn);
-    TX_CK(cudaMemcpyAsync(c->prev_in.p, prev_inout, (size_t) B * 4, cudaMemcpyHostToDevice, s), fn);
+    TX_STEP(c->best.ensure(fb * 4), fn, "alloc");
+    TX_STEP(c->rtok.ensure(rb * 4), fn, "alloc");
+    TX_STEP(c->rframe.ensure(rb * 4), fn, "alloc");
+    TX_STEP(c->otok.ensure(rb * 4), fn, "alloc");
+    TX_STEP(c->oframe.ensure(rb * 4), fn, "alloc");
+    TX_STEP(c->roff.ensure((size_t) B * 8), fn, "alloc");
+    TX_STEP(c->foff.ensure((size_t) B * 8), fn, "alloc");
+    TX_STEP(c->nfr.ensure((size_t) B * 4), fn, "alloc");
+    TX_STEP(c->prev_in.ensure((size_t) B * 4), fn, "alloc");
+    TX_STEP(c->prev_out.ensure((size_t) B * 4), fn, "alloc");
+    TX_STEP(c->counts.ensure((size_t) B * 4), fn, "alloc");
+    TX_STEP(c->offs.ensure((size_t) (B + 1) * 8), fn, "alloc");
+    TX_STEP(cudaMemcpyAsync(c->foff.p, frame_offsets, (size_t) B * 8, cudaMemcpyHostToDevice, s), fn, "copy");
+    TX_STEP(cudaMemcpyAsync(c->roff.p, roff.data(), (size_t) B * 8, cudaMemcpyHostToDevice, s), fn, "copy");
+    TX_STEP(cudaMemcpyAsync(c->nfr.p, n_frames, (size_t) B * 4, cudaMemcpyHostToDevice, s), fn, "copy");
+    TX_STEP(cudaMemcpyAsync(c->prev_in.p, prev_inout, (size_t) B * 4, cudaMemcpyHostToDevice, s), fn, "copy");
     if (frames > 0) {
         const pk_status st = ctc_frame_tokens(c, fn, head, dlog, frames, draw, duni);
         if (st != PK_OK) return st;
@@ -469,12 +481,11 @@ pk_status ctc_decode(pk_ctc * c, const char * fn, pk_mx4 * head, const float * l
     ctc_collapse_kernel<<<B, kTxtThreads, 0, s>>>(c->best.as<int>(), c->foff.as<int64_t>(), c->nfr.as<int>(),
                                                   c->roff.as<int64_t>(), c->prev_in.as<int>(), c->blank, c->rtok.as<int>(),
                                                   c->rframe.as<int>(), c->counts.as<int>(), c->prev_out.as<int>());
-    TX_CK(cudaGetLastError(), fn);
+    TX_STEP(cudaGetLastError(), fn, "collapse launch");
     scan_offsets_kernel<<<1, kTxtThreads, 0, s>>>(c->counts.as<int>(), B, c->offs.as<int64_t>());
-    TX_CK(cudaGetLastError(), fn);
-    TX_CK(cudaMemcpyAsync(token_offsets, c->offs.p, (size_t) (B + 1) * 8, cudaMemcpyDeviceToHost, s),
-          fn);
-    TX_CK(cudaStreamSynchronize(s), fn);
+    TX_STEP(cudaGetLastError(), fn, "scan launch");
+    TX_STEP(cudaMemcpyAsync(token_offsets, c->offs.p, (size_t) (B + 1) * 8, cudaMemcpyDeviceToHost, s), fn, "offsets copy");
+    TX_STEP(cudaStreamSynchronize(s), fn, "sync");
     if (head && mx4_take_timeout(head)) {
         char msg[160];
         std::snprintf(msg, sizeof(msg), "%s: a device-side wait of the head's product ran out", fn);
@@ -493,15 +504,14 @@ pk_status ctc_decode(pk_ctc * c, const char * fn, pk_mx4 * head, const float * l
     if (first_frame)
         gather_regions_kernel<<<B, kTxtThreads, 0, s>>>(c->rframe.as<int>(), c->roff.as<int64_t>(),
                                                         c->offs.as<int64_t>(), c->oframe.as<int>());
-    TX_CK(cudaGetLastError(), fn);
+    TX_STEP(cudaGetLastError(), fn, "gather launch");
     if (total > 0) {
-        TX_CK(cudaMemcpyAsync(tokens, c->otok.p, (size_t) total * 4, cudaMemcpyDeviceToHost, s), fn);
+        TX_STEP(cudaMemcpyAsync(tokens, c->otok.p, (size_t) total * 4, cudaMemcpyDeviceToHost, s), fn, "copy");
         if (first_frame)
-            TX_CK(cudaMemcpyAsync(first_frame, c->oframe.p, (size_t) total * 4, cudaMemcpyDeviceToHost, s),
-                  fn);
+            TX_STEP(cudaMemcpyAsync(first_frame, c->oframe.p, (size_t) total * 4, cudaMemcpyDeviceToHost, s), fn, "copy");
     }
-    TX_CK(cudaMemcpyAsync(prev_inout, c->prev_out.p, (size_t) B * 4, cudaMemcpyDeviceToHost, s), fn);
-    TX_CK(cudaStreamSynchronize(s), fn);
+    TX_STEP(cudaMemcpyAsync(prev_inout, c->prev_out.p, (size_t) B * 4, cudaMemcpyDeviceToHost, s), fn, "copy");
+    TX_STEP(cudaStreamSynchronize(s), fn, "sync");
     return PK_OK;
 }
 

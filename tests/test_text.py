@@ -229,3 +229,25 @@ def test_detokenize_edges(built, orc):
     assert got == [b"hello worldx y", b"", b"", b"", b"hel"]
     for b, t in enumerate(lists):
         assert got[b] == orc.detokenize(P, t, blank_id=0, bos_id=7)
+
+
+@pytest.mark.gpu
+def test_ctc_errors_name_the_step(built):
+    """Utterances that overlap want more output than the device has: the message says which call ran out of memory
+    at which step, and the handle goes on working."""
+    pk, L, abi = built, built.lib(), built.abi
+    frames, B = 1 << 20, 1 << 20                           # 2^40 output tokens
+    logits = np.zeros(frames, np.float32)
+    ctc = pk.CtcGreedy(1, 0)
+    foff, n = np.zeros(B, np.int64), np.full(B, frames, np.int32)
+    prev, toff = np.full(B, -1, np.int32), np.zeros(B + 1, np.int64)
+    rest = (foff.ctypes.data, n.ctypes.data, B)
+    tail = (prev.ctypes.data, None, 0, toff.ctypes.data, None, None)
+    assert L.pk_ctc_greedy(ctc._h, logits.ctypes.data, 0, *rest, *tail) == abi.PK_ERR_OOM
+    assert L.pk_last_error().startswith(b"pk_ctc_greedy: alloc: ")
+    assert L.pk_ctc_decode(ctc._h, None, logits.ctypes.data, 0, *rest, None, *tail) == abi.PK_ERR_OOM
+    assert L.pk_last_error().startswith(b"pk_ctc_decode: alloc: ")
+    assert (prev == -1).all()
+    got, _, _ = ctc.decode(np.zeros((3, 1), np.float32), [0], [3])
+    assert got[0].tolist() == []
+    ctc.close()
