@@ -404,7 +404,7 @@ pk_status ctc_frame_tokens(pk_ctc * c, const char * fn, pk_mx4 * head, const flo
 
 // pk_ctc_greedy and pk_ctc_decode: frames -> tokens -> collapse -> host arrays. `logits` are logits,
 // or, with a head, its input frames.
-pk_status ctc_decode(pk_ctc * c, const char * fn, pk_mx4 * head, const float * logits, int32_t logits_on_device,
+pk_status ctc_run(pk_ctc * c, const char * fn, pk_mx4 * head, const float * logits, int32_t logits_on_device,
                      const int64_t * frame_offsets, const int32_t * n_frames, int32_t B, const pk_ctc_draw * draw,
                      int32_t * prev_inout, int32_t * tokens, int64_t tokens_cap, int64_t * token_offsets, int32_t * first_frame,
                      int64_t * tokens_needed) {
@@ -513,6 +513,13 @@ pk_status ctc_decode(pk_ctc * c, const char * fn, pk_mx4 * head, const float * l
     TX_STEP(cudaMemcpyAsync(prev_inout, c->prev_out.p, (size_t) B * 4, cudaMemcpyDeviceToHost, s), fn, "copy");
     TX_STEP(cudaStreamSynchronize(s), fn, "sync");
     return PK_OK;
+}
+
+// The same; nothing of a call that failed reads the caller's buffers any more when it returns.
+template <class... A> pk_status ctc_decode(pk_ctc * c, A... args) {
+    const pk_status st = ctc_run(c, args...);
+    if (c && st != PK_OK) cudaStreamSynchronize(c->stream);
+    return st;
 }
 
 }  // namespace

@@ -251,3 +251,27 @@ def test_ctc_errors_name_the_step(built):
     got, _, _ = ctc.decode(np.zeros((3, 1), np.float32), [0], [3])
     assert got[0].tolist() == []
     ctc.close()
+
+
+@pytest.mark.gpu
+def test_ctc_errors_leave_nothing_running(built):
+    """A call that fails has nothing queued that still reads the caller's buffers when it returns."""
+    import time
+
+    import torch
+    pk, L, abi = built, built.lib(), built.abi
+    frames, B = 1 << 28, 1 << 14                           # 2^42 output tokens
+    logits = torch.zeros(frames, pin_memory=True)          # 1 GiB, some 20 ms of copying
+    ctc = pk.CtcGreedy(1, 0)
+    foff, n = np.zeros(B, np.int64), np.full(B, frames, np.int32)
+    prev, toff = np.full(B, -1, np.int32), np.zeros(B + 1, np.int64)
+    torch.cuda.synchronize()
+    for _ in range(2):                                     # the second time the buffers before the failing one are there
+        rc = L.pk_ctc_greedy(ctc._h, logits.data_ptr(), 0, foff.ctypes.data, n.ctypes.data, B, prev.ctypes.data, None, 0,
+                             toff.ctypes.data, None, None)
+        t0 = time.perf_counter()
+        torch.cuda.synchronize()
+        waited = time.perf_counter() - t0
+        assert rc == abi.PK_ERR_OOM
+        assert waited < 0.003, waited
+    ctc.close()
