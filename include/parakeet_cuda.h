@@ -418,7 +418,9 @@ PK_API pk_status pk_ctc_create(int device, int32_t vocab_size, int32_t blank_id,
 PK_API void      pk_ctc_destroy(pk_ctc * c);
 
 /* logits: [sum n_frames][vocab_size] f32, utterance b at rows frame_offsets[b] ..
- * frame_offsets[b] + n_frames[b] - 1. Each frame's argmax is the first index of
+ * frame_offsets[b] + n_frames[b] - 1 (they may lie anywhere, in any order, and
+ * overlap; rows that none covers are not read, unless few lie between two
+ * utterances). Each frame's argmax is the first index of
  * its maximum (`>` scan from index 0, so a NaN at index 0 wins and other NaNs
  * never do); a frame emits its argmax when it is not blank and differs from the
  * previous frame's argmax. prev_inout[b] (host) is the argmax of the frame

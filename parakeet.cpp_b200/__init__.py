@@ -371,6 +371,11 @@ class CtcGreedy:
             raise ValueError(f"{len(foff)} frame offsets and {len(prev)} previous tokens for {B} utterances")
         return n_frames, foff, prev
 
+    @staticmethod
+    def _rows(foff, n_frames):
+        """Rows up to the last one that an utterance covers."""
+        return int((foff + n_frames)[n_frames > 0].max(initial=0))
+
     def decode(self, logits, frame_offsets, n_frames, prev=None, on_device=False, with_frames=False):
         """logits: [frames][vocab] float32 (numpy, or a device pointer int with on_device).
         Returns (token lists, frame lists or None, new prev array)."""
@@ -385,7 +390,7 @@ class CtcGreedy:
             lp = C.c_void_p(int(logits))
         else:
             logits = np.ascontiguousarray(logits, dtype=np.float32)
-            total = int((foff + n_frames).max()) if B else 0
+            total = self._rows(foff, n_frames)
             if logits.size < total * self.vocab_size:
                 raise ValueError(f"logits hold {logits.size} values, the utterances read {total} x {self.vocab_size}")
             lp = _p(logits)
@@ -406,7 +411,7 @@ class CtcGreedy:
         n_frames, foff, prev = self._windows(frame_offsets, n_frames, prev)
         B = len(n_frames)
         cap = int(n_frames.sum())
-        total = int((foff + n_frames).max()) if B else 0
+        total = self._rows(foff, n_frames)
         toks = np.zeros(max(cap, 1), np.int32)
         frs = np.zeros(max(cap, 1), np.int32) if with_frames else None
         toff = np.zeros(B + 1, np.int64)

@@ -14,6 +14,7 @@
 #include <cstdint>
 #include <cstdio>
 #include <cstring>
+#include <new>
 #include <vector>
 
 namespace pk {
@@ -354,24 +355,49 @@ namespace {
 
 // Frames per product of pk_ctc_decode, and values of its logits (1 GiB of them).
 constexpr int64_t kHeadFrames = 16384, kHeadLogits = 1ll << 28;
+constexpr int64_t kMaxValues = 1ll << 46;   // before a frame: more than there are addresses for, far from overflow
 
-// Logits of every frame (`x` itself, or head * x) to its token in c->best: the argmax or a draw.
-pk_status ctc_frame_tokens(pk_ctc * c, const char * fn, pk_mx4 * head, const float * dx, int64_t frames, const pk_ctc_draw * draw,
-                           const float * duni) {
+// Rows [begin, end) of the caller's frames that the utterances cover; in the handle's own arrays the stretches
+// follow each other, this one from row `at` on.
+struct Stretch {
+    int64_t begin, end, at;
+};
+
+// Utterances as stretches, and their rows in the handle's arrays. What lies between two utterances is left out
+// where that is dearer to take along than to part: a product, a draw and their launches for every stretch cost
+// some 15 us, as much as 4096 frames more of a 4-bit head or, copied from the host, 1 MiB.
+constexpr int64_t kGapFrames = 4096, kGapBytes = 1 << 20;
+
+std::vector<Stretch> stretches(const int64_t * offset, const int32_t * n, int32_t B, int64_t gap, std::vector<int64_t> & row) {
+    std::vector<int32_t> order;
+    for (int32_t b = 0; b < B; ++b)
+        if (n[b] > 0) order.push_back(b);
+    std::stable_sort(order.begin(), order.end(), [&](int32_t a, int32_t b) { return offset[a] < offset[b]; });
+    std::vector<Stretch> out;
+    for (const int32_t b : order) {
+        if (out.empty() || offset[b] > out.back().end + gap) {
+            const int64_t at = out.empty() ? 0 : out.back().at + out.back().end - out.back().begin;
+            out.push_back(Stretch{offset[b], offset[b], at});
+        }
+        Stretch & s = out.back();
+        s.end = std::max(s.end, offset[b] + n[b]);
+        row[(size_t) b] = s.at + offset[b] - s.begin;
+    }
+    return out;
+}
+
+// Logits of `frames` frames (`dx` itself, or head * dx, `step` frames a product) to their tokens in c->best from
+// row `at` on: the argmax or a draw.
+pk_status ctc_frame_tokens(pk_ctc * c, const char * fn, pk_mx4 * head, const float * dx, int64_t frames, int64_t step, int64_t at,
+                           const pk_ctc_draw * draw, const float * duni) {
     using namespace pk;
     cudaStream_t s = c->stream;
     int K = c->V;
     if (head) mx4_dims(head, nullptr, nullptr, &K);
-    const int64_t step = head ? std::min({frames, kHeadFrames, std::max<int64_t>(kHeadLogits / c->V, 1)}) : frames;
-    if (head) {
-        const int64_t ws = pk_mx4_workspace(head, step);
-        TX_STEP(c->logits.ensure((size_t) step * c->V * 4), fn, "alloc");
-        TX_STEP(c->work.ensure((size_t) std::max<int64_t>(ws, 1)), fn, "alloc");
-    }
     for (int64_t f = 0; f < frames; f += step) {
         const int64_t n = std::min(step, frames - f);
         const float * logits = dx + f * (int64_t) K;
-        int * best = c->best.as<int>() + f;
+        int * best = c->best.as<int>() + at + f;
         if (head) {
             const pk_status st = pk_mx4_linear(head, logits, PK_GGML_F32, n, K, c->logits.p, PK_GGML_F32, c->V, c->work.p,
                                                (int64_t) c->work.cap, s);
@@ -422,17 +448,19 @@ pk_status ctc_run(pk_ctc * c, const char * fn, pk_mx4 * head, const float * logi
         if (tokens_needed) *tokens_needed = 0;
         return PK_OK;
     }
-    // utterance frame ranges: inside [0, frames) of the logits array, non-negative
-    int64_t frames = 0;
-    std::vector<int64_t> roff((size_t) B);   // each utterance's output region (its frame count)
+    int width = c->V;
+    if (head) mx4_dims(head, nullptr, nullptr, &width);
+    std::vector<int64_t> roff((size_t) B), row((size_t) B);   // each utterance's output region (its frame count), first frame
     int64_t rtotal = 0;
     for (int b = 0; b < B; ++b) {
-        if (n_frames[b] < 0 || frame_offsets[b] < 0)
-            return invalid("negative frame offset or count");
-        frames = std::max<int64_t>(frames, frame_offsets[b] + n_frames[b]);
+        if (n_frames[b] < 0 || frame_offsets[b] < 0 || frame_offsets[b] > kMaxValues / width)
+            return invalid("frame offset or count negative or out of range");
         roff[b] = rtotal;
         rtotal += n_frames[b];
     }
+    const std::vector<Stretch> parts = stretches(frame_offsets, n_frames, B,
+        logits_on_device ? kGapFrames : std::min(kGapFrames, kGapBytes / (4 * (int64_t) width)), row);
+    const int64_t frames = parts.empty() ? 0 : parts.back().at + parts.back().end - parts.back().begin;
     if (logits_on_device && (reinterpret_cast<uintptr_t>(logits) & 3u))
         return invalid("device logits must be 4-byte aligned");
     if (frames > 0 && !logits) return invalid("null logits");
@@ -442,20 +470,18 @@ pk_status ctc_run(pk_ctc * c, const char * fn, pk_mx4 * head, const float * logi
     TX_STEP(cudaSetDevice(c->device), fn, "cudaSetDevice");
     cudaStream_t s = c->stream;
     const size_t fb = (size_t) std::max<int64_t>(frames, 1);
-    const float * dlog = logits;
-    int width = c->V;
-    if (head) mx4_dims(head, nullptr, nullptr, &width);
+    Buf & in = head ? c->frames : c->logits;
     if (!logits_on_device && frames > 0) {
-        Buf & in = head ? c->frames : c->logits;
         TX_STEP(in.ensure(fb * width * 4), fn, "alloc");
-        TX_STEP(cudaMemcpyAsync(in.p, logits, (size_t) frames * width * 4, cudaMemcpyHostToDevice, s), fn, head ? "frames copy" : "logits copy");
-        dlog = in.as<float>();
+        for (const Stretch & p : parts)
+            TX_STEP(cudaMemcpyAsync(in.as<float>() + p.at * width, logits + p.begin * width, (size_t) (p.end - p.begin) * width * 4,
+                                    cudaMemcpyHostToDevice, s), fn, head ? "frames copy" : "logits copy");
     }
-    const float * duni = draw ? draw->uniforms : nullptr;
     if (draw && !draw->uniforms_on_device && frames > 0) {
         TX_STEP(c->uniforms.ensure(fb * 4), fn, "alloc");
-        TX_STEP(cudaMemcpyAsync(c->uniforms.p, draw->uniforms, (size_t) frames * 4, cudaMemcpyHostToDevice, s), fn, "random numbers copy");
-        duni = c->uniforms.as<float>();
+        for (const Stretch & p : parts)
+            TX_STEP(cudaMemcpyAsync(c->uniforms.as<float>() + p.at, draw->uniforms + p.begin, (size_t) (p.end - p.begin) * 4,
+                                    cudaMemcpyHostToDevice, s), fn, "random numbers copy");
     }
     const size_t rb = (size_t) std::max<int64_t>(rtotal, 1);
     TX_STEP(c->best.ensure(fb * 4), fn, "alloc");
@@ -470,12 +496,22 @@ pk_status ctc_run(pk_ctc * c, const char * fn, pk_mx4 * head, const float * logi
     TX_STEP(c->prev_out.ensure((size_t) B * 4), fn, "alloc");
     TX_STEP(c->counts.ensure((size_t) B * 4), fn, "alloc");
     TX_STEP(c->offs.ensure((size_t) (B + 1) * 8), fn, "alloc");
-    TX_STEP(cudaMemcpyAsync(c->foff.p, frame_offsets, (size_t) B * 8, cudaMemcpyHostToDevice, s), fn, "copy");
+    TX_STEP(cudaMemcpyAsync(c->foff.p, row.data(), (size_t) B * 8, cudaMemcpyHostToDevice, s), fn, "copy");
     TX_STEP(cudaMemcpyAsync(c->roff.p, roff.data(), (size_t) B * 8, cudaMemcpyHostToDevice, s), fn, "copy");
     TX_STEP(cudaMemcpyAsync(c->nfr.p, n_frames, (size_t) B * 4, cudaMemcpyHostToDevice, s), fn, "copy");
     TX_STEP(cudaMemcpyAsync(c->prev_in.p, prev_inout, (size_t) B * 4, cudaMemcpyHostToDevice, s), fn, "copy");
-    if (frames > 0) {
-        const pk_status st = ctc_frame_tokens(c, fn, head, dlog, frames, draw, duni);
+    int64_t step = 1;
+    for (const Stretch & p : parts) step = std::max(step, p.end - p.begin);
+    if (head) {
+        step = std::min({step, kHeadFrames, std::max<int64_t>(kHeadLogits / c->V, 1)});
+        const int64_t ws = pk_mx4_workspace(head, step);
+        TX_STEP(c->logits.ensure((size_t) step * c->V * 4), fn, "alloc");
+        TX_STEP(c->work.ensure((size_t) std::max<int64_t>(ws, 1)), fn, "alloc");
+    }
+    for (const Stretch & p : parts) {
+        const float * dx = logits_on_device ? logits + p.begin * width : in.as<float>() + p.at * width;
+        const float * duni = !draw ? nullptr : draw->uniforms_on_device ? draw->uniforms + p.begin : c->uniforms.as<float>() + p.at;
+        const pk_status st = ctc_frame_tokens(c, fn, head, dx, p.end - p.begin, step, p.at, draw, duni);
         if (st != PK_OK) return st;
     }
     ctc_collapse_kernel<<<B, kTxtThreads, 0, s>>>(c->best.as<int>(), c->foff.as<int64_t>(), c->nfr.as<int>(),
@@ -516,8 +552,15 @@ pk_status ctc_run(pk_ctc * c, const char * fn, pk_mx4 * head, const float * logi
 }
 
 // The same; nothing of a call that failed reads the caller's buffers any more when it returns.
-template <class... A> pk_status ctc_decode(pk_ctc * c, A... args) {
-    const pk_status st = ctc_run(c, args...);
+template <class... A> pk_status ctc_decode(pk_ctc * c, const char * fn, A... args) {
+    pk_status st;
+    try {
+        st = ctc_run(c, fn, args...);
+    } catch (const std::bad_alloc &) {
+        char msg[64];
+        std::snprintf(msg, sizeof(msg), "%s: host memory", fn);
+        st = pk::set_error(PK_ERR_OOM, msg);
+    }
     if (c && st != PK_OK) cudaStreamSynchronize(c->stream);
     return st;
 }

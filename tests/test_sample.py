@@ -606,3 +606,53 @@ def test_arrays_too_short_are_refused(built):
             call(x, [0, 4], [4, 5])
         with pytest.raises(pk.PkError):                    # lengths agree: on to the handle, which is null here
             call(x, [0, 4], [4, 4], prev=[1, 2])
+
+
+@pytest.mark.gpu
+def test_ctc_reads_only_its_utterances(built):
+    """A short window far into a large buffer costs the window: no memory for the frames before it. Utterances far
+    apart, out of order, overlapping and empty ones between them are what they are side by side."""
+    import torch
+    pk = built
+    rng = np.random.default_rng(6)
+    v, k, far = 33, 32, 1 << 25
+    head = pk.Mx4Linear(rng.standard_normal((v, k)).astype(np.float32))
+    x = torch.empty(far + 64, k, device="cuda")            # 4 GiB, of which three pieces are used
+    parts = {0: 700, 5000: 3, 5003: 40, 12000: 9, far: 64}
+    for a, n in parts.items():
+        x[a:a + n] = torch.from_numpy(rng.standard_normal((n, k)).astype(np.float32)).cuda()
+    u = torch.rand(far + 64, device="cuda")
+    offs = np.array([12000, far, 0, 7, 5003, 5000, 40, far + 10], np.int64)
+    n = np.array([9, 64, 700, 0, 40, 43, 500, 50], np.int32)
+    prev = np.array([1, 2, 3, 4, 5, 6, 7, 8], np.int32)
+    for kw in (dict(), dict(uniforms=u.data_ptr(), uniforms_on_device=True, temperature=0.8, top_p=0.95)):
+        ctc = pk.CtcGreedy(v, 0)
+        torch.cuda.synchronize()
+        ctc.decode_frames(x.data_ptr(), [3], [5], head=head, on_device=True, **kw)
+        free = torch.cuda.mem_get_info()[0]
+        ctc.decode_frames(x.data_ptr(), [far], [64], head=head, on_device=True, **kw)
+        assert free - torch.cuda.mem_get_info()[0] <= 16 << 20   # 128 MiB for the frames before it
+        got, frames, after = ctc.decode_frames(x.data_ptr(), offs, n, head=head, on_device=True, prev=prev, with_frames=True, **kw)
+        for i in range(len(n)):
+            one = dict(kw, uniforms=u[offs[i]:].data_ptr()) if kw else {}
+            t, f, p = ctc.decode_frames(x[offs[i]:].data_ptr(), [0], [n[i]], head=head, on_device=True, prev=prev[i:i + 1],
+                                        with_frames=True, **one)
+            assert np.array_equal(got[i], t[0]) and np.array_equal(frames[i], f[0]) and after[i] == p[0], i
+        ctc.close()
+    # the same utterances from host memory, logits and uniforms of a gap worth leaving out
+    total = 40_000
+    lg = rng.standard_normal((total, v)).astype(np.float32)
+    uu = rng.random(total).astype(np.float32)
+    ctc = pk.CtcGreedy(v, 0)
+    o, m = np.array([39_000, 0, 20_000], np.int64), np.array([1000, 300, 77], np.int32)
+    for kw in (dict(), dict(uniforms=uu, top_k=9)):
+        got, _, _ = ctc.decode_frames(lg, o, m, **kw)
+        for i in range(3):
+            one = dict(kw, uniforms=uu[o[i]:o[i] + m[i]]) if kw else {}
+            t, _, _ = ctc.decode_frames(lg[o[i]:o[i] + m[i]], [0], [m[i]], **one)
+            assert np.array_equal(got[i], t[0])
+    greedy, _, _ = ctc.decode(lg, o, m)
+    assert all(np.array_equal(a, b) for a, b in zip(greedy, ctc.decode_frames(lg, o, m)[0]))
+    with pytest.raises(pk.PkError, match="out of range"):
+        ctc.decode_frames(x.data_ptr(), [1 << 62], [4], on_device=True)
+    ctc.close()
