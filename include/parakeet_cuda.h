@@ -499,6 +499,10 @@ typedef struct pk_mx4 pk_mx4;
  * and bias are device pointers (earlier work on the device is waited for), else host
  * pointers. Blocks until the layer is laid out; the caller keeps its buffers. */
 PK_API pk_status pk_mx4_create(int device, const pk_tensor * weight, int32_t on_device, const float * bias, pk_mx4 ** out);
+/* Options of a layer: PK_OPT_TIMEOUT_US, the bound on each device-side wait of its products (microseconds;
+ * 2 s unless set), and PK_OPT_TEST_STALL, a test hook: the first block of the next product loads nothing, so
+ * that waits of its own run out. */
+PK_API pk_status pk_mx4_set_option(pk_mx4 * w, int32_t option, int64_t value);
 /* Waits for the device's queued work, so no call on the layer is still running. */
 PK_API void      pk_mx4_destroy(pk_mx4 * w);
 /* Bytes of device workspace that pk_mx4_linear needs for `rows` rows (never less for

@@ -70,7 +70,7 @@ def lib():
             "pk_mx4_quantize": ([I32, P, I32, I64, I64, I64, P, P, P], I32),
             "pk_mx4_dequantize": ([I32, P, P, I64, I64, P, I32, I64, P], I32),
             "pk_mx4_create": ([I32, P, I32, P, P], I32), "pk_mx4_destroy": ([P], None),
-            "pk_mx4_workspace": ([P, I64], I64),
+            "pk_mx4_workspace": ([P, I64], I64), "pk_mx4_set_option": ([P, I32, I64], I32),
             "pk_mx4_linear": ([P, P, I32, I64, I64, P, I32, I64, P, I64, P], I32),
             "pk_sample": ([I32, P, P], I32),
             "pk_ctc_decode": ([P, P, P, I32, P, P, I32, P, P, P, I64, P, P, P], I32),
@@ -545,6 +545,10 @@ class Mx4Linear:
             self.close()
         except Exception:
             pass
+
+    def set_option(self, option: int, value: int) -> None:
+        """pk_mx4_set_option: PK_OPT_TIMEOUT_US or PK_OPT_TEST_STALL of this layer."""
+        _check(lib().pk_mx4_set_option(self.h, option, value), "pk_mx4_set_option")
 
     def workspace(self, rows: int) -> int:
         """Bytes of device workspace that forward() needs for `rows` rows."""

@@ -465,7 +465,16 @@ __global__ void __launch_bounds__(kQThreads) mx4_repack_kernel(const unsigned ch
 // tensor memory and issues its four products, warps from 4 on empty the accumulator, of which there are
 // two, so that a tile's epilogue runs under the next tile's products. Each stage has tensor-memory
 // columns of its own for its scales: they are free when the stage is.
-constexpr long long kWaitNs = 2000000000LL;             // bound on every device-side wait
+constexpr long long kWaitNs = 2000000000LL;             // bound on every device-side wait, unless a layer sets another
+
+// Of a product's waits: their bound, where to tell that one ran out, and (a test's) that the first block, or a
+// pair's second, loads nothing, so that its waits run out.
+struct Waits {
+    long long ns;
+    int * err;
+    int stall;
+};
+
 constexpr int kTM = 128;
 template <bool BOX> constexpr int tc_stages() { return BOX ? 5 : 4; }
 // Warps of the epilogue, for each 32 rows two where TMA stores y and four where the warps do (16391 x 1025:
@@ -483,8 +492,8 @@ struct TcSmem {
 
 // The wait of a whole warp, of one mind about its outcome.
 template <bool CLUSTER = false>
-__device__ __forceinline__ bool warp_wait(unsigned long long * b, unsigned parity, int * err) {
-    return __all_sync(0xFFFFFFFFu, mbar_wait<CLUSTER>(b, parity, kWaitNs, err));
+__device__ __forceinline__ bool warp_wait(unsigned long long * b, unsigned parity, long long ns, int * err) {
+    return __all_sync(0xFFFFFFFFu, mbar_wait<CLUSTER>(b, parity, ns, err));
 }
 
 // The four products of a stage of 256 values and the copies of their scales (columns ca: 8 for x, then
@@ -609,7 +618,7 @@ template <class T, int BN, bool BOX>
 __global__ void __launch_bounds__(tc_threads<BOX>(), 1)
 mx4_tc_kernel(const __grid_constant__ CUtensorMap amap, const unsigned char * __restrict__ ascale, long long M, int K,
               const __grid_constant__ CUtensorMap wmap, const unsigned char * __restrict__ wscale, int N,
-              const float * __restrict__ bias, T * __restrict__ y, long long ldy, const __grid_constant__ CUtensorMap ymap, int * err_out) {
+              const float * __restrict__ bias, T * __restrict__ y, long long ldy, const __grid_constant__ CUtensorMap ymap, const Waits w) {
     constexpr int STAGES = tc_stages<BOX>(), EPI = epi_warps<BOX>();
     extern __shared__ __align__(1024) unsigned char raw[];
     unsigned char * ring = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t) 1023);
@@ -647,13 +656,13 @@ mx4_tc_kernel(const __grid_constant__ CUtensorMap amap, const unsigned char * __
             unsigned it = 0;
             bool ok = true;
             asm volatile("griddepcontrol.wait;" ::: "memory");   // the rows' codes and scales are there
-            for (long long t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+            for (long long t = w.stall && blockIdx.x == 0 ? tiles : blockIdx.x; t < tiles && ok; t += gridDim.x) {
                 const int m = (int) (t / nt), n0 = (int) (t % nt) * BN;
                 const unsigned char * as = ascale + (size_t) m * chunks * 512;
                 const unsigned char * bs = wscale + (size_t) (n0 >> 7) * chunks * 512;
                 for (int ks = 0; ks < nks; ++ks, ++it) {
                     const int s = (int) (it % STAGES);
-                    if (!mbar_wait(&S.empty[s], ((it / STAGES) & 1u) ^ 1u, kWaitNs, &S.err)) { ok = false; break; }
+                    if (!mbar_wait(&S.empty[s], ((it / STAGES) & 1u) ^ 1u, w.ns, &S.err)) { ok = false; break; }
                     unsigned char * a = ring + s * tc_stage_bytes<BN>(), * b = a + kTM * 128, * sa = b + BN * 128;
                     mbar_expect(&S.full[s], tc_stage_bytes<BN>());
                     tma_load_2d(a, &amap, ks * 128, m * kTM, &S.full[s]);
@@ -670,10 +679,10 @@ mx4_tc_kernel(const __grid_constant__ CUtensorMap amap, const unsigned char * __
         bool ok = true;
         for (long long t = blockIdx.x; t < tiles && ok; t += gridDim.x, ++tile) {
             const unsigned buf = tile & 1u, shift = (unsigned) ((int) (t % nt) * BN & 127) >> 5;
-            if (!warp_wait(&S.acc_empty[buf], ((tile >> 1) & 1u) ^ 1u, &S.err)) break;
+            if (!warp_wait(&S.acc_empty[buf], ((tile >> 1) & 1u) ^ 1u, w.ns, &S.err)) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             for (int ks = 0; ks < nks; ++ks) {
-                if (!warp_wait(&S.full[s], ph, &S.err)) { ok = false; break; }
+                if (!warp_wait(&S.full[s], ph, w.ns, &S.err)) { ok = false; break; }
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const unsigned a = smem_u32(ring) + s * tc_stage_bytes<BN>(), b = a + kTM * 128u, sa = b + BN * 128u;
                 if (elect_one()) {
@@ -696,7 +705,7 @@ mx4_tc_kernel(const __grid_constant__ CUtensorMap amap, const unsigned char * __
             const long long m0 = (t / nt) * kTM + q * 32;
             const int n0 = (int) (t % nt) * BN;
             const unsigned buf = tile & 1u;
-            if (!warp_wait(&S.acc_full[buf], (tile >> 1) & 1u, &S.err)) break;
+            if (!warp_wait(&S.acc_full[buf], (tile >> 1) & 1u, w.ns, &S.err)) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const int rows = (int) max(0LL, min(32LL, M - m0));
             store_tile<T, BN, BOX, EPI / 4>(tmem + buf * BN + ((unsigned) (q * 32) << 16), st, half, lane, m0, rows, n0, N, bias, y, ldy, &ymap);
@@ -711,7 +720,7 @@ mx4_tc_kernel(const __grid_constant__ CUtensorMap amap, const unsigned char * __
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(512u) : "memory");
     }
-    if (threadIdx.x == 0 && S.err != 0) atomicExch_system(err_out, 1);
+    if (threadIdx.x == 0 && S.err != 0) atomicExch_system(w.err, 1);
 }
 
 // ---- many rows: pairs of blocks ---------------------------------------------------
@@ -745,7 +754,7 @@ template <class T, int BN, bool BOX>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(tc_threads<BOX>(), 1)
 mx4_pair_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap asmap, long long M, int K,
                 const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap wsmap, int N,
-                const float * __restrict__ bias, T * __restrict__ y, long long ldy, const __grid_constant__ CUtensorMap ymap, int * err_out) {
+                const float * __restrict__ bias, T * __restrict__ y, long long ldy, const __grid_constant__ CUtensorMap ymap, const Waits w) {
     constexpr int EPI = epi_warps<BOX>();
     extern __shared__ __align__(1024) unsigned char raw[];
     unsigned char * ring = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t) 1023);
@@ -785,11 +794,11 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant_
             unsigned it = 0;
             bool ok = true;
             asm volatile("griddepcontrol.wait;" ::: "memory");   // the rows' codes and scales are there
-            for (long long t = first; t < tiles && ok; t += step) {
+            for (long long t = w.stall && blockIdx.x == 1 ? tiles : first; t < tiles && ok; t += step) {
                 const int m = (int) (t / nt) * 2 + (int) rank, n0 = (int) (t % nt) * BN;
                 for (int ks = 0; ks < nks; ++ks, ++it) {
                     const int s = (int) (it % kPStages);
-                    if (!mbar_wait(&S.empty[s], ((it / kPStages) & 1u) ^ 1u, kWaitNs, &S.err)) { ok = false; break; }
+                    if (!mbar_wait(&S.empty[s], ((it / kPStages) & 1u) ^ 1u, w.ns, &S.err)) { ok = false; break; }
                     unsigned char * a = ring + s * pair_stage<BN>(), * b = a + kTM * 128, * sa = b + BN / 2 * 128;
                     // rows past M or N, and their scales, read as zeros
                     const unsigned bar = mbar_at(&S.full[s], 0);
@@ -812,10 +821,10 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant_
             bool ok = true;
             for (long long t = first; t < tiles && ok; t += step, ++tile) {
                 const unsigned buf = tile & 1u, shift = (unsigned) ((int) (t % nt) * BN & 127) >> 5;
-                if (!warp_wait<true>(&S.acc_empty[buf], ((tile >> 1) & 1u) ^ 1u, &S.err)) break;
+                if (!warp_wait<true>(&S.acc_empty[buf], ((tile >> 1) & 1u) ^ 1u, w.ns, &S.err)) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 for (int ks = 0; ks < nks; ++ks) {
-                    if (!warp_wait<true>(&S.full[s], ph, &S.err)) { ok = false; break; }
+                    if (!warp_wait<true>(&S.full[s], ph, w.ns, &S.err)) { ok = false; break; }
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     const unsigned a = smem_u32(ring) + s * pair_stage<BN>(), b = a + kTM * 128u, sa = b + BN / 2 * 128u;
                     if (elect_one()) {
@@ -841,7 +850,7 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant_
             const long long m0 = ((t / nt) * 2 + rank) * kTM + q * 32;
             const int n0 = (int) (t % nt) * BN;
             const unsigned buf = tile & 1u;
-            if (!warp_wait(&S.acc_full[buf], (tile >> 1) & 1u, &S.err)) break;
+            if (!warp_wait(&S.acc_full[buf], (tile >> 1) & 1u, w.ns, &S.err)) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const int rows = (int) max(0LL, min(32LL, M - m0));
             store_tile<T, BN, BOX, EPI / 4>(tmem + buf * BN + ((unsigned) (q * 32) << 16), st, half, lane, m0, rows, n0, N, bias, y, ldy, &ymap);
@@ -857,7 +866,7 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant_
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(512u) : "memory");
     }
-    if (threadIdx.x == 0 && S.err != 0) atomicExch_system(err_out, 1);
+    if (threadIdx.x == 0 && S.err != 0) atomicExch_system(w.err, 1);
 }
 
 // ---- few rows: quantisation and product in one kernel -----------------------------
@@ -892,7 +901,7 @@ template <class TX, class TY, bool VEC>
 __global__ void __launch_bounds__(kFewThreads, 1)
 mx4_few_kernel(const TX * __restrict__ x, long long ldx, int M, int K, const __grid_constant__ CUtensorMap wmap,
                const unsigned char * __restrict__ wscale, int N, const float * __restrict__ bias, TY * __restrict__ y, long long ldy,
-               int * err_out) {
+               const Waits w) {
     extern __shared__ __align__(1024) unsigned char raw[];
     const int chunks = scale_chunks(K), nks = chunks / 2, nt = (N + kFewN - 1) / kFewN;
     unsigned char * a = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t) 1023);
@@ -930,12 +939,12 @@ mx4_few_kernel(const TX * __restrict__ x, long long ldx, int M, int K, const __g
         if (lane == 0) {
             unsigned it = 0;
             bool ok = true;
-            for (int t = blockIdx.x; t < nt && ok; t += gridDim.x) {
+            for (int t = w.stall && blockIdx.x == 0 ? nt : blockIdx.x; t < nt && ok; t += gridDim.x) {
                 const int n0 = t * kFewN;
                 const unsigned char * bs = wscale + (size_t) (n0 >> 7) * chunks * 512;
                 for (int ks = 0; ks < nks; ++ks, ++it) {
                     const int s = (int) (it % kFewStages);
-                    if (!mbar_wait(&S.empty[s], ((it / kFewStages) & 1u) ^ 1u, kWaitNs, &S.err)) { ok = false; break; }
+                    if (!mbar_wait(&S.empty[s], ((it / kFewStages) & 1u) ^ 1u, w.ns, &S.err)) { ok = false; break; }
                     unsigned char * b = ring + s * kFewStage;
                     mbar_expect(&S.full[s], kFewStage);
                     tma_load_2d(b, &wmap, ks * 128, n0, &S.full[s]);
@@ -946,13 +955,13 @@ mx4_few_kernel(const TX * __restrict__ x, long long ldx, int M, int K, const __g
         }
     } else if (warp == 1) {
         unsigned tile = 0, s = 0, ph = 0;
-        bool ok = warp_wait(&S.a_full, 0u, &S.err);
+        bool ok = warp_wait(&S.a_full, 0u, w.ns, &S.err);
         for (int t = blockIdx.x; t < nt && ok; t += gridDim.x, ++tile) {
             const unsigned buf = tile & 1u, shift = (unsigned) ((t * kFewN) & 127) >> 5;
-            if (!warp_wait(&S.acc_empty[buf], ((tile >> 1) & 1u) ^ 1u, &S.err)) break;
+            if (!warp_wait(&S.acc_empty[buf], ((tile >> 1) & 1u) ^ 1u, w.ns, &S.err)) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             for (int ks = 0; ks < nks; ++ks) {
-                if (!warp_wait(&S.full[s], ph, &S.err)) { ok = false; break; }
+                if (!warp_wait(&S.full[s], ph, w.ns, &S.err)) { ok = false; break; }
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const unsigned kb = smem_u32(ring) + s * kFewStage;
                 if (elect_one()) {
@@ -999,7 +1008,7 @@ mx4_few_kernel(const TX * __restrict__ x, long long ldx, int M, int K, const __g
         unsigned tile = 0;
         for (int t = blockIdx.x; t < nt; t += gridDim.x, ++tile) {
             const unsigned buf = tile & 1u;
-            if (!warp_wait(&S.acc_full[buf], (tile >> 1) & 1u, &S.err)) break;
+            if (!warp_wait(&S.acc_full[buf], (tile >> 1) & 1u, w.ns, &S.err)) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             store_tile<TY, kFewN, false, 2>(tmem + buf * kFewN, out + half * kOutBytes, half, lane, 0, M, t * kFewN, N, bias, y, ldy, nullptr);
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -1012,7 +1021,7 @@ mx4_few_kernel(const TX * __restrict__ x, long long ldx, int M, int K, const __g
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(256u) : "memory");
     }
-    if (threadIdx.x == 0 && S.err != 0) atomicExch_system(err_out, 1);
+    if (threadIdx.x == 0 && S.err != 0) atomicExch_system(w.err, 1);
 }
 
 // Lanes of a row, as a power of two.
@@ -1086,6 +1095,8 @@ struct pk_mx4 {
     float * bias = nullptr;             // padded to whole tiles, or null
     int * err = nullptr;                // host memory that the device sees: a bounded wait ran out
     int * err_dev = nullptr;
+    long long wait_ns = pk::kWaitNs;
+    int stall = 0;                      // the next product's, see Waits
     alignas(64) CUtensorMap map[3];     // codes in boxes of kBox[i] rows
     alignas(64) CUtensorMap smap[2];    // scales: the two atoms of a stage of 128 rows, of 256 rows
 };
@@ -1122,6 +1133,7 @@ template <class F> cudaError_t allow_smem(F kernel, size_t bytes, int device, un
 
 struct Call {
     const pk_mx4 * w;
+    Waits waits;
     const void * x;
     long long ldx, M;
     void * y;
@@ -1154,7 +1166,7 @@ cudaError_t launch_tc_as(const Call & c, const CUtensorMap & amap, const unsigne
     if (e != cudaSuccess) return e;
     const long long tiles = (c.M + kTM - 1) / kTM * ((c.w->N + BN - 1) / BN);
     return launch_after(kernel, (unsigned) std::min<long long>(tiles, 148), tc_threads<BOX>(), smem, c.s,
-        amap, xs, c.M, c.w->K, wmap, c.w->scales, c.w->N, c.w->bias, static_cast<T *>(c.y), c.ldy, ymap, c.w->err_dev);
+        amap, xs, c.M, c.w->K, wmap, c.w->scales, c.w->N, c.w->bias, static_cast<T *>(c.y), c.ldy, ymap, c.waits);
 }
 
 template <class T, int BN, bool BOX>
@@ -1169,7 +1181,7 @@ cudaError_t launch_pair_as(const Call & c, const CUtensorMap & amap, const unsig
     if (e != cudaSuccess) return e;
     const long long tiles = (c.M + 2 * kTM - 1) / (2 * kTM) * ((c.w->N + BN - 1) / BN);
     return launch_after(kernel, (unsigned) (2 * std::min<long long>(tiles, 74)), tc_threads<BOX>(), smem, c.s,
-        amap, asmap, c.M, c.w->K, c.w->map[BN > 128 ? 2 : 0], c.w->smap[BN > 128 ? 1 : 0], c.w->N, c.w->bias, static_cast<T *>(c.y), c.ldy, ymap, c.w->err_dev);
+        amap, asmap, c.M, c.w->K, c.w->map[BN > 128 ? 2 : 0], c.w->smap[BN > 128 ? 1 : 0], c.w->N, c.w->bias, static_cast<T *>(c.y), c.ldy, ymap, c.waits);
 }
 
 template <class TX, class TY, bool VEC>
@@ -1180,7 +1192,7 @@ cudaError_t launch_few_as(const Call & c) {
     if (e != cudaSuccess) return e;
     const int grid = std::min((c.w->N + kFewN - 1) / kFewN, 148);
     return launch_on(kernel, dim3(grid), kFewThreads, few_smem(c.w->chunks / 2), c.s, static_cast<const TX *>(c.x), c.ldx, (int) c.M, c.w->K,
-                     c.w->map[0], c.w->scales, c.w->N, c.w->bias, static_cast<TY *>(c.y), c.ldy, c.w->err_dev);
+                     c.w->map[0], c.w->scales, c.w->N, c.w->bias, static_cast<TY *>(c.y), c.ldy, c.waits);
 }
 
 template <class TX, class TY> cudaError_t launch_few_xy(const Call & c) {
@@ -1370,6 +1382,22 @@ extern "C" PK_API pk_status pk_mx4_create(int device, const pk_tensor * weight, 
     return PK_OK;
 }
 
+extern "C" PK_API pk_status pk_mx4_set_option(pk_mx4 * w, int32_t option, int64_t value) {
+    const char * fn = "pk_mx4_set_option";
+    if (!w) return op_fail(PK_ERR_INVALID, fn, "null layer");
+    switch (option) {
+        case PK_OPT_TIMEOUT_US:
+            if (value <= 0 || value > INT64_MAX / 1000) return op_fail(PK_ERR_INVALID, fn, "timeout must be > 0");
+            __atomic_store_n(&w->wait_ns, (long long) value * 1000, __ATOMIC_RELAXED);
+            return PK_OK;
+        case PK_OPT_TEST_STALL:
+            __atomic_store_n(&w->stall, value != 0 ? 1 : 0, __ATOMIC_RELAXED);
+            return PK_OK;
+        default:
+            return op_fail(PK_ERR_INVALID, fn, "a layer has PK_OPT_TIMEOUT_US and PK_OPT_TEST_STALL");
+    }
+}
+
 namespace {
 
 size_t ws_codes(const pk_mx4 * w, int64_t rows) { return ((size_t) rows * w->nb * 16 + 255) / 256 * 256; }
@@ -1405,7 +1433,8 @@ extern "C" PK_API pk_status pk_mx4_linear(pk_mx4 * w, const void * x, int32_t x_
     cudaStream_t s = (cudaStream_t) stream;
     unsigned char * xc = static_cast<unsigned char *>(workspace);
     unsigned char * xs = xc + ws_codes(w, rows);
-    const Call c{w, x, x_stride, rows, y, y_stride, s};
+    const Waits waits{__atomic_load_n(&w->wait_ns, __ATOMIC_RELAXED), w->err_dev, __atomic_exchange_n(&w->stall, 0, __ATOMIC_RELAXED)};
+    const Call c{w, waits, x, x_stride, rows, y, y_stride, s};
     cudaError_t e;
     if (few(w, rows)) {
         e = x_type == PK_GGML_F32 ? launch_few<float>(c, y_type)

@@ -560,3 +560,46 @@ def test_an_error_stays_with_its_call(built):
             small.forward(x.data_ptr(), 4, y.data_ptr())
         torch.cuda.synchronize()
         assert torch.ones(3, device="cuda").sum().item() == 3
+
+
+def test_option_refusals(built):
+    assert built.lib().pk_mx4_set_option(None, built.abi.PK_OPT_TIMEOUT_US, 5) == built.abi.PK_ERR_INVALID
+
+
+def stalled(pk, layer, x, y, ws):
+    """Queues a product whose first block's (or pair's second block's) loads never come, its waits bounded to 20 ms."""
+    import torch
+    layer.set_option(pk.abi.PK_OPT_TIMEOUT_US, 20_000)
+    layer.set_option(pk.abi.PK_OPT_TEST_STALL, 1)
+    layer.forward(x.data_ptr(), x.shape[0], y.data_ptr(), workspace=ws.data_ptr(), workspace_bytes=ws.numel(),
+                  stream=torch.cuda.current_stream().cuda_stream)
+    layer.set_option(pk.abi.PK_OPT_TIMEOUT_US, 2_000_000)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("r,n,k", [(5, 333, 640), (200, 64, 640), (200, 333, 640), (3000, 640, 512)], ids=["few", "one tile", "unaligned", "TMA"])
+def test_a_wait_that_runs_out_is_reported(built, r, n, k):
+    """The call after it says so, once; the layer then works as before."""
+    import time
+
+    import torch
+    pk = built
+    rng = np.random.default_rng(r)
+    w = rng.standard_normal((n, k)).astype(np.float32)
+    x = rng.standard_normal((r, k)).astype(np.float32)
+    layer = pk.Mx4Linear(w)
+    for option, value in ((pk.abi.PK_OPT_TIMEOUT_US, 0), (pk.abi.PK_OPT_TIMEOUT_US, -1), (pk.abi.PK_OPT_MATH, 1)):
+        with pytest.raises(pk.PkError):
+            layer.set_option(option, value)
+    dx, y = torch.from_numpy(x).cuda(), torch.zeros(r, n, device="cuda")
+    ws = torch.zeros(max(1, layer.workspace(r)), dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    for _ in range(2):
+        t0 = time.perf_counter()
+        stalled(pk, layer, dx, y, ws)
+        torch.cuda.synchronize()
+        assert 0.015 < time.perf_counter() - t0 < 1.0
+        with pytest.raises(pk.PkError) as e:
+            product(pk, w, x, layer=layer)
+        assert e.value.status == pk.abi.PK_ERR_TIMEOUT
+        check_product(ref_quantize(w)[2], *product(pk, w, x, layer=layer))
