@@ -740,9 +740,17 @@ struct PairSmem {
     unsigned long long full[kPStages], empty[kPStages], acc_full[2], acc_empty[2], done;
     unsigned tmem;
     int err;
+    unsigned loads;              // stages that this block's loader issued
+    unsigned its_loads;          // the other block's, and whether a wait of its ran out
+    int its_err;
 };
 template <int BN, bool BOX> constexpr size_t pair_smem() {
     return 1024 + (size_t) kPStages * pair_stage<BN>() + epi_warps<BOX>() * kOutBytes + sizeof(PairSmem);
+}
+
+__device__ __forceinline__ void put_at(unsigned * p, unsigned rank, unsigned v) {   // to the same place of block `rank`
+    asm volatile("{ .reg .b32 a; mapa.shared::cluster.u32 a, %0, %1; st.shared::cluster.u32 [a], %2; }"
+                 :: "r"(smem_u32(p)), "r"(rank), "r"(v) : "memory");
 }
 
 __device__ __forceinline__ void cluster_meet() {
@@ -776,6 +784,7 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant_
         }
         mbar_init(&S.done, 1);
         S.err = 0;
+        S.loads = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 2) {
@@ -809,11 +818,7 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant_
                     tma_load_2d_pair(sa + kScaleA, &wsmap, ks * 256, n0 >> 7, bar);
                 }
             }
-            // nothing in flight when the blocks end, however the others ended
-            if (rank == 0)
-                for (unsigned j = it > kPStages ? it - kPStages : 0; j < it; ++j) mbar_drain(&S.full[j % kPStages], (j / kPStages) & 1u);
-            else if (!ok)
-                for (int j = 0; j < 200; ++j) __nanosleep(1000);
+            S.loads = it;
         }
     } else if (warp == 1) {
         if (rank == 0) {
@@ -836,11 +841,9 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant_
                     if (++s == kPStages) { s = 0; ph ^= 1u; }
                 }
             }
-            // no product in flight either
+            // no product in flight when the blocks end
             if (elect_one()) umma_commit_pair(&S.done);
             mbar_drain(&S.done, 0u);
-        } else {
-            mbar_drain(&S.done, 0u);                      // the products read this block's memory until then
         }
     } else if (warp >= 4) {
         const int q = warp & 3, half = (warp - 4) >> 2;
@@ -861,7 +864,26 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant_
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
+    if (threadIdx.x == 0) {
+        put_at(&S.its_loads, rank ^ 1u, S.loads);
+        put_at(reinterpret_cast<unsigned *>(&S.its_err), rank ^ 1u, (unsigned) S.err);
+    }
     cluster_meet();                                       // the other's memory and barriers are used no more
+    if (threadIdx.x == 0) mbar_drain(&S.done, 0u);        // the second block's too: its arrival comes from the first's products
+    // Where no wait ran out every stage was multiplied, so its loads have come. Otherwise one block may have issued
+    // stages that the other has not (five at most: a stage is free again once both blocks' was multiplied). The
+    // first block, whose barriers count both blocks' bytes, sets the counts right and waits for what was issued.
+    if (S.err | S.its_err) {
+        if (rank == 0 && threadIdx.x == 0) {
+            const unsigned least = min(S.loads, S.its_loads), most = max(S.loads, S.its_loads);
+            for (unsigned j = least; j < most; ++j) {
+                if (S.loads < most) mbar_expect(&S.full[j % kPStages], pair_bytes<BN>());
+                else mbar_complete(&S.full[j % kPStages], pair_bytes<BN>());
+            }
+            for (unsigned j = most > kPStages ? most - kPStages : 0; j < most; ++j) mbar_drain(&S.full[j % kPStages], (j / kPStages) & 1u);
+        }
+        cluster_meet();
+    }
     if (warp == 2) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(512u) : "memory");

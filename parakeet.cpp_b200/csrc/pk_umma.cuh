@@ -189,6 +189,11 @@ __device__ __forceinline__ void mbar_expect(unsigned long long * b, unsigned byt
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" :: "r"(smem_u32(b)), "r"(bytes) : "memory");
 }
 
+// Counts `bytes` as arrived on the barrier's phase, in place of a copy that was expected and never issued.
+__device__ __forceinline__ void mbar_complete(unsigned long long * b, unsigned bytes) {
+    asm volatile("mbarrier.complete_tx.relaxed.cta.shared::cta.b64 [%0], %1;" :: "r"(smem_u32(b)), "r"(bytes) : "memory");
+}
+
 // 32 columns of this warp's 32 tensor-memory lanes (issue only; tcgen05.wait::ld before use).
 __device__ __forceinline__ void tmem_load32(unsigned taddr, unsigned * v) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 "

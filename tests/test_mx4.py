@@ -603,3 +603,29 @@ def test_a_wait_that_runs_out_is_reported(built, r, n, k):
             product(pk, w, x, layer=layer)
         assert e.value.status == pk.abi.PK_ERR_TIMEOUT
         check_product(ref_quantize(w)[2], *product(pk, w, x, layer=layer))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("r,n,k", [(2600, 1300, 2048), (2561, 1152, 2055)], ids=["192", "128"])
+@pytest.mark.parametrize("y_dtype,ypad", [("f32", 0), ("f32", 1)], ids=["TMA", "unaligned"])
+def test_a_pair_whose_wait_runs_out(built, r, n, k, y_dtype, ypad):
+    """One block of a pair has loads in flight that the other never matches: both end once those have come."""
+    import torch
+    pk = built
+    rng = np.random.default_rng(k)
+    w = rng.standard_normal((n, k)).astype(np.float32)
+    x = rng.standard_normal((r, k)).astype(np.float32)
+    layer = pk.Mx4Linear(w)
+    dx, y = torch.from_numpy(x).cuda(), torch.zeros(r, n + ypad, device="cuda")
+    ws = torch.zeros(layer.workspace(r), dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    for _ in range(2):
+        layer.set_option(pk.abi.PK_OPT_TIMEOUT_US, 20_000)
+        layer.set_option(pk.abi.PK_OPT_TEST_STALL, 1)
+        layer.forward(dx.data_ptr(), r, y.data_ptr(), y_stride=n + ypad, workspace=ws.data_ptr(), workspace_bytes=ws.numel())
+        layer.set_option(pk.abi.PK_OPT_TIMEOUT_US, 2_000_000)
+        torch.cuda.synchronize()
+        with pytest.raises(pk.PkError) as e:
+            layer.forward(dx.data_ptr(), r, y.data_ptr(), y_stride=n + ypad, workspace=ws.data_ptr(), workspace_bytes=ws.numel())
+        assert e.value.status == pk.abi.PK_ERR_TIMEOUT
+        check_product(ref_quantize(w)[2], *product(pk, w, x, None, "f32", y_dtype, 0, ypad, layer=layer))
