@@ -516,10 +516,16 @@ PK_API int64_t   pk_mx4_workspace(const pk_mx4 * w, int64_t rows);
  * alone until it has run: calls that may overlap (two streams, two captured graphs) each
  * need their own. Calls on one layer may overlap otherwise. PK_ERR_TIMEOUT: a bounded
  * device-side wait of an EARLIER call on this layer ran out and that call's y is not
- * to be used (reported once). */
+ * to be used; the reporting call itself has queued nothing. Each is reported to one
+ * call; see pk_mx4_timeouts where that may be another caller's. */
 PK_API pk_status pk_mx4_linear(pk_mx4 * w, const void * x, int32_t x_type, int64_t rows, int64_t x_stride, void * y,
                                int32_t y_type, int64_t y_stride, void * workspace, int64_t workspace_bytes,
                                void * stream);
+/* How often products of pk_mx4_linear on this layer were found to have run into that
+ * bound; it never falls. For callers that replay captured graphs or share a layer: a y
+ * that was computed (and waited for) between two equal answers is good. -1 for a null
+ * layer. pk_ctc_decode's products count and report only there. */
+PK_API int64_t   pk_mx4_timeouts(pk_mx4 * w);
 
 /* ---- drawing tokens from logits -----------------------------------------------
  *
@@ -586,7 +592,8 @@ typedef struct pk_ctc_draw {
  * whose logits the layer `head` (N = vocab_size, on the handle's device) computes, or,
  * with head = NULL, logits [frames][vocab_size]; each frame's token is the argmax
  * (draw = NULL) or drawn (pk_sample). Repeats and blanks then collapse as in
- * pk_ctc_greedy, whose other arguments, results and waiting these are. A frame
+ * pk_ctc_greedy, whose other arguments, results and waiting these are.
+ * PK_ERR_TIMEOUT: a bounded device-side wait of this call's own product ran out. A frame
  * without any logit above -infinity counts as blank when drawn. */
 PK_API pk_status pk_ctc_decode(pk_ctc * c, pk_mx4 * head, const float * frames, int32_t frames_on_device,
                                const int64_t * frame_offsets, const int32_t * n_frames, int32_t B,

@@ -71,6 +71,7 @@ def lib():
             "pk_mx4_dequantize": ([I32, P, P, I64, I64, P, I32, I64, P], I32),
             "pk_mx4_create": ([I32, P, I32, P, P], I32), "pk_mx4_destroy": ([P], None),
             "pk_mx4_workspace": ([P, I64], I64), "pk_mx4_set_option": ([P, I32, I64], I32),
+            "pk_mx4_timeouts": ([P], I64),
             "pk_mx4_linear": ([P, P, I32, I64, I64, P, I32, I64, P, I64, P], I32),
             "pk_sample": ([I32, P, P], I32),
             "pk_ctc_decode": ([P, P, P, I32, P, P, I32, P, P, P, I64, P, P, P], I32),
@@ -549,6 +550,11 @@ class Mx4Linear:
     def set_option(self, option: int, value: int) -> None:
         """pk_mx4_set_option: PK_OPT_TIMEOUT_US or PK_OPT_TEST_STALL of this layer."""
         _check(lib().pk_mx4_set_option(self.h, option, value), "pk_mx4_set_option")
+
+    def timeouts(self) -> int:
+        """How often a forward() was found to have run into its waits' bound: a result that was computed, and
+        waited for, between two equal answers is good (see pk_mx4_timeouts)."""
+        return int(lib().pk_mx4_timeouts(self.h))
 
     def workspace(self, rows: int) -> int:
         """Bytes of device workspace that forward() needs for `rows` rows."""

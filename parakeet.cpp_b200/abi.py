@@ -107,7 +107,7 @@ EXPORTED_SYMBOLS = [
     "pk_ctc_create", "pk_ctc_destroy", "pk_ctc_greedy", "pk_vocab_create", "pk_vocab_destroy",
     "pk_detokenize", "pk_prefetch_batch", "pk_shard_balanced",
     "pk_mx4_quantize", "pk_mx4_dequantize", "pk_mx4_create", "pk_mx4_destroy", "pk_mx4_workspace",
-    "pk_mx4_set_option",
+    "pk_mx4_set_option", "pk_mx4_timeouts",
     "pk_mx4_linear", "pk_sample", "pk_ctc_decode",
 ]
 

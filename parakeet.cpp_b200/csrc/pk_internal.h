@@ -281,8 +281,14 @@ cudaError_t launch_extract_field(const int32_t * ust, int B, int field, int32_t 
 
 // pk_mx4.cu: a layer's device, outputs N and inputs K (any may be null).
 void mx4_dims(const pk_mx4 * w, int * device, int * N, int * K);
-// Whether a device-side wait of a finished call on the layer ran out (asked once).
-bool mx4_take_timeout(pk_mx4 * w);
+// pk_mx4_linear under another entry point's name, whose products report a wait that ran out to that one's own
+// error word (null: to the layer's).
+pk_status mx4_linear(pk_mx4 * w, const char * fn, const void * x, int32_t x_type, int64_t rows, int64_t x_stride, void * y,
+                     int32_t y_type, int64_t y_stride, void * workspace, int64_t workspace_bytes, void * stream, int * err_dev);
+// Error words: host memory that the devices see. A device sets one, the host asks and clears it.
+int * take_error_word(cudaError_t & e);
+void give_error_word(int * w);
+bool take_error(int * w);
 
 // Read-only view of a context for entry points defined outside pk_api.cu.
 struct CtxView {

@@ -1071,10 +1071,15 @@ cudaError_t launch_quantize(const void * x, int type, long long rows, int K, lon
 #undef PK_Q2
 }
 
-// Host-visible error words of the layers, from pages that stay: a layer's creation pays for no
-// pinned allocation of its own.
+// Host-visible error words of the layers and of pk_ctc handles, from pages that stay: creating one pays for
+// no pinned allocation of its own.
 std::mutex error_lock;
 std::vector<int *> free_words;
+
+constexpr int64_t kMaxDim = 1 << 20;        // K, N
+constexpr int64_t kMaxRows = 0x7FFFFFFF;
+
+}  // namespace
 
 void give_error_word(int * w) {
     std::lock_guard<std::mutex> g(error_lock);
@@ -1103,10 +1108,9 @@ int * take_error_word(cudaError_t & e) {
     return w;
 }
 
-constexpr int64_t kMaxDim = 1 << 20;        // K, N
-constexpr int64_t kMaxRows = 0x7FFFFFFF;
+// Whether a wait of a finished product that reports to `w` ran out (asked once).
+bool take_error(int * w) { return __atomic_exchange_n(w, 0, __ATOMIC_ACQ_REL) != 0; }
 
-}  // namespace
 }  // namespace pk
 
 struct pk_mx4 {
@@ -1115,8 +1119,10 @@ struct pk_mx4 {
     unsigned char * codes = nullptr;    // [N][16 nb]; owns the memory of all three
     unsigned char * scales = nullptr;   // atoms
     float * bias = nullptr;             // padded to whole tiles, or null
-    int * err = nullptr;                // host memory that the device sees: a bounded wait ran out
+    int * err = nullptr;                // host memory that the device sees: a wait of a pk_mx4_linear ran out
     int * err_dev = nullptr;
+    long long timeouts = 0;             // times that it was found so
+    int unreported = 0;                 // and no pk_mx4_linear has said so yet
     long long wait_ns = pk::kWaitNs;
     int stall = 0;                      // the next product's, see Waits
     alignas(64) CUtensorMap map[3];     // codes in boxes of kBox[i] rows
@@ -1266,8 +1272,6 @@ void mx4_dims(const pk_mx4 * w, int * device, int * N, int * K) {
     if (N) *N = w->N;
     if (K) *K = w->K;
 }
-
-bool mx4_take_timeout(pk_mx4 * w) { return __atomic_exchange_n(w->err, 0, __ATOMIC_ACQ_REL) != 0; }
 
 }  // namespace pk
 
@@ -1422,6 +1426,12 @@ extern "C" PK_API pk_status pk_mx4_set_option(pk_mx4 * w, int32_t option, int64_
 
 namespace {
 
+void notice_timeout(pk_mx4 * w) {
+    if (!take_error(w->err)) return;
+    __atomic_fetch_add(&w->timeouts, 1, __ATOMIC_ACQ_REL);
+    __atomic_store_n(&w->unreported, 1, __ATOMIC_RELEASE);
+}
+
 size_t ws_codes(const pk_mx4 * w, int64_t rows) { return ((size_t) rows * w->nb * 16 + 255) / 256 * 256; }
 
 }  // namespace
@@ -1432,10 +1442,10 @@ extern "C" PK_API int64_t pk_mx4_workspace(const pk_mx4 * w, int64_t rows) {
     return (int64_t) (ws_codes(w, rows) + (size_t) ((rows + 127) / 128) * w->chunks * 512);
 }
 
-extern "C" PK_API pk_status pk_mx4_linear(pk_mx4 * w, const void * x, int32_t x_type, int64_t rows, int64_t x_stride, void * y,
-                                          int32_t y_type, int64_t y_stride, void * workspace, int64_t workspace_bytes,
-                                          void * stream) {
-    const char * fn = "pk_mx4_linear";
+// A product that reports to the error word `err_dev` (the device's address of it); null: to the layer's, whose
+// unreported timeouts it then tells of instead of running.
+pk_status pk::mx4_linear(pk_mx4 * w, const char * fn, const void * x, int32_t x_type, int64_t rows, int64_t x_stride, void * y,
+                         int32_t y_type, int64_t y_stride, void * workspace, int64_t workspace_bytes, void * stream, int * err_dev) {
     if (!w) return op_fail(PK_ERR_INVALID, fn, "null layer");
     if (elem_size(x_type) == 0 || elem_size(y_type) == 0) return op_fail(PK_ERR_INVALID, fn, "element types must be F32, F16 or BF16");
     if (rows < 0 || rows > kMaxRows) return op_fail(PK_ERR_INVALID, fn, "rows must be in [0, 2^31)");
@@ -1449,13 +1459,18 @@ extern "C" PK_API pk_status pk_mx4_linear(pk_mx4 * w, const void * x, int32_t x_
     if (!aligned_to(workspace, 256)) return op_fail(PK_ERR_INVALID, fn, "workspace must be 256-byte aligned");
     if (workspace_bytes < need)
         return op_fail(PK_ERR_INVALID, fn, "workspace_bytes is below pk_mx4_workspace(w, rows)");
-    if (mx4_take_timeout(w)) return op_fail(PK_ERR_TIMEOUT, fn, "a device-side wait of an earlier call ran out");
+    if (!err_dev) {
+        notice_timeout(w);
+        if (__atomic_exchange_n(&w->unreported, 0, __ATOMIC_ACQ_REL))
+            return op_fail(PK_ERR_TIMEOUT, fn, "a device-side wait of an earlier call ran out; this call did not run");
+        err_dev = w->err_dev;
+    }
     DeviceScope dev(w->device);
     if (dev.err != cudaSuccess) return op_cuda_fail(dev.err, fn);
     cudaStream_t s = (cudaStream_t) stream;
     unsigned char * xc = static_cast<unsigned char *>(workspace);
     unsigned char * xs = xc + ws_codes(w, rows);
-    const Waits waits{__atomic_load_n(&w->wait_ns, __ATOMIC_RELAXED), w->err_dev, __atomic_exchange_n(&w->stall, 0, __ATOMIC_RELAXED)};
+    const Waits waits{__atomic_load_n(&w->wait_ns, __ATOMIC_RELAXED), err_dev, __atomic_exchange_n(&w->stall, 0, __ATOMIC_RELAXED)};
     const Call c{w, waits, x, x_stride, rows, y, y_stride, s};
     cudaError_t e;
     if (few(w, rows)) {
@@ -1468,4 +1483,16 @@ extern "C" PK_API pk_status pk_mx4_linear(pk_mx4 * w, const void * x, int32_t x_
                 : y_type == PK_GGML_F16 ? launch_product<__half>(c, y_type, xc, xs) : launch_product<__nv_bfloat16>(c, y_type, xc, xs);
     }
     return e == cudaSuccess ? PK_OK : op_cuda_fail(e, fn);
+}
+
+extern "C" PK_API pk_status pk_mx4_linear(pk_mx4 * w, const void * x, int32_t x_type, int64_t rows, int64_t x_stride, void * y,
+                                          int32_t y_type, int64_t y_stride, void * workspace, int64_t workspace_bytes,
+                                          void * stream) {
+    return pk::mx4_linear(w, "pk_mx4_linear", x, x_type, rows, x_stride, y, y_type, y_stride, workspace, workspace_bytes, stream, nullptr);
+}
+
+extern "C" PK_API int64_t pk_mx4_timeouts(pk_mx4 * w) {
+    if (!w) return -1;
+    notice_timeout(w);
+    return __atomic_load_n(&w->timeouts, __ATOMIC_ACQUIRE);
 }

@@ -299,6 +299,7 @@ struct pk_ctc {
     int V = 0, blank = 0;
     pk::Buf logits, best, foff, roff, nfr, prev_in, prev_out, rtok, rframe, counts, offs, otok, oframe;
     pk::Buf frames, work, uniforms;   // pk_ctc_decode: encoder frames, product workspace, random numbers
+    int * err = nullptr, * err_dev = nullptr;   // its products' error word, on the host and on the device
 };
 
 struct pk_vocab {
@@ -348,6 +349,7 @@ extern "C" PK_API void pk_ctc_destroy(pk_ctc * c) {
                         &c->counts, &c->offs, &c->otok, &c->oframe, &c->frames, &c->work, &c->uniforms})
         b->release();
     if (c->stream) cudaStreamDestroy(c->stream);
+    if (c->err) pk::give_error_word(c->err);
     delete c;
 }
 
@@ -399,8 +401,8 @@ pk_status ctc_frame_tokens(pk_ctc * c, const char * fn, pk_mx4 * head, const flo
         const float * logits = dx + f * (int64_t) K;
         int * best = c->best.as<int>() + at + f;
         if (head) {
-            const pk_status st = pk_mx4_linear(head, logits, PK_GGML_F32, n, K, c->logits.p, PK_GGML_F32, c->V, c->work.p,
-                                               (int64_t) c->work.cap, s);
+            const pk_status st = mx4_linear(head, fn, logits, PK_GGML_F32, n, K, c->logits.p, PK_GGML_F32, c->V, c->work.p,
+                                            (int64_t) c->work.cap, s, c->err_dev);
             if (st != PK_OK) return st;
             logits = c->logits.as<float>();
         }
@@ -507,6 +509,17 @@ pk_status ctc_run(pk_ctc * c, const char * fn, pk_mx4 * head, const float * logi
         const int64_t ws = pk_mx4_workspace(head, step);
         TX_STEP(c->logits.ensure((size_t) step * c->V * 4), fn, "alloc");
         TX_STEP(c->work.ensure((size_t) std::max<int64_t>(ws, 1)), fn, "alloc");
+        if (!c->err) {
+            cudaError_t e = cudaSuccess;
+            c->err = take_error_word(e);
+            if (c->err) e = cudaHostGetDevicePointer(reinterpret_cast<void **>(&c->err_dev), c->err, 0);
+            if (c->err && e != cudaSuccess) {
+                give_error_word(c->err);
+                c->err = nullptr;
+            }
+            TX_STEP(e, fn, "error word");
+        }
+        take_error(c->err);                               // of a call that ended before it asked
     }
     for (const Stretch & p : parts) {
         const float * dx = logits_on_device ? logits + p.begin * width : in.as<float>() + p.at * width;
@@ -522,7 +535,7 @@ pk_status ctc_run(pk_ctc * c, const char * fn, pk_mx4 * head, const float * logi
     TX_STEP(cudaGetLastError(), fn, "scan launch");
     TX_STEP(cudaMemcpyAsync(token_offsets, c->offs.p, (size_t) (B + 1) * 8, cudaMemcpyDeviceToHost, s), fn, "offsets copy");
     TX_STEP(cudaStreamSynchronize(s), fn, "sync");
-    if (head && mx4_take_timeout(head)) {
+    if (c->err && take_error(c->err)) {
         char msg[160];
         std::snprintf(msg, sizeof(msg), "%s: a device-side wait of the head's product ran out", fn);
         return set_error(PK_ERR_TIMEOUT, msg);

@@ -564,6 +564,7 @@ def test_an_error_stays_with_its_call(built):
 
 def test_option_refusals(built):
     assert built.lib().pk_mx4_set_option(None, built.abi.PK_OPT_TIMEOUT_US, 5) == built.abi.PK_ERR_INVALID
+    assert built.lib().pk_mx4_timeouts(None) == -1
 
 
 def stalled(pk, layer, x, y, ws):
@@ -629,3 +630,63 @@ def test_a_pair_whose_wait_runs_out(built, r, n, k, y_dtype, ypad):
             layer.forward(dx.data_ptr(), r, y.data_ptr(), y_stride=n + ypad, workspace=ws.data_ptr(), workspace_bytes=ws.numel())
         assert e.value.status == pk.abi.PK_ERR_TIMEOUT
         check_product(ref_quantize(w)[2], *product(pk, w, x, None, "f32", y_dtype, 0, ypad, layer=layer))
+
+
+@pytest.mark.gpu
+def test_timeouts_reach_their_own_caller(built):
+    """A decode through a shared head neither takes nor gets the report of somebody else's product; its own product's
+    goes to it alone. Replays of a captured product count."""
+    import torch
+    pk = built
+    rng = np.random.default_rng(0)
+    r, n, k = 300, 65, 96
+    w = rng.integers(-2, 3, (n, k)).astype(np.float32)     # exact whichever kernel takes it
+    x = rng.integers(-2, 3, (r, k)).astype(np.float32)
+    head, ctc, other = pk.Mx4Linear(w), pk.CtcGreedy(n, 0), pk.CtcGreedy(n, 0)
+    dx, y = torch.from_numpy(x).cuda(), torch.zeros(r, n, device="cuda")
+    ws = torch.zeros(head.workspace(r), dtype=torch.uint8, device="cuda")
+    want = ctc.decode_frames(x, [0], [r], head=head)[0][0]
+    timeout = pk.abi.PK_ERR_TIMEOUT
+
+    def refused(f):
+        with pytest.raises(pk.PkError) as e:
+            f()
+        assert e.value.status == timeout
+        return str(e.value)
+
+    def forward():
+        head.forward(dx.data_ptr(), r, y.data_ptr(), workspace=ws.data_ptr(), workspace_bytes=ws.numel())
+
+    stalled(pk, head, dx, y, ws)                           # somebody's product, still waiting or done
+    for i in range(2):
+        assert np.array_equal(ctc.decode_frames(x, [0], [r], head=head)[0][0], want)
+        torch.cuda.synchronize()
+    assert head.timeouts() == 1 and head.timeouts() == 1   # asking does not take the report
+    assert "did not run" in refused(forward)
+    forward()
+    assert head.timeouts() == 1
+    # a decode's own product; other handles and forward() hear nothing of it
+    head.set_option(pk.abi.PK_OPT_TIMEOUT_US, 20_000)
+    head.set_option(pk.abi.PK_OPT_TEST_STALL, 1)
+    prev = np.array([3], np.int32)
+    assert "pk_ctc_decode" in refused(lambda: ctc.decode_frames(x, [0], [r], head=head, prev=prev))
+    head.set_option(pk.abi.PK_OPT_TIMEOUT_US, 2_000_000)
+    forward()
+    assert head.timeouts() == 1
+    for c in (other, ctc):
+        assert np.array_equal(c.decode_frames(x, [0], [r], head=head)[0][0], want)
+    g = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g):
+        stalled(pk, head, dx, y, ws)
+    assert head.timeouts() == 1
+    for i in range(2):
+        g.replay()
+        torch.cuda.synchronize()
+        assert head.timeouts() == 2 + i
+    refused(forward)
+    forward()
+    torch.cuda.synchronize()
+    assert head.timeouts() == 3 and torch.equal(y.cpu(), torch.from_numpy(x @ w.T))
+    ctc.close()
+    other.close()
