@@ -690,3 +690,15 @@ def test_timeouts_reach_their_own_caller(built):
     assert head.timeouts() == 3 and torch.equal(y.cpu(), torch.from_numpy(x @ w.T))
     ctc.close()
     other.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("r", [3, 40, 700, 2600])
+def test_nonfinite_weights_stay_in_their_outputs(built, r):
+    rng = np.random.default_rng(r)
+    n, k = 1300, 1601
+    w = rng.standard_normal((n, k)).astype(np.float32)
+    w[0, 5], w[700, k - 1], w[n - 1, 900] = np.nan, np.inf, -np.inf
+    seen, y = product(built, w, rng.standard_normal((r, k)))
+    assert np.isnan(y[:, [0, 700, n - 1]]).all()
+    check_product(ref_quantize(w)[2], seen, y)

@@ -656,3 +656,91 @@ def test_ctc_reads_only_its_utterances(built):
     with pytest.raises(pk.PkError, match="out of range"):
         ctc.decode_frames(x.data_ptr(), [1 << 62], [4], on_device=True)
     ctc.close()
+
+
+def strictly(seen, u, tok, lp, **kw):
+    """check(), with no way round it: where u times the kept sum lies nearer to a border between two kept tokens
+    than the weights' roundings move it (each weight by 2^-44 and 2^-42 of itself, the border and the sum once
+    each), the token is one of the two, and it is that token's log-probability. f32 sums are allowed for only where
+    pk_sample takes them: rows with nothing cut of up to 2048 logits from 1184 rows on, and top-p without a cut by
+    k for up to 16384 logits, except for few long rows (up to 296 of more than 2048) and many short ones (2960
+    and more of up to 1056). Their sums are off by 58 and 66 times 2^-24 (see check), the f32 logarithm by two
+    steps of itself and one of its argument."""
+    kw = {**DEFAULTS, **kw}
+    r, v = seen.shape
+    near = 0
+    for i in range(r):
+        o = {n: (x[i] if np.ndim(x) else x) for n, x in kw.items()}
+        temp, k, p, m = np.float64(np.float32(o["temperature"])), int(o["top_k"]), np.float64(np.float32(o["top_p"])), np.float64(np.float32(o["min_p"]))
+        l = np.where(np.isnan(seen[i]), -np.inf, seen[i].astype(np.float64))
+        a = (l - l.max()) / temp
+        w = np.exp(a)
+        w[w < 2.0 ** -44] = 0.0
+        order = np.argsort(-l, kind="stable")
+        s = w[order]
+        if 0 < k < v:
+            s[k:] = 0.0
+        slack = 2 * (v * 2.0 ** -44 + s.sum() * 2.0 ** -42)
+        if p < 1:
+            before = np.cumsum(s) - s
+            assert np.abs(before - p * s.sum())[s > 0].min() > slack       # the cut itself is never in doubt
+            s = np.where((before < p * s.sum()) | (np.arange(v) == 0), s, 0.0)
+        if m > 0:
+            assert np.abs(s[s > 0] / m - 1).min() > 1e-12
+            s = np.where(s >= m, s, 0.0)
+        w = np.zeros(v)
+        w[order] = s
+        some = np.flatnonzero(w)
+        ends = np.cumsum(w[some])
+        x = float(np.float32(u[i])) * ends[-1]
+        j = min(int(np.searchsorted(ends, x, side="right")), len(some) - 1)
+        allowed = {int(some[j])}
+        if j > 0 and x - ends[j - 1] <= slack:
+            allowed.add(int(some[j - 1]))
+        if j + 1 < len(some) and ends[j] - x <= slack:
+            allowed.add(int(some[j + 1]))
+        near += len(allowed) > 1
+        assert int(tok[i]) in allowed, (i, tok[i], allowed, o, u[i])
+        want = a[tok[i]] - np.log(ends[-1])
+        cut = 0 < k <= int((l > l.max() - 31 * temp).sum())    # fewer than k tokens with any weight are not cut by k
+        filters = 0 < k < v or p < 1 or m > 0 or any(np.ndim(x) for n, x in kw.items() if n != "temperature")
+        f32 = (v <= 2048 and r >= 1184) if not filters else (
+            not cut and p < 1 and v <= 16384 and not (v <= 1056 and r >= 2960) and not (r <= 296 and v > 2048))
+        tol = 2.0 ** -24 * abs(want) + v * 2.0 ** -43 + 2.0 ** -40
+        if f32:
+            tol += 2.0 ** -24 * ((66 if filters else 58) + 1 + 2 * abs(np.log(ends[-1])) + 3 * abs(a[tok[i]]))
+        assert abs(lp[i] - want) <= tol, (i, lp[i], want, tol)
+    assert near <= r // 100 + 1                            # or the test says little
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kw", [dict(), dict(temperature=0.7), dict(top_k=50), dict(top_p=0.9), dict(top_p=0.97, min_p=0.003, temperature=1.3),
+                                dict(top_k=30, top_p=0.9, min_p=0.01)], ids=["plain", "T", "k", "p", "pm", "kpm"])
+@pytest.mark.parametrize("r,v", [(40, 33), (40, 1025), (300, 8193), (600, 2048), (1200, 1025), (3000, 1025), (20, 40001)])
+def test_tokens_strictly(built, r, v, kw):
+    rng = np.random.default_rng(r + v)
+    l = rng.standard_normal((r, v)) * rng.choice([0.3, 2.5], (r, 1))
+    l[rng.random((r, v)) < 0.1] = -np.inf
+    u = rng.random(r).astype(np.float32)
+    u[0], u[1] = 0.0, 1 - 2.0 ** -24
+    seen, tok, lp = run(built, l, u, "f32", 1, 0, **kw)
+    strictly(seen, u, tok, lp, **kw)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("r,v", [(2, 500_001), (80, 102_001), (40, 204_001)])
+def test_rows_past_shared_memory(built, r, v, dtype):
+    """Rows whose share of a cluster's block does not fit its shared memory are read anew in each pass."""
+    rng = np.random.default_rng(v)
+    l = rng.standard_normal((r, v)).astype(np.float32) * 3
+    l[:, ::5] = -np.inf
+    l[:, 7::1001] = np.nan
+    l[-1, [5, v - 1]] = np.inf
+    if r > 2:
+        l[1], l[2] = -np.inf, 0.0
+    u = rng.random(r).astype(np.float32)
+    some = np.unique(np.concatenate([np.arange(min(r, 6)), [r - 1]]))
+    for kw in (dict(), dict(temperature=0.0), dict(top_k=40), dict(top_k=5000, top_p=0.9), dict(top_p=0.95, temperature=0.8), dict(min_p=0.01)):
+        seen, tok, lp = run(built, l, u, dtype, 3, 1, **kw)
+        check(seen[some], u[some], tok[some], lp[some], **kw)
