@@ -45,9 +45,9 @@ constexpr int kList = 128;                 // tokens that are ranked against eac
 constexpr int kMaxCluster = 8;
 constexpr unsigned kFull = 0xFFFFFFFFu;
 
-// 2^(j / 32), j = 0 .. 31.
+// 2^(j / 32), j = 0 .. 31, the first with its last bit set (see weight_onto).
 __device__ const double kExp2[32] = {
-    0x1.0000000000000p+0, 0x1.059b0d3158574p+0, 0x1.0b5586cf9890fp+0, 0x1.11301d0125b51p+0,
+    0x1.0000000000001p+0, 0x1.059b0d3158574p+0, 0x1.0b5586cf9890fp+0, 0x1.11301d0125b51p+0,
     0x1.172b83c7d517bp+0, 0x1.1d4873168b9aap+0, 0x1.2387a6e756238p+0, 0x1.29e9df51fdee1p+0,
     0x1.306fe0a31b715p+0, 0x1.371a7373aa9cbp+0, 0x1.3dea64c123422p+0, 0x1.44e086061892dp+0,
     0x1.4bfdad5362a27p+0, 0x1.5342b569d4f82p+0, 0x1.5ab07dd485429p+0, 0x1.6247eb03a5585p+0,
@@ -67,9 +67,9 @@ struct Row {
 // = 1 + t q(t) with q cubic, interpolating at the four Chebyshev nodes of [-1/2, 1/2] (off by
 // 2^-42.5 at most; exactly 1 at t = 0). Adding a number of [2^52, 2^53) rounds the product to an
 // integer in the low bits. A product halfway between two integers would go to the one that makes the
-// sum so far even, and sums would depend on their order: the last bit of the value at t is set (1 still
-// rounds to 2^43), which leaves the product its lowest bit far below a half, 2^-9 at the most, and no
-// product is halfway. `entry(n)` gives 2^43 * table[n % 32] with n % 32 taken off the exponent
+// sum so far even, and sums would depend on their order. None is halfway: a table entry's lowest bit is at
+// 2^-46 or below (1 is held as 1 + 2^-52 for that), the polynomial's at 2^0 or below, so that of their
+// product times 2^43 is at 2^-3 or below; 1 still rounds to 2^43. `entry(n)` gives 2^43 * table[n % 32] with n % 32 taken off the exponent
 // field's place 15 bits up, where all of n is added. All callers share these operations.
 template <class F>
 __device__ __forceinline__ double weight_onto(float v, const Row & r, double onto, F entry) {
@@ -82,7 +82,6 @@ __device__ __forceinline__ double weight_onto(float v, const Row & r, double ont
     q = fma(q, t, 0.00023459619820112603);
     q = fma(q, t, 0.021660849392187844);
     q = fma(q, t, 1.0);
-    q = __hiloint2double(__double2hiint(q), __double2loint(q) | 1);
     const int n = __double2loint(y);
     const double e = entry(n);
     return fma(q, __hiloint2double(__double2hiint(e) + (n << 15), __double2loint(e)), onto);
