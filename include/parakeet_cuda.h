@@ -548,7 +548,9 @@ PK_API int64_t   pk_mx4_timeouts(pk_mx4 * w);
  * exponentials in 64-bit floating point), so the token is the same whatever the batch, and
  * tokens with less than 2^-44 of the largest weight are never drawn. Where 32-bit sums with
  * a proven bound tell the token they are used instead: it is the same one, and the
- * log-probability is then within 2^-17, mostly 2^-23, of its value. */
+ * log-probability is then within 2^-17, mostly 2^-23, of its value. Whether they are
+ * tried goes by the number of rows, so within that bound a log-probability may differ
+ * with the batch. */
 #define PK_SAMPLE_MAX_VOCAB 524288
 
 typedef struct pk_sample_args {

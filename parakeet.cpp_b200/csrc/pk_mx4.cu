@@ -268,8 +268,8 @@ __device__ __forceinline__ unsigned scale_word(unsigned sb) {
 // rows of up to 256 values: 2^gs lanes a row, and the next rows instead of the next segments (483966 rows of
 // 49 bf16: 24 us, a warp a row 114).
 // ATOMS: scales in the product's layout, zeros for the blocks past K that its stages read.
-// Bound: HBM from f32 (66044 x 1024: 44 us, 6.9 TB/s read and written), instructions from half precision
-// (66043 x 1000 bf16: 31 us, 5.4 TB/s).
+// Bound: HBM from f32 (66044 x 1024: 44 us, of which the 270 MB read are 6.1 TB/s; the 36 MB written stay in
+// L2), instructions from half precision (66043 x 1000 bf16: 32 us for 132 MB read and 35 written).
 template <class T, bool VEC, bool ATOMS, bool SHORT>
 __global__ void __launch_bounds__(kQThreads) mx4_quantize_kernel(const T * __restrict__ x, long long rows, int K, long long ldx, int gs,
                                                                  unsigned char * __restrict__ codes,
@@ -378,7 +378,7 @@ template <> __device__ __forceinline__ void codes_to_values(unsigned q, unsigned
 }
 
 // The value of each code, eight a lane, rows and lanes as in the quantisation. Bound: HBM, writing y
-// (66043 x 1000 bf16: 33 us, 5.1 TB/s).
+// (66043 x 1000 bf16: 34 us for 35 MB read, mostly from L2, and 132 written).
 template <class T, bool VEC, bool SHORT>
 __global__ void __launch_bounds__(kQThreads) mx4_dequantize_kernel(const unsigned char * __restrict__ codes,
                                                                    const unsigned char * __restrict__ scales, long long rows,
@@ -477,8 +477,9 @@ struct Waits {
 
 constexpr int kTM = 128;
 template <bool BOX> constexpr int tc_stages() { return BOX ? 5 : 4; }
-// Warps of the epilogue, for each 32 rows two where TMA stores y and four where the warps do (16391 x 1025:
-// 37 us against 41 with two; 66044 x 640 by TMA: 92 us against 99 with four).
+// Warps of the epilogue, for each 32 rows two where TMA stores y and four where the warps do (layers replayed
+// from a graph, quantisation included: 16391 x 1024 by 1025 34.9 us, with two 36.8; 66044 x 1024 by 640, by TMA,
+// 90.4 us, with four, whose staging costs a stage of the ring, 94.4).
 template <bool BOX> constexpr int epi_warps() { return BOX ? 8 : 16; }
 template <bool BOX> constexpr int tc_threads() { return 32 * (4 + epi_warps<BOX>()); }
 constexpr unsigned kScaleA = 1024;                      // two atoms of 128 rows
@@ -900,8 +901,8 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant_
 // a graph 5.2 and 6.6 us for 1 x 1024, 6.4 and 6.8 for 16, 7.8 and 7.0 for 32; 8.5 and 8.2 for 16 x 2048,
 // 10.8 and 8.6 for 32: hence the bound on the values of x. Not so
 // for more rows: at 64 the rows' loads, again in every block, take longer than the second launch
-// (14.3 us against 11.4), and at 66044 two kernels are 97 us against 111 with the codes kept on the
-// SM, sixteen warps of one block being too few to keep x streaming.
+// (called from Python 14.3 us against 11.4), and at 66044 keeping the codes on the SM took a seventh longer
+// than two kernels, sixteen warps of one block being too few to keep x streaming.
 constexpr int kFewRows = 32;
 constexpr int kFewK = 2048;                             // the rows' codes stay in shared memory
 constexpr int kFewX = 32768;                            // every block quantises all of x
@@ -1235,8 +1236,8 @@ template <class TX> cudaError_t launch_few(const Call & c, int y_type) {
 bool few(const pk_mx4 * w, int64_t rows) { return rows <= kFewRows && w->K <= kFewK && rows * w->K <= kFewX; }
 
 // Tile width of the single blocks: fewest rounds of tiles over the SMs, a round costed by the rows that
-// a tile loads. (192, with fewer loads a product, was slower where K is short: 66044 x 640 x 1024 97 us
-// against 94, 16391 x 1025 44 against 41; where K is long the pairs are faster.)
+// a tile loads. (192, with fewer loads a product, was slower where K is short: by 3 % for 66044 x 1024 by 640, by
+// 7 % for 16391 x 1024 by 1025; where K is long the pairs are faster.)
 bool narrow_tiles(long long M, int N) {
     auto cost = [&](int bn) { return ((M + kTM - 1) / kTM * ((N + bn - 1) / bn) + 147) / 148 * (kTM + bn); };
     return cost(64) < cost(128);
@@ -1249,8 +1250,11 @@ template <class T> cudaError_t launch_product(const Call & c, int y_type, const 
     if (e != cudaSuccess) return e;
     const bool box = map_y(&ymap, c.y, y_type, c.M, c.w->N, c.ldy, e);
     if (e != cudaSuccess) return e;
-    // Pairs where there are tiles for all of them and K is long: 135 us against 159 at K = 4096 (8192 x
-    // 8192), but 51 against 45 at K = 1024 (16391 x 1025), where stores count more than loads.
+    // Pairs where there are tiles for all of them and K is long. Layers replayed from a graph, pairs and single
+    // blocks, at K = 1024, 1536, 1792, 2048 and 4096: 16391 rows by 1025 42 us and 35, 48 and 45, 50 and 50, 52 and
+    // 54, 83 and 91; 66044 by 640 98 and 91, 128 and 127, 145 and 147, 159 and 165, 286 and 304. With more work for
+    // each load pairs gain earlier (8192 by 8192 at 1024: 53 and 62, at 512: 47 and 41), with few tiles never (2600
+    // by 1300, 1.6 rounds of pairs, at 4096: 24.3 and 23.4); the rule is set by the first two.
     if (c.w->K > 1536 && (c.M + 2 * kTM - 1) / (2 * kTM) * ((c.w->N + 127) / 128) >= 74) {
         const long long mp = (c.M + 2 * kTM - 1) / (2 * kTM);
         const long long r128 = (mp * ((c.w->N + 127) / 128) + 73) / 74 * (kTM + 64), r192 = (mp * ((c.w->N + 191) / 192) + 73) / 74 * (kTM + 96);

@@ -13,10 +13,11 @@
 // rows, since a row has as many borders as tokens.
 //
 // Rows of up to 2048 logits with nothing cut, as a CTC path has them by the ten thousand, are summed in
-// f32 first: four instructions a token instead of twenty. That settles the token unless the random
-// number lies within a proven bound of a border (one or two rows in a hundred), and those rows go on to
-// the f64 sums, so the token is the same; the log-probability then has f32's sum, 2^-18 off at most.
-// 66044 rows of 1025: see draw_f32.
+// f32 first: four instructions a token for weight and sum instead of twenty. That settles the token unless
+// the random number lies within a proven bound of a border (one or two rows in a hundred), and those rows go
+// on to the f64 sums, so the token is the same; the log-probability then has f32's sum, 2^-18 off at most
+// (see draw_f32). 66044 rows of 1025 take 67 us replayed from a graph, 865 warp instructions a row, 26 for
+// every 32 logits: most of them stage the row, find its maximum and scan.
 //
 // A team of threads (a warp, a block, or a cluster of blocks) holds one row in shared memory:
 //  1. load, largest and smallest logit;
@@ -1250,24 +1251,25 @@ cudaError_t launch_cluster(const pk_sample_args & a, int blocks, cudaStream_t s)
 
 template <class T, bool FILTERS>
 cudaError_t dispatch(const pk_sample_args & a, cudaStream_t s) {
-    // A row a warp, in blocks of eight, from one block an SM on with nothing cut (1500 rows of 600: 5.7 us, with
-    // a block of 128 a row 6.1; 700 rows: 5.3 and 3.9; 20000 rows of 2048: 43 and 81) and from 20 rows an SM on
-    // with filters, if three such blocks and their bins fit an SM (6000 rows of 1025, top-p: 52 us and 58, 1500
-    // rows of top-k: 42 and 30; 6000 rows of 1150: 69 and 59).
+    // All figures here: replayed from a graph, peaked logits (spread 2.5 and a few likely tokens), p = 0.9.
+    // A row a warp, in blocks of eight, from one block an SM on with nothing cut (1500 rows of 600: 5.8 us, with
+    // a block of 128 a row 7.2; 700 rows: 5.4 and 4.3; 20000 rows of 2048: 45 and 85) and from 20 rows an SM on
+    // with filters, if three such blocks and their bins fit an SM (6000 rows of 1025, top-p: 54 us and 62, 1500
+    // rows with k = 64: 53 and 35; 6000 rows of 1150: 70 and 64).
     if (FILTERS ? a.vocab <= 1056 && a.rows >= 20 * 148 : a.vocab <= 2048 && a.rows >= 8 * 148) return launch_block<T, FILTERS, 32>(a, s);
     // Few rows of a large vocabulary over clusters. A cluster's barriers cost more than they save below (one
-    // row with top-p, in one block of 512 and in a cluster of eight: of 8193 13 us and 20, of 20000 22 us
-    // and 21, of 50000 45 us and 23).
+    // row with top-p, in one block of 512 and in a cluster of eight: of 8193 14 us and 23, of 20000 24 us
+    // and 23, of 50000 48 us and 25).
     int blocks = 1;
     if (a.vocab > 16384)
         while (blocks < kMaxCluster && a.rows * blocks * 2 <= 148) blocks *= 2;
     while (blocks < kMaxCluster && (size_t) (a.vocab / blocks) * 4 > 200 * 1024) blocks *= 2;
     if (blocks > 1) return launch_cluster<T, FILTERS>(a, blocks, s);
     // Otherwise a row a block, of as many threads as let every row have its block at once (450 rows of 4097,
-    // top-p, in blocks of 128, 256 and 512: 26 us, 20, 25; 296 rows: 25, 18, 14), though of at least 256 for
-    // up to 2048 logits (one row of 1600: 6.3 us, of 512 7.8). Past that the fewest threads that a row's length
-    // leaves busy: 128 up to 5120 (4096 rows of 4097: 79 us, 89, 170), 256 up to 16384 (4096 rows of 8193:
-    // 143 us, 131, 232), 512.
+    // top-p, in blocks of 128, 256 and 512: 27 us, 22, 26; 296 rows: 26, 20, 15), though of at least 256 for
+    // up to 2048 logits (one row of 1600: 6.7 us, of 512 8.2). Past that the fewest threads that a row's length
+    // leaves busy: 128 up to 5120 (4096 rows of 4097: 90 us, 100, 172), 256 up to 16384 (4096 rows of 8193:
+    // 219 us, 160, 242), 512.
     const bool wave512 = a.rows <= 2 * 148 && a.vocab > 2048, wave256 = a.rows <= 4 * 148;
     if (a.vocab > 16384 || wave512) return launch_block<T, FILTERS, 512>(a, s);
     if (a.vocab > 5120 || wave256) return launch_block<T, FILTERS, 256>(a, s);
