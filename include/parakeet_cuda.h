@@ -478,7 +478,8 @@ PK_API pk_status pk_detokenize(pk_vocab * v, const int32_t * tokens, int32_t tok
  * without waiting for it; they allocate nothing and may be captured into a CUDA
  * graph. They leave the caller's current device as it was. Pointers are aligned to
  * their element; rows may start at any multiple of that (16-byte aligned rows are
- * read fastest). Inputs, outputs and workspace must not overlap. */
+ * read fastest) and are at most 2^29 - 1 elements apart. Inputs, outputs and workspace
+ * must not overlap. */
 
 /* x: [rows][row_stride] of x_type, of which the first `cols` of each row are read.
  * codes: [rows][16 * nb], nb = ceil(cols / 32), value 2i of a row in the low half of
