@@ -528,6 +528,53 @@ PK_API pk_status pk_mx4_linear(pk_mx4 * w, const void * x, int32_t x_type, int64
  * layer. pk_ctc_decode's products count and report only there. */
 PK_API int64_t   pk_mx4_timeouts(pk_mx4 * w);
 
+/* ---- 8-bit floating point with a scale for each block of 128 --------------------
+ *
+ * No counterpart in the reference. Between f16 and MXFP4: a value is held as one e4m3
+ * code (three bits of fraction, magnitudes up to 448, the smallest 2^-9) and one
+ * power-of-two scale byte (e8m0) per block: value = e4m3 * 2^(byte - 127); byte 255 makes
+ * its whole block NaN, code 0x7F or 0xFF its value. Blocks are 128 consecutive values of a
+ * row of x, and 128 rows by 128 values of a weight matrix.
+ *
+ * Quantisation of a block: the exponent is the smallest, not below -127, that brings the
+ * largest magnitude to at most 448, and each code the e4m3 value nearest to
+ * x / 2^exponent, a tie going to the even code; nothing saturates. A block of zeros gets
+ * byte 0; a block that holds an infinity or a NaN gets byte 255. A last block that an edge
+ * cuts short is filled up with zeros.
+ *
+ * Device, stream, waiting, alignment, strides and overlap as for pk_mx4_quantize above. */
+
+/* x: [rows][row_stride] of x_type, of which the first `cols` of each row are read.
+ * codes: [rows][16 * ceil(cols / 16)], zeros behind `cols` (8-byte aligned); scales:
+ * [rows][ceil(cols / 128)]. */
+PK_API pk_status pk_fp8_quantize(int device, const void * x, int32_t x_type, int64_t rows, int64_t cols,
+                                 int64_t row_stride, uint8_t * codes, uint8_t * scales, void * stream);
+/* The values that codes and scales stand for, rounded to y_type: y is [rows][row_stride],
+ * the first `cols` of each row are written. */
+PK_API pk_status pk_fp8_dequantize(int device, const uint8_t * codes, const uint8_t * scales, int64_t rows,
+                                   int64_t cols, void * y, int32_t y_type, int64_t row_stride, void * stream);
+
+/* A linear layer [N][K] held in 8 bits on one device. */
+typedef struct pk_fp8 pk_fp8;
+
+/* As pk_mx4_create; weight types F32, F16, BF16 and Q8_0 (K then a multiple of 32). */
+PK_API pk_status pk_fp8_create(int device, const pk_tensor * weight, int32_t on_device, const float * bias, pk_fp8 ** out);
+/* As pk_mx4_set_option. */
+PK_API pk_status pk_fp8_set_option(pk_fp8 * w, int32_t option, int64_t value);
+/* Waits for the device's queued work, so no call on the layer is still running. */
+PK_API void      pk_fp8_destroy(pk_fp8 * w);
+/* Bytes of device workspace that pk_fp8_linear needs for `rows` rows (never less for
+ * more rows), 0 where it needs none; -1 for a null layer. */
+PK_API int64_t   pk_fp8_workspace(const pk_fp8 * w, int64_t rows);
+/* y[m][n] = bias[n] + sum_k q(x)[m][k] * W[n][k]: each row of x is quantised as
+ * pk_fp8_quantize does, products are exact and sums are held in 32 bits; y rounds once to
+ * y_type. Arguments, workspace and PK_ERR_TIMEOUT as for pk_mx4_linear. */
+PK_API pk_status pk_fp8_linear(pk_fp8 * w, const void * x, int32_t x_type, int64_t rows, int64_t x_stride, void * y,
+                               int32_t y_type, int64_t y_stride, void * workspace, int64_t workspace_bytes,
+                               void * stream);
+/* As pk_mx4_timeouts; pk_ctc_decode_fp8's products count and report only there. */
+PK_API int64_t   pk_fp8_timeouts(pk_fp8 * w);
+
 /* ---- drawing tokens from logits -----------------------------------------------
  *
  * No counterpart in the reference, whose decoders take the argmax. For each row of
@@ -602,6 +649,12 @@ PK_API pk_status pk_ctc_decode(pk_ctc * c, pk_mx4 * head, const float * frames, 
                                const int64_t * frame_offsets, const int32_t * n_frames, int32_t B,
                                const pk_ctc_draw * draw, int32_t * prev_inout, int32_t * tokens, int64_t tokens_cap,
                                int64_t * token_offsets, int32_t * first_frame, int64_t * tokens_needed);
+
+/* The same with a head held in 8 bits. */
+PK_API pk_status pk_ctc_decode_fp8(pk_ctc * c, pk_fp8 * head, const float * frames, int32_t frames_on_device,
+                                   const int64_t * frame_offsets, const int32_t * n_frames, int32_t B,
+                                   const pk_ctc_draw * draw, int32_t * prev_inout, int32_t * tokens, int64_t tokens_cap,
+                                   int64_t * token_offsets, int32_t * first_frame, int64_t * tokens_needed);
 
 #ifdef __cplusplus
 }

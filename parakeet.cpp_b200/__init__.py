@@ -73,8 +73,15 @@ def lib():
             "pk_mx4_workspace": ([P, I64], I64), "pk_mx4_set_option": ([P, I32, I64], I32),
             "pk_mx4_timeouts": ([P], I64),
             "pk_mx4_linear": ([P, P, I32, I64, I64, P, I32, I64, P, I64, P], I32),
+            "pk_fp8_quantize": ([I32, P, I32, I64, I64, I64, P, P, P], I32),
+            "pk_fp8_dequantize": ([I32, P, P, I64, I64, P, I32, I64, P], I32),
+            "pk_fp8_create": ([I32, P, I32, P, P], I32), "pk_fp8_destroy": ([P], None),
+            "pk_fp8_workspace": ([P, I64], I64), "pk_fp8_set_option": ([P, I32, I64], I32),
+            "pk_fp8_timeouts": ([P], I64),
+            "pk_fp8_linear": ([P, P, I32, I64, I64, P, I32, I64, P, I64, P], I32),
             "pk_sample": ([I32, P, P], I32),
             "pk_ctc_decode": ([P, P, P, I32, P, P, I32, P, P, P, I64, P, P, P], I32),
+            "pk_ctc_decode_fp8": ([P, P, P, I32, P, P, I32, P, P, P, I64, P, P, P], I32),
         }
         for name, (args, res) in sigs.items():
             f = getattr(L, name)
@@ -404,8 +411,8 @@ class CtcGreedy:
 
     def decode_frames(self, frames, frame_offsets, n_frames, head=None, uniforms=None, temperature=1.0, top_k=0, top_p=1.0,
                       min_p=0.0, prev=None, on_device=False, uniforms_on_device=False, with_frames=False):
-        """pk_ctc_decode: decode() from encoder frames through `head` (an Mx4Linear, vocab_size wide), or from logits
-        without one; with `uniforms` (one random number per frame) each frame's token is drawn, else the argmax.
+        """pk_ctc_decode: decode() from encoder frames through `head` (an Mx4Linear or Fp8Linear, vocab_size wide), or
+        from logits without one; with `uniforms` (one random number per frame) each frame's token is drawn, else the argmax.
         frames / uniforms: float32 arrays, or device pointers (int) with their flag."""
         if head is not None and not head.h.value:
             raise ValueError("the head is closed")
@@ -436,9 +443,10 @@ class CtcGreedy:
                 up = _p(uniforms)
             top_k = max(0, min(int(top_k), self.vocab_size))
             draw = abi.pk_ctc_draw(temperature, top_k, top_p, min_p, up, 1 if uniforms_on_device else 0, 0)
-        _check(lib().pk_ctc_decode(self._h, head.h if head is not None else None, fp, 1 if on_device else 0, _p(foff),
-                                   _p(n_frames), B, C.byref(draw) if draw is not None else None, _p(prev), _p(toks), cap,
-                                   _p(toff), _p(frs) if with_frames else None, C.byref(need)), "pk_ctc_decode")
+        fn = "pk_ctc_decode_fp8" if isinstance(head, Fp8Linear) else "pk_ctc_decode"
+        _check(getattr(lib(), fn)(self._h, head.h if head is not None else None, fp, 1 if on_device else 0, _p(foff),
+                                  _p(n_frames), B, C.byref(draw) if draw is not None else None, _p(prev), _p(toks), cap,
+                                  _p(toff), _p(frs) if with_frames else None, C.byref(need)), fn)
         out = [toks[toff[b]:toff[b + 1]].copy() for b in range(B)]
         fo = [frs[toff[b]:toff[b + 1]].copy() for b in range(B)] if with_frames else None
         return out, fo, prev
@@ -508,8 +516,25 @@ def mx4_dequantize(codes: int, scales: int, rows: int, cols: int, out: int, dtyp
                                    cols if row_stride is None else row_stride, stream), "pk_mx4_dequantize")
 
 
-class Mx4Linear:
-    """A linear layer [n][k] held in MXFP4 on one device (pk_mx4)."""
+def fp8_quantize(x: int, rows: int, cols: int, codes: int, scales: int, dtype: str = "f32",
+                 row_stride: Optional[int] = None, device: int = 0, stream: int = 0) -> None:
+    """pk_fp8_quantize on device pointers: rows of `dtype` ("f32", "f16", "bf16") to e4m3 codes
+    [rows][16 * ceil(cols / 16)] and scales [rows][ceil(cols / 128)]. Queued on `stream`."""
+    _check(lib().pk_fp8_quantize(device, x, _DTYPE[dtype], rows, cols, cols if row_stride is None else row_stride,
+                                 codes, scales, stream), "pk_fp8_quantize")
+
+
+def fp8_dequantize(codes: int, scales: int, rows: int, cols: int, out: int, dtype: str = "f32",
+                   row_stride: Optional[int] = None, device: int = 0, stream: int = 0) -> None:
+    """pk_fp8_dequantize on device pointers: the values of codes and scales. Queued on `stream`."""
+    _check(lib().pk_fp8_dequantize(device, codes, scales, rows, cols, out, _DTYPE[dtype],
+                                   cols if row_stride is None else row_stride, stream), "pk_fp8_dequantize")
+
+
+class _Linear:
+    """A linear layer [n][k] held in few bits on one device; `_kind` begins its entry points' names."""
+
+    _kind = ""
 
     def __init__(self, weight, n: Optional[int] = None, k: Optional[int] = None, bias=None, dtype: str = "f32",
                  on_device: bool = False, device: int = 0):
@@ -532,13 +557,21 @@ class Mx4Linear:
                     raise ValueError(f"bias has {bias.size} entries for {n} outputs")
             bp = _p(bias)
         h = C.c_void_p()
-        _check(lib().pk_mx4_create(device, C.byref(t), 1 if on_device else 0, bp, C.byref(h)), "pk_mx4_create")
+        self._call("create", device, C.byref(t), 1 if on_device else 0, bp, C.byref(h))
         self.h = h
         self.n, self.k, self.device = int(n), int(k), device
+        self._linear = self._fn("linear")
+
+    @classmethod
+    def _fn(cls, what):
+        return getattr(lib(), cls._kind + "_" + what)
+
+    def _call(self, what, *args):
+        _check(self._fn(what)(*args), self._kind + "_" + what)
 
     def close(self):
         if getattr(self, "h", None) is not None and self.h.value:
-            lib().pk_mx4_destroy(self.h)
+            self._fn("destroy")(self.h)
             self.h = C.c_void_p()
 
     def __del__(self):
@@ -548,25 +581,38 @@ class Mx4Linear:
             pass
 
     def set_option(self, option: int, value: int) -> None:
-        """pk_mx4_set_option: PK_OPT_TIMEOUT_US or PK_OPT_TEST_STALL of this layer."""
-        _check(lib().pk_mx4_set_option(self.h, option, value), "pk_mx4_set_option")
+        """PK_OPT_TIMEOUT_US or PK_OPT_TEST_STALL of this layer (see pk_mx4_set_option)."""
+        self._call("set_option", self.h, option, value)
 
     def timeouts(self) -> int:
         """How often a forward() was found to have run into its waits' bound: a result that was computed, and
         waited for, between two equal answers is good (see pk_mx4_timeouts)."""
-        return int(lib().pk_mx4_timeouts(self.h))
+        return int(self._fn("timeouts")(self.h))
 
     def workspace(self, rows: int) -> int:
         """Bytes of device workspace that forward() needs for `rows` rows."""
-        return int(lib().pk_mx4_workspace(self.h, rows))
+        return int(self._fn("workspace")(self.h, rows))
 
     def forward(self, x: int, rows: int, y: int, x_dtype: str = "f32", y_dtype: str = "f32",
                 x_stride: Optional[int] = None, y_stride: Optional[int] = None, workspace: int = 0,
                 workspace_bytes: int = 0, stream: int = 0) -> None:
-        """pk_mx4_linear on device pointers: y = q(x) W^T + bias. Queued on `stream`."""
-        _check(lib().pk_mx4_linear(self.h, x, _DTYPE[x_dtype], rows, self.k if x_stride is None else x_stride, y,
-                                   _DTYPE[y_dtype], self.n if y_stride is None else y_stride, workspace, workspace_bytes,
-                                   stream), "pk_mx4_linear")
+        """y = q(x) W^T + bias on device pointers (see pk_mx4_linear). Queued on `stream`."""
+        _check(self._linear(self.h, x, _DTYPE[x_dtype], rows, self.k if x_stride is None else x_stride, y,
+                            _DTYPE[y_dtype], self.n if y_stride is None else y_stride, workspace, workspace_bytes,
+                            stream), self._kind + "_linear")
+
+
+class Mx4Linear(_Linear):
+    """A linear layer [n][k] held in MXFP4 on one device (pk_mx4)."""
+
+    _kind = "pk_mx4"
+
+
+class Fp8Linear(_Linear):
+    """A linear layer [n][k] held in 8-bit floating point with scales of 128 x 128 (pk_fp8); the GGUF tensors that it
+    takes are F32, F16, BF16 and Q8_0."""
+
+    _kind = "pk_fp8"
 
 
 def sample(logits: int, rows: int, vocab: int, uniforms: int, tokens: int, dtype: str = "f32",

@@ -109,6 +109,8 @@ EXPORTED_SYMBOLS = [
     "pk_mx4_quantize", "pk_mx4_dequantize", "pk_mx4_create", "pk_mx4_destroy", "pk_mx4_workspace",
     "pk_mx4_set_option", "pk_mx4_timeouts",
     "pk_mx4_linear", "pk_sample", "pk_ctc_decode",
+    "pk_fp8_quantize", "pk_fp8_dequantize", "pk_fp8_create", "pk_fp8_destroy", "pk_fp8_workspace",
+    "pk_fp8_set_option", "pk_fp8_timeouts", "pk_fp8_linear", "pk_ctc_decode_fp8",
 ]
 
 

@@ -285,6 +285,10 @@ void mx4_dims(const pk_mx4 * w, int * device, int * N, int * K);
 // error word (null: to the layer's).
 pk_status mx4_linear(pk_mx4 * w, const char * fn, const void * x, int32_t x_type, int64_t rows, int64_t x_stride, void * y,
                      int32_t y_type, int64_t y_stride, void * workspace, int64_t workspace_bytes, void * stream, int * err_dev);
+// pk_fp8.cu: the same of a layer in 8 bits.
+void fp8_dims(const pk_fp8 * w, int * device, int * N, int * K);
+pk_status fp8_linear(pk_fp8 * w, const char * fn, const void * x, int32_t x_type, int64_t rows, int64_t x_stride, void * y,
+                     int32_t y_type, int64_t y_stride, void * workspace, int64_t workspace_bytes, void * stream, int * err_dev);
 // Error words: host memory that the devices see. A device sets one, the host asks and clears it.
 int * take_error_word(cudaError_t & e);
 void give_error_word(int * w);

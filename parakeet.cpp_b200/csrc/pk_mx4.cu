@@ -9,25 +9,16 @@
 // x / 2^(B - 127) is an exact f32 product with 2^(127 - B) and the code its nearest value, ties
 // to the even code.
 
-#include "pk_ops.cuh"
-#include "pk_umma.cuh"
+#include "pk_product.cuh"
+#include "pk_rows.cuh"
 
 #include <algorithm>
 #include <mutex>
 #include <new>
-#include <utility>
 #include <vector>
 
 namespace pk {
-
-cudaError_t encode_2d(void * map, CUtensorMapDataType type, size_t esize, const void * base, long long rows, long long cols,
-                      int box_rows, int box_cols, CUtensorMapSwizzle swz);   // pk_encproj.cu
-cudaError_t encode_2d_strided(void * map, CUtensorMapDataType type, const void * base, long long rows, long long cols,
-                              long long stride, int box_rows, int box_cols, CUtensorMapSwizzle swz);
-
 namespace {
-
-constexpr int kQThreads = 256;
 
 // Scales in the layout of the product: 128-row atoms of 4 blocks (K = 128) each, 512 bytes; row r,
 // block b at byte (r % 32) * 16 + (r / 32) * 4 + b: 32 rows of four words, a word = the four
@@ -54,152 +45,6 @@ __device__ __forceinline__ unsigned cvt_e2m1x2(float lo, float hi) {
     unsigned r;
     asm("{ .reg .b8 t; cvt.rn.satfinite.e2m1x2.f32 t, %1, %2; cvt.u32.u8 %0, t; }" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
-}
-
-// Eight consecutive elements of a row, as loaded.
-template <class T> struct alignas(16) Eight { T e[8]; };
-
-// The four values from column c of a row on, zeros for what is not in the row. 16-byte aligned.
-__device__ __forceinline__ void four_of(const float * __restrict__ row, int c, int K, unsigned * w) {
-    if (c >= 0 && c + 4 <= K) {
-        const uint4 q = __ldg(reinterpret_cast<const uint4 *>(row + c));
-        w[0] = q.x;
-        w[1] = q.y;
-        w[2] = q.z;
-        w[3] = q.w;
-        return;
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = 0;
-    if (c >= K) return;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        if (c + i < 0 || c + i >= K) continue;
-        w[i] = __float_as_uint(__ldg(row + c + i));
-    }
-}
-
-// Words from byte `off` (below 16, whole elements) of N + 4 words on, N of them, to the front.
-template <int N, int ES>
-__device__ __forceinline__ void shift_words(unsigned * w, int off) {
-#pragma unroll
-    for (int i = 0; i < N + 2; ++i) w[i] = off & 8 ? w[i + 2] : w[i];
-#pragma unroll
-    for (int i = 0; i < N + 1; ++i) w[i] = off & 4 ? w[i + 1] : w[i];
-    if constexpr (ES == 2) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], (off & 2) * 8);
-    }
-}
-
-// Eight elements of a row from column c (a multiple of eight) on, zeros from column K on. VEC: rows are
-// 16-byte aligned. Otherwise f32 loads the aligned 16 bytes around and shifts them into place (66043 x 1000:
-// 62 us, element by element 74); half precision goes by elements, whose second to eighth load hits the first
-// one's lines (49 us; the other way 66, for the row ends' sake).
-template <class T, bool VEC>
-__device__ __forceinline__ Eight<T> load8(const T * __restrict__ row, int c, int K) {
-    Eight<T> v;
-    if constexpr (!VEC && sizeof(T) == 4) {
-        const int off = (int) (reinterpret_cast<uintptr_t>(row) & 15), at = c - off / 4;
-        unsigned w[12];
-        four_of(row, at, K, w);
-        four_of(row, at + 4, K, w + 4);
-        four_of(row, at + 8, off ? K : 0, w + 8);
-        shift_words<8, 4>(w, off);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v.e[i] = __uint_as_float(w[i]);
-    } else if (VEC && c + 8 <= K) {
-#pragma unroll
-        for (int i = 0; i < (int) sizeof(T) / 2; ++i)
-            reinterpret_cast<uint4 *>(v.e)[i] = __ldcs(reinterpret_cast<const uint4 *>(row + c) + i);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v.e[i] = from_f32<T>(0.0f);
-        if (c < K) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (c + i < K) v.e[i] = row[c + i];
-        }
-    }
-    return v;
-}
-
-// The other way: a group of `lanes` neighbouring lanes, this one the sub-th, has eight elements each from
-// column c on; what lies before column K is stored. The whole warp calls. `on`: this lane's row is there.
-// Not VEC: each lane stores the aligned 16 bytes that its neighbour's elements begin, what the ends of a row
-// or of the warp's piece of it cut by elements (66043 x 1000 bf16: 67 us, by elements throughout 175).
-template <class T, bool VEC>
-__device__ __forceinline__ void store8(T * __restrict__ row, int c, int K, const Eight<T> & o, int sub, int lanes, bool on) {
-    if constexpr (VEC) {
-        if (!on) return;
-        if (c + 8 <= K) {
-#pragma unroll
-            for (int i = 0; i < (int) sizeof(T) / 2; ++i) reinterpret_cast<uint4 *>(row + c)[i] = reinterpret_cast<const uint4 *>(o.e)[i];
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (c + i < K) row[c + i] = o.e[i];
-        }
-    } else {
-        constexpr int ES = (int) sizeof(T), N = 2 * ES, PER = 16 / ES;
-        const unsigned * own = reinterpret_cast<const unsigned *>(o.e);
-        const int off = (int) (reinterpret_cast<uintptr_t>(row) & 15), bytes = K * ES;
-        unsigned w[N + 4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = __shfl_up_sync(0xFFFFFFFFu, own[N - 4 + i], 1);
-#pragma unroll
-        for (int i = 0; i < N; ++i) w[4 + i] = own[i];
-        if (!on) return;
-        shift_words<N, ES>(w, (16 - off) & 15);
-        char * at = reinterpret_cast<char *>(row);
-        const int from = sub == 0 ? c * ES : 0;          // what lies before is another warp's
-#pragma unroll
-        for (int i = 0; i < N; i += 4) {
-            if (off == 0) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) w[i + j] = own[i + j];
-            }
-            const int b = c * ES - off + 4 * i;
-            if (b >= from && b + 16 <= bytes) {
-                *reinterpret_cast<uint4 *>(at + b) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
-            } else if (b < bytes) {
-#pragma unroll
-                for (int j = 0; j < PER; ++j) {
-                    const int e = b + j * ES;
-                    if (e < from || e >= bytes) continue;
-                    if constexpr (ES == 4) *reinterpret_cast<unsigned *>(at + e) = w[i + j];
-                    else *reinterpret_cast<unsigned short *>(at + e) = (unsigned short) (w[i + (j >> 1)] >> (16 * (j & 1)));
-                }
-            }
-        }
-        if (sub == lanes - 1) {                          // the end of the last lane's elements has no lane behind it
-#pragma unroll
-            for (int j = 1; j < 8; ++j)
-                if ((8 - j) * ES <= off && c + j < K) row[c + j] = o.e[j];
-        }
-    }
-}
-
-// Largest magnitude of three; a NaN if one is.
-__device__ __forceinline__ float max3_abs(float a, float b, float c) {
-    float m;
-    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(fabsf(a)), "f"(fabsf(b)), "f"(fabsf(c)));
-    return m;
-}
-
-// Bits of the largest magnitude (as f32; Inf < NaN as integers, in each type).
-__device__ __forceinline__ unsigned amax_bits(const Eight<float> & v) {
-    const float m = max3_abs(max3_abs(v.e[0], v.e[1], v.e[2]), max3_abs(v.e[3], v.e[4], v.e[5]), max3_abs(v.e[6], v.e[7], 0.0f));
-    return __float_as_uint(m);
-}
-// In half precision two at a time; the larger of the two halves is taken once four lanes have theirs.
-template <class T2> __device__ __forceinline__ T2 pair_of(unsigned w) { return *reinterpret_cast<const T2 *>(&w); }
-template <class T2> __device__ __forceinline__ unsigned word_of(T2 p) { return *reinterpret_cast<const unsigned *>(&p); }
-template <class T2, class T>
-__device__ __forceinline__ T2 amax_pair(const Eight<T> & v) {
-    const unsigned * w = reinterpret_cast<const unsigned *>(v.e);
-    return __hmax2_nan(__hmax2_nan(__habs2(pair_of<T2>(w[0])), __habs2(pair_of<T2>(w[1]))),
-                       __hmax2_nan(__habs2(pair_of<T2>(w[2])), __habs2(pair_of<T2>(w[3]))));
 }
 
 // Eight codes and their block's scale byte; four neighbouring lanes hold a block.
@@ -465,16 +310,6 @@ __global__ void __launch_bounds__(kQThreads) mx4_repack_kernel(const unsigned ch
 // tensor memory and issues its four products, warps from 4 on empty the accumulator, of which there are
 // two, so that a tile's epilogue runs under the next tile's products. Each stage has tensor-memory
 // columns of its own for its scales: they are free when the stage is.
-constexpr long long kWaitNs = 2000000000LL;             // bound on every device-side wait, unless a layer sets another
-
-// Of a product's waits: their bound, where to tell that one ran out, and (a test's) that the first block, or a
-// pair's second, loads nothing, so that its waits run out.
-struct Waits {
-    long long ns;
-    int * err;
-    int stall;
-};
-
 constexpr int kTM = 128;
 template <bool BOX> constexpr int tc_stages() { return BOX ? 5 : 4; }
 // Warps of the epilogue, for each 32 rows two where TMA stores y and four where the warps do (layers replayed
@@ -490,12 +325,6 @@ struct TcSmem {
     unsigned tmem;
     int err;
 };
-
-// The wait of a whole warp, of one mind about its outcome.
-template <bool CLUSTER = false>
-__device__ __forceinline__ bool warp_wait(unsigned long long * b, unsigned parity, long long ns, int * err) {
-    return __all_sync(0xFFFFFFFFu, mbar_wait<CLUSTER>(b, parity, ns, err));
-}
 
 // The four products of a stage of 256 values and the copies of their scales (columns ca: 8 for x, then
 // NA per chunk for the weights), by one elected lane. The whole warp runs the loop around it, so that
@@ -523,14 +352,6 @@ template <int BN> constexpr unsigned tc_stage_bytes() { return kTM * 128u + BN *
 constexpr unsigned kOutBytes = 4096;                    // an epilogue warp's 32 staged rows of 128 bytes
 template <int BN, bool BOX> constexpr size_t tc_smem_bytes() {
     return 1024 + (size_t) tc_stages<BOX>() * tc_stage_bytes<BN>() + epi_warps<BOX>() * kOutBytes + sizeof(TcSmem);
-}
-
-// Wait with a bound and nothing else to end it: for copies in flight before an early exit.
-__device__ __forceinline__ void mbar_drain(unsigned long long * b, unsigned parity) {
-    unsigned long long t0, now;
-    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t0));
-    now = t0;
-    while (!mbar_test(b, parity) && (long long) (now - t0) <= kWaitNs) asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
 }
 
 // A warp's 32 rows of an accumulator to y, 128 bytes of them in every STEP (the `half`-th), through shared
@@ -747,16 +568,6 @@ struct PairSmem {
 };
 template <int BN, bool BOX> constexpr size_t pair_smem() {
     return 1024 + (size_t) kPStages * pair_stage<BN>() + epi_warps<BOX>() * kOutBytes + sizeof(PairSmem);
-}
-
-__device__ __forceinline__ void put_at(unsigned * p, unsigned rank, unsigned v) {   // to the same place of block `rank`
-    asm volatile("{ .reg .b32 a; mapa.shared::cluster.u32 a, %0, %1; st.shared::cluster.u32 [a], %2; }"
-                 :: "r"(smem_u32(p)), "r"(rank), "r"(v) : "memory");
-}
-
-__device__ __forceinline__ void cluster_meet() {
-    __syncwarp();
-    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 template <class T, int BN, bool BOX>
@@ -1047,16 +858,6 @@ mx4_few_kernel(const TX * __restrict__ x, long long ldx, int M, int K, const __g
     if (threadIdx.x == 0 && S.err != 0) atomicExch_system(w.err, 1);
 }
 
-// Lanes of a row, as a power of two.
-inline int row_lanes(long long K) { return K <= 32 ? 2 : K <= 64 ? 3 : K <= 128 ? 4 : 5; }
-
-// Launch of a row kernel: a warp for 32 lanes' rows, up to a few waves; with few rows a warp for each 256 values.
-inline dim3 row_blocks(long long rows, long long K) {
-    const long long per = (kQThreads / 32) << (5 - row_lanes(K)), x = std::min<long long>((rows + per - 1) / per, 148LL * 32);
-    const long long segs = (K + 255) / 256;
-    return dim3((unsigned) x, (unsigned) std::max<long long>(1, std::min<long long>(segs, 148 * 8 / x)));
-}
-
 template <bool ATOMS>
 cudaError_t launch_quantize(const void * x, int type, long long rows, int K, long long ldx, unsigned char * codes,
                             unsigned char * scales, cudaStream_t s) {
@@ -1114,18 +915,12 @@ bool take_error(int * w) { return __atomic_exchange_n(w, 0, __ATOMIC_ACQ_REL) !=
 
 }  // namespace pk
 
-struct pk_mx4 {
+struct pk_mx4 : pk::LayerWaits {
     int device = 0;
     int N = 0, K = 0, nb = 0, chunks = 0;
     unsigned char * codes = nullptr;    // [N][16 nb]; owns the memory of all three
     unsigned char * scales = nullptr;   // atoms
     float * bias = nullptr;             // padded to whole tiles, or null
-    int * err = nullptr;                // host memory that the device sees: a wait of a pk_mx4_linear ran out
-    int * err_dev = nullptr;
-    long long timeouts = 0;             // times that it was found so
-    int unreported = 0;                 // and no pk_mx4_linear has said so yet
-    long long wait_ns = pk::kWaitNs;
-    int stall = 0;                      // the next product's, see Waits
     alignas(64) CUtensorMap map[3];     // codes in boxes of kBox[i] rows
     alignas(64) CUtensorMap smap[2];    // scales: the two atoms of a stage of 128 rows, of 256 rows
 };
@@ -1152,14 +947,6 @@ bool map_y(CUtensorMap * map, void * y, int type, long long M, int N, long long 
     return true;
 }
 
-// Raises a kernel's limit of shared memory, once per device (`set`: the devices done).
-template <class F> cudaError_t allow_smem(F kernel, size_t bytes, int device, unsigned long long & set) {
-    if (__atomic_load_n(&set, __ATOMIC_RELAXED) >> device & 1) return cudaSuccess;
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) bytes);
-    if (e == cudaSuccess) __atomic_fetch_or(&set, 1ull << device, __ATOMIC_RELAXED);
-    return e;
-}
-
 struct Call {
     const pk_mx4 * w;
     Waits waits;
@@ -1169,22 +956,6 @@ struct Call {
     long long ldy;
     cudaStream_t s;
 };
-
-// Launch of a product behind the quantisation of its rows, which lets it start before it has ended.
-template <class... P, class... A>
-cudaError_t launch_after(void (*kernel)(P...), unsigned grid, unsigned threads, size_t smem, cudaStream_t s, A &&... args) {
-    cudaLaunchConfig_t cfg{};
-    cudaLaunchAttribute at[1];
-    cfg.gridDim = dim3(grid);
-    cfg.blockDim = dim3(threads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = s;
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, std::forward<A>(args)...);
-}
 
 template <class T, int BN, bool BOX>
 cudaError_t launch_tc_as(const Call & c, const CUtensorMap & amap, const unsigned char * xs, const CUtensorMap & wmap, const CUtensorMap & ymap) {
@@ -1414,27 +1185,10 @@ extern "C" PK_API pk_status pk_mx4_create(int device, const pk_tensor * weight, 
 
 extern "C" PK_API pk_status pk_mx4_set_option(pk_mx4 * w, int32_t option, int64_t value) {
     const char * fn = "pk_mx4_set_option";
-    if (!w) return op_fail(PK_ERR_INVALID, fn, "null layer");
-    switch (option) {
-        case PK_OPT_TIMEOUT_US:
-            if (value <= 0 || value > INT64_MAX / 1000) return op_fail(PK_ERR_INVALID, fn, "timeout must be > 0");
-            __atomic_store_n(&w->wait_ns, (long long) value * 1000, __ATOMIC_RELAXED);
-            return PK_OK;
-        case PK_OPT_TEST_STALL:
-            __atomic_store_n(&w->stall, value != 0 ? 1 : 0, __ATOMIC_RELAXED);
-            return PK_OK;
-        default:
-            return op_fail(PK_ERR_INVALID, fn, "a layer has PK_OPT_TIMEOUT_US and PK_OPT_TEST_STALL");
-    }
+    return w ? set_wait_option(*w, fn, option, value) : op_fail(PK_ERR_INVALID, fn, "null layer");
 }
 
 namespace {
-
-void notice_timeout(pk_mx4 * w) {
-    if (!take_error(w->err)) return;
-    __atomic_fetch_add(&w->timeouts, 1, __ATOMIC_ACQ_REL);
-    __atomic_store_n(&w->unreported, 1, __ATOMIC_RELEASE);
-}
 
 size_t ws_codes(const pk_mx4 * w, int64_t rows) { return ((size_t) rows * w->nb * 16 + 255) / 256 * 256; }
 
@@ -1464,7 +1218,7 @@ pk_status pk::mx4_linear(pk_mx4 * w, const char * fn, const void * x, int32_t x_
     if (workspace_bytes < need)
         return op_fail(PK_ERR_INVALID, fn, "workspace_bytes is below pk_mx4_workspace(w, rows)");
     if (!err_dev) {
-        notice_timeout(w);
+        notice_timeout(*w);
         if (__atomic_exchange_n(&w->unreported, 0, __ATOMIC_ACQ_REL))
             return op_fail(PK_ERR_TIMEOUT, fn, "a device-side wait of an earlier call ran out; this call did not run");
         err_dev = w->err_dev;
@@ -1497,6 +1251,6 @@ extern "C" PK_API pk_status pk_mx4_linear(pk_mx4 * w, const void * x, int32_t x_
 
 extern "C" PK_API int64_t pk_mx4_timeouts(pk_mx4 * w) {
     if (!w) return -1;
-    notice_timeout(w);
+    notice_timeout(*w);
     return __atomic_load_n(&w->timeouts, __ATOMIC_ACQUIRE);
 }

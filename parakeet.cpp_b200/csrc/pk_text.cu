@@ -390,21 +390,31 @@ std::vector<Stretch> stretches(const int64_t * offset, const int32_t * n, int32_
     return out;
 }
 
+// The layer that makes logits of frames: in 4 bits, in 8 bits, or none.
+struct Head {
+    pk_mx4 * mx4 = nullptr;
+    pk_fp8 * fp8 = nullptr;
+    explicit operator bool() const { return mx4 || fp8; }
+    void dims(int * device, int * N, int * K) const { mx4 ? pk::mx4_dims(mx4, device, N, K) : pk::fp8_dims(fp8, device, N, K); }
+    int64_t workspace(int64_t rows) const { return mx4 ? pk_mx4_workspace(mx4, rows) : pk_fp8_workspace(fp8, rows); }
+    template <class... A> pk_status linear(A... args) const { return mx4 ? pk::mx4_linear(mx4, args...) : pk::fp8_linear(fp8, args...); }
+};
+
 // Logits of `frames` frames (`dx` itself, or head * dx, `step` frames a product) to their tokens in c->best from
 // row `at` on: the argmax or a draw.
-pk_status ctc_frame_tokens(pk_ctc * c, const char * fn, pk_mx4 * head, const float * dx, int64_t frames, int64_t step, int64_t at,
+pk_status ctc_frame_tokens(pk_ctc * c, const char * fn, const Head & head, const float * dx, int64_t frames, int64_t step, int64_t at,
                            const pk_ctc_draw * draw, const float * duni) {
     using namespace pk;
     cudaStream_t s = c->stream;
     int K = c->V;
-    if (head) mx4_dims(head, nullptr, nullptr, &K);
+    if (head) head.dims(nullptr, nullptr, &K);
     for (int64_t f = 0; f < frames; f += step) {
         const int64_t n = std::min(step, frames - f);
         const float * logits = dx + f * (int64_t) K;
         int * best = c->best.as<int>() + at + f;
         if (head) {
-            const pk_status st = mx4_linear(head, fn, logits, PK_GGML_F32, n, K, c->logits.p, PK_GGML_F32, c->V, c->work.p,
-                                            (int64_t) c->work.cap, s, c->err_dev);
+            const pk_status st = head.linear(fn, logits, PK_GGML_F32, n, (int64_t) K, c->logits.p, PK_GGML_F32, (int64_t) c->V, c->work.p,
+                                             (int64_t) c->work.cap, s, c->err_dev);
             if (st != PK_OK) return st;
             logits = c->logits.as<float>();
         }
@@ -434,7 +444,7 @@ pk_status ctc_frame_tokens(pk_ctc * c, const char * fn, pk_mx4 * head, const flo
 
 // pk_ctc_greedy and pk_ctc_decode: frames -> tokens -> collapse -> host arrays. `logits` are logits,
 // or, with a head, its input frames.
-pk_status ctc_run(pk_ctc * c, const char * fn, pk_mx4 * head, const float * logits, int32_t logits_on_device,
+pk_status ctc_run(pk_ctc * c, const char * fn, const Head & head, const float * logits, int32_t logits_on_device,
                      const int64_t * frame_offsets, const int32_t * n_frames, int32_t B, const pk_ctc_draw * draw,
                      int32_t * prev_inout, int32_t * tokens, int64_t tokens_cap, int64_t * token_offsets, int32_t * first_frame,
                      int64_t * tokens_needed) {
@@ -453,7 +463,7 @@ pk_status ctc_run(pk_ctc * c, const char * fn, pk_mx4 * head, const float * logi
         return PK_OK;
     }
     int width = c->V;
-    if (head) mx4_dims(head, nullptr, nullptr, &width);
+    if (head) head.dims(nullptr, nullptr, &width);
     std::vector<int64_t> roff((size_t) B), row((size_t) B);   // each utterance's output region (its frame count), first frame
     int64_t rtotal = 0;
     for (int b = 0; b < B; ++b) {
@@ -508,7 +518,7 @@ pk_status ctc_run(pk_ctc * c, const char * fn, pk_mx4 * head, const float * logi
     for (const Stretch & p : parts) step = std::max(step, p.end - p.begin);
     if (head) {
         step = std::min({step, kHeadFrames, std::max<int64_t>(kHeadLogits / c->V, 1)});
-        const int64_t ws = pk_mx4_workspace(head, step);
+        const int64_t ws = head.workspace(step);
         TX_STEP(c->logits.ensure((size_t) step * c->V * 4), fn, "alloc");
         TX_STEP(c->work.ensure((size_t) std::max<int64_t>(ws, 1)), fn, "alloc");
         if (!c->err) {
@@ -586,25 +596,50 @@ extern "C" PK_API pk_status pk_ctc_greedy(pk_ctc * c, const float * logits, int3
                                           const int64_t * frame_offsets, const int32_t * n_frames, int32_t B,
                                           int32_t * prev_inout, int32_t * tokens, int64_t tokens_cap,
                                           int64_t * token_offsets, int32_t * first_frame, int64_t * tokens_needed) {
-    return ctc_decode(c, "pk_ctc_greedy", nullptr, logits, logits_on_device, frame_offsets, n_frames, B, nullptr, prev_inout, tokens,
+    return ctc_decode(c, "pk_ctc_greedy", Head{}, logits, logits_on_device, frame_offsets, n_frames, B, nullptr, prev_inout, tokens,
                       tokens_cap, token_offsets, first_frame, tokens_needed);
 }
+
+namespace {
+
+pk_status ctc_decode_head(pk_ctc * c, const char * fn, const Head & head, const float * frames, int32_t frames_on_device,
+                          const int64_t * frame_offsets, const int32_t * n_frames, int32_t B, const pk_ctc_draw * draw,
+                          int32_t * prev_inout, int32_t * tokens, int64_t tokens_cap, int64_t * token_offsets, int32_t * first_frame,
+                          int64_t * tokens_needed) {
+    using namespace pk;
+    char msg[160];
+    if (c && head) {
+        int device = 0, N = 0;
+        head.dims(&device, &N, nullptr);
+        if (device != c->device || N != c->V) {
+            std::snprintf(msg, sizeof(msg), "%s: the head must be on the handle's device and vocab_size wide", fn);
+            return set_error(PK_ERR_INVALID, msg);
+        }
+    }
+    if (c && c->V > PK_SAMPLE_MAX_VOCAB && draw) {
+        std::snprintf(msg, sizeof(msg), "%s: vocab_size is above PK_SAMPLE_MAX_VOCAB", fn);
+        return set_error(PK_ERR_INVALID, msg);
+    }
+    return ctc_decode(c, fn, head, frames, frames_on_device, frame_offsets, n_frames, B, draw, prev_inout, tokens, tokens_cap,
+                      token_offsets, first_frame, tokens_needed);
+}
+
+}  // namespace
 
 extern "C" PK_API pk_status pk_ctc_decode(pk_ctc * c, pk_mx4 * head, const float * frames, int32_t frames_on_device,
                                           const int64_t * frame_offsets, const int32_t * n_frames, int32_t B,
                                           const pk_ctc_draw * draw, int32_t * prev_inout, int32_t * tokens, int64_t tokens_cap,
                                           int64_t * token_offsets, int32_t * first_frame, int64_t * tokens_needed) {
-    using namespace pk;
-    if (c && head) {
-        int device = 0, N = 0;
-        mx4_dims(head, &device, &N, nullptr);
-        if (device != c->device || N != c->V)
-            return set_error(PK_ERR_INVALID, "pk_ctc_decode: the head must be on the handle's device and vocab_size wide");
-    }
-    if (c && c->V > PK_SAMPLE_MAX_VOCAB && draw)
-        return set_error(PK_ERR_INVALID, "pk_ctc_decode: vocab_size is above PK_SAMPLE_MAX_VOCAB");
-    return ctc_decode(c, "pk_ctc_decode", head, frames, frames_on_device, frame_offsets, n_frames, B, draw, prev_inout, tokens,
-                      tokens_cap, token_offsets, first_frame, tokens_needed);
+    return ctc_decode_head(c, "pk_ctc_decode", Head{head, nullptr}, frames, frames_on_device, frame_offsets, n_frames, B, draw,
+                           prev_inout, tokens, tokens_cap, token_offsets, first_frame, tokens_needed);
+}
+
+extern "C" PK_API pk_status pk_ctc_decode_fp8(pk_ctc * c, pk_fp8 * head, const float * frames, int32_t frames_on_device,
+                                              const int64_t * frame_offsets, const int32_t * n_frames, int32_t B,
+                                              const pk_ctc_draw * draw, int32_t * prev_inout, int32_t * tokens, int64_t tokens_cap,
+                                              int64_t * token_offsets, int32_t * first_frame, int64_t * tokens_needed) {
+    return ctc_decode_head(c, "pk_ctc_decode_fp8", Head{nullptr, head}, frames, frames_on_device, frame_offsets, n_frames, B, draw,
+                           prev_inout, tokens, tokens_cap, token_offsets, first_frame, tokens_needed);
 }
 
 extern "C" PK_API pk_status pk_vocab_create(int device, const uint8_t * piece_bytes, const int64_t * piece_offsets,

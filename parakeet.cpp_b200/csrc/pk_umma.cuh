@@ -1,6 +1,6 @@
 // pk_umma.cuh -- sm_100a building blocks shared by libparakeet_cuda's tensor-memory
 // kernels (pk_encproj.cu: the enc-proj GEMM; pk_bulk.cu: the step loop for large
-// live batches; pk_mx4.cu: the 4-bit product): mbarrier waits bounded in time, tcgen05.mma operand descriptors
+// live batches; pk_mx4.cu, pk_fp8.cu: the 4-bit and 8-bit products): mbarrier waits bounded in time, tcgen05.mma operand descriptors
 // for 128-byte-swizzled K-major f16 tiles, the kind::f16 instruction descriptor,
 // MMA issue / commit and 2-D TMA tile loads.
 #pragma once
@@ -126,6 +126,31 @@ __device__ __forceinline__ void umma_mxf4(unsigned tmem_d, unsigned long long ad
                      :: "r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate) : "memory");
 }
 
+// kind::mxf8f6f4 instruction descriptor: f32 accumulator, e4m3 A and B, both K-major, e8m0 scales; `id` (0 to 3)
+// names the byte of each row's 4-byte scale word that a K = 32 product reads.
+__host__ __device__ constexpr unsigned umma_idesc_mxf8(int m, int n, int id) {
+    return ((unsigned) id << 4)               // B scale id
+         | (0u << 7) | (0u << 10)             // A, B format e4m3
+         | ((unsigned) (n >> 3) << 17)        // N / 8
+         | (1u << 23)                         // e8m0 scales
+         | ((unsigned) (m >> 7) << 27)        // M / 128
+         | ((unsigned) id << 29);             // A scale id
+}
+
+// One block-scaled product of 32 values of K (32 bytes of each operand row); scales and PAIR as above.
+template <bool PAIR>
+__device__ __forceinline__ void umma_mxf8(unsigned tmem_d, unsigned long long adesc, unsigned long long bdesc, unsigned idesc,
+                                          unsigned sfa, unsigned sfb, unsigned accumulate) {
+    if (PAIR)
+        asm volatile("{ .reg .pred p; setp.ne.b32 p, %6, 0;\n"
+                     "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p; }"
+                     :: "r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate) : "memory");
+    else
+        asm volatile("{ .reg .pred p; setp.ne.b32 p, %6, 0;\n"
+                     "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p; }"
+                     :: "r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate) : "memory");
+}
+
 // 512 bytes of scale words (32 rows of 16 bytes) from shared memory to four tensor-memory columns,
 // the same for each of the four lane quarters. Ordered before products that the same thread issues.
 template <bool PAIR>
@@ -192,6 +217,14 @@ __device__ __forceinline__ void mbar_expect(unsigned long long * b, unsigned byt
 // Counts `bytes` as arrived on the barrier's phase, in place of a copy that was expected and never issued.
 __device__ __forceinline__ void mbar_complete(unsigned long long * b, unsigned bytes) {
     asm volatile("mbarrier.complete_tx.relaxed.cta.shared::cta.b64 [%0], %1;" :: "r"(smem_u32(b)), "r"(bytes) : "memory");
+}
+
+// 16 columns of this warp's 32 tensor-memory lanes (issue only; tcgen05.wait::ld before use).
+__device__ __forceinline__ void tmem_load16(unsigned taddr, unsigned * v) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+                   "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+                 : "r"(taddr));
 }
 
 // 32 columns of this warp's 32 tensor-memory lanes (issue only; tcgen05.wait::ld before use).
