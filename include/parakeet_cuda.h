@@ -625,6 +625,67 @@ typedef struct pk_sample_args {
  * as for pk_mx4_quantize above. Needs no workspace. */
 PK_API pk_status pk_sample(int device, const pk_sample_args * args, void * stream);
 
+/* ---- verification of drafted tokens ---------------------------------------------
+ *
+ * No counterpart in the reference. A cheap model (the draft) proposed tokens one after the
+ * other; the target's logits of all their positions, and of the one behind, came from one
+ * pass. Position j of a sequence has two distributions: p_j, by which pk_sample would draw
+ * from the target's row j with the sequence's settings, and q_j, the same of the draft's
+ * row. With u_j of the caller's random numbers:
+ *
+ *   draft d_j is accepted   when u_j q_j(d_j) < p_j(d_j) and all before it are
+ *   at the first that is not a token is drawn from max(p_j - q_j, 0), or from p_j where that is
+ *                           zero throughout
+ *   past the last draft      a token is drawn from p_n (n: the number of drafts)
+ *
+ * and every drawn token by the sequence's last random number, as pk_sample draws: the lowest
+ * index at which the running sum exceeds u times the total. If the drafts were drawn from q,
+ * the tokens are distributed as if drawn from p one after the other.
+ *
+ * draft_logits = NULL: the drafts were not drawn (looked up, or the draft's argmax): q_j is 1
+ * for d_j, so it is accepted when u_j < p_j(d_j), and the token drawn in its place is another.
+ * A draft outside [0, vocab) has no probability and is rejected (pk_sample's -1 among them).
+ * T <= 0 or NaN: p_j is 1 for the first of the largest logits. A target's row without any
+ * logit above -infinity accepts nothing and gives token -1. u is clamped to [0, 1), NaN to 0.
+ * Weights count as in pk_sample, which tells the same token from a row as a call here without
+ * drafts; differences p - q below 2^-43 of the larger may be lost. */
+#define PK_VERIFY_MAX_DRAFTS 65535
+
+typedef struct pk_verify_args {
+    const void *    logits;       /* target: [sequences][max_drafts + 1] rows of logits_type, row_stride apart */
+    const void *    draft_logits; /* draft: [sequences][max_drafts] rows of logits_type, draft_stride apart, or NULL */
+    int32_t         logits_type;  /* PK_GGML_F32, PK_GGML_F16 or PK_GGML_BF16 */
+    int32_t         vocab;        /* 1 .. PK_SAMPLE_MAX_VOCAB */
+    int64_t         sequences;    /* sequences * (2 * max_drafts + 1) below 2^28 */
+    int32_t         max_drafts;   /* 0 .. PK_VERIFY_MAX_DRAFTS */
+    int32_t         reserved;     /* 0 */
+    int64_t         row_stride;   /* elements, >= vocab */
+    int64_t         draft_stride; /* the same; not read without draft_logits */
+    const int32_t * drafts;       /* [sequences][max_drafts] */
+    const int32_t * n_drafts;     /* [sequences], clamped to [0, max_drafts], or NULL: max_drafts each; rows behind are not read */
+    const float *   uniforms;     /* [sequences][max_drafts + 1] random numbers in [0, 1) */
+    int32_t *       tokens;       /* [sequences][max_drafts + 1]: accepted drafts, the drawn token, then -1 */
+    int32_t *       accepted;     /* [sequences]: number of drafts accepted */
+    float *         logprobs;     /* [sequences][max_drafts + 1] or NULL: of each token under p; -infinity for -1 */
+    /* settings of every sequence, or, where the array is not NULL, of each by itself */
+    float           temperature;
+    int32_t         top_k;
+    float           top_p;
+    float           min_p;
+    const float *   temperatures; /* [sequences] or NULL */
+    const int32_t * top_ks;       /* [sequences] or NULL */
+    const float *   top_ps;       /* [sequences] or NULL */
+    const float *   min_ps;       /* [sequences] or NULL */
+    void *          workspace;    /* pk_verify_workspace() bytes, 8-byte aligned, for this call alone until it has run */
+    int64_t         workspace_bytes;
+} pk_verify_args;
+
+/* Bytes of device workspace for these sizes; -1 for sizes that are refused. */
+PK_API int64_t   pk_verify_workspace(int64_t sequences, int32_t max_drafts, int32_t vocab);
+/* Every pointer is a device pointer on `device`; stream, waiting, alignment, strides and overlap
+ * as for pk_mx4_quantize above. */
+PK_API pk_status pk_verify(int device, const pk_verify_args * args, void * stream);
+
 /* ---- CTC decode from encoder frames, greedy or drawn ---------------------------- */
 
 /* Settings of a drawn CTC path (see pk_sample); one random number per frame. */

@@ -80,6 +80,7 @@ def lib():
             "pk_fp8_timeouts": ([P], I64),
             "pk_fp8_linear": ([P, P, I32, I64, I64, P, I32, I64, P, I64, P], I32),
             "pk_sample": ([I32, P, P], I32),
+            "pk_verify_workspace": ([I64, I32, I32], I64), "pk_verify": ([I32, P, P], I32),
             "pk_ctc_decode": ([P, P, P, I32, P, P, I32, P, P, P, I64, P, P, P], I32),
             "pk_ctc_decode_fp8": ([P, P, P, I32, P, P, I32, P, P, P, I64, P, P, P], I32),
         }
@@ -628,3 +629,29 @@ def sample(logits: int, rows: int, vocab: int, uniforms: int, tokens: int, dtype
     a = abi.pk_sample_args(logits, _DTYPE[dtype], vocab, rows, vocab if row_stride is None else row_stride, uniforms,
                            tokens, logprobs, temperature, top_k, top_p, min_p, temperatures, top_ks, top_ps, min_ps)
     _check(lib().pk_sample(device, C.byref(a), stream), "pk_sample")
+
+
+def verify_workspace(sequences: int, max_drafts: int, vocab: int) -> int:
+    """Bytes of device workspace that verify() needs for these sizes."""
+    return int(lib().pk_verify_workspace(sequences, max_drafts, vocab))
+
+
+def verify(logits: int, sequences: int, max_drafts: int, vocab: int, drafts: int, uniforms: int, tokens: int, accepted: int,
+           draft_logits: int = 0, n_drafts: int = 0, dtype: str = "f32", row_stride: Optional[int] = None,
+           draft_stride: Optional[int] = None, logprobs: int = 0, temperature: float = 1.0, top_k: int = 0, top_p: float = 1.0,
+           min_p: float = 0.0, temperatures: int = 0, top_ks: int = 0, top_ps: int = 0, min_ps: int = 0, workspace: int = 0,
+           workspace_bytes: int = 0, device: int = 0, stream: int = 0) -> None:
+    """pk_verify on device pointers: the drafts of each sequence that the target accepts and the token behind them, by the
+    sequence's random numbers. logits: the target's rows [sequences][max_drafts + 1]; draft_logits: the rows
+    [sequences][max_drafts] that the drafts were drawn from (0: they were not drawn). Settings as for sample(), by
+    sequence. Queued on `stream`."""
+    if not 0 < vocab <= abi.PK_SAMPLE_MAX_VOCAB:
+        raise ValueError(f"vocab {vocab} is not in [1, {abi.PK_SAMPLE_MAX_VOCAB}]")
+    if not 0 <= max_drafts <= abi.PK_VERIFY_MAX_DRAFTS:
+        raise ValueError(f"max_drafts {max_drafts} is not in [0, {abi.PK_VERIFY_MAX_DRAFTS}]")
+    top_k = max(0, min(int(top_k), vocab))
+    a = abi.pk_verify_args(logits, draft_logits, _DTYPE[dtype], vocab, sequences, max_drafts, 0,
+                           vocab if row_stride is None else row_stride, vocab if draft_stride is None else draft_stride,
+                           drafts, n_drafts, uniforms, tokens, accepted, logprobs, temperature, top_k, top_p, min_p,
+                           temperatures, top_ks, top_ps, min_ps, workspace, workspace_bytes)
+    _check(lib().pk_verify(device, C.byref(a), stream), "pk_verify")

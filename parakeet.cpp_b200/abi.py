@@ -13,6 +13,7 @@ PK_OPT_TIMEOUT_US, PK_OPT_MATH, PK_OPT_MAX_SYMBOLS, PK_OPT_TEST_STALL, PK_OPT_BU
 PK_OPT_BULK_SCREEN, PK_OPT_BULK_I8, PK_OPT_BULK_TMA_A = 6, 7, 8
 PK_GGML_F32, PK_GGML_F16, PK_GGML_Q8_0, PK_GGML_BF16, PK_GGML_MXFP4 = 0, 1, 8, 30, 39
 PK_SAMPLE_MAX_VOCAB = 524288
+PK_VERIFY_MAX_DRAFTS = 65535
 PK_MATH_F32, PK_MATH_TC, PK_MATH_Q8 = 0, 1, 2
 
 STATUS_NAMES = {0: "PK_OK", 1: "PK_ERR_DMODEL", 2: "PK_ERR_INVALID", 3: "PK_ERR_MODEL",
@@ -93,6 +94,16 @@ class pk_sample_args(C.Structure):
                 ("temperatures", C.c_void_p), ("top_ks", C.c_void_p), ("top_ps", C.c_void_p), ("min_ps", C.c_void_p)]
 
 
+class pk_verify_args(C.Structure):
+    _fields_ = [("logits", C.c_void_p), ("draft_logits", C.c_void_p), ("logits_type", C.c_int32), ("vocab", C.c_int32),
+                ("sequences", C.c_int64), ("max_drafts", C.c_int32), ("reserved", C.c_int32), ("row_stride", C.c_int64),
+                ("draft_stride", C.c_int64), ("drafts", C.c_void_p), ("n_drafts", C.c_void_p), ("uniforms", C.c_void_p),
+                ("tokens", C.c_void_p), ("accepted", C.c_void_p), ("logprobs", C.c_void_p),
+                ("temperature", C.c_float), ("top_k", C.c_int32), ("top_p", C.c_float), ("min_p", C.c_float),
+                ("temperatures", C.c_void_p), ("top_ks", C.c_void_p), ("top_ps", C.c_void_p), ("min_ps", C.c_void_p),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64)]
+
+
 class pk_ctc_draw(C.Structure):
     _fields_ = [("temperature", C.c_float), ("top_k", C.c_int32), ("top_p", C.c_float), ("min_p", C.c_float),
                 ("uniforms", C.c_void_p), ("uniforms_on_device", C.c_int32), ("reserved", C.c_int32)]
@@ -111,6 +122,7 @@ EXPORTED_SYMBOLS = [
     "pk_mx4_linear", "pk_sample", "pk_ctc_decode",
     "pk_fp8_quantize", "pk_fp8_dequantize", "pk_fp8_create", "pk_fp8_destroy", "pk_fp8_workspace",
     "pk_fp8_set_option", "pk_fp8_timeouts", "pk_fp8_linear", "pk_ctc_decode_fp8",
+    "pk_verify_workspace", "pk_verify",
 ]
 
 
