@@ -676,11 +676,12 @@ typedef struct pk_verify_args {
     const int32_t * top_ks;       /* [sequences] or NULL */
     const float *   top_ps;       /* [sequences] or NULL */
     const float *   min_ps;       /* [sequences] or NULL */
-    void *          workspace;    /* pk_verify_workspace() bytes, 8-byte aligned, for this call alone until it has run */
+    void *          workspace;    /* pk_verify_workspace() bytes (0: may be NULL), 8-byte aligned, for this call alone until it has run */
     int64_t         workspace_bytes;
 } pk_verify_args;
 
-/* Bytes of device workspace for these sizes; -1 for sizes that are refused. */
+/* Bytes of device workspace for these sizes, 0 where none is needed (vocabularies of up to some
+ * 22,000); -1 for sizes that are refused. */
 PK_API int64_t   pk_verify_workspace(int64_t sequences, int32_t max_drafts, int32_t vocab);
 /* Every pointer is a device pointer on `device`; stream, waiting, alignment, strides and overlap
  * as for pk_mx4_quantize above. */

@@ -125,18 +125,24 @@ struct TeamBins {
     u64 w[kList];
 };
 
-// The threads of one row. CL: several blocks of a cluster, each with a slice of the row.
-template <int NT, bool CL>
+// The threads of one row. CL: several blocks of a cluster, each with a slice of the row. NM: one of several teams of a
+// block, which meet at barriers of their own.
+template <int NT, bool CL, bool NM = false>
 struct Team {
     int tid, rank, blocks;
     unsigned phase;
     TeamSmem<NT> * s;
     double mine;                             // this lane's entry of the exponential's table
     unsigned level = 0;                      // levels of bins so far
+    int bar = 0;                             // its barrier
 
+    // This block's threads by themselves.
+    __device__ __forceinline__ Team<NT, false, NM> alone() const { return Team<NT, false, NM>{tid, 0, 1, 0, s, 0.0, 0, bar}; }
     __device__ __forceinline__ int lane() const { return tid & 31; }
     __device__ __forceinline__ void sync() const {
-        if (NT == 32) __syncwarp(); else __syncthreads();
+        if (NT == 32) __syncwarp();
+        else if (NM) asm volatile("barrier.sync %0, %1;" :: "r"(bar), "n"(NT) : "memory");
+        else __syncthreads();
     }
     // Every block's slot written before it is complete, what was read before it may be overwritten.
     __device__ __forceinline__ void meet() const { cg::this_cluster().sync(); }
@@ -362,8 +368,8 @@ struct Share {
 // Bins the level's range and finds the bin in which the running sum over falling logits (from L.above
 // on) reaches `need` >= 1: of counts, or (WEIGHTS) of weights. With `share`, need is worked out from
 // it first. False: the range does not hold that much; L.with is then what it and its tail hold.
-template <bool WEIGHTS, class T, int NT, bool CL, bool RES>
-__device__ bool find_bin(Team<NT, CL> & team, TeamBins<NT> * B, const Slice<T, RES> & l, const Row & row, Level & L, u64 & need,
+template <bool WEIGHTS, class T, int NT, bool CL, bool RES, bool NM>
+__device__ bool find_bin(Team<NT, CL, NM> & team, TeamBins<NT> * B, const Slice<T, RES> & l, const Row & row, Level & L, u64 & need,
                          const Share * share) {
     constexpr int NB = bins_of<NT>(), PER = NB / NT;
     TeamSmem<NT> * s = team.s;
@@ -418,7 +424,7 @@ __device__ bool find_bin(Team<NT, CL> & team, TeamBins<NT> * B, const Slice<T, R
         sum += w;
     }
     u64 total;
-    Team<NT, false> block{team.tid, 0, 1, 0, s, 0.0};            // the bins are the cluster's already
+    auto block = team.alone();            // the bins are the cluster's already
     u64 before = L.above + block.scan(sum, total);
     total += L.above + rest;
     if (WEIGHTS && share) need = max((u64) ceil(share->p * (double) (total + share->lump)), 1ull);
@@ -447,8 +453,8 @@ __device__ bool find_bin(Team<NT, CL> & team, TeamBins<NT> * B, const Slice<T, R
 // Puts the slice's elements that `want` names on the list, and joins the lists of a cluster's blocks.
 // The number of them; past kList the list is not complete and not to be used. RANGE: also their largest
 // and smallest value; with `few` false nothing is listed, as there are more than kList.
-template <bool RANGE, class T, int NT, bool CL, bool RES, class F>
-__device__ int gather(Team<NT, CL> & team, TeamBins<NT> * B, const Slice<T, RES> & l, int s0, const Pair *& list, F want, bool few,
+template <bool RANGE, class T, int NT, bool CL, bool RES, bool NM, class F>
+__device__ int gather(Team<NT, CL, NM> & team, TeamBins<NT> * B, const Slice<T, RES> & l, int s0, const Pair *& list, F want, bool few,
                       float & hi, float & lo) {
     TeamSmem<NT> * s = team.s;
     if (RANGE) {
@@ -562,8 +568,8 @@ __device__ __forceinline__ void weigh_list(int tid, TeamBins<NT> * B, const Pair
 
 // The cut inside the bin that find_bin found: everything above the returned logit is kept, and
 // `ties` of those equal to it, which may be all (`partial` false).
-template <bool WEIGHTS, class T, int NT, bool CL, bool RES>
-__device__ float find_cut(Team<NT, CL> & team, TeamBins<NT> * B, const Slice<T, RES> & l, const Row & row, Level L, u64 need,
+template <bool WEIGHTS, class T, int NT, bool CL, bool RES, bool NM>
+__device__ float find_cut(Team<NT, CL, NM> & team, TeamBins<NT> * B, const Slice<T, RES> & l, const Row & row, Level L, u64 need,
                           u64 & ties, bool & partial) {
     constexpr int NB = bins_of<NT>();
     TeamSmem<NT> * s = team.s;
@@ -649,9 +655,9 @@ enum { kNothing = 0, kCut = 1, kDrawn = 2 };
 constexpr double kOff = 70.0 * 0x1p-24;
 constexpr double kFix = 1099511627776.0;        // 2^40
 
-template <class T, int NT>
-__device__ int nucleus_cut(Team<NT, false> & team, TeamBins<NT> * B, const Slice<T, true> & l, float hi, float low, float temp,
-                           float p, int vocab, float & cut, u64 & ties, bool & partial) {
+template <class T, int NT, bool NM>
+__device__ int nucleus_cut(Team<NT, false, NM> & team, TeamBins<NT> * B, const Slice<T, true> & l, float hi, float low, float temp,
+                           float p, int vocab, float & cut, u64 & ties, bool & partial, double & kept) {
     constexpr int NB = bins_of<NT>(), PER = NB / NT;
     TeamSmem<NT> * s = team.s;
     const Row32 r(hi, temp);
@@ -762,6 +768,7 @@ __device__ int nucleus_cut(Team<NT, false> & team, TeamBins<NT> * B, const Slice
                     s->cut = B->list[j].v;
                     s->cut_ties = t;
                     s->cut_partial = t * w < x.same;
+                    s->found_sum = over + t * w;
                     s->found = kCut;
                 }
             }
@@ -769,6 +776,7 @@ __device__ int nucleus_cut(Team<NT, false> & team, TeamBins<NT> * B, const Slice
     team.sync();
     const int state = s->found;
     if (state == kCut) {
+        kept = (double) s->found_sum * (1.0 / kFix);
         cut = s->cut;
         ties = s->cut_ties;
         partial = s->cut_partial != 0;
@@ -784,9 +792,10 @@ template <int NT, bool CL, bool RES> constexpr bool nucleus_fits() { return RES 
 // have weight; min-p raises it) that are above `cut`, or equal to it and among the first `ties` (`partial`: which are
 // not all). True where the answer was had on the way: from `listed`, called with a list of all tokens that may be kept
 // (of the first so many of them those before which less than `need` lies, or, where that is 0, the share of their
-// weight), or from `sure`, which is asked once the cut is known without f64 sums. `s0`: index of the slice's first.
-template <class T, int NT, bool CL, bool RES, class Listed, class Sure>
-__device__ bool cut_row(Team<NT, CL> & team, TeamBins<NT> * bins, const Slice<T, RES> & l, int s0, const Row & r, float hi, float lo, float temp_f,
+// weight), or from `sure`, which is asked once the cut is known without f64 sums, and told the weight from the cut on
+// as f32 sums have it. `s0`: index of the slice's first.
+template <class T, int NT, bool CL, bool RES, bool NM, class Listed, class Sure>
+__device__ bool cut_row(Team<NT, CL, NM> & team, TeamBins<NT> * bins, const Slice<T, RES> & l, int s0, const Row & r, float hi, float lo, float temp_f,
                         int vocab, int k, float p, float m, float & least, float & cut, u64 & ties, bool & partial, Listed listed, Sure sure) {
     const double temp = (double) temp_f;
     constexpr int NB = bins_of<NT>();
@@ -817,8 +826,9 @@ __device__ bool cut_row(Team<NT, CL> & team, TeamBins<NT> * bins, const Slice<T,
     // (64 rows of 8193, each with its own settings: 16 us against 19).
     if constexpr (nucleus_fits<NT, CL, RES>()) {
         if (!(p >= 1.0f) && !(cut > -CUDART_INF_F) && vocab <= 64 * NT) {
-            known = nucleus_cut<T, NT>(team, bins, l, hi, low, temp_f, p, vocab, cut, ties, partial);
-            if (known == kCut && !partial && sure()) return true;
+            double kept = 0.0;
+            known = nucleus_cut<T, NT>(team, bins, l, hi, low, temp_f, p, vocab, cut, ties, partial, kept);
+            if (known == kCut && !partial && sure(kept)) return true;
         }
     }
     if (!(p >= 1.0f) && known == kNothing) {

@@ -60,7 +60,7 @@ __device__ void draw_listed(Team<NT, CL> & team, TeamBins<NT> * B, const Pair * 
             rank[q] = a;
             if (a.n < k) sum += B->w[j];
         });
-    Team<NT, false> block{team.tid, 0, 1, 0, team.s, 0.0};
+    auto block = team.alone();
     if (need == 0) {
         sum = block.sum(sum);
         need = p >= 1.0f ? ~0ull : max((u64) ceil(p > 0.0f ? (double) p * (double) sum : 0.0), 1ull);
@@ -294,7 +294,7 @@ sample_kernel(pk_sample_args a, int slice, int teams, int row_floats) {
             [&](const Pair * list, int n, int first, float share, u64 need) {
                 draw_listed<NT, CL>(team, bins, list, n, a, row, r, hi, inv_t, first, share, need, least);
             },
-            [&] {
+            [&](double) {
                 if constexpr (nucleus_fits<NT, CL, RES>())
                     return nucleus_draw<T, NT>(team, l, len, hi, temp_f, least, cut, a.uniforms[row], a, row) == kDrawn;
                 return false;

@@ -5,56 +5,653 @@
 // the sequence's settings. A draft d is accepted when u q(d) < p(d). At the first that is not, the token is drawn
 // from max(p - q, 0), and behind the last draft from p.
 //
-// Two kernels. The first takes a team of threads per row, as pk_sample does, and leaves of each row what the
-// second needs: its largest logit, its cut, the sum of its weights and the draft's weight. The second takes a block
-// (or cluster) per sequence: it tests all drafts at once and draws from the one row, or two, that the first
-// rejection names, reading them again. Weights are pk_sample's integers, so sums are exact whatever their order;
-// the weights of the tested tokens alone are f64 exponentials that nothing cuts off.
+// Vocabularies whose two rows fit a block's shared memory take one kernel: a block (a warp for short rows) goes over
+// a sequence's positions and stops at the first rejection, whose rows it then holds; what lies behind is never read.
+// With few sequences the blocks of a cluster share the positions out and tell each other the outcomes. The two rows
+// of a position go to two teams of threads. What a test needs of a row is its largest logit, its cut, the sum of its
+// weights and the draft's weight: the sum by f32 with a proven bound, by pk_sample's whole numbers where that cannot
+// tell. Draws always go by whole numbers, so that sums are exact whatever their order.
+//
+// Longer rows take two kernels, see below.
 
 #include "pk_draw.cuh"
 
 namespace pk {
 namespace {
 
-// What the draw needs of a row.
+// What the test and the draw need of a row.
 struct RowStat {
     double drafted;       // weight of the draft, relative to the largest; 0 if it is cut
-    u64 total;            // of the weights kept; 0: no logit above -infinity
+    u64 total;            // of the weights kept, times 2^43; 0: no logit above -infinity
     float hi;             // largest logit (0 where it is +infinity)
-    float from, cut;      // kept: at least `from`, and above `cut` or equal to it up to index `last`
+    float from, cut;      // kept: at least `from`, which is not below `cut`, and above `cut` or up to index `last`
     int last;
     int flags;
 };
-enum { kInf = 1, kGreedy = 2 };   // the largest is +infinity; the first of the largest alone is kept
-
-struct Plan {
-    pk_verify_args a;
-    RowStat * stats;      // [sequences][max_drafts + 1] of the target, [sequences][max_drafts] of the draft
-};
+// The largest is +infinity; the first of the largest alone is kept; the total is off by kOff of itself at most.
+enum { kInf = 1, kGreedy = 2, kNear = 4 };
+constexpr int kAny = 0x7FFFFFFF;
 
 __device__ __forceinline__ int drafts_of(const pk_verify_args & a, long long seq) {
     return a.n_drafts ? max(0, min(a.n_drafts[seq], a.max_drafts)) : a.max_drafts;
 }
 __device__ __forceinline__ float temperature_of(const pk_verify_args & a, long long seq) { return a.temperatures ? a.temperatures[seq] : a.temperature; }
+__device__ __forceinline__ float number_of(float u) { return u > 0.0f ? fminf(u, 0x1.fffffep-1f) : 0.0f; }
 
 // A logit as a row's statistics see it.
 __device__ __forceinline__ float seen(float v, int flags) {
     return flags & kInf ? (v == CUDART_INF_F ? 0.0f : -CUDART_INF_F) : v;
 }
 
+// A row's weights, times 2^43 and whole: weight_warp's, as its numbers are needed there.
+__device__ __forceinline__ Row row_of(float hi, double temp) {
+    Row r;
+    r.top = (double) hi;
+    r.c = 46.166241308446828384 * (1.0 / temp);                  // 32 log2(e) / T, as pk_sample has it
+    // below 2^-44 of the largest, see pk_sample.cu
+    r.base = fmaxf(__double2float_ru(r.top - 31.0 * temp), -3.402823466e+38f);
+    return r;
+}
+
+// Weight of a draft with logit v: what min-p asks for and the cut it is subject to, not `base`.
+__device__ __forceinline__ double draft_weight(float v, int draft, const RowStat & st, const Row & r, double temp, float m) {
+    const float floor = fmaxf(!(m > 0.0f) ? -CUDART_INF_F : m >= 1.0f ? st.hi : __double2float_ru(r.top + temp * log((double) m)), -3.402823466e+38f);
+    if (!(v >= floor && (v > st.cut || (v == st.cut && draft <= st.last)))) return 0.0;
+    // pk_sample's weight as it is before it is rounded, to 2^-42 of itself
+    if (v >= r.base) return weight_onto(v, r, 0.0, [](int n) { return table_entry(n & 31); }) * (1.0 / kOne);
+    return exp(((double) v - r.top) / temp);
+}
+
+// A team's list holds all that may be kept, of the first `first` those before which less than `need` lies (0: the share
+// of their weight), of these those from `least` on: the sum of what is kept, and the last of it in the order, told by the
+// thread that has it to f(logit, index, sum).
+template <int NT, bool CL, bool NM, class F>
+__device__ void keep_listed(Team<NT, CL, NM> & team, TeamBins<NT> * bins, const Pair * list, int count, const Row & r, int first, float share, u64 need,
+                            float least, F f) {
+    weigh_list<NT>(team.tid, bins, list, count, r, false);
+    team.sync();
+    constexpr int SH = sharers<NT>(), PER = (kList * SH + NT - 1) / NT;
+    Rank rank[PER];
+    u64 sum = 0;
+#pragma unroll
+    for (int q = 0; q < PER; ++q) rank[q].n = kList;
+    over_list<NT, Rank>(team.tid, count,
+        [&](Rank & b, int j, int i) {
+            const Pair me = list[j], o = list[i];
+            if (i < count && (o.v > me.v || (o.v == me.v && o.i < me.i))) { b.w += bins->w[i]; ++b.n; }
+        },
+        [&](int j, const Rank & b, int q) {
+            rank[q] = b;
+            if (b.n < first) sum += bins->w[j];
+        });
+    auto block = team.alone();
+    if (need == 0) {
+        sum = block.sum(sum);
+        need = share >= 1.0f ? ~0ull : max((u64) ceil(share > 0.0f ? (double) share * (double) sum : 0.0), 1ull);
+    }
+    // the weights stay below 2^51 in all, their number below 2^8: one sum
+    u64 kept = 0;
+#pragma unroll
+    for (int q = 0; q < PER; ++q) {
+        const int j = (team.tid + q * NT) / SH;
+        if (j < count && team.tid % SH == 0 && rank[q].n < first && rank[q].w < need && list[j].v >= least) kept += bins->w[j] + (1ull << 52);
+    }
+    kept = block.sum(kept);
+    const int all = (int) (kept >> 52);
+#pragma unroll
+    for (int q = 0; q < PER; ++q) {
+        const int j = (team.tid + q * NT) / SH;
+        if (j < count && team.tid % SH == 0 && rank[q].n == all - 1) f(list[j].v, list[j].i, kept & ((1ull << 52) - 1));
+    }
+}
+
+constexpr double kShare = 1125899906842624.0;           // 2^50: probabilities as integers, whose sums f64 holds
+constexpr double kMagic = 6755399441055744.0;           // 1.5 * 2^52: what is added to it is rounded to an integer
+constexpr double kFine = 68719476736.0;                 // 2^36: f32 sums as integers
+
+// What f32's weights of a row, all 2^-off of what they should be, are to be multiplied by: |off| is below 2^-4 (k is
+// below 10^6 and rounded once), where four terms tell 2^off to 2^-28.
+__device__ __forceinline__ double scale_of(const Row32 & f, float hi) {
+    const double x = 0.6931471805599453 * ((double) f.k - (double) hi * (double) f.c);
+    return 1.0 + x * (1.0 + x * (0.5 + x * (1.0 / 6.0 + x * (1.0 / 24.0))));
+}
+
+// Log-probability of the token with logit v: log() of a number below 2^16 in f32 is off by a unit, 2^-20, at most.
+__device__ __forceinline__ float logprob_of(float v, const RowStat & p, double heat) {
+    return (float) ((v == p.hi ? 0.0 : ((double) v - (double) p.hi) / heat) - (double) logf((float) ((double) p.total * (1.0 / kOne))));
+}
+
+// The sum of a resident row's weights that are kept. A thread's are at most 176 (45,000 logits over 256 threads), below
+// 2^51 in all, so its sum is whole.
+template <class T, int NT, bool NM>
+__device__ u64 exact_sum(Team<NT, false, NM> & team, const Slice<T, true> & l, const Row & r, float from, float cut, int last) {
+    double onto = kZero;
+    l.template quads<NT>(team.tid, [&](float4 v, int i) {
+        bool keep[4] = {v.x >= from, v.y >= from, v.z >= from, v.w >= from};
+        if (last != kAny) {
+            keep[0] = keep[0] && (v.x > cut || i <= last);
+            keep[1] = keep[1] && (v.y > cut || i + 1 <= last);
+            keep[2] = keep[2] && (v.z > cut || i + 2 <= last);
+            keep[3] = keep[3] && (v.w > cut || i + 3 <= last);
+        }
+        if (!__any_sync(kFull, keep[0] || keep[1] || keep[2] || keep[3])) return;
+        const float x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const double w = weight_warp(x[q], r, team.mine, onto);
+            if (keep[q]) onto = w;
+        }
+    });
+    return team.sum(whole(onto));
+}
+
+// Statistics of a resident row into `st` (shared memory), by its team; complete once the team has met.
+template <class T, int NT, bool FILTERS, bool NM>
+__device__ void row_stat(Team<NT, false, NM> & team, TeamBins<NT> * bins, Slice<T, true> l, const pk_verify_args & a, long long seq, int draft,
+                         RowStat * st) {
+    const float temp_f = temperature_of(a, seq);
+    const double temp = (double) temp_f;
+    float hi = -CUDART_INF_F, lo = CUDART_INF_F;                 // fmaxf and fminf pass over NaN
+    l.template each<NT>(team.tid, [&](float v, int) {
+        hi = fmaxf(hi, v);
+        if (FILTERS && v > -CUDART_INF_F) lo = fminf(lo, v);
+    });
+    team.template range<FILTERS>(hi, lo);
+    const bool one = team.tid == 0;
+    const int flags = hi == CUDART_INF_F ? kInf : 0;
+    if (hi == -CUDART_INF_F || !(temp_f > 0.0f)) {
+        // nothing to draw, or the first index of the largest
+        u64 first = ~0ull;
+        if (hi > -CUDART_INF_F)
+            for (int i = team.tid; i < l.n && first == ~0ull; i += NT)
+                if (l(i) == hi) first = (u64) i;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) first = min(first, __shfl_xor_sync(kFull, first, o));
+        if (NT > 32) {
+            team.sync();
+            if (team.lane() == 0) team.s->wscan[team.tid >> 5] = first;
+            team.sync();
+#pragma unroll
+            for (int i = 0; i < NT / 32; ++i) first = min(first, team.s->wscan[i]);
+        }
+        if (one) {
+            st->flags = flags | kGreedy;
+            st->hi = st->from = st->cut = flags & kInf ? 0.0f : hi;
+            st->last = (int) min(first, (u64) kAny);
+            st->total = first == ~0ull ? 0ull : (u64) kOne;
+            st->drafted = first != ~0ull && draft == (int) first ? 1.0 : 0.0;
+        }
+    }
+    if (flags & kInf) {                                          // zeros where it is +infinity, nothing elsewhere
+        team.sync();
+        for (int i = team.tid; i < l.n; i += NT) l.sm[l.skew + i] = seen(l.sm[l.skew + i], kInf);
+        team.sync();
+        hi = lo = 0.0f;
+    }
+    if (hi == -CUDART_INF_F || !(temp_f > 0.0f)) return;
+    const Row r = row_of(hi, temp);
+    float least = r.base;                                        // kept: >= least, and what the cut says
+    float cut = -CUDART_INF_F;
+    u64 ties = ~0ull;
+    bool partial = false;
+    const float m = a.min_ps ? a.min_ps[seq] : a.min_p;
+    auto leave = [&](float from, float cut_at, int last, u64 sum, int more) {
+        st->flags = flags | more;
+        st->hi = hi;
+        st->from = from;
+        st->cut = cut_at;
+        st->last = last;
+        st->total = sum;
+        st->drafted = draft >= 0 && draft < l.n ? draft_weight(l(draft), draft, *st, r, temp, m) : 0.0;
+    };
+    if constexpr (FILTERS) {
+        const float p = a.top_ps ? a.top_ps[seq] : a.top_p;
+        const int k = a.top_ks ? a.top_ks[seq] : a.top_k;
+        const bool done = cut_row<T, NT, false, true>(team, bins, l, 0, r, hi, lo, temp_f, a.vocab, k, p, m, least, cut, ties, partial,
+            [&](const Pair * list, int count, int first, float share, u64 need) {
+                keep_listed(team, bins, list, count, r, first, share, need, least,
+                            [&](float v, int i, u64 sum) { leave(v, v, i, sum, 0); });
+            },
+            [&](double kept) {
+                if (!(cut >= least)) return false;               // min-p drops more
+                if (one) leave(cut, cut, kAny, (u64) (kept * scale_of(Row32(hi, temp_f), hi) * kOne), kNear);
+                return true;
+            });
+        if (done) return;
+    }
+    const float from = fmaxf(least, cut);
+    int last = kAny;
+    if (FILTERS && partial && cut >= least) {
+        // equal logits at the cut, not all of which are kept, go by index: the last of them that is
+        const int len = run_of<NT>(l.n), i0 = team.tid * len;
+        unsigned equal = 0;
+        for (int j = 0; j < len; ++j) equal += l(i0 + j) == cut ? 1u : 0u;
+        u64 all;
+        const u64 before = team.scan((u64) equal, all);
+        if (one) team.s->found = kAny;
+        team.sync();
+        if (before < ties && ties <= before + equal) {
+            int i = i0;
+            for (u64 left = ties - before;; ++i)
+                if (l(i) == cut && --left == 0) break;
+            team.s->found = i;
+        }
+        team.sync();
+        last = team.s->found;
+    }
+    // The sum by f32, as nucleus_cut takes it: off by kOff of itself at most for up to 64 logits a thread.
+    if (l.n <= 64 * NT && last == kAny) {
+        const Row32 f(hi, temp_f);
+        if (f.fine) {
+            float part[4] = {};
+            l.template quads<NT>(team.tid, [&](float4 v, int) {
+                // a NaN is not kept; nothing of what has no weight counts
+                part[0] += !FILTERS || v.x >= from ? f.weight(v.x) : 0.0f;
+                part[1] += !FILTERS || v.y >= from ? f.weight(v.y) : 0.0f;
+                part[2] += !FILTERS || v.z >= from ? f.weight(v.z) : 0.0f;
+                part[3] += !FILTERS || v.w >= from ? f.weight(v.w) : 0.0f;
+            });
+            const float mine = (part[0] + part[1]) + (part[2] + part[3]);
+            // a thread's at most 68 weights stay below 128, all threads' below 2^52; a NaN gives more than that
+            constexpr u64 kBad = 1ull << 54;
+            static_assert(NT <= 512, "honest sums below kBad, NT times kBad below 2^64");
+            const u64 sum = team.sum(mine < 128.0f ? __double2ull_rn((double) mine * kFine) : kBad);
+            if (sum < kBad) {
+                if (one) leave(from, cut, last, (u64) ((double) sum * scale_of(f, hi) * (kOne / kFine)), kNear);
+                return;
+            }
+        }
+    }
+    const u64 sum = exact_sum<T, NT>(team, l, r, from, cut, last);
+    if (one) leave(from, cut, last, sum, 0);
+}
+
+// The exact sum of a row whose statistics have f32's; complete once the team has met.
+template <class T, int NT, bool NM>
+__device__ void settle(Team<NT, false, NM> & team, const Slice<T, true> & l, double temp, RowStat * st) {
+    if (!(st->flags & kNear)) return;
+    const u64 sum = exact_sum<T, NT>(team, l, row_of(st->hi, temp), st->from, st->cut, st->last);
+    if (team.tid == 0) {
+        st->total = sum;
+        st->flags &= ~kNear;
+    }
+}
+
+enum { kAll, kLess, kWithout };                          // draws: from p, from what p has more than q, from p without the draft
+
+// The draw by f32 weights, where they can tell the token; false where they cannot. The group's threads come together on
+// entry.
+//
+// With w^ off by 2^-24 (8 + 2.78 |x|) of itself and sums by kOff, see pk_sample.cu, a probability p^ = w^ / S^ is
+// off by 2^-24 (8 + 2.78 |x| + 70 + 2) of itself, and over all tokens by 2^-24 (8 + 41 + 72) = 121 2^-24 at most (V <= 22528).
+// max(p - q, 0) is off by no more than both, 242 2^-24 in any sum over tokens; the subtraction, 1 more, and a thread's
+// additions, 19. So sums are off by E = 262 2^-24 (in units of p's sum: 70 2^-24 where q has no part), u times the total by as
+// much, and a token is settled if t is more than 2 E from its borders (2.5 E, against what else is rounded).
+template <class T, int G>
+__device__ bool draw_near(Team<G, false> & group, const Slice<T, true> & pl, const Slice<T, true> & ql, const RowStat * st, int mode, int draft,
+                          float temp, float u, int32_t * token, float * logprob) {
+    const RowStat & p = st[0], & q = st[1];
+    const int len = run_of<G>(pl.n);
+    if (len > 64 || (p.flags & kGreedy) || p.last != kAny || (mode == kLess && ((q.flags & kGreedy) || q.last != kAny))) return false;
+    const Row32 pr(p.hi, temp), qr(mode == kLess ? q.hi : 0.0f, temp);
+    if (!pr.fine || !qr.fine) return false;
+    constexpr double kUnit = 274877906944.0;             // 2^38
+    const float sp = mode == kLess ? (float) (scale_of(pr, p.hi) * kOne / (double) p.total) : 1.0f;
+    const float sq = mode == kLess ? (float) (scale_of(qr, q.hi) * kOne / (double) q.total) : 0.0f;
+    const float p_from = p.from, q_from = q.from;
+    auto weigh = [&](int i) {
+        const float x = pl(i);
+        float w = x >= p_from ? pr.weight(x) : 0.0f;
+        if (mode == kLess) {
+            const float y = ql(i);
+            const float less = y >= q_from ? qr.weight(y) * sq : 0.0f;
+            w = fmaxf(fmaf(w, sp, -less), 0.0f);
+        }
+        if (mode == kWithout && i == draft) w = 0.0f;
+        return w;
+    };
+    const int i0 = group.tid * len;
+    float part[4] = {};
+    int j = 0;
+    for (; j + 4 <= len; j += 4) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) part[k] += weigh(i0 + j + k);
+    }
+    for (; j < len; ++j) part[0] += weigh(i0 + j);
+    const float mine = (part[0] + part[1]) + (part[2] + part[3]);
+    const u64 sum = __double2ull_rn((double) fminf(mine, 128.0f) * kUnit);
+    u64 total;
+    const u64 before = group.scan(sum, total);
+    const double t = (double) number_of(u) * (double) total;
+    const double edge = mode == kLess ? 2.5 * 262.0 * 0x1p-24 * kUnit
+                                      : 2.5 * kOff * ((double) p.total * (1.0 / kOne) / scale_of(pr, p.hi)) * kUnit;
+    if (group.tid == 0) group.s->found = -1;
+    group.sync();
+    if ((double) before <= t && t < (double) (before + sum)) {
+        group.s->found = group.tid;
+        group.s->found_before = before;
+    }
+    group.sync();
+    const int who = group.s->found;
+    group.sync();
+    if (group.tid == 0) group.s->found = 0;
+    group.sync();
+    if (who >= 0 && group.tid < 32) {
+        const int e = min((who + 1) * len, pl.n);
+        u64 run = group.s->found_before;
+        for (int c = who * len; c < e; c += 32) {
+            const int i = c + group.tid;
+            const u64 w = i < e ? __double2ull_rn((double) weigh(i) * kUnit) : 0ull;
+            const u64 upto = run + warp_scan(w, group.tid);
+            if ((double) upto - t > edge && t - (double) (upto - w) > edge) {
+                *token = i;
+                if (logprob) *logprob = logprob_of(pl(i), p, (double) temp);
+                group.s->found = 1;
+            }
+            run = __shfl_sync(kFull, upto, 31);
+            if ((double) run > t) break;
+        }
+    }
+    group.sync();
+    const bool done = group.s->found != 0;
+    group.sync();
+    return done;
+}
+
+template <int NT, bool DUAL> constexpr int group_of() { return DUAL ? 2 * NT : NT; }
+template <int NT, bool DUAL, bool FILTERS> struct SeqSmem {
+    TeamSmem<NT> team[DUAL ? 2 : 1];
+    TeamSmem<group_of<NT, DUAL>()> group;
+    RowStat st[2];
+    int code[2];
+};
+template <int NT, bool DUAL> struct SeqBins { TeamBins<NT> bins[DUAL ? 2 : 1]; };
+constexpr int kSeqGroups = 8;                            // sequences of a block where each has a warp
+
+// DUAL: the target's row and the draft's go to a team of NT threads each, otherwise to one team, one after the other.
+template <class T, int NT, bool DUAL, bool FILTERS>
+__global__ void __launch_bounds__(NT == 32 ? 256 : group_of<NT, DUAL>(), NT == 32 ? 4 : 1024 / group_of<NT, DUAL>())
+verify_sequence_kernel(const pk_verify_args a, int rows_each, int row_floats) {
+    constexpr int G = group_of<NT, DUAL>(), GROUPS = NT == 32 ? kSeqGroups : 1;
+    extern __shared__ __align__(16) unsigned char raw[];
+    const int g = NT == 32 ? (int) threadIdx.x >> 5 : 0;
+    const int blocks = NT == 32 ? 1 : (int) cg::this_cluster().num_blocks(), rank = NT == 32 ? 0 : (int) cg::this_cluster().block_rank();
+    const long long seq = NT == 32 ? (long long) blockIdx.x * GROUPS + g : (long long) (blockIdx.x / blocks);
+    if (NT == 32 && seq >= a.sequences) return;                  // warps by themselves: nothing to meet
+    float * rows_at = reinterpret_cast<float *>(raw) + (size_t) g * rows_each * row_floats;
+    auto * states = reinterpret_cast<SeqSmem<NT, DUAL, FILTERS> *>(reinterpret_cast<float *>(raw) + (size_t) GROUPS * rows_each * row_floats);
+    SeqSmem<NT, DUAL, FILTERS> & S = states[g];
+    SeqBins<NT, DUAL> * B = reinterpret_cast<SeqBins<NT, DUAL> *>(states + GROUPS) + g;
+    Team<G, false> group;
+    group.tid = NT == 32 ? (int) threadIdx.x & 31 : (int) threadIdx.x;
+    group.blocks = 1;
+    group.rank = 0;
+    group.phase = 0;
+    group.s = &S.group;
+    const int own = DUAL ? group.tid / NT : 0;                   // this thread's row
+    Team<NT, false, DUAL> team;
+    team.tid = DUAL ? group.tid % NT : group.tid;
+    team.blocks = 1;
+    team.rank = 0;
+    team.phase = 0;
+    team.s = &S.team[own];
+    team.bar = 1 + own;
+    team.mine = table_entry(team.lane());
+    group.mine = team.mine;
+
+    const int d = a.max_drafts, n = drafts_of(a, seq), v = a.vocab;
+    const int32_t * drafts = a.drafts + seq * d;
+    const float * u = a.uniforms + seq * (d + 1);
+    int32_t * tokens = a.tokens + seq * (d + 1);
+    float * logprobs = a.logprobs ? a.logprobs + seq * (d + 1) : nullptr;
+    const float temp_f = temperature_of(a, seq);
+    const double temp = (double) temp_f;
+    const int g_len = run_of<G>(v), t_len = run_of<NT>(v);
+    Slice<T, true> rows[2];
+    auto slice = [&](int which, int pos) {
+        Slice<T, true> & l = rows[which];
+        l.gl = which == 0 ? static_cast<const T *>(a.logits) + (seq * (d + 1) + pos) * a.row_stride
+                          : static_cast<const T *>(a.draft_logits) + (seq * d + pos) * a.draft_stride;
+        l.n = v;
+        l.sm = rows_at + which * row_floats;
+        l.skew = (int) ((reinterpret_cast<uintptr_t>(l.gl) & 15) / sizeof(T)) & 3;
+        l.inf = false;
+        l.pad = max(((l.skew + v + 3) & ~3) - l.skew, max(NT * t_len, G * g_len));
+    };
+    enum { kAccepted, kRejected, kEnd };
+    for (int base = 0, round = 0;; base += blocks, ++round) {
+        const int pos = base + rank;
+        const bool two = a.draft_logits && pos < n;
+        int code = kAccepted, draft = -1;
+        if (pos <= n) {
+            if (pos < n) draft = drafts[pos];
+            slice(0, pos);
+            if (two) slice(1, pos);
+            if (!DUAL || own == 0 || two) {
+                const int end = DUAL || !two ? 1 : 2;
+                for (int i = 0; i < end; ++i) load_slice<T, NT>(rows[DUAL ? own : i], team.tid);
+                team.sync();
+                for (int i = 0; i < end; ++i) {
+                    const int which = DUAL ? own : i;
+                    row_stat<T, NT, FILTERS>(team, &B->bins[own], rows[which], a, seq, draft, &S.st[which]);
+                    if (end > 1) team.sync();
+                }
+            }
+            group.sync();
+            if (pos == n) {
+                code = kEnd;
+            } else {
+                // u q(d) < p(d), as u w_q(d) P < w_p(d) Q; f32 sums may leave it open
+                const bool inside = draft >= 0 && draft < v;
+                const double x = (double) number_of(u[pos]);
+                auto sides = [&](double & l, double & r) {
+                    const RowStat & p = S.st[0], & q = S.st[1];
+                    l = two ? x * q.drafted * (double) p.total : inside ? x * (double) p.total * (1.0 / kOne) : 0.0;
+                    r = two ? p.drafted * (double) q.total : p.drafted;
+                    // no logit in the draft's row: its tokens have no probability
+                    if (two && q.total == 0) { l = 0.0; r = p.drafted; }
+                    if (p.total == 0) r = 0.0;
+                };
+                double l, r;
+                sides(l, r);
+                const int near = (S.st[0].flags | (two ? S.st[1].flags : 0)) & kNear;
+                if (near && fmax(l, r) > 0.0 && fabs(l - r) <= 5.0 * kOff * fmax(l, r)) {
+                    group.sync();
+                    if (!DUAL || own == 0 || two)
+                        for (int i = 0; i < (DUAL || !two ? 1 : 2); ++i) settle<T, NT>(team, rows[DUAL ? own : i], temp, &S.st[DUAL ? own : i]);
+                    group.sync();
+                    sides(l, r);
+                }
+                code = l < r ? kAccepted : kRejected;
+            }
+        }
+        int first = code != kAccepted ? 0 : -1;                  // of the blocks, the first that did not accept
+        if (NT > 32 && blocks > 1) {
+            if (group.tid == 0) S.code[round & 1] = code;
+            cg::this_cluster().sync();
+            int its = kAccepted;
+            if (group.lane() < blocks) its = *cg::this_cluster().map_shared_rank(&S.code[round & 1], group.lane());
+            const unsigned not_accepted = __ballot_sync(kFull, its != kAccepted);
+            first = not_accepted ? __ffs((int) not_accepted) - 1 : -1;
+        }
+        if (code == kAccepted && pos < n && (first < 0 || rank < first) && group.tid == 0) {
+            tokens[pos] = draft;
+            if (logprobs) logprobs[pos] = logprob_of(rows[0](draft), S.st[0], S.st[0].flags & kGreedy ? 1.0 : temp);
+        }
+        if (first < 0) {
+            group.sync();                                        // the rows' memory is read
+            continue;
+        }
+        // a block's codes stay while others may read them
+        __syncwarp();
+        if (NT > 32 && blocks > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+        if (rank == first) {
+            for (int j = pos + 1 + group.tid; j <= d; j += G) {
+                tokens[j] = -1;
+                if (logprobs) logprobs[j] = -CUDART_INF_F;
+            }
+            if (group.tid == 0) a.accepted[seq] = pos;
+            int mode = kAll;
+            if (code == kRejected) mode = two ? (S.st[1].total ? kLess : kAll) : a.draft_logits ? kAll : kWithout;
+            const double heat = S.st[0].flags & kGreedy ? 1.0 : temp;
+            if (S.st[0].total == 0) {                            // nothing to draw from
+                if (group.tid == 0) {
+                    tokens[pos] = -1;
+                    if (logprobs) logprobs[pos] = -CUDART_INF_F;
+                }
+            } else if (!draw_near<T, G>(group, rows[0], rows[1], S.st, mode, draft, temp_f, u[d], tokens + pos, logprobs ? logprobs + pos : nullptr)) {
+                if (mode == kLess) {
+                    if (!DUAL || own == 0 || two)
+                        for (int i = 0; i < (DUAL ? 1 : 2); ++i) settle<T, NT>(team, rows[DUAL ? own : i], temp, &S.st[DUAL ? own : i]);
+                }
+                if (group.tid == 0) S.group.found = -1;
+                group.sync();
+                const RowStat p = S.st[0], q = S.st[1];
+                const Row pr = row_of(p.hi, heat), qr = row_of(mode == kLess ? q.hi : 0.0f, heat);
+                const double sp = kShare / (double) p.total, sq = mode == kLess ? kShare / (double) q.total : 0.0;
+                // what token i weighs in the draw, a whole number; the whole warp calls
+                const bool p_cut = p.last != kAny, q_cut = q.last != kAny;
+                auto weigh = [&](int i, bool in) -> double {
+                    const float x = in ? rows[0](i) : -CUDART_INF_F;
+                    bool keep = x >= p.from;
+                    if (p_cut) keep = keep && (x > p.cut || i <= p.last);
+                    if (mode == kWithout) keep = keep && i != draft;
+                    if (FILTERS && !__any_sync(kFull, keep)) return 0.0;
+                    double w = weight_warp(x, pr, team.mine) - kZero;
+                    if (mode == kLess) {
+                        const float y = in ? rows[1](i) : -CUDART_INF_F;
+                        bool less = y >= q.from;
+                        if (q_cut) less = less && (y > q.cut || i <= q.last);
+                        const double z = weight_warp(y, qr, team.mine) - kZero;
+                        // the two products rounded alike: equal rows leave nothing
+                        w = __dmul_rn(w, sp) - (less ? __dmul_rn(z, sq) : 0.0);
+                        w = (w + kMagic) - kMagic;
+                        keep = keep && w > 0.0;
+                    }
+                    return keep ? w : 0.0;
+                };
+                const int i0 = group.tid * g_len;
+                u64 total = 0, before = 0, sum = 0;
+                for (;;) {
+                    // a thread's run: fewer than 2^9 weights of 2^43 at most, or shares of 2^50 in all
+                    double run = 0.0;
+#pragma unroll 4
+                    for (int j = 0; j < g_len; ++j) run += weigh(i0 + j, i0 + j < v);
+                    sum = (u64) run;
+                    before = group.scan(sum, total);
+                    if (total > 0 || mode == kAll) break;
+                    mode = kAll;                                 // q has all that p has: only a draft that q never draws ends here
+                }
+                const u64 t = place_of(u[d], total);
+                if (before <= t && t < before + sum) {
+                    S.group.found = group.tid;
+                    S.group.found_before = before;
+                }
+                group.sync();
+                const int who = S.group.found;
+                if (group.tid < 32) {
+                    // the run again, 32 elements at a time
+                    const int e = min((who + 1) * g_len, v);
+                    u64 run = S.group.found_before;
+                    for (int c = who * g_len; c < e; c += 32) {
+                        const int i = c + group.tid;
+                        const u64 w = (u64) weigh(i, i < e), upto = run + warp_scan(w, group.tid);
+                        if (upto - w <= t && t < upto) {
+                            const float x = rows[0](i);
+                            tokens[pos] = i;
+                            if (logprobs) logprobs[pos] = logprob_of(x, p, heat);
+                        }
+                        run = __shfl_sync(kFull, upto, 31);
+                        if (run > t) break;
+                    }
+                }
+            }
+        }
+        if (NT > 32 && blocks > 1) {
+            __syncwarp();
+            asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+        }
+        return;
+    }
+}
+
+template <class T, int NT, bool DUAL, bool FILTERS>
+cudaError_t launch_sequences(const pk_verify_args & a, int blocks, cudaStream_t s) {
+    constexpr int G = group_of<NT, DUAL>(), GROUPS = NT == 32 ? kSeqGroups : 1;
+    const int rows_each = a.draft_logits ? 2 : 1;
+    const int row_floats = (std::max({a.vocab, NT * run_of<NT>(a.vocab), G * run_of<G>(a.vocab)}) + 3 + 3) / 4 * 4;
+    const size_t smem = GROUPS * ((size_t) rows_each * row_floats * 4 + sizeof(SeqSmem<NT, DUAL, FILTERS>) + (FILTERS ? sizeof(SeqBins<NT, DUAL>) : 0));
+    auto kernel = verify_sequence_kernel<T, NT, DUAL, FILTERS>;
+    static unsigned long long set;                               // devices on which the limit is raised
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e != cudaSuccess) return e;
+    if (!(__atomic_load_n(&set, __ATOMIC_RELAXED) >> device & 1)) {
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) kSmemCap);
+        if (e != cudaSuccess) return e;
+        __atomic_fetch_or(&set, 1ull << device, __ATOMIC_RELAXED);
+    }
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute at[1];
+    cfg.gridDim = dim3((unsigned) (NT == 32 ? (a.sequences + GROUPS - 1) / GROUPS : a.sequences * blocks));
+    cfg.blockDim = dim3(NT == 32 ? 32 * GROUPS : G);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    if (NT > 32) {
+        at[0].id = cudaLaunchAttributeClusterDimension;
+        at[0].val.clusterDim.x = (unsigned) blocks;
+        at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+        cfg.attrs = at;
+        cfg.numAttrs = 1;
+    }
+    return cudaLaunchKernelEx(&cfg, kernel, a, rows_each, row_floats);
+}
+
+// Whether the kernel above can hold a position's rows: beside them there are up to 2048 logits' room in front of and
+// behind each, and 25 KB of the teams'.
+bool resident(int vocab, bool two) { return (size_t) vocab * 4 * (two ? 2 : 1) <= 176 * 1024; }
+
+template <class T, bool FILTERS, int NT> cudaError_t sequences_block(const pk_verify_args & a, cudaStream_t s) {
+    // the blocks of a cluster share the positions out while there are SMs for all
+    const int room = 148 * std::max(1, 1024 / (2 * NT));
+    const int blocks = (int) std::max<long long>(1, std::min<long long>({(long long) kMaxCluster, (long long) a.max_drafts + 1, room / std::max<long long>(1, a.sequences)}));
+    if constexpr (NT <= 256) {
+        if (!a.draft_logits) return launch_sequences<T, 2 * NT, false, FILTERS>(a, blocks, s);
+    } else if (!a.draft_logits) {
+        return launch_sequences<T, NT, false, FILTERS>(a, blocks, s);
+    }
+    return launch_sequences<T, NT, true, FILTERS>(a, blocks, s);
+}
+
+template <class T, bool FILTERS> cudaError_t sequences_dispatch(const pk_verify_args & a, cudaStream_t s) {
+    if (a.vocab <= 1056 && a.sequences >= 4 * 148) return launch_sequences<T, 32, false, FILTERS>(a, 1, s);
+    if (a.vocab <= 2048) return sequences_block<T, FILTERS, 128>(a, s);
+    if (a.sequences * (a.max_drafts + 1) <= 148 || a.vocab > 16384) return sequences_block<T, FILTERS, 512>(a, s);
+    return sequences_block<T, FILTERS, 256>(a, s);
+}
+
+// ---- long rows ---------------------------------------------------------------------
+//
+// Two kernels. The first takes a block or cluster per row, as pk_sample does, and leaves the row's statistics; all rows at
+// once. The second takes a block or cluster per sequence: it tests all drafts at once and draws from the one row, or
+// two, that the first rejection names, reading them again.
+
+struct Plan {
+    pk_verify_args a;
+    RowStat * stats;      // [sequences][max_drafts + 1] of the target, [sequences][max_drafts] of the draft
+};
+
 template <class T, int NT, bool FILTERS, bool CL, bool RES>
-__global__ void __launch_bounds__(NT == 32 ? 256 : NT, NT == 32 ? (FILTERS ? 4 : 5) : 1024 / NT)
-verify_rows_kernel(const Plan plan, int slice, int teams, int row_floats) {
+__global__ void __launch_bounds__(NT, 1024 / NT) verify_rows_kernel(const Plan plan, int slice, int row_floats) {
     extern __shared__ __align__(16) unsigned char raw[];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const pk_verify_args & a = plan.a;
-    const int t_in = NT == 32 ? (int) threadIdx.x >> 5 : 0;      // team within the block
     Team<NT, CL> team;
-    team.tid = NT == 32 ? (int) threadIdx.x & 31 : (int) threadIdx.x;
+    team.tid = (int) threadIdx.x;
     team.blocks = CL ? (int) cg::this_cluster().num_blocks() : 1;
     team.rank = CL ? (int) cg::this_cluster().block_rank() : 0;
     team.phase = 0;
-    const long long id = CL ? (long long) (blockIdx.x / team.blocks) : (long long) blockIdx.x * teams + t_in;
+    const long long id = (long long) (blockIdx.x / team.blocks);
     const long long targets = a.sequences * (a.max_drafts + 1);
     const bool target = id < targets;
     const long long at = target ? id : id - targets;
@@ -64,16 +661,15 @@ verify_rows_kernel(const Plan plan, int slice, int teams, int row_floats) {
     const int pos = (int) (at - seq * per), n = drafts_of(a, seq);
     if (target ? pos > n : pos >= n) return;                     // behind the last draft
     float * rows_at = reinterpret_cast<float *>(raw);
-    TeamSmem<NT> * state = reinterpret_cast<TeamSmem<NT> *>(rows_at + (size_t) teams * row_floats);
-    team.s = state + t_in;
-    TeamBins<NT> * bins = reinterpret_cast<TeamBins<NT> *>(state + teams) + t_in;
+    team.s = reinterpret_cast<TeamSmem<NT> *>(rows_at + row_floats);
+    TeamBins<NT> * bins = reinterpret_cast<TeamBins<NT> *>(team.s + 1);
     team.mine = table_entry(team.lane());
     const int s0 = min(team.rank * slice, a.vocab);
     const T * row_at = target ? static_cast<const T *>(a.logits) + at * a.row_stride : static_cast<const T *>(a.draft_logits) + at * a.draft_stride;
     Slice<T, RES> l;
     l.n = min(slice, a.vocab - s0);
     l.gl = row_at + s0;
-    l.sm = rows_at + (size_t) t_in * row_floats;
+    l.sm = rows_at;
     l.skew = RES ? (int) ((reinterpret_cast<uintptr_t>(l.gl) & 15) / sizeof(T)) & 3 : 0;
     l.inf = false;
     const int len = run_of<NT>(l.n);
@@ -94,6 +690,7 @@ verify_rows_kernel(const Plan plan, int slice, int teams, int row_floats) {
     const int draft = pos < n ? a.drafts[seq * a.max_drafts + pos] : -1;
     const bool one = team.tid == 0 && team.rank == 0;
     RowStat st;
+    st.drafted = 0.0;
     st.flags = hi == CUDART_INF_F ? kInf : 0;
     if (hi == -CUDART_INF_F || !(temp_f > 0.0f)) {
         // nothing to draw, or the first index of the largest
@@ -120,7 +717,7 @@ verify_rows_kernel(const Plan plan, int slice, int teams, int row_floats) {
         if (one) {
             st.flags |= kGreedy;
             st.hi = st.from = st.cut = st.flags & kInf ? 0.0f : hi;
-            st.last = (int) min(first, (u64) 0x7FFFFFFF);
+            st.last = (int) min(first, (u64) kAny);
             st.total = first == ~0ull ? 0ull : (u64) kOne;
             st.drafted = first != ~0ull && draft == (int) first ? 1.0 : 0.0;
             *out = st;
@@ -136,28 +733,19 @@ verify_rows_kernel(const Plan plan, int slice, int teams, int row_floats) {
         l.inf = true;
         hi = lo = 0.0f;
     }
-    Row r;
-    r.top = (double) hi;
-    r.c = 46.166241308446828384 / temp;                          // 32 log2(e) / T
-    r.base = fmaxf(__double2float_ru(r.top - 31.0 * temp), -3.402823466e+38f);
+    const Row r = row_of(hi, temp);
     float least = r.base;                                        // kept: >= least, and what the cut says
     float cut = -CUDART_INF_F;
     u64 ties = ~0ull, total = 0;
     bool partial = false;
     const float m = a.min_ps ? a.min_ps[seq] : a.min_p;
-    // The draft's weight is not subject to `base`; what min-p asks for and the cut it is.
     auto leave = [&](float from, float cut_at, int last, u64 sum) {
         st.hi = hi;
         st.from = from;
         st.cut = cut_at;
         st.last = last;
         st.total = sum;
-        st.drafted = 0.0;
-        if (draft >= 0 && draft < a.vocab) {
-            const float v = seen(to_f32(row_at[draft]), st.flags);
-            const float floor = fmaxf(!(m > 0.0f) ? -CUDART_INF_F : m >= 1.0f ? hi : __double2float_ru(r.top + temp * log((double) m)), -3.402823466e+38f);
-            if (v >= floor && (v > cut_at || (v == cut_at && draft <= last))) st.drafted = v == hi ? 1.0 : exp(((double) v - r.top) / temp);
-        }
+        if (draft >= 0 && draft < a.vocab) st.drafted = draft_weight(seen(to_f32(row_at[draft]), st.flags), draft, st, r, temp, m);
         *out = st;
     };
     if constexpr (FILTERS) {
@@ -165,47 +753,10 @@ verify_rows_kernel(const Plan plan, int slice, int teams, int row_floats) {
         const int k = a.top_ks ? a.top_ks[seq] : a.top_k;
         const bool done = cut_row<T, NT, CL, RES>(team, bins, l, s0, r, hi, lo, temp_f, a.vocab, k, p, m, least, cut, ties, partial,
             [&](const Pair * list, int count, int first, float share, u64 need) {
-                // all that may be kept is on the list: the sum of what is, and the last of it in the order
-                weigh_list<NT>(team.tid, bins, list, count, r, false);
-                team.sync();
-                constexpr int SH = sharers<NT>(), PER = (kList * SH + NT - 1) / NT;
-                Rank rank[PER];
-                u64 sum = 0;
-#pragma unroll
-                for (int q = 0; q < PER; ++q) rank[q].n = kList;
-                over_list<NT, Rank>(team.tid, count,
-                    [&](Rank & b, int j, int i) {
-                        const Pair me = list[j], o = list[i];
-                        if (i < count && (o.v > me.v || (o.v == me.v && o.i < me.i))) { b.w += bins->w[i]; ++b.n; }
-                    },
-                    [&](int j, const Rank & b, int q) {
-                        rank[q] = b;
-                        if (b.n < first) sum += bins->w[j];
-                    });
-                Team<NT, false> block{team.tid, 0, 1, 0, team.s, 0.0};
-                if (need == 0) {
-                    sum = block.sum(sum);
-                    need = share >= 1.0f ? ~0ull : max((u64) ceil(share > 0.0f ? (double) share * (double) sum : 0.0), 1ull);
-                }
-                u64 kept = 0;
-                int tokens = 0;
-#pragma unroll
-                for (int q = 0; q < PER; ++q) {
-                    const int j = (team.tid + q * NT) / SH;
-                    if (j < count && team.tid % SH == 0 && rank[q].n < first && rank[q].w < need && list[j].v >= least) {
-                        kept += bins->w[j];
-                        ++tokens;
-                    }
-                }
-                kept = block.sum(kept);
-                const int all = (int) block.sum((u64) tokens);
-#pragma unroll
-                for (int q = 0; q < PER; ++q) {
-                    const int j = (team.tid + q * NT) / SH;
-                    if (j < count && team.tid % SH == 0 && rank[q].n == all - 1 && team.rank == 0) leave(least, list[j].v, list[j].i, kept);
-                }
+                keep_listed(team, bins, list, count, r, first, share, need, least,
+                            [&](float v, int i, u64 sum) { if (team.rank == 0) leave(v, v, i, sum); });
             },
-            [] { return false; });
+            [](double) { return false; });
         if (done) {
             if (CL) team.meet();
             return;
@@ -248,7 +799,7 @@ verify_rows_kernel(const Plan plan, int slice, int teams, int row_floats) {
             leave(from, cut, s0 + i, total);
         }
     } else if (one) {
-        leave(from, cut, 0x7FFFFFFF, total);
+        leave(from, cut, kAny, total);
     }
     if (CL) team.meet();                                         // a block's memory stays while others may read it
 }
@@ -267,14 +818,12 @@ template <class T> struct DrawRow {
         from = s.from;
         cut = s.cut;
         last = s.last;
-        r.top = (double) s.hi;
-        r.c = 46.166241308446828384 / (flags & kGreedy ? 1.0 : (double) temp);
-        r.base = s.from;
+        r = row_of(s.hi, flags & kGreedy ? 1.0 : (double) temp);
     }
     // Weight of token i with logit v (times 2^43, a whole number); the whole warp calls.
     __device__ __forceinline__ double weight(float v, int i, double mine) const {
         v = seen(v, flags);
-        const bool keep = v >= from && (v > cut || (v == cut && i <= last));
+        const bool keep = v >= from && (v > cut || i <= last);
         const double w = weight_warp(keep ? v : (float) r.top, r, mine) - kZero;
         return keep ? w : 0.0;
     }
@@ -282,7 +831,6 @@ template <class T> struct DrawRow {
 
 constexpr int kDrawThreads = 512;
 constexpr int kDrawWarps = kDrawThreads / 32;
-constexpr double kShare = 1152921504606846976.0;        // 2^60: probabilities as integers
 
 template <class T, bool CL>
 __global__ void __launch_bounds__(kDrawThreads) verify_draw_kernel(const Plan plan) {
@@ -307,8 +855,7 @@ __global__ void __launch_bounds__(kDrawThreads) verify_draw_kernel(const Plan pl
         double qd;
         if (a.draft_logits) qd = qs[j].total ? qs[j].drafted / ((double) qs[j].total * (1.0 / kOne)) : 0.0;
         else qd = drafts[j] >= 0 && drafts[j] < v ? 1.0 : 0.0;
-        const float x = u[j] > 0.0f ? fminf(u[j], 0x1.fffffep-1f) : 0.0f;
-        if (!((double) x * qd < pd)) atomicMin(&s_first, j);
+        if (!((double) number_of(u[j]) * qd < pd)) atomicMin(&s_first, j);
     }
     __syncthreads();
     const int first = s_first;
@@ -357,10 +904,10 @@ __global__ void __launch_bounds__(kDrawThreads) verify_draw_kernel(const Plan pl
         if (mode == kLess) {
             // the two products rounded alike: equal rows leave nothing
             const double less = qr.weight(in ? to_f32(qr.at[i]) : -CUDART_INF_F, i, mine);
-            w = fmax(__dmul_rn(w, sp) - __dmul_rn(less, sq), 0.0);
+            w = fmax((__dmul_rn(w, sp) - __dmul_rn(less, sq) + kMagic) - kMagic, 0.0);
         }
         if (mode == kWithout && i == out) w = 0.0;
-        return in ? __double2ull_rn(w) : 0ull;
+        return in ? (u64) w : 0ull;
     };
     auto stretch = [&](int begin, int end) {             // its sum, over a warp
         u64 s = 0;
@@ -439,7 +986,6 @@ __global__ void __launch_bounds__(kDrawThreads) verify_draw_kernel(const Plan pl
 
 template <class T, int NT, bool FILTERS, bool CL, bool RES>
 cudaError_t launch_rows(const Plan & p, long long rows, int blocks, int slice, int row_floats, size_t smem, cudaStream_t s) {
-    const int teams = NT == 32 ? 8 : 1;
     auto kernel = verify_rows_kernel<T, NT, FILTERS, CL, RES>;
     static unsigned long long set;                               // devices on which the limit is raised
     int device = 0;
@@ -452,8 +998,8 @@ cudaError_t launch_rows(const Plan & p, long long rows, int blocks, int slice, i
     }
     cudaLaunchConfig_t cfg{};
     cudaLaunchAttribute at[1];
-    cfg.gridDim = dim3((unsigned) (CL ? rows * blocks : (rows + teams - 1) / teams));
-    cfg.blockDim = dim3(NT == 32 ? 256 : NT);
+    cfg.gridDim = dim3((unsigned) (rows * blocks));
+    cfg.blockDim = dim3(NT);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
     if (CL) {
@@ -463,14 +1009,7 @@ cudaError_t launch_rows(const Plan & p, long long rows, int blocks, int slice, i
         cfg.attrs = at;
         cfg.numAttrs = 1;
     }
-    return cudaLaunchKernelEx(&cfg, kernel, p, slice, teams, row_floats);
-}
-
-template <class T, bool FILTERS, int NT>
-cudaError_t rows_block(const Plan & p, long long rows, cudaStream_t s) {
-    int row_floats;
-    const size_t smem = team_bytes<NT, FILTERS>(p.a.vocab, row_floats);
-    return launch_rows<T, NT, FILTERS, false, true>(p, rows, 1, p.a.vocab, row_floats, smem, s);
+    return cudaLaunchKernelEx(&cfg, kernel, p, slice, row_floats);
 }
 
 template <class T, bool FILTERS>
@@ -483,21 +1022,18 @@ cudaError_t rows_cluster(const Plan & p, long long rows, int blocks, cudaStream_
     return launch_rows<T, 1024, FILTERS, true, false>(p, rows, blocks, slice, 0, smem - (size_t) row_floats * 4, s);
 }
 
-// Teams by rows and vocabulary as in pk_sample, whose figures hold here too: most of a row's time is the same.
+// Blocks by rows and vocabulary as in pk_sample.
 template <class T, bool FILTERS>
 cudaError_t rows_dispatch(const Plan & p, cudaStream_t s) {
     const int v = p.a.vocab;
     const long long rows = p.a.sequences * (p.a.max_drafts + 1) + (p.a.draft_logits ? p.a.sequences * p.a.max_drafts : 0);
-    if (FILTERS ? v <= 1056 && rows >= 20 * 148 : v <= 2048 && rows >= 8 * 148) return rows_block<T, FILTERS, 32>(p, rows, s);
     int blocks = 1;
-    if (v > 16384)
-        while (blocks < kMaxCluster && rows * blocks * 2 <= 148) blocks *= 2;
+    while (blocks < kMaxCluster && rows * blocks * 2 <= 148) blocks *= 2;
     while (blocks < kMaxCluster && (size_t) (v / blocks) * 4 > 200 * 1024) blocks *= 2;
     if (blocks > 1) return rows_cluster<T, FILTERS>(p, rows, blocks, s);
-    const bool wave512 = rows <= 2 * 148 && v > 2048, wave256 = rows <= 4 * 148;
-    if (v > 16384 || wave512) return rows_block<T, FILTERS, 512>(p, rows, s);
-    if (v > 5120 || wave256) return rows_block<T, FILTERS, 256>(p, rows, s);
-    return rows_block<T, FILTERS, 128>(p, rows, s);
+    int row_floats;
+    const size_t smem = team_bytes<512, FILTERS>(v, row_floats);
+    return launch_rows<T, 512, FILTERS, false, true>(p, rows, 1, v, row_floats, smem, s);
 }
 
 template <class T, bool CL>
@@ -518,11 +1054,11 @@ cudaError_t launch_draw(const Plan & p, int blocks, cudaStream_t s) {
 }
 
 template <class T> cudaError_t dispatch(const Plan & p, bool filters, cudaStream_t s) {
+    if (resident(p.a.vocab, p.a.draft_logits != nullptr)) return filters ? sequences_dispatch<T, true>(p.a, s) : sequences_dispatch<T, false>(p.a, s);
     const cudaError_t e = filters ? rows_dispatch<T, true>(p, s) : rows_dispatch<T, false>(p, s);
     if (e != cudaSuccess) return e;
     int blocks = 1;
-    if (p.a.vocab > 16384)
-        while (blocks < kMaxCluster && p.a.sequences * blocks * 2 <= 148) blocks *= 2;
+    while (blocks < kMaxCluster && p.a.sequences * blocks * 2 <= 148) blocks *= 2;
     return blocks > 1 ? launch_draw<T, true>(p, blocks, s) : launch_draw<T, false>(p, 1, s);
 }
 
@@ -538,7 +1074,7 @@ int64_t rows_of(int64_t sequences, int32_t max_drafts, int32_t vocab) {
 
 extern "C" PK_API int64_t pk_verify_workspace(int64_t sequences, int32_t max_drafts, int32_t vocab) {
     const int64_t rows = pk::rows_of(sequences, max_drafts, vocab);
-    return rows < 0 ? -1 : rows * (int64_t) sizeof(pk::RowStat);
+    return rows < 0 ? -1 : pk::resident(vocab, true) ? 0 : rows * (int64_t) sizeof(pk::RowStat);
 }
 
 extern "C" PK_API pk_status pk_verify(int device, const pk_verify_args * a, void * stream) {
@@ -554,7 +1090,7 @@ extern "C" PK_API pk_status pk_verify(int device, const pk_verify_args * a, void
     if (a->row_stride < a->vocab || a->row_stride > (INT64_MAX >> 34) ||
         (a->draft_logits && (a->draft_stride < a->vocab || a->draft_stride > (INT64_MAX >> 34))))
         return op_fail(PK_ERR_INVALID, fn, "row_stride and draft_stride must be at least vocab");
-    if (a->sequences > 0 && (!a->logits || !a->uniforms || !a->tokens || !a->accepted || !a->workspace || (a->max_drafts > 0 && !a->drafts)))
+    if (a->sequences > 0 && (!a->logits || !a->uniforms || !a->tokens || !a->accepted || (a->max_drafts > 0 && !a->drafts)))
         return op_fail(PK_ERR_INVALID, fn, "null pointer");
     if (!aligned_to(a->logits, (size_t) es) || !aligned_to(a->draft_logits, (size_t) es))
         return op_fail(PK_ERR_INVALID, fn, "logits must be aligned to their element");
@@ -563,8 +1099,9 @@ extern "C" PK_API pk_status pk_verify(int device, const pk_verify_args * a, void
                            (const void *) a->top_ks, (const void *) a->top_ps, (const void *) a->min_ps})
         if (!aligned_to(q, 4)) return op_fail(PK_ERR_INVALID, fn, "arrays must be 4-byte aligned");
     if (!aligned_to(a->workspace, 8)) return op_fail(PK_ERR_INVALID, fn, "workspace must be 8-byte aligned");
-    if (a->workspace_bytes < rows * (int64_t) sizeof(RowStat))
-        return op_fail(PK_ERR_INVALID, fn, "workspace_bytes is below pk_verify_workspace()");
+    if (a->sequences > 0 && !resident(a->vocab, a->draft_logits && a->max_drafts > 0) &&
+        (!a->workspace || a->workspace_bytes < rows * (int64_t) sizeof(RowStat)))
+        return op_fail(PK_ERR_INVALID, fn, "workspace is null or workspace_bytes below pk_verify_workspace()");
     if (!device_ok(device)) return op_fail(PK_ERR_NO_DEVICE, fn, "no sm_100 device with that index");
     if (a->sequences == 0) return PK_OK;
     DeviceScope dev(device);
