@@ -16,6 +16,8 @@
 
 #include "pk_draw.cuh"
 
+#include <type_traits>
+
 namespace pk {
 namespace {
 
@@ -358,8 +360,82 @@ __device__ bool draw_near(Team<G, false> & group, const Slice<T, true> & pl, con
     return done;
 }
 
+// ---- the test of a draft where nothing is cut ---------------------------------------
+//
+// 1 / p(d) is the sum of exp((l_i - l_d) / T): one pass over the row as it comes from memory, without the largest logit
+// and without shared memory. As in pk_sample.cu a weight w^ of a logit x = log2 w away is off by 2^-24 (8 + 2.78 |x|)
+// of itself; with p = w / S, the sum of p |x| is at most the entropy and |log2 p(d)|, 15.5 + 24 for S < 2^24, and the
+// additions of a thread's quarter are 46 at most; the draft's own weight, by which the sum is divided, is off by 8:
+// 172 2^-24 together. What it leaves open, and rows with NaN or infinities that matter, are left to the row's statistics.
+constexpr double kQuick = 180.0 * 0x1p-24;
+
+// A thread's part of the sum.
+template <class T, int NT>
+__device__ __forceinline__ float quick_part(const T * __restrict__ g, int n, int tid, float c, float k) {
+    constexpr int W = 16 / (int) sizeof(T);
+    auto weight = [&](float v) {
+        float w;
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w) : "f"(fmaf(v, c, -k)));
+        return w;
+    };
+    const int head = min(n, (int) ((16 - (reinterpret_cast<uintptr_t>(g) & 15)) & 15) / (int) sizeof(T)), vecs = (n - head) / W;
+    float part[4] = {};
+    const uint4 * at = reinterpret_cast<const uint4 *>(g + head);
+    auto add = [&](const uint4 & q) {
+        const unsigned w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if constexpr (sizeof(T) == 4) {
+                part[j] += weight(__uint_as_float(w[j]));
+            } else {
+                T e[2];
+                *reinterpret_cast<unsigned *>(e) = w[j];
+                part[j] += weight(to_f32(e[0]));
+                part[j] += weight(to_f32(e[1]));
+            }
+        }
+    };
+    int i = tid;
+    for (; i + 7 * NT < vecs; i += 8 * NT) {
+        uint4 q[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) q[j] = __ldg(at + i + j * NT);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) add(q[j]);
+    }
+    for (; i < vecs; i += NT) add(__ldg(at + i));
+    if (tid < 16) {                                      // fewer than W at either end
+        const int e = tid < 8 ? tid : head + vecs * W + tid - 8;
+        if (tid < 8 ? e < head : e < n) part[0] += weight(to_f32(g[e]));
+    }
+    return (part[0] + part[1]) + (part[2] + part[3]);
+}
+
+// 1 / p(d) of a row by its team; no number, or 2^24 and more, where it does not tell.
+template <class T, int NT, bool NM>
+__device__ double quick_sum(Team<NT, false, NM> & team, const T * row, int n, int draft, float temp) {
+    const float c = 1.4426950408889634f * (1.0f / temp), v = to_f32(row[draft]), k = v * c;
+    const bool fine = c > 1e-30f && c < 1e30f && fabsf(k) < 1e6f;   // the same for all
+    double sum = 0.0;
+    if (fine) sum = (double) quick_part<T, NT>(row, n, team.tid, c, k);
+    sum = warp_sum(sum);
+    if (NT > 32) {
+        team.sync();
+        if (team.lane() == 0) team.s->wscan[team.tid >> 5] = (u64) __double_as_longlong(sum);
+        team.sync();
+        sum = 0.0;
+#pragma unroll
+        for (int i = 0; i < NT / 32; ++i) sum += __longlong_as_double((long long) team.s->wscan[i]);
+    }
+    float own;                                           // the draft's own weight: one, but for the rounding of k
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(own) : "f"(fmaf(v, c, -k)));
+    return fine ? sum / (double) own : __longlong_as_double(0x7FF8000000000000ll);
+}
+
 template <int NT, bool DUAL> constexpr int group_of() { return DUAL ? 2 * NT : NT; }
-template <int NT, bool DUAL, bool FILTERS> struct SeqSmem {
+struct SeqSums { double quick[2]; };                    // of the test where nothing is cut
+struct NoSums {};
+template <int NT, bool DUAL, bool FILTERS> struct SeqSmem : std::conditional_t<FILTERS, NoSums, SeqSums> {
     TeamSmem<NT> team[DUAL ? 2 : 1];
     TeamSmem<group_of<NT, DUAL>()> group;
     RowStat st[2];
@@ -423,22 +499,45 @@ verify_sequence_kernel(const pk_verify_args a, int rows_each, int row_floats) {
         const int pos = base + rank;
         const bool two = a.draft_logits && pos < n;
         int code = kAccepted, draft = -1;
+        float quick_log = CUDART_INF_F;
         if (pos <= n) {
             if (pos < n) draft = drafts[pos];
             slice(0, pos);
             if (two) slice(1, pos);
-            if (!DUAL || own == 0 || two) {
-                const int end = DUAL || !two ? 1 : 2;
-                for (int i = 0; i < end; ++i) load_slice<T, NT>(rows[DUAL ? own : i], team.tid);
-                team.sync();
-                for (int i = 0; i < end; ++i) {
-                    const int which = DUAL ? own : i;
-                    row_stat<T, NT, FILTERS>(team, &B->bins[own], rows[which], a, seq, draft, &S.st[which]);
-                    if (end > 1) team.sync();
+            bool open = true;                                    // whether the draft stands
+            if constexpr (!FILTERS) {
+                if (pos < n && draft >= 0 && draft < v && temp_f > 0.0f && (a.draft_logits == nullptr || two)) {
+                    if (!DUAL || own == 0 || two) {
+                        for (int i = 0; i < (DUAL || !two ? 1 : 2); ++i) {
+                            const int which = DUAL ? own : i;
+                            const double sum = quick_sum<T, NT>(team, rows[which].gl, v, draft, temp_f);
+                            if (team.tid == 0) S.quick[which] = sum;
+                        }
+                    }
+                    group.sync();
+                    // u q(d) < p(d) by more than the sums are off by, twice
+                    const double p = S.quick[0], q = two ? S.quick[1] : 1.0;
+                    open = !(p < 0x1p24 && q < 0x1p24 && (double) number_of(u[pos]) * p * (1.0 + 4.0 * kQuick) < q);
+                    if (!open && logprobs && group.tid == 0) quick_log = -logf((float) p);
+                    group.sync();
                 }
             }
-            group.sync();
-            if (pos == n) {
+            if (open) {
+                if (!DUAL || own == 0 || two) {
+                    const int end = DUAL || !two ? 1 : 2;
+                    for (int i = 0; i < end; ++i) load_slice<T, NT>(rows[DUAL ? own : i], team.tid);
+                    team.sync();
+                    for (int i = 0; i < end; ++i) {
+                        const int which = DUAL ? own : i;
+                        row_stat<T, NT, FILTERS>(team, &B->bins[own], rows[which], a, seq, draft, &S.st[which]);
+                        if (end > 1) team.sync();
+                    }
+                }
+                group.sync();
+            }
+            if (!open) {
+                code = kAccepted;
+            } else if (pos == n) {
                 code = kEnd;
             } else {
                 // u q(d) < p(d), as u w_q(d) P < w_p(d) Q; f32 sums may leave it open
@@ -476,7 +575,8 @@ verify_sequence_kernel(const pk_verify_args a, int rows_each, int row_floats) {
         }
         if (code == kAccepted && pos < n && (first < 0 || rank < first) && group.tid == 0) {
             tokens[pos] = draft;
-            if (logprobs) logprobs[pos] = logprob_of(rows[0](draft), S.st[0], S.st[0].flags & kGreedy ? 1.0 : temp);
+            if (logprobs)
+                logprobs[pos] = !FILTERS && quick_log < CUDART_INF_F ? quick_log : logprob_of(rows[0](draft), S.st[0], S.st[0].flags & kGreedy ? 1.0 : temp);
         }
         if (first < 0) {
             group.sync();                                        // the rows' memory is read
@@ -612,21 +712,24 @@ cudaError_t launch_sequences(const pk_verify_args & a, int blocks, cudaStream_t 
 bool resident(int vocab, bool two) { return (size_t) vocab * 4 * (two ? 2 : 1) <= 176 * 1024; }
 
 template <class T, bool FILTERS, int NT> cudaError_t sequences_block(const pk_verify_args & a, cudaStream_t s) {
-    // the blocks of a cluster share the positions out while there are SMs for all
-    const int room = 148 * std::max(1, 1024 / (2 * NT));
-    const int blocks = (int) std::max<long long>(1, std::min<long long>({(long long) kMaxCluster, (long long) a.max_drafts + 1, room / std::max<long long>(1, a.sequences)}));
-    if constexpr (NT <= 256) {
-        if (!a.draft_logits) return launch_sequences<T, 2 * NT, false, FILTERS>(a, blocks, s);
-    } else if (!a.draft_logits) {
-        return launch_sequences<T, NT, false, FILTERS>(a, blocks, s);
-    }
-    return launch_sequences<T, NT, true, FILTERS>(a, blocks, s);
+    // The blocks of a cluster share the positions out while there is room for them (four drafts by 8193, temperature alone, 64
+    // sequences in clusters of 4, 2 and 1: 25.5 us, 25.9, 26.9; of 5, which no longer all run at once, 29.8). With filters a
+    // position takes longer and more blocks than there is room for still pay (64 sequences, settings mixed: of 5 37.6 us, of 4
+    // 41.1, of 1 85; 256 of eight drafts, top-p: of 2 120 us, of 1 136; 300: 155 and 159).
+    const long long room = 148 * std::max(1, 1024 / (2 * NT)), share = (FILTERS ? room * 7 / 4 : room) / std::max<long long>(1, a.sequences);
+    const int blocks = (int) std::max<long long>(1, std::min<long long>({FILTERS ? kMaxCluster : 4, (long long) a.max_drafts + 1, share}));
+    if (a.draft_logits) return launch_sequences<T, NT, true, FILTERS>(a, blocks, s);
+    return launch_sequences<T, NT <= 256 ? 2 * NT : NT, false, FILTERS>(a, blocks, s);
 }
 
+// A warp per sequence for many short rows (2000 of four drafts by 1025, temperature alone: 44 us, a block of 256 52; top-k and
+// top-p 178 and 220). Otherwise two teams of 128 threads for short rows (400 by 4000, temperature alone: 30 us, of 256 40), of
+// 512 for long ones (300 of three drafts by 16000, top-p: 199 us, of 256 331) and for few with filters (8 by 8193, top-p: 25 us
+// and 35), of 256 in between.
 template <class T, bool FILTERS> cudaError_t sequences_dispatch(const pk_verify_args & a, cudaStream_t s) {
     if (a.vocab <= 1056 && a.sequences >= 4 * 148) return launch_sequences<T, 32, false, FILTERS>(a, 1, s);
-    if (a.vocab <= 2048) return sequences_block<T, FILTERS, 128>(a, s);
-    if (a.sequences * (a.max_drafts + 1) <= 148 || a.vocab > 16384) return sequences_block<T, FILTERS, 512>(a, s);
+    if (a.vocab <= (FILTERS ? 2048 : 6144)) return sequences_block<T, FILTERS, 128>(a, s);
+    if (FILTERS ? a.vocab > 12288 || a.sequences * (a.max_drafts + 1) <= 148 : a.vocab > 16384) return sequences_block<T, FILTERS, 512>(a, s);
     return sequences_block<T, FILTERS, 256>(a, s);
 }
 

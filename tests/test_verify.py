@@ -155,9 +155,10 @@ def check(call, drafts, u, counts=None, excused=0, **kw):
     """Tokens and counts equal. Weights are rounded to 2^-43 of the largest one by one, which moves a distribution's
     sums by v 2^-43 at most, the difference of two by twice that, its product with u by as much again; nearer than
     (v + 4) 2^-41 to a border the definition's other answer is the fixed point's. At most `excused` sequences may be.
-    Log-probabilities: rounded once; the logarithm of a sum off by v 2^-43, or, of f32 weights, by 70 2^-24 of itself (8
-    for each exponential, 2.78 log2 V <= 42 for its argument, 19 for the additions), rounded to f32 (one 2^-24 of it, 16 of
-    the logarithm, which is below 16)."""
+    Log-probabilities, in units of 2^-24: (l - l_0) / T by f32's 1 / T and log2(e), three roundings, and rounded once; the
+    logarithm of a sum of f32 weights, off by 8 for each exponential, 2.78 for each unit of its argument (log2 V and
+    24 at most on average) and the additions (v / 512 and 24), to f32 (one, and 16 for a logarithm below 17); or of a
+    sum off by v 2^-43."""
     tok, acc, lp = call.answer()
     p, q = call.seen()
     near_ones = 0
@@ -174,7 +175,7 @@ def check(call, drafts, u, counts=None, excused=0, **kw):
             if np.isinf(x):
                 assert lp[i, j] == x
             else:
-                tol = 2.0 ** -24 * abs(x) + call.v * 2.0 ** -43 + 87 * 2.0 ** -24
+                tol = 2.0 ** -24 * (5 * abs(x) + 8 + 2.78 * (np.log2(call.v) + 24) + call.v / 512 + 24 + 17) + call.v * 2.0 ** -43
                 assert abs(lp[i, j] - x) <= tol, (i, j, lp[i, j], x)
         assert np.isneginf(lp[i, len(want):]).all()
     assert near_ones <= excused
