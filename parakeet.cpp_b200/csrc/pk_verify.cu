@@ -735,8 +735,8 @@ template <class T, bool FILTERS> cudaError_t sequences_dispatch(const pk_verify_
 
 // ---- long rows ---------------------------------------------------------------------
 //
-// Two kernels. The first takes a block or cluster per row, as pk_sample does, and leaves the row's statistics; all rows at
-// once. The second takes a block or cluster per sequence: it tests all drafts at once and draws from the one row, or
+// Two kernels. The first takes a block or cluster per row, all rows at once, and leaves what the test needs of it; with filters
+// as pk_sample does. The second takes a block or cluster per sequence: it tests all drafts at once and draws from the one row, or
 // two, that the first rejection names, reading them again.
 
 struct Plan {
@@ -744,7 +744,7 @@ struct Plan {
     RowStat * stats;      // [sequences][max_drafts + 1] of the target, [sequences][max_drafts] of the draft
 };
 
-template <class T, int NT, bool FILTERS, bool CL, bool RES>
+template <class T, int NT, bool CL, bool RES>
 __global__ void __launch_bounds__(NT, 1024 / NT) verify_rows_kernel(const Plan plan, int slice, int row_floats) {
     extern __shared__ __align__(16) unsigned char raw[];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -786,9 +786,9 @@ __global__ void __launch_bounds__(NT, 1024 / NT) verify_rows_kernel(const Plan p
     float hi = -CUDART_INF_F, lo = CUDART_INF_F;                 // fmaxf and fminf pass over NaN
     l.template each<NT>(team.tid, [&](float v, int) {
         hi = fmaxf(hi, v);
-        if (FILTERS && v > -CUDART_INF_F) lo = fminf(lo, v);
+        if (v > -CUDART_INF_F) lo = fminf(lo, v);
     });
-    team.template range<FILTERS>(hi, lo);
+    team.template range<true>(hi, lo);
     RowStat * out = plan.stats + id;
     const int draft = pos < n ? a.drafts[seq * a.max_drafts + pos] : -1;
     const bool one = team.tid == 0 && team.rank == 0;
@@ -851,19 +851,17 @@ __global__ void __launch_bounds__(NT, 1024 / NT) verify_rows_kernel(const Plan p
         if (draft >= 0 && draft < a.vocab) st.drafted = draft_weight(seen(to_f32(row_at[draft]), st.flags), draft, st, r, temp, m);
         *out = st;
     };
-    if constexpr (FILTERS) {
-        const float p = a.top_ps ? a.top_ps[seq] : a.top_p;
-        const int k = a.top_ks ? a.top_ks[seq] : a.top_k;
-        const bool done = cut_row<T, NT, CL, RES>(team, bins, l, s0, r, hi, lo, temp_f, a.vocab, k, p, m, least, cut, ties, partial,
-            [&](const Pair * list, int count, int first, float share, u64 need) {
-                keep_listed(team, bins, list, count, r, first, share, need, least,
-                            [&](float v, int i, u64 sum) { if (team.rank == 0) leave(v, v, i, sum); });
-            },
-            [](double) { return false; });
-        if (done) {
-            if (CL) team.meet();
-            return;
-        }
+    const float p = a.top_ps ? a.top_ps[seq] : a.top_p;
+    const int k = a.top_ks ? a.top_ks[seq] : a.top_k;
+    const bool done = cut_row<T, NT, CL, RES>(team, bins, l, s0, r, hi, lo, temp_f, a.vocab, k, p, m, least, cut, ties, partial,
+        [&](const Pair * list, int count, int first, float share, u64 need) {
+            keep_listed(team, bins, list, count, r, first, share, need, least,
+                        [&](float v, int i, u64 sum) { if (team.rank == 0) leave(v, v, i, sum); });
+        },
+        [](double) { return false; });
+    if (done) {
+        if (CL) team.meet();
+        return;
     }
     const int i0 = RES ? team.tid * len : min(team.tid * len, l.n), i1 = RES ? i0 + len : min(i0 + len, l.n);
     // a run has fewer than 2^9 elements, so its sum stays below 2^53 and is whole
@@ -874,27 +872,25 @@ __global__ void __launch_bounds__(NT, 1024 / NT) verify_rows_kernel(const Plan p
     for (int j = 0; j < len; ++j) {
         const float v = RES || i0 + j < i1 ? l(i0 + j) : -CUDART_INF_F;
         bool keep = v >= from;
-        if (FILTERS) {
-            if (partial && v == cut) {
-                ++equal;
-                keep = false;
-            }
-            if (!__any_sync(kFull, keep)) continue;
+        if (partial && v == cut) {
+            ++equal;
+            keep = false;
         }
+        if (!__any_sync(kFull, keep)) continue;
         const double w = weight_warp(v, r, team.mine, onto);
         if (keep) onto = w;
     }
     u64 sum = whole(onto);
     bool mine = false;                                           // the last of the ties that are kept is in this run
     u64 before = 0;
-    if (FILTERS && partial) {
+    if (partial) {
         u64 all;
         before = team.scan((u64) equal, all);
         if (cut >= least && before < ties) sum += min((u64) equal, ties - before) * weight_one(cut, r);
         mine = before < ties && ties <= before + equal;
     }
     total = team.sum(sum);
-    if (FILTERS && partial) {
+    if (partial) {
         if (mine) {
             int i = i0;
             for (u64 left = ties - before; i < i1; ++i)
@@ -935,7 +931,50 @@ template <class T> struct DrawRow {
 constexpr int kDrawThreads = 512;
 constexpr int kDrawWarps = kDrawThreads / 32;
 
+// Without filters the test takes 1 / p(d) by f32, see quick_part: a block or cluster per row and draft, the sum to
+// `drafted` of the row's place.
 template <class T, bool CL>
+__global__ void __launch_bounds__(kDrawThreads) verify_sums_kernel(const Plan plan) {
+    const pk_verify_args & a = plan.a;
+    __shared__ float sums[kDrawWarps];
+    __shared__ float its;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int tid = threadIdx.x;
+    const int blocks = CL ? (int) cg::this_cluster().num_blocks() : 1, rank = CL ? (int) cg::this_cluster().block_rank() : 0;
+    const long long id = blockIdx.x / blocks, drafts = a.sequences * a.max_drafts;
+    const long long at = id < drafts ? id : id - drafts, seq = at / a.max_drafts;
+    const int pos = (int) (at - seq * a.max_drafts), draft = a.drafts[at], v = a.vocab;
+    if (pos >= drafts_of(a, seq)) return;                        // behind the last draft
+    const T * row = id < drafts ? static_cast<const T *>(a.logits) + (seq * (a.max_drafts + 1) + pos) * a.row_stride
+                                : static_cast<const T *>(a.draft_logits) + at * a.draft_stride;
+    const float temp_f = temperature_of(a, seq), c = 1.4426950408889634f * (1.0f / temp_f);
+    const bool inside = draft >= 0 && draft < v;
+    const float l = inside ? to_f32(row[draft]) : CUDART_NAN_F, k = l * c;
+    const bool fine = temp_f > 0.0f && c > 1e-30f && c < 1e30f && fabsf(k) < 1e6f;    // the same for all
+    const int slice = ((v + blocks - 1) / blocks + 31) & ~31, s0 = min(rank * slice, v);
+    float sum = fine ? quick_part<T, kDrawThreads>(row + s0, min(slice, v - s0), tid, c, k) : 0.0f;
+    sum = warp_sum(sum);
+    if ((tid & 31) == 0) sums[tid >> 5] = sum;
+    __syncthreads();
+    sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kDrawWarps; ++i) sum += sums[i];
+    if (CL) {
+        if (tid == 0) its = sum;
+        cg::this_cluster().sync();
+        sum = 0.0f;
+        for (int b = 0; b < blocks; ++b) sum += *cg::this_cluster().map_shared_rank(&its, b);
+        cg::this_cluster().sync();                               // its memory stays while others read it
+    }
+    float own;                                                   // the draft's own weight: one, but for the rounding of k
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(own) : "f"(fmaf(l, c, -k)));
+    const long long place = id < drafts ? seq * (a.max_drafts + 1) + pos : a.sequences * (a.max_drafts + 1) + at;
+    if (tid == 0 && rank == 0) plan.stats[place].drafted = fine ? (double) (sum / own) : (double) CUDART_NAN_F;
+}
+
+// FILTERS: the rows' statistics are there. Otherwise the test's sums are, and what else is needed of the few rows that
+// it leaves open, or that are drawn from, is found here.
+template <class T, bool CL, bool FILTERS>
 __global__ void __launch_bounds__(kDrawThreads) verify_draw_kernel(const Plan plan) {
     const pk_verify_args & a = plan.a;
     __shared__ u64 sums[kDrawWarps];
@@ -946,6 +985,7 @@ __global__ void __launch_bounds__(kDrawThreads) verify_draw_kernel(const Plan pl
     const int blocks = CL ? (int) cg::this_cluster().num_blocks() : 1, rank = CL ? (int) cg::this_cluster().block_rank() : 0;
     const long long seq = blockIdx.x / blocks;
     const int d = a.max_drafts, n = drafts_of(a, seq), v = a.vocab;
+    unsigned phase = 0;                                  // the exchanges take turns
     if (tid == 0) s_first = n;
     const double mine = table_entry(lane);
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -953,45 +993,152 @@ __global__ void __launch_bounds__(kDrawThreads) verify_draw_kernel(const Plan pl
     const RowStat * ps = plan.stats + seq * (d + 1), * qs = plan.stats + a.sequences * (d + 1) + seq * d;
     const int32_t * drafts = a.drafts + seq * d;
     const float * u = a.uniforms + seq * (d + 1);
-    for (int j = tid; j < n; j += kDrawThreads) {
-        const double pd = ps[j].total ? ps[j].drafted / ((double) ps[j].total * (1.0 / kOne)) : 0.0;
-        double qd;
-        if (a.draft_logits) qd = qs[j].total ? qs[j].drafted / ((double) qs[j].total * (1.0 / kOne)) : 0.0;
-        else qd = drafts[j] >= 0 && drafts[j] < v ? 1.0 : 0.0;
-        if (!((double) number_of(u[j]) * qd < pd)) atomicMin(&s_first, j);
-    }
-    __syncthreads();
-    const int first = s_first;
     const float temp = temperature_of(a, seq);
+    auto target_row = [&](int j) { return static_cast<const T *>(a.logits) + (seq * (d + 1) + j) * a.row_stride; };
+    auto draft_row = [&](int j) { return static_cast<const T *>(a.draft_logits) + (seq * d + j) * a.draft_stride; };
+    // over all threads of all blocks
+    auto join_all = [&](u64 x, auto join) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) x = join(x, __shfl_xor_sync(kFull, x, o));
+        __syncthreads();
+        if (lane == 0) sums[warp] = x;
+        __syncthreads();
+        x = sums[0];
+#pragma unroll
+        for (int i = 1; i < kDrawWarps; ++i) x = join(x, sums[i]);
+        if (CL) {
+            if (tid == 0) exchange[phase] = x;
+            cg::this_cluster().sync();
+            for (int b = 0; b < blocks; ++b) x = b == 0 ? *cg::this_cluster().map_shared_rank(&exchange[phase], 0)
+                                                        : join(x, *cg::this_cluster().map_shared_rank(&exchange[phase], b));
+            phase ^= 1;
+        }
+        return x;
+    };
+    const int all = kDrawThreads * blocks, me = rank * kDrawThreads + tid;
+    // a row's statistics by whole numbers, where nothing is cut; the same for every thread. Without `sum` the total is only
+    // known to be more than nothing.
+    auto stat_of = [&](const T * row, int draft, bool with_sum) {
+        RowStat st;
+        st.drafted = 0.0;
+        st.last = kAny;
+        float hi = -CUDART_INF_F;                        // fmaxf passes over NaN
+#pragma unroll 8
+        for (int i = me; i < v; i += all) hi = fmaxf(hi, to_f32(row[i]));
+        hi = __uint_as_float((unsigned) join_all((u64) __float_as_uint(hi), [](u64 x, u64 y) {
+            return (u64) __float_as_uint(fmaxf(__uint_as_float((unsigned) x), __uint_as_float((unsigned) y)));
+        }));
+        st.flags = hi == CUDART_INF_F ? kInf : 0;
+        if (hi == -CUDART_INF_F || !(temp > 0.0f)) {
+            u64 first = (u64) kAny;                      // nothing to draw, or the first index of the largest
+            if (hi > -CUDART_INF_F)
+                for (int i = me; i < v && first == (u64) kAny; i += all)
+                    if (to_f32(row[i]) == hi) first = (u64) i;
+            first = join_all(first, [](u64 x, u64 y) { return min(x, y); });
+            st.flags |= kGreedy;
+            st.hi = st.from = st.cut = st.flags & kInf ? 0.0f : hi;
+            st.last = (int) first;
+            st.total = first == (u64) kAny ? 0ull : (u64) kOne;
+            if (first != (u64) kAny && draft == (int) first) st.drafted = 1.0;
+            return st;
+        }
+        if (st.flags & kInf) hi = 0.0f;
+        const Row r = row_of(hi, (double) temp);
+        st.hi = hi;
+        st.from = r.base;
+        st.cut = -CUDART_INF_F;
+        st.total = 1;
+        if (!with_sum) return st;
+        u64 sum = 0;
+        for (int i = me; i - lane < v; i += 8 * all) {   // eight loads on their way
+            float x[8];
+            double onto = kZero;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = i + j * all < v ? seen(to_f32(row[i + j * all]), st.flags) : -CUDART_INF_F;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const double w = weight_warp(x[j], r, mine, onto);
+                if (x[j] >= r.base) onto = w;
+            }
+            sum += whole(onto);
+        }
+        st.total = join_all(sum, [](u64 x, u64 y) { return x + y; });
+        if (draft >= 0 && draft < v) st.drafted = draft_weight(seen(to_f32(row[draft]), st.flags), draft, st, r, (double) temp, 0.0f);
+        return st;
+    };
+    auto less = [&](const RowStat & p, const RowStat * q, int j) {   // u q(d) < p(d)
+        const double pd = p.total ? p.drafted / ((double) p.total * (1.0 / kOne)) : 0.0;
+        const double qd = q ? (q->total ? q->drafted / ((double) q->total * (1.0 / kOne)) : 0.0) : drafts[j] >= 0 && drafts[j] < v ? 1.0 : 0.0;
+        return (double) number_of(u[j]) * qd < pd;
+    };
+    // the test's answer: 1 accepted, -1 rejected, 0 open; the sums' errors as for quick_part, of slices over 512 threads
+    auto told = [&](int j) {
+        const double sp = ps[j].drafted, sq = a.draft_logits ? qs[j].drafted : 1.0;
+        if (!(sp < 0x1p24 && sq < 0x1p24)) return 0;
+        const double edge = 0x1p-23 * (double) (16.0f + 2.78f * (2.0f * log2f((float) v) + log2f((float) sp) + log2f((float) sq)) +
+                                                2.0f * ((float) v * (1.0f / (4.0f * kDrawThreads)) + 24.0f + 9.0f));
+        const double l = (double) number_of(u[j]) * sp;
+        return l * (1.0 + edge) < sq ? 1 : l > sq * (1.0 + edge) ? -1 : 0;
+    };
+    auto logprob_at = [&](int j, float x) { if (a.logprobs) a.logprobs[seq * (d + 1) + j] = x; };
+    RowStat p, q;
+    int first = 0;
+    for (;;) {
+        // the first from `first` on that is not accepted
+        for (int j = first + tid; j < n; j += kDrawThreads)
+            if (FILTERS ? !less(ps[j], a.draft_logits ? qs + j : nullptr, j) : told(j) < 1) atomicMin(&s_first, j);
+        __syncthreads();
+        const int until = s_first;
+        if (rank == 0) {
+            for (int j = first + tid; j < until; j += kDrawThreads) {
+                a.tokens[seq * (d + 1) + j] = drafts[j];
+                logprob_at(j, FILTERS ? (float) (log(ps[j].drafted) - log((double) ps[j].total * (1.0 / kOne))) : -logf((float) ps[j].drafted));
+            }
+        }
+        first = until;
+        if (FILTERS) {
+            p = ps[first];
+            if (first < n && a.draft_logits) q = qs[first];
+            break;
+        }
+        const bool rejected = first < n && told(first) < 0;
+        p = stat_of(target_row(first), first < n ? drafts[first] : -1, first < n && (a.draft_logits || !rejected));
+        if (first == n) break;
+        if (a.draft_logits) q = stat_of(draft_row(first), drafts[first], true);
+        if (rejected || !less(p, a.draft_logits ? &q : nullptr, first)) break;
+        if (rank == 0 && tid == 0) {
+            a.tokens[seq * (d + 1) + first] = drafts[first];
+            logprob_at(first, (float) (log(p.drafted) - log((double) p.total * (1.0 / kOne))));
+        }
+        ++first;
+        __syncthreads();
+        if (tid == 0) s_first = n;
+        __syncthreads();
+    }
     if (rank == 0) {
-        for (int j = tid; j <= d; j += kDrawThreads) {
-            if (j == first) continue;
-            const bool ok = j < first;
-            a.tokens[seq * (d + 1) + j] = ok ? drafts[j] : -1;
-            if (a.logprobs)
-                a.logprobs[seq * (d + 1) + j] = ok ? (float) (log(ps[j].drafted) - log((double) ps[j].total * (1.0 / kOne))) : -CUDART_INF_F;
+        for (int j = first + 1 + tid; j <= d; j += kDrawThreads) {
+            a.tokens[seq * (d + 1) + j] = -1;
+            logprob_at(j, -CUDART_INF_F);
         }
         if (tid == 0) a.accepted[seq] = first;
     }
-    const RowStat p = ps[first];
     if (p.total == 0) {                                  // nothing to draw from
         if (rank == 0 && tid == 0) {
             a.tokens[seq * (d + 1) + first] = -1;
-            if (a.logprobs) a.logprobs[seq * (d + 1) + first] = -CUDART_INF_F;
+            logprob_at(first, -CUDART_INF_F);
         }
+        if (CL && !FILTERS) cg::this_cluster().sync();   // exchanges are read
         return;
     }
     DrawRow<T> pr, qr;
-    pr.set(static_cast<const T *>(a.logits) + (seq * (d + 1) + first) * a.row_stride, p, temp);
-    enum { kAll, kLess, kWithout };                      // from p, from what p has more than q, from p without the draft
+    pr.set(target_row(first), p, temp);
     int mode = kAll, out = -1;
     double sp = 0.0, sq = 0.0;
     if (first < n) {
         if (a.draft_logits) {
-            const RowStat q = qs[first];
             if (q.total) {
                 mode = kLess;
-                qr.set(static_cast<const T *>(a.draft_logits) + (seq * d + first) * a.draft_stride, q, temp);
+                qr.set(draft_row(first), q, temp);
                 sp = kShare / (double) p.total;
                 sq = kShare / (double) q.total;
             }
@@ -1000,29 +1147,39 @@ __global__ void __launch_bounds__(kDrawThreads) verify_draw_kernel(const Plan pl
             mode = kWithout;
         }
     }
-    // what token i weighs in the draw; the whole warp calls, lanes past `end` for nothing
-    auto weigh = [&](int i, int end) -> u64 {
-        const bool in = i < end;
-        double w = pr.weight(in ? to_f32(pr.at[i]) : -CUDART_INF_F, i, mine);
+    // what token i, of logits x and y in the two rows, weighs in the draw, a whole number; the whole warp calls
+    auto weigh = [&](int i, float x, float y) {
+        double w = pr.weight(x, i, mine);
         if (mode == kLess) {
             // the two products rounded alike: equal rows leave nothing
-            const double less = qr.weight(in ? to_f32(qr.at[i]) : -CUDART_INF_F, i, mine);
-            w = fmax((__dmul_rn(w, sp) - __dmul_rn(less, sq) + kMagic) - kMagic, 0.0);
+            w = fmax((__dmul_rn(w, sp) - __dmul_rn(qr.weight(y, i, mine), sq) + kMagic) - kMagic, 0.0);
         }
-        if (mode == kWithout && i == out) w = 0.0;
-        return in ? (u64) w : 0ull;
+        return mode == kWithout && i == out ? 0.0 : w;
     };
-    auto stretch = [&](int begin, int end) {             // its sum, over a warp
+    auto target_at = [&](int i, int end) { return i < end ? to_f32(pr.at[i]) : -CUDART_INF_F; };
+    auto draft_at = [&](int i, int end) { return mode == kLess && i < end ? to_f32(qr.at[i]) : -CUDART_INF_F; };
+    auto stretch = [&](int begin, int end) {             // its sum, over a warp: eight loads of each row on their way
         u64 s = 0;
-#pragma unroll 4
-        for (int i = begin; i < end; i += 32) s += weigh(i + lane, end);
+        for (int b = begin; b < end; b += 256) {
+            const int i = b + lane;
+            float x[8], y[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = target_at(i + 32 * j, end);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) y[j] = draft_at(i + 32 * j, end);
+            double run = 0.0;                            // eight weights of 2^43, or shares of 2^50 in all
+#pragma unroll
+            for (int j = 0; j < 8; ++j) run += weigh(i + 32 * j, x[j], y[j]);
+            s += (u64) run;
+        }
         return warp_sum(s);
     };
     const int part = ((v + kDrawWarps * blocks - 1) / (kDrawWarps * blocks) + 31) & ~31;
     const int begin = min((rank * kDrawWarps + warp) * part, v), end = min(begin + part, v);
     u64 total = 0, before = 0;
-    for (int phase = 0;; ++phase) {
+    for (;;) {
         const u64 s = stretch(begin, end);
+        __syncthreads();
         if (lane == 0) sums[warp] = s;
         __syncthreads();
         u64 own = 0;
@@ -1042,12 +1199,14 @@ __global__ void __launch_bounds__(kDrawThreads) verify_draw_kernel(const Plan pl
                 if (b < rank) before += o;
                 total += o;
             }
+            phase ^= 1;
         }
         if (total > 0 || mode == kAll) break;
         mode = kAll;                                     // q has all that p has: only a draft that q never draws ends here
-        __syncthreads();
     }
     const u64 t = place_of(u[d], total);
+    u64 whole_row = p.total;
+    if (!FILTERS && mode != kLess) whole_row = total + (mode == kWithout && out >= 0 && out < v ? weight_one(seen(to_f32(pr.at[out]), pr.flags), pr.r) : 0ull);
     if (tid == 0) s_warp = -1;
     __syncthreads();
     if (lane == 0 && before <= t && t < before + sums[warp]) {
@@ -1070,15 +1229,13 @@ __global__ void __launch_bounds__(kDrawThreads) verify_draw_kernel(const Plan pl
     for (int i = 0; i < warp; ++i) before += sums[i];
     if (!(before <= t && t < before + s)) return;
     for (int i = b1; i < e1; i += 32) {
-        const u64 w = weigh(i + lane, e1);
+        const u64 w = (u64) weigh(i + lane, target_at(i + lane, e1), draft_at(i + lane, e1));
         const u64 x = before + warp_scan(w, lane);
         if (x - w <= t && t < x) {
             const float l = seen(to_f32(pr.at[i + lane]), pr.flags);
             a.tokens[seq * (d + 1) + first] = i + lane;
             const double tt = pr.flags & kGreedy ? 1.0 : (double) temp;
-            if (a.logprobs)
-                a.logprobs[seq * (d + 1) + first] =
-                    (float) ((l == p.hi ? 0.0 : ((double) l - (double) p.hi) / tt) - log((double) p.total * (1.0 / kOne)));
+            logprob_at(first, (float) ((l == p.hi ? 0.0 : ((double) l - (double) p.hi) / tt) - log((double) whole_row * (1.0 / kOne))));
         }
         before = __shfl_sync(kFull, x, 31);
         if (before > t) break;
@@ -1087,9 +1244,9 @@ __global__ void __launch_bounds__(kDrawThreads) verify_draw_kernel(const Plan pl
 
 // ---- launches -----------------------------------------------------------------------
 
-template <class T, int NT, bool FILTERS, bool CL, bool RES>
+template <class T, int NT, bool CL, bool RES>
 cudaError_t launch_rows(const Plan & p, long long rows, int blocks, int slice, int row_floats, size_t smem, cudaStream_t s) {
-    auto kernel = verify_rows_kernel<T, NT, FILTERS, CL, RES>;
+    auto kernel = verify_rows_kernel<T, NT, CL, RES>;
     static unsigned long long set;                               // devices on which the limit is raised
     int device = 0;
     cudaError_t e = cudaGetDevice(&device);
@@ -1115,54 +1272,78 @@ cudaError_t launch_rows(const Plan & p, long long rows, int blocks, int slice, i
     return cudaLaunchKernelEx(&cfg, kernel, p, slice, row_floats);
 }
 
-template <class T, bool FILTERS>
+template <class T>
 cudaError_t rows_cluster(const Plan & p, long long rows, int blocks, cudaStream_t s) {
     // slices of whole 16 bytes, so that every slice is aligned as its row is
     const int slice = ((p.a.vocab + blocks - 1) / blocks + 31) / 32 * 32;
     int row_floats;
-    const size_t smem = team_bytes<1024, FILTERS>(slice, row_floats);
-    if (smem <= kSmemCap) return launch_rows<T, 1024, FILTERS, true, true>(p, rows, blocks, slice, row_floats, smem, s);
-    return launch_rows<T, 1024, FILTERS, true, false>(p, rows, blocks, slice, 0, smem - (size_t) row_floats * 4, s);
+    const size_t smem = team_bytes<1024, true>(slice, row_floats);
+    if (smem <= kSmemCap) return launch_rows<T, 1024, true, true>(p, rows, blocks, slice, row_floats, smem, s);
+    return launch_rows<T, 1024, true, false>(p, rows, blocks, slice, 0, smem - (size_t) row_floats * 4, s);
 }
 
 // Blocks by rows and vocabulary as in pk_sample.
-template <class T, bool FILTERS>
+template <class T>
 cudaError_t rows_dispatch(const Plan & p, cudaStream_t s) {
     const int v = p.a.vocab;
     const long long rows = p.a.sequences * (p.a.max_drafts + 1) + (p.a.draft_logits ? p.a.sequences * p.a.max_drafts : 0);
     int blocks = 1;
     while (blocks < kMaxCluster && rows * blocks * 2 <= 148) blocks *= 2;
     while (blocks < kMaxCluster && (size_t) (v / blocks) * 4 > 200 * 1024) blocks *= 2;
-    if (blocks > 1) return rows_cluster<T, FILTERS>(p, rows, blocks, s);
+    if (blocks > 1) return rows_cluster<T>(p, rows, blocks, s);
     int row_floats;
-    const size_t smem = team_bytes<512, FILTERS>(v, row_floats);
-    return launch_rows<T, 512, FILTERS, false, true>(p, rows, 1, v, row_floats, smem, s);
+    const size_t smem = team_bytes<512, true>(v, row_floats);
+    return launch_rows<T, 512, false, true>(p, rows, 1, v, row_floats, smem, s);
 }
 
-template <class T, bool CL>
-cudaError_t launch_draw(const Plan & p, int blocks, cudaStream_t s) {
+template <class T, bool CL, bool FILTERS>
+cudaError_t launch_draw(const Plan & p, int blocks, bool behind, cudaStream_t s) {   // behind: a kernel that lets it start
     cudaLaunchConfig_t cfg{};
     cudaLaunchAttribute at[2];
     cfg.gridDim = dim3((unsigned) (p.a.sequences * blocks));
     cfg.blockDim = dim3(kDrawThreads);
     cfg.stream = s;
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
-    at[1].id = cudaLaunchAttributeClusterDimension;
-    at[1].val.clusterDim.x = (unsigned) blocks;
-    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = (unsigned) blocks;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
-    cfg.numAttrs = CL ? 2 : 1;
-    return cudaLaunchKernelEx(&cfg, verify_draw_kernel<T, CL>, p);
+    cfg.numAttrs = behind ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, verify_draw_kernel<T, CL, FILTERS>, p);
+}
+
+template <class T> cudaError_t launch_sums(const Plan & p, cudaStream_t s) {
+    const long long rows = p.a.sequences * p.a.max_drafts * (p.a.draft_logits ? 2 : 1);
+    int blocks = 1;
+    while (blocks < kMaxCluster && rows * blocks * 2 <= 2 * 148) blocks *= 2;
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute at[1];
+    cfg.gridDim = dim3((unsigned) (rows * blocks));
+    cfg.blockDim = dim3(kDrawThreads);
+    cfg.stream = s;
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = (unsigned) blocks;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = blocks > 1 ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, blocks > 1 ? verify_sums_kernel<T, true> : verify_sums_kernel<T, false>, p);
+}
+
+template <class T, bool FILTERS> cudaError_t long_rows(const Plan & p, cudaStream_t s) {
+    cudaError_t e;
+    const bool rows = FILTERS || p.a.max_drafts > 0;             // the draw's own rows need no test
+    if constexpr (FILTERS) e = rows_dispatch<T>(p, s);
+    else e = rows ? launch_sums<T>(p, s) : cudaSuccess;
+    if (e != cudaSuccess) return e;
+    int blocks = 1;
+    while (blocks < kMaxCluster && p.a.sequences * blocks * 2 <= 148) blocks *= 2;
+    return blocks > 1 ? launch_draw<T, true, FILTERS>(p, blocks, rows, s) : launch_draw<T, false, FILTERS>(p, 1, rows, s);
 }
 
 template <class T> cudaError_t dispatch(const Plan & p, bool filters, cudaStream_t s) {
     if (resident(p.a.vocab, p.a.draft_logits != nullptr)) return filters ? sequences_dispatch<T, true>(p.a, s) : sequences_dispatch<T, false>(p.a, s);
-    const cudaError_t e = filters ? rows_dispatch<T, true>(p, s) : rows_dispatch<T, false>(p, s);
-    if (e != cudaSuccess) return e;
-    int blocks = 1;
-    while (blocks < kMaxCluster && p.a.sequences * blocks * 2 <= 148) blocks *= 2;
-    return blocks > 1 ? launch_draw<T, true>(p, blocks, s) : launch_draw<T, false>(p, 1, s);
+    return filters ? long_rows<T, true>(p, s) : long_rows<T, false>(p, s);
 }
 
 // Rows of a call, -1 for sizes that are refused.

@@ -286,7 +286,7 @@ def test_large_vocabularies(built, s, d, v, kw):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("certain", [False, True])
-@pytest.mark.parametrize("s,d,v", [(64, 4, 500), (30, 6, 8193)])
+@pytest.mark.parametrize("s,d,v", [(64, 4, 500), (30, 6, 8193), (12, 3, 30000)])
 def test_settings_and_counts_of_each_sequence(built, s, d, v, certain):
     """Settings, numbers of drafts (out of range among them) and masks by sequence; what lies behind the drafts is
     not read, nor are the drafts behind the first rejection needed."""
@@ -311,7 +311,7 @@ def test_settings_and_counts_of_each_sequence(built, s, d, v, certain):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("kw", SETTINGS)
-@pytest.mark.parametrize("v", [40, 1500, 9000])
+@pytest.mark.parametrize("v", [40, 1500, 9000, 30000])
 def test_special_values(built, v, kw):
     """Infinities, NaN and rows without any logit, in the target and in the draft; drafts that no one drew."""
     rng = np.random.default_rng(v)
@@ -358,7 +358,7 @@ def test_cut_inside_equal_logits(built, v, kw):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("kw", [{}, dict(temperature=0.8, top_k=50, top_p=0.9, min_p=0.001)])
-@pytest.mark.parametrize("s,v", [(3, 8193), (2000, 1025), (2, 131072)])
+@pytest.mark.parametrize("s,v", [(3, 8193), (2000, 1025), (2, 131072), (200, 24000)])
 def test_without_drafts_it_is_sample(built, s, v, kw):
     import torch
     rng = np.random.default_rng(s)
@@ -399,6 +399,26 @@ def test_tokens_are_distributed_as_the_target(built, kw):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("s,d,v", [(64, 4, 500), (30, 6, 8193), (12, 3, 30000)])
+def test_temperatures_and_counts_without_filters(built, s, d, v):
+    """Temperatures, numbers of drafts and masks by sequence, with nothing else to cut."""
+    rng = np.random.default_rng(v + 1)
+    kw = dict(temperature=np.where(rng.random(s) < 0.15, 0.0, 0.3 + 1.2 * rng.random(s)))
+    p, q, drafts, u = make(rng, s, d, v)
+    mask = rng.random((s, 1, v)) < 0.3
+    mask[rng.random(s) < 0.1] = True
+    p, q = np.where(mask, -np.inf, p), np.where(mask, -np.inf, q)
+    counts = rng.integers(-2, d + 3, s)
+    drafts[rng.random((s, d)) < 0.1] = -1
+    u[:, :d] *= rng.random((s, 1))                        # many accepted
+    for i in range(s):
+        n = max(0, min(int(counts[i]), d))
+        p[i, n + 1:], q[i, n:], drafts[i, n:] = np.nan, np.inf, 1 << 30
+    check(Call(built, p, q, drafts, u, counts=counts, **kw).run(), drafts, u, counts, **kw)
+    check(Call(built, p, None, drafts, u, counts=counts, **kw).run(), drafts, u, counts, **kw)
+
+
+@pytest.mark.gpu
 def test_many_drafts(built):
     """More drafts than a block has threads, most of them accepted."""
     rng = np.random.default_rng(2)
@@ -408,12 +428,12 @@ def test_many_drafts(built):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kw", [dict(temperature=0.8, top_p=0.9), dict(temperature=0.8)])
 @pytest.mark.parametrize("v", [500, 8193, 40000])
-def test_captured_and_replayed(built, v):
+def test_captured_and_replayed(built, v, kw):
     """Two graphs with workspaces of their own replayed on two streams, with new inputs each time."""
     import torch
     rng = np.random.default_rng(v)
-    kw = dict(temperature=0.8, top_p=0.9)
     first = [make(rng, 4, 3, v, **kw) for _ in range(2)]
     calls = [Call(built, *x, **kw) for x in first]
     graphs, streams = [torch.cuda.CUDAGraph() for _ in calls], [torch.cuda.Stream() for _ in calls]
