@@ -439,9 +439,9 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant_
                 unsigned v[32];
                 tmem_load32(acc + c, v);
                 asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                if (lap && i == half) {
+                if (lap ? i == half : i + 2 >= chunks) {         // what the next products wait for is read
                     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                    if (lane == 0) mbar_arrive_at(&S.acc_empty[buf], 0);
+                    if (lane == 0) mbar_arrive_at_relaxed(&S.acc_empty[buf], 0);
                 }
                 if (n < N) {
                     T * o = y + (m0 + c) * ldy + n;
@@ -455,10 +455,6 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant_
                             if (r < rows) put(o, __uint_as_float(v[r]) + bv);
                     }
                 }
-            }
-            if (!lap) {
-                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                if (lane == 0) mbar_arrive_at(&S.acc_empty[buf], 0);
             }
         }
     }

@@ -187,6 +187,12 @@ __device__ __forceinline__ void mbar_arrive_at(unsigned long long * b, unsigned 
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" :: "r"(mbar_at(b, rank)) : "memory");
 }
 
+// The same without releasing anything: for a thread that has read tensor memory (tcgen05.wait::ld) and tells so. Releasing
+// would first wait for its global stores.
+__device__ __forceinline__ void mbar_arrive_at_relaxed(unsigned long long * b, unsigned rank) {
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" :: "r"(mbar_at(b, rank)) : "memory");
+}
+
 __device__ __forceinline__ void umma_commit(unsigned long long * b) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];"
                  :: "r"(smem_u32(b)) : "memory");
