@@ -648,7 +648,10 @@ PK_API pk_status pk_sample(int device, const pk_sample_args * args, void * strea
  * T <= 0 or NaN: p_j is 1 for the first of the largest logits. A target's row without any
  * logit above -infinity accepts nothing and gives token -1. u is clamped to [0, 1), NaN to 0.
  * Weights count as in pk_sample, which tells the same token from a row as a call here without
- * drafts; differences p - q below 2^-43 of the larger may be lost. */
+ * drafts; differences p - q below 2^-43 of the larger may be lost. Where 32-bit sums with a proven
+ * bound tell the answer they are used instead; log-probabilities are then within 2^-15 (the largest
+ * vocabularies; 2^-16 up to 16384), mostly 2^-22, of their value, and may differ within that with the
+ * number of sequences. */
 #define PK_VERIFY_MAX_DRAFTS 65535
 
 typedef struct pk_verify_args {

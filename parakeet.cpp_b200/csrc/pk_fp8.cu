@@ -97,7 +97,8 @@ template <int LG> __device__ __forceinline__ uint2 quantize8(const Eight<__half>
 // A warp's 256 values of a row, two blocks: eight per lane. Where a row goes on, the next 256 follow in the
 // same warp, gridDim.y segments further on; several loads are in flight before the first is used. SHORT, for rows
 // of up to 256 values: 2^gs lanes a row, and the next rows instead of the next segments.
-// ATOMS: scales in the product's layout.
+// ATOMS: scales in the product's layout. Bound: HBM from f32 (66044 x 1024: 44 us, 270 MB read), instructions from half precision
+// (66043 x 1000 bf16: 37 us for 132 MB read and 66 written, of which the codes stay in L2).
 template <class T, bool VEC, bool ATOMS, bool SHORT>
 __global__ void __launch_bounds__(kQThreads) fp8_quantize_kernel(const T * __restrict__ x, long long rows, int K, long long ldx, int gs,
                                                                  unsigned char * __restrict__ codes,
@@ -171,7 +172,7 @@ template <class T> __device__ __forceinline__ void codes_to_values(uint2 q, unsi
     }
 }
 
-// The value of each code, eight a lane, rows and lanes as in the quantisation.
+// The value of each code, eight a lane, rows and lanes as in the quantisation. Bound: HBM, writing y (66043 x 1000 bf16: 35 us).
 template <class T, bool VEC, bool SHORT>
 __global__ void __launch_bounds__(kQThreads) fp8_dequantize_kernel(const unsigned char * __restrict__ codes,
                                                                    const unsigned char * __restrict__ scales, long long rows,
@@ -305,7 +306,10 @@ template <class T> __device__ __forceinline__ void put(T * y, float v) { *y = fr
 // cycles of products, at 128 24 KB for 256: the L2 gives an SM some 50 bytes a cycle, so wide tiles pay. Warp 0
 // loads, warp 1 of the first block issues, warps from 4 on empty the accumulators, of which there are two. Two of
 // 256 columns and the scales' 32 are more than there is: they overlap by 32 columns, which are emptied first.
-// Both blocks' loads arrive on the first one's barriers.
+// Both blocks' loads arrive on the first one's barriers. Measured, replayed from a graph, quantisation included: 8192 x 4096 by
+// 8192 bf16 212 us (64 to 192 columns: 540, 295, 242), of which the product 190, 2.9 PFLOP/s, its operands at some 45 bytes a
+// cycle and SM from L2; 66044 x 1024 by 640 f32 110 us, the product 65 of them, for 169 MB of y and 411 MB of operands from L2;
+// with sixteen epilogue warps in place of eight the same within 1 %.
 constexpr int kPStages = 6;
 constexpr int kPEpi = 8;                                 // warps of the epilogue
 constexpr int kPThreads = 32 * (4 + kPEpi);
@@ -660,7 +664,7 @@ fp8_split_kernel(const TX * __restrict__ x, long long ldx, long long M, int K, c
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const unsigned acc = tmem + ((unsigned) (q * 32) << 16);
             const float bv = bias && n < N ? __ldg(bias + n) : 0.0f;
-            const int each = p.bm / p.split;             // rows that a block of the cluster adds up
+            const int lg = 31 - __clz(p.bm / p.split);   // of the rows that a block of the cluster adds up, a power of two
             for (int c = 0; c < rows; c += 16) {
                 unsigned v[16];
                 tmem_load16(acc + c, v);
@@ -676,10 +680,9 @@ fp8_split_kernel(const TX * __restrict__ x, long long ldx, long long M, int K, c
 #pragma unroll
                     for (int r = 0; r < 16; ++r) {
                         if (c + r >= rows) break;
-                        const int owner = (c + r) / each;
+                        const int owner = (c + r) >> lg, place = (rank << lg) + c + r - (owner << lg);
                         unsigned at;
-                        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;"
-                                     : "=r"(at) : "r"(smem_u32(sums + (size_t) (rank * each + c + r - owner * each) * kTN + q * 32 + lane)), "r"(owner));
+                        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(sums + place * kTN + q * 32 + lane)), "r"(owner));
                         asm volatile("st.shared::cluster.u32 [%0], %1;" :: "r"(at), "r"(v[r]) : "memory");
                     }
                 }
@@ -776,7 +779,8 @@ int split_of(long long tiles, int nb) {
     return s;
 }
 
-// Rows that the cluster kernel quantises itself: none of its blocks more than these values.
+// Rows that the cluster kernel quantises itself, none of its blocks more than these values (a row of 640 by 8198, replayed from a
+// graph: 6.6 us, 8.7 with a launch for each).
 constexpr long long kFusedRows = 32, kFusedValues = 32768;
 bool plan_fused(const pk_fp8 * w, long long M, SplitPlan & p) {
     if (M > kFusedRows) return false;
@@ -786,10 +790,12 @@ bool plan_fused(const pk_fp8 * w, long long M, SplitPlan & p) {
     return fit_split(p, w->K, true);
 }
 
-// Few tiles, codes from the row kernel.
+// Few tiles and a long K, codes from the row kernel. Replayed from a graph, this way and in pairs of blocks: 64 rows of 4096 by
+// 1024 11.2 us and 14.5, 128 13.8 and 14.7, 40 of 4096 by 4096 13.2 and 14.7; 64 of 2048 by 4096 11.3 and 10.3, 64 of 640 by 8198
+// 11.1 and 7.7, 128 of 1024 by 4096 12.9 and 8.3.
 bool plan_split(const pk_fp8 * w, long long M, SplitPlan & p) {
     const long long nt = (w->N + kTN - 1) / kTN;
-    if (M > 128) return false;
+    if (M > 128 || w->nb < 26) return false;
     p.bm = M <= 32 ? 32 : M <= 64 ? 64 : 128;
     const long long tiles = nt * ((M + p.bm - 1) / p.bm);
     if (tiles > 148) return false;

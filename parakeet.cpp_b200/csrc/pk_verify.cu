@@ -13,6 +13,11 @@
 // tell. Draws always go by whole numbers, so that sums are exact whatever their order.
 //
 // Longer rows take two kernels, see below.
+//
+// Measured (calls among others, Python's included): 1024 sequences of four drafts by 8193 f32 logits, temperature alone, 105 us,
+// of which the rows up to the first rejections are 192 MB, 29 us; most of the rest is the latency of a block's steps, two blocks
+// of 512 threads an SM. 256 of eight by 8193 bf16, top-p and min-p, 135 us: the cuts of two rows a position, as long as in
+// pk_sample. One of four, top-k and top-p, 22 us, the chain of a cut and a draw.
 
 #include "pk_draw.cuh"
 
@@ -649,7 +654,7 @@ verify_sequence_kernel(const pk_verify_args a, int rows_each, int row_floats) {
                 }
                 group.sync();
                 const int who = S.group.found;
-                if (group.tid < 32) {
+                if (who >= 0 && group.tid < 32) {
                     // the run again, 32 elements at a time
                     const int e = min((who + 1) * g_len, v);
                     u64 run = S.group.found_before;
@@ -735,7 +740,8 @@ template <class T, bool FILTERS> cudaError_t sequences_dispatch(const pk_verify_
 
 // ---- long rows ---------------------------------------------------------------------
 //
-// Two kernels. The first takes a block or cluster per row, all rows at once, and leaves what the test needs of it; with filters
+// Two kernels (4 sequences of eight looked-up drafts by 131072 bf16: 27.5 us, two launches and the draw's passes over one row,
+// 16,384 logits a block). The first takes a block or cluster per row, all rows at once, and leaves what the test needs of it; with filters
 // as pk_sample does. The second takes a block or cluster per sequence: it tests all drafts at once and draws from the one row, or
 // two, that the first rejection names, reading them again.
 
