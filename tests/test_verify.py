@@ -419,6 +419,19 @@ def test_temperatures_and_counts_without_filters(built, s, d, v):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("temperature", [np.inf, 1e30, 300.0, 1e-3, 1e-20, 1e-38, -1.0, np.nan])
+@pytest.mark.parametrize("kw", [{}, dict(top_p=0.9), dict(min_p=0.3)])
+def test_extreme_temperatures(built, temperature, kw):
+    rng = np.random.default_rng(6)
+    for s, d, v in ((5, 2, 300), (2, 2, 7000)):
+        p, q, drafts, u = make(rng, s, d, v, gap=0.3)
+        if temperature > 100:                            # equal weights: any cut falls among them, by the logits' order
+            drafts = rng.integers(0, v, (s, d)).astype(np.int32)
+        check(Call(built, p, q, drafts, u, temperature=temperature, **kw).run(), drafts, u, temperature=temperature, **kw)
+        check(Call(built, p, None, drafts, u, temperature=temperature, **kw).run(), drafts, u, temperature=temperature, **kw)
+
+
+@pytest.mark.gpu
 def test_many_drafts(built):
     """More drafts than a block has threads, most of them accepted."""
     rng = np.random.default_rng(2)
