@@ -8,9 +8,10 @@
 // Vocabularies whose two rows fit a block's shared memory take one kernel: a block (a warp for short rows) goes over
 // a sequence's positions and stops at the first rejection, whose rows it then holds; what lies behind is never read.
 // With few sequences the blocks of a cluster share the positions out and tell each other the outcomes. The two rows
-// of a position go to two teams of threads. What a test needs of a row is its largest logit, its cut, the sum of its
-// weights and the draft's weight: the sum by f32 with a proven bound, by pk_sample's whole numbers where that cannot
-// tell. Draws always go by whole numbers, so that sums are exact whatever their order.
+// of a position go to two teams of threads. Without filters a draft is first tested in one pass over its rows. Otherwise
+// what a test needs of a row is its largest logit, its cut, the sum of its weights and the draft's weight. Sums, of tests
+// and of draws, go by f32 with a proven bound, and by pk_sample's whole numbers, exact whatever their order, where that
+// leaves the answer open.
 //
 // Longer rows take two kernels, see below.
 //
