@@ -926,10 +926,12 @@ template <class T> struct DrawRow {
         last = s.last;
         r = row_of(s.hi, flags & kGreedy ? 1.0 : (double) temp);
     }
+    // Whether token i is kept, its logit as `seen` has it.
+    __device__ __forceinline__ bool keeps(float v, int i) const { return v >= from && (v > cut || i <= last); }
     // Weight of token i with logit v (times 2^43, a whole number); the whole warp calls.
     __device__ __forceinline__ double weight(float v, int i, double mine) const {
         v = seen(v, flags);
-        const bool keep = v >= from && (v > cut || i <= last);
+        const bool keep = keeps(v, i);
         const double w = weight_warp(keep ? v : (float) r.top, r, mine) - kZero;
         return keep ? w : 0.0;
     }
@@ -1213,7 +1215,15 @@ __global__ void __launch_bounds__(kDrawThreads) verify_draw_kernel(const Plan pl
     }
     const u64 t = place_of(u[d], total);
     u64 whole_row = p.total;
-    if (!FILTERS && mode != kLess) whole_row = total + (mode == kWithout && out >= 0 && out < v ? weight_one(seen(to_f32(pr.at[out]), pr.flags), pr.r) : 0ull);
+    if (!FILTERS && mode != kLess) {
+        // the row's weights: those of the draw, and the draft's, which the draw leaves out, if the row keeps it (a greedy row keeps
+        // the first of its largest alone)
+        whole_row = total;
+        if (mode == kWithout && out >= 0 && out < v) {
+            const float l = seen(to_f32(pr.at[out]), pr.flags);
+            if (pr.keeps(l, out)) whole_row += weight_one(l, pr.r);
+        }
+    }
     if (tid == 0) s_warp = -1;
     __syncthreads();
     if (lane == 0 && before <= t && t < before + sums[warp]) {

@@ -552,3 +552,89 @@ def test_draft_and_verify_through_both_heads(built, kw):
         assert tok[i].tolist() == want + [-1] * (d + 1 - len(want)) or near <= (v + 4) * 2.0 ** -41
         assert acc[i] == len(want) - 1 or near <= (v + 4) * 2.0 ** -41
     assert 0 < acc.sum() and (acc < d).any()
+
+
+# Rows too long for a block's shared memory: one of up to 45056 logits fits, or two of 22528. v is above both.
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("certain", [True, False])
+@pytest.mark.parametrize("kw", [dict(temperature=0.0), dict(temperature=-1.0, top_p=0.9), dict(temperature=np.nan, top_k=5)])
+@pytest.mark.parametrize("v", [45057, 131072])
+def test_greedy_long_rows(built, v, kw, certain):
+    """T <= 0: the first of the largest alone is kept, so its log-probability is 0 whatever draft was rejected for it, one just
+    below the largest, a later one as large or a second +infinity among them."""
+    rng = np.random.default_rng(v)
+    s, d = 8, 2
+    p, q, drafts, u = make(rng, s, d, v, certain=certain, **kw)
+    top = p.argmax(2)
+    for i, off in enumerate((0.5, 0.01, 20.0)):
+        drafts[i, 0] = (top[i, 0] + 7) % v
+        p[i, 0, drafts[i, 0]] = p[i, 0, top[i, 0]] - off
+    p[3, 0, [11, 40]], drafts[3, 0] = 50.0, 40                   # a later one of the largest
+    p[4, 0, [9, 30, v - 1]], drafts[4, 0] = np.inf, v - 1        # a second +infinity
+    drafts[5, :], drafts[6, 0], drafts[6, 1] = top[5, :d], top[6, 0], (top[6, 1] + 1) % v
+    p[7, 0], drafts[7] = 0.0, [v // 2, 0]                        # all alike
+    call = Call(built, p, q, drafts, u, **kw).run()
+    check(call, drafts, u, **kw)
+    tok, acc, lp = call.answer()
+    assert (lp[np.arange(s), acc] == 0).all()
+    if certain:
+        assert acc.tolist()[:5] == [0] * 5 and acc[5] == 2 and acc[6] == 1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kw", [{}, dict(temperature=0.6), dict(temperature=0.7, top_k=20), dict(top_p=0.9), dict(temperature=1.3, top_k=50, top_p=0.95, min_p=0.01)])
+@pytest.mark.parametrize("s,d,v,dtype", [(3, 3, 50001, "f32"), (1, 8, 131072, "bf16"), (80, 1, 45057, "f16"), (200, 1, 45057, "f32"), (2, 1, 524288, "f32")])
+def test_long_rows_with_drafts_that_were_looked_up(built, s, d, v, dtype, kw):
+    p, q, drafts, u = make(np.random.default_rng(v + s), s, d, v, certain=True, **kw)
+    drafts[::3, 0] = (drafts[::3, 0] + 1) % v                    # unlikely ones among them
+    check(Call(built, p, q, drafts, u, dtype=dtype, **kw).run(), drafts, u, excused=1, **kw)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("certain", [True, False])
+@pytest.mark.parametrize("filters", [False, True])
+def test_long_rows_with_settings_and_counts_of_each_sequence(built, filters, certain):
+    """As for short rows: settings (greedy ones among them), numbers of drafts and masks by sequence, drafts out of range."""
+    rng = np.random.default_rng(4)
+    s, d, v = 20, 3, 46001
+    kw = dict(temperature=np.where(rng.random(s) < 0.3, 0.0, 0.3 + 1.2 * rng.random(s)))
+    if filters:
+        kw.update(top_k=np.where(rng.random(s) < 0.4, 0, rng.integers(1, 100, s)), top_p=np.where(rng.random(s) < 0.4, 1.0, 0.4 + 0.6 * rng.random(s)),
+                  min_p=np.where(rng.random(s) < 0.6, 0.0, 0.1 * rng.random(s)))
+    p, q, drafts, u = make(rng, s, d, v, certain=certain)
+    mask = rng.random((s, 1, v)) < 0.3
+    mask[[4, 9]] = True
+    p = np.where(mask, -np.inf, p)
+    q = None if certain else np.where(mask, -np.inf, q)
+    counts = rng.integers(-2, d + 3, s)
+    drafts[rng.random((s, d)) < 0.1] = -1
+    for i in range(s):
+        n = max(0, min(int(counts[i]), d))
+        p[i, n + 1:], drafts[i, n:] = np.nan, 1 << 30
+        if not certain:
+            q[i, n:] = np.inf
+    check(Call(built, p, q, drafts, u, counts=counts, pad=3, shift=1, **kw).run(), drafts, u, counts, excused=1, **kw)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kw", SETTINGS)
+def test_long_rows_with_special_values(built, kw):
+    """Infinities, NaN, rows without any logit, equal logits and drafts that no one drew."""
+    v, s, d = 45601, 18, 2
+    rng = np.random.default_rng(v)
+    p, q, drafts, u = make(rng, s, d, v, **kw)
+    p[0, 0], q[1, 0], p[2, 2] = -np.inf, -np.inf, -np.inf
+    p[3, 0, 5], p[5, 0, [3, 9]] = np.inf, np.inf
+    q[4, 0, 7], q[5, 0, [9, 11]] = np.inf, np.inf
+    p[6, 0, 4], q[6, 0, 5] = np.nan, np.nan
+    p[7, 0], q[7, 0] = np.nan, np.nan
+    p[8], q[8] = np.finfo(np.float32).min, np.finfo(np.float32).min
+    p[9, :, : v - 1], q[9, :, : v - 1] = np.finfo(np.float32).min, np.finfo(np.float32).min
+    drafts[10], drafts[11], drafts[12], drafts[13] = -1, v, np.iinfo(np.int32).max, np.iinfo(np.int32).min
+    q[14] = p[14, :d]
+    u[14], u[15], u[16] = 1 - 2.0 ** -24, np.nan, 2.0
+    p[17] = np.round(p[17])                                              # cuts among equal logits
+    drafts[3, 0], drafts[5, 0] = 7, 9
+    check(Call(built, p, q, drafts, u, **kw).run(), drafts, u, excused=1, **kw)
+    check(Call(built, p, None, drafts, u, **kw).run(), drafts, u, excused=1, **kw)
