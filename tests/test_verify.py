@@ -638,3 +638,16 @@ def test_long_rows_with_special_values(built, kw):
     drafts[3, 0], drafts[5, 0] = 7, 9
     check(Call(built, p, q, drafts, u, **kw).run(), drafts, u, excused=1, **kw)
     check(Call(built, p, None, drafts, u, **kw).run(), drafts, u, excused=1, **kw)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("certain", [True, False])
+@pytest.mark.parametrize("temperature", [1e-2, 1e-3, 1e-20, 1e-38, 0.0, -1.0, np.nan])
+@pytest.mark.parametrize("kw", [{}, dict(top_p=0.9), dict(min_p=0.3)])
+def test_drafts_of_low_temperatures(built, temperature, kw, certain):
+    """Drafts drawn at the temperature that they are verified with: no answer needs the excuse of a border."""
+    rng = np.random.default_rng(9)
+    kw = dict(kw, temperature=temperature)
+    for s, d, v in ((6, 3, 300), (3, 2, 7000), (2, 2, 46000)):
+        p, q, drafts, u = make(rng, s, d, v, gap=0.3, certain=certain, **kw)
+        check(Call(built, p, q, drafts, u, **kw).run(), drafts, u, **kw)
