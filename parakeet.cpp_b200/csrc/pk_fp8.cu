@@ -325,6 +325,7 @@ struct PairSmem {
     int its_err;
 };
 constexpr size_t kPSmem = 1024 + (size_t) kPStages * kPStage + 2 * kPQuad + sizeof(PairSmem);
+static_assert(sharing_ruled_out(kPSmem, kPSmem) && sharing_ruled_out(kPSmem, kClusterSmem), "it takes all of the tensor memory");
 
 template <class T>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPThreads, 1)
@@ -769,6 +770,7 @@ bool fit_split(SplitPlan & p, int K, bool fused) {
     if (rest + std::min(most, 2) * stage > kSmemCap) return false;
     p.stages = (int) std::min<size_t>({(size_t) kSMaxStages, (size_t) most, (kSmemCap - rest) / stage});
     p.smem = rest + p.stages * stage;
+    if (p.split > 1) p.smem = std::max(p.smem, kClusterSmem);    // with half of the tensor memory, see there
     return true;
 }
 

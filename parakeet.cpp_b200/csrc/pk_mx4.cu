@@ -569,6 +569,8 @@ struct PairSmem {
 template <int BN, bool BOX> constexpr size_t pair_smem() {
     return 1024 + (size_t) kPStages * pair_stage<BN>() + epi_warps<BOX>() * kOutBytes + sizeof(PairSmem);
 }
+static_assert(sharing_ruled_out(pair_smem<128, true>(), pair_smem<128, true>()) && sharing_ruled_out(pair_smem<128, true>(), kClusterSmem),
+              "it takes all of the tensor memory");
 
 template <class T, int BN, bool BOX>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(tc_threads<BOX>(), 1)

@@ -18,6 +18,17 @@ namespace {
 
 constexpr long long kWaitNs = 2000000000LL;             // bound on every device-side wait, unless a layer sets another
 
+// An allocation of tensor memory waits, without a bound, until an SM's 512 columns have room, and nothing but shared
+// memory, registers and threads keeps blocks off an SM. Blocks of a cluster hold their columns while they wait for the
+// cluster's others to have theirs, so two clusters that each held what the other waits for would never end. Shared memory
+// rules that out: a block of a cluster that takes half of the columns asks for kClusterSmem at least, so that two fit an SM,
+// not three, and none beside a block that takes all columns. (The blocks of pk_bulk.cu, which take all and wait for their grid,
+// have 193 KB. Blocks without a cluster hold columns too, and wait for nobody.)
+constexpr size_t kSmSmem = 228 * 1024, kBlockSmem = 1024;      // of an SM; what each block takes beside its own
+constexpr size_t kClusterSmem = 76 * 1024;
+constexpr bool sharing_ruled_out(size_t a, size_t b) { return a + b + 2 * kBlockSmem > kSmSmem; }
+static_assert(3 * (kClusterSmem + kBlockSmem) > kSmSmem, "no three blocks of half the columns");
+
 // Of a product's waits: their bound, where to tell that one ran out, and (a test's) that the first block, or a
 // pair's second, loads nothing, so that its waits run out.
 struct Waits {

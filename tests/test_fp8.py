@@ -576,3 +576,31 @@ def test_ctc_through_a_head(built, orc, frames):
     with pytest.raises(ValueError):
         ctc.decode_frames(x, [0], [frames], head=head)
     ctc.close()
+
+
+@pytest.mark.gpu
+def test_products_on_many_streams_at_once(built):
+    """Products of every kind, in clusters and in pairs of blocks, in 8 bits and in 4, that share the device's SMs and
+    their tensor memory: each gives what it gives by itself."""
+    import torch
+    pk = built
+    rng = np.random.default_rng(12)
+    jobs = []
+    for i, (kind, r, n, k) in enumerate([(pk.Fp8Linear, 1, 1000, 1024), (pk.Fp8Linear, 16, 512, 1024), (pk.Fp8Linear, 30, 384, 1000), (pk.Fp8Linear, 60, 333, 4099),
+                                         (pk.Fp8Linear, 128, 700, 4096), (pk.Fp8Linear, 700, 640, 512), (pk.Fp8Linear, 5, 200, 300), (pk.Mx4Linear, 2600, 1300, 512),
+                                         (pk.Mx4Linear, 7, 2000, 640), (pk.Mx4Linear, 100, 320, 1024), (pk.Fp8Linear, 3000, 300, 640), (pk.Fp8Linear, 2, 1024, 900)]):
+        layer = kind(rng.standard_normal((n, k)).astype(np.float32))
+        x, y = torch.from_numpy(rng.standard_normal((r, k)).astype(np.float32)).cuda(), torch.zeros(r, n, device="cuda")
+        ws = torch.zeros(max(1, layer.workspace(r)), dtype=torch.uint8, device="cuda")
+        torch.cuda.synchronize()
+        layer.forward(x.data_ptr(), r, y.data_ptr(), workspace=ws.data_ptr(), workspace_bytes=ws.numel())
+        torch.cuda.synchronize()
+        jobs.append((layer, x, y, ws, torch.cuda.Stream(), y.clone()))
+        y.zero_()
+    torch.cuda.synchronize()
+    for _ in range(100):
+        for layer, x, y, ws, st, _ in jobs:
+            layer.forward(x.data_ptr(), x.shape[0], y.data_ptr(), workspace=ws.data_ptr(), workspace_bytes=ws.numel(), stream=st.cuda_stream)
+    torch.cuda.synchronize()
+    for layer, _, y, _, _, want in jobs:
+        assert torch.equal(y, want) and layer.timeouts() == 0
