@@ -70,6 +70,18 @@ __device__ __forceinline__ double draft_weight(float v, int draft, const RowStat
     return exp(((double) v - r.top) / temp);
 }
 
+// Whether a draft of logit v, below all that can have weight (`base`), is not among the first k. Where fewer than k logits can
+// have weight cut_row cuts nothing; of what lies below them nothing is drawn, but a draft there has its own probability. The
+// same for all threads, who all call.
+template <class T, int NT, bool CL, bool RES, bool NM>
+__device__ __forceinline__ bool beyond_k(Team<NT, CL, NM> & team, const Slice<T, RES> & l, int s0, int draft, float v, float base, float cut, int k,
+                                         int vocab) {
+    if (!(k > 0 && k < vocab && v < base && v > -CUDART_INF_F) || cut > -CUDART_INF_F) return false;
+    unsigned before = 0;
+    l.template each<NT>(team.tid, [&](float x, int i) { before += x > v || (x == v && s0 + i < draft) ? 1u : 0u; });
+    return team.sum((u64) before) >= (u64) k;
+}
+
 // A team's list holds all that may be kept, of the first `first` those before which less than `need` lies (0: the share
 // of their weight), of these those from `least` on: the sum of what is kept, and the last of it in the order, told by the
 // thread that has it to f(logit, index, sum).
@@ -203,6 +215,7 @@ __device__ void row_stat(Team<NT, false, NM> & team, TeamBins<NT> * bins, Slice<
     u64 ties = ~0ull;
     bool partial = false;
     const float m = a.min_ps ? a.min_ps[seq] : a.min_p;
+    bool beyond = false;                                         // the draft is not among the first k
     auto leave = [&](float from, float cut_at, int last, u64 sum, int more) {
         st->flags = flags | more;
         st->hi = hi;
@@ -210,7 +223,7 @@ __device__ void row_stat(Team<NT, false, NM> & team, TeamBins<NT> * bins, Slice<
         st->cut = cut_at;
         st->last = last;
         st->total = sum;
-        st->drafted = draft >= 0 && draft < l.n ? draft_weight(l(draft), draft, *st, r, temp, m) : 0.0;
+        st->drafted = draft >= 0 && draft < l.n && !beyond ? draft_weight(l(draft), draft, *st, r, temp, m) : 0.0;
     };
     if constexpr (FILTERS) {
         const float p = a.top_ps ? a.top_ps[seq] : a.top_p;
@@ -226,6 +239,7 @@ __device__ void row_stat(Team<NT, false, NM> & team, TeamBins<NT> * bins, Slice<
                 return true;
             });
         if (done) return;
+        if (draft >= 0 && draft < l.n) beyond = beyond_k(team, l, 0, draft, l(draft), r.base, cut, k, a.vocab);
     }
     const float from = fmaxf(least, cut);
     int last = kAny;
@@ -849,13 +863,15 @@ __global__ void __launch_bounds__(NT, 1024 / NT) verify_rows_kernel(const Plan p
     u64 ties = ~0ull, total = 0;
     bool partial = false;
     const float m = a.min_ps ? a.min_ps[seq] : a.min_p;
+    const bool inside = draft >= 0 && draft < a.vocab;
+    bool beyond = false;                                         // the draft is not among the first k
     auto leave = [&](float from, float cut_at, int last, u64 sum) {
         st.hi = hi;
         st.from = from;
         st.cut = cut_at;
         st.last = last;
         st.total = sum;
-        if (draft >= 0 && draft < a.vocab) st.drafted = draft_weight(seen(to_f32(row_at[draft]), st.flags), draft, st, r, temp, m);
+        if (inside && !beyond) st.drafted = draft_weight(seen(to_f32(row_at[draft]), st.flags), draft, st, r, temp, m);
         *out = st;
     };
     const float p = a.top_ps ? a.top_ps[seq] : a.top_p;
@@ -870,6 +886,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) verify_rows_kernel(const Plan p
         if (CL) team.meet();
         return;
     }
+    if (inside) beyond = beyond_k(team, l, s0, draft, seen(to_f32(row_at[draft]), st.flags), r.base, cut, k, a.vocab);
     const int i0 = RES ? team.tid * len : min(team.tid * len, l.n), i1 = RES ? i0 + len : min(i0 + len, l.n);
     // a run has fewer than 2^9 elements, so its sum stays below 2^53 and is whole
     double onto = kZero;

@@ -651,3 +651,31 @@ def test_drafts_of_low_temperatures(built, temperature, kw, certain):
     for s, d, v in ((6, 3, 300), (3, 2, 7000), (2, 2, 46000)):
         p, q, drafts, u = make(rng, s, d, v, gap=0.3, certain=certain, **kw)
         check(Call(built, p, q, drafts, u, **kw).run(), drafts, u, **kw)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kw", [dict(top_k=11), dict(top_k=700), dict(top_k=11, min_p=1e-25), dict(top_k=60, top_p=0.99999)])
+@pytest.mark.parametrize("v", [24, 1030, 1500, 9000, 30000, 46001])
+def test_drafts_below_all_weight(built, v, kw):
+    """At a low temperature fewer than k tokens weigh as much as 2^-44 of the largest. A draft below them is kept or cut by
+    its rank all the same: with equal rows in the target and the draft it is accepted if it is among the first k, and
+    rejected if not."""
+    rng = np.random.default_rng(v)
+    s, d = 12, 2
+    kw = dict(kw, temperature=0.05)
+    p = rng.standard_normal((s, d + 1, v)) * 2
+    p[::3] = np.round(p[::3])                                    # ties, which go by index
+    q = p[:, :d].copy()
+    ranks = rng.integers(0, v, (s, d))
+    k = min(kw["top_k"], v - 1)
+    ranks[:4, 0], ranks[4:8, 0], ranks[8, 0] = rng.integers(0, k, 4), rng.integers(k, v, 4), k
+    order = np.argsort(-p.astype(np.float32), axis=2, kind="stable")
+    drafts = np.array([[order[i, j, ranks[i, j]] for j in range(d)] for i in range(s)], np.int32)
+    u = rng.random((s, d + 1)).astype(np.float32)
+    call = Call(built, p, q, drafts, u, **kw).run()
+    check(call, drafts, u, **kw)
+    _, acc, _ = call.answer()
+    assert ((acc > 0) <= (ranks[:, 0] < kw["top_k"])).all()
+    check(Call(built, p, None, drafts, u, **kw).run(), drafts, u, **kw)
+    u[:, :d] = 0.0                                               # 0 q(d) < p(d): accepted wherever the target keeps it
+    check(Call(built, p, None, drafts, u, **kw).run(), drafts, u, **kw)
