@@ -141,8 +141,14 @@ __device__ __forceinline__ float logprob_of(float v, const RowStat & p, double h
     return (float) ((v == p.hi ? 0.0 : ((double) v - (double) p.hi) / heat) - (double) logf((float) ((double) p.total * (1.0 / kOne))));
 }
 
-// The sum of a resident row's weights that are kept. A thread's are at most 176 (45,000 logits over 256 threads), below
-// 2^51 in all, so its sum is whole.
+// The rows that a block's shared memory holds, one of so many logits or two of half as many, and the longest that a warp and
+// teams of 128 and 256 threads are given; the rest go to 512.
+constexpr int kResident = 176 * 1024 / 4, kWarpMost = 1056, k128Most = 6144, k256Most = 16384;
+constexpr int logits_each(int logits, int threads) { return ((logits + 6) / 4 + threads - 1) / threads * 4; }   // of a thread, in quads
+
+// The sum of a resident row's weights that are kept. A thread's are at most 92 of 2^43, below 2^50 in all, so its sum is whole.
+static_assert(logits_each(kWarpMost, 32) <= 92 && logits_each(k128Most, 128) <= 92 && logits_each(k256Most, 256) <= 92 &&
+              logits_each(kResident, 512) <= 92, "a thread's logits");
 template <class T, int NT, bool NM>
 __device__ u64 exact_sum(Team<NT, false, NM> & team, const Slice<T, true> & l, const Row & r, float from, float cut, int last) {
     double onto = kZero;
@@ -469,6 +475,9 @@ template <class T, int NT, bool DUAL, bool FILTERS>
 __global__ void __launch_bounds__(NT == 32 ? 256 : group_of<NT, DUAL>(), NT == 32 ? 4 : 1024 / group_of<NT, DUAL>())
 verify_sequence_kernel(const pk_verify_args a, int rows_each, int row_floats) {
     constexpr int G = group_of<NT, DUAL>(), GROUPS = NT == 32 ? kSeqGroups : 1;
+    // rows of whole 16 bytes (row_floats is a multiple of four), the states and the bins behind them
+    static_assert(alignof(SeqSmem<NT, DUAL, FILTERS>) <= 8 && sizeof(SeqSmem<NT, DUAL, FILTERS>) % 8 == 0 && alignof(SeqBins<NT, DUAL>) <= 8 &&
+                  sizeof(SeqBins<NT, DUAL>) % 8 == 0, "what follows the rows is aligned");
     extern __shared__ __align__(16) unsigned char raw[];
     const int g = NT == 32 ? (int) threadIdx.x >> 5 : 0;
     const int blocks = NT == 32 ? 1 : (int) cg::this_cluster().num_blocks(), rank = NT == 32 ? 0 : (int) cg::this_cluster().block_rank();
@@ -526,7 +535,7 @@ verify_sequence_kernel(const pk_verify_args a, int rows_each, int row_floats) {
             if (two) slice(1, pos);
             bool open = true;                                    // whether the draft stands
             if constexpr (!FILTERS) {
-                if (pos < n && draft >= 0 && draft < v && temp_f > 0.0f && (a.draft_logits == nullptr || two)) {
+                if (pos < n && draft >= 0 && draft < v && temp_f > 0.0f) {
                     if (!DUAL || own == 0 || two) {
                         for (int i = 0; i < (DUAL || !two ? 1 : 2); ++i) {
                             const int which = DUAL ? own : i;
@@ -621,8 +630,7 @@ verify_sequence_kernel(const pk_verify_args a, int rows_each, int row_floats) {
                 }
             } else if (!draw_near<T, G>(group, rows[0], rows[1], S.st, mode, draft, temp_f, u[d], tokens + pos, logprobs ? logprobs + pos : nullptr)) {
                 if (mode == kLess) {
-                    if (!DUAL || own == 0 || two)
-                        for (int i = 0; i < (DUAL ? 1 : 2); ++i) settle<T, NT>(team, rows[DUAL ? own : i], temp, &S.st[DUAL ? own : i]);
+                    for (int i = 0; i < (DUAL ? 1 : 2); ++i) settle<T, NT>(team, rows[DUAL ? own : i], temp, &S.st[DUAL ? own : i]);
                 }
                 if (group.tid == 0) S.group.found = -1;
                 group.sync();
@@ -729,7 +737,7 @@ cudaError_t launch_sequences(const pk_verify_args & a, int blocks, cudaStream_t 
 
 // Whether the kernel above can hold a position's rows: beside them there are up to 2048 logits' room in front of and
 // behind each, and 25 KB of the teams'.
-bool resident(int vocab, bool two) { return (size_t) vocab * 4 * (two ? 2 : 1) <= 176 * 1024; }
+bool resident(int vocab, bool two) { return vocab <= (two ? kResident / 2 : kResident); }
 
 template <class T, bool FILTERS, int NT> cudaError_t sequences_block(const pk_verify_args & a, cudaStream_t s) {
     // The blocks of a cluster share the positions out while there is room for them (four drafts by 8193, temperature alone, 64
@@ -747,9 +755,9 @@ template <class T, bool FILTERS, int NT> cudaError_t sequences_block(const pk_ve
 // 512 for long ones (300 of three drafts by 16000, top-p: 199 us, of 256 331) and for few with filters (8 by 8193, top-p: 25 us
 // and 35), of 256 in between.
 template <class T, bool FILTERS> cudaError_t sequences_dispatch(const pk_verify_args & a, cudaStream_t s) {
-    if (a.vocab <= 1056 && a.sequences >= 4 * 148) return launch_sequences<T, 32, false, FILTERS>(a, 1, s);
-    if (a.vocab <= (FILTERS ? 2048 : 6144)) return sequences_block<T, FILTERS, 128>(a, s);
-    if (FILTERS ? a.vocab > 12288 || a.sequences * (a.max_drafts + 1) <= 148 : a.vocab > 16384) return sequences_block<T, FILTERS, 512>(a, s);
+    if (a.vocab <= kWarpMost && a.sequences >= 4 * 148) return launch_sequences<T, 32, false, FILTERS>(a, 1, s);
+    if (a.vocab <= (FILTERS ? 2048 : k128Most)) return sequences_block<T, FILTERS, 128>(a, s);
+    if (FILTERS ? a.vocab > 12288 || a.sequences * (a.max_drafts + 1) <= 148 : a.vocab > k256Most) return sequences_block<T, FILTERS, 512>(a, s);
     return sequences_block<T, FILTERS, 256>(a, s);
 }
 
