@@ -70,16 +70,13 @@ __device__ __forceinline__ double draft_weight(float v, int draft, const RowStat
     return exp(((double) v - r.top) / temp);
 }
 
-// Whether a draft of logit v, below all that can have weight (`base`), is not among the first k. Where fewer than k logits can
-// have weight cut_row cuts nothing; of what lies below them nothing is drawn, but a draft there has its own probability. The
-// same for all threads, who all call.
+// The tokens before a draft of logit v, in the order that top-k goes by. Where fewer than k logits can have weight cut_row cuts
+// nothing; of what lies below them nothing is drawn, but a draft there has its own probability, and is cut by its rank.
 template <class T, int NT, bool CL, bool RES, bool NM>
-__device__ __forceinline__ bool beyond_k(Team<NT, CL, NM> & team, const Slice<T, RES> & l, int s0, int draft, float v, float base, float cut, int k,
-                                         int vocab) {
-    if (!(k > 0 && k < vocab && v < base && v > -CUDART_INF_F) || cut > -CUDART_INF_F) return false;
+__device__ __forceinline__ u64 rank_of(Team<NT, CL, NM> & team, const Slice<T, RES> & l, int s0, int draft, float v) {
     unsigned before = 0;
     l.template each<NT>(team.tid, [&](float x, int i) { before += x > v || (x == v && s0 + i < draft) ? 1u : 0u; });
-    return team.sum((u64) before) >= (u64) k;
+    return team.sum((u64) before);
 }
 
 // A team's list holds all that may be kept, of the first `first` those before which less than `need` lies (0: the share
@@ -221,7 +218,6 @@ __device__ void row_stat(Team<NT, false, NM> & team, TeamBins<NT> * bins, Slice<
     u64 ties = ~0ull;
     bool partial = false;
     const float m = a.min_ps ? a.min_ps[seq] : a.min_p;
-    bool beyond = false;                                         // the draft is not among the first k
     auto leave = [&](float from, float cut_at, int last, u64 sum, int more) {
         st->flags = flags | more;
         st->hi = hi;
@@ -229,7 +225,7 @@ __device__ void row_stat(Team<NT, false, NM> & team, TeamBins<NT> * bins, Slice<
         st->cut = cut_at;
         st->last = last;
         st->total = sum;
-        st->drafted = draft >= 0 && draft < l.n && !beyond ? draft_weight(l(draft), draft, *st, r, temp, m) : 0.0;
+        st->drafted = draft >= 0 && draft < l.n ? draft_weight(l(draft), draft, *st, r, temp, m) : 0.0;
     };
     if constexpr (FILTERS) {
         const float p = a.top_ps ? a.top_ps[seq] : a.top_p;
@@ -245,7 +241,6 @@ __device__ void row_stat(Team<NT, false, NM> & team, TeamBins<NT> * bins, Slice<
                 return true;
             });
         if (done) return;
-        if (draft >= 0 && draft < l.n) beyond = beyond_k(team, l, 0, draft, l(draft), r.base, cut, k, a.vocab);
     }
     const float from = fmaxf(least, cut);
     int last = kAny;
@@ -563,6 +558,21 @@ verify_sequence_kernel(const pk_verify_args a, int rows_each, int row_floats) {
                     }
                 }
                 group.sync();
+                if constexpr (FILTERS) {
+                    // see rank_of; the statistics are not changed before all threads have looked
+                    const int k = a.top_ks ? a.top_ks[seq] : a.top_k;
+                    auto low = [&](const RowStat & st) { return !(st.flags & kGreedy) && !(st.cut > -CUDART_INF_F) && st.drafted > 0.0 && st.drafted < 0x1p-44; };
+                    if (k > 0 && k < v && (low(S.st[0]) || (two && low(S.st[1])))) {
+                        group.sync();
+                        if (!DUAL || own == 0 || two)
+                            for (int i = 0; i < (DUAL || !two ? 1 : 2); ++i) {
+                                const int which = DUAL ? own : i;
+                                const u64 rank = rank_of(team, rows[which], 0, draft, rows[which](draft));
+                                if (team.tid == 0 && rank >= (u64) k && low(S.st[which])) S.st[which].drafted = 0.0;
+                            }
+                        group.sync();
+                    }
+                }
             }
             if (!open) {
                 code = kAccepted;
@@ -894,7 +904,10 @@ __global__ void __launch_bounds__(NT, 1024 / NT) verify_rows_kernel(const Plan p
         if (CL) team.meet();
         return;
     }
-    if (inside) beyond = beyond_k(team, l, s0, draft, seen(to_f32(row_at[draft]), st.flags), r.base, cut, k, a.vocab);
+    if (inside && k > 0 && k < a.vocab && !(cut > -CUDART_INF_F)) {
+        const float v = seen(to_f32(row_at[draft]), st.flags);
+        if (v < r.base && v > -CUDART_INF_F) beyond = rank_of(team, l, s0, draft, v) >= (u64) k;   // the same for all threads
+    }
     const int i0 = RES ? team.tid * len : min(team.tid * len, l.n), i1 = RES ? i0 + len : min(i0 + len, l.n);
     // a run has fewer than 2^9 elements, so its sum stays below 2^53 and is whole
     double onto = kZero;
