@@ -65,6 +65,7 @@ __device__ __forceinline__ Row row_of(float hi, double temp) {
 __device__ __forceinline__ double draft_weight(float v, int draft, const RowStat & st, const Row & r, double temp, float m) {
     const float floor = fmaxf(!(m > 0.0f) ? -CUDART_INF_F : m >= 1.0f ? st.hi : __double2float_ru(r.top + temp * log((double) m)), -3.402823466e+38f);
     if (!(v >= floor && (v > st.cut || (v == st.cut && draft <= st.last)))) return 0.0;
+    if (v == st.hi) return 1.0;                                  // the table's first entry is one and a bit
     // pk_sample's weight as it is before it is rounded, to 2^-42 of itself
     if (v >= r.base) return weight_onto(v, r, 0.0, [](int n) { return table_entry(n & 31); }) * (1.0 / kOne);
     return exp(((double) v - r.top) / temp);
@@ -133,9 +134,17 @@ __device__ __forceinline__ double scale_of(const Row32 & f, float hi) {
     return 1.0 + x * (1.0 + x * (0.5 + x * (1.0 / 6.0 + x * (1.0 / 24.0))));
 }
 
+// A row's total, times 2^43, from the sum of its f32 weights. Where nearly all of it is the largest's, by what that alone gives: a
+// row that leaves nothing else has exactly one. Either way the sum is off by less than kOff of itself: by the additions' 19 2^-24
+// and a little of the rest, below 2^-20, in the first case.
+__device__ __forceinline__ u64 total_of(double sum, const Row32 & f, float hi) {
+    const double own = (double) f.weight(hi);
+    return (u64) ((sum - own < 0x1p-20 * own ? sum / own : sum * scale_of(f, hi)) * kOne);
+}
+
 // Log-probability of the token with logit v: log() of a number below 2^16 in f32 is off by a unit, 2^-20, at most.
 __device__ __forceinline__ float logprob_of(float v, const RowStat & p, double heat) {
-    return (float) ((v == p.hi ? 0.0 : ((double) v - (double) p.hi) / heat) - (double) logf((float) ((double) p.total * (1.0 / kOne))));
+    return fminf((float) ((v == p.hi ? 0.0 : ((double) v - (double) p.hi) / heat) - (double) logf((float) ((double) p.total * (1.0 / kOne)))), 0.0f);
 }
 
 // The rows that a block's shared memory holds, one of so many logits or two of half as many, and the longest that a warp and
@@ -237,7 +246,7 @@ __device__ void row_stat(Team<NT, false, NM> & team, TeamBins<NT> * bins, Slice<
             },
             [&](double kept) {
                 if (!(cut >= least)) return false;               // min-p drops more
-                if (one) leave(cut, cut, kAny, (u64) (kept * scale_of(Row32(hi, temp_f), hi) * kOne), kNear);
+                if (one) leave(cut, cut, kAny, total_of(kept, Row32(hi, temp_f), hi), kNear);
                 return true;
             });
         if (done) return;
@@ -280,7 +289,7 @@ __device__ void row_stat(Team<NT, false, NM> & team, TeamBins<NT> * bins, Slice<
             static_assert(NT <= 512, "honest sums below kBad, NT times kBad below 2^64");
             const u64 sum = team.sum(mine < 128.0f ? __double2ull_rn((double) mine * kFine) : kBad);
             if (sum < kBad) {
-                if (one) leave(from, cut, last, (u64) ((double) sum * scale_of(f, hi) * (kOne / kFine)), kNear);
+                if (one) leave(from, cut, last, total_of((double) sum * (1.0 / kFine), f, hi), kNear);
                 return;
             }
         }
@@ -542,7 +551,7 @@ verify_sequence_kernel(const pk_verify_args a, int rows_each, int row_floats) {
                     // u q(d) < p(d) by more than the sums are off by, twice
                     const double p = S.quick[0], q = two ? S.quick[1] : 1.0;
                     open = !(p < 0x1p24 && q < 0x1p24 && (double) number_of(u[pos]) * p * (1.0 + 4.0 * kQuick) < q);
-                    if (!open && logprobs && group.tid == 0) quick_log = -logf((float) p);
+                    if (!open && logprobs && group.tid == 0) quick_log = fminf(-logf((float) p), 0.0f);
                     group.sync();
                 }
             }
@@ -1127,7 +1136,7 @@ __global__ void __launch_bounds__(kDrawThreads) verify_draw_kernel(const Plan pl
         const double l = (double) number_of(u[j]) * sp;
         return l * (1.0 + edge) < sq ? 1 : l > sq * (1.0 + edge) ? -1 : 0;
     };
-    auto logprob_at = [&](int j, float x) { if (a.logprobs) a.logprobs[seq * (d + 1) + j] = x; };
+    auto logprob_at = [&](int j, float x) { if (a.logprobs) a.logprobs[seq * (d + 1) + j] = fminf(x, 0.0f); };
     RowStat p, q;
     int first = 0;
     for (;;) {

@@ -679,3 +679,35 @@ def test_drafts_below_all_weight(built, v, kw):
     check(Call(built, p, None, drafts, u, **kw).run(), drafts, u, **kw)
     u[:, :d] = 0.0                                               # 0 q(d) < p(d): accepted wherever the target keeps it
     check(Call(built, p, None, drafts, u, **kw).run(), drafts, u, **kw)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kw", [dict(top_k=1), dict(top_k=1, top_p=0.9, min_p=0.05), dict(top_p=0.5), dict(min_p=0.5), dict(top_k=500, top_p=0.5, min_p=0.05), {}])
+@pytest.mark.parametrize("certain", [False, True])
+@pytest.mark.parametrize("s,v", [(5, 300), (700, 300), (6, 1500), (5, 9000), (40, 7000), (3, 18000), (3, 46001)])
+def test_certain_tokens_have_probability_one(built, s, v, certain, kw):
+    """Rows of which one token is all that is left, by the filters or by its lead (60, in units of T): its log-probability is
+    0, accepted or drawn, and no log-probability is above."""
+    rng = np.random.default_rng(v + s)
+    d = 2
+    p = rng.standard_normal((s, d + 1, v)) * 3 + rng.uniform(-40, 40, (s, d + 1, 1))
+    top = rng.integers(0, v, (s, d + 1))
+    for i in range(s):
+        for j in range(d + 1):
+            p[i, j, top[i, j]] = p[i, j].max() + 60 * 0.7
+    q = None if certain else p[:, :d] + 0.3 * rng.standard_normal((s, d, v))
+    drafts = top[:, :d].astype(np.int32).copy()
+    drafts[::3, 1] = (drafts[::3, 1] + 1) % v
+    u = rng.random((s, d + 1)).astype(np.float32)
+    kw = dict(kw, temperature=0.7)
+    call = Call(built, p, q, drafts, u, **kw).run()
+    # Nothing cut: a second draft has e^-60 or less in both rows, and may stand. Where it is rejected, p - q is at most
+    # 2 v e^-60 < 2^-66 in all, below the 2^-43 that may be lost, and the token may come from p.
+    nothing_cut = not certain and len(kw) == 1
+    check(call, drafts, u, excused=-(-s // 3) if nothing_cut else 0, **kw)
+    tok, acc, lp = call.answer()
+    assert (lp[tok == top] == 0).all() and (lp <= 0).all() and (tok[:, 0] == top[:, 0]).all()
+    assert nothing_cut or ((lp[tok >= 0] == 0).all() and acc.min() == 1 and acc.max() == 2)
+    p, q, drafts, u = make(rng, s, d, v, spread=6.0, gap=0.2, certain=certain, **kw)
+    tok, _, lp = Call(built, p, q, drafts, u, **kw).run().answer()
+    assert (lp <= 0).all()
