@@ -651,7 +651,7 @@ PK_API pk_status pk_sample(int device, const pk_sample_args * args, void * strea
  * drafts; differences p - q below 2^-43 of the larger may be lost. Where 32-bit sums with a proven
  * bound tell the answer they are used instead; log-probabilities are then within 2^-15 (the largest
  * vocabularies; 2^-16 up to 16384), mostly 2^-22, of their value, and may differ within that with the
- * number of sequences. */
+ * number of sequences. None is above 0, and a token that is all that is left of its row has 0. */
 #define PK_VERIFY_MAX_DRAFTS 65535
 
 typedef struct pk_verify_args {

@@ -774,15 +774,19 @@ bool fit_split(SplitPlan & p, int K, bool fused) {
     return true;
 }
 
-// The most blocks of K a tile is parted over: up to eight, while all tiles' blocks run at once.
+// The most blocks of K a tile is parted over: up to eight, while there are SMs for all tiles' blocks. (Sixteen clusters of eight
+// do not run at once all the same: see plan_split.)
 int split_of(long long tiles, int nb) {
     int s = 1;
     while (s < 8 && tiles * s * 2 <= 148 && s * 2 <= nb) s *= 2;
     return s;
 }
 
-// Rows that the cluster kernel quantises itself, none of its blocks more than these values (a row of 640 by 8198, replayed from a
-// graph: 6.6 us, 8.7 with a launch for each).
+// Rows that the cluster kernel quantises itself, none of its blocks more than these values. Replayed from a graph, this way and in
+// two launches, the second in pairs of blocks: a row of 640 by 8198 6.5 us and 6.9, of 1024 by 1024 5.7 and 7.5, of 2048 by 8198
+// 9.0 and 9.8; 16 rows of 1024 by 1024 6.7 and 7.7, of 640 by 8198 8.0 and 7.0; 32 of 2048 by 1024 8.0 and 9.8, of 1024 by 1024 7.8
+// and 7.6, of 640 by 8198 10.2 and 7.2. So it is sooner for few rows and for long ones; from some 16 rows on of a wide layer it
+// is not, from a program's calls either (one row of 640 by 8198 8.2 us and 8.3, 32 12.3 and 8.3).
 constexpr long long kFusedRows = 32, kFusedValues = 32768;
 bool plan_fused(const pk_fp8 * w, long long M, SplitPlan & p) {
     if (M > kFusedRows) return false;
@@ -792,9 +796,11 @@ bool plan_fused(const pk_fp8 * w, long long M, SplitPlan & p) {
     return fit_split(p, w->K, true);
 }
 
-// Few tiles and a long K, codes from the row kernel. Replayed from a graph, this way and in pairs of blocks: 64 rows of 4096 by
-// 1024 11.2 us and 14.5, 128 13.8 and 14.7, 40 of 4096 by 4096 13.2 and 14.7; 64 of 2048 by 4096 11.3 and 10.3, 64 of 640 by 8198
-// 11.1 and 7.7, 128 of 1024 by 4096 12.9 and 8.3.
+// Few tiles and a long K, codes from the row kernel. Replayed from a graph, this way and in pairs of blocks, 64 rows: by 1024
+// outputs, K of 1024 9.4 us and 7.8, 2048 10.0 and 10.0, 2560 10.7 and 11.2, 3328 11.4 and 12.8, 4096 11.5 and 14.3, 8192 13.9 and
+// 23.1; by 4096, K of 2560 12.3 and 11.4, 3328 13.6 and 12.9, 4096 14.3 and 14.5, 8192 17.9 and 23.4. 128 rows by 1024: 2560 13.3 and
+// 11.3, 3328 14.1 and 13.1, 4096 14.1 and 14.5. By 2048 outputs, which ask for 16 clusters of eight blocks, not all of them run at
+// once and pairs are sooner (K of 4096: 20.1 and 14.3), up to K of some 8192 (25.3 and 23.2).
 bool plan_split(const pk_fp8 * w, long long M, SplitPlan & p) {
     const long long nt = (w->N + kTN - 1) / kTN;
     if (M > 128 || w->nb < 26) return false;

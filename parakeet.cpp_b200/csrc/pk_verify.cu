@@ -17,8 +17,10 @@
 //
 // Measured (calls among others, Python's included): 1024 sequences of four drafts by 8193 f32 logits, temperature alone, 105 us,
 // of which the rows up to the first rejections are 192 MB, 29 us; most of the rest is the latency of a block's steps, two blocks
-// of 512 threads an SM. 256 of eight by 8193 bf16, top-p and min-p, 135 us: the cuts of two rows a position, as long as in
-// pk_sample. One of four, top-k and top-p, 22 us, the chain of a cut and a draw.
+// of 512 threads an SM. 256 of eight by 8193 bf16, top-p and min-p, 132 to 144 us for some 1830 rows: the cuts of two rows a position,
+// chains of block-wide steps with 44 % of the warps that an SM can hold, one position after the other. It is not what cutting
+// rows takes: pk_sample cuts as many, and draws from all of them, in 71 us. One of four, top-k and top-p, 22 us, the chain of a
+// cut, an exchange and a draw over all logits; pk_sample takes 9 us for a row with these settings, replayed from a graph.
 
 #include "pk_draw.cuh"
 
@@ -769,10 +771,14 @@ template <class T, bool FILTERS, int NT> cudaError_t sequences_block(const pk_ve
     return launch_sequences<T, NT <= 256 ? 2 * NT : NT, false, FILTERS>(a, blocks, s);
 }
 
-// A warp per sequence for many short rows (2000 of four drafts by 1025, temperature alone: 44 us, a block of 256 52; top-k and
-// top-p 178 and 220). Otherwise two teams of 128 threads for short rows (400 by 4000, temperature alone: 30 us, of 256 40), of
-// 512 for long ones (300 of three drafts by 16000, top-p: 199 us, of 256 331) and for few with filters (8 by 8193, top-p: 25 us
-// and 35), of 256 in between.
+// Replayed from a graph, four drafts a sequence. A warp per sequence for many short rows (by 1025, a warp and two teams of 128
+// threads: 2000 sequences, temperature alone, 45 us and 50; top-k 173 and 199; min-p 48 and 65; by 300 27 and 46, 142 and 200, 35
+// and 63. But top-p 203 and 143, and of 592 sequences, where it begins, 41 and 20, so that the teams would be sooner up to some
+// 1500). Otherwise two teams of 128 for short rows (128 and 256: 400 by 4000, temperature alone, 29 us and 36, by 6100 39 and 45,
+// by 8193 46 and 54, but 64 by 8193 29 and 25; top-p, 400 by 2040 63 and 70, by 4000 104 and 93), of 512 for long ones (256 and
+// 512: temperature alone, 300 by 12000 49 us and 68, by 16000 76 and 79, by 19000 94 and 90; top-p, 64 by 8193 55 and 62, by
+// 12000 97 and 71, 300 by 12000 169 and 175, by 16000 235 and 212) and for few with filters (8 by 8193, top-p: 34 us and 25), of
+// 256 in between.
 template <class T, bool FILTERS> cudaError_t sequences_dispatch(const pk_verify_args & a, cudaStream_t s) {
     if (a.vocab <= kWarpMost && a.sequences >= 4 * 148) return launch_sequences<T, 32, false, FILTERS>(a, 1, s);
     if (a.vocab <= (FILTERS ? 2048 : k128Most)) return sequences_block<T, FILTERS, 128>(a, s);
@@ -782,10 +788,13 @@ template <class T, bool FILTERS> cudaError_t sequences_dispatch(const pk_verify_
 
 // ---- long rows ---------------------------------------------------------------------
 //
-// Two kernels (4 sequences of eight looked-up drafts by 131072 bf16: 27.5 us, two launches and the draw's passes over one row,
-// 16,384 logits a block). The first takes a block or cluster per row, all rows at once, and leaves what the test needs of it; with filters
+// Two kernels (4 sequences of eight looked-up drafts by 131072 bf16: 27 us, two launches and the draw's passes over one row,
+// 16,384 logits a block; of two models 61; with top-p 117 and 154, with top-k 61 and 90; 32 of four by 50000 f32, two models, 49,
+// with top-p 125). The first takes a block or cluster per row, all rows at once, and leaves what the test needs of it; with filters
 // as pk_sample does. The second takes a block or cluster per sequence: it tests all drafts at once and draws from the one row, or
-// two, that the first rejection names, reading them again.
+// two, that the first rejection names, reading them again. But at T <= 0 without filters the first tells nothing, and the second
+// settles the positions one after the other, two passes over each row of theirs: 4 sequences of eight looked-up drafts by 131072
+// bf16 take 36 us where the first is rejected, 129 where all are accepted, of two models 61 and 211.
 
 struct Plan {
     pk_verify_args a;
